@@ -228,6 +228,65 @@ int janus_attention_noalloc(janus_ctx *ctx, const float *q, const void *k_cache,
                             uint32_t max_seq_len, const int32_t *d_row_base,
                             const int32_t *d_seq_lens, uint32_t max_len_hint, float scale);
 
+/* ---- heads and attention of packed rows --------------------------------- */
+/* No counterpart in the reference, which runs a prompt token by token and
+ * keeps a copy of a shared prompt per sequence. Rows of several sequences are
+ * packed one behind the other; a sequence's K and V lie in consecutive cache
+ * rows as above. The split partials of the two attentions go into the
+ * context's attention workspace (janus_set_stream): a first call of a shape
+ * outside any capture makes it large enough.
+ *
+ * RMS norm of each query and key head, rotation and KV append in one pass.
+ * Row r at position p = d_positions[r] (position for all when NULL):
+ *   y = x / sqrt(mean(x^2) + eps) * gamma over each head (q_gamma / k_gamma
+ *       [head_dim], NULL: y = x), then the half-split rotation of janus_rope
+ *       with d_table[p] (at least max_seq_len rows);
+ *   q_out[r] = the rotated query heads ([rows][heads][head_dim], out_dtype),
+ *   k_cache / v_cache row (row_base[r] + p) = the rotated key heads and the
+ *   value heads as they are, stored as kv_dtype.
+ * q, k and v are of in_dtype, rows *_stride elements apart (0: contiguous), so
+ * that the parts of one fused product can be passed. d_row_base NULL means
+ * r * max_seq_len. A row whose position is outside [0, max_seq_len) is left
+ * out; one whose row base is negative (padding) is not appended. Rows of one
+ * call must go to different cache rows. q_out may be q where both are
+ * contiguous and of one type; no other buffers may overlap. head_dim is even,
+ * at most 1024; 64, 128 and 256 with 16-byte aligned buffers and strides take
+ * the vector kernel. */
+int janus_qk_norm_rope(janus_ctx *ctx, const void *q, const void *k, const void *v, int in_dtype, uint32_t q_stride,
+                       uint32_t k_stride, uint32_t v_stride, const float *q_gamma, const float *k_gamma, float eps,
+                       const float *d_table, void *q_out, int out_dtype, void *k_cache, void *v_cache, int kv_dtype,
+                       uint32_t rows, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t position,
+                       uint32_t max_seq_len, const int32_t *d_row_base, const int32_t *d_positions);
+/* Causal attention of packed rows: whole prompts, chunks of prompts behind
+ * their context, drafted tokens, single tokens, mixed as they come. Sequence
+ * s has the q rows [q_start[s], q_start[s+1]) (d_q_start: nseq + 1 ascending
+ * values; NULL: rows / nseq rows each), which are the last of its len_s
+ * positions: its row i of n sees positions [0, len_s - n + 1 + i) at cache rows
+ * row_base[s] + position. len_s = d_seq_lens[s] (NULL: n, a whole prompt),
+ * at most max_seq_len; d_row_base NULL means s * max_seq_len (d_q_start itself
+ * for K and V packed like q). A row that sees nothing (len_s < n - i, or a
+ * negative row base) is 0; rows outside the sequences are left as they are.
+ * q and out are [rows][heads][head_dim] of dtype: F32 on an F32 or F16 cache,
+ * or F16 on an F16 cache (probabilities rounded to binary16, sums in binary32).
+ * An infinity or NaN where a row does not look does not reach it. max_len_hint
+ * (0: max_seq_len) is about the longest len_s: it plans the split, whatever the
+ * lengths turn out to be. head_dim 64 or 128; q, caches and out 16-byte
+ * aligned; scale <= 0 selects 1/sqrt(head_dim). */
+int janus_prompt_attention(janus_ctx *ctx, const void *q, int dtype, const void *k_cache, const void *v_cache,
+                           int kv_dtype, void *out, uint32_t rows, uint32_t nseq, uint32_t heads, uint32_t kv_heads,
+                           uint32_t head_dim, uint32_t max_seq_len, const int32_t *d_q_start,
+                           const int32_t *d_row_base, const int32_t *d_seq_lens, uint32_t max_len_hint, float scale);
+/* Decode attention (one query per sequence) of a batch that shares a prefix:
+ * sequence b sees the cache rows [prefix_row, prefix_row + prefix_len), which
+ * are read once for the whole batch, and then its own [row_base[b],
+ * row_base[b] + len_b), len_b = d_seq_lens[b] (seq_len for all when NULL), at
+ * most max_seq_len; both may be empty. Types, tables, hint and scale as above. */
+int janus_prefix_attention(janus_ctx *ctx, const void *q, int dtype, const void *k_cache, const void *v_cache,
+                           int kv_dtype, void *out, uint32_t batch, uint32_t heads, uint32_t kv_heads,
+                           uint32_t head_dim, uint32_t prefix_row, uint32_t prefix_len, uint32_t seq_len,
+                           uint32_t max_seq_len, const int32_t *d_row_base, const int32_t *d_seq_lens,
+                           uint32_t max_len_hint, float scale);
+
 /* ---- embedding (model/transformer/embedding.rs:16-198) ---------------- */
 /* out[b][:] = table[ids[b]][:] decoded as the table's binary16 values.
  * h_ids are host token ids checked against the vocabulary. */

@@ -100,6 +100,10 @@ _SIGNATURES = {
     "janus_kv_update": (I32, [P, P, P, P, P, I32, U32, U32, U32, U32, U32, P, P]),
     "janus_attention": (I32, [P, P, P, P, I32, P, U32, U32, U32, U32, U32, U32, P, P, U32, F32]),
     "janus_attention_noalloc": (I32, [P, P, P, P, I32, P, U32, U32, U32, U32, U32, U32, P, P, U32, F32]),
+    "janus_qk_norm_rope": (I32, [P, P, P, P, I32, U32, U32, U32, P, P, F32, P, P, I32, P, P, I32, U32, U32, U32, U32,
+                                 U32, U32, P, P]),
+    "janus_prompt_attention": (I32, [P, P, I32, P, P, I32, P, U32, U32, U32, U32, U32, U32, P, P, P, U32, F32]),
+    "janus_prefix_attention": (I32, [P, P, I32, P, P, I32, P, U32, U32, U32, U32, U32, U32, U32, U32, P, P, U32, F32]),
     "janus_embed": (I32, [P, P, P, U32, P]),
     "janus_embed_device": (I32, [P, P, P, U32, P]),
     "janus_argmax": (I32, [P, P, P, U32, U32, I32]),

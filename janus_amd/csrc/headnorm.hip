@@ -1,0 +1,242 @@
+// headnorm.hip -- RMS norm of the query and key heads, rotation and KV append
+// in one pass.
+//
+// Row r at position p, head vector x of D values, gain g (or none):
+//   y = x / sqrt(mean(x^2) + eps) * g             (y = x without a gain)
+//   z_i = y_i c_i - y_{i + D/2} s_i,  z_{i + D/2} = y_i s_i + y_{i + D/2} c_i
+// with (c_i, s_i) = table[p][i]. Query heads go to q_out, key heads and the
+// untouched value heads to the row's cache row.
+#include "internal.h"
+
+namespace janus {
+namespace {
+
+struct HeadArgs {
+    const void *q, *k, *v;
+    uint32_t q_stride, k_stride, v_stride;   // elements from a row to the next
+    const float *q_gamma, *k_gamma;
+    const float *table;                      // [max_seq][D / 2] (cos, sin)
+    void *q_out, *kc, *vc;
+    const int32_t *row_base, *positions;
+    uint32_t rows, heads, kv_heads, hd, position, max_seq;
+    uint32_t parts;                          // groups of a row
+    float eps;
+};
+
+struct Place {
+    uint32_t pos;
+    bool rotates, appends;
+    size_t cache_row;
+};
+
+__device__ __forceinline__ Place place_of(const HeadArgs &a, uint32_t row) {
+    const int32_t p = a.positions ? a.positions[row] : (int32_t)a.position;
+    const int64_t base = a.row_base ? (int64_t)a.row_base[row] : (int64_t)row * a.max_seq;
+    Place r;
+    r.rotates = p >= 0 && (uint32_t)p < a.max_seq;
+    r.appends = r.rotates && base >= 0;
+    r.pos = r.rotates ? (uint32_t)p : 0u;
+    r.cache_row = r.appends ? (size_t)base + r.pos : 0;
+    return r;
+}
+
+// E consecutive values as floats, and back; the address is a multiple of their size (at most 16 bytes).
+template <typename T, int E> __device__ __forceinline__ void load_e(const T *p, float (&x)[E]) {
+    typedef T vec __attribute__((ext_vector_type(E < 16 / (int)sizeof(T) ? E : 16 / (int)sizeof(T))));
+    constexpr int N = sizeof(vec) / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < E; i += N) {
+        const vec v = *(const vec *)(p + i);
+#pragma unroll
+        for (int j = 0; j < N; ++j) x[i + j] = (float)v[j];
+    }
+}
+template <typename T, int E> __device__ __forceinline__ void store_e(T *p, const float (&x)[E]) {
+    typedef T vec __attribute__((ext_vector_type(E < 16 / (int)sizeof(T) ? E : 16 / (int)sizeof(T))));
+    constexpr int N = sizeof(vec) / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < E; i += N) {
+        vec v;
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = (T)x[i + j];
+        *(vec *)(p + i) = v;
+    }
+}
+
+// D / 2 / E lanes share a head: each holds E values of the first half and the
+// E values that they turn with. A lane group takes up to U heads of one row,
+// `parts` apart, and loads the row's (cos, sin) once for them.
+template <typename IN, typename OUT, typename KV, int D, int E, int U>
+__global__ __launch_bounds__(256) void head_kernel(HeadArgs a) {
+    constexpr uint32_t L = D / 2 / E;
+    const uint32_t units = a.heads + 2 * a.kv_heads;
+    const uint64_t grp = ((uint64_t)blockIdx.x * 256u + threadIdx.x) / L;
+    const uint32_t row = (uint32_t)(grp / a.parts), part = (uint32_t)(grp % a.parts), at = threadIdx.x % L * E;
+    if (row >= a.rows) return;
+    float x0[U][E], x1[U][E];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t h = part + u * a.parts;
+        if (h >= units) break;
+        const IN *src = h < a.heads ? (const IN *)a.q + (size_t)row * a.q_stride + (size_t)h * D
+                        : h < a.heads + a.kv_heads
+                            ? (const IN *)a.k + (size_t)row * a.k_stride + (size_t)(h - a.heads) * D
+                            : (const IN *)a.v + (size_t)row * a.v_stride + (size_t)(h - a.heads - a.kv_heads) * D;
+        load_e<IN, E>(src + at, x0[u]);
+        load_e<IN, E>(src + D / 2 + at, x1[u]);
+    }
+    const Place pl = place_of(a, row);
+    float cs[2 * E];
+    load_e<float, 2 * E>(a.table + ((size_t)pl.pos * (D / 2) + at) * 2, cs);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t h = part + u * a.parts;
+        if (h >= units) break;
+        const bool is_q = h < a.heads, is_k = !is_q && h < a.heads + a.kv_heads;
+        const float *gamma = is_q ? a.q_gamma : is_k ? a.k_gamma : nullptr;
+        if (gamma) {
+            float s = 0.0f;
+#pragma unroll
+            for (int i = 0; i < E; ++i) s = fmaf(x0[u][i], x0[u][i], fmaf(x1[u][i], x1[u][i], s));
+#pragma unroll
+            for (int o = L / 2; o > 0; o >>= 1) s += shfl_xor(s, o);
+            const float r = 1.0f / sqrtf(s * (1.0f / D) + a.eps);
+            float g0[E], g1[E];
+            load_e<float, E>(gamma + at, g0);
+            load_e<float, E>(gamma + D / 2 + at, g1);
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                x0[u][i] = x0[u][i] * r * g0[i];
+                x1[u][i] = x1[u][i] * r * g1[i];
+            }
+        }
+        if (is_q || is_k) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const float p = x0[u][i], n = x1[u][i], c = cs[2 * i], s = cs[2 * i + 1];
+                x0[u][i] = p * c - n * s;
+                x1[u][i] = p * s + n * c;
+            }
+        }
+        if (is_q) {
+            OUT *o = (OUT *)a.q_out + ((size_t)row * a.heads + h) * D + at;
+            if (pl.rotates) {
+                store_e<OUT, E>(o, x0[u]);
+                store_e<OUT, E>(o + D / 2, x1[u]);
+            }
+        } else if (pl.appends) {
+            const uint32_t kh = h - a.heads - (is_k ? 0u : a.kv_heads);
+            KV *o = (KV *)(is_k ? a.kc : a.vc) + (pl.cache_row * a.kv_heads + kh) * D + at;
+            store_e<KV, E>(o, x0[u]);
+            store_e<KV, E>(o + D / 2, x1[u]);
+        }
+    }
+}
+
+// Any even head dim up to 1024 and any alignment: a wavefront per head.
+template <typename IN, typename OUT, typename KV>
+__global__ __launch_bounds__(256) void head_any_kernel(HeadArgs a) {
+    const uint32_t units = a.heads + 2 * a.kv_heads, half = a.hd / 2, lane = threadIdx.x & 63u;
+    const uint64_t unit = (uint64_t)blockIdx.x * 4u + (threadIdx.x >> 6);
+    const uint32_t row = (uint32_t)(unit / units), h = (uint32_t)(unit % units);
+    if (row >= a.rows) return;
+    const Place pl = place_of(a, row);
+    const bool is_q = h < a.heads, is_k = !is_q && h < a.heads + a.kv_heads;
+    const uint32_t kh = h - a.heads - (is_k ? 0u : a.kv_heads);
+    const IN *src = is_q   ? (const IN *)a.q + (size_t)row * a.q_stride + (size_t)h * a.hd
+                    : is_k ? (const IN *)a.k + (size_t)row * a.k_stride + (size_t)kh * a.hd
+                           : (const IN *)a.v + (size_t)row * a.v_stride + (size_t)kh * a.hd;
+    float x0[8], x1[8], s = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const uint32_t i = lane + 64u * j;
+        x0[j] = i < half ? (float)src[i] : 0.0f;
+        x1[j] = i < half ? (float)src[i + half] : 0.0f;
+        s = fmaf(x0[j], x0[j], fmaf(x1[j], x1[j], s));
+    }
+    const float *gamma = is_q ? a.q_gamma : is_k ? a.k_gamma : nullptr;
+    const float r = gamma ? 1.0f / sqrtf(wave_sum(s) / (float)a.hd + a.eps) : 1.0f;
+    if (is_q ? !pl.rotates : !pl.appends) return;
+    const size_t to = is_q ? ((size_t)row * a.heads + h) * a.hd : (pl.cache_row * a.kv_heads + kh) * a.hd;
+    KV *kv = (KV *)(is_k ? a.kc : a.vc);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const uint32_t i = lane + 64u * j;
+        if (i >= half) break;
+        float p = x0[j], n = x1[j];
+        if (gamma) {
+            p = p * r * gamma[i];
+            n = n * r * gamma[i + half];
+        }
+        if (is_q || is_k) {
+            const float *t = a.table + ((size_t)pl.pos * half + i) * 2;
+            const float c = t[0], sn = t[1], y = p * c - n * sn;
+            n = p * sn + n * c;
+            p = y;
+        }
+        if (is_q) {
+            ((OUT *)a.q_out)[to + i] = (OUT)p;
+            ((OUT *)a.q_out)[to + half + i] = (OUT)n;
+        } else {
+            kv[to + i] = (KV)p;
+            kv[to + half + i] = (KV)n;
+        }
+    }
+}
+
+template <typename IN, typename OUT, typename KV, int D>
+void launch_dim(janus_ctx *ctx, HeadArgs a) {
+    // 16 bytes of a binary16 half, or of a binary32 one
+    constexpr int E = sizeof(IN) == 2 ? 8 : 4;
+    constexpr uint32_t L = D / 2 / E;
+    const uint32_t units = a.heads + 2 * a.kv_heads;
+    // one head per lane group while that leaves CUs idle, then four
+    const bool many = (uint64_t)a.rows * units * L >= (uint64_t)ctx->num_cus * 4096u;
+    a.parts = many ? (units + 3) / 4 : units;
+    const uint32_t grid = (uint32_t)(((uint64_t)a.rows * a.parts * L + 255) / 256);
+    if (many) hipLaunchKernelGGL((head_kernel<IN, OUT, KV, D, E, 4>), dim3(grid), dim3(256), 0, ctx->stream, a);
+    else hipLaunchKernelGGL((head_kernel<IN, OUT, KV, D, E, 1>), dim3(grid), dim3(256), 0, ctx->stream, a);
+}
+
+template <typename IN, typename OUT, typename KV>
+void launch_types(janus_ctx *ctx, const HeadArgs &a) {
+    // the vector kernel reads and writes 16 bytes (8 of a binary16 output of binary32 rows) at a time
+    const uintptr_t ptrs = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.q_out | (uintptr_t)a.kc |
+                           (uintptr_t)a.vc | (uintptr_t)a.table | (uintptr_t)a.q_gamma | (uintptr_t)a.k_gamma;
+    const bool aligned = (ptrs & 15u) == 0 && ((a.q_stride | a.k_stride | a.v_stride) * sizeof(IN) & 15u) == 0;
+    if (aligned && a.hd == 64) launch_dim<IN, OUT, KV, 64>(ctx, a);
+    else if (aligned && a.hd == 128) launch_dim<IN, OUT, KV, 128>(ctx, a);
+    else if (aligned && a.hd == 256) launch_dim<IN, OUT, KV, 256>(ctx, a);
+    else {
+        const uint64_t heads = (uint64_t)a.rows * (a.heads + 2 * a.kv_heads);
+        hipLaunchKernelGGL((head_any_kernel<IN, OUT, KV>), dim3((uint32_t)((heads + 3) / 4)), dim3(256), 0, ctx->stream, a);
+    }
+}
+
+template <typename IN, typename OUT>
+void launch_kv(janus_ctx *ctx, const HeadArgs &a, int kv_dt) {
+    if (kv_dt == JANUS_DT_F16) launch_types<IN, OUT, _Float16>(ctx, a);
+    else launch_types<IN, OUT, float>(ctx, a);
+}
+
+}  // namespace
+
+int qk_norm_rope_launch(janus_ctx *ctx, const void *q, const void *k, const void *v, int in_dt, uint32_t q_stride,
+                        uint32_t k_stride, uint32_t v_stride, const float *q_gamma, const float *k_gamma, float eps,
+                        const float *table, void *q_out, int out_dt, void *kc, void *vc, int kv_dt, uint32_t rows,
+                        uint32_t heads, uint32_t kv_heads, uint32_t hd, uint32_t position, uint32_t max_seq,
+                        const int32_t *row_base, const int32_t *positions) {
+    const HeadArgs a{q, k, v, q_stride, k_stride, v_stride, q_gamma, k_gamma, table, q_out, kc, vc,
+                     row_base, positions, rows, heads, kv_heads, hd, position, max_seq, 0, eps};
+    if (in_dt == JANUS_DT_F16) {
+        if (out_dt == JANUS_DT_F16) launch_kv<_Float16, _Float16>(ctx, a, kv_dt);
+        else launch_kv<_Float16, float>(ctx, a, kv_dt);
+    } else {
+        if (out_dt == JANUS_DT_F16) launch_kv<float, _Float16>(ctx, a, kv_dt);
+        else launch_kv<float, float>(ctx, a, kv_dt);
+    }
+    JANUS_LAUNCH_CHECK(ctx);
+    return JANUS_OK;
+}
+
+}  // namespace janus

@@ -274,6 +274,23 @@ bool prefill_attention_supported(uint32_t hd);
 int prefill_attention_launch(janus_ctx *ctx, const float *q, const void *kc, const void *vc, int kv_dt, void *out,
                              uint32_t n, uint32_t p0, uint32_t heads, uint32_t kv_heads, uint32_t hd, float scale,
                              int out_f16);
+// Attention of packed rows (packed.hip); q and out are of q_dt. Split partials
+// go into the context's attention workspace, grown on demand.
+int prompt_attention_launch(janus_ctx *ctx, const void *q, int q_dt, const void *kc, const void *vc, int kv_dt,
+                            void *out, uint32_t rows, uint32_t nseq, uint32_t heads, uint32_t kv_heads, uint32_t hd,
+                            uint32_t max_seq, const int32_t *q_start, const int32_t *row_base,
+                            const int32_t *seq_lens, uint32_t max_len, float scale);
+int prefix_attention_launch(janus_ctx *ctx, const void *q, int q_dt, const void *kc, const void *vc, int kv_dt,
+                            void *out, uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t hd,
+                            uint32_t prefix_row, uint32_t prefix_len, uint32_t seq_len, uint32_t max_seq,
+                            const int32_t *row_base, const int32_t *seq_lens, uint32_t max_len, float scale);
+// RMS norm of the q and k heads (gammas may be null), rotation, KV append
+// (headnorm.hip); strides in elements from a row to the next.
+int qk_norm_rope_launch(janus_ctx *ctx, const void *q, const void *k, const void *v, int in_dt, uint32_t q_stride,
+                        uint32_t k_stride, uint32_t v_stride, const float *q_gamma, const float *k_gamma, float eps,
+                        const float *table, void *q_out, int out_dt, void *kc, void *vc, int kv_dt, uint32_t rows,
+                        uint32_t heads, uint32_t kv_heads, uint32_t hd, uint32_t position, uint32_t max_seq,
+                        const int32_t *row_base, const int32_t *positions);
 // Looks up, once per device, the device address of the fixed attention
 // scratch (kAttnScratchBytes) and stores it in ctx->attn_scratch. Called by
 // janus_create with the context's device current.

@@ -187,6 +187,101 @@ int janus_attention_noalloc(janus_ctx *ctx, const float *q, const void *k_cache,
                             d_row_base, d_seq_lens, max_len, scale, 0, ctx->attn_scratch, kAttnScratchBytes);
 }
 
+namespace {
+// Host checks shared by the attentions of packed rows.
+int packed_args(janus_ctx *ctx, const char *name, const void *q, int q_dt, const void *k_cache, const void *v_cache,
+                int kv_dt, const void *out, uint32_t heads, uint32_t kv_heads, uint32_t hd) {
+    const std::string n = name;
+    if (!q || !k_cache || !v_cache || !out) return fail(ctx, JANUS_E_INVALID_ARG, n + ": null buffer");
+    if ((((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) & 15u) != 0)
+        return fail(ctx, JANUS_E_INVALID_ARG, n + ": q, the caches and out must be 16-byte aligned");
+    if (!is_act_dtype(q_dt) || !is_act_dtype(kv_dt))
+        return fail(ctx, JANUS_E_UNSUPPORTED_DTYPE, n + ": rows and cache must be F32 or F16");
+    if (q_dt == JANUS_DT_F16 && kv_dt != JANUS_DT_F16)
+        return fail(ctx, JANUS_E_UNSUPPORTED_DTYPE, n + ": F16 rows need an F16 cache");
+    if (kv_heads == 0 || heads == 0 || heads % kv_heads)
+        return fail(ctx, JANUS_E_INVALID_DIM, n + ": heads must be a multiple of kv_heads");
+    if (hd != 64 && hd != 128) return fail(ctx, JANUS_E_INVALID_DIM, n + ": head_dim must be 64 or 128");
+    if (heads > 65536u) return fail(ctx, JANUS_E_INVALID_DIM, n + ": more than 65536 heads");
+    return JANUS_OK;
+}
+}  // namespace
+
+int janus_prompt_attention(janus_ctx *ctx, const void *q, int q_dt, const void *k_cache, const void *v_cache,
+                           int kv_dt, void *out, uint32_t rows, uint32_t nseq, uint32_t heads, uint32_t kv_heads,
+                           uint32_t hd, uint32_t max_seq_len, const int32_t *d_q_start, const int32_t *d_row_base,
+                           const int32_t *d_seq_lens, uint32_t max_len_hint, float scale) {
+    if (check_ctx(ctx)) return JANUS_E_INVALID_ARG;
+    if (int e = packed_args(ctx, "prompt_attention", q, q_dt, k_cache, v_cache, kv_dt, out, heads, kv_heads, hd))
+        return e;
+    if (rows == 0 || nseq == 0) return JANUS_OK;
+    if (!d_q_start && rows % nseq)
+        return fail(ctx, JANUS_E_INVALID_DIM, "prompt_attention: without q_start, rows must be a multiple of nseq");
+    if (!d_q_start && !d_seq_lens && rows / nseq > max_seq_len)
+        return fail(ctx, JANUS_E_KV_OVERFLOW, "prompt_attention: rows of a sequence exceed max_seq_len");
+    if (int e = need_device(ctx)) return e;
+    DeviceGuard g(ctx->device);
+    if (!(scale > 0.0f)) scale = 1.0f / sqrtf((float)hd);
+    return prompt_attention_launch(ctx, q, q_dt, k_cache, v_cache, kv_dt, out, rows, nseq, heads, kv_heads, hd,
+                                   max_seq_len, d_q_start, d_row_base, d_seq_lens,
+                                   max_len_hint ? max_len_hint : max_seq_len, scale);
+}
+
+int janus_prefix_attention(janus_ctx *ctx, const void *q, int q_dt, const void *k_cache, const void *v_cache,
+                           int kv_dt, void *out, uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t hd,
+                           uint32_t prefix_row, uint32_t prefix_len, uint32_t seq_len, uint32_t max_seq_len,
+                           const int32_t *d_row_base, const int32_t *d_seq_lens, uint32_t max_len_hint, float scale) {
+    if (check_ctx(ctx)) return JANUS_E_INVALID_ARG;
+    if (int e = packed_args(ctx, "prefix_attention", q, q_dt, k_cache, v_cache, kv_dt, out, heads, kv_heads, hd))
+        return e;
+    if (!d_seq_lens && seq_len > max_seq_len)
+        return fail(ctx, JANUS_E_KV_OVERFLOW, "prefix_attention: seq_len exceeds max_seq_len");
+    if (prefix_row > 0x7fffffffu || prefix_len > 0x7fffffffu)
+        return fail(ctx, JANUS_E_INVALID_DIM, "prefix_attention: prefix beyond 2^31 rows");
+    if (batch == 0) return JANUS_OK;
+    if (int e = need_device(ctx)) return e;
+    DeviceGuard g(ctx->device);
+    if (!(scale > 0.0f)) scale = 1.0f / sqrtf((float)hd);
+    const uint32_t max_len = d_seq_lens ? (max_len_hint ? max_len_hint : max_seq_len) : seq_len;
+    return prefix_attention_launch(ctx, q, q_dt, k_cache, v_cache, kv_dt, out, batch, heads, kv_heads, hd, prefix_row,
+                                   prefix_len, seq_len, max_seq_len, d_row_base, d_seq_lens, max_len, scale);
+}
+
+int janus_qk_norm_rope(janus_ctx *ctx, const void *q, const void *k, const void *v, int in_dt, uint32_t q_stride,
+                       uint32_t k_stride, uint32_t v_stride, const float *q_gamma, const float *k_gamma, float eps,
+                       const float *d_table, void *q_out, int out_dt, void *k_cache, void *v_cache, int kv_dt,
+                       uint32_t rows, uint32_t heads, uint32_t kv_heads, uint32_t hd, uint32_t position,
+                       uint32_t max_seq_len, const int32_t *d_row_base, const int32_t *d_positions) {
+    if (check_ctx(ctx)) return JANUS_E_INVALID_ARG;
+    if (!q || !k || !v || !d_table || !q_out || !k_cache || !v_cache)
+        return fail(ctx, JANUS_E_INVALID_ARG, "qk_norm_rope: null buffer");
+    if (!is_act_dtype(in_dt) || !is_act_dtype(out_dt) || !is_act_dtype(kv_dt))
+        return fail(ctx, JANUS_E_UNSUPPORTED_DTYPE, "qk_norm_rope: rows, output and cache must be F32 or F16");
+    if (hd == 0 || hd % 2 || hd > 1024)
+        return fail(ctx, JANUS_E_INVALID_DIM, "qk_norm_rope: head_dim must be even, at most 1024");
+    if (heads == 0 || kv_heads == 0 || heads > 65536u || kv_heads > 65536u)
+        return fail(ctx, JANUS_E_INVALID_DIM, "qk_norm_rope: 1 to 65536 heads");
+    if (!q_stride) q_stride = heads * hd;
+    if (!k_stride) k_stride = kv_heads * hd;
+    if (!v_stride) v_stride = kv_heads * hd;
+    if (q_stride < heads * hd || k_stride < kv_heads * hd || v_stride < kv_heads * hd)
+        return fail(ctx, JANUS_E_INVALID_DIM, "qk_norm_rope: a row stride is shorter than the row");
+    if (q == q_out && (in_dt != out_dt || q_stride != heads * hd))
+        return fail(ctx, JANUS_E_INVALID_ARG, "qk_norm_rope: in place only for contiguous rows of one type");
+    if (!d_positions && position >= max_seq_len)
+        return fail(ctx, JANUS_E_KV_OVERFLOW, "KV cache position " + std::to_string(position) +
+                                                  " exceeds max_seq_len " + std::to_string(max_seq_len));
+    if (rows == 0) return JANUS_OK;
+    // one launch: at most 2^32 lanes, 64 for a head of any size
+    if ((uint64_t)rows * ((uint64_t)heads + 2 * kv_heads) >= (1ull << 26))
+        return fail(ctx, JANUS_E_INVALID_DIM, "qk_norm_rope: more rows than one launch takes");
+    if (int e = need_device(ctx)) return e;
+    DeviceGuard g(ctx->device);
+    return qk_norm_rope_launch(ctx, q, k, v, in_dt, q_stride, k_stride, v_stride, q_gamma, k_gamma, eps, d_table,
+                               q_out, out_dt, k_cache, v_cache, kv_dt, rows, heads, kv_heads, hd, position,
+                               max_seq_len, d_row_base, d_positions);
+}
+
 int janus_embed(janus_ctx *ctx, const janus_weight *table, const uint32_t *h_ids, uint32_t batch, float *out) {
     if (check_ctx(ctx)) return JANUS_E_INVALID_ARG;
     if (!table || !h_ids || !out) return fail(ctx, JANUS_E_INVALID_ARG, "embed: null argument");

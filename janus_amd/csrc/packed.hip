@@ -1,0 +1,614 @@
+// packed.hip -- attention of packed rows over the KV cache: causal attention of
+// the prompts, chunks and drafted tokens of several requests in one launch, and
+// decode attention of a batch behind a shared prefix.
+//
+// The queries of a KV head that read the same K and V are the columns of one
+// matrix product: column c of a sequence of n rows is query head c % G of its
+// row c / G (G heads per KV head), so few rows of many heads fill a tile as many
+// rows of few heads do, and K and V are read once for all of them. A workgroup
+// takes 128 columns (four wavefronts of 32), passes over the positions in tiles
+// that go through LDS, and keeps the running maximum m, the sum l and the output
+// O^T in registers:
+//   S^T = K Q^T (positions x columns), p = 2^(scale log2(e) (s - m)),
+//   l <- l 2^(m_old - m) + sum p,  O^T <- O^T 2^(m_old - m) + V^T P^T.
+// A lane's column is one query, so m, l and the rescale are per lane, and P is
+// the second product's operand as it lies; V's operand is read from LDS with the
+// transposing load in the position order that matches.
+//   binary16 rows and cache: v_mfma_f32_32x32x16_f16, P rounded to binary16 (its
+//     errors average out over the positions and stay below the output's own
+//     rounding);
+//   binary32 rows, binary16 cache: q and P in two binary16 parts each (22 bits);
+//   binary32 rows and cache: v_mfma_f32_32x32x2_f32, nothing rounded.
+// m follows the maximum only when that would grow by more than a few powers of
+// two (an exponent bias leaves P room), so most tiles rescale nothing.
+//
+// Few columns on a long context: the positions are split over workgroups, each
+// of which writes (m, l) and its output, and a second launch joins them. A
+// shared prefix is a sequence of its own with one row per request and no causal
+// limit; its parts and those of the requests' own positions are joined alike.
+#include <algorithm>
+
+#include "internal.h"
+
+namespace janus {
+namespace {
+
+typedef _Float16 ph8 __attribute__((ext_vector_type(8)));
+typedef short ps4 __attribute__((ext_vector_type(4)));
+typedef float pf16 __attribute__((ext_vector_type(16)));
+
+constexpr uint32_t COLS = 128;   // columns per workgroup
+
+struct PackedArgs {
+    const void *q;            // [rows][heads][D]
+    const void *kc, *vc;      // [cache rows][kv_heads][D]
+    void *out;                // [rows][heads][D]
+    float *part;              // split: [rows][heads][slots][D], then (m, l) [rows][heads][slots][2]
+    float *part_ml;
+    const int32_t *q_start;   // [nseq + 1], or null: rows / nseq rows each
+    const int32_t *row_base;  // null: s * max_seq
+    const int32_t *seq_lens;  // null: seq_len, or as many as the sequence has rows
+    uint32_t rows, nseq, heads, kv_heads, G;
+    uint32_t max_seq;
+    int64_t seq_len;          // < 0: the rows
+    uint32_t splits;          // workgroups per tile (prefix: per own tile)
+    uint32_t slots;           // partials per row and head (0: results are written)
+    uint32_t prefix_row, prefix_len, prefix_tiles, prefix_splits;
+    float scale2;             // scale * log2(e)
+};
+
+// What a workgroup works on.
+struct Work {
+    uint32_t row0, n;         // rows of the sequence (of the batch, for a prefix)
+    uint32_t c0;              // first column
+    size_t kv_row;            // cache row of position 0
+    uint32_t len;             // positions
+    bool causal;
+    uint32_t split, splits, slot;
+};
+
+__device__ __forceinline__ float swap32(float v) {   // value of lane ^ 32
+    const uint32_t u = __float_as_uint(v);
+    auto p = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __uint_as_float((__lane_id() & 32) ? p[0] : p[1]);
+}
+
+// Rows [first, first + n) and positions of sequence s; whatever the tables hold,
+// rows stay inside [0, rows) and len within [0, max_seq].
+__device__ __forceinline__ void rows_of(const PackedArgs &a, uint32_t s, uint32_t &first, uint32_t &n) {
+    const int32_t lim = (int32_t)a.rows, b = min(max(a.q_start[s], 0), lim), e = min(max(a.q_start[s + 1], b), lim);
+    first = (uint32_t)b;
+    n = (uint32_t)(e - b);
+}
+
+__device__ __forceinline__ void context_of(const PackedArgs &a, uint32_t s, Work &w) {
+    const int64_t base = a.row_base ? (int64_t)a.row_base[s] : (int64_t)s * a.max_seq;
+    const uint32_t len = a.seq_lens ? (uint32_t)max(a.seq_lens[s], 0) : a.seq_len < 0 ? w.n : (uint32_t)a.seq_len;
+    w.len = base < 0 ? 0u : min(len, a.max_seq);
+    w.kv_row = base < 0 ? 0 : (size_t)base;
+}
+
+// The sequence and tile of tile number t (sequences in order, a sequence's tiles
+// from its last to its first, the longest first); false: there is none.
+__device__ __forceinline__ bool find_tile(const PackedArgs &a, uint32_t t, Work &w) {
+    const uint32_t lane = threadIdx.x & 63u;
+    w.causal = true;
+    if (!a.q_start) {
+        w.n = a.rows / a.nseq;
+        const uint32_t each = (uint32_t)(((uint64_t)w.n * a.G + COLS - 1) / COLS), s = t / each;
+        if (s >= a.nseq) return false;
+        w.row0 = s * w.n;
+        w.c0 = (each - 1 - t % each) * COLS;
+        context_of(a, s, w);
+        return true;
+    }
+    for (uint32_t s0 = 0; s0 < a.nseq; s0 += 64) {
+        uint32_t first = 0, n = 0;
+        if (s0 + lane < a.nseq) rows_of(a, s0 + lane, first, n);
+        const uint32_t mine = (uint32_t)(((uint64_t)n * a.G + COLS - 1) / COLS);
+        uint32_t upto = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t v = __shfl_up(upto, o, 64);
+            if ((int)lane >= o) upto += v;
+        }
+        const uint64_t hit = __ballot(t < upto);
+        if (hit) {
+            const int at = __ffsll((unsigned long long)hit) - 1;
+            const uint32_t s = s0 + at;
+            const uint32_t before = __builtin_amdgcn_readlane(upto - mine, at);
+            w.row0 = __builtin_amdgcn_readlane(first, at);
+            w.n = __builtin_amdgcn_readlane(n, at);
+            w.c0 = (__builtin_amdgcn_readlane(mine, at) - 1 - (t - before)) * COLS;
+            context_of(a, s, w);
+            return true;
+        }
+        t -= __builtin_amdgcn_readlane(upto, 63);
+    }
+    return false;
+}
+
+// LDS of a tile of TP positions: K rows, then V rows, 16-byte segments permuted
+// within a row so that the reads below meet each bank as rarely as they can.
+//   K: 32 lanes read a segment of 32 rows; V binary16: 16 lanes read 32 bytes of
+//   each of 4 rows (transposing read); V binary32: 32 lanes read 128 bytes of a
+//   row, the other half of the wavefront the row 4 below.
+template <typename KV, int D> struct Lay {
+    static constexpr uint32_t RB = D * sizeof(KV), SEGS = RB / 16;
+    static __device__ __forceinline__ uint32_t k_swz(uint32_t row) {
+        return SEGS >= 16 ? (row & 15u) : (((row >> 1) & 7u) ^ ((row & 1u) << 2));
+    }
+    static __device__ __forceinline__ uint32_t v_swz(uint32_t row) {
+        return sizeof(KV) == 4 ? ((row >> 2) & 1u) << 3 : SEGS >= 16 ? (row & 3u) << 2 : ((row >> 1) & 1u) << 2;
+    }
+};
+
+// Sum that is NaN exactly if the 16 bytes hold an infinity or NaN.
+template <typename KV> __device__ __forceinline__ float odd_sum(const ju4 &v, float s) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(KV) == 2) s = __builtin_amdgcn_fdot2(__builtin_bit_cast(jh2, (uint32_t)v[i]), (jh2)(_Float16)0.0f, s, false);
+        else s = fmaf(__uint_as_float(v[i]), 0.0f, s);
+    }
+    return s;
+}
+
+// The finite values of the 16 bytes, others as 0.
+template <typename KV> __device__ __forceinline__ ju4 finite_part(ju4 v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(KV) == 2) {
+            if ((v[i] & 0x7c00u) == 0x7c00u) v[i] &= 0xffff0000u;
+            if ((v[i] & 0x7c000000u) == 0x7c000000u) v[i] &= 0xffffu;
+        } else if ((v[i] & 0x7f800000u) == 0x7f800000u) {
+            v[i] = 0u;
+        }
+    }
+    return v;
+}
+
+// Q: _Float16 or float rows; KV: the cache's type.
+template <typename Q, typename KV, int D>
+__global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedArgs a) {
+    constexpr bool H = sizeof(KV) == 2;            // binary16 cache
+    constexpr bool TWO = H && sizeof(Q) == 4;      // q and P in two parts
+    constexpr int TP = sizeof(Q) == 2 ? 64 : 32;   // positions per tile
+    constexpr int NB = TP / 32, ND = D / 32;
+    typedef Lay<KV, D> Y;
+    constexpr uint32_t VB = TP * Y::RB, FLAGS = 2 * VB, BUF = FLAGS + 16;   // bytes of a buffer
+    constexpr int LD = TP * Y::SEGS / 256;         // 16-byte segments per thread, of K and of V
+    static_assert(LD >= 1 && LD * 256 == TP * (int)Y::SEGS, "tile load");
+    // p carries 2^BIAS; m may lag behind the maximum by 2^SLACK (p stays below 2^16)
+    constexpr float BIAS = !H ? 0.0f : TWO ? 13.0f : 6.0f, SLACK = !H ? 8.0f : TWO ? 2.0f : 8.0f;
+    extern __shared__ __align__(16) unsigned char smem[];
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t col = lane & 31u, h = lane >> 5;
+
+    // neighbouring workgroups take the KV heads, so that with 8 of them each XCD
+    // keeps the K and V of one head in its L2
+    const uint32_t kvh = blockIdx.x % a.kv_heads, id = blockIdx.x / a.kv_heads;
+    Work w;
+    if (id < a.prefix_tiles * a.prefix_splits) {
+        w.split = id % a.prefix_splits;
+        w.splits = a.prefix_splits;
+        w.slot = w.split;
+        w.row0 = 0;
+        w.n = a.rows;
+        w.c0 = id / a.prefix_splits * COLS;
+        w.kv_row = a.prefix_row;
+        w.len = a.prefix_len;
+        w.causal = false;
+    } else {
+        const uint32_t rest = id - a.prefix_tiles * a.prefix_splits;
+        w.split = rest % a.splits;
+        w.splits = a.splits;
+        w.slot = a.prefix_splits + w.split;
+        if (!find_tile(a, rest / a.splits, w)) return;
+    }
+    const uint32_t ncols = w.n * a.G;   // n * G <= rows * heads < 2^32
+    // positions that row i sees: the first len, or len - n + 1 + i
+    auto seen_of = [&](uint32_t i) -> uint32_t {
+        if (!w.causal) return w.len;
+        const int64_t s = (int64_t)w.len - w.n + 1 + i;
+        return s < 0 ? 0u : (uint32_t)s;
+    };
+    const uint32_t wc0 = w.c0 + 32u * wave;
+    const bool idle = wc0 >= ncols;     // uniform: this wavefront only helps to load
+    const uint32_t wave_lo = idle ? 0u : seen_of(wc0 / a.G), wave_hi = idle ? 0u : seen_of(min(wc0 + 31u, ncols - 1) / a.G);
+    const uint32_t end_all = seen_of(min(w.c0 + COLS - 1, ncols - 1) / a.G);
+    // this workgroup's part of the positions
+    const uint32_t per = (((end_all + w.splits - 1) / w.splits) + TP - 1) / TP * TP;
+    const uint32_t p0 = min(w.split * per, end_all), p1 = min(p0 + per, end_all);
+
+    const uint32_t c = min(wc0 + col, ncols - 1), qrow = c / a.G, head = kvh * a.G + c % a.G;
+    const bool mine = wc0 + col < ncols;
+    const uint32_t seen = seen_of(qrow);
+    const size_t qat = ((size_t)(w.row0 + qrow) * a.heads + head);
+
+    const uint32_t kvrow = a.kv_heads * Y::RB;   // bytes from a position to the next
+    const unsigned char *kc = (const unsigned char *)a.kc + (w.kv_row * a.kv_heads + kvh) * Y::RB;
+    const unsigned char *vc = (const unsigned char *)a.vc + (w.kv_row * a.kv_heads + kvh) * Y::RB;
+
+    ju4 kr[LD], vr[LD];
+    auto load = [&](uint32_t p) {
+        const unsigned char *kp = kc + (size_t)p * kvrow, *vp = vc + (size_t)p * kvrow;
+        const uint32_t last = p1 - 1 - p;   // rows beyond the part repeat its last one
+#pragma unroll
+        for (int j = 0; j < LD; ++j) {
+            const uint32_t s = threadIdx.x + 256u * j, off = min(s / Y::SEGS, last) * kvrow + s % Y::SEGS * 16u;
+            kr[j] = *(const ju4 *)(kp + off);
+            vr[j] = *(const ju4 *)(vp + off);
+        }
+    };
+    auto store = [&](unsigned char *t) {
+        float oddv = 0.0f, oddk = 0.0f;
+#pragma unroll
+        for (int j = 0; j < LD; ++j) {
+            oddv = odd_sum<KV>(vr[j], oddv);
+            if (TWO) oddk = odd_sum<KV>(kr[j], oddk);
+        }
+        const uint32_t any = (uint32_t)(__any(oddv != oddv) != 0) | (uint32_t)(__any(oddk != oddk) != 0) << 1;
+        if (lane == 0) *(uint32_t *)(t + FLAGS + 4 * wave) = any;
+        // A probability of 0 does not mask an infinity or NaN of V: such values stay
+        // out of the products and are added on their own, for the rows that see them.
+        if (any & 1u)
+#pragma unroll
+            for (int j = 0; j < LD; ++j) vr[j] = finite_part<KV>(vr[j]);
+#pragma unroll
+        for (int j = 0; j < LD; ++j) {
+            const uint32_t s = threadIdx.x + 256u * j, row = s / Y::SEGS, seg = s % Y::SEGS;
+            *(ju4 *)(t + row * Y::RB + (seg ^ Y::k_swz(row)) * 16u) = kr[j];
+            *(ju4 *)(t + VB + row * Y::RB + (seg ^ Y::v_swz(row)) * 16u) = vr[j];
+        }
+    };
+    if (p0 < p1) load(p0);
+
+    // q of this lane's column
+    const Q *qp = (const Q *)a.q + qat * D;
+    constexpr int QN = H ? D / 16 : 1;
+    ph8 qh[QN], ql[TWO ? QN : 1];
+    jf4 qf[H ? 1 : D / 8];
+    float sc2 = a.scale2, qs = 1.0f;
+    bool q_inf = false;
+    if constexpr (!H) {
+#pragma unroll
+        for (int s = 0; s < D / 8; ++s) qf[s] = *(const jf4 *)(qp + 8 * s + 4 * h);
+    } else if constexpr (!TWO) {
+#pragma unroll
+        for (int s = 0; s < QN; ++s) qh[s] = *(const ph8 *)(qp + 16 * s + 8 * h);
+    } else {
+        // scaled so that the largest element is 2^14 .. 2^15: the parts hold 22 bits of
+        // it, and of the others down to 2^-39 of it
+        float qmax = 0.0f;
+        jf4 x[QN][2];
+#pragma unroll
+        for (int s = 0; s < QN; ++s) {
+            x[s][0] = *(const jf4 *)(qp + 16 * s + 8 * h);
+            x[s][1] = *(const jf4 *)(qp + 16 * s + 8 * h + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) qmax = fmaxf(qmax, fmaxf(fabsf(x[s][0][i]), fabsf(x[s][1][i])));
+        }
+        qmax = fmaxf(qmax, swap32(qmax));
+        int qe = 0;
+        (void)frexpf(qmax, &qe);
+        const int sh = max(qe - 15, -100);
+        qs = ldexpf(1.0f, -sh);
+        q_inf = __any(qmax == INFINITY);
+        sc2 *= ldexpf(1.0f, sh);
+#pragma unroll
+        for (int s = 0; s < QN; ++s)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float y = x[s][i >> 2][i & 3] * qs;
+                const _Float16 hi = (_Float16)y;
+                qh[s][i] = hi;
+                ql[s][i] = (_Float16)(y - (float)hi);
+            }
+    }
+
+    pf16 o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[d] = (pf16){};
+    float m = -INFINITY, l = 0.0f;
+
+    if (p0 < p1) store(smem);
+    uint32_t buf = 0;
+    for (uint32_t p = p0; p < p1; p += TP) {
+        const bool more = p + TP < p1;
+        if (more) load(p + TP);
+        __syncthreads();
+        const unsigned char *kt = smem + buf * BUF, *vt = kt + VB;
+        if (p < wave_hi) {
+            const uint4 f = *(const uint4 *)(kt + FLAGS);
+            const uint32_t flags = __builtin_amdgcn_readfirstlane(f.x | f.y | f.z | f.w);
+            pf16 s[NB];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                s[b] = (pf16){};
+                const uint32_t row = 32u * b + col, swz = Y::k_swz(row);
+                if constexpr (H) {
+                    pf16 lo = (pf16){};
+#pragma unroll
+                    for (int t = 0; t < QN; ++t) {
+                        const ph8 k = *(const ph8 *)(kt + row * Y::RB + ((2u * t + h) ^ swz) * 16u);
+                        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[t], s[b], 0, 0, 0);
+                        if constexpr (TWO) lo = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[t], lo, 0, 0, 0);
+                    }
+                    if constexpr (TWO) {
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) s[b][v] += lo[v];
+                    }
+                } else {
+                    pf16 s2 = (pf16){};
+#pragma unroll
+                    for (int t = 0; t < D / 8; ++t) {
+                        const jf4 k = *(const jf4 *)(kt + row * Y::RB + ((2u * t + h) ^ swz) * 16u);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if (t & 1) s2 = __builtin_amdgcn_mfma_f32_32x32x2f32(k[i], qf[t][i], s2, 0, 0, 0);
+                            else s[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(k[i], qf[t][i], s[b], 0, 0, 0);
+                        }
+                    }
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) s[b][v] += s2[v];
+                }
+            }
+            if constexpr (TWO)
+                // an infinity times a part of q that is 0 or of the other sign would make
+                // a NaN of an infinite score: such tiles take q whole
+                if (q_inf || (flags & 2u)) {
+                    s[0] = (pf16){};
+#pragma unroll 1
+                    for (uint32_t d = 0; d < D; ++d) {
+                        const float x = (float)qp[d];
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) {
+                            const uint32_t row = 8u * (v >> 2) + 4u * h + (v & 3);
+                            s[0][v] = fmaf(x, (float)*(const _Float16 *)(kt + row * Y::RB + ((d / 8) ^ Y::k_swz(row)) * 16u + d % 8 * 2u), s[0][v]);
+                        }
+                    }
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) s[0][v] *= qs;
+                }
+            // s[b][v]: position p + 32 b + 8 (v / 4) + 4 h + v % 4
+            if (p + TP > min(wave_lo, p1)) {
+                const uint32_t lim = min(seen, p1);
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v)
+                        s[b][v] = p + 32 * b + 8 * (v >> 2) + 4 * h + (v & 3) < lim ? s[b][v] : -INFINITY;
+            }
+            float bm = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) bm = fmaxf(bm, s[b][v]);
+            bm = fmaxf(bm, swap32(bm));
+            if (__any((bm - m) * sc2 > SLACK || (m == -INFINITY && bm != -INFINITY))) {
+                const float mn = fmaxf(m, bm), alpha = mn == m ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * sc2);
+                m = mn;
+                l *= alpha;
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) o[d][v] *= alpha;
+            }
+            // while only masked or NaN scores have come, m counts as 0: 2^-inf is 0, a NaN stays
+            const float mr = m == -INFINITY ? 0.0f : m, ms = sizeof(Q) == 2 ? BIAS - mr * sc2 : 0.0f;
+            float sum = 0.0f;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    // binary32 rows: the difference is exact near the maximum
+                    s[b][v] = sizeof(Q) == 2 ? __builtin_amdgcn_exp2f(fmaf(s[b][v], sc2, ms))
+                                             : __builtin_amdgcn_exp2f(fmaf(s[b][v] - mr, sc2, BIAS));
+                    sum += s[b][v];
+                }
+            l += sum;
+            if constexpr (H) {
+                // lanes 16 g + i of half h read dims 32 d + 16 g + 4 (i % 4) .. of positions
+                // 4 h + i / 4 (+ 8) of a step and receive dim 32 d + 16 g + i of four positions
+                const uint32_t i = lane & 15u, g = (lane >> 4) & 1u;
+                const uint32_t vrow = 4u * h + (i >> 2), vseg = 2u * g + ((i & 3u) >> 1), vin = (i & 1u) * 8u;
+#pragma unroll
+                for (int t = 0; t < 2 * NB; ++t) {
+                    ph8 ph, pl;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float x = s[t >> 1][8 * (t & 1) + e];
+                        ph[e] = (_Float16)x;
+                        if constexpr (TWO) pl[e] = (_Float16)(x - (float)ph[e]);
+                    }
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) {
+                        const uint32_t at = (16u * t + vrow) * Y::RB + ((4u * d + vseg) ^ Y::v_swz(vrow)) * 16u + vin;
+                        typedef __attribute__((address_space(3))) ps4 *lds4;
+                        const ps4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(vt + at));
+                        const ps4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(vt + at + 8 * Y::RB));
+                        const ph8 v = __builtin_bit_cast(ph8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph, o[d], 0, 0, 0);
+                        if constexpr (TWO) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl, o[d], 0, 0, 0);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    const uint32_t row = 8u * (v >> 2) + 4u * h + (v & 3);
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) {
+                        const float x = *(const float *)(vt + row * Y::RB + ((8u * d + (col >> 2)) ^ Y::v_swz(row)) * 16u + (col & 3u) * 4u);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, s[0][v], o[d], 0, 0, 0);
+                    }
+                }
+            }
+            if (flags & 1u) {
+                // the infinities and NaN of V, for the columns that see their position
+                const uint32_t lim = min(seen, p1);
+#pragma unroll 1
+                for (uint32_t j = 0; j < min((uint32_t)TP, p1 - p); ++j) {
+                    float ph = 0.0f;   // p of position j, held by half (j / 4) % 2
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) ph = 32u * b + 8u * (v >> 2) + (v & 3) + (j & 4u) == j ? s[b][v] : ph;
+                    const float other = swap32(ph), pj = ((j >> 2) & 1u) == h ? ph : other;
+                    const KV *vrow = (const KV *)(vc + (size_t)(p + j) * kvrow);
+#pragma unroll
+                    for (int d = 0; d < ND; ++d)
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) {
+                            const float x = (float)vrow[32 * d + 8 * (v >> 2) + 4 * h + (v & 3)];
+                            if (p + j < lim && (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u) o[d][v] = fmaf(pj, x, o[d][v]);
+                        }
+                }
+            }
+        }
+        buf ^= 1u;
+        if (more) store(smem + buf * BUF);   // last read before the barrier above
+    }
+    if (idle || !mine) return;
+    l += swap32(l);
+    if (a.slots) {
+        const size_t at = qat * a.slots + w.slot;
+        if (h == 0) *(float2 *)(a.part_ml + 2 * at) = make_float2(m / qs, l);
+        if (p0 >= p1) return;   // the join reads no output of a part without positions
+        float *to = a.part + at * D;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                *(jf4 *)(to + 32 * d + 8 * j + 4 * h) = jf4{o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]};
+        return;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;   // a row that sees nothing is 0
+    Q *to = (Q *)a.out + qat * D;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            typedef Q q4 __attribute__((ext_vector_type(4)));
+            q4 y;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = (Q)(o[d][4 * j + i] * inv);
+            *(q4 *)(to + 32 * d + 8 * j + 4 * h) = y;
+        }
+}
+
+// Joins the parts of a row and head: a wavefront each. A part holds m, l and the
+// output before the division; one without positions has l = 0 and no output, one
+// with only NaN scores an m of -infinity and a NaN l.
+template <typename Q, int D>
+__global__ __launch_bounds__(256) void packed_join_kernel(PackedArgs a) {
+    const uint64_t at = (uint64_t)blockIdx.x * 4u + (threadIdx.x >> 6);
+    const uint32_t lane = threadIdx.x & 63u, row = (uint32_t)(at / a.heads);
+    if (row >= a.rows) return;
+    // rows outside the sequences are not written
+    if (a.q_start && ((int32_t)row < a.q_start[0] || (int32_t)row >= a.q_start[a.nseq])) return;
+    const float *ml = a.part_ml + at * a.slots * 2;
+    const float *part = a.part + at * a.slots * D;
+    constexpr int E = D / 64;
+    float M = -INFINITY;
+    for (uint32_t s = lane; s < a.slots; s += 64) M = fmaxf(M, ml[2 * s]);
+    M = wave_max(M);
+    float l = 0.0f, o[E] = {};
+    for (uint32_t s = 0; s < a.slots; ++s) {
+        const float ms = ml[2 * s], ls = ml[2 * s + 1];
+        if (ls == 0.0f) continue;
+        const float wgt = ms == M ? 1.0f : __builtin_amdgcn_exp2f((ms - M) * a.scale2);
+        l = fmaf(ls, wgt, l);
+#pragma unroll
+        for (int i = 0; i < E; ++i) o[i] = fmaf(part[(size_t)s * D + E * lane + i], wgt, o[i]);
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int i = 0; i < E; ++i) ((Q *)a.out)[at * D + E * lane + i] = (Q)(o[i] * inv);
+}
+
+template <typename Q, typename KV, int D>
+int launch(janus_ctx *ctx, const PackedArgs &a, uint32_t blocks) {
+    constexpr int TP = sizeof(Q) == 2 ? 64 : 32;
+    constexpr size_t lds = 2 * (2 * TP * D * sizeof(KV) + 16);
+    static const hipError_t attr = hipFuncSetAttribute((const void *)packed_attn_kernel<Q, KV, D>,
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    (void)attr;
+    hipLaunchKernelGGL((packed_attn_kernel<Q, KV, D>), dim3(blocks), dim3(256), lds, ctx->stream, a);
+    JANUS_LAUNCH_CHECK(ctx);
+    if (a.slots) {
+        const uint64_t heads = (uint64_t)a.rows * a.heads;
+        hipLaunchKernelGGL((packed_join_kernel<Q, D>), dim3((uint32_t)((heads + 3) / 4)), dim3(256), 0, ctx->stream, a);
+        JANUS_LAUNCH_CHECK(ctx);
+    }
+    return JANUS_OK;
+}
+
+int launch_typed(janus_ctx *ctx, const PackedArgs &a, int q_dt, int kv_dt, uint32_t hd, uint32_t blocks) {
+    if (q_dt == JANUS_DT_F16) return hd == 64 ? launch<_Float16, _Float16, 64>(ctx, a, blocks) : launch<_Float16, _Float16, 128>(ctx, a, blocks);
+    if (kv_dt == JANUS_DT_F16) return hd == 64 ? launch<float, _Float16, 64>(ctx, a, blocks) : launch<float, _Float16, 128>(ctx, a, blocks);
+    return hd == 64 ? launch<float, float, 64>(ctx, a, blocks) : launch<float, float, 128>(ctx, a, blocks);
+}
+
+// Workgroups per tile so that `tiles` of them fill the CUs about four times
+// over, each with 256 positions at least.
+uint32_t plan_splits(const janus_ctx *ctx, uint64_t tiles, uint32_t max_len) {
+    const uint64_t want = 4ull * ctx->num_cus / std::max<uint64_t>(tiles, 1);
+    return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(want, (max_len + 255) / 256));
+}
+
+int run(janus_ctx *ctx, PackedArgs a, int q_dt, int kv_dt, uint32_t hd, uint64_t tiles) {
+    const uint64_t blocks = tiles * a.kv_heads;
+    if (blocks * 256 >= (1ull << 32) || (uint64_t)a.rows * a.heads >= (1ull << 25))
+        return fail(ctx, JANUS_E_INVALID_DIM, "attention: more rows than one launch takes");
+    if (a.slots) {
+        const size_t parts = (size_t)a.rows * a.heads * a.slots;
+        if (int e = ensure_attn_ws(ctx, parts * (hd + 2) * sizeof(float))) return e;
+        a.part = (float *)ctx->attn_ws;
+        a.part_ml = a.part + parts * hd;
+    }
+    return launch_typed(ctx, a, q_dt, kv_dt, hd, (uint32_t)blocks);
+}
+
+}  // namespace
+
+int prompt_attention_launch(janus_ctx *ctx, const void *q, int q_dt, const void *kc, const void *vc, int kv_dt,
+                            void *out, uint32_t rows, uint32_t nseq, uint32_t heads, uint32_t kv_heads, uint32_t hd,
+                            uint32_t max_seq, const int32_t *q_start, const int32_t *row_base,
+                            const int32_t *seq_lens, uint32_t max_len, float scale) {
+    PackedArgs a{};
+    a.q = q; a.kc = kc; a.vc = vc; a.out = out;
+    a.q_start = q_start; a.row_base = row_base; a.seq_lens = seq_lens;
+    a.rows = rows; a.nseq = nseq; a.heads = heads; a.kv_heads = kv_heads; a.G = heads / kv_heads;
+    a.max_seq = max_seq;
+    a.seq_len = -1;
+    a.scale2 = scale * 1.4426950408889634f;
+    // at most so many tiles: every sequence's last one may be part empty
+    const uint64_t tiles = (uint64_t)rows * a.G / COLS + nseq;
+    a.splits = plan_splits(ctx, tiles * kv_heads, std::min(max_len, max_seq));
+    a.slots = a.splits > 1 ? a.splits : 0;
+    return run(ctx, a, q_dt, kv_dt, hd, tiles * a.splits);
+}
+
+int prefix_attention_launch(janus_ctx *ctx, const void *q, int q_dt, const void *kc, const void *vc, int kv_dt,
+                            void *out, uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t hd,
+                            uint32_t prefix_row, uint32_t prefix_len, uint32_t seq_len, uint32_t max_seq,
+                            const int32_t *row_base, const int32_t *seq_lens, uint32_t max_len, float scale) {
+    PackedArgs a{};
+    a.q = q; a.kc = kc; a.vc = vc; a.out = out;
+    a.row_base = row_base; a.seq_lens = seq_lens;
+    a.rows = a.nseq = batch; a.heads = heads; a.kv_heads = kv_heads; a.G = heads / kv_heads;
+    a.max_seq = max_seq;
+    a.seq_len = seq_len;
+    a.prefix_row = prefix_row; a.prefix_len = prefix_len;
+    a.scale2 = scale * 1.4426950408889634f;
+    const uint64_t own_tiles = (uint64_t)batch * ((a.G + COLS - 1) / COLS);
+    if (prefix_len) {
+        a.prefix_tiles = (uint32_t)(((uint64_t)batch * a.G + COLS - 1) / COLS);
+        a.prefix_splits = plan_splits(ctx, (uint64_t)a.prefix_tiles * kv_heads, prefix_len);
+    }
+    a.splits = plan_splits(ctx, own_tiles * kv_heads, std::min(max_len, max_seq));
+    a.slots = a.prefix_splits + a.splits > 1 ? a.prefix_splits + a.splits : 0;
+    return run(ctx, a, q_dt, kv_dt, hd, (uint64_t)a.prefix_tiles * a.prefix_splits + own_tiles * a.splits);
+}
+
+}  // namespace janus

@@ -246,6 +246,121 @@ def compute_attention_noalloc(engine, query, key_cache, value_cache, output, bat
         scale))
 
 
+# ---- heads and attention of packed rows ----------------------------------------------
+
+def _index(t: Optional[torch.Tensor], least: int, engine: ComputeEngine, name: str) -> Optional[int]:
+    """An int32 table of at least `least` entries on the engine's device, or None."""
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or t.numel() < least:
+        raise ValueError(f"{name}: an int32 tensor of {least} values")
+    return _on(t, engine, name)
+
+
+def _on(t: torch.Tensor, engine: ComputeEngine, name: str) -> int:
+    if t.is_cuda and t.device.index != engine.device:
+        raise ValueError(f"{name} is on {t.device}, the engine on cuda:{engine.device}")
+    return _ptr(t)
+
+
+def _heads3(t: torch.Tensor, name: str) -> tuple[int, int, int]:
+    if t.dim() != 3:
+        raise ValueError(f"{name}: [rows, heads, head_dim] expected, got {tuple(t.shape)}")
+    return tuple(t.shape)
+
+
+def _row_stride(t: torch.Tensor, engine: ComputeEngine, name: str) -> tuple[int, int]:
+    """(address, elements from a row to the next) of [rows, heads, head_dim]
+    whose rows are contiguous, such as a part of a fused product's rows."""
+    rows, heads, hd = t.shape
+    if not t.is_cuda or t.device.index != engine.device:
+        raise ValueError(f"{name}: a tensor on cuda:{engine.device} expected, got {t.device}")
+    if (t.stride(2) != 1 and hd > 1) or (t.stride(1) != hd and heads > 1) or (rows > 1 and t.stride(0) < heads * hd):
+        raise ValueError(f"{name}: the heads of a row must be contiguous")
+    return t.data_ptr(), t.stride(0) if rows > 1 else heads * hd
+
+
+def _cache_pair(key_cache, value_cache, engine, head_dim: int) -> tuple[int, int, int, int, int]:
+    """(K address, V address, dtype, rows, kv heads) of one layer's caches [rows, kv_heads, head_dim]."""
+    n, kvh, hd = _heads3(key_cache, "key_cache")
+    if key_cache.shape != value_cache.shape or key_cache.dtype != value_cache.dtype or hd != head_dim:
+        raise ValueError("key and value caches: one shape and type, with the rows' head_dim")
+    return _on(key_cache, engine, "key_cache"), _on(value_cache, engine, "value_cache"), _dt(key_cache), n, kvh
+
+
+def qk_norm_rope(engine, query, key, value, q_gamma, k_gamma, epsilon: float, rope_cache, output, key_cache,
+                 value_cache, max_seq_len: int, position: int = 0, row_base: Optional[torch.Tensor] = None,
+                 positions: Optional[torch.Tensor] = None) -> None:
+    """RMS norm of each query and key head (q_gamma, k_gamma: [head_dim], or None
+    for no norm), rotation, and the append of K and V to the cache, in one pass
+    (janus_qk_norm_rope in include/janus_hip.h). query, key and value are [rows,
+    heads, head_dim], also as parts of one fused product's rows; output [rows,
+    heads, head_dim] receives the rotated queries and may be query."""
+    rows, heads, hd = _heads3(query, "query")
+    kc, vc, kv_dt, cache_rows, kvh = _cache_pair(key_cache, value_cache, engine, hd)
+    if tuple(key.shape) != (rows, kvh, hd) or tuple(value.shape) != (rows, kvh, hd):
+        raise ValueError(f"key and value: [{rows}, {kvh}, {hd}] expected")
+    if tuple(output.shape) != (rows, heads, hd):
+        raise ValueError("output: the query's shape expected")
+    if query.dtype != key.dtype or query.dtype != value.dtype:
+        raise ValueError("query, key and value: one type expected")
+    for g in (q_gamma, k_gamma):
+        if g is not None and (g.dtype != torch.float32 or g.numel() != hd):
+            raise ValueError(f"gamma: {hd} float32 values expected")
+    if rope_cache.dtype != torch.float32 or rope_cache.numel() < max_seq_len * hd:
+        raise ValueError(f"rope_cache: {max_seq_len} rows of {hd} float32 values expected")
+    if row_base is None and rows * max_seq_len > cache_rows:
+        raise ValueError("without row_base the cache holds max_seq_len rows for each row")
+    q, qs = _row_stride(query, engine, "query")
+    k, ks = _row_stride(key, engine, "key")
+    v, vs = _row_stride(value, engine, "value")
+    engine._check(engine.lib.janus_qk_norm_rope(
+        engine.ctx, q, k, v, _dt(query), qs, ks, vs, None if q_gamma is None else _on(q_gamma, engine, "q_gamma"),
+        None if k_gamma is None else _on(k_gamma, engine, "k_gamma"), epsilon, _on(rope_cache, engine, "rope_cache"),
+        _on(output, engine, "output"), _dt(output), kc, vc, kv_dt, rows, heads, kvh, hd, position, max_seq_len,
+        _index(row_base, rows, engine, "row_base"), _index(positions, rows, engine, "positions")))
+
+
+def prompt_attention(engine, query, key_cache, value_cache, output, nseq: int, max_seq_len: int,
+                     q_start: Optional[torch.Tensor] = None, row_base: Optional[torch.Tensor] = None,
+                     seq_lens: Optional[torch.Tensor] = None, max_len_hint: int = 0, scale: float = 0.0) -> None:
+    """Causal attention of the packed rows of nseq sequences against one layer's
+    cache (janus_prompt_attention in include/janus_hip.h): sequence s has the
+    rows [q_start[s], q_start[s + 1]) of query [rows, heads, head_dim], the last
+    of its seq_lens[s] positions, which lie in the cache from row_base[s] on."""
+    rows, heads, hd = _heads3(query, "query")
+    kc, vc, kv_dt, cache_rows, kvh = _cache_pair(key_cache, value_cache, engine, hd)
+    if output.shape != query.shape or output.dtype != query.dtype:
+        raise ValueError("output: the query's shape and type expected")
+    if row_base is None and nseq * max_seq_len > cache_rows:
+        raise ValueError("without row_base the cache holds max_seq_len rows for each sequence")
+    engine._check(engine.lib.janus_prompt_attention(
+        engine.ctx, _on(query, engine, "query"), _dt(query), kc, vc, kv_dt, _on(output, engine, "output"), rows, nseq,
+        heads, kvh, hd, max_seq_len, _index(q_start, nseq + 1, engine, "q_start"),
+        _index(row_base, nseq, engine, "row_base"), _index(seq_lens, nseq, engine, "seq_lens"), max_len_hint, scale))
+
+
+def prefix_attention(engine, query, key_cache, value_cache, output, prefix_row: int, prefix_len: int,
+                     max_seq_len: int, seq_len: int = 0, row_base: Optional[torch.Tensor] = None,
+                     seq_lens: Optional[torch.Tensor] = None, max_len_hint: int = 0, scale: float = 0.0) -> None:
+    """One decode query per sequence against a prefix that all of them share,
+    cache rows [prefix_row, prefix_row + prefix_len), and its own positions behind
+    it, [row_base[b], row_base[b] + seq_lens[b]) (janus_prefix_attention in
+    include/janus_hip.h)."""
+    batch, heads, hd = _heads3(query, "query")
+    kc, vc, kv_dt, cache_rows, kvh = _cache_pair(key_cache, value_cache, engine, hd)
+    if output.shape != query.shape or output.dtype != query.dtype:
+        raise ValueError("output: the query's shape and type expected")
+    if prefix_row < 0 or prefix_len < 0 or prefix_row + prefix_len > cache_rows:
+        raise ValueError("the prefix lies beyond the cache")
+    if row_base is None and (seq_lens is not None or seq_len) and batch * max_seq_len > cache_rows:
+        raise ValueError("without row_base the cache holds max_seq_len rows for each sequence")
+    engine._check(engine.lib.janus_prefix_attention(
+        engine.ctx, _on(query, engine, "query"), _dt(query), kc, vc, kv_dt, _on(output, engine, "output"), batch,
+        heads, kvh, hd, prefix_row, prefix_len, seq_len, max_seq_len, _index(row_base, batch, engine, "row_base"),
+        _index(seq_lens, batch, engine, "seq_lens"), max_len_hint, scale))
+
+
 # ---- embedding and sampling ---------------------------------------------------------
 
 def embed_tokens(engine, table: GpuTensor, token_ids: Sequence[int], output) -> None:

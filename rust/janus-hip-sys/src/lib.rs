@@ -249,6 +249,74 @@ unsafe extern "C" {
         max_len_hint: u32,
         scale: c_float,
     ) -> c_int;
+    pub fn janus_qk_norm_rope(
+        ctx: *mut janus_ctx,
+        q: *const c_void,
+        k: *const c_void,
+        v: *const c_void,
+        in_dtype: c_int,
+        q_stride: u32,
+        k_stride: u32,
+        v_stride: u32,
+        q_gamma: *const c_float,
+        k_gamma: *const c_float,
+        eps: c_float,
+        d_table: *const c_float,
+        q_out: *mut c_void,
+        out_dtype: c_int,
+        k_cache: *mut c_void,
+        v_cache: *mut c_void,
+        kv_dtype: c_int,
+        rows: u32,
+        heads: u32,
+        kv_heads: u32,
+        head_dim: u32,
+        position: u32,
+        max_seq_len: u32,
+        d_row_base: *const i32,
+        d_positions: *const i32,
+    ) -> c_int;
+    pub fn janus_prompt_attention(
+        ctx: *mut janus_ctx,
+        q: *const c_void,
+        dtype: c_int,
+        k_cache: *const c_void,
+        v_cache: *const c_void,
+        kv_dtype: c_int,
+        out: *mut c_void,
+        rows: u32,
+        nseq: u32,
+        heads: u32,
+        kv_heads: u32,
+        head_dim: u32,
+        max_seq_len: u32,
+        d_q_start: *const i32,
+        d_row_base: *const i32,
+        d_seq_lens: *const i32,
+        max_len_hint: u32,
+        scale: c_float,
+    ) -> c_int;
+    pub fn janus_prefix_attention(
+        ctx: *mut janus_ctx,
+        q: *const c_void,
+        dtype: c_int,
+        k_cache: *const c_void,
+        v_cache: *const c_void,
+        kv_dtype: c_int,
+        out: *mut c_void,
+        batch: u32,
+        heads: u32,
+        kv_heads: u32,
+        head_dim: u32,
+        prefix_row: u32,
+        prefix_len: u32,
+        seq_len: u32,
+        max_seq_len: u32,
+        d_row_base: *const i32,
+        d_seq_lens: *const i32,
+        max_len_hint: u32,
+        scale: c_float,
+    ) -> c_int;
     pub fn janus_embed(
         ctx: *mut janus_ctx,
         table: *const janus_weight,
