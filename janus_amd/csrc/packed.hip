@@ -35,9 +35,13 @@ namespace {
 
 typedef _Float16 ph8 __attribute__((ext_vector_type(8)));
 typedef short ps4 __attribute__((ext_vector_type(4)));
+typedef float pf4 __attribute__((ext_vector_type(4)));
 typedef float pf16 __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) ps4 *lds4;
 
-constexpr uint32_t COLS = 128;   // columns per workgroup
+// Columns per workgroup: 128 through shared tiles, 32 where every wavefront reads
+// its own positions (binary32 caches).
+constexpr uint32_t cols_of(bool kv_f16) { return kv_f16 ? 128u : 32u; }
 
 struct PackedArgs {
     const void *q;            // [rows][heads][D]
@@ -73,39 +77,47 @@ __device__ __forceinline__ float swap32(float v) {   // value of lane ^ 32
     return __uint_as_float((__lane_id() & 32) ? p[0] : p[1]);
 }
 
-// Rows [first, first + n) and positions of sequence s; whatever the tables hold,
-// rows stay inside [0, rows) and len within [0, max_seq].
-__device__ __forceinline__ void rows_of(const PackedArgs &a, uint32_t s, uint32_t &first, uint32_t &n) {
-    const int32_t lim = (int32_t)a.rows, b = min(max(a.q_start[s], 0), lim), e = min(max(a.q_start[s + 1], b), lim);
-    first = (uint32_t)b;
-    n = (uint32_t)(e - b);
+__device__ __forceinline__ float swap16(float v) {   // value of lane ^ 16
+    const uint32_t u = __float_as_uint(v);
+    auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return __uint_as_float((__lane_id() & 16) ? p[0] : p[1]);
 }
 
-__device__ __forceinline__ void context_of(const PackedArgs &a, uint32_t s, Work &w) {
+// Rows [first, first + n), first cache row and positions of sequence s. Whatever
+// the tables hold, rows stay inside [0, rows) and positions within [0, max_seq].
+__device__ __forceinline__ void sequence_of(const PackedArgs &a, uint32_t s, Work &w) {
     const int64_t base = a.row_base ? (int64_t)a.row_base[s] : (int64_t)s * a.max_seq;
-    const uint32_t len = a.seq_lens ? (uint32_t)max(a.seq_lens[s], 0) : a.seq_len < 0 ? w.n : (uint32_t)a.seq_len;
+    const int32_t given = a.seq_lens ? a.seq_lens[s] : 0;
+    if (a.q_start) {
+        const int32_t b = a.q_start[s], e = a.q_start[s + 1], lim = (int32_t)a.rows;
+        const int32_t first = min(max(b, 0), lim);
+        w.row0 = (uint32_t)first;
+        w.n = (uint32_t)(min(max(e, first), lim) - first);
+    } else {
+        w.n = a.rows / a.nseq;
+        w.row0 = s * w.n;
+    }
+    const uint32_t len = a.seq_lens ? (uint32_t)max(given, 0) : a.seq_len < 0 ? w.n : (uint32_t)a.seq_len;
     w.len = base < 0 ? 0u : min(len, a.max_seq);
     w.kv_row = base < 0 ? 0 : (size_t)base;
 }
 
 // The sequence and tile of tile number t (sequences in order, a sequence's tiles
 // from its last to its first, the longest first); false: there is none.
-__device__ __forceinline__ bool find_tile(const PackedArgs &a, uint32_t t, Work &w) {
+template <uint32_t COLS> __device__ __forceinline__ bool find_tile(const PackedArgs &a, uint32_t t, Work &w) {
     const uint32_t lane = threadIdx.x & 63u;
     w.causal = true;
     if (!a.q_start) {
-        w.n = a.rows / a.nseq;
-        const uint32_t each = (uint32_t)(((uint64_t)w.n * a.G + COLS - 1) / COLS), s = t / each;
+        const uint32_t each = (uint32_t)(((uint64_t)(a.rows / a.nseq) * a.G + COLS - 1) / COLS), s = t / each;
         if (s >= a.nseq) return false;
-        w.row0 = s * w.n;
+        sequence_of(a, s, w);
         w.c0 = (each - 1 - t % each) * COLS;
-        context_of(a, s, w);
         return true;
     }
-    for (uint32_t s0 = 0; s0 < a.nseq; s0 += 64) {
-        uint32_t first = 0, n = 0;
-        if (s0 + lane < a.nseq) rows_of(a, s0 + lane, first, n);
-        const uint32_t mine = (uint32_t)(((uint64_t)n * a.G + COLS - 1) / COLS);
+    for (uint32_t s0 = 0; s0 < a.nseq; s0 += 64) {   // a lane per sequence
+        Work x;
+        sequence_of(a, min(s0 + lane, a.nseq - 1), x);
+        const uint32_t mine = s0 + lane < a.nseq ? (uint32_t)(((uint64_t)x.n * a.G + COLS - 1) / COLS) : 0u;
         uint32_t upto = mine;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -115,12 +127,12 @@ __device__ __forceinline__ bool find_tile(const PackedArgs &a, uint32_t t, Work 
         const uint64_t hit = __ballot(t < upto);
         if (hit) {
             const int at = __ffsll((unsigned long long)hit) - 1;
-            const uint32_t s = s0 + at;
-            const uint32_t before = __builtin_amdgcn_readlane(upto - mine, at);
-            w.row0 = __builtin_amdgcn_readlane(first, at);
-            w.n = __builtin_amdgcn_readlane(n, at);
-            w.c0 = (__builtin_amdgcn_readlane(mine, at) - 1 - (t - before)) * COLS;
-            context_of(a, s, w);
+            auto pick = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane(v, at); };
+            w.row0 = pick(x.row0);
+            w.n = pick(x.n);
+            w.len = pick(x.len);
+            w.kv_row = pick((uint32_t)x.kv_row);   // below 2^31
+            w.c0 = (pick(mine) - 1 - (t - pick(upto - mine))) * COLS;
             return true;
         }
         t -= __builtin_amdgcn_readlane(upto, 63);
@@ -128,19 +140,36 @@ __device__ __forceinline__ bool find_tile(const PackedArgs &a, uint32_t t, Work 
     return false;
 }
 
+// Positions that row i of the work sees: all, or len - n + 1 + i.
+__device__ __forceinline__ uint32_t seen_of(const Work &w, uint32_t i) {
+    if (!w.causal) return w.len;
+    const int64_t s = (int64_t)w.len - w.n + 1 + i;
+    return s < 0 ? 0u : (uint32_t)s;
+}
+
 // LDS of a tile of TP positions: K rows, then V rows, 16-byte segments permuted
-// within a row so that the reads below meet each bank as rarely as they can.
-//   K: 32 lanes read a segment of 32 rows; V binary16: 16 lanes read 32 bytes of
-//   each of 4 rows (transposing read); V binary32: 32 lanes read 128 bytes of a
-//   row, the other half of the wavefront the row 4 below.
-template <typename KV, int D> struct Lay {
-    static constexpr uint32_t RB = D * sizeof(KV), SEGS = RB / 16;
+// within a row so that the reads below meet each bank as rarely as they can: 32
+// lanes read a segment of 32 rows of K, 16 lanes 32 bytes of each of 4 rows of V
+// (transposing read).
+template <int D> struct Lay {
+    static constexpr uint32_t RB = D * 2, SEGS = RB / 16;
     static __device__ __forceinline__ uint32_t k_swz(uint32_t row) {
         return SEGS >= 16 ? (row & 15u) : (((row >> 1) & 7u) ^ ((row & 1u) << 2));
     }
     static __device__ __forceinline__ uint32_t v_swz(uint32_t row) {
-        return sizeof(KV) == 4 ? ((row >> 2) & 1u) << 3 : SEGS >= 16 ? (row & 3u) << 2 : ((row >> 1) & 1u) << 2;
+        return SEGS >= 16 ? (row & 3u) << 2 : ((row >> 1) & 1u) << 2;
     }
+    // few columns: 64 lanes read 32 bytes of each of 16 rows of V
+    static __device__ __forceinline__ uint32_t few_swz(uint32_t row) {
+        return SEGS >= 16 ? (row & 7u) << 1 : ((row >> 1) & 3u) << 1;
+    }
+};
+
+// p carries 2^BIAS; m may lag behind the maximum by 2^SLACK (p stays below 2^16
+// where it becomes binary16)
+template <typename Q, typename KV> struct Range {
+    static constexpr bool H = sizeof(KV) == 2, TWO = H && sizeof(Q) == 4;   // TWO: q and P in two parts
+    static constexpr float BIAS = !H ? 0.0f : TWO ? 13.0f : 6.0f, SLACK = TWO ? 2.0f : 8.0f;
 };
 
 // Sum that is NaN exactly if the 16 bytes hold an infinity or NaN.
@@ -167,19 +196,372 @@ template <typename KV> __device__ __forceinline__ ju4 finite_part(ju4 v) {
     return v;
 }
 
+// 2^sh that takes the largest of the elements to 2^14 .. 2^15 (below 2^-85 no
+// score counts), so that two binary16 parts hold 22 bits of it, and of the others
+// down to 2^-39 of it.
+__device__ __forceinline__ float two_part_scale(float qmax) {
+    int qe = 0;
+    (void)frexpf(qmax, &qe);
+    return ldexpf(1.0f, -max(qe - 15, -100));
+}
+
+// Results of up to 32 columns and the positions [p0, p1): the wavefronts take
+// steps of positions in turn, each reading its own K and V, and are joined
+// through LDS. A column is a lane of 16; NT column tiles share the operands.
+//   S^T [16 positions x 16 columns]: lane 16 g + i holds positions 4 g + v of
+//   column i. K comes from memory as the operand: position i, its dims by g.
+//   binary16: steps of 32 positions (two S^T), v_mfma_f32_16x16x32_f16; V through
+//     LDS and the transposing read, dims 16 d + 4 g + v of column i in o[d];
+//   binary32: steps of 16, v_mfma_f32_16x16x4_f32 with k = g the position 4 g + v,
+//     so V is the operand as loaded: dims 4 (i + 16 e) + c in tile 4 e + c, and
+//     o[4 e + c] holds dims 4 (4 g + v + 16 e) + c.
+template <typename Q, typename KV, int D, int NT>
+__device__ __forceinline__ void few_columns(const PackedArgs &a, const Work &w, uint32_t kvh, uint32_t ncols,
+                                            uint32_t p0, uint32_t p1, unsigned char *smem) {
+    typedef Range<Q, KV> R;
+    typedef Lay<D> Y;
+    constexpr bool H = R::H, TWO = R::TWO;
+    constexpr int STEP = H ? 32 : 16, NB = STEP / 16;
+    constexpr int KS = H ? D / 32 : D / 16;          // 16-byte loads of K per position tile
+    constexpr int VS = STEP * D * (int)sizeof(KV) / 1024;   // 16-byte loads of V per step
+    constexpr int ND = D / 16;
+    constexpr uint32_t RB = D * sizeof(KV);
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t i = lane & 15u, g = lane >> 4;
+    const uint32_t kvrow = a.kv_heads * RB;          // bytes from a position to the next
+    const unsigned char *kc = (const unsigned char *)a.kc + (w.kv_row * a.kv_heads + kvh) * RB;
+    const unsigned char *vc = (const unsigned char *)a.vc + (w.kv_row * a.kv_heads + kvh) * RB;
+
+    ju4 kr[NB][KS], vr[VS];
+    auto load_k = [&](uint32_t p) {
+        const unsigned char *at = kc + (size_t)p * kvrow;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int t = 0; t < KS; ++t)
+                kr[b][t] = *(const ju4 *)(at + (min(16u * b + i, p1 - 1 - p) * kvrow + (4u * t + g) * 16u));
+    };
+    auto load_v = [&](uint32_t p) {
+        const unsigned char *at = vc + (size_t)p * kvrow;
+#pragma unroll
+        for (int j = 0; j < VS; ++j) {
+            // binary16: in order; binary32: position 4 g + j / E, segment i + 16 (j % E)
+            constexpr int E = D / 64;
+            const uint32_t s = lane + 64u * j, row = H ? s / Y::SEGS : 4u * g + j / E, seg = H ? s % Y::SEGS : i + 16u * (j % E);
+            vr[j] = *(const ju4 *)(at + (min(row, p1 - 1 - p) * kvrow + seg * 16u));
+        }
+    };
+    uint32_t p = p0 + STEP * wave;
+    if (p < p1) {
+        load_k(p);
+        load_v(p);
+    }
+
+    // q of the lane's columns
+    constexpr int QN = D / 32;
+    ph8 qh[H ? NT : 1][QN], ql[TWO ? NT : 1][QN];
+    jf4 qf[H ? 1 : NT][D / 16];
+    float sc2[NT], qs[NT];
+    uint32_t lim[NT];
+    const Q *qp[NT];
+    bool q_inf = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const uint32_t c = min(w.c0 + 16u * n + i, ncols - 1), row = c / a.G;
+        lim[n] = min(seen_of(w, row), p1);
+        qp[n] = (const Q *)a.q + ((size_t)(w.row0 + row) * a.heads + kvh * a.G + (c - row * a.G)) * D;
+        sc2[n] = a.scale2;
+        qs[n] = 1.0f;
+        if constexpr (!H) {
+#pragma unroll
+            for (int t = 0; t < D / 16; ++t) qf[n][t] = *(const jf4 *)(qp[n] + 16 * t + 4 * g);
+        } else if constexpr (!TWO) {
+#pragma unroll
+            for (int t = 0; t < QN; ++t) qh[n][t] = *(const ph8 *)(qp[n] + 32 * t + 8 * g);
+        } else {
+            jf4 x[QN][2];
+            float qmax = 0.0f;
+#pragma unroll
+            for (int t = 0; t < QN; ++t) {
+                x[t][0] = *(const jf4 *)(qp[n] + 32 * t + 8 * g);
+                x[t][1] = *(const jf4 *)(qp[n] + 32 * t + 8 * g + 4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) qmax = fmaxf(qmax, fmaxf(fabsf(x[t][0][e]), fabsf(x[t][1][e])));
+            }
+            qmax = fmaxf(qmax, swap16(qmax));
+            qmax = fmaxf(qmax, swap32(qmax));
+            q_inf = q_inf || __any(qmax == INFINITY);
+            qs[n] = two_part_scale(qmax);
+            sc2[n] = a.scale2 / qs[n];
+#pragma unroll
+            for (int t = 0; t < QN; ++t)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float y = x[t][e >> 2][e & 3] * qs[n];
+                    qh[n][t][e] = (_Float16)y;
+                    ql[n][t][e] = (_Float16)(y - (float)qh[n][t][e]);
+                }
+        }
+    }
+    const uint32_t lo = min(seen_of(w, w.c0 / a.G), p1);   // every column sees [0, lo)
+
+    pf4 o[NT][ND];
+    float m[NT], l[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        m[n] = -INFINITY;
+        l[n] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[n][d] = (pf4){};
+    }
+    unsigned char *vt = smem + wave * (32u * Y::RB);   // this wavefront's V tile (binary16)
+    for (; p < p1; p += 4 * STEP) {
+        const bool more = p + 4 * STEP < p1;
+        pf4 s[NT][NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                s[n][b] = (pf4){};
+                pf4 s2 = (pf4){};
+#pragma unroll
+                for (int t = 0; t < KS; ++t) {
+                    if constexpr (H) {
+                        const ph8 k = __builtin_bit_cast(ph8, kr[b][t]);
+                        s[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[n][t], s[n][b], 0, 0, 0);
+                        if constexpr (TWO) s2 = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[n][t], s2, 0, 0, 0);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float k = __uint_as_float(kr[b][t][e]);
+                            if (t & 1) s2 = __builtin_amdgcn_mfma_f32_16x16x4f32(k, qf[n][t][e], s2, 0, 0, 0);
+                            else s[n][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(k, qf[n][t][e], s[n][b], 0, 0, 0);
+                        }
+                    }
+                }
+                if constexpr (TWO || !H) {
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) s[n][b][v] += s2[v];
+                }
+            }
+        if constexpr (TWO) {
+            float odd = 0.0f;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int t = 0; t < KS; ++t) odd = odd_sum<KV>(kr[b][t], odd);
+            // an infinity times a part of q that is 0 or of the other sign would make a
+            // NaN of an infinite score: such steps take q whole
+            if (q_inf || __any(odd != odd)) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) {
+                            const uint32_t at = min(16u * b + 4u * g + v, p1 - 1 - p);
+                            const KV *k = (const KV *)(kc + (size_t)(p + at) * kvrow);
+                            float x = 0.0f;
+#pragma unroll 1
+                            for (int d = 0; d < D; ++d) x = fmaf((float)qp[n][d], (float)k[d], x);
+                            s[n][b][v] = x * qs[n];
+                        }
+            }
+        }
+        if (more) load_k(p + 4 * STEP);
+        // An infinity or NaN of V stays out of the products and is added on its own.
+        float odd = 0.0f;
+#pragma unroll
+        for (int j = 0; j < VS; ++j) odd = odd_sum<KV>(vr[j], odd);
+        const bool odd_v = __any(odd != odd);
+        if (odd_v)
+#pragma unroll
+            for (int j = 0; j < VS; ++j) vr[j] = finite_part<KV>(vr[j]);
+        if constexpr (H) {
+#pragma unroll
+            for (int j = 0; j < VS; ++j) {
+                const uint32_t at = lane + 64u * j, row = at / Y::SEGS, seg = at % Y::SEGS;
+                *(ju4 *)(vt + row * Y::RB + (seg ^ Y::few_swz(row)) * 16u) = vr[j];
+            }
+            if (more) load_v(p + 4 * STEP);
+        }
+        if (p + STEP > lo) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) s[n][b][v] = p + 16 * b + 4 * g + v < lim[n] ? s[n][b][v] : -INFINITY;
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            float bm = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) bm = fmaxf(bm, s[n][b][v]);
+            bm = fmaxf(bm, swap16(bm));
+            bm = fmaxf(bm, swap32(bm));
+            if (__any((bm - m[n]) * sc2[n] > R::SLACK || (m[n] == -INFINITY && bm != -INFINITY))) {
+                const float mn = fmaxf(m[n], bm), alpha = mn == m[n] ? 1.0f : __builtin_amdgcn_exp2f((m[n] - mn) * sc2[n]);
+                m[n] = mn;
+                l[n] *= alpha;
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) o[n][d][v] *= alpha;
+            }
+            const float mr = m[n] == -INFINITY ? 0.0f : m[n];
+            float sum = 0.0f;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    s[n][b][v] = __builtin_amdgcn_exp2f(fmaf(s[n][b][v] - mr, sc2[n], R::BIAS));
+                    sum += s[n][b][v];
+                }
+            l[n] += sum;
+        }
+        if constexpr (H) {
+            ph8 ph[NT], pl[TWO ? NT : 1];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float x = s[n][e >> 2][e & 3];
+                    ph[n][e] = (_Float16)x;
+                    if constexpr (TWO) pl[n][e] = (_Float16)(x - (float)ph[n][e]);
+                }
+            // lane 16 g + i reads dims 16 d + 4 (i % 4) .. of position 4 g + i / 4 and
+            // receives dim 16 d + i of positions 4 g .. 4 g + 3
+            const uint32_t row = 4u * g + (i >> 2);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                const uint32_t at = row * Y::RB + ((2u * d + ((i & 3u) >> 1)) ^ Y::few_swz(row)) * 16u + (i & 1u) * 8u;
+                const ps4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(vt + at));
+                const ps4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(vt + at + 16 * Y::RB));
+                const ph8 v = __builtin_bit_cast(ph8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[n], o[n][d], 0, 0, 0);
+                    if constexpr (TWO) o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[n], o[n][d], 0, 0, 0);
+                }
+            }
+        } else {
+            constexpr int E = D / 64;
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+                            o[n][4 * e + c] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[v * E + e][c]), s[n][0][v], o[n][4 * e + c], 0, 0, 0);
+            if (more) load_v(p + 4 * STEP);
+        }
+        if (odd_v) {
+#pragma unroll 1
+            for (uint32_t j = 0; j < min((uint32_t)STEP, p1 - p); ++j) {
+                const KV *row = (const KV *)(vc + (size_t)(p + j) * kvrow);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float mine = 0.0f;
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) mine = 4u * (j >> 4) + (j & 3u) == 4u * b + v ? s[n][b][v] : mine;
+                    const float pj = __shfl(mine, (int)(((j >> 2) & 3u) * 16u + i), 64);
+#pragma unroll
+                    for (int d = 0; d < ND; ++d)
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) {
+                            const float x = (float)row[H ? 16 * d + 4 * g + v : 4 * (4 * g + v + 16 * (d >> 2)) + (d & 3)];
+                            if (p + j < lim[n] && (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u) o[n][d][v] = fmaf(pj, x, o[n][d][v]);
+                        }
+                }
+            }
+        }
+    }
+
+    // join the wavefronts that had positions
+    constexpr uint32_t C = 16 * NT, OS = D + 4;   // padded: 16 columns meet 16 bank groups
+    const uint32_t nw = min((p1 - min(p0, p1) + STEP - 1) / STEP, 4u);
+    float2 *ml = (float2 *)smem;                   // [wave][column]
+    float *oo = (float *)(smem + 4 * 32 * sizeof(float2));   // [wave][column][OS]
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        l[n] += swap16(l[n]);
+        l[n] += swap32(l[n]);
+        m[n] = m[n] / qs[n];
+        if (g == 0) ml[wave * C + 16 * n + i] = make_float2(m[n], l[n]);
+    }
+    __syncthreads();
+    if (wave < nw) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            float M = -INFINITY;
+            for (uint32_t x = 0; x < nw; ++x) M = fmaxf(M, ml[x * C + 16 * n + i].x);
+            const float f = m[n] == M ? 1.0f : __builtin_amdgcn_exp2f((m[n] - M) * a.scale2);
+            float *to = oo + (wave * C + 16 * n + i) * OS;
+            if constexpr (H) {
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+                    *(jf4 *)(to + 16 * d + 4 * g) = jf4{o[n][d][0] * f, o[n][d][1] * f, o[n][d][2] * f, o[n][d][3] * f};
+            } else {
+#pragma unroll
+                for (int e = 0; e < D / 64; ++e)
+#pragma unroll
+                    for (int v = 0; v < 4; ++v)
+                        *(jf4 *)(to + 4 * (4 * g + v + 16 * e)) = jf4{o[n][4 * e][v] * f, o[n][4 * e + 1][v] * f, o[n][4 * e + 2][v] * f, o[n][4 * e + 3][v] * f};
+            }
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t at = threadIdx.x; at < C * (D / 4); at += 256) {
+        const uint32_t col = at / (D / 4), dim = at % (D / 4) * 4u, c = w.c0 + col;
+        if (c >= ncols) break;
+        float M = -INFINITY, lt = 0.0f;
+        for (uint32_t x = 0; x < nw; ++x) M = fmaxf(M, ml[x * C + col].x);
+        jf4 sum = {};
+        for (uint32_t x = 0; x < nw; ++x) {
+            const float2 y = ml[x * C + col];
+            lt = fmaf(y.y, y.x == M ? 1.0f : __builtin_amdgcn_exp2f((y.x - M) * a.scale2), lt);
+            const jf4 z = *(const jf4 *)(oo + (x * C + col) * OS + dim);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[e] += z[e];
+        }
+        const uint32_t row = c / a.G;
+        const size_t qat = (size_t)(w.row0 + row) * a.heads + kvh * a.G + (c - row * a.G);
+        if (a.slots) {
+            const size_t part = qat * a.slots + w.slot;
+            if (dim == 0) *(float2 *)(a.part_ml + 2 * part) = make_float2(M, lt);
+            if (nw) *(jf4 *)(a.part + part * D + dim) = sum;   // the join reads no output of a part without positions
+        } else {
+            const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;   // a row that sees nothing is 0
+            typedef Q q4 __attribute__((ext_vector_type(4)));
+            q4 y;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = (Q)(sum[e] * inv);
+            *(q4 *)((Q *)a.out + qat * D + dim) = y;
+        }
+    }
+}
+
 // Q: _Float16 or float rows; KV: the cache's type.
 template <typename Q, typename KV, int D>
 __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedArgs a) {
-    constexpr bool H = sizeof(KV) == 2;            // binary16 cache
-    constexpr bool TWO = H && sizeof(Q) == 4;      // q and P in two parts
+    typedef Range<Q, KV> R;
+    typedef Lay<D> Y;
+    constexpr bool H = R::H, TWO = R::TWO;
+    constexpr uint32_t COLS = cols_of(H);
     constexpr int TP = sizeof(Q) == 2 ? 64 : 32;   // positions per tile
     constexpr int NB = TP / 32, ND = D / 32;
-    typedef Lay<KV, D> Y;
     constexpr uint32_t VB = TP * Y::RB, FLAGS = 2 * VB, BUF = FLAGS + 16;   // bytes of a buffer
     constexpr int LD = TP * Y::SEGS / 256;         // 16-byte segments per thread, of K and of V
     static_assert(LD >= 1 && LD * 256 == TP * (int)Y::SEGS, "tile load");
-    // p carries 2^BIAS; m may lag behind the maximum by 2^SLACK (p stays below 2^16)
-    constexpr float BIAS = !H ? 0.0f : TWO ? 13.0f : 6.0f, SLACK = !H ? 8.0f : TWO ? 2.0f : 8.0f;
     extern __shared__ __align__(16) unsigned char smem[];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t col = lane & 31u, h = lane >> 5;
@@ -203,26 +585,25 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedArgs a) {
         w.split = rest % a.splits;
         w.splits = a.splits;
         w.slot = a.prefix_splits + w.split;
-        if (!find_tile(a, rest / a.splits, w)) return;
+        if (!find_tile<COLS>(a, rest / a.splits, w)) return;
     }
     const uint32_t ncols = w.n * a.G;   // n * G <= rows * heads < 2^32
-    // positions that row i sees: the first len, or len - n + 1 + i
-    auto seen_of = [&](uint32_t i) -> uint32_t {
-        if (!w.causal) return w.len;
-        const int64_t s = (int64_t)w.len - w.n + 1 + i;
-        return s < 0 ? 0u : (uint32_t)s;
-    };
-    const uint32_t wc0 = w.c0 + 32u * wave;
-    const bool idle = wc0 >= ncols;     // uniform: this wavefront only helps to load
-    const uint32_t wave_lo = idle ? 0u : seen_of(wc0 / a.G), wave_hi = idle ? 0u : seen_of(min(wc0 + 31u, ncols - 1) / a.G);
-    const uint32_t end_all = seen_of(min(w.c0 + COLS - 1, ncols - 1) / a.G);
+    const uint32_t end_all = seen_of(w, min(w.c0 + COLS - 1, ncols - 1) / a.G);
     // this workgroup's part of the positions
     const uint32_t per = (((end_all + w.splits - 1) / w.splits) + TP - 1) / TP * TP;
     const uint32_t p0 = min(w.split * per, end_all), p1 = min(p0 + per, end_all);
-
+    if (!H || ncols - w.c0 <= 32) {
+        if (ncols - w.c0 <= 16) few_columns<Q, KV, D, 1>(a, w, kvh, ncols, p0, p1, smem);
+        else few_columns<Q, KV, D, 2>(a, w, kvh, ncols, p0, p1, smem);
+        return;
+    }
+    if constexpr (H) {
+    const uint32_t wc0 = w.c0 + 32u * wave;
+    const bool idle = wc0 >= ncols;     // uniform: this wavefront only helps to load
+    const uint32_t wave_lo = idle ? 0u : seen_of(w, wc0 / a.G), wave_hi = idle ? 0u : seen_of(w, min(wc0 + 31u, ncols - 1) / a.G);
     const uint32_t c = min(wc0 + col, ncols - 1), qrow = c / a.G, head = kvh * a.G + c % a.G;
     const bool mine = wc0 + col < ncols;
-    const uint32_t seen = seen_of(qrow);
+    const uint32_t seen = seen_of(w, qrow);
     const size_t qat = ((size_t)(w.row0 + qrow) * a.heads + head);
 
     const uint32_t kvrow = a.kv_heads * Y::RB;   // bytes from a position to the next
@@ -265,20 +646,14 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedArgs a) {
 
     // q of this lane's column
     const Q *qp = (const Q *)a.q + qat * D;
-    constexpr int QN = H ? D / 16 : 1;
+    constexpr int QN = D / 16;
     ph8 qh[QN], ql[TWO ? QN : 1];
-    jf4 qf[H ? 1 : D / 8];
     float sc2 = a.scale2, qs = 1.0f;
     bool q_inf = false;
-    if constexpr (!H) {
-#pragma unroll
-        for (int s = 0; s < D / 8; ++s) qf[s] = *(const jf4 *)(qp + 8 * s + 4 * h);
-    } else if constexpr (!TWO) {
+    if constexpr (!TWO) {
 #pragma unroll
         for (int s = 0; s < QN; ++s) qh[s] = *(const ph8 *)(qp + 16 * s + 8 * h);
     } else {
-        // scaled so that the largest element is 2^14 .. 2^15: the parts hold 22 bits of
-        // it, and of the others down to 2^-39 of it
         float qmax = 0.0f;
         jf4 x[QN][2];
 #pragma unroll
@@ -289,20 +664,16 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedArgs a) {
             for (int i = 0; i < 4; ++i) qmax = fmaxf(qmax, fmaxf(fabsf(x[s][0][i]), fabsf(x[s][1][i])));
         }
         qmax = fmaxf(qmax, swap32(qmax));
-        int qe = 0;
-        (void)frexpf(qmax, &qe);
-        const int sh = max(qe - 15, -100);
-        qs = ldexpf(1.0f, -sh);
         q_inf = __any(qmax == INFINITY);
-        sc2 *= ldexpf(1.0f, sh);
+        qs = two_part_scale(qmax);
+        sc2 /= qs;
 #pragma unroll
         for (int s = 0; s < QN; ++s)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float y = x[s][i >> 2][i & 3] * qs;
-                const _Float16 hi = (_Float16)y;
-                qh[s][i] = hi;
-                ql[s][i] = (_Float16)(y - (float)hi);
+                qh[s][i] = (_Float16)y;
+                ql[s][i] = (_Float16)(y - (float)qh[s][i]);
             }
     }
 
@@ -326,31 +697,16 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedArgs a) {
             for (int b = 0; b < NB; ++b) {
                 s[b] = (pf16){};
                 const uint32_t row = 32u * b + col, swz = Y::k_swz(row);
-                if constexpr (H) {
-                    pf16 lo = (pf16){};
+                pf16 lo = (pf16){};
 #pragma unroll
-                    for (int t = 0; t < QN; ++t) {
-                        const ph8 k = *(const ph8 *)(kt + row * Y::RB + ((2u * t + h) ^ swz) * 16u);
-                        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[t], s[b], 0, 0, 0);
-                        if constexpr (TWO) lo = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[t], lo, 0, 0, 0);
-                    }
-                    if constexpr (TWO) {
+                for (int t = 0; t < QN; ++t) {
+                    const ph8 k = *(const ph8 *)(kt + row * Y::RB + ((2u * t + h) ^ swz) * 16u);
+                    s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[t], s[b], 0, 0, 0);
+                    if constexpr (TWO) lo = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[t], lo, 0, 0, 0);
+                }
+                if constexpr (TWO) {
 #pragma unroll
-                        for (int v = 0; v < 16; ++v) s[b][v] += lo[v];
-                    }
-                } else {
-                    pf16 s2 = (pf16){};
-#pragma unroll
-                    for (int t = 0; t < D / 8; ++t) {
-                        const jf4 k = *(const jf4 *)(kt + row * Y::RB + ((2u * t + h) ^ swz) * 16u);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            if (t & 1) s2 = __builtin_amdgcn_mfma_f32_32x32x2f32(k[i], qf[t][i], s2, 0, 0, 0);
-                            else s[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(k[i], qf[t][i], s[b], 0, 0, 0);
-                        }
-                    }
-#pragma unroll
-                    for (int v = 0; v < 16; ++v) s[b][v] += s2[v];
+                    for (int v = 0; v < 16; ++v) s[b][v] += lo[v];
                 }
             }
             if constexpr (TWO)
@@ -385,7 +741,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedArgs a) {
 #pragma unroll
                 for (int v = 0; v < 16; ++v) bm = fmaxf(bm, s[b][v]);
             bm = fmaxf(bm, swap32(bm));
-            if (__any((bm - m) * sc2 > SLACK || (m == -INFINITY && bm != -INFINITY))) {
+            if (__any((bm - m) * sc2 > R::SLACK || (m == -INFINITY && bm != -INFINITY))) {
                 const float mn = fmaxf(m, bm), alpha = mn == m ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * sc2);
                 m = mn;
                 l *= alpha;
@@ -395,7 +751,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedArgs a) {
                     for (int v = 0; v < 16; ++v) o[d][v] *= alpha;
             }
             // while only masked or NaN scores have come, m counts as 0: 2^-inf is 0, a NaN stays
-            const float mr = m == -INFINITY ? 0.0f : m, ms = sizeof(Q) == 2 ? BIAS - mr * sc2 : 0.0f;
+            const float mr = m == -INFINITY ? 0.0f : m, ms = sizeof(Q) == 2 ? R::BIAS - mr * sc2 : 0.0f;
             float sum = 0.0f;
 #pragma unroll
             for (int b = 0; b < NB; ++b)
@@ -403,11 +759,11 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedArgs a) {
                 for (int v = 0; v < 16; ++v) {
                     // binary32 rows: the difference is exact near the maximum
                     s[b][v] = sizeof(Q) == 2 ? __builtin_amdgcn_exp2f(fmaf(s[b][v], sc2, ms))
-                                             : __builtin_amdgcn_exp2f(fmaf(s[b][v] - mr, sc2, BIAS));
+                                             : __builtin_amdgcn_exp2f(fmaf(s[b][v] - mr, sc2, R::BIAS));
                     sum += s[b][v];
                 }
             l += sum;
-            if constexpr (H) {
+            {
                 // lanes 16 g + i of half h read dims 32 d + 16 g + 4 (i % 4) .. of positions
                 // 4 h + i / 4 (+ 8) of a step and receive dim 32 d + 16 g + i of four positions
                 const uint32_t i = lane & 15u, g = (lane >> 4) & 1u;
@@ -424,22 +780,11 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedArgs a) {
 #pragma unroll
                     for (int d = 0; d < ND; ++d) {
                         const uint32_t at = (16u * t + vrow) * Y::RB + ((4u * d + vseg) ^ Y::v_swz(vrow)) * 16u + vin;
-                        typedef __attribute__((address_space(3))) ps4 *lds4;
                         const ps4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(vt + at));
                         const ps4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(vt + at + 8 * Y::RB));
                         const ph8 v = __builtin_bit_cast(ph8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
                         o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph, o[d], 0, 0, 0);
                         if constexpr (TWO) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl, o[d], 0, 0, 0);
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    const uint32_t row = 8u * (v >> 2) + 4u * h + (v & 3);
-#pragma unroll
-                    for (int d = 0; d < ND; ++d) {
-                        const float x = *(const float *)(vt + row * Y::RB + ((8u * d + (col >> 2)) ^ Y::v_swz(row)) * 16u + (col & 3u) * 4u);
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, s[0][v], o[d], 0, 0, 0);
                     }
                 }
             }
@@ -494,6 +839,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedArgs a) {
             for (int i = 0; i < 4; ++i) y[i] = (Q)(o[d][4 * j + i] * inv);
             *(q4 *)(to + 32 * d + 8 * j + 4 * h) = y;
         }
+    }
 }
 
 // Joins the parts of a row and head: a wavefront each. A part holds m, l and the
@@ -506,20 +852,40 @@ __global__ __launch_bounds__(256) void packed_join_kernel(PackedArgs a) {
     if (row >= a.rows) return;
     // rows outside the sequences are not written
     if (a.q_start && ((int32_t)row < a.q_start[0] || (int32_t)row >= a.q_start[a.nseq])) return;
-    const float *ml = a.part_ml + at * a.slots * 2;
-    const float *part = a.part + at * a.slots * D;
     constexpr int E = D / 64;
-    float M = -INFINITY;
-    for (uint32_t s = lane; s < a.slots; s += 64) M = fmaxf(M, ml[2 * s]);
-    M = wave_max(M);
-    float l = 0.0f, o[E] = {};
-    for (uint32_t s = 0; s < a.slots; ++s) {
-        const float ms = ml[2 * s], ls = ml[2 * s + 1];
-        if (ls == 0.0f) continue;
-        const float wgt = ms == M ? 1.0f : __builtin_amdgcn_exp2f((ms - M) * a.scale2);
-        l = fmaf(ls, wgt, l);
+    const float2 *ml = (const float2 *)a.part_ml + at * a.slots;
+    const float *part = a.part + at * a.slots * D + E * lane;
+    constexpr int U = 8;
+    typedef float vec __attribute__((ext_vector_type(E)));
+    float M = -INFINITY, l = 0.0f;
+    vec o = {};
+    for (uint32_t s0 = 0; s0 < a.slots; s0 += 64) {   // lane s: part s0 + s
+        const float2 p = s0 + lane < a.slots ? ml[s0 + lane] : make_float2(-INFINITY, 0.0f);
+        const float m0 = M;
+        M = fmaxf(M, wave_max(p.x));
+        const float w = p.y == 0.0f ? 0.0f : p.x == M ? 1.0f : __builtin_amdgcn_exp2f((p.x - M) * a.scale2);
+        const float old = M == m0 ? 1.0f : __builtin_amdgcn_exp2f((m0 - M) * a.scale2);
+        l = fmaf(l, old, wave_sum(p.y * w));
+        o *= old;
+        // U parts in flight; those without positions repeat the first that has some
+        const uint64_t has = __ballot(p.y != 0.0f);
+        if (!has) continue;
+        const uint32_t first = __ffsll((unsigned long long)has) - 1, n = 64 - __builtin_clzll(has);
+        for (uint32_t s = 0; s < n; s += U) {
+            vec x[U];
 #pragma unroll
-        for (int i = 0; i < E; ++i) o[i] = fmaf(part[(size_t)s * D + E * lane + i], wgt, o[i]);
+            for (uint32_t u = 0; u < U; ++u) {
+                const uint32_t k = s + u < 64 && (has >> ((s + u) & 63) & 1) ? s + u : first;
+                x[u] = *(const vec *)(part + (size_t)(s0 + k) * D);
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u) {
+                const bool there = s + u < 64 && (has >> ((s + u) & 63) & 1);
+                const float wu = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), (s + u) & 63));
+#pragma unroll
+                for (int i = 0; i < E; ++i) o[i] = there ? fmaf(x[u][i], wu, o[i]) : o[i];
+            }
+        }
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
@@ -528,8 +894,9 @@ __global__ __launch_bounds__(256) void packed_join_kernel(PackedArgs a) {
 
 template <typename Q, typename KV, int D>
 int launch(janus_ctx *ctx, const PackedArgs &a, uint32_t blocks) {
-    constexpr int TP = sizeof(Q) == 2 ? 64 : 32;
-    constexpr size_t lds = 2 * (2 * TP * D * sizeof(KV) + 16);
+    // two tiles of K and V, or the join of the wavefronts of few columns
+    constexpr size_t tiles = sizeof(KV) == 2 ? 2 * (2 * (sizeof(Q) == 2 ? 64 : 32) * D * 2 + 16) : 0;
+    constexpr size_t lds = std::max<size_t>(tiles, 4 * 32 * (8 + (D + 4) * 4));
     static const hipError_t attr = hipFuncSetAttribute((const void *)packed_attn_kernel<Q, KV, D>,
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     (void)attr;
@@ -549,10 +916,10 @@ int launch_typed(janus_ctx *ctx, const PackedArgs &a, int q_dt, int kv_dt, uint3
     return hd == 64 ? launch<float, float, 64>(ctx, a, blocks) : launch<float, float, 128>(ctx, a, blocks);
 }
 
-// Workgroups per tile so that `tiles` of them fill the CUs about four times
-// over, each with 256 positions at least.
+// Workgroups per tile so that `tiles` of them fill the CUs (two on each), each
+// with 256 positions at least.
 uint32_t plan_splits(const janus_ctx *ctx, uint64_t tiles, uint32_t max_len) {
-    const uint64_t want = 4ull * ctx->num_cus / std::max<uint64_t>(tiles, 1);
+    const uint64_t want = 2ull * ctx->num_cus / std::max<uint64_t>(tiles, 1);
     return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(want, (max_len + 255) / 256));
 }
 
@@ -583,8 +950,11 @@ int prompt_attention_launch(janus_ctx *ctx, const void *q, int q_dt, const void 
     a.seq_len = -1;
     a.scale2 = scale * 1.4426950408889634f;
     // at most so many tiles: every sequence's last one may be part empty
-    const uint64_t tiles = (uint64_t)rows * a.G / COLS + nseq;
-    a.splits = plan_splits(ctx, tiles * kv_heads, std::min(max_len, max_seq));
+    const uint32_t cols = cols_of(kv_dt == JANUS_DT_F16);
+    const uint64_t tiles = (uint64_t)rows * a.G / cols + nseq;
+    // about as many as sequences of equal rows have
+    const uint64_t likely = (uint64_t)nseq * (((rows + nseq - 1) / nseq * (uint64_t)a.G + cols - 1) / cols);
+    a.splits = plan_splits(ctx, likely * kv_heads, std::min(max_len, max_seq));
     a.slots = a.splits > 1 ? a.splits : 0;
     return run(ctx, a, q_dt, kv_dt, hd, tiles * a.splits);
 }
@@ -601,9 +971,10 @@ int prefix_attention_launch(janus_ctx *ctx, const void *q, int q_dt, const void 
     a.seq_len = seq_len;
     a.prefix_row = prefix_row; a.prefix_len = prefix_len;
     a.scale2 = scale * 1.4426950408889634f;
-    const uint64_t own_tiles = (uint64_t)batch * ((a.G + COLS - 1) / COLS);
+    const uint32_t cols = cols_of(kv_dt == JANUS_DT_F16);
+    const uint64_t own_tiles = (uint64_t)batch * ((a.G + cols - 1) / cols);
     if (prefix_len) {
-        a.prefix_tiles = (uint32_t)(((uint64_t)batch * a.G + COLS - 1) / COLS);
+        a.prefix_tiles = (uint32_t)(((uint64_t)batch * a.G + cols - 1) / cols);
         a.prefix_splits = plan_splits(ctx, (uint64_t)a.prefix_tiles * kv_heads, prefix_len);
     }
     a.splits = plan_splits(ctx, own_tiles * kv_heads, std::min(max_len, max_seq));
