@@ -191,18 +191,18 @@ namespace {
 // Host checks shared by the attentions of packed rows.
 int packed_args(janus_ctx *ctx, const char *name, const void *q, int q_dt, const void *k_cache, const void *v_cache,
                 int kv_dt, const void *out, uint32_t heads, uint32_t kv_heads, uint32_t hd) {
-    const std::string n = name;
-    if (!q || !k_cache || !v_cache || !out) return fail(ctx, JANUS_E_INVALID_ARG, n + ": null buffer");
+    auto no = [&](int code, const char *why) { return fail(ctx, code, std::string(name) + ": " + why); };
+    if (!q || !k_cache || !v_cache || !out) return no(JANUS_E_INVALID_ARG, "null buffer");
     if ((((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) & 15u) != 0)
-        return fail(ctx, JANUS_E_INVALID_ARG, n + ": q, the caches and out must be 16-byte aligned");
+        return no(JANUS_E_INVALID_ARG, "q, the caches and out must be 16-byte aligned");
     if (!is_act_dtype(q_dt) || !is_act_dtype(kv_dt))
-        return fail(ctx, JANUS_E_UNSUPPORTED_DTYPE, n + ": rows and cache must be F32 or F16");
+        return no(JANUS_E_UNSUPPORTED_DTYPE, "rows and cache must be F32 or F16");
     if (q_dt == JANUS_DT_F16 && kv_dt != JANUS_DT_F16)
-        return fail(ctx, JANUS_E_UNSUPPORTED_DTYPE, n + ": F16 rows need an F16 cache");
+        return no(JANUS_E_UNSUPPORTED_DTYPE, "F16 rows need an F16 cache");
     if (kv_heads == 0 || heads == 0 || heads % kv_heads)
-        return fail(ctx, JANUS_E_INVALID_DIM, n + ": heads must be a multiple of kv_heads");
-    if (hd != 64 && hd != 128) return fail(ctx, JANUS_E_INVALID_DIM, n + ": head_dim must be 64 or 128");
-    if (heads > 65536u) return fail(ctx, JANUS_E_INVALID_DIM, n + ": more than 65536 heads");
+        return no(JANUS_E_INVALID_DIM, "heads must be a multiple of kv_heads");
+    if (hd != 64 && hd != 128) return no(JANUS_E_INVALID_DIM, "head_dim must be 64 or 128");
+    if (heads > 65536u) return no(JANUS_E_INVALID_DIM, "more than 65536 heads");
     return JANUS_OK;
 }
 }  // namespace

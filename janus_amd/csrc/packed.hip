@@ -305,6 +305,17 @@ __device__ __forceinline__ void few_columns(const PackedArgs &a, const Work &w, 
     }
     const uint32_t lo = min(seen_of(w, w.c0 / a.G), p1);   // every column sees [0, lo)
 
+    // q has arrived before the steps begin: a wait for it among them would be one for
+    // the loads of the next step too
+    if constexpr (!TWO) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int t = 0; t < (H ? QN : D / 16); ++t) {
+                if constexpr (H) asm volatile("" : "+v"(qh[n][t]));
+                else asm volatile("" : "+v"(qf[n][t]));
+            }
+    }
     pf4 o[NT][ND];
     float m[NT], l[NT];
 #pragma unroll
@@ -683,6 +694,12 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedArgs a) {
     float m = -INFINITY, l = 0.0f;
 
     if (p0 < p1) store(smem);
+    // q has arrived before the tiles begin: a wait for it among them would be one for
+    // the loads of the next tile too
+    if constexpr (!TWO) {
+#pragma unroll
+        for (int s = 0; s < QN; ++s) asm volatile("" : "+v"(qh[s]));
+    }
     uint32_t buf = 0;
     for (uint32_t p = p0; p < p1; p += TP) {
         const bool more = p + TP < p1;
@@ -692,22 +709,37 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedArgs a) {
         if (p < wave_hi) {
             const uint4 f = *(const uint4 *)(kt + FLAGS);
             const uint32_t flags = __builtin_amdgcn_readfirstlane(f.x | f.y | f.z | f.w);
-            pf16 s[NB];
+            pf16 s[NB], lo = (pf16){};
+            ph8 k[NB][QN];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const uint32_t row = 32u * b + col, swz = Y::k_swz(row);
+#pragma unroll
+                for (int t = 0; t < QN; ++t) k[b][t] = *(const ph8 *)(kt + row * Y::RB + ((2u * t + h) ^ swz) * 16u);
+            }
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 s[b] = (pf16){};
-                const uint32_t row = 32u * b + col, swz = Y::k_swz(row);
-                pf16 lo = (pf16){};
 #pragma unroll
                 for (int t = 0; t < QN; ++t) {
-                    const ph8 k = *(const ph8 *)(kt + row * Y::RB + ((2u * t + h) ^ swz) * 16u);
-                    s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[t], s[b], 0, 0, 0);
-                    if constexpr (TWO) lo = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[t], lo, 0, 0, 0);
+                    s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[b][t], qh[t], s[b], 0, 0, 0);
+                    if constexpr (TWO) lo = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[b][t], ql[t], lo, 0, 0, 0);
                 }
-                if constexpr (TWO) {
+            }
+            // The operands of 32 positions are requested together, and those of the
+            // next 32 one by one behind the products: left to itself the compiler
+            // waits for each before it asks for the next.
+            __builtin_amdgcn_sched_group_barrier(0x100, QN, 0);
+            if constexpr (NB == 2)
 #pragma unroll
-                    for (int v = 0; v < 16; ++v) s[b][v] += lo[v];
+                for (int t = 0; t < QN; ++t) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
                 }
+            __builtin_amdgcn_sched_group_barrier(0x008, NB == 2 ? QN : 2 * QN, 0);
+            if constexpr (TWO) {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) s[0][v] += lo[v];
             }
             if constexpr (TWO)
                 // an infinity times a part of q that is 0 or of the other sign would make
@@ -735,11 +767,14 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedArgs a) {
                     for (int v = 0; v < 16; ++v)
                         s[b][v] = p + 32 * b + 8 * (v >> 2) + 4 * h + (v & 3) < lim ? s[b][v] : -INFINITY;
             }
-            float bm = -INFINITY;
+            float top[4];
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+            for (int v = 0; v < 4; ++v) {
+                top[v] = s[0][v];
 #pragma unroll
-                for (int v = 0; v < 16; ++v) bm = fmaxf(bm, s[b][v]);
+                for (int x = v + 4; x < 16 * NB; x += 4) top[v] = fmaxf(top[v], s[x >> 4][x & 15]);
+            }
+            float bm = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
             bm = fmaxf(bm, swap32(bm));
             if (__any((bm - m) * sc2 > R::SLACK || (m == -INFINITY && bm != -INFINITY))) {
                 const float mn = fmaxf(m, bm), alpha = mn == m ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * sc2);
@@ -752,7 +787,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedArgs a) {
             }
             // while only masked or NaN scores have come, m counts as 0: 2^-inf is 0, a NaN stays
             const float mr = m == -INFINITY ? 0.0f : m, ms = sizeof(Q) == 2 ? R::BIAS - mr * sc2 : 0.0f;
-            float sum = 0.0f;
+            float sum[4] = {};
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -760,9 +795,9 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedArgs a) {
                     // binary32 rows: the difference is exact near the maximum
                     s[b][v] = sizeof(Q) == 2 ? __builtin_amdgcn_exp2f(fmaf(s[b][v], sc2, ms))
                                              : __builtin_amdgcn_exp2f(fmaf(s[b][v] - mr, sc2, R::BIAS));
-                    sum += s[b][v];
+                    sum[v & 3] += s[b][v];
                 }
-            l += sum;
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             {
                 // lanes 16 g + i of half h read dims 32 d + 16 g + 4 (i % 4) .. of positions
                 // 4 h + i / 4 (+ 8) of a step and receive dim 32 d + 16 g + i of four positions

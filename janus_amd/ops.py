@@ -248,44 +248,47 @@ def compute_attention_noalloc(engine, query, key_cache, value_cache, output, bat
 
 # ---- heads and attention of packed rows ----------------------------------------------
 
-def _index(t: Optional[torch.Tensor], least: int, engine: ComputeEngine, name: str) -> Optional[int]:
-    """An int32 table of at least `least` entries on the engine's device, or None."""
+def _buf(t: torch.Tensor, dev: int, name: str) -> int:
+    """Address of a contiguous tensor on the engine's device."""
+    if t.get_device() != dev or not t.is_contiguous():
+        raise ValueError(f"{name}: a contiguous tensor on cuda:{dev} expected, got {t.device}, strides {t.stride()}")
+    return t.data_ptr()
+
+
+def _table(t: Optional[torch.Tensor], dtype: torch.dtype, least: int, dev: int, name: str) -> Optional[int]:
+    """Address of a table of at least `least` values, or None."""
     if t is None:
         return None
-    if t.dtype != torch.int32 or t.numel() < least:
-        raise ValueError(f"{name}: an int32 tensor of {least} values")
-    return _on(t, engine, name)
+    if t.dtype is not dtype or t.numel() < least:
+        raise ValueError(f"{name}: at least {least} values of {dtype} expected, got {t.numel()} of {t.dtype}")
+    return _buf(t, dev, name)
 
 
-def _on(t: torch.Tensor, engine: ComputeEngine, name: str) -> int:
-    if t.is_cuda and t.device.index != engine.device:
-        raise ValueError(f"{name} is on {t.device}, the engine on cuda:{engine.device}")
-    return _ptr(t)
+def _heads(t: torch.Tensor, dev: int, name: str) -> tuple[int, int]:
+    """(address, elements from a row to the next) of [rows, heads, head_dim]
+    whose heads lie one behind the other, such as a part of a fused product's rows."""
+    rows, heads, hd = t.shape
+    row, head, one = t.stride()
+    if t.get_device() != dev or (one != 1 and hd != 1) or (head != hd and heads != 1) or (row < heads * hd and rows > 1):
+        raise ValueError(f"{name}: [rows, heads, head_dim] on cuda:{dev} with contiguous rows expected, got {t.device}, "
+                         f"strides {t.stride()}")
+    return t.data_ptr(), row if rows > 1 else heads * hd
 
 
-def _heads3(t: torch.Tensor, name: str) -> tuple[int, int, int]:
+def _caches(key_cache: torch.Tensor, value_cache: torch.Tensor, hd: int, dev: int) -> tuple[int, int, int, int, int]:
+    """(K address, V address, dtype, rows, kv heads) of one layer's caches [rows, kv_heads, head_dim]."""
+    shape = key_cache.shape
+    if len(shape) != 3 or shape[2] != hd or value_cache.shape != shape or key_cache.dtype is not value_cache.dtype:
+        raise ValueError(f"key and value caches: [rows, kv_heads, {hd}] of one type expected, got {tuple(shape)} and "
+                         f"{tuple(value_cache.shape)}")
+    return (_buf(key_cache, dev, "key_cache"), _buf(value_cache, dev, "value_cache"), _dt(key_cache), shape[0],
+            shape[1])
+
+
+def _three(t: torch.Tensor, name: str):
     if t.dim() != 3:
         raise ValueError(f"{name}: [rows, heads, head_dim] expected, got {tuple(t.shape)}")
-    return tuple(t.shape)
-
-
-def _row_stride(t: torch.Tensor, engine: ComputeEngine, name: str) -> tuple[int, int]:
-    """(address, elements from a row to the next) of [rows, heads, head_dim]
-    whose rows are contiguous, such as a part of a fused product's rows."""
-    rows, heads, hd = t.shape
-    if not t.is_cuda or t.device.index != engine.device:
-        raise ValueError(f"{name}: a tensor on cuda:{engine.device} expected, got {t.device}")
-    if (t.stride(2) != 1 and hd > 1) or (t.stride(1) != hd and heads > 1) or (rows > 1 and t.stride(0) < heads * hd):
-        raise ValueError(f"{name}: the heads of a row must be contiguous")
-    return t.data_ptr(), t.stride(0) if rows > 1 else heads * hd
-
-
-def _cache_pair(key_cache, value_cache, engine, head_dim: int) -> tuple[int, int, int, int, int]:
-    """(K address, V address, dtype, rows, kv heads) of one layer's caches [rows, kv_heads, head_dim]."""
-    n, kvh, hd = _heads3(key_cache, "key_cache")
-    if key_cache.shape != value_cache.shape or key_cache.dtype != value_cache.dtype or hd != head_dim:
-        raise ValueError("key and value caches: one shape and type, with the rows' head_dim")
-    return _on(key_cache, engine, "key_cache"), _on(value_cache, engine, "value_cache"), _dt(key_cache), n, kvh
+    return t.shape
 
 
 def qk_norm_rope(engine, query, key, value, q_gamma, k_gamma, epsilon: float, rope_cache, output, key_cache,
@@ -296,29 +299,28 @@ def qk_norm_rope(engine, query, key, value, q_gamma, k_gamma, epsilon: float, ro
     (janus_qk_norm_rope in include/janus_hip.h). query, key and value are [rows,
     heads, head_dim], also as parts of one fused product's rows; output [rows,
     heads, head_dim] receives the rotated queries and may be query."""
-    rows, heads, hd = _heads3(query, "query")
-    kc, vc, kv_dt, cache_rows, kvh = _cache_pair(key_cache, value_cache, engine, hd)
-    if tuple(key.shape) != (rows, kvh, hd) or tuple(value.shape) != (rows, kvh, hd):
-        raise ValueError(f"key and value: [{rows}, {kvh}, {hd}] expected")
-    if tuple(output.shape) != (rows, heads, hd):
-        raise ValueError("output: the query's shape expected")
-    if query.dtype != key.dtype or query.dtype != value.dtype:
+    dev = engine.device
+    shape = _three(query, "query")
+    rows, heads, hd = shape
+    kc, vc, kv_dt, cache_rows, kvh = _caches(key_cache, value_cache, hd, dev)
+    kv_shape = (rows, kvh, hd)
+    if key.shape != kv_shape or value.shape != kv_shape or output.shape != shape:
+        raise ValueError(f"key and value: {kv_shape}, output: {tuple(shape)} expected, got {tuple(key.shape)}, "
+                         f"{tuple(value.shape)}, {tuple(output.shape)}")
+    dtype = query.dtype
+    if key.dtype is not dtype or value.dtype is not dtype:
         raise ValueError("query, key and value: one type expected")
-    for g in (q_gamma, k_gamma):
-        if g is not None and (g.dtype != torch.float32 or g.numel() != hd):
-            raise ValueError(f"gamma: {hd} float32 values expected")
-    if rope_cache.dtype != torch.float32 or rope_cache.numel() < max_seq_len * hd:
-        raise ValueError(f"rope_cache: {max_seq_len} rows of {hd} float32 values expected")
     if row_base is None and rows * max_seq_len > cache_rows:
         raise ValueError("without row_base the cache holds max_seq_len rows for each row")
-    q, qs = _row_stride(query, engine, "query")
-    k, ks = _row_stride(key, engine, "key")
-    v, vs = _row_stride(value, engine, "value")
+    q, qs = _heads(query, dev, "query")
+    k, ks = _heads(key, dev, "key")
+    v, vs = _heads(value, dev, "value")
+    f32, i32 = torch.float32, torch.int32
     engine._check(engine.lib.janus_qk_norm_rope(
-        engine.ctx, q, k, v, _dt(query), qs, ks, vs, None if q_gamma is None else _on(q_gamma, engine, "q_gamma"),
-        None if k_gamma is None else _on(k_gamma, engine, "k_gamma"), epsilon, _on(rope_cache, engine, "rope_cache"),
-        _on(output, engine, "output"), _dt(output), kc, vc, kv_dt, rows, heads, kvh, hd, position, max_seq_len,
-        _index(row_base, rows, engine, "row_base"), _index(positions, rows, engine, "positions")))
+        engine.ctx, q, k, v, _dt(query), qs, ks, vs, _table(q_gamma, f32, hd, dev, "q_gamma"),
+        _table(k_gamma, f32, hd, dev, "k_gamma"), epsilon, _table(rope_cache, f32, max_seq_len * hd, dev, "rope_cache"),
+        _buf(output, dev, "output"), _dt(output), kc, vc, kv_dt, rows, heads, kvh, hd, position, max_seq_len,
+        _table(row_base, i32, rows, dev, "row_base"), _table(positions, i32, rows, dev, "positions")))
 
 
 def prompt_attention(engine, query, key_cache, value_cache, output, nseq: int, max_seq_len: int,
@@ -328,16 +330,20 @@ def prompt_attention(engine, query, key_cache, value_cache, output, nseq: int, m
     cache (janus_prompt_attention in include/janus_hip.h): sequence s has the
     rows [q_start[s], q_start[s + 1]) of query [rows, heads, head_dim], the last
     of its seq_lens[s] positions, which lie in the cache from row_base[s] on."""
-    rows, heads, hd = _heads3(query, "query")
-    kc, vc, kv_dt, cache_rows, kvh = _cache_pair(key_cache, value_cache, engine, hd)
-    if output.shape != query.shape or output.dtype != query.dtype:
+    dev = engine.device
+    shape = _three(query, "query")
+    rows, heads, hd = shape
+    kc, vc, kv_dt, cache_rows, kvh = _caches(key_cache, value_cache, hd, dev)
+    if output.shape != shape or output.dtype is not query.dtype:
         raise ValueError("output: the query's shape and type expected")
     if row_base is None and nseq * max_seq_len > cache_rows:
         raise ValueError("without row_base the cache holds max_seq_len rows for each sequence")
+    i32 = torch.int32
     engine._check(engine.lib.janus_prompt_attention(
-        engine.ctx, _on(query, engine, "query"), _dt(query), kc, vc, kv_dt, _on(output, engine, "output"), rows, nseq,
-        heads, kvh, hd, max_seq_len, _index(q_start, nseq + 1, engine, "q_start"),
-        _index(row_base, nseq, engine, "row_base"), _index(seq_lens, nseq, engine, "seq_lens"), max_len_hint, scale))
+        engine.ctx, _buf(query, dev, "query"), _dt(query), kc, vc, kv_dt, _buf(output, dev, "output"), rows, nseq,
+        heads, kvh, hd, max_seq_len, _table(q_start, i32, nseq + 1, dev, "q_start"),
+        _table(row_base, i32, nseq, dev, "row_base"), _table(seq_lens, i32, nseq, dev, "seq_lens"), max_len_hint,
+        scale))
 
 
 def prefix_attention(engine, query, key_cache, value_cache, output, prefix_row: int, prefix_len: int,
@@ -347,18 +353,21 @@ def prefix_attention(engine, query, key_cache, value_cache, output, prefix_row: 
     cache rows [prefix_row, prefix_row + prefix_len), and its own positions behind
     it, [row_base[b], row_base[b] + seq_lens[b]) (janus_prefix_attention in
     include/janus_hip.h)."""
-    batch, heads, hd = _heads3(query, "query")
-    kc, vc, kv_dt, cache_rows, kvh = _cache_pair(key_cache, value_cache, engine, hd)
-    if output.shape != query.shape or output.dtype != query.dtype:
+    dev = engine.device
+    shape = _three(query, "query")
+    batch, heads, hd = shape
+    kc, vc, kv_dt, cache_rows, kvh = _caches(key_cache, value_cache, hd, dev)
+    if output.shape != shape or output.dtype is not query.dtype:
         raise ValueError("output: the query's shape and type expected")
     if prefix_row < 0 or prefix_len < 0 or prefix_row + prefix_len > cache_rows:
         raise ValueError("the prefix lies beyond the cache")
     if row_base is None and (seq_lens is not None or seq_len) and batch * max_seq_len > cache_rows:
         raise ValueError("without row_base the cache holds max_seq_len rows for each sequence")
+    i32 = torch.int32
     engine._check(engine.lib.janus_prefix_attention(
-        engine.ctx, _on(query, engine, "query"), _dt(query), kc, vc, kv_dt, _on(output, engine, "output"), batch,
-        heads, kvh, hd, prefix_row, prefix_len, seq_len, max_seq_len, _index(row_base, batch, engine, "row_base"),
-        _index(seq_lens, batch, engine, "seq_lens"), max_len_hint, scale))
+        engine.ctx, _buf(query, dev, "query"), _dt(query), kc, vc, kv_dt, _buf(output, dev, "output"), batch, heads,
+        kvh, hd, prefix_row, prefix_len, seq_len, max_seq_len, _table(row_base, i32, batch, dev, "row_base"),
+        _table(seq_lens, i32, batch, dev, "seq_lens"), max_len_hint, scale))
 
 
 # ---- embedding and sampling ---------------------------------------------------------

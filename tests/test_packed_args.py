@@ -92,6 +92,7 @@ def test_head_refusals(vctx):
 def test_tensor_checks():
     """The Python wrappers refuse shapes, types and devices that the C call could not see."""
     eng = ops.ComputeEngine(-1)
+    eng.device = 0
     q, kv = torch.zeros(4, 8, 64), torch.zeros(32, 2, 64)
     idx = torch.zeros(5, dtype=torch.int32)
     with pytest.raises(ValueError):   # CPU tensors
@@ -104,7 +105,7 @@ def test_tensor_checks():
         ops.prompt_attention(eng, q.view(4, 512), kv, kv, q, 1, 32)
     with pytest.raises(ValueError, match="key and value caches"):
         ops.prompt_attention(eng, q, kv, kv.half(), q, 1, 32)
-    with pytest.raises(ValueError):
-        ops._index(idx.long(), 5, eng, "q_start")
-    with pytest.raises(ValueError):
-        ops._index(idx, 6, eng, "q_start")
+    with pytest.raises(ValueError, match="q_start"):
+        ops._table(idx.long(), torch.int32, 5, 0, "q_start")
+    with pytest.raises(ValueError, match="at least 6"):
+        ops._table(idx, torch.int32, 6, 0, "q_start")
