@@ -196,6 +196,10 @@ template <typename KV> __device__ __forceinline__ ju4 finite_part(ju4 v) {
     return v;
 }
 
+// Most columns that few_columns takes (two column tiles of two-part q and P would
+// not fit the registers).
+template <typename Q, typename KV> constexpr uint32_t few_of() { return Range<Q, KV>::TWO ? 16u : 32u; }
+
 // 2^sh that takes the largest of the elements to 2^14 .. 2^15 (below 2^-85 no
 // score counts), so that two binary16 parts hold 22 bits of it, and of the others
 // down to 2^-39 of it.
@@ -561,22 +565,319 @@ __device__ __forceinline__ void few_columns(const PackedArgs &a, const Work &w, 
     }
 }
 
+// 16 bytes per lane from base + off straight into LDS at lds + 16 * lane (lds is
+// uniform and goes to M0). Inline assembly, so that the compiler does not wait for
+// these requests at its LDS reads: the loop below waits for them itself.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void lds_request(const unsigned char *base, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds)
+                 : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+// Columns [c, end) of a tile that met an infinity or NaN, on one wavefront: lanes are
+// positions for the scores and dims for the output, everything in binary32, and
+// masked positions stay out of every sum.
+template <typename Q, int D>
+__device__ __forceinline__ void odd_columns(const PackedArgs &a, const Work &w, uint32_t kvh, uint32_t c, uint32_t end,
+                                         uint32_t p0, uint32_t p1) {
+    constexpr int E = D / 64;
+    const uint32_t lane = threadIdx.x & 63u;
+    const size_t kvrow = (size_t)a.kv_heads * D;
+    const _Float16 *kc = (const _Float16 *)a.kc + (w.kv_row * a.kv_heads + kvh) * D;
+    const _Float16 *vc = (const _Float16 *)a.vc + (w.kv_row * a.kv_heads + kvh) * D;
+#pragma unroll 1
+    for (; c < end; ++c) {
+        const uint32_t row = c / a.G, lim = min(seen_of(w, row), p1);
+        const size_t qat = (size_t)(w.row0 + row) * a.heads + kvh * a.G + (c - row * a.G);
+        const Q *q = (const Q *)a.q + qat * D;
+        float m = -INFINITY, l = 0.0f, o[E] = {};
+#pragma unroll 1
+        for (uint32_t p = p0; p < lim; p += 64) {
+            float s = 0.0f;
+            const _Float16 *k = kc + min(p + lane, lim - 1) * kvrow;
+#pragma unroll 1
+            for (int d = 0; d < D; ++d) s = fmaf((float)q[d], (float)k[d], s);
+            s = p + lane < lim ? s : -INFINITY;
+            const float mn = fmaxf(m, wave_max(s)), mr = mn == -INFINITY ? 0.0f : mn;
+            const float alpha = mn == m ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * a.scale2);
+            const float x = __builtin_amdgcn_exp2f((s - mr) * a.scale2);
+            m = mn;
+            l = l * alpha + wave_sum(x);
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] *= alpha;
+#pragma unroll 1
+            for (uint32_t j = 0; j < min(64u, lim - p); ++j) {
+                const float y = __shfl(x, (int)j, 64);
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[e] = fmaf(y, (float)vc[(p + j) * kvrow + E * lane + e], o[e]);
+            }
+        }
+        if (a.slots) {
+            const size_t at = qat * a.slots + w.slot;
+            if (lane == 0) *(float2 *)(a.part_ml + 2 * at) = make_float2(m, l);
+#pragma unroll
+            for (int e = 0; e < E; ++e) a.part[at * D + E * lane + e] = o[e];
+        } else {
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+            for (int e = 0; e < E; ++e) ((Q *)a.out)[qat * D + E * lane + e] = (Q)(o[e] * inv);
+        }
+    }
+}
+
+// 17 or 33 to 128 columns on a binary16 cache: K and V pass through LDS for all four
+// wavefronts, 32 columns each, requested a tile ahead straight into LDS.
+//
+// The vector unit is as busy as the matrix unit (a wavefront's tile of 64 positions
+// is 32 MFMAs of 17 ns, about 100 other instructions of 2.1 ns and 32 exponentials
+// of 5.2 ns, and only the exponentials overlap with the MFMAs of the other
+// wavefront in full), so whatever a score does not need is kept out: no look at the
+// values on their way (an infinity or NaN shows in the sums at the end, and the
+// wavefront then takes odd_columns), offsets made once, l summed from pairs of P.
+// Tried and slower: the scores of the next tile before the softmax of this one
+// (32 registers more, which spill).
+//   S^T: position 8 (v / 4) + 4 h + v % 4 of column lane % 32 in s[v], h = lane / 32
+template <typename Q, int D>
+__device__ __forceinline__ void wide_tile(const PackedArgs &a, const Work &w, uint32_t kvh, uint32_t ncols, uint32_t p0,
+                                          uint32_t p1, unsigned char *smem) {
+    typedef Range<Q, _Float16> R;
+    typedef Lay<D> Y;
+    constexpr bool TWO = R::TWO;
+    constexpr int TP = sizeof(Q) == 2 ? 64 : 32;   // positions per tile
+    constexpr int NB = TP / 32, ND = D / 32, QN = D / 16;
+    constexpr uint32_t TB = TP * Y::RB;            // bytes of a tile of K or V; LDS: K, V, K, V
+    constexpr int LD = TB / 4096;                  // 1 KB requests per wavefront and tile
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t col = lane & 31u, h = lane >> 5;
+    const uint32_t kvrow = a.kv_heads * Y::RB;     // bytes from a position to the next
+    const unsigned char *kc = (const unsigned char *)a.kc + (w.kv_row * a.kv_heads + kvh) * Y::RB;
+    const unsigned char *vc = (const unsigned char *)a.vc + (w.kv_row * a.kv_heads + kvh) * Y::RB;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)smem;
+    // request j of this wavefront: row and permuted segment of its lanes
+    auto row_of = [&](int j) { return (lane + 64u * (wave * LD + j)) / Y::SEGS; };
+    auto seg_of = [&](int j, bool v) { return (lane % Y::SEGS ^ (v ? Y::v_swz(row_of(j)) : Y::k_swz(row_of(j)))) * 16u; };
+    uint32_t ko[LD], vo[LD];
+#pragma unroll
+    for (int j = 0; j < LD; ++j) {
+        ko[j] = row_of(j) * kvrow + seg_of(j, false);
+        vo[j] = row_of(j) * kvrow + seg_of(j, true);
+    }
+    // the tile of positions from p on into buffer b: K, then V
+    auto request = [&](uint32_t p, uint32_t b) {
+        const unsigned char *kp = kc + (size_t)p * kvrow, *vp = vc + (size_t)p * kvrow;
+        const uint32_t to = lds0 + b * 2 * TB + wave * LD * 1024u;
+        if (p + TP <= p1) {
+#pragma unroll
+            for (int j = 0; j < LD; ++j) {
+                lds_request(kp, ko[j], to + j * 1024u);
+                lds_request(vp, vo[j], to + TB + j * 1024u);
+            }
+        } else {   // rows beyond the part repeat its last one
+#pragma unroll
+            for (int j = 0; j < LD; ++j) {
+                const uint32_t at = min(row_of(j), p1 - 1 - p) * kvrow;
+                lds_request(kp, at + seg_of(j, false), to + j * 1024u);
+                lds_request(vp, at + seg_of(j, true), to + TB + j * 1024u);
+            }
+        }
+    };
+    if (p0 < p1) request(p0, 0);
+
+    const uint32_t wc0 = w.c0 + 32u * wave;
+    const bool idle = wc0 >= ncols;     // uniform: this wavefront only helps to load
+    const uint32_t wave_lo = idle ? 0u : seen_of(w, wc0 / a.G);
+    const uint32_t wave_hi = idle ? 0u : min(seen_of(w, min(wc0 + 31u, ncols - 1) / a.G), p1);
+    const uint32_t c = min(wc0 + col, ncols - 1), qrow = c / a.G, head = kvh * a.G + (c - qrow * a.G);
+    const uint32_t lim = min(seen_of(w, qrow), p1);
+    const size_t qat = ((size_t)(w.row0 + qrow) * a.heads + head);
+
+    // q of this lane's column
+    const Q *qp = (const Q *)a.q + qat * D;
+    ph8 qh[QN], ql[TWO ? QN : 1];
+    float sc2 = a.scale2, qs = 1.0f;
+    if constexpr (!TWO) {
+#pragma unroll
+        for (int s = 0; s < QN; ++s) qh[s] = *(const ph8 *)(qp + 16 * s + 8 * h);
+    } else {
+        float qmax = 0.0f;
+        jf4 x[QN][2];
+#pragma unroll
+        for (int s = 0; s < QN; ++s) {
+            x[s][0] = *(const jf4 *)(qp + 16 * s + 8 * h);
+            x[s][1] = *(const jf4 *)(qp + 16 * s + 8 * h + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) qmax = fmaxf(qmax, fmaxf(fabsf(x[s][0][i]), fabsf(x[s][1][i])));
+        }
+        qs = two_part_scale(fmaxf(qmax, swap32(qmax)));
+        sc2 /= qs;
+#pragma unroll
+        for (int s = 0; s < QN; ++s)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float y = x[s][i >> 2][i & 3] * qs;
+                qh[s][i] = (_Float16)y;
+                ql[s][i] = (_Float16)(y - (float)qh[s][i]);
+            }
+    }
+
+    pf16 o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[d] = (pf16){};
+    float m = -INFINITY, l = 0.0f;
+    // q has arrived before the tiles begin: the compiler's wait for it among them
+    // would be one for the next tile too
+    if constexpr (!TWO) {
+#pragma unroll
+        for (int t = 0; t < QN; ++t) asm volatile("" : "+v"(qh[t]));
+    }
+    // lanes 16 g + i of half h read dims 32 d + 16 g + 4 (i % 4) .. of positions
+    // 4 h + i / 4 (+ 8) of a step of V and receive dim 32 d + 16 g + i of four positions
+    const uint32_t vrow = 4u * h + ((lane & 15u) >> 2);
+    const uint32_t vat = vrow * Y::RB + ((2u * ((lane >> 4) & 1u) + ((lane & 3u) >> 1)) ^ Y::v_swz(vrow)) * 16u + (lane & 1u) * 8u;
+    const uint32_t kat = col * Y::RB + (h ^ Y::k_swz(col)) * 16u;
+    uint32_t b = 0;
+    for (uint32_t p = p0; p < p1; p += TP, b ^= 1u) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();   // this tile is there, the other buffer has been read
+        if (p + TP < p1) request(p + TP, b ^ 1u);
+        if (p >= wave_hi) continue;
+        const unsigned char *kt = smem + b * 2 * TB, *vt = kt + TB;
+        pf16 s[NB], lo = (pf16){};
+        ph8 k[NB][QN];
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int t = 0; t < QN; ++t) k[n][t] = *(const ph8 *)(kt + (kat ^ (t * 32u)) + n * 32 * Y::RB);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            s[n] = (pf16){};
+#pragma unroll
+            for (int t = 0; t < QN; ++t) {
+                s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[n][t], qh[t], s[n], 0, 0, 0);
+                if constexpr (TWO) lo = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[n][t], ql[t], lo, 0, 0, 0);
+            }
+        }
+        // The operands of 32 positions are requested together, and those of the next
+        // 32 one by one behind the products: left to itself the compiler waits for
+        // each before it asks for the next.
+        __builtin_amdgcn_sched_group_barrier(0x100, QN, 0);
+        if constexpr (NB == 2)
+#pragma unroll
+            for (int t = 0; t < QN; ++t) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+        __builtin_amdgcn_sched_group_barrier(0x008, NB == 2 ? QN : 2 * QN, 0);
+        if constexpr (TWO) {
+#pragma unroll
+            for (int v = 0; v < 16; ++v) s[0][v] += lo[v];
+        }
+        if (p + TP > min(wave_lo, p1)) {
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) s[n][v] = p + 32 * n + 8 * (v >> 2) + 4 * h + (v & 3) < lim ? s[n][v] : -INFINITY;
+        }
+        float top[2];
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+            top[v] = s[0][v];
+#pragma unroll
+            for (int x = v + 2; x < 16 * NB; x += 2) top[v] = fmaxf(top[v], s[x >> 4][x & 15]);
+        }
+        float bm = fmaxf(top[0], top[1]);
+        bm = fmaxf(bm, swap32(bm));
+        if (__any((bm - m) * sc2 > R::SLACK || (m == -INFINITY && bm != -INFINITY))) {
+            const float mn = fmaxf(m, bm), alpha = mn == m ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * sc2);
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) o[d][v] *= alpha;
+        }
+        // while only masked or NaN scores have come, m counts as 0: 2^-inf is 0, a NaN stays
+        const float mr = m == -INFINITY ? 0.0f : m, ms = R::BIAS - mr * sc2;
+        float sum[2] = {};
+#pragma unroll
+        for (int t = 0; t < 2 * NB; ++t) {
+            ph8 ph, pl;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float y = s[t >> 1][8 * (t & 1) + e];
+                // binary32 rows: the difference is exact near the maximum
+                const float x = __builtin_amdgcn_exp2f(TWO ? fmaf(y - mr, sc2, R::BIAS) : fmaf(y, sc2, ms));
+                ph[e] = (_Float16)x;
+                if constexpr (TWO) {
+                    pl[e] = (_Float16)(x - (float)ph[e]);
+                    sum[e & 1] += x;
+                }
+            }
+            if constexpr (!TWO) {   // of P as rounded: both sums see the same weights
+                const jh2 one = {(_Float16)1.0f, (_Float16)1.0f};
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) sum[(e >> 1) & 1] = __builtin_amdgcn_fdot2(jh2{ph[e], ph[e + 1]}, one, sum[(e >> 1) & 1], false);
+            }
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                const unsigned char *at = vt + (vat ^ (d * 64u)) + 16 * t * Y::RB;
+                const ps4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)at);
+                const ps4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + 8 * Y::RB));
+                const ph8 v = __builtin_bit_cast(ph8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph, o[d], 0, 0, 0);
+                if constexpr (TWO) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl, o[d], 0, 0, 0);
+            }
+        }
+        l += sum[0] + sum[1];
+    }
+
+    l += swap32(l);
+    // an infinity or NaN anywhere makes the sum a NaN
+    float odd = l * 0.0f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) odd = fmaf(o[d][v], 0.0f, odd);
+    if (idle) return;
+    if (__any(odd != odd)) {
+        odd_columns<Q, D>(a, w, kvh, wc0, min(wc0 + 32u, ncols), p0, p1);
+        return;
+    }
+    if (wc0 + col >= ncols) return;
+    if (a.slots) {
+        const size_t at = qat * a.slots + w.slot;
+        if (h == 0) *(float2 *)(a.part_ml + 2 * at) = make_float2(m / qs, l);
+        if (p0 >= p1) return;   // the join reads no output of a part without positions
+        float *to = a.part + at * D;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                *(jf4 *)(to + 32 * d + 8 * j + 4 * h) = jf4{o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]};
+        return;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;   // a row that sees nothing is 0
+    Q *to = (Q *)a.out + qat * D;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            typedef Q q4 __attribute__((ext_vector_type(4)));
+            q4 y;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = (Q)(o[d][4 * j + i] * inv);
+            *(q4 *)(to + 32 * d + 8 * j + 4 * h) = y;
+        }
+}
+
 // Q: _Float16 or float rows; KV: the cache's type.
 template <typename Q, typename KV, int D>
 __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedArgs a) {
-    typedef Range<Q, KV> R;
-    typedef Lay<D> Y;
-    constexpr bool H = R::H, TWO = R::TWO;
-    constexpr uint32_t COLS = cols_of(H);
-    constexpr int TP = sizeof(Q) == 2 ? 64 : 32;   // positions per tile
-    constexpr int NB = TP / 32, ND = D / 32;
-    constexpr uint32_t VB = TP * Y::RB, FLAGS = 2 * VB, BUF = FLAGS + 16;   // bytes of a buffer
-    constexpr int LD = TP * Y::SEGS / 256;         // 16-byte segments per thread, of K and of V
-    static_assert(LD >= 1 && LD * 256 == TP * (int)Y::SEGS, "tile load");
+    constexpr bool H = sizeof(KV) == 2;
+    constexpr uint32_t COLS = cols_of(H), TP = 64;   // parts begin at whole tiles
     extern __shared__ __align__(16) unsigned char smem[];
-    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t col = lane & 31u, h = lane >> 5;
-
     // neighbouring workgroups take the KV heads, so that with 8 of them each XCD
     // keeps the K and V of one head in its L2
     const uint32_t kvh = blockIdx.x % a.kv_heads, id = blockIdx.x / a.kv_heads;
@@ -603,278 +904,14 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedArgs a) {
     // this workgroup's part of the positions
     const uint32_t per = (((end_all + w.splits - 1) / w.splits) + TP - 1) / TP * TP;
     const uint32_t p0 = min(w.split * per, end_all), p1 = min(p0 + per, end_all);
-    if (!H || ncols - w.c0 <= 32) {
-        if (ncols - w.c0 <= 16) few_columns<Q, KV, D, 1>(a, w, kvh, ncols, p0, p1, smem);
-        else few_columns<Q, KV, D, 2>(a, w, kvh, ncols, p0, p1, smem);
-        return;
-    }
     if constexpr (H) {
-    const uint32_t wc0 = w.c0 + 32u * wave;
-    const bool idle = wc0 >= ncols;     // uniform: this wavefront only helps to load
-    const uint32_t wave_lo = idle ? 0u : seen_of(w, wc0 / a.G), wave_hi = idle ? 0u : seen_of(w, min(wc0 + 31u, ncols - 1) / a.G);
-    const uint32_t c = min(wc0 + col, ncols - 1), qrow = c / a.G, head = kvh * a.G + c % a.G;
-    const bool mine = wc0 + col < ncols;
-    const uint32_t seen = seen_of(w, qrow);
-    const size_t qat = ((size_t)(w.row0 + qrow) * a.heads + head);
-
-    const uint32_t kvrow = a.kv_heads * Y::RB;   // bytes from a position to the next
-    const unsigned char *kc = (const unsigned char *)a.kc + (w.kv_row * a.kv_heads + kvh) * Y::RB;
-    const unsigned char *vc = (const unsigned char *)a.vc + (w.kv_row * a.kv_heads + kvh) * Y::RB;
-
-    ju4 kr[LD], vr[LD];
-    auto load = [&](uint32_t p) {
-        const unsigned char *kp = kc + (size_t)p * kvrow, *vp = vc + (size_t)p * kvrow;
-        const uint32_t last = p1 - 1 - p;   // rows beyond the part repeat its last one
-#pragma unroll
-        for (int j = 0; j < LD; ++j) {
-            const uint32_t s = threadIdx.x + 256u * j, off = min(s / Y::SEGS, last) * kvrow + s % Y::SEGS * 16u;
-            kr[j] = *(const ju4 *)(kp + off);
-            vr[j] = *(const ju4 *)(vp + off);
-        }
-    };
-    auto store = [&](unsigned char *t) {
-        float oddv = 0.0f, oddk = 0.0f;
-#pragma unroll
-        for (int j = 0; j < LD; ++j) {
-            oddv = odd_sum<KV>(vr[j], oddv);
-            if (TWO) oddk = odd_sum<KV>(kr[j], oddk);
-        }
-        const uint32_t any = (uint32_t)(__any(oddv != oddv) != 0) | (uint32_t)(__any(oddk != oddk) != 0) << 1;
-        if (lane == 0) *(uint32_t *)(t + FLAGS + 4 * wave) = any;
-        // A probability of 0 does not mask an infinity or NaN of V: such values stay
-        // out of the products and are added on their own, for the rows that see them.
-        if (any & 1u)
-#pragma unroll
-            for (int j = 0; j < LD; ++j) vr[j] = finite_part<KV>(vr[j]);
-#pragma unroll
-        for (int j = 0; j < LD; ++j) {
-            const uint32_t s = threadIdx.x + 256u * j, row = s / Y::SEGS, seg = s % Y::SEGS;
-            *(ju4 *)(t + row * Y::RB + (seg ^ Y::k_swz(row)) * 16u) = kr[j];
-            *(ju4 *)(t + VB + row * Y::RB + (seg ^ Y::v_swz(row)) * 16u) = vr[j];
-        }
-    };
-    if (p0 < p1) load(p0);
-
-    // q of this lane's column
-    const Q *qp = (const Q *)a.q + qat * D;
-    constexpr int QN = D / 16;
-    ph8 qh[QN], ql[TWO ? QN : 1];
-    float sc2 = a.scale2, qs = 1.0f;
-    bool q_inf = false;
-    if constexpr (!TWO) {
-#pragma unroll
-        for (int s = 0; s < QN; ++s) qh[s] = *(const ph8 *)(qp + 16 * s + 8 * h);
-    } else {
-        float qmax = 0.0f;
-        jf4 x[QN][2];
-#pragma unroll
-        for (int s = 0; s < QN; ++s) {
-            x[s][0] = *(const jf4 *)(qp + 16 * s + 8 * h);
-            x[s][1] = *(const jf4 *)(qp + 16 * s + 8 * h + 4);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) qmax = fmaxf(qmax, fmaxf(fabsf(x[s][0][i]), fabsf(x[s][1][i])));
-        }
-        qmax = fmaxf(qmax, swap32(qmax));
-        q_inf = __any(qmax == INFINITY);
-        qs = two_part_scale(qmax);
-        sc2 /= qs;
-#pragma unroll
-        for (int s = 0; s < QN; ++s)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float y = x[s][i >> 2][i & 3] * qs;
-                qh[s][i] = (_Float16)y;
-                ql[s][i] = (_Float16)(y - (float)qh[s][i]);
-            }
-    }
-
-    pf16 o[ND];
-#pragma unroll
-    for (int d = 0; d < ND; ++d) o[d] = (pf16){};
-    float m = -INFINITY, l = 0.0f;
-
-    if (p0 < p1) store(smem);
-    // q has arrived before the tiles begin: a wait for it among them would be one for
-    // the loads of the next tile too
-    if constexpr (!TWO) {
-#pragma unroll
-        for (int s = 0; s < QN; ++s) asm volatile("" : "+v"(qh[s]));
-    }
-    uint32_t buf = 0;
-    for (uint32_t p = p0; p < p1; p += TP) {
-        const bool more = p + TP < p1;
-        if (more) load(p + TP);
-        __syncthreads();
-        const unsigned char *kt = smem + buf * BUF, *vt = kt + VB;
-        if (p < wave_hi) {
-            const uint4 f = *(const uint4 *)(kt + FLAGS);
-            const uint32_t flags = __builtin_amdgcn_readfirstlane(f.x | f.y | f.z | f.w);
-            pf16 s[NB], lo = (pf16){};
-            ph8 k[NB][QN];
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const uint32_t row = 32u * b + col, swz = Y::k_swz(row);
-#pragma unroll
-                for (int t = 0; t < QN; ++t) k[b][t] = *(const ph8 *)(kt + row * Y::RB + ((2u * t + h) ^ swz) * 16u);
-            }
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                s[b] = (pf16){};
-#pragma unroll
-                for (int t = 0; t < QN; ++t) {
-                    s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[b][t], qh[t], s[b], 0, 0, 0);
-                    if constexpr (TWO) lo = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[b][t], ql[t], lo, 0, 0, 0);
-                }
-            }
-            // The operands of 32 positions are requested together, and those of the
-            // next 32 one by one behind the products: left to itself the compiler
-            // waits for each before it asks for the next.
-            __builtin_amdgcn_sched_group_barrier(0x100, QN, 0);
-            if constexpr (NB == 2)
-#pragma unroll
-                for (int t = 0; t < QN; ++t) {
-                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-                }
-            __builtin_amdgcn_sched_group_barrier(0x008, NB == 2 ? QN : 2 * QN, 0);
-            if constexpr (TWO) {
-#pragma unroll
-                for (int v = 0; v < 16; ++v) s[0][v] += lo[v];
-            }
-            if constexpr (TWO)
-                // an infinity times a part of q that is 0 or of the other sign would make
-                // a NaN of an infinite score: such tiles take q whole
-                if (q_inf || (flags & 2u)) {
-                    s[0] = (pf16){};
-#pragma unroll 1
-                    for (uint32_t d = 0; d < D; ++d) {
-                        const float x = (float)qp[d];
-#pragma unroll
-                        for (int v = 0; v < 16; ++v) {
-                            const uint32_t row = 8u * (v >> 2) + 4u * h + (v & 3);
-                            s[0][v] = fmaf(x, (float)*(const _Float16 *)(kt + row * Y::RB + ((d / 8) ^ Y::k_swz(row)) * 16u + d % 8 * 2u), s[0][v]);
-                        }
-                    }
-#pragma unroll
-                    for (int v = 0; v < 16; ++v) s[0][v] *= qs;
-                }
-            // s[b][v]: position p + 32 b + 8 (v / 4) + 4 h + v % 4
-            if (p + TP > min(wave_lo, p1)) {
-                const uint32_t lim = min(seen, p1);
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-#pragma unroll
-                    for (int v = 0; v < 16; ++v)
-                        s[b][v] = p + 32 * b + 8 * (v >> 2) + 4 * h + (v & 3) < lim ? s[b][v] : -INFINITY;
-            }
-            float top[4];
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                top[v] = s[0][v];
-#pragma unroll
-                for (int x = v + 4; x < 16 * NB; x += 4) top[v] = fmaxf(top[v], s[x >> 4][x & 15]);
-            }
-            float bm = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-            bm = fmaxf(bm, swap32(bm));
-            if (__any((bm - m) * sc2 > R::SLACK || (m == -INFINITY && bm != -INFINITY))) {
-                const float mn = fmaxf(m, bm), alpha = mn == m ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * sc2);
-                m = mn;
-                l *= alpha;
-#pragma unroll
-                for (int d = 0; d < ND; ++d)
-#pragma unroll
-                    for (int v = 0; v < 16; ++v) o[d][v] *= alpha;
-            }
-            // while only masked or NaN scores have come, m counts as 0: 2^-inf is 0, a NaN stays
-            const float mr = m == -INFINITY ? 0.0f : m, ms = sizeof(Q) == 2 ? R::BIAS - mr * sc2 : 0.0f;
-            float sum[4] = {};
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    // binary32 rows: the difference is exact near the maximum
-                    s[b][v] = sizeof(Q) == 2 ? __builtin_amdgcn_exp2f(fmaf(s[b][v], sc2, ms))
-                                             : __builtin_amdgcn_exp2f(fmaf(s[b][v] - mr, sc2, R::BIAS));
-                    sum[v & 3] += s[b][v];
-                }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            {
-                // lanes 16 g + i of half h read dims 32 d + 16 g + 4 (i % 4) .. of positions
-                // 4 h + i / 4 (+ 8) of a step and receive dim 32 d + 16 g + i of four positions
-                const uint32_t i = lane & 15u, g = (lane >> 4) & 1u;
-                const uint32_t vrow = 4u * h + (i >> 2), vseg = 2u * g + ((i & 3u) >> 1), vin = (i & 1u) * 8u;
-#pragma unroll
-                for (int t = 0; t < 2 * NB; ++t) {
-                    ph8 ph, pl;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float x = s[t >> 1][8 * (t & 1) + e];
-                        ph[e] = (_Float16)x;
-                        if constexpr (TWO) pl[e] = (_Float16)(x - (float)ph[e]);
-                    }
-#pragma unroll
-                    for (int d = 0; d < ND; ++d) {
-                        const uint32_t at = (16u * t + vrow) * Y::RB + ((4u * d + vseg) ^ Y::v_swz(vrow)) * 16u + vin;
-                        const ps4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(vt + at));
-                        const ps4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(vt + at + 8 * Y::RB));
-                        const ph8 v = __builtin_bit_cast(ph8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph, o[d], 0, 0, 0);
-                        if constexpr (TWO) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl, o[d], 0, 0, 0);
-                    }
-                }
-            }
-            if (flags & 1u) {
-                // the infinities and NaN of V, for the columns that see their position
-                const uint32_t lim = min(seen, p1);
-#pragma unroll 1
-                for (uint32_t j = 0; j < min((uint32_t)TP, p1 - p); ++j) {
-                    float ph = 0.0f;   // p of position j, held by half (j / 4) % 2
-#pragma unroll
-                    for (int b = 0; b < NB; ++b)
-#pragma unroll
-                        for (int v = 0; v < 16; ++v) ph = 32u * b + 8u * (v >> 2) + (v & 3) + (j & 4u) == j ? s[b][v] : ph;
-                    const float other = swap32(ph), pj = ((j >> 2) & 1u) == h ? ph : other;
-                    const KV *vrow = (const KV *)(vc + (size_t)(p + j) * kvrow);
-#pragma unroll
-                    for (int d = 0; d < ND; ++d)
-#pragma unroll
-                        for (int v = 0; v < 16; ++v) {
-                            const float x = (float)vrow[32 * d + 8 * (v >> 2) + 4 * h + (v & 3)];
-                            if (p + j < lim && (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u) o[d][v] = fmaf(pj, x, o[d][v]);
-                        }
-                }
-            }
-        }
-        buf ^= 1u;
-        if (more) store(smem + buf * BUF);   // last read before the barrier above
-    }
-    if (idle || !mine) return;
-    l += swap32(l);
-    if (a.slots) {
-        const size_t at = qat * a.slots + w.slot;
-        if (h == 0) *(float2 *)(a.part_ml + 2 * at) = make_float2(m / qs, l);
-        if (p0 >= p1) return;   // the join reads no output of a part without positions
-        float *to = a.part + at * D;
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                *(jf4 *)(to + 32 * d + 8 * j + 4 * h) = jf4{o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]};
-        return;
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;   // a row that sees nothing is 0
-    Q *to = (Q *)a.out + qat * D;
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            typedef Q q4 __attribute__((ext_vector_type(4)));
-            q4 y;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] = (Q)(o[d][4 * j + i] * inv);
-            *(q4 *)(to + 32 * d + 8 * j + 4 * h) = y;
+        if (ncols - w.c0 > few_of<Q, KV>()) {
+            wide_tile<Q, D>(a, w, kvh, ncols, p0, p1, smem);
+            return;
         }
     }
+    if (few_of<Q, KV>() == 16 || ncols - w.c0 <= 16) few_columns<Q, KV, D, 1>(a, w, kvh, ncols, p0, p1, smem);
+    else few_columns<Q, KV, D, few_of<Q, KV>() / 16>(a, w, kvh, ncols, p0, p1, smem);
 }
 
 // Joins the parts of a row and head: a wavefront each. A part holds m, l and the
@@ -930,7 +967,7 @@ __global__ __launch_bounds__(256) void packed_join_kernel(PackedArgs a) {
 template <typename Q, typename KV, int D>
 int launch(janus_ctx *ctx, const PackedArgs &a, uint32_t blocks) {
     // two tiles of K and V, or the join of the wavefronts of few columns
-    constexpr size_t tiles = sizeof(KV) == 2 ? 2 * (2 * (sizeof(Q) == 2 ? 64 : 32) * D * 2 + 16) : 0;
+    constexpr size_t tiles = sizeof(KV) == 2 ? 4 * (sizeof(Q) == 2 ? 64 : 32) * D * 2 : 0;
     constexpr size_t lds = std::max<size_t>(tiles, 4 * 32 * (8 + (D + 4) * 4));
     static const hipError_t attr = hipFuncSetAttribute((const void *)packed_attn_kernel<Q, KV, D>,
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, lds);

@@ -20,7 +20,9 @@ def attend(q, k, v, seen, rows_f16, cache_f16, scale=None):
     The output is off by at most (2 eta + weights' rounding + n additions) of
     sum_j p_j |v_j|, and its own rounding. Weights: binary16 rows round them to
     binary16 (2^-11, and 2^-31 of the largest where they are tiny), binary32 rows
-    on a binary16 cache to two parts (2^-22, and 2^-38 of the largest)."""
+    on a binary16 cache to two parts (2^-22, and 2^-38 of the largest). Where the
+    rounded weights are also summed, sum p (1 + d) v / sum p (1 + d) is off by
+    sum p d (v - out) <= max |d| (sum p |v| + |out|)."""
     q, k, v = q.double(), k.double(), v.double()
     n, heads, hd = q.shape
     rep = heads // k.shape[1]
@@ -55,7 +57,7 @@ def attend(q, k, v, seen, rows_f16, cache_f16, scale=None):
         steps = torch.as_tensor(seen).double()[:, None].clamp(max=length) * 2 * U32 + 16 * U32
         pv = p @ vh.abs()
         out[:, h] = p @ vh
-        tol[:, h] = (2 * eta + weight + steps) * pv + floor / total.clamp(min=1e-300) * (there.double() @ vh.abs()) \
+        tol[:, h] = (2 * eta + weight + steps) * pv + weight * out[:, h].abs() + floor / total.clamp(min=1e-300) * (there.double() @ vh.abs()) \
             + (U16 if rows_f16 else U32) * out[:, h].abs() + 1e-30
         if rows_f16:
             tol[:, h] += 2.0 ** -25   # half a step of binary16's smallest values
