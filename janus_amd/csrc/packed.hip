@@ -39,9 +39,9 @@ typedef float pf4 __attribute__((ext_vector_type(4)));
 typedef float pf16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) ps4 *lds4;
 
-// Columns per workgroup: 128 through shared tiles, 32 where every wavefront reads
+// Columns per workgroup: 128 through shared tiles, 64 where every wavefront reads
 // its own positions (binary32 caches).
-constexpr uint32_t cols_of(bool kv_f16) { return kv_f16 ? 128u : 32u; }
+constexpr uint32_t cols_of(bool kv_f16) { return kv_f16 ? 128u : 64u; }
 
 struct PackedArgs {
     const void *q;            // [rows][heads][D]
@@ -55,9 +55,12 @@ struct PackedArgs {
     uint32_t rows, nseq, heads, kv_heads, G;
     uint32_t max_seq;
     int64_t seq_len;          // < 0: the rows
-    uint32_t splits;          // workgroups per tile (prefix: per own tile)
+    uint32_t splits;          // most parts of a tile's positions (1: never split)
+    uint32_t target;          // parts per KV head to aim at
     uint32_t slots;           // partials per row and head (0: results are written)
     uint32_t prefix_row, prefix_len, prefix_tiles, prefix_splits;
+    uint32_t prefix_blocks, own_blocks, mix, pairs;   // workgroups; runs of `mix` of both alternate
+    uint32_t longest;         // 1: tiles by the position that they reach
     float scale2;             // scale * log2(e)
 };
 
@@ -68,7 +71,7 @@ struct Work {
     size_t kv_row;            // cache row of position 0
     uint32_t len;             // positions
     bool causal;
-    uint32_t split, splits, slot;
+    uint32_t part, parts, chunk, slot;   // positions [part chunk, + chunk); slot of the partials
 };
 
 __device__ __forceinline__ float swap32(float v) {   // value of lane ^ 32
@@ -102,23 +105,94 @@ __device__ __forceinline__ void sequence_of(const PackedArgs &a, uint32_t s, Wor
     w.kv_row = base < 0 ? 0 : (size_t)base;
 }
 
-// The sequence and tile of tile number t (sequences in order, a sequence's tiles
-// from its last to its first, the longest first); false: there is none.
-template <uint32_t COLS> __device__ __forceinline__ bool find_tile(const PackedArgs &a, uint32_t t, Work &w) {
+// The sequence, tile and part of task t; false: there is none. A sequence's tiles
+// go from its last to its first.
+//
+// Splitting (few tiles): the tables give the positions of all tiles, and every part
+// gets as many, so that long and short contexts take equal workgroups (drafted
+// tokens of 16 requests with 200 to 4000 positions: 44 -> 39 us against equal counts
+// of parts). Every
+// workgroup finds the same numbers.
+//
+// With `longest`, the tiles of all sequences go by the position that they reach, the
+// farthest first, so that no long one is begun when the others are done; else the
+// sequences follow each other, which keeps their K and V in L2. Binary32 caches take
+// the former (six prompts of 33 to 512 rows at 32/32/128: 92 -> 75 us), where a
+// position costs 16 times the matrix time; binary16 caches the latter (24 prompts
+// of 3 to 700 rows at 32/8/128: 94 against 98 us).
+template <uint32_t COLS> __device__ __forceinline__ bool find_task(const PackedArgs &a, uint32_t t, Work &w) {
     const uint32_t lane = threadIdx.x & 63u;
     w.causal = true;
-    if (!a.q_start) {
+    w.part = 0;
+    w.parts = 1;
+    w.chunk = 0x80000000u;
+    if (!a.q_start && a.splits == 1) {
         const uint32_t each = (uint32_t)(((uint64_t)(a.rows / a.nseq) * a.G + COLS - 1) / COLS), s = t / each;
         if (s >= a.nseq) return false;
         sequence_of(a, s, w);
         w.c0 = (each - 1 - t % each) * COLS;
         return true;
     }
-    for (uint32_t s0 = 0; s0 < a.nseq; s0 += 64) {   // a lane per sequence
-        Work x;
+    // a lane per sequence; tiles of it
+    Work x;
+    auto sequence = [&](uint32_t s0) -> uint32_t {
         sequence_of(a, min(s0 + lane, a.nseq - 1), x);
-        const uint32_t mine = s0 + lane < a.nseq ? (uint32_t)(((uint64_t)x.n * a.G + COLS - 1) / COLS) : 0u;
-        uint32_t upto = mine;
+        return s0 + lane < a.nseq ? (uint32_t)(((uint64_t)x.n * a.G + COLS - 1) / COLS) : 0u;
+    };
+    auto take = [&](int at, uint32_t tile) {
+        auto pick = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane(v, at); };
+        w.row0 = pick(x.row0);
+        w.n = pick(x.n);
+        w.len = pick(x.len);
+        w.kv_row = pick((uint32_t)x.kv_row);   // below 2^31
+        w.c0 = tile * COLS;
+        return true;
+    };
+    uint32_t mine = sequence(0);
+    if (a.longest) {   // at most 16 sequences, not split
+        // levels: a tile's distance from position 0 in tiles; lane j counts those from lo + j step on
+        const uint32_t before = x.len > x.n ? (uint32_t)min((uint64_t)(x.len - x.n) * a.G / COLS, (uint64_t)1 << 30) : 0u;
+        const uint32_t top = before + mine;
+        uint32_t most = mine ? top : 0u;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) most = max(most, (uint32_t)shfl_xor((int)most, o));
+        most = __builtin_amdgcn_readfirstlane(most);
+        uint32_t lo = 0, above = 0;   // level of task t, tiles above it
+        for (uint32_t step = 1u << max(0, 26 - (int)__builtin_clz(most | 1u));; step = step > 64 ? step >> 6 : 1) {
+            const uint32_t level = lo + lane * step;
+            uint32_t count = 0;
+            for (uint32_t s = 0; s < a.nseq; ++s)
+                count += (uint32_t)min(max((int32_t)(__builtin_amdgcn_readlane(top, s) - level), 0), (int32_t)__builtin_amdgcn_readlane(mine, s));
+            const uint64_t hit = __ballot(count > t);   // the first lanes: count falls with the level
+            if (!hit) return false;
+            const int at = 63 - __builtin_clzll(hit);
+            lo = __builtin_amdgcn_readlane(level, at);
+            if (at < 63) above = __builtin_amdgcn_readlane(count, at + 1);   // else as found with the longer step
+            if (step == 1) break;
+        }
+        uint64_t has = __ballot(mine && before <= lo && lo < top);
+        for (uint32_t r = t - above; r; --r) has &= has - 1;
+        const int at = __ffsll((unsigned long long)has) - 1;
+        return take(at, lo - __builtin_amdgcn_readlane(before, at));
+    }
+    if (a.splits > 1) {
+        float total = 0.0f;
+        uint32_t longest = 0;
+        for (uint32_t s0 = 0; s0 < a.nseq; s0 += 64) {
+            const uint32_t tiles = s0 ? sequence(s0) : mine;
+            total += (float)tiles * (float)x.len;
+            longest = max(longest, tiles ? x.len : 0u);
+        }
+        total = wave_sum_dpp(total);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) longest = max(longest, (uint32_t)shfl_xor((int)longest, o));
+        const uint32_t even = (uint32_t)fminf(total / (float)a.target, 1e9f) + 1, least = (longest + a.splits - 1) / a.splits;
+        w.chunk = __builtin_amdgcn_readfirstlane((max(max(even, least), 128u) + 63u) / 64u * 64u);
+        if (a.nseq > 64) mine = sequence(0);
+    }
+    for (uint32_t s0 = 0;;) {
+        const uint32_t parts = max((x.len + w.chunk - 1) / w.chunk, 1u), tasks = mine * parts;
+        uint32_t upto = tasks;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const uint32_t v = __shfl_up(upto, o, 64);
@@ -127,17 +201,15 @@ template <uint32_t COLS> __device__ __forceinline__ bool find_tile(const PackedA
         const uint64_t hit = __ballot(t < upto);
         if (hit) {
             const int at = __ffsll((unsigned long long)hit) - 1;
-            auto pick = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane(v, at); };
-            w.row0 = pick(x.row0);
-            w.n = pick(x.n);
-            w.len = pick(x.len);
-            w.kv_row = pick((uint32_t)x.kv_row);   // below 2^31
-            w.c0 = (pick(mine) - 1 - (t - pick(upto - mine))) * COLS;
-            return true;
+            const uint32_t r = t - __builtin_amdgcn_readlane(upto - tasks, at);
+            w.parts = __builtin_amdgcn_readlane(parts, at);
+            w.part = r % w.parts;
+            return take(at, __builtin_amdgcn_readlane(mine, at) - 1 - r / w.parts);
         }
         t -= __builtin_amdgcn_readlane(upto, 63);
+        if ((s0 += 64) >= a.nseq) return false;
+        mine = sequence(s0);
     }
-    return false;
 }
 
 // Positions that row i of the work sees: all, or len - n + 1 + i.
@@ -196,8 +268,8 @@ template <typename KV> __device__ __forceinline__ ju4 finite_part(ju4 v) {
     return v;
 }
 
-// Most columns that few_columns takes (two column tiles of two-part q and P would
-// not fit the registers).
+// Most columns that few_columns takes on a binary16 cache (two column tiles of
+// two-part q and P would not fit the registers).
 template <typename Q, typename KV> constexpr uint32_t few_of() { return Range<Q, KV>::TWO ? 16u : 32u; }
 
 // 2^sh that takes the largest of the elements to 2^14 .. 2^15 (below 2^-85 no
@@ -209,9 +281,10 @@ __device__ __forceinline__ float two_part_scale(float qmax) {
     return ldexpf(1.0f, -max(qe - 15, -100));
 }
 
-// Results of up to 32 columns and the positions [p0, p1): the wavefronts take
-// steps of positions in turn, each reading its own K and V, and are joined
-// through LDS. A column is a lane of 16; NT column tiles share the operands.
+// Results of up to 16 NT CW columns and the positions [p0, p1), no barrier on the
+// way: the wavefronts are CW groups of columns (1 or 2) by 4 / CW of positions; those
+// of a group take steps of positions in turn, each reading its own K and V, and are
+// joined through LDS. A column is a lane of 16; NT column tiles share the operands.
 //   S^T [16 positions x 16 columns]: lane 16 g + i holds positions 4 g + v of
 //   column i. K comes from memory as the operand: position i, its dims by g.
 //   binary16: steps of 32 positions (two S^T), v_mfma_f32_16x16x32_f16; V through
@@ -221,7 +294,7 @@ __device__ __forceinline__ float two_part_scale(float qmax) {
 //     o[4 e + c] holds dims 4 (4 g + v + 16 e) + c.
 template <typename Q, typename KV, int D, int NT>
 __device__ __forceinline__ void few_columns(const PackedArgs &a, const Work &w, uint32_t kvh, uint32_t ncols,
-                                            uint32_t p0, uint32_t p1, unsigned char *smem) {
+                                            uint32_t p0, uint32_t p1, uint32_t cw, unsigned char *smem) {
     typedef Range<Q, KV> R;
     typedef Lay<D> Y;
     constexpr bool H = R::H, TWO = R::TWO;
@@ -232,10 +305,14 @@ __device__ __forceinline__ void few_columns(const PackedArgs &a, const Work &w, 
     constexpr uint32_t RB = D * sizeof(KV);
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t i = lane & 15u, g = lane >> 4;
+    const uint32_t pw = 4u / cw, cg = wave & (cw - 1u), pg = wave / cw;   // this wavefront's columns and positions
+    const uint32_t c0 = w.c0 + 16u * NT * cg;
     const uint32_t kvrow = a.kv_heads * RB;          // bytes from a position to the next
     const unsigned char *kc = (const unsigned char *)a.kc + (w.kv_row * a.kv_heads + kvh) * RB;
     const unsigned char *vc = (const unsigned char *)a.vc + (w.kv_row * a.kv_heads + kvh) * RB;
 
+    // the positions that this wavefront's columns see at all
+    const uint32_t e1 = c0 < ncols ? min(seen_of(w, min(c0 + 16u * NT - 1, ncols - 1) / a.G), p1) : 0u;
     ju4 kr[NB][KS], vr[VS];
     auto load_k = [&](uint32_t p) {
         const unsigned char *at = kc + (size_t)p * kvrow;
@@ -243,7 +320,7 @@ __device__ __forceinline__ void few_columns(const PackedArgs &a, const Work &w, 
         for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int t = 0; t < KS; ++t)
-                kr[b][t] = *(const ju4 *)(at + (min(16u * b + i, p1 - 1 - p) * kvrow + (4u * t + g) * 16u));
+                kr[b][t] = *(const ju4 *)(at + (min(16u * b + i, e1 - 1 - p) * kvrow + (4u * t + g) * 16u));
     };
     auto load_v = [&](uint32_t p) {
         const unsigned char *at = vc + (size_t)p * kvrow;
@@ -252,11 +329,11 @@ __device__ __forceinline__ void few_columns(const PackedArgs &a, const Work &w, 
             // binary16: in order; binary32: position 4 g + j / E, segment i + 16 (j % E)
             constexpr int E = D / 64;
             const uint32_t s = lane + 64u * j, row = H ? s / Y::SEGS : 4u * g + j / E, seg = H ? s % Y::SEGS : i + 16u * (j % E);
-            vr[j] = *(const ju4 *)(at + (min(row, p1 - 1 - p) * kvrow + seg * 16u));
+            vr[j] = *(const ju4 *)(at + (min(row, e1 - 1 - p) * kvrow + seg * 16u));
         }
     };
-    uint32_t p = p0 + STEP * wave;
-    if (p < p1) {
+    uint32_t p = p0 + STEP * pg;
+    if (p < e1) {
         load_k(p);
         load_v(p);
     }
@@ -266,14 +343,15 @@ __device__ __forceinline__ void few_columns(const PackedArgs &a, const Work &w, 
     ph8 qh[H ? NT : 1][QN], ql[TWO ? NT : 1][QN];
     jf4 qf[H ? 1 : NT][D / 16];
     float sc2[NT], qs[NT];
-    uint32_t lim[NT];
+    uint32_t lim[NT], qat[NT];
     const Q *qp[NT];
     bool q_inf = false;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        const uint32_t c = min(w.c0 + 16u * n + i, ncols - 1), row = c / a.G;
+        const uint32_t c = min(c0 + 16u * n + i, ncols - 1), row = c / a.G;
         lim[n] = min(seen_of(w, row), p1);
-        qp[n] = (const Q *)a.q + ((size_t)(w.row0 + row) * a.heads + kvh * a.G + (c - row * a.G)) * D;
+        qat[n] = (w.row0 + row) * a.heads + kvh * a.G + (c - row * a.G);   // below 2^25
+        qp[n] = (const Q *)a.q + (size_t)qat[n] * D;
         sc2[n] = a.scale2;
         qs[n] = 1.0f;
         if constexpr (!H) {
@@ -307,7 +385,7 @@ __device__ __forceinline__ void few_columns(const PackedArgs &a, const Work &w, 
                 }
         }
     }
-    const uint32_t lo = min(seen_of(w, w.c0 / a.G), p1);   // every column sees [0, lo)
+    const uint32_t lo = c0 < ncols ? min(seen_of(w, c0 / a.G), p1) : 0u;   // every column sees [0, lo)
 
     // q has arrived before the steps begin: a wait for it among them would be one for
     // the loads of the next step too
@@ -330,8 +408,8 @@ __device__ __forceinline__ void few_columns(const PackedArgs &a, const Work &w, 
         for (int d = 0; d < ND; ++d) o[n][d] = (pf4){};
     }
     unsigned char *vt = smem + wave * (32u * Y::RB);   // this wavefront's V tile (binary16)
-    for (; p < p1; p += 4 * STEP) {
-        const bool more = p + 4 * STEP < p1;
+    for (const uint32_t stride = pw * STEP; p < e1; p += stride) {
+        const bool more = p + stride < e1;
         pf4 s[NT][NB];
 #pragma unroll
         for (int b = 0; b < NB; ++b)
@@ -374,7 +452,7 @@ __device__ __forceinline__ void few_columns(const PackedArgs &a, const Work &w, 
                     for (int b = 0; b < NB; ++b)
 #pragma unroll
                         for (int v = 0; v < 4; ++v) {
-                            const uint32_t at = min(16u * b + 4u * g + v, p1 - 1 - p);
+                            const uint32_t at = min(16u * b + 4u * g + v, e1 - 1 - p);
                             const KV *k = (const KV *)(kc + (size_t)(p + at) * kvrow);
                             float x = 0.0f;
 #pragma unroll 1
@@ -383,7 +461,7 @@ __device__ __forceinline__ void few_columns(const PackedArgs &a, const Work &w, 
                         }
             }
         }
-        if (more) load_k(p + 4 * STEP);
+        if (more) load_k(p + stride);
         // An infinity or NaN of V stays out of the products and is added on its own.
         float odd = 0.0f;
 #pragma unroll
@@ -398,7 +476,7 @@ __device__ __forceinline__ void few_columns(const PackedArgs &a, const Work &w, 
                 const uint32_t at = lane + 64u * j, row = at / Y::SEGS, seg = at % Y::SEGS;
                 *(ju4 *)(vt + row * Y::RB + (seg ^ Y::few_swz(row)) * 16u) = vr[j];
             }
-            if (more) load_v(p + 4 * STEP);
+            if (more) load_v(p + stride);
         }
         if (p + STEP > lo) {
 #pragma unroll
@@ -473,11 +551,11 @@ __device__ __forceinline__ void few_columns(const PackedArgs &a, const Work &w, 
 #pragma unroll
                         for (int n = 0; n < NT; ++n)
                             o[n][4 * e + c] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[v * E + e][c]), s[n][0][v], o[n][4 * e + c], 0, 0, 0);
-            if (more) load_v(p + 4 * STEP);
+            if (more) load_v(p + stride);
         }
         if (odd_v) {
 #pragma unroll 1
-            for (uint32_t j = 0; j < min((uint32_t)STEP, p1 - p); ++j) {
+            for (uint32_t j = 0; j < min((uint32_t)STEP, e1 - p); ++j) {
                 const KV *row = (const KV *)(vc + (size_t)(p + j) * kvrow);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
@@ -499,12 +577,11 @@ __device__ __forceinline__ void few_columns(const PackedArgs &a, const Work &w, 
         }
     }
 
-    // join the wavefronts that had positions
-    constexpr uint32_t C = 16 * NT, OS = D + 4;   // padded: 16 columns meet 16 bank groups
-    const uint32_t nw = min((p1 - min(p0, p1) + STEP - 1) / STEP, 4u);
-    float2 *ml = (float2 *)smem;                   // [wave][column]
-    float *oo = (float *)(smem + 4 * 32 * sizeof(float2));   // [wave][column][OS]
-    __syncthreads();
+    // join the wavefronts of a group
+    constexpr uint32_t C = 16 * NT, OS = D + 4;    // padded: 16 columns meet 16 bank groups
+    float *oo = (float *)smem;                     // [wave][column][OS], over the V tiles
+    float2 *ml = (float2 *)(smem + 4 * 32 * OS * 4);   // [wave][column]
+    float4 *fin = (float4 *)(ml + 4 * 32);         // [group][column]: m, l, 1 / l, row and head
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         l[n] += swap16(l[n]);
@@ -512,55 +589,58 @@ __device__ __forceinline__ void few_columns(const PackedArgs &a, const Work &w, 
         m[n] = m[n] / qs[n];
         if (g == 0) ml[wave * C + 16 * n + i] = make_float2(m[n], l[n]);
     }
-    __syncthreads();
-    if (wave < nw) {
+    __syncthreads();   // also: every V tile has been read
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            float M = -INFINITY;
-            for (uint32_t x = 0; x < nw; ++x) M = fmaxf(M, ml[x * C + 16 * n + i].x);
-            const float f = m[n] == M ? 1.0f : __builtin_amdgcn_exp2f((m[n] - M) * a.scale2);
-            float *to = oo + (wave * C + 16 * n + i) * OS;
-            if constexpr (H) {
+    for (int n = 0; n < NT; ++n) {
+        float2 all[4];   // of the group; a wavefront beyond it repeats one
+        float M = -INFINITY, lt = 0.0f;
 #pragma unroll
-                for (int d = 0; d < ND; ++d)
-                    *(jf4 *)(to + 16 * d + 4 * g) = jf4{o[n][d][0] * f, o[n][d][1] * f, o[n][d][2] * f, o[n][d][3] * f};
-            } else {
-#pragma unroll
-                for (int e = 0; e < D / 64; ++e)
-#pragma unroll
-                    for (int v = 0; v < 4; ++v)
-                        *(jf4 *)(to + 4 * (4 * g + v + 16 * e)) = jf4{o[n][4 * e][v] * f, o[n][4 * e + 1][v] * f, o[n][4 * e + 2][v] * f, o[n][4 * e + 3][v] * f};
-            }
+        for (uint32_t x = 0; x < 4; ++x) {
+            all[x] = ml[(cg + min(x, pw - 1u) * cw) * C + 16 * n + i];
+            M = fmaxf(M, all[x].x);
         }
+#pragma unroll
+        for (uint32_t x = 0; x < 4; ++x)
+            if (x < pw) lt = fmaf(all[x].y, all[x].x == M ? 1.0f : __builtin_amdgcn_exp2f((all[x].x - M) * a.scale2), lt);
+        const float f = m[n] == M ? 1.0f : __builtin_amdgcn_exp2f((m[n] - M) * a.scale2);
+        float *to = oo + (wave * C + 16 * n + i) * OS;
+        if constexpr (H) {
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+                *(jf4 *)(to + 16 * d + 4 * g) = jf4{o[n][d][0] * f, o[n][d][1] * f, o[n][d][2] * f, o[n][d][3] * f};
+        } else {
+#pragma unroll
+            for (int e = 0; e < D / 64; ++e)
+#pragma unroll
+                for (int v = 0; v < 4; ++v)
+                    *(jf4 *)(to + 4 * (4 * g + v + 16 * e)) = jf4{o[n][4 * e][v] * f, o[n][4 * e + 1][v] * f, o[n][4 * e + 2][v] * f, o[n][4 * e + 3][v] * f};
+        }
+        if (pg == 0 && g == 0)   // a row that sees nothing is 0
+            fin[cg * C + 16 * n + i] = make_float4(M, lt, lt == 0.0f ? 0.0f : 1.0f / lt, __uint_as_float(qat[n]));
     }
     __syncthreads();
-#pragma unroll
-    for (uint32_t at = threadIdx.x; at < C * (D / 4); at += 256) {
-        const uint32_t col = at / (D / 4), dim = at % (D / 4) * 4u, c = w.c0 + col;
-        if (c >= ncols) break;
-        float M = -INFINITY, lt = 0.0f;
-        for (uint32_t x = 0; x < nw; ++x) M = fmaxf(M, ml[x * C + col].x);
-        jf4 sum = {};
-        for (uint32_t x = 0; x < nw; ++x) {
-            const float2 y = ml[x * C + col];
-            lt = fmaf(y.y, y.x == M ? 1.0f : __builtin_amdgcn_exp2f((y.x - M) * a.scale2), lt);
-            const jf4 z = *(const jf4 *)(oo + (x * C + col) * OS + dim);
+    const uint32_t cols = min(C * cw, ncols - w.c0);
+    for (uint32_t at = threadIdx.x; at < cols * (D / 4); at += 256) {
+        const uint32_t x = at / (D / 4), dim = at % (D / 4) * 4u, group = x / C;
+        const float4 f = fin[x];
+        const float *from = oo + (size_t)(group * C + x % C) * OS + dim;   // wavefront `group`, then every cw-th
+        jf4 sum = *(const jf4 *)from;
+        for (uint32_t y = 1; y < pw; ++y) {
+            const jf4 z = *(const jf4 *)(from + y * cw * C * OS);
 #pragma unroll
             for (int e = 0; e < 4; ++e) sum[e] += z[e];
         }
-        const uint32_t row = c / a.G;
-        const size_t qat = (size_t)(w.row0 + row) * a.heads + kvh * a.G + (c - row * a.G);
+        const size_t to = __float_as_uint(f.w);
         if (a.slots) {
-            const size_t part = qat * a.slots + w.slot;
-            if (dim == 0) *(float2 *)(a.part_ml + 2 * part) = make_float2(M, lt);
-            if (nw) *(jf4 *)(a.part + part * D + dim) = sum;   // the join reads no output of a part without positions
+            const size_t part = to * a.slots + w.slot;
+            if (dim == 0) *(float2 *)(a.part_ml + 2 * part) = make_float2(f.x, f.y);
+            *(jf4 *)(a.part + part * D + dim) = sum;
         } else {
-            const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;   // a row that sees nothing is 0
             typedef Q q4 __attribute__((ext_vector_type(4)));
             q4 y;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = (Q)(sum[e] * inv);
-            *(q4 *)((Q *)a.out + qat * D + dim) = y;
+            for (int e = 0; e < 4; ++e) y[e] = (Q)(sum[e] * f.z);
+            *(q4 *)((Q *)a.out + to * D + dim) = y;
         }
     }
 }
@@ -876,16 +956,32 @@ __device__ __forceinline__ void wide_tile(const PackedArgs &a, const Work &w, ui
 template <typename Q, typename KV, int D>
 __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedArgs a) {
     constexpr bool H = sizeof(KV) == 2;
-    constexpr uint32_t COLS = cols_of(H), TP = 64;   // parts begin at whole tiles
+    constexpr uint32_t COLS = cols_of(H);
     extern __shared__ __align__(16) unsigned char smem[];
     // neighbouring workgroups take the KV heads, so that with 8 of them each XCD
     // keeps the K and V of one head in its L2
-    const uint32_t kvh = blockIdx.x % a.kv_heads, id = blockIdx.x / a.kv_heads;
+    uint32_t block = blockIdx.x;
+    bool shared = block < a.prefix_blocks;
+    if (a.pairs) {   // runs of prefix and own workgroups in turn, then what is left of either
+        const uint32_t run = block / a.mix;
+        if (run < 2 * a.pairs) {
+            shared = !(run & 1u);
+            block -= (run + 1) / 2 * a.mix;
+        } else {
+            block -= a.pairs * a.mix;
+            shared = block < a.prefix_blocks;
+            if (!shared) block -= a.prefix_blocks - a.pairs * a.mix;
+        }
+    } else if (!shared) {
+        block -= a.prefix_blocks;
+    }
+    const uint32_t kvh = block % a.kv_heads, id = block / a.kv_heads;
     Work w;
-    if (id < a.prefix_tiles * a.prefix_splits) {
-        w.split = id % a.prefix_splits;
-        w.splits = a.prefix_splits;
-        w.slot = w.split;
+    if (shared) {
+        w.part = id % a.prefix_splits;
+        w.parts = a.prefix_splits;
+        w.chunk = ((a.prefix_len + a.prefix_splits - 1) / a.prefix_splits + 63u) / 64u * 64u;
+        w.slot = w.part;
         w.row0 = 0;
         w.n = a.rows;
         w.c0 = id / a.prefix_splits * COLS;
@@ -893,25 +989,29 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedArgs a) {
         w.len = a.prefix_len;
         w.causal = false;
     } else {
-        const uint32_t rest = id - a.prefix_tiles * a.prefix_splits;
-        w.split = rest % a.splits;
-        w.splits = a.splits;
-        w.slot = a.prefix_splits + w.split;
-        if (!find_tile<COLS>(a, rest / a.splits, w)) return;
+        if (!find_task<COLS>(a, id, w)) return;
+        w.slot = a.prefix_splits + w.part;
     }
     const uint32_t ncols = w.n * a.G;   // n * G <= rows * heads < 2^32
     const uint32_t end_all = seen_of(w, min(w.c0 + COLS - 1, ncols - 1) / a.G);
-    // this workgroup's part of the positions
-    const uint32_t per = (((end_all + w.splits - 1) / w.splits) + TP - 1) / TP * TP;
-    const uint32_t p0 = min(w.split * per, end_all), p1 = min(p0 + per, end_all);
+    const uint32_t p0 = min(w.part * w.chunk, end_all), p1 = min(p0 + w.chunk, end_all);
+    if (!shared && a.slots && w.part + 1 == w.parts && w.parts < a.splits) {   // parts that there are none of
+        const uint32_t none = a.splits - w.parts, cols = min(COLS, ncols - w.c0);
+        for (uint32_t x = threadIdx.x; x < cols * none; x += 256) {
+            const uint32_t c = w.c0 + x / none, row = c / a.G;
+            const size_t qat = (size_t)(w.row0 + row) * a.heads + kvh * a.G + (c - row * a.G);
+            *(float2 *)(a.part_ml + 2 * (qat * a.slots + w.slot + 1 + x % none)) = make_float2(-INFINITY, 0.0f);
+        }
+    }
     if constexpr (H) {
         if (ncols - w.c0 > few_of<Q, KV>()) {
             wide_tile<Q, D>(a, w, kvh, ncols, p0, p1, smem);
             return;
         }
     }
-    if (few_of<Q, KV>() == 16 || ncols - w.c0 <= 16) few_columns<Q, KV, D, 1>(a, w, kvh, ncols, p0, p1, smem);
-    else few_columns<Q, KV, D, few_of<Q, KV>() / 16>(a, w, kvh, ncols, p0, p1, smem);
+    const uint32_t cols = ncols - w.c0;
+    if (few_of<Q, KV>() == 16 || cols <= 16) few_columns<Q, KV, D, 1>(a, w, kvh, ncols, p0, p1, 1, smem);
+    else few_columns<Q, KV, D, 2>(a, w, kvh, ncols, p0, p1, cols > 32 ? 2 : 1, smem);
 }
 
 // Joins the parts of a row and head: a wavefront each. A part holds m, l and the
@@ -968,7 +1068,7 @@ template <typename Q, typename KV, int D>
 int launch(janus_ctx *ctx, const PackedArgs &a, uint32_t blocks) {
     // two tiles of K and V, or the join of the wavefronts of few columns
     constexpr size_t tiles = sizeof(KV) == 2 ? 4 * (sizeof(Q) == 2 ? 64 : 32) * D * 2 : 0;
-    constexpr size_t lds = std::max<size_t>(tiles, 4 * 32 * (8 + (D + 4) * 4));
+    constexpr size_t lds = std::max<size_t>(tiles, 4 * 32 * ((D + 4) * 4 + 8) + 64 * 16);
     static const hipError_t attr = hipFuncSetAttribute((const void *)packed_attn_kernel<Q, KV, D>,
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     (void)attr;
@@ -988,24 +1088,42 @@ int launch_typed(janus_ctx *ctx, const PackedArgs &a, int q_dt, int kv_dt, uint3
     return hd == 64 ? launch<float, float, 64>(ctx, a, blocks) : launch<float, float, 128>(ctx, a, blocks);
 }
 
-// Workgroups per tile so that `tiles` of them fill the CUs (two on each), each
-// with 256 positions at least.
-uint32_t plan_splits(const janus_ctx *ctx, uint64_t tiles, uint32_t max_len) {
+// Parts of a tile so that `tiles` of them fill the CUs (two workgroups on each),
+// each with `least` positions at least.
+uint32_t plan_splits(const janus_ctx *ctx, uint64_t tiles, uint32_t max_len, uint32_t least) {
     const uint64_t want = 2ull * ctx->num_cus / std::max<uint64_t>(tiles, 1);
-    return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(want, (max_len + 255) / 256));
+    return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(want, (max_len + least - 1) / least));
 }
 
-int run(janus_ctx *ctx, PackedArgs a, int q_dt, int kv_dt, uint32_t hd, uint64_t tiles) {
-    const uint64_t blocks = tiles * a.kv_heads;
-    if (blocks * 256 >= (1ull << 32) || (uint64_t)a.rows * a.heads >= (1ull << 25))
+// The parts of a request's own positions, where `likely` tiles are expected and
+// there are at most `tiles`: returns the tasks per KV head.
+uint64_t plan_own(const janus_ctx *ctx, PackedArgs &a, uint64_t likely, uint64_t tiles, uint32_t max_len) {
+    const uint32_t want = plan_splits(ctx, likely * a.kv_heads, max_len, 128);
+    a.splits = 1;
+    if (want == 1) return tiles;
+    // of several requests one may take four times the mean (the workspace is sized for that)
+    a.splits = a.nseq == 1 ? want : std::min(4 * want, std::max(2u, (max_len + 127) / 128));
+    a.target = std::max(1u, 2u * (uint32_t)ctx->num_cus / a.kv_heads);
+    return tiles + a.target + 1;   // sum of tiles * ceil(len / chunk) <= target + tiles
+}
+
+int run(janus_ctx *ctx, PackedArgs a, int q_dt, int kv_dt, uint32_t hd, uint64_t own_tasks) {
+    const uint64_t prefix = (uint64_t)a.prefix_tiles * a.prefix_splits * a.kv_heads, own = own_tasks * a.kv_heads;
+    if ((prefix + own) * 256 >= (1ull << 32) || (uint64_t)a.rows * a.heads >= (1ull << 25))
         return fail(ctx, JANUS_E_INVALID_DIM, "attention: more rows than one launch takes");
+    a.prefix_blocks = (uint32_t)prefix;
+    a.own_blocks = (uint32_t)own;
+    // A prefix is bound by the matrix unit, the requests' own positions by memory: a
+    // CU gets one workgroup of each.
+    a.mix = ((uint32_t)ctx->num_cus + a.kv_heads - 1) / a.kv_heads * a.kv_heads;
+    a.pairs = std::min(a.prefix_blocks, a.own_blocks) / a.mix;
     if (a.slots) {
         const size_t parts = (size_t)a.rows * a.heads * a.slots;
         if (int e = ensure_attn_ws(ctx, parts * (hd + 2) * sizeof(float))) return e;
         a.part = (float *)ctx->attn_ws;
         a.part_ml = a.part + parts * hd;
     }
-    return launch_typed(ctx, a, q_dt, kv_dt, hd, (uint32_t)blocks);
+    return launch_typed(ctx, a, q_dt, kv_dt, hd, (uint32_t)(prefix + own));
 }
 
 }  // namespace
@@ -1026,9 +1144,10 @@ int prompt_attention_launch(janus_ctx *ctx, const void *q, int q_dt, const void 
     const uint64_t tiles = (uint64_t)rows * a.G / cols + nseq;
     // about as many as sequences of equal rows have
     const uint64_t likely = (uint64_t)nseq * (((rows + nseq - 1) / nseq * (uint64_t)a.G + cols - 1) / cols);
-    a.splits = plan_splits(ctx, likely * kv_heads, std::min(max_len, max_seq));
+    const uint64_t tasks = plan_own(ctx, a, likely, tiles, std::min(max_len, max_seq));
     a.slots = a.splits > 1 ? a.splits : 0;
-    return run(ctx, a, q_dt, kv_dt, hd, tiles * a.splits);
+    a.longest = kv_dt != JANUS_DT_F16 && a.splits == 1 && nseq > 1 && nseq <= 16 && likely * kv_heads > 2u * (uint32_t)ctx->num_cus;
+    return run(ctx, a, q_dt, kv_dt, hd, tasks);
 }
 
 int prefix_attention_launch(janus_ctx *ctx, const void *q, int q_dt, const void *kc, const void *vc, int kv_dt,
@@ -1047,11 +1166,11 @@ int prefix_attention_launch(janus_ctx *ctx, const void *q, int q_dt, const void 
     const uint64_t own_tiles = (uint64_t)batch * ((a.G + cols - 1) / cols);
     if (prefix_len) {
         a.prefix_tiles = (uint32_t)(((uint64_t)batch * a.G + cols - 1) / cols);
-        a.prefix_splits = plan_splits(ctx, (uint64_t)a.prefix_tiles * kv_heads, prefix_len);
+        a.prefix_splits = plan_splits(ctx, (uint64_t)a.prefix_tiles * kv_heads, prefix_len, 256);
     }
-    a.splits = plan_splits(ctx, own_tiles * kv_heads, std::min(max_len, max_seq));
+    const uint64_t tasks = plan_own(ctx, a, own_tiles, own_tiles, std::min(max_len, max_seq));
     a.slots = a.prefix_splits + a.splits > 1 ? a.prefix_splits + a.splits : 0;
-    return run(ctx, a, q_dt, kv_dt, hd, (uint64_t)a.prefix_tiles * a.prefix_splits + own_tiles * a.splits);
+    return run(ctx, a, q_dt, kv_dt, hd, tasks);
 }
 
 }  // namespace janus
