@@ -663,6 +663,7 @@ template <typename Q, int D>
 __device__ __forceinline__ void odd_columns(const PackedArgs &a, const Work &w, uint32_t kvh, uint32_t c, uint32_t end,
                                          uint32_t p0, uint32_t p1) {
     constexpr int E = D / 64;
+    constexpr float BIAS = Range<Q, _Float16>::BIAS;
     const uint32_t lane = threadIdx.x & 63u;
     const size_t kvrow = (size_t)a.kv_heads * D;
     const _Float16 *kc = (const _Float16 *)a.kc + (w.kv_row * a.kv_heads + kvh) * D;
@@ -682,7 +683,7 @@ __device__ __forceinline__ void odd_columns(const PackedArgs &a, const Work &w, 
             s = p + lane < lim ? s : -INFINITY;
             const float mn = fmaxf(m, wave_max(s)), mr = mn == -INFINITY ? 0.0f : mn;
             const float alpha = mn == m ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * a.scale2);
-            const float x = __builtin_amdgcn_exp2f((s - mr) * a.scale2);
+            const float x = __builtin_amdgcn_exp2f(fmaf(s - mr, a.scale2, BIAS));   // parts are joined with others'
             m = mn;
             l = l * alpha + wave_sum(x);
 #pragma unroll
@@ -805,7 +806,8 @@ __device__ __forceinline__ void wide_tile(const PackedArgs &a, const Work &w, ui
     pf16 o[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[d] = (pf16){};
-    float m = -INFINITY, l = 0.0f;
+    // p = 2^(s sc2 + c), c = BIAS - m sc2 rounded: one FMA a score
+    float m = -INFINITY, c2 = INFINITY, l = 0.0f;
     // q has arrived before the tiles begin: the compiler's wait for it among them
     // would be one for the next tile too
     if constexpr (!TWO) {
@@ -824,7 +826,7 @@ __device__ __forceinline__ void wide_tile(const PackedArgs &a, const Work &w, ui
         if (p + TP < p1) request(p + TP, b ^ 1u);
         if (p >= wave_hi) continue;
         const unsigned char *kt = smem + b * 2 * TB, *vt = kt + TB;
-        pf16 s[NB], lo = (pf16){};
+        pf16 s[NB];
         ph8 k[NB][QN];
 #pragma unroll
         for (int n = 0; n < NB; ++n)
@@ -833,11 +835,11 @@ __device__ __forceinline__ void wide_tile(const PackedArgs &a, const Work &w, ui
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
             s[n] = (pf16){};
+            if constexpr (TWO)   // the small parts first
 #pragma unroll
-            for (int t = 0; t < QN; ++t) {
-                s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[n][t], qh[t], s[n], 0, 0, 0);
-                if constexpr (TWO) lo = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[n][t], ql[t], lo, 0, 0, 0);
-            }
+                for (int t = 0; t < QN; ++t) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[n][t], ql[t], s[n], 0, 0, 0);
+#pragma unroll
+            for (int t = 0; t < QN; ++t) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[n][t], qh[t], s[n], 0, 0, 0);
         }
         // The operands of 32 positions are requested together, and those of the next
         // 32 one by one behind the products: left to itself the compiler waits for
@@ -850,10 +852,6 @@ __device__ __forceinline__ void wide_tile(const PackedArgs &a, const Work &w, ui
                 __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             }
         __builtin_amdgcn_sched_group_barrier(0x008, NB == 2 ? QN : 2 * QN, 0);
-        if constexpr (TWO) {
-#pragma unroll
-            for (int v = 0; v < 16; ++v) s[0][v] += lo[v];
-        }
         if (p + TP > min(wave_lo, p1)) {
 #pragma unroll
             for (int n = 0; n < NB; ++n)
@@ -869,17 +867,20 @@ __device__ __forceinline__ void wide_tile(const PackedArgs &a, const Work &w, ui
         }
         float bm = fmaxf(top[0], top[1]);
         bm = fmaxf(bm, swap32(bm));
-        if (__any((bm - m) * sc2 > R::SLACK || (m == -INFINITY && bm != -INFINITY))) {
-            const float mn = fmaxf(m, bm), alpha = mn == m ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * sc2);
-            m = mn;
+        if (__any(fmaf(bm, sc2, c2) > R::BIAS + R::SLACK)) {
+            m = fmaxf(m, bm);
+            const float cn = fmaf(-m, sc2, R::BIAS), alpha = cn == c2 ? 1.0f : __builtin_amdgcn_exp2f(cn - c2);
+            c2 = cn;
             l *= alpha;
+            // scores so large that c does not hold their last bits: odd_columns takes the difference instead
+            if (fabsf(c2) > 4194304.0f && c2 != INFINITY) l = NAN;
 #pragma unroll
             for (int d = 0; d < ND; ++d)
 #pragma unroll
                 for (int v = 0; v < 16; ++v) o[d][v] *= alpha;
         }
         // while only masked or NaN scores have come, m counts as 0: 2^-inf is 0, a NaN stays
-        const float mr = m == -INFINITY ? 0.0f : m, ms = R::BIAS - mr * sc2;
+        const float c0 = c2 == INFINITY ? 0.0f : c2;
         float sum[2] = {};
 #pragma unroll
         for (int t = 0; t < 2 * NB; ++t) {
@@ -887,11 +888,10 @@ __device__ __forceinline__ void wide_tile(const PackedArgs &a, const Work &w, ui
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const float y = s[t >> 1][8 * (t & 1) + e];
-                // binary32 rows: the difference is exact near the maximum
-                const float x = __builtin_amdgcn_exp2f(TWO ? fmaf(y - mr, sc2, R::BIAS) : fmaf(y, sc2, ms));
+                const float x = __builtin_amdgcn_exp2f(fmaf(y, sc2, c0));
                 ph[e] = (_Float16)x;
                 if constexpr (TWO) {
-                    pl[e] = (_Float16)(x - (float)ph[e]);
+                    pl[e] = (_Float16)fmaf((float)ph[e], -1.0f, x);
                     sum[e & 1] += x;
                 }
             }
@@ -928,14 +928,16 @@ __device__ __forceinline__ void wide_tile(const PackedArgs &a, const Work &w, ui
     if (wc0 + col >= ncols) return;
     if (a.slots) {
         const size_t at = qat * a.slots + w.slot;
-        if (h == 0) *(float2 *)(a.part_ml + 2 * at) = make_float2(m / qs, l);
+        // what the rounding of c shifted, since the parts are joined by m
+        const float back = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(R::BIAS - fmaf(m, sc2, c2));
+        if (h == 0) *(float2 *)(a.part_ml + 2 * at) = make_float2(m / qs, l * back);
         if (p0 >= p1) return;   // the join reads no output of a part without positions
         float *to = a.part + at * D;
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                *(jf4 *)(to + 32 * d + 8 * j + 4 * h) = jf4{o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]};
+                *(jf4 *)(to + 32 * d + 8 * j + 4 * h) = jf4{o[d][4 * j] * back, o[d][4 * j + 1] * back, o[d][4 * j + 2] * back, o[d][4 * j + 3] * back};
         return;
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;   // a row that sees nothing is 0

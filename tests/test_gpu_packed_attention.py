@@ -98,6 +98,47 @@ def test_score_ranges(engine, types, sigma):
     _prompt(engine, types, 4, 2, 128, [(70, 300)], sigma=sigma)
 
 
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("rows", [3, 70])
+def test_scores_beyond_their_own_last_bits(engine, types, rows):
+    """Scores whose spacing is far above 1: the farthest ahead takes all weight."""
+    qt, kt = TYPES[types]
+    gen = torch.Generator().manual_seed(21)
+    hd, n, size = 128, 1100, 3e4 if qt == torch.float16 else 1e8
+    q = (_rand(gen, rows, 2, hd).sign() * size).to(qt)
+    k = _rand(gen, n, 1, hd).sign().to(kt) * 64
+    v = _rand(gen, n, 1, hd, dtype=kt)
+    out = torch.empty(q.shape, dtype=qt, device=DEV)
+    ops.prompt_attention(engine, q.to(DEV), k.to(DEV), v.to(DEV), out, 1, n, seq_lens=_i32([n]))
+    s = torch.einsum("rhd,jd->rhj", q.double(), k[:, 0].double())
+    for r in range(rows):
+        seen = s[r, :, :n - rows + 1 + r]
+        top = seen.amax(-1, keepdim=True)
+        first = (seen == top).double()   # equal ones share the weight
+        want = first @ v[:seen.shape[1], 0].double() / first.sum(-1, keepdim=True)
+        tol = 2.0 ** (-10 if qt == torch.float16 else -20) * v.abs().max().double()
+        check(out[r], want, tol.expand_as(want), (types, r))
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("rows", [2, 40])
+def test_infinity_in_one_part_of_a_split_context(engine, types, rows):
+    qt, kt = TYPES[types]
+    gen = torch.Generator().manual_seed(22)
+    heads, kvh, hd, n = 32, 8, 128, 3000
+    q = _rand(gen, rows, heads, hd, dtype=qt)
+    k, v = (_rand(gen, n, kvh, hd, dtype=kt) for _ in range(2))
+    want, tol = attend(q, k, v, [n - rows + 1 + r for r in range(rows)], qt == torch.float16, kt == torch.float16)
+    v[1500, 0, 5], v[200, 7, 9] = math.inf, math.nan
+    out = torch.empty(q.shape, dtype=qt, device=DEV)
+    ops.prompt_attention(engine, q.to(DEV), k.to(DEV), v.to(DEV), out, 1, n, seq_lens=_i32([n]))
+    got = out.float().cpu()
+    assert (got[:, :4, 5] == math.inf).all() and got[:, 28:, 9].isnan().all()
+    got[:, :4, 5] = want[:, :4, 5].float()
+    got[:, 28:, 9] = want[:, 28:, 9].float()
+    check(got, want, tol + 2.0 ** -20 * want.abs(), types)
+
+
 def test_rising_scores(engine):
     # the maximum moves with every tile: each rescales what came before
     for types, (qt, kt) in sorted(TYPES.items()):
