@@ -1168,7 +1168,14 @@ int prefix_attention_launch(janus_ctx *ctx, const void *q, int q_dt, const void 
     const uint64_t own_tiles = (uint64_t)batch * ((a.G + cols - 1) / cols);
     if (prefix_len) {
         a.prefix_tiles = (uint32_t)(((uint64_t)batch * a.G + cols - 1) / cols);
-        a.prefix_splits = plan_splits(ctx, (uint64_t)a.prefix_tiles * kv_heads, prefix_len, 256);
+        // One workgroup per CU, beside those of the own positions: half the partials of
+        // two per CU (64 requests behind 16384 positions: 78 against 88 us). A part
+        // reads K and V once and writes a row per column, so it has at least two
+        // positions for each column, and 128 for the four wavefronts (16 requests
+        // behind 3000 positions: 15.7 us, with 256 18; 32 behind 4096: 22.6 us with
+        // 256, 26.6 with 128).
+        const uint32_t held = (uint32_t)std::min<uint64_t>((uint64_t)batch * a.G, cols);
+        a.prefix_splits = plan_splits(ctx, 2ull * a.prefix_tiles * kv_heads, prefix_len, std::max(128u, 2 * held));
     }
     const uint64_t tasks = plan_own(ctx, a, own_tiles, own_tiles, std::min(max_len, max_seq));
     a.slots = a.prefix_splits + a.splits > 1 ? a.prefix_splits + a.splits : 0;
