@@ -6,6 +6,14 @@
 //   z_i = y_i c_i - y_{i + D/2} s_i,  z_{i + D/2} = y_i s_i + y_{i + D/2} c_i
 // with (c_i, s_i) = table[p][i]. Query heads go to q_out, key heads and the
 // untouched value heads to the row's cache row.
+//
+// Bound by HBM: every value is read and written once. A head is held by the lanes
+// that load it, 16 bytes of either half each, so the norm is a sum over 4 to 32
+// lanes and the turn stays in a lane. Outputs are stored past the caches: 8192
+// binary16 rows of a 32/8/128 product (202 MB) take 38.8 us (5.2 TB/s; a copy
+// reaches 4.7), 47 with ordinary stores; followed by the attention that reads
+// them, both take the same. Four heads of a row per lane group (the table read
+// once for them) took 41 us, and 49.5 with ordinary stores.
 #include "internal.h"
 
 namespace janus {
@@ -19,7 +27,6 @@ struct HeadArgs {
     void *q_out, *kc, *vc;
     const int32_t *row_base, *positions;
     uint32_t rows, heads, kv_heads, hd, position, max_seq;
-    uint32_t parts;                          // groups of a row
     float eps;
 };
 
@@ -59,77 +66,64 @@ template <typename T, int E> __device__ __forceinline__ void store_e(T *p, const
         vec v;
 #pragma unroll
         for (int j = 0; j < N; ++j) v[j] = (T)x[i + j];
-        *(vec *)(p + i) = v;
+        __builtin_nontemporal_store(v, (vec *)(p + i));
     }
 }
 
 // D / 2 / E lanes share a head: each holds E values of the first half and the
-// E values that they turn with. A lane group takes up to U heads of one row,
-// `parts` apart, and loads the row's (cos, sin) once for them.
-template <typename IN, typename OUT, typename KV, int D, int E, int U>
+// E values that they turn with.
+template <typename IN, typename OUT, typename KV, int D, int E>
 __global__ __launch_bounds__(256) void head_kernel(HeadArgs a) {
     constexpr uint32_t L = D / 2 / E;
     const uint32_t units = a.heads + 2 * a.kv_heads;
-    const uint64_t grp = ((uint64_t)blockIdx.x * 256u + threadIdx.x) / L;
-    const uint32_t row = (uint32_t)(grp / a.parts), part = (uint32_t)(grp % a.parts), at = threadIdx.x % L * E;
+    const uint32_t unit = (uint32_t)(((uint64_t)blockIdx.x * 256u + threadIdx.x) / L), at = threadIdx.x % L * E;
+    const uint32_t row = unit / units, h = unit % units;
     if (row >= a.rows) return;
-    float x0[U][E], x1[U][E];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const uint32_t h = part + u * a.parts;
-        if (h >= units) break;
-        const IN *src = h < a.heads ? (const IN *)a.q + (size_t)row * a.q_stride + (size_t)h * D
-                        : h < a.heads + a.kv_heads
-                            ? (const IN *)a.k + (size_t)row * a.k_stride + (size_t)(h - a.heads) * D
-                            : (const IN *)a.v + (size_t)row * a.v_stride + (size_t)(h - a.heads - a.kv_heads) * D;
-        load_e<IN, E>(src + at, x0[u]);
-        load_e<IN, E>(src + D / 2 + at, x1[u]);
-    }
+    const bool is_q = h < a.heads, is_k = !is_q && h < a.heads + a.kv_heads;
+    const uint32_t kh = h - a.heads - (is_k ? 0u : a.kv_heads);
+    const IN *src = is_q   ? (const IN *)a.q + (size_t)row * a.q_stride + (size_t)h * D
+                    : is_k ? (const IN *)a.k + (size_t)row * a.k_stride + (size_t)kh * D
+                           : (const IN *)a.v + (size_t)row * a.v_stride + (size_t)kh * D;
+    float x0[E], x1[E];
+    load_e<IN, E>(src + at, x0);
+    load_e<IN, E>(src + D / 2 + at, x1);
     const Place pl = place_of(a, row);
-    float cs[2 * E];
-    load_e<float, 2 * E>(a.table + ((size_t)pl.pos * (D / 2) + at) * 2, cs);
+    const float *gamma = is_q ? a.q_gamma : is_k ? a.k_gamma : nullptr;
+    if (gamma) {
+        float g0[E], g1[E], s = 0.0f;
+        load_e<float, E>(gamma + at, g0);
+        load_e<float, E>(gamma + D / 2 + at, g1);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const uint32_t h = part + u * a.parts;
-        if (h >= units) break;
-        const bool is_q = h < a.heads, is_k = !is_q && h < a.heads + a.kv_heads;
-        const float *gamma = is_q ? a.q_gamma : is_k ? a.k_gamma : nullptr;
-        if (gamma) {
-            float s = 0.0f;
+        for (int i = 0; i < E; ++i) s = fmaf(x0[i], x0[i], fmaf(x1[i], x1[i], s));
 #pragma unroll
-            for (int i = 0; i < E; ++i) s = fmaf(x0[u][i], x0[u][i], fmaf(x1[u][i], x1[u][i], s));
+        for (int o = L / 2; o > 0; o >>= 1) s += shfl_xor(s, o);
+        const float r = 1.0f / sqrtf(s * (1.0f / D) + a.eps);
 #pragma unroll
-            for (int o = L / 2; o > 0; o >>= 1) s += shfl_xor(s, o);
-            const float r = 1.0f / sqrtf(s * (1.0f / D) + a.eps);
-            float g0[E], g1[E];
-            load_e<float, E>(gamma + at, g0);
-            load_e<float, E>(gamma + D / 2 + at, g1);
-#pragma unroll
-            for (int i = 0; i < E; ++i) {
-                x0[u][i] = x0[u][i] * r * g0[i];
-                x1[u][i] = x1[u][i] * r * g1[i];
-            }
+        for (int i = 0; i < E; ++i) {
+            x0[i] = x0[i] * r * g0[i];
+            x1[i] = x1[i] * r * g1[i];
         }
-        if (is_q || is_k) {
+    }
+    if (is_q || is_k) {
+        float cs[2 * E];
+        load_e<float, 2 * E>(a.table + ((size_t)pl.pos * (D / 2) + at) * 2, cs);
 #pragma unroll
-            for (int i = 0; i < E; ++i) {
-                const float p = x0[u][i], n = x1[u][i], c = cs[2 * i], s = cs[2 * i + 1];
-                x0[u][i] = p * c - n * s;
-                x1[u][i] = p * s + n * c;
-            }
+        for (int i = 0; i < E; ++i) {
+            const float p = x0[i], n = x1[i], c = cs[2 * i], s = cs[2 * i + 1];
+            x0[i] = p * c - n * s;
+            x1[i] = p * s + n * c;
         }
-        if (is_q) {
-            OUT *o = (OUT *)a.q_out + ((size_t)row * a.heads + h) * D + at;
-            if (pl.rotates) {
-                store_e<OUT, E>(o, x0[u]);
-                store_e<OUT, E>(o + D / 2, x1[u]);
-            }
-        } else if (pl.appends) {
-            const uint32_t kh = h - a.heads - (is_k ? 0u : a.kv_heads);
-            KV *o = (KV *)(is_k ? a.kc : a.vc) + (pl.cache_row * a.kv_heads + kh) * D + at;
-            store_e<KV, E>(o, x0[u]);
-            store_e<KV, E>(o + D / 2, x1[u]);
+    }
+    if (is_q) {
+        OUT *o = (OUT *)a.q_out + ((size_t)row * a.heads + h) * D + at;
+        if (pl.rotates) {
+            store_e<OUT, E>(o, x0);
+            store_e<OUT, E>(o + D / 2, x1);
         }
+    } else if (pl.appends) {
+        KV *o = (KV *)(is_k ? a.kc : a.vc) + (pl.cache_row * a.kv_heads + kh) * D + at;
+        store_e<KV, E>(o, x0);
+        store_e<KV, E>(o + D / 2, x1);
     }
 }
 
@@ -185,17 +179,10 @@ __global__ __launch_bounds__(256) void head_any_kernel(HeadArgs a) {
 }
 
 template <typename IN, typename OUT, typename KV, int D>
-void launch_dim(janus_ctx *ctx, HeadArgs a) {
-    // 16 bytes of a binary16 half, or of a binary32 one
-    constexpr int E = sizeof(IN) == 2 ? 8 : 4;
-    constexpr uint32_t L = D / 2 / E;
-    const uint32_t units = a.heads + 2 * a.kv_heads;
-    // one head per lane group while that leaves CUs idle, then four
-    const bool many = (uint64_t)a.rows * units * L >= (uint64_t)ctx->num_cus * 4096u;
-    a.parts = many ? (units + 3) / 4 : units;
-    const uint32_t grid = (uint32_t)(((uint64_t)a.rows * a.parts * L + 255) / 256);
-    if (many) hipLaunchKernelGGL((head_kernel<IN, OUT, KV, D, E, 4>), dim3(grid), dim3(256), 0, ctx->stream, a);
-    else hipLaunchKernelGGL((head_kernel<IN, OUT, KV, D, E, 1>), dim3(grid), dim3(256), 0, ctx->stream, a);
+void launch_dim(janus_ctx *ctx, const HeadArgs &a) {
+    constexpr int E = 16 / sizeof(IN);
+    const uint64_t lanes = (uint64_t)a.rows * (a.heads + 2 * a.kv_heads) * (D / 2 / E);
+    hipLaunchKernelGGL((head_kernel<IN, OUT, KV, D, E>), dim3((uint32_t)((lanes + 255) / 256)), dim3(256), 0, ctx->stream, a);
 }
 
 template <typename IN, typename OUT, typename KV>
@@ -227,7 +214,7 @@ int qk_norm_rope_launch(janus_ctx *ctx, const void *q, const void *k, const void
                         uint32_t heads, uint32_t kv_heads, uint32_t hd, uint32_t position, uint32_t max_seq,
                         const int32_t *row_base, const int32_t *positions) {
     const HeadArgs a{q, k, v, q_stride, k_stride, v_stride, q_gamma, k_gamma, table, q_out, kc, vc,
-                     row_base, positions, rows, heads, kv_heads, hd, position, max_seq, 0, eps};
+                     row_base, positions, rows, heads, kv_heads, hd, position, max_seq, eps};
     if (in_dt == JANUS_DT_F16) {
         if (out_dt == JANUS_DT_F16) launch_kv<_Float16, _Float16>(ctx, a, kv_dt);
         else launch_kv<_Float16, float>(ctx, a, kv_dt);
