@@ -39,10 +39,6 @@ typedef float pf4 __attribute__((ext_vector_type(4)));
 typedef float pf16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) ps4 *lds4;
 
-// Columns per workgroup: 128 through shared tiles, 64 where every wavefront reads
-// its own positions (binary32 caches).
-constexpr uint32_t cols_of(bool kv_f16) { return kv_f16 ? 128u : 64u; }
-
 struct PackedArgs {
     const void *q;            // [rows][heads][D]
     const void *kc, *vc;      // [cache rows][kv_heads][D]
@@ -53,6 +49,7 @@ struct PackedArgs {
     const int32_t *row_base;  // null: s * max_seq
     const int32_t *seq_lens;  // null: seq_len, or as many as the sequence has rows
     uint32_t rows, nseq, heads, kv_heads, G;
+    uint32_t cols;            // columns per workgroup: 16 to 128, a power of two
     uint32_t max_seq;
     int64_t seq_len;          // < 0: the rows
     uint32_t splits;          // most parts of a tile's positions (1: never split)
@@ -120,24 +117,24 @@ __device__ __forceinline__ void sequence_of(const PackedArgs &a, uint32_t s, Wor
 // the former (six prompts of 33 to 512 rows at 32/32/128: 92 -> 75 us), where a
 // position costs 16 times the matrix time; binary16 caches the latter (24 prompts
 // of 3 to 700 rows at 32/8/128: 94 against 98 us).
-template <uint32_t COLS> __device__ __forceinline__ bool find_task(const PackedArgs &a, uint32_t t, Work &w) {
-    const uint32_t lane = threadIdx.x & 63u;
+__device__ __forceinline__ bool find_task(const PackedArgs &a, uint32_t t, Work &w) {
+    const uint32_t lane = threadIdx.x & 63u, shift = 31u - __builtin_clz(a.cols);
     w.causal = true;
     w.part = 0;
     w.parts = 1;
     w.chunk = 0x80000000u;
     if (!a.q_start && a.splits == 1) {
-        const uint32_t each = (uint32_t)(((uint64_t)(a.rows / a.nseq) * a.G + COLS - 1) / COLS), s = t / each;
+        const uint32_t each = (a.rows / a.nseq * a.G + a.cols - 1) >> shift, s = t / each;
         if (s >= a.nseq) return false;
         sequence_of(a, s, w);
-        w.c0 = (each - 1 - t % each) * COLS;
+        w.c0 = (each - 1 - t % each) << shift;
         return true;
     }
     // a lane per sequence; tiles of it
     Work x;
     auto sequence = [&](uint32_t s0) -> uint32_t {
         sequence_of(a, min(s0 + lane, a.nseq - 1), x);
-        return s0 + lane < a.nseq ? (uint32_t)(((uint64_t)x.n * a.G + COLS - 1) / COLS) : 0u;
+        return s0 + lane < a.nseq ? (x.n * a.G + a.cols - 1) >> shift : 0u;   // n G < 2^25
     };
     auto take = [&](int at, uint32_t tile) {
         auto pick = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane(v, at); };
@@ -145,13 +142,13 @@ template <uint32_t COLS> __device__ __forceinline__ bool find_task(const PackedA
         w.n = pick(x.n);
         w.len = pick(x.len);
         w.kv_row = pick((uint32_t)x.kv_row);   // below 2^31
-        w.c0 = tile * COLS;
+        w.c0 = tile << shift;
         return true;
     };
     uint32_t mine = sequence(0);
     if (a.longest) {   // at most 16 sequences, not split
         // levels: a tile's distance from position 0 in tiles; lane j counts those from lo + j step on
-        const uint32_t before = x.len > x.n ? (uint32_t)min((uint64_t)(x.len - x.n) * a.G / COLS, (uint64_t)1 << 30) : 0u;
+        const uint32_t before = x.len > x.n ? (uint32_t)min((uint64_t)(x.len - x.n) * a.G >> shift, (uint64_t)1 << 30) : 0u;
         const uint32_t top = before + mine;
         uint32_t most = mine ? top : 0u;
 #pragma unroll
@@ -958,7 +955,6 @@ __device__ __forceinline__ void wide_tile(const PackedArgs &a, const Work &w, ui
 template <typename Q, typename KV, int D>
 __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedArgs a) {
     constexpr bool H = sizeof(KV) == 2;
-    constexpr uint32_t COLS = cols_of(H);
     extern __shared__ __align__(16) unsigned char smem[];
     // neighbouring workgroups take the KV heads, so that with 8 of them each XCD
     // keeps the K and V of one head in its L2
@@ -986,19 +982,19 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedArgs a) {
         w.slot = w.part;
         w.row0 = 0;
         w.n = a.rows;
-        w.c0 = id / a.prefix_splits * COLS;
+        w.c0 = id / a.prefix_splits * a.cols;
         w.kv_row = a.prefix_row;
         w.len = a.prefix_len;
         w.causal = false;
     } else {
-        if (!find_task<COLS>(a, id, w)) return;
+        if (!find_task(a, id, w)) return;
         w.slot = a.prefix_splits + w.part;
     }
-    const uint32_t ncols = w.n * a.G;   // n * G <= rows * heads < 2^32
-    const uint32_t end_all = seen_of(w, min(w.c0 + COLS - 1, ncols - 1) / a.G);
+    const uint32_t ncols = min(w.n * a.G, w.c0 + a.cols);   // up to the tile's last column; n G < 2^25
+    const uint32_t end_all = seen_of(w, (ncols - 1) / a.G);
     const uint32_t p0 = min(w.part * w.chunk, end_all), p1 = min(p0 + w.chunk, end_all);
     if (!shared && a.slots && w.part + 1 == w.parts && w.parts < a.splits) {   // parts that there are none of
-        const uint32_t none = a.splits - w.parts, cols = min(COLS, ncols - w.c0);
+        const uint32_t none = a.splits - w.parts, cols = ncols - w.c0;
         for (uint32_t x = threadIdx.x; x < cols * none; x += 256) {
             const uint32_t c = w.c0 + x / none, row = c / a.G;
             const size_t qat = (size_t)(w.row0 + row) * a.heads + kvh * a.G + (c - row * a.G);
@@ -1097,16 +1093,51 @@ uint32_t plan_splits(const janus_ctx *ctx, uint64_t tiles, uint32_t max_len, uin
     return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(want, (max_len + least - 1) / least));
 }
 
+// Whether q and P are in two parts (binary32 rows on a binary16 cache).
+bool two_parts(int q_dt, int kv_dt) { return q_dt != kv_dt; }
+
 // The parts of a request's own positions, where `likely` tiles are expected and
-// there are at most `tiles`: returns the tasks per KV head.
-uint64_t plan_own(const janus_ctx *ctx, PackedArgs &a, uint64_t likely, uint64_t tiles, uint32_t max_len) {
-    const uint32_t want = plan_splits(ctx, likely * a.kv_heads, max_len, 128);
+// there are at most `tiles`: returns the tasks per KV head. Parts cost a second
+// launch (about 5 us) unless the results are joined anyway, so there are none below
+// about twice what a workgroup passes over in that time: 640 positions in binary16,
+// 384 where scores cost more (one prompt of 512 rows at 32/8/128 in binary16: 16 us in
+// one part, 25 in two).
+uint64_t plan_own(const janus_ctx *ctx, PackedArgs &a, int q_dt, int kv_dt, uint64_t likely, uint64_t tiles,
+                  uint32_t max_len) {
+    const uint32_t whole = a.prefix_splits ? 0 : q_dt == JANUS_DT_F16 || (two_parts(q_dt, kv_dt) && a.cols == 16) ? 640 : 384;
+    const uint32_t want = max_len < whole ? 1 : plan_splits(ctx, likely * a.kv_heads, max_len, q_dt == JANUS_DT_F16 && a.cols > 32 && !a.prefix_splits ? 256 : 128);
     a.splits = 1;
     if (want == 1) return tiles;
     // of several requests one may take four times the mean (the workspace is sized for that)
     a.splits = a.nseq == 1 ? want : std::min(4 * want, std::max(2u, (max_len + 127) / 128));
     a.target = std::max(1u, 2u * (uint32_t)ctx->num_cus / a.kv_heads);
     return tiles + a.target + 1;   // sum of tiles * ceil(len / chunk) <= target + tiles
+}
+
+// Columns per workgroup for `groups` runs of `columns` columns each on up to max_len
+// positions (of the caches' capacity, where the caller gave no hint). Many columns
+// share the K and V that a workgroup reads and few fill the CUs without splitting the
+// positions. At 32/8/128, us with 128 (or 64 for binary32 caches), 64, 32 and 16:
+//   binary16              one prompt of 256: 15.7 14.8 19.1 10.7, 1024: 43 28 39 57
+//   two parts             256: 19.3 17.8 19.5 12.5, 1024: 58 44 51 63
+//   binary32 caches       256: 25.9 - 28.6 16.0, 1024: 119 - 106 116
+//   16 behind a prefix of 500, two parts: 12.9 12.9 13.1 11.3; binary32 20 - 15.8 11.6
+//   64 behind a prefix of 4000, two parts: 26 30 40 33; binary32 59 - 57 61
+uint32_t plan_cols(const janus_ctx *ctx, const PackedArgs &a, int q_dt, int kv_dt, uint64_t groups, uint64_t columns,
+                   uint32_t max_len) {
+    const uint64_t cus = (uint64_t)ctx->num_cus;
+    auto tiles = [&](uint32_t cols) { return groups * ((columns + cols - 1) / cols) * a.kv_heads; };
+    if (kv_dt != JANUS_DT_F16) {
+        if (a.prefix_len) return columns * a.kv_heads >= 32 * cus ? 64 : columns * a.kv_heads >= 4 * cus ? 32 : 16;
+        if (tiles(64) >= (max_len <= 128 ? cus * 3 / 4 : 3 * cus)) return 64;
+        return tiles(32) >= 2 * cus ? 32 : 16;
+    }
+    if (two_parts(q_dt, kv_dt)) {
+        if (columns <= 32) return 16;
+        if (a.prefix_len ? max_len <= 2048 && columns * a.kv_heads <= 4 * cus : max_len <= 512 && tiles(16) <= (max_len <= 256 ? 2 : 4) * cus) return 16;
+    }
+    if (tiles(128) >= 2 * cus) return 128;
+    return max_len <= (a.prefix_len && !two_parts(q_dt, kv_dt) ? 2048 : 1024) ? 64 : 128;
 }
 
 int run(janus_ctx *ctx, PackedArgs a, int q_dt, int kv_dt, uint32_t hd, uint64_t own_tasks) {
@@ -1141,12 +1172,13 @@ int prompt_attention_launch(janus_ctx *ctx, const void *q, int q_dt, const void 
     a.max_seq = max_seq;
     a.seq_len = -1;
     a.scale2 = scale * 1.4426950408889634f;
+    const uint64_t mean = (uint64_t)((rows + nseq - 1) / nseq) * a.G;   // columns of a sequence
+    const uint32_t cols = a.cols = plan_cols(ctx, a, q_dt, kv_dt, nseq, mean, std::min(max_len, max_seq));
     // at most so many tiles: every sequence's last one may be part empty
-    const uint32_t cols = cols_of(kv_dt == JANUS_DT_F16);
     const uint64_t tiles = (uint64_t)rows * a.G / cols + nseq;
     // about as many as sequences of equal rows have
-    const uint64_t likely = (uint64_t)nseq * (((rows + nseq - 1) / nseq * (uint64_t)a.G + cols - 1) / cols);
-    const uint64_t tasks = plan_own(ctx, a, likely, tiles, std::min(max_len, max_seq));
+    const uint64_t likely = (uint64_t)nseq * ((mean + cols - 1) / cols);
+    const uint64_t tasks = plan_own(ctx, a, q_dt, kv_dt, likely, tiles, std::min(max_len, max_seq));
     a.slots = a.splits > 1 ? a.splits : 0;
     a.longest = kv_dt != JANUS_DT_F16 && a.splits == 1 && nseq > 1 && nseq <= 16 && likely * kv_heads > 2u * (uint32_t)ctx->num_cus;
     return run(ctx, a, q_dt, kv_dt, hd, tasks);
@@ -1164,20 +1196,20 @@ int prefix_attention_launch(janus_ctx *ctx, const void *q, int q_dt, const void 
     a.seq_len = seq_len;
     a.prefix_row = prefix_row; a.prefix_len = prefix_len;
     a.scale2 = scale * 1.4426950408889634f;
-    const uint32_t cols = cols_of(kv_dt == JANUS_DT_F16);
+    const uint32_t cols = a.cols = plan_cols(ctx, a, q_dt, kv_dt, 1, (uint64_t)batch * a.G, std::max(prefix_len, std::min(max_len, max_seq)));
     const uint64_t own_tiles = (uint64_t)batch * ((a.G + cols - 1) / cols);
     if (prefix_len) {
         a.prefix_tiles = (uint32_t)(((uint64_t)batch * a.G + cols - 1) / cols);
         // One workgroup per CU, beside those of the own positions: half the partials of
-        // two per CU (64 requests behind 16384 positions: 78 against 88 us). A part
-        // reads K and V once and writes a row per column, so it has at least two
-        // positions for each column, and 128 for the four wavefronts (16 requests
-        // behind 3000 positions: 15.7 us, with 256 18; 32 behind 4096: 22.6 us with
-        // 256, 26.6 with 128).
+        // two per CU (64 requests behind 16384 positions: 78 against 88 us; 32 behind
+        // 8192 with one own: 27 against 34). A part reads K and V once and writes a row
+        // per column, so it has at least two positions for each column, and 128 for the
+        // four wavefronts (16 requests behind 3000 positions: 15.7 us, with 256 18; 32
+        // behind 4096: 22.6 us with 256, 26.6 with 128).
         const uint32_t held = (uint32_t)std::min<uint64_t>((uint64_t)batch * a.G, cols);
         a.prefix_splits = plan_splits(ctx, 2ull * a.prefix_tiles * kv_heads, prefix_len, std::max(128u, 2 * held));
     }
-    const uint64_t tasks = plan_own(ctx, a, own_tiles, own_tiles, std::min(max_len, max_seq));
+    const uint64_t tasks = plan_own(ctx, a, q_dt, kv_dt, own_tiles, own_tiles, std::min(max_len, max_seq));
     a.slots = a.prefix_splits + a.splits > 1 ? a.prefix_splits + a.splits : 0;
     return run(ctx, a, q_dt, kv_dt, hd, tasks);
 }
