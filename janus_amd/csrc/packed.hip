@@ -83,6 +83,25 @@ __device__ __forceinline__ float swap16(float v) {   // value of lane ^ 16
     return __uint_as_float((__lane_id() & 16) ? p[0] : p[1]);
 }
 
+// Sum over the lanes up to this one, and the maximum over all, without LDS traffic.
+__device__ __forceinline__ uint32_t scan_dpp(uint32_t v) {
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);   // row_shr:1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);   // row_bcast:15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);   // row_bcast:31 into rows 2 and 3
+    return v;
+}
+__device__ __forceinline__ uint32_t max_dpp(uint32_t v) {
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, false));   // row_ror:8, 4, 2, 1
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x122, 0xf, 0xf, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xf, 0xf, false));
+    return max(max((uint32_t)__builtin_amdgcn_readlane(v, 0), (uint32_t)__builtin_amdgcn_readlane(v, 16)),
+               max((uint32_t)__builtin_amdgcn_readlane(v, 32), (uint32_t)__builtin_amdgcn_readlane(v, 48)));
+}
+
 // Rows [first, first + n), first cache row and positions of sequence s. Whatever
 // the tables hold, rows stay inside [0, rows) and positions within [0, max_seq].
 __device__ __forceinline__ void sequence_of(const PackedArgs &a, uint32_t s, Work &w) {
@@ -150,10 +169,7 @@ __device__ __forceinline__ bool find_task(const PackedArgs &a, uint32_t t, Work 
         // levels: a tile's distance from position 0 in tiles; lane j counts those from lo + j step on
         const uint32_t before = x.len > x.n ? (uint32_t)min((uint64_t)(x.len - x.n) * a.G >> shift, (uint64_t)1 << 30) : 0u;
         const uint32_t top = before + mine;
-        uint32_t most = mine ? top : 0u;
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) most = max(most, (uint32_t)shfl_xor((int)most, o));
-        most = __builtin_amdgcn_readfirstlane(most);
+        const uint32_t most = max_dpp(mine ? top : 0u);
         uint32_t lo = 0, above = 0;   // level of task t, tiles above it
         for (uint32_t step = 1u << max(0, 26 - (int)__builtin_clz(most | 1u));; step = step > 64 ? step >> 6 : 1) {
             const uint32_t level = lo + lane * step;
@@ -181,20 +197,14 @@ __device__ __forceinline__ bool find_task(const PackedArgs &a, uint32_t t, Work 
             longest = max(longest, tiles ? x.len : 0u);
         }
         total = wave_sum_dpp(total);
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) longest = max(longest, (uint32_t)shfl_xor((int)longest, o));
+        longest = max_dpp(longest);
         const uint32_t even = (uint32_t)fminf(total / (float)a.target, 1e9f) + 1, least = (longest + a.splits - 1) / a.splits;
         w.chunk = __builtin_amdgcn_readfirstlane((max(max(even, least), 128u) + 63u) / 64u * 64u);
         if (a.nseq > 64) mine = sequence(0);
     }
     for (uint32_t s0 = 0;;) {
         const uint32_t parts = max((x.len + w.chunk - 1) / w.chunk, 1u), tasks = mine * parts;
-        uint32_t upto = tasks;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t v = __shfl_up(upto, o, 64);
-            if ((int)lane >= o) upto += v;
-        }
+        const uint32_t upto = scan_dpp(tasks);
         const uint64_t hit = __ballot(t < upto);
         if (hit) {
             const int at = __ffsll((unsigned long long)hit) - 1;
@@ -1098,14 +1108,17 @@ bool two_parts(int q_dt, int kv_dt) { return q_dt != kv_dt; }
 
 // The parts of a request's own positions, where `likely` tiles are expected and
 // there are at most `tiles`: returns the tasks per KV head. Parts cost a second
-// launch (about 5 us) unless the results are joined anyway, so there are none below
-// about twice what a workgroup passes over in that time: 640 positions in binary16,
-// 384 where scores cost more (one prompt of 512 rows at 32/8/128 in binary16: 16 us in
-// one part, 25 in two).
+// launch (about 5 us) unless the results are joined anyway, and where there is a tile
+// for nearly every CU a second workgroup on each gains only a quarter to a third. So
+// contexts stay whole below some lengths, by the time that a position takes (one
+// prompt of 512 rows at 32/8/128 in binary16: 16 us in one part, 25 in two).
 uint64_t plan_own(const janus_ctx *ctx, PackedArgs &a, int q_dt, int kv_dt, uint64_t likely, uint64_t tiles,
                   uint32_t max_len) {
-    const uint32_t whole = a.prefix_splits ? 0 : q_dt == JANUS_DT_F16 || (two_parts(q_dt, kv_dt) && a.cols == 16) ? 640 : 384;
-    const uint32_t want = max_len < whole ? 1 : plan_splits(ctx, likely * a.kv_heads, max_len, q_dt == JANUS_DT_F16 && a.cols > 32 && !a.prefix_splits ? 256 : 128);
+    const bool cheap = q_dt == JANUS_DT_F16 || (two_parts(q_dt, kv_dt) && a.cols == 16);
+    const bool busy = 3 * likely * a.kv_heads >= 2ull * (uint32_t)ctx->num_cus;
+    const uint32_t whole = a.prefix_splits ? 0 : cheap ? (busy ? 1280 : 640) : busy ? 768 : 384;
+    const uint32_t least = q_dt == JANUS_DT_F16 && a.cols > 32 && !a.prefix_splits ? 256 : 128;
+    const uint32_t want = max_len < whole ? 1 : plan_splits(ctx, likely * a.kv_heads, max_len, least);
     a.splits = 1;
     if (want == 1) return tiles;
     // of several requests one may take four times the mean (the workspace is sized for that)
@@ -1123,20 +1136,22 @@ uint64_t plan_own(const janus_ctx *ctx, PackedArgs &a, int q_dt, int kv_dt, uint
 //   binary32 caches       256: 25.9 - 28.6 16.0, 1024: 119 - 106 116
 //   16 behind a prefix of 500, two parts: 12.9 12.9 13.1 11.3; binary32 20 - 15.8 11.6
 //   64 behind a prefix of 4000, two parts: 26 30 40 33; binary32 59 - 57 61
+//   11 prompts of 12 to 244: binary16 15.5 19.5 28 36, two parts 21 25 33 43,
+//     binary32 43 - 50 57
 uint32_t plan_cols(const janus_ctx *ctx, const PackedArgs &a, int q_dt, int kv_dt, uint64_t groups, uint64_t columns,
                    uint32_t max_len) {
     const uint64_t cus = (uint64_t)ctx->num_cus;
     auto tiles = [&](uint32_t cols) { return groups * ((columns + cols - 1) / cols) * a.kv_heads; };
     if (kv_dt != JANUS_DT_F16) {
         if (a.prefix_len) return columns * a.kv_heads >= 32 * cus ? 64 : columns * a.kv_heads >= 4 * cus ? 32 : 16;
-        if (tiles(64) >= (max_len <= 128 ? cus * 3 / 4 : 3 * cus)) return 64;
+        if (tiles(64) >= (max_len <= 128 ? cus * 3 / 4 : max_len <= 256 ? cus * 7 / 4 : 3 * cus)) return 64;
         return tiles(32) >= 2 * cus ? 32 : 16;
     }
     if (two_parts(q_dt, kv_dt)) {
         if (columns <= 32) return 16;
         if (a.prefix_len ? max_len <= 2048 && columns * a.kv_heads <= 4 * cus : max_len <= 512 && tiles(16) <= (max_len <= 256 ? 2 : 4) * cus) return 16;
     }
-    if (tiles(128) >= 2 * cus) return 128;
+    if (tiles(128) >= cus * 3 / 4) return 128;
     return max_len <= (a.prefix_len && !two_parts(q_dt, kv_dt) ? 2048 : 1024) ? 64 : 128;
 }
 
