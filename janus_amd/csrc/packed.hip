@@ -83,6 +83,14 @@ __device__ __forceinline__ float swap16(float v) {   // value of lane ^ 16
     return __uint_as_float((__lane_id() & 16) ? p[0] : p[1]);
 }
 
+// The kernel's arguments, read where they are used: held from the start they fill the
+// scalar registers, and what spills takes vector registers and scratch.
+__device__ __forceinline__ const PackedArgs &late_args() {
+    auto at = (const PackedArgs __attribute__((address_space(4))) *)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(at));
+    return *(const PackedArgs *)at;
+}
+
 // Sum over the lanes up to this one, and the maximum over all, without LDS traffic.
 __device__ __forceinline__ uint32_t scan_dpp(uint32_t v) {
     v += __builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);   // row_shr:1, 2, 4, 8
@@ -585,6 +593,7 @@ __device__ __forceinline__ void few_columns(const PackedArgs &a, const Work &w, 
     }
 
     // join the wavefronts of a group
+    const PackedArgs &z = late_args();
     constexpr uint32_t C = 16 * NT, OS = D + 4;    // padded: 16 columns meet 16 bank groups
     float *oo = (float *)smem;                     // [wave][column][OS], over the V tiles
     float2 *ml = (float2 *)(smem + 4 * 32 * OS * 4);   // [wave][column]
@@ -608,8 +617,8 @@ __device__ __forceinline__ void few_columns(const PackedArgs &a, const Work &w, 
         }
 #pragma unroll
         for (uint32_t x = 0; x < 4; ++x)
-            if (x < pw) lt = fmaf(all[x].y, all[x].x == M ? 1.0f : __builtin_amdgcn_exp2f((all[x].x - M) * a.scale2), lt);
-        const float f = m[n] == M ? 1.0f : __builtin_amdgcn_exp2f((m[n] - M) * a.scale2);
+            if (x < pw) lt = fmaf(all[x].y, all[x].x == M ? 1.0f : __builtin_amdgcn_exp2f((all[x].x - M) * z.scale2), lt);
+        const float f = m[n] == M ? 1.0f : __builtin_amdgcn_exp2f((m[n] - M) * z.scale2);
         float *to = oo + (wave * C + 16 * n + i) * OS;
         if constexpr (H) {
 #pragma unroll
@@ -633,21 +642,21 @@ __device__ __forceinline__ void few_columns(const PackedArgs &a, const Work &w, 
         const float *from = oo + (size_t)(group * C + x % C) * OS + dim;   // wavefront `group`, then every cw-th
         jf4 sum = *(const jf4 *)from;
         for (uint32_t y = 1; y < pw; ++y) {
-            const jf4 z = *(const jf4 *)(from + y * cw * C * OS);
+            const jf4 more = *(const jf4 *)(from + y * cw * C * OS);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sum[e] += z[e];
+            for (int e = 0; e < 4; ++e) sum[e] += more[e];
         }
         const size_t to = __float_as_uint(f.w);
-        if (a.slots) {
-            const size_t part = to * a.slots + w.slot;
-            if (dim == 0) *(float2 *)(a.part_ml + 2 * part) = make_float2(f.x, f.y);
-            *(jf4 *)(a.part + part * D + dim) = sum;
+        if (z.slots) {
+            const size_t part = to * z.slots + w.slot;
+            if (dim == 0) *(float2 *)(z.part_ml + 2 * part) = make_float2(f.x, f.y);
+            *(jf4 *)(z.part + part * D + dim) = sum;
         } else {
             typedef Q q4 __attribute__((ext_vector_type(4)));
             q4 y;
 #pragma unroll
             for (int e = 0; e < 4; ++e) y[e] = (Q)(sum[e] * f.z);
-            *(q4 *)((Q *)a.out + to * D + dim) = y;
+            *(q4 *)((Q *)z.out + to * D + dim) = y;
         }
     }
 }
@@ -933,13 +942,14 @@ __device__ __forceinline__ void wide_tile(const PackedArgs &a, const Work &w, ui
         return;
     }
     if (wc0 + col >= ncols) return;
-    if (a.slots) {
-        const size_t at = qat * a.slots + w.slot;
+    const PackedArgs &z = late_args();
+    if (z.slots) {
+        const size_t at = qat * z.slots + w.slot;
         // what the rounding of c shifted, since the parts are joined by m
         const float back = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(R::BIAS - fmaf(m, sc2, c2));
-        if (h == 0) *(float2 *)(a.part_ml + 2 * at) = make_float2(m / qs, l * back);
+        if (h == 0) *(float2 *)(z.part_ml + 2 * at) = make_float2(m / qs, l * back);
         if (p0 >= p1) return;   // the join reads no output of a part without positions
-        float *to = a.part + at * D;
+        float *to = z.part + at * D;
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -948,7 +958,7 @@ __device__ __forceinline__ void wide_tile(const PackedArgs &a, const Work &w, ui
         return;
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;   // a row that sees nothing is 0
-    Q *to = (Q *)a.out + qat * D;
+    Q *to = (Q *)z.out + qat * D;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
