@@ -271,7 +271,7 @@ int janus_qk_norm_rope(janus_ctx *ctx, const void *q, const void *k, const void 
  * An infinity or NaN where a row does not look does not reach it. max_len_hint
  * (0: max_seq_len) is about the longest len_s: it plans the split, whatever the
  * lengths turn out to be. head_dim 64 or 128; q, caches and out 16-byte
- * aligned; scale <= 0 selects 1/sqrt(head_dim). */
+ * aligned; out may be q. scale <= 0 selects 1/sqrt(head_dim). */
 int janus_prompt_attention(janus_ctx *ctx, const void *q, int dtype, const void *k_cache, const void *v_cache,
                            int kv_dtype, void *out, uint32_t rows, uint32_t nseq, uint32_t heads, uint32_t kv_heads,
                            uint32_t head_dim, uint32_t max_seq_len, const int32_t *d_q_start,

@@ -6,26 +6,35 @@
 // matrix product: column c of a sequence of n rows is query head c % G of its
 // row c / G (G heads per KV head), so few rows of many heads fill a tile as many
 // rows of few heads do, and K and V are read once for all of them. A workgroup
-// takes 128 columns (four wavefronts of 32), passes over the positions in tiles
-// that go through LDS, and keeps the running maximum m, the sum l and the output
-// O^T in registers:
+// takes up to 128 columns, passes over the positions and keeps the running maximum
+// m, the sum l and the output O^T in registers:
 //   S^T = K Q^T (positions x columns), p = 2^(scale log2(e) (s - m)),
 //   l <- l 2^(m_old - m) + sum p,  O^T <- O^T 2^(m_old - m) + V^T P^T.
 // A lane's column is one query, so m, l and the rescale are per lane, and P is
-// the second product's operand as it lies; V's operand is read from LDS with the
-// transposing load in the position order that matches.
-//   binary16 rows and cache: v_mfma_f32_32x32x16_f16, P rounded to binary16 (its
-//     errors average out over the positions and stay below the output's own
-//     rounding);
+// the second product's operand as it lies; V's operand in binary16 is read from LDS
+// with the transposing load in the position order that matches.
+//   binary16 rows and cache: f16 MFMAs, P rounded to binary16 (its errors average
+//     out over the positions and stay below the output's own rounding);
 //   binary32 rows, binary16 cache: q and P in two binary16 parts each (22 bits);
-//   binary32 rows and cache: v_mfma_f32_32x32x2_f32, nothing rounded.
+//   binary32 rows and cache: f32 MFMAs, nothing rounded.
 // m follows the maximum only when that would grow by more than a few powers of
 // two (an exponent bias leaves P room), so most tiles rescale nothing.
+//
+// wide_tile (17 or 33 columns and more on a binary16 cache) shares K and V through
+// LDS; few_columns (the others) gives every wavefront positions of its own.
 //
 // Few columns on a long context: the positions are split over workgroups, each
 // of which writes (m, l) and its output, and a second launch joins them. A
 // shared prefix is a sequence of its own with one row per request and no causal
 // limit; its parts and those of the requests' own positions are joined alike.
+//
+// Measured (32/8/128 heads, binary16 unless named, the launches of a call back to
+// back): a prompt of 8192 rows 557 us, 986 TFLOP/s (a large matrix product reaches
+// 1050); 24 prompts of 3 to 700 rows 79 us (174 MB, 34 GFLOP); the last 512 binary32
+// rows of 8192 on a binary16 cache 145 us (67 GFLOP twice, for the two parts); six
+// prompts of 33 to 512 rows at 32/32/128 in binary32 70 us (4.5 GFLOP; 121 TFLOP/s
+// on long ones); five drafted tokens each of 16 requests 38 us (137 MB); 64 binary32
+// rows behind 16384 positions 70 us (206 MB).
 #include <algorithm>
 
 #include "internal.h"
@@ -135,8 +144,7 @@ __device__ __forceinline__ void sequence_of(const PackedArgs &a, uint32_t s, Wor
 // Splitting (few tiles): the tables give the positions of all tiles, and every part
 // gets as many, so that long and short contexts take equal workgroups (drafted
 // tokens of 16 requests with 200 to 4000 positions: 44 -> 39 us against equal counts
-// of parts). Every
-// workgroup finds the same numbers.
+// of parts). Every workgroup finds the same numbers.
 //
 // With `longest`, the tiles of all sequences go by the position that they reach, the
 // farthest first, so that no long one is begun when the others are done; else the
@@ -1087,9 +1095,13 @@ int launch(janus_ctx *ctx, const PackedArgs &a, uint32_t blocks) {
     // two tiles of K and V, or the join of the wavefronts of few columns
     constexpr size_t tiles = sizeof(KV) == 2 ? 4 * (sizeof(Q) == 2 ? 64 : 32) * D * 2 : 0;
     constexpr size_t lds = std::max<size_t>(tiles, 4 * 32 * ((D + 4) * 4 + 8) + 64 * 16);
-    static const hipError_t attr = hipFuncSetAttribute((const void *)packed_attn_kernel<Q, KV, D>,
-                                                       hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    (void)attr;
+    static std::atomic<uint64_t> asked{0};   // devices on which the kernel may take that much
+    const uint64_t bit = 1ull << (ctx->device & 63);
+    if (!(asked.load(std::memory_order_relaxed) & bit)) {
+        JANUS_HIP_CHECK(ctx, hipFuncSetAttribute((const void *)packed_attn_kernel<Q, KV, D>,
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+        asked.fetch_or(bit, std::memory_order_relaxed);
+    }
     hipLaunchKernelGGL((packed_attn_kernel<Q, KV, D>), dim3(blocks), dim3(256), lds, ctx->stream, a);
     JANUS_LAUNCH_CHECK(ctx);
     if (a.slots) {
@@ -1197,13 +1209,15 @@ int prompt_attention_launch(janus_ctx *ctx, const void *q, int q_dt, const void 
     a.max_seq = max_seq;
     a.seq_len = -1;
     a.scale2 = scale * 1.4426950408889634f;
+    max_len = std::min(max_len, max_seq);
+    if (!seq_lens) max_len = std::min(max_len, q_start ? rows : rows / nseq);
     const uint64_t mean = (uint64_t)((rows + nseq - 1) / nseq) * a.G;   // columns of a sequence
-    const uint32_t cols = a.cols = plan_cols(ctx, a, q_dt, kv_dt, nseq, mean, std::min(max_len, max_seq));
+    const uint32_t cols = a.cols = plan_cols(ctx, a, q_dt, kv_dt, nseq, mean, max_len);
     // at most so many tiles: every sequence's last one may be part empty
     const uint64_t tiles = (uint64_t)rows * a.G / cols + nseq;
     // about as many as sequences of equal rows have
     const uint64_t likely = (uint64_t)nseq * ((mean + cols - 1) / cols);
-    const uint64_t tasks = plan_own(ctx, a, q_dt, kv_dt, likely, tiles, std::min(max_len, max_seq));
+    const uint64_t tasks = plan_own(ctx, a, q_dt, kv_dt, likely, tiles, max_len);
     a.slots = a.splits > 1 ? a.splits : 0;
     a.longest = kv_dt != JANUS_DT_F16 && a.splits == 1 && nseq > 1 && nseq <= 16 && likely * kv_heads > 2u * (uint32_t)ctx->num_cus;
     return run(ctx, a, q_dt, kv_dt, hd, tasks);
