@@ -21,7 +21,8 @@ def _rand(gen, *shape, dtype=torch.float32, sigma=1.0):
     return (torch.randn(*shape, generator=gen) * sigma).to(dtype)
 
 
-def _prompt(engine, types, heads, kvh, hd, seqs, cap=None, seed=0, sigma=1.5, poison=True, behind=0, scale=0.0, hint=0):
+def _prompt(engine, types, heads, kvh, hd, seqs, cap=None, seed=0, sigma=1.5, poison=True, behind=0, scale=0.0, hint=0,
+            device="cpu"):
     """seqs: (rows, length) of each; cache rows that no sequence owns hold NaN and
     infinities. Checks every row and that the rows behind stay as they were."""
     qt, kt = TYPES[types]
@@ -45,11 +46,12 @@ def _prompt(engine, types, heads, kvh, hd, seqs, cap=None, seed=0, sigma=1.5, po
                          row_base=_i32([s * cap for s in slots]), seq_lens=_i32([m for _, m in seqs]),
                          max_len_hint=hint, scale=scale)
     engine.sync()
-    for s, (n, m), i in zip(slots, seqs, starts):
-        want, tol = attend(q[i:i + n], k[s * cap:s * cap + m], v[s * cap:s * cap + m],
-                           [max(0, m - n + 1 + r) for r in range(n)], qt == torch.float16, kt == torch.float16,
-                           scale or None)
-        check(out[i:i + n], want, tol, (types, n, m))
+    with torch.device(device):
+        for s, (n, m), i in zip(slots, seqs, starts):
+            want, tol = attend(q[i:i + n].to(device), k[s * cap:s * cap + m].to(device), v[s * cap:s * cap + m].to(device),
+                               [max(0, m - n + 1 + r) for r in range(n)], qt == torch.float16, kt == torch.float16,
+                               scale or None)
+            check(out[i:i + n], want.cpu(), tol.cpu(), (types, n, m))
     assert (out[rows:] == 7.0).all()
 
 
@@ -220,7 +222,7 @@ def test_infinite_keys(engine):
         check(got, want, tol, types)
 
 
-def _prefix(engine, types, heads, kvh, hd, batch, prefix, lens, cap=None, seed=0, first=3, seq_len=None):
+def _prefix(engine, types, heads, kvh, hd, batch, prefix, lens, cap=None, seed=0, first=3, seq_len=None, device="cpu"):
     qt, kt = TYPES[types]
     gen = torch.Generator().manual_seed(seed)
     cap = cap or max(1, max(lens))
@@ -236,11 +238,13 @@ def _prefix(engine, types, heads, kvh, hd, batch, prefix, lens, cap=None, seed=0
     out = torch.empty(q.shape, dtype=qt, device=DEV)
     ops.prefix_attention(engine, q.to(DEV), kc.to(DEV), vc.to(DEV), out, first, prefix, cap, row_base=_i32(base),
                          seq_lens=_i32(lens) if seq_len is None else None, seq_len=seq_len or 0)
-    for r, (b, n) in enumerate(zip(base, lens)):
-        kk = torch.cat([k[first:first + prefix], k[b:b + n]])
-        vv = torch.cat([v[first:first + prefix], v[b:b + n]])
-        want, tol = attend(q[r:r + 1], kk, vv, [prefix + n], qt == torch.float16, kt == torch.float16)
-        check(out[r:r + 1], want, tol, (types, r, n))
+    q, k, v = (x.to(device) for x in (q, k, v))
+    with torch.device(device):
+        for r, (b, n) in enumerate(zip(base, lens)):
+            kk = torch.cat([k[first:first + prefix], k[b:b + n]])
+            vv = torch.cat([v[first:first + prefix], v[b:b + n]])
+            want, tol = attend(q[r:r + 1], kk, vv, [prefix + n], qt == torch.float16, kt == torch.float16)
+            check(out[r:r + 1], want.cpu(), tol.cpu(), (types, r, n))
 
 
 @pytest.mark.parametrize("types", sorted(TYPES))
@@ -261,6 +265,106 @@ def test_prefix_alone_and_one_length_for_all(engine, types):
     _prefix(engine, types, 8, 2, 64, 4, 300, [21] * 4, cap=32, seq_len=21)
     _prefix(engine, types, 8, 2, 64, 4, 0, [0, 5, 0, 1])
     _prefix(engine, types, 32, 8, 128, 2, 0, [900, 1500])
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+def test_enough_prefix_and_own_workgroups_to_alternate(engine, types):
+    # 64 requests: two rounds of own workgroups, one and more of the prefix's
+    _prefix(engine, types, 32, 8, 128, 64, 8300, [(i * 53) % 150 for i in range(64)], cap=150, device=DEV)
+    _prefix(engine, types, 16, 8, 64, 130, 4200, [(i * 29) % 40 for i in range(130)], cap=40, device=DEV)
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("heads,kvh,rows", [(8, 8, 300), (8, 1, 90), (32, 8, 20)])
+def test_long_contexts_in_tiles_of_every_width(engine, types, heads, kvh, rows):
+    _prompt(engine, types, heads, kvh, 64, [(rows, 1900)], device=DEV)
+    _prompt(engine, types, heads, kvh, 128, [(rows, rows + 700), (1, 650)], device=DEV)
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("nseq", [11, 20])
+def test_many_tiles_of_many_heads(engine, types, nseq):
+    # more tiles than two for each CU: by the position they reach (few sequences on a binary32 cache) or in order
+    seqs = [(128, 128), (5, 9), (0, 0), (100, 127), (2, 1), (128, 100)]
+    _prompt(engine, types, 32, 32, 64, [seqs[i % 6] if i % 7 else (110 + i % 9, 120) for i in range(nseq)], cap=128, device=DEV)
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+def test_split_contexts_of_more_sequences_than_lanes(engine, types):
+    _prompt(engine, types, 4, 1, 64, [((i * 5) % 3, (i * 211) % 1500) for i in range(131)], cap=1500, device=DEV)
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("rows,n", [(1, 1), (3, 2000), (70, 70), (200, 1400)])
+def test_in_place(engine, types, rows, n):
+    qt, kt = TYPES[types]
+    gen = torch.Generator().manual_seed(31)
+    q = _rand(gen, rows, 8, 128, dtype=qt).to(DEV)
+    k, v = (_rand(gen, n, 2, 128, dtype=kt).to(DEV) for _ in range(2))
+    lens = _i32([n])
+    want, got = torch.empty_like(q), q.clone()
+    ops.prompt_attention(engine, q, k, v, want, 1, n, seq_lens=lens)
+    ops.prompt_attention(engine, got, k, v, got, 1, n, seq_lens=lens)
+    assert torch.equal(got, want)
+    base, own = _i32([0] * rows), _i32([i % 2 for i in range(rows)])
+    got = q.clone()
+    ops.prefix_attention(engine, q, k, v, want, 0, n, 1, row_base=base, seq_lens=own)
+    ops.prefix_attention(engine, got, k, v, got, 0, n, 1, row_base=base, seq_lens=own)
+    assert torch.equal(got, want)
+
+
+def test_sequences_that_share_cache_rows(engine):
+    """The same cache rows under several sequences: every one reads them."""
+    gen = torch.Generator().manual_seed(32)
+    q = _rand(gen, 6, 8, 64, dtype=torch.float16)
+    k, v = (_rand(gen, 90, 2, 64, dtype=torch.float16) for _ in range(2))
+    out = torch.empty(q.shape, dtype=q.dtype, device=DEV)
+    ops.prompt_attention(engine, q.to(DEV), k.to(DEV), v.to(DEV), out, 3, 90, row_base=_i32([0, 0, 10]),
+                         seq_lens=_i32([80, 40, 80]))
+    for s, (b, m) in enumerate(((0, 80), (0, 40), (10, 80))):
+        want, tol = attend(q[2 * s:2 * s + 2], k[b:b + m], v[b:b + m], [m - 1, m], True, True)
+        check(out[2 * s:2 * s + 2], want, tol, s)
+
+
+def test_two_contexts_at_once(engine):
+    """Split calls of two contexts on two streams, many in flight: each has its own
+    partials, and every result has the bits of the calls alone."""
+    gen = torch.Generator().manual_seed(33)
+    heads, kvh, hd, cap = 32, 8, 128, 3000
+    k, v = (_rand(gen, 2 * cap, kvh, hd, dtype=torch.float16).to(DEV) for _ in range(2))
+    lens, own, base = _i32([cap, 2500]), _i32([300] * 16), _i32([cap + 100 * i for i in range(16)])
+    q1, q2 = (_rand(gen, n, heads, hd, dtype=torch.float16).to(DEV) for n in (4, 16))
+    engs = [ops.ComputeEngine(0) for _ in range(2)]
+    sides = [torch.cuda.Stream() for _ in range(2)]
+
+    def call(eng, which, out):
+        if which == 0:
+            ops.prompt_attention(eng, q1, k, v, out, 2, cap, seq_lens=lens)
+        else:
+            ops.prefix_attention(eng, q2, k, v, out, 0, cap, 300, row_base=base, seq_lens=own)
+
+    try:
+        torch.cuda.synchronize()
+        for eng, side in zip(engs, sides):
+            eng.bind_stream(side)
+        alone = [torch.empty_like(q1), torch.empty_like(q2)]
+        for i in (0, 1):
+            call(engs[i], i, alone[i])
+            engs[i].sync()
+        outs = [[torch.empty_like(alone[i]) for _ in range(20)] for i in (0, 1)]
+        torch.cuda.synchronize()
+        for j in range(20):
+            for i in (0, 1):
+                call(engs[i], i, outs[i][j])
+        for eng in engs:
+            eng.sync()
+        for i in (0, 1):
+            for j, out in enumerate(outs[i]):
+                assert torch.equal(out, alone[i]), (i, j)
+    finally:
+        for eng in engs:
+            eng.sync()
+            eng.close()
 
 
 def test_agrees_with_decode_attention(engine):
