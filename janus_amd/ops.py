@@ -261,34 +261,36 @@ def _table(t: Optional[torch.Tensor], dtype: torch.dtype, least: int, dev: int, 
         return None
     if t.dtype is not dtype or t.numel() < least:
         raise ValueError(f"{name}: at least {least} values of {dtype} expected, got {t.numel()} of {t.dtype}")
-    return _buf(t, dev, name)
+    if t.get_device() != dev or not t.is_contiguous():
+        return _buf(t, dev, name)
+    return t.data_ptr()
 
 
-def _heads(t: torch.Tensor, dev: int, name: str) -> tuple[int, int]:
-    """(address, elements from a row to the next) of [rows, heads, head_dim]
-    whose heads lie one behind the other, such as a part of a fused product's rows."""
-    rows, heads, hd = t.shape
+def _stride(t: torch.Tensor, rows: int, heads: int, hd: int, dev: int, name: str) -> int:
+    """Elements from a row to the next of [rows, heads, head_dim] whose heads lie
+    one behind the other, such as a part of a fused product's rows."""
     row, head, one = t.stride()
     if t.get_device() != dev or (one != 1 and hd != 1) or (head != hd and heads != 1) or (row < heads * hd and rows > 1):
         raise ValueError(f"{name}: [rows, heads, head_dim] on cuda:{dev} with contiguous rows expected, got {t.device}, "
                          f"strides {t.stride()}")
-    return t.data_ptr(), row if rows > 1 else heads * hd
+    return row if rows > 1 else heads * hd
 
 
 def _caches(key_cache: torch.Tensor, value_cache: torch.Tensor, hd: int, dev: int) -> tuple[int, int, int, int, int]:
     """(K address, V address, dtype, rows, kv heads) of one layer's caches [rows, kv_heads, head_dim]."""
-    shape = key_cache.shape
-    if len(shape) != 3 or shape[2] != hd or value_cache.shape != shape or key_cache.dtype is not value_cache.dtype:
+    shape, dtype = key_cache.shape, key_cache.dtype
+    if len(shape) != 3 or shape[2] != hd or value_cache.shape != shape or value_cache.dtype is not dtype:
         raise ValueError(f"key and value caches: [rows, kv_heads, {hd}] of one type expected, got {tuple(shape)} and "
                          f"{tuple(value_cache.shape)}")
-    return (_buf(key_cache, dev, "key_cache"), _buf(value_cache, dev, "value_cache"), _dt(key_cache), shape[0],
-            shape[1])
+    return (_buf(key_cache, dev, "key_cache"), _buf(value_cache, dev, "value_cache"),
+            _TORCH_DT[dtype] if dtype in _TORCH_DT else _dt(key_cache), shape[0], shape[1])
 
 
 def _three(t: torch.Tensor, name: str):
-    if t.dim() != 3:
-        raise ValueError(f"{name}: [rows, heads, head_dim] expected, got {tuple(t.shape)}")
-    return t.shape
+    shape = t.shape
+    if len(shape) != 3:
+        raise ValueError(f"{name}: [rows, heads, head_dim] expected, got {tuple(shape)}")
+    return shape
 
 
 def qk_norm_rope(engine, query, key, value, q_gamma, k_gamma, epsilon: float, rope_cache, output, key_cache,
@@ -303,24 +305,24 @@ def qk_norm_rope(engine, query, key, value, q_gamma, k_gamma, epsilon: float, ro
     shape = _three(query, "query")
     rows, heads, hd = shape
     kc, vc, kv_dt, cache_rows, kvh = _caches(key_cache, value_cache, hd, dev)
-    kv_shape = (rows, kvh, hd)
+    kv_shape, dtype = (rows, kvh, hd), query.dtype
     if key.shape != kv_shape or value.shape != kv_shape or output.shape != shape:
         raise ValueError(f"key and value: {kv_shape}, output: {tuple(shape)} expected, got {tuple(key.shape)}, "
                          f"{tuple(value.shape)}, {tuple(output.shape)}")
-    dtype = query.dtype
     if key.dtype is not dtype or value.dtype is not dtype:
         raise ValueError("query, key and value: one type expected")
     if row_base is None and rows * max_seq_len > cache_rows:
         raise ValueError("without row_base the cache holds max_seq_len rows for each row")
-    q, qs = _heads(query, dev, "query")
-    k, ks = _heads(key, dev, "key")
-    v, vs = _heads(value, dev, "value")
     f32, i32 = torch.float32, torch.int32
-    engine._check(engine.lib.janus_qk_norm_rope(
-        engine.ctx, q, k, v, _dt(query), qs, ks, vs, _table(q_gamma, f32, hd, dev, "q_gamma"),
+    status = engine.lib.janus_qk_norm_rope(
+        engine.ctx, query.data_ptr(), key.data_ptr(), value.data_ptr(), _dt(query),
+        _stride(query, rows, heads, hd, dev, "query"), _stride(key, rows, kvh, hd, dev, "key"),
+        _stride(value, rows, kvh, hd, dev, "value"), _table(q_gamma, f32, hd, dev, "q_gamma"),
         _table(k_gamma, f32, hd, dev, "k_gamma"), epsilon, _table(rope_cache, f32, max_seq_len * hd, dev, "rope_cache"),
         _buf(output, dev, "output"), _dt(output), kc, vc, kv_dt, rows, heads, kvh, hd, position, max_seq_len,
-        _table(row_base, i32, rows, dev, "row_base"), _table(positions, i32, rows, dev, "positions")))
+        _table(row_base, i32, rows, dev, "row_base"), _table(positions, i32, rows, dev, "positions"))
+    if status:
+        engine._check(status)
 
 
 def prompt_attention(engine, query, key_cache, value_cache, output, nseq: int, max_seq_len: int,
@@ -339,11 +341,13 @@ def prompt_attention(engine, query, key_cache, value_cache, output, nseq: int, m
     if row_base is None and nseq * max_seq_len > cache_rows:
         raise ValueError("without row_base the cache holds max_seq_len rows for each sequence")
     i32 = torch.int32
-    engine._check(engine.lib.janus_prompt_attention(
+    status = engine.lib.janus_prompt_attention(
         engine.ctx, _buf(query, dev, "query"), _dt(query), kc, vc, kv_dt, _buf(output, dev, "output"), rows, nseq,
         heads, kvh, hd, max_seq_len, _table(q_start, i32, nseq + 1, dev, "q_start"),
         _table(row_base, i32, nseq, dev, "row_base"), _table(seq_lens, i32, nseq, dev, "seq_lens"), max_len_hint,
-        scale))
+        scale)
+    if status:
+        engine._check(status)
 
 
 def prefix_attention(engine, query, key_cache, value_cache, output, prefix_row: int, prefix_len: int,
@@ -364,10 +368,12 @@ def prefix_attention(engine, query, key_cache, value_cache, output, prefix_row: 
     if row_base is None and (seq_lens is not None or seq_len) and batch * max_seq_len > cache_rows:
         raise ValueError("without row_base the cache holds max_seq_len rows for each sequence")
     i32 = torch.int32
-    engine._check(engine.lib.janus_prefix_attention(
+    status = engine.lib.janus_prefix_attention(
         engine.ctx, _buf(query, dev, "query"), _dt(query), kc, vc, kv_dt, _buf(output, dev, "output"), batch, heads,
         kvh, hd, prefix_row, prefix_len, seq_len, max_seq_len, _table(row_base, i32, batch, dev, "row_base"),
-        _table(seq_lens, i32, batch, dev, "seq_lens"), max_len_hint, scale))
+        _table(seq_lens, i32, batch, dev, "seq_lens"), max_len_hint, scale)
+    if status:
+        engine._check(status)
 
 
 # ---- embedding and sampling ---------------------------------------------------------
