@@ -311,8 +311,8 @@ def qk_norm_rope(engine, query, key, value, q_gamma, k_gamma, epsilon: float, ro
                          f"{tuple(value.shape)}, {tuple(output.shape)}")
     if key.dtype is not dtype or value.dtype is not dtype:
         raise ValueError("query, key and value: one type expected")
-    if row_base is None and rows * max_seq_len > cache_rows:
-        raise ValueError("without row_base the cache holds max_seq_len rows for each row")
+    if max_seq_len < 0 or (row_base is None and rows * max_seq_len > cache_rows):
+        raise ValueError("max_seq_len below 0, or without row_base fewer cache rows than max_seq_len for each row")
     f32, i32 = torch.float32, torch.int32
     status = engine.lib.janus_qk_norm_rope(
         engine.ctx, query.data_ptr(), key.data_ptr(), value.data_ptr(), _dt(query),
@@ -338,8 +338,9 @@ def prompt_attention(engine, query, key_cache, value_cache, output, nseq: int, m
     kc, vc, kv_dt, cache_rows, kvh = _caches(key_cache, value_cache, hd, dev)
     if output.shape != shape or output.dtype is not query.dtype:
         raise ValueError("output: the query's shape and type expected")
-    if row_base is None and nseq * max_seq_len > cache_rows:
-        raise ValueError("without row_base the cache holds max_seq_len rows for each sequence")
+    if nseq < 0 or max_seq_len < 0 or (row_base is None and nseq * max_seq_len > cache_rows):
+        raise ValueError("nseq or max_seq_len below 0, or without row_base fewer cache rows than max_seq_len for each "
+                         "sequence")
     i32 = torch.int32
     status = engine.lib.janus_prompt_attention(
         engine.ctx, _buf(query, dev, "query"), _dt(query), kc, vc, kv_dt, _buf(output, dev, "output"), rows, nseq,
@@ -365,8 +366,10 @@ def prefix_attention(engine, query, key_cache, value_cache, output, prefix_row: 
         raise ValueError("output: the query's shape and type expected")
     if prefix_row < 0 or prefix_len < 0 or prefix_row + prefix_len > cache_rows:
         raise ValueError("the prefix lies beyond the cache")
-    if row_base is None and (seq_lens is not None or seq_len) and batch * max_seq_len > cache_rows:
-        raise ValueError("without row_base the cache holds max_seq_len rows for each sequence")
+    if max_seq_len < 0 or seq_len < 0 or (row_base is None and (seq_lens is not None or seq_len)
+                                          and batch * max_seq_len > cache_rows):
+        raise ValueError("max_seq_len or seq_len below 0, or without row_base fewer cache rows than max_seq_len for each "
+                         "sequence")
     i32 = torch.int32
     status = engine.lib.janus_prefix_attention(
         engine.ctx, _buf(query, dev, "query"), _dt(query), kc, vc, kv_dt, _buf(output, dev, "output"), batch, heads,

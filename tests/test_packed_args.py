@@ -109,3 +109,15 @@ def test_tensor_checks():
         ops._table(idx.long(), torch.int32, 5, 0, "q_start")
     with pytest.raises(ValueError, match="at least 6"):
         ops._table(idx, torch.int32, 6, 0, "q_start")
+    for kw in (dict(nseq=-1, max_seq_len=8), dict(nseq=1, max_seq_len=-1), dict(nseq=5, max_seq_len=8)):
+        with pytest.raises(ValueError, match="below 0"):
+            ops.prompt_attention(eng, q, kv, kv, q, **kw)
+    for kw in (dict(max_seq_len=-1), dict(max_seq_len=8, seq_len=-1), dict(max_seq_len=9, seq_len=1)):
+        with pytest.raises(ValueError, match="below 0"):
+            ops.prefix_attention(eng, q, kv, kv, q, 0, 8, **kw)
+    for row, n in ((-1, 4), (0, 33), (30, 3)):
+        with pytest.raises(ValueError, match="beyond the cache"):
+            ops.prefix_attention(eng, q, kv, kv, q, row, n, 8)
+    for size in (-1, 9):
+        with pytest.raises(ValueError, match="below 0"):
+            ops.qk_norm_rope(eng, q, kv[:4], kv[:4], None, None, 1e-5, torch.zeros(9 * 64), q, kv, kv, size)
