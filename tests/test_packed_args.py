@@ -109,6 +109,7 @@ def test_tensor_checks():
         ops._table(idx.long(), torch.int32, 5, 0, "q_start")
     with pytest.raises(ValueError, match="at least 6"):
         ops._table(idx, torch.int32, 6, 0, "q_start")
+    eng.device = -1   # that of CPU tensors: sizes are looked at next
     for kw in (dict(nseq=-1, max_seq_len=8), dict(nseq=1, max_seq_len=-1), dict(nseq=5, max_seq_len=8)):
         with pytest.raises(ValueError, match="below 0"):
             ops.prompt_attention(eng, q, kv, kv, q, **kw)
