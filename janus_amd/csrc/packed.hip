@@ -149,9 +149,11 @@ __device__ __forceinline__ void sequence_of(const PackedArgs &a, uint32_t s, Wor
 // With `longest`, the tiles of all sequences go by the position that they reach, the
 // farthest first, so that no long one is begun when the others are done; else the
 // sequences follow each other, which keeps their K and V in L2. Binary32 caches take
-// the former (six prompts of 33 to 512 rows at 32/32/128: 92 -> 75 us), where a
-// position costs 16 times the matrix time; binary16 caches the latter (24 prompts
-// of 3 to 700 rows at 32/8/128: 94 against 98 us).
+// the former (six prompts of 33 to 512 rows at 32/32/128: 92 -> 75 us; 20 of 3 to 69
+// behind 85 positions: 38 -> 33), where a position costs 16 times the matrix time;
+// binary16 caches the latter (24 prompts of 3 to 700 rows at 32/8/128: 94 against 98
+// us; binary32 rows on them: 20 of 3 to 69 rows at 32/32/128 21 against 22.6, six of
+// 31 to 633 at 40/8/128 47 against 42).
 __device__ __forceinline__ bool find_task(const PackedArgs &a, uint32_t t, Work &w) {
     const uint32_t lane = threadIdx.x & 63u, shift = 31u - __builtin_clz(a.cols);
     w.causal = true;
@@ -181,7 +183,7 @@ __device__ __forceinline__ bool find_task(const PackedArgs &a, uint32_t t, Work 
         return true;
     };
     uint32_t mine = sequence(0);
-    if (a.longest) {   // at most 16 sequences, not split
+    if (a.longest) {   // at most 64 sequences, not split
         // levels: a tile's distance from position 0 in tiles; lane j counts those from lo + j step on
         const uint32_t before = x.len > x.n ? (uint32_t)min((uint64_t)(x.len - x.n) * a.G >> shift, (uint64_t)1 << 30) : 0u;
         const uint32_t top = before + mine;
@@ -1219,7 +1221,7 @@ int prompt_attention_launch(janus_ctx *ctx, const void *q, int q_dt, const void 
     const uint64_t likely = (uint64_t)nseq * ((mean + cols - 1) / cols);
     const uint64_t tasks = plan_own(ctx, a, q_dt, kv_dt, likely, tiles, max_len);
     a.slots = a.splits > 1 ? a.splits : 0;
-    a.longest = kv_dt != JANUS_DT_F16 && a.splits == 1 && nseq > 1 && nseq <= 16 && likely * kv_heads > 2u * (uint32_t)ctx->num_cus;
+    a.longest = kv_dt != JANUS_DT_F16 && a.splits == 1 && nseq > 1 && nseq <= 64 && likely * kv_heads > 2u * (uint32_t)ctx->num_cus;
     return run(ctx, a, q_dt, kv_dt, hd, tasks);
 }
 
