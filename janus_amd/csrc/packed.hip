@@ -746,13 +746,12 @@ __device__ __forceinline__ void odd_columns(const PackedArgs &a, const Work &w, 
 // Tried and slower: the scores of the next tile before the softmax of this one
 // (32 registers more, which spill).
 //   S^T: position 8 (v / 4) + 4 h + v % 4 of column lane % 32 in s[v], h = lane / 32
-template <typename Q, int D>
+template <typename Q, int D, int TP>
 __device__ __forceinline__ void wide_tile(const PackedArgs &a, const Work &w, uint32_t kvh, uint32_t ncols, uint32_t p0,
                                           uint32_t p1, unsigned char *smem) {
     typedef Range<Q, _Float16> R;
     typedef Lay<D> Y;
     constexpr bool TWO = R::TWO;
-    constexpr int TP = sizeof(Q) == 2 ? 64 : 32;   // positions per tile
     constexpr int NB = TP / 32, ND = D / 32, QN = D / 16;
     constexpr uint32_t TB = TP * Y::RB;            // bytes of a tile of K or V; LDS: K, V, K, V
     constexpr int LD = TB / 4096;                  // 1 KB requests per wavefront and tile
@@ -1033,8 +1032,14 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedArgs a) {
     }
     if constexpr (H) {
         if (ncols - w.c0 > few_of<Q, KV>()) {
-            wide_tile<Q, D>(a, w, kvh, ncols, p0, p1, smem);
+            wide_tile<Q, D, sizeof(Q) == 2 ? 64 : 32>(a, w, kvh, ncols, p0, p1, smem);
             return;
+        }
+        if constexpr (sizeof(Q) == 2) {
+            if (!shared && a.splits > 1 && (ncols - w.c0 > 16 || w.chunk >= 256)) {
+                wide_tile<Q, D, 32>(a, w, kvh, ncols, p0, p1, smem);
+                return;
+            }
         }
     }
     const uint32_t cols = ncols - w.c0;
@@ -1136,12 +1141,12 @@ bool two_parts(int q_dt, int kv_dt) { return q_dt != kv_dt; }
 // for nearly every CU a second workgroup on each gains only a quarter to a third. So
 // contexts stay whole below some lengths, by the time that a position takes (one
 // prompt of 512 rows at 32/8/128 in binary16: 16 us in one part, 25 in two).
-uint64_t plan_own(const janus_ctx *ctx, PackedArgs &a, int q_dt, int kv_dt, uint64_t likely, uint64_t tiles,
-                  uint32_t max_len) {
+uint64_t plan_own(const janus_ctx *ctx, PackedArgs &a, int q_dt, int kv_dt, uint64_t columns, uint64_t likely,
+                  uint64_t tiles, uint32_t max_len) {
     const bool cheap = q_dt == JANUS_DT_F16 || (two_parts(q_dt, kv_dt) && a.cols == 16);
     const bool busy = 3 * likely * a.kv_heads >= 2ull * (uint32_t)ctx->num_cus;
     const uint32_t whole = a.prefix_splits ? 0 : cheap ? (busy ? 1280 : 640) : busy ? 768 : 384;
-    const uint32_t least = q_dt == JANUS_DT_F16 && a.cols > 32 && !a.prefix_splits ? 256 : 128;
+    const uint32_t least = q_dt == JANUS_DT_F16 && columns > 16 && a.cols > 32 && !a.prefix_splits ? 256 : 128;
     const uint32_t want = max_len < whole ? 1 : plan_splits(ctx, likely * a.kv_heads, max_len, least);
     a.splits = 1;
     if (want == 1) return tiles;
@@ -1172,7 +1177,7 @@ uint32_t plan_cols(const janus_ctx *ctx, const PackedArgs &a, int q_dt, int kv_d
         return tiles(32) >= 2 * cus ? 32 : 16;
     }
     if (two_parts(q_dt, kv_dt)) {
-        if (columns <= 32) return 16;
+        if (columns <= 16 || (columns <= 32 && max_len <= 1536)) return 16;
         if (a.prefix_len ? max_len <= 2048 && columns * a.kv_heads <= 4 * cus : max_len <= 512 && tiles(16) <= (max_len <= 256 ? 2 : 4) * cus) return 16;
     }
     if (tiles(128) >= cus * 3 / 4) return 128;
@@ -1219,7 +1224,7 @@ int prompt_attention_launch(janus_ctx *ctx, const void *q, int q_dt, const void 
     const uint64_t tiles = (uint64_t)rows * a.G / cols + nseq;
     // about as many as sequences of equal rows have
     const uint64_t likely = (uint64_t)nseq * ((mean + cols - 1) / cols);
-    const uint64_t tasks = plan_own(ctx, a, q_dt, kv_dt, likely, tiles, max_len);
+    const uint64_t tasks = plan_own(ctx, a, q_dt, kv_dt, mean, likely, tiles, max_len);
     a.slots = a.splits > 1 ? a.splits : 0;
     a.longest = kv_dt != JANUS_DT_F16 && a.splits == 1 && nseq > 1 && nseq <= 64 && likely * kv_heads > 2u * (uint32_t)ctx->num_cus;
     return run(ctx, a, q_dt, kv_dt, hd, tasks);
@@ -1250,7 +1255,7 @@ int prefix_attention_launch(janus_ctx *ctx, const void *q, int q_dt, const void 
         const uint32_t held = (uint32_t)std::min<uint64_t>((uint64_t)batch * a.G, cols);
         a.prefix_splits = plan_splits(ctx, 2ull * a.prefix_tiles * kv_heads, prefix_len, std::max(128u, 2 * held));
     }
-    const uint64_t tasks = plan_own(ctx, a, q_dt, kv_dt, own_tiles, own_tiles, std::min(max_len, max_seq));
+    const uint64_t tasks = plan_own(ctx, a, q_dt, kv_dt, a.G, own_tiles, own_tiles, std::min(max_len, max_seq));
     a.slots = a.prefix_splits + a.splits > 1 ? a.prefix_splits + a.splits : 0;
     return run(ctx, a, q_dt, kv_dt, hd, tasks);
 }
