@@ -20,8 +20,9 @@
 // m follows the maximum only when that would grow by more than a few powers of
 // two (an exponent bias leaves P room), so most tiles rescale nothing.
 //
-// wide_tile (17 or 33 columns and more on a binary16 cache) shares K and V through
-// LDS; few_columns (the others) gives every wavefront positions of its own.
+// wide_tile (on a binary16 cache 33 columns and more, in two parts 17, and fewer on
+// split contexts) shares K and V through LDS; few_columns (the others) gives every
+// wavefront positions of its own.
 //
 // Few columns on a long context: the positions are split over workgroups, each
 // of which writes (m, l) and its output, and a second launch joins them. A
@@ -734,8 +735,8 @@ __device__ __forceinline__ void odd_columns(const PackedArgs &a, const Work &w, 
     }
 }
 
-// 17 or 33 to 128 columns on a binary16 cache: K and V pass through LDS for all four
-// wavefronts, 32 columns each, requested a tile ahead straight into LDS.
+// Up to 128 columns on a binary16 cache: K and V pass through LDS for all four
+// wavefronts, 32 columns each, requested a tile of TP positions ahead straight into LDS.
 //
 // The vector unit is as busy as the matrix unit (a wavefront's tile of 64 positions
 // is 32 MFMAs of 17 ns, about 100 other instructions of 2.1 ns and 32 exponentials
@@ -1035,8 +1036,15 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedArgs a) {
             wide_tile<Q, D, sizeof(Q) == 2 ? 64 : 32>(a, w, kvh, ncols, p0, p1, smem);
             return;
         }
+        // Few columns of a split context on binary16 rows: one wavefront computes and all
+        // four request, a tile of 32 positions ahead, which keeps more reads in flight than
+        // few_columns does (one token each of 16 requests behind up to 4000 positions: 29.5
+        // us against 31.8; five: 33.8 against 37.1; 8 requests behind 4096 shared: 16.0
+        // against 16.8). Not worth its start where parts are short and columns few (one
+        // token of one request behind 4000: 13.4 against 12.0) or nothing is split (five
+        // tokens behind up to 600: 14.2 against 12.5), nor with the products of two parts.
         if constexpr (sizeof(Q) == 2) {
-            if (!shared && a.splits > 1 && (ncols - w.c0 > 16 || w.chunk >= 256)) {
+            if (shared ? ncols - w.c0 > 16 : a.splits > 1 && (ncols - w.c0 > 16 || w.chunk >= 256)) {
                 wide_tile<Q, D, 32>(a, w, kvh, ncols, p0, p1, smem);
                 return;
             }
@@ -1167,17 +1175,24 @@ uint64_t plan_own(const janus_ctx *ctx, PackedArgs &a, int q_dt, int kv_dt, uint
 //   64 behind a prefix of 4000, two parts: 26 30 40 33; binary32 59 - 57 61
 //   11 prompts of 12 to 244: binary16 15.5 19.5 28 36, two parts 21 25 33 43,
 //     binary32 43 - 50 57
+// Once a context is long enough to be split, the columns of a sequence stay together,
+// since each tile of them reads K and V: 16 times 5 rows (20 columns) behind up to 1200
+// positions, binary32: 27 with 32, 35 with 16; up to 400: 23 and 16; two parts behind
+// up to 4000: 36 with 128, 58 with 16, up to 1000: 19 and 17.6; 12 rows (48 columns)
+// behind up to 4000, binary32: 100 with 64, 150 with 16.
 uint32_t plan_cols(const janus_ctx *ctx, const PackedArgs &a, int q_dt, int kv_dt, uint64_t groups, uint64_t columns,
                    uint32_t max_len) {
     const uint64_t cus = (uint64_t)ctx->num_cus;
     auto tiles = [&](uint32_t cols) { return groups * ((columns + cols - 1) / cols) * a.kv_heads; };
     if (kv_dt != JANUS_DT_F16) {
         if (a.prefix_len) return columns * a.kv_heads >= 32 * cus ? 64 : columns * a.kv_heads >= 4 * cus ? 32 : 16;
+        if (columns > 16 && columns <= 32 && max_len > 550) return 32;
+        if (columns > 32 && columns <= 64 && max_len > 1100) return 64;
         if (tiles(64) >= (max_len <= 128 ? cus * 3 / 4 : max_len <= 256 ? cus * 7 / 4 : 3 * cus)) return 64;
         return tiles(32) >= 2 * cus ? 32 : 16;
     }
     if (two_parts(q_dt, kv_dt)) {
-        if (columns <= 16 || (columns <= 32 && max_len <= 1536)) return 16;
+        if (columns <= 16 || (columns <= 32 && max_len <= 1200)) return 16;
         if (a.prefix_len ? max_len <= 2048 && columns * a.kv_heads <= 4 * cus : max_len <= 512 && tiles(16) <= (max_len <= 256 ? 2 : 4) * cus) return 16;
     }
     if (tiles(128) >= cus * 3 / 4) return 128;

@@ -282,6 +282,15 @@ def test_long_contexts_in_tiles_of_every_width(engine, types, heads, kvh, rows):
 
 
 @pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("rows,length", [(1, 2500), (5, 700), (5, 1500), (8, 2500), (12, 1300)])
+def test_drafts_behind_long_contexts(engine, types, rows, length):
+    # 4 to 48 columns of a sequence in one tile, split or whole; one context shorter than a part
+    seqs = [(rows, length), (rows, length // 3), (1, 90), (rows, length - 77), (0, 40), (rows, rows)]
+    for hd in (64, 128):
+        _prompt(engine, types, 32, 8, hd, seqs, device=DEV)
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
 @pytest.mark.parametrize("nseq", [11, 20])
 def test_many_tiles_of_many_heads(engine, types, nseq):
     # more tiles than two for each CU: by the position they reach (few sequences on a binary32 cache) or in order
