@@ -1173,6 +1173,8 @@ uint64_t plan_own(const janus_ctx *ctx, PackedArgs &a, int q_dt, int kv_dt, uint
 //   binary32 caches       256: 25.9 - 28.6 16.0, 1024: 119 - 106 116
 //   16 behind a prefix of 500, two parts: 12.9 12.9 13.1 11.3; binary32 20 - 15.8 11.6
 //   64 behind a prefix of 4000, two parts: 26 30 40 33; binary32 59 - 57 61
+//   8 behind a prefix of 10000, two parts: 21.7 21.7 - 17.9; 22: 25.6 32 - 30.5
+//   22 behind a prefix of 10000, binary32: - 64 53 61; of 500: - 21.0 16.3 12.6
 //   11 prompts of 12 to 244: binary16 15.5 19.5 28 36, two parts 21 25 33 43,
 //     binary32 43 - 50 57
 // Once a context is long enough to be split, the columns of a sequence stay together,
@@ -1182,10 +1184,13 @@ uint64_t plan_own(const janus_ctx *ctx, PackedArgs &a, int q_dt, int kv_dt, uint
 // behind up to 4000, binary32: 100 with 64, 150 with 16.
 uint32_t plan_cols(const janus_ctx *ctx, const PackedArgs &a, int q_dt, int kv_dt, uint64_t groups, uint64_t columns,
                    uint32_t max_len) {
-    const uint64_t cus = (uint64_t)ctx->num_cus;
+    const uint64_t cus = (uint64_t)ctx->num_cus, load = columns * a.kv_heads;
     auto tiles = [&](uint32_t cols) { return groups * ((columns + cols - 1) / cols) * a.kv_heads; };
     if (kv_dt != JANUS_DT_F16) {
-        if (a.prefix_len) return columns * a.kv_heads >= 32 * cus ? 64 : columns * a.kv_heads >= 4 * cus ? 32 : 16;
+        if (a.prefix_len) {
+            if (load >= 32 * cus) return 64;
+            return a.prefix_len >= 1024 && load >= (a.prefix_len >= 4096 ? 2 : 4) * cus ? 32 : 16;
+        }
         if (columns > 16 && columns <= 32 && max_len > 550) return 32;
         if (columns > 32 && columns <= 64 && max_len > 1100) return 64;
         if (tiles(64) >= (max_len <= 128 ? cus * 3 / 4 : max_len <= 256 ? cus * 7 / 4 : 3 * cus)) return 64;
@@ -1193,7 +1198,11 @@ uint32_t plan_cols(const janus_ctx *ctx, const PackedArgs &a, int q_dt, int kv_d
     }
     if (two_parts(q_dt, kv_dt)) {
         if (columns <= 16 || (columns <= 32 && max_len <= 1200)) return 16;
-        if (a.prefix_len ? max_len <= 2048 && columns * a.kv_heads <= 4 * cus : max_len <= 512 && tiles(16) <= (max_len <= 256 ? 2 : 4) * cus) return 16;
+        if (a.prefix_len) {
+            if (load <= 6 * cus && load * max_len <= 16384 * cus) return 16;
+        } else if (max_len <= 512 && tiles(16) <= (max_len <= 256 ? 2 : 4) * cus) {
+            return 16;
+        }
     }
     if (tiles(128) >= cus * 3 / 4) return 128;
     return max_len <= (a.prefix_len && !two_parts(q_dt, kv_dt) ? 2048 : 1024) ? 64 : 128;
