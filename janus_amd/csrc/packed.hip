@@ -1175,6 +1175,8 @@ uint64_t plan_own(const janus_ctx *ctx, PackedArgs &a, int q_dt, int kv_dt, uint
 //   64 behind a prefix of 4000, two parts: 26 30 40 33; binary32 59 - 57 61
 //   8 behind a prefix of 10000, two parts: 21.7 21.7 - 17.9; 22: 25.6 32 - 30.5
 //   22 behind a prefix of 10000, binary32: - 64 53 61; of 500: - 21.0 16.3 12.6
+//   30 rows behind 500, binary16: 16 15.8 - 11.2; three of 2 to 40 behind up to 900: 15
+//     14.8 - 12.4, behind up to 1900: 20 20 - 31; two parts 21 20.2 - 14.5, 26 26 - 32
 //   11 prompts of 12 to 244: binary16 15.5 19.5 28 36, two parts 21 25 33 43,
 //     binary32 43 - 50 57
 // Once a context is long enough to be split, the columns of a sequence stay together,
@@ -1196,6 +1198,7 @@ uint32_t plan_cols(const janus_ctx *ctx, const PackedArgs &a, int q_dt, int kv_d
         if (tiles(64) >= (max_len <= 128 ? cus * 3 / 4 : max_len <= 256 ? cus * 7 / 4 : 3 * cus)) return 64;
         return tiles(32) >= 2 * cus ? 32 : 16;
     }
+    if (!a.prefix_len && columns > 32 && max_len <= 1100 && tiles(16) <= 2 * cus) return 16;
     if (two_parts(q_dt, kv_dt)) {
         if (columns <= 16 || (columns <= 32 && max_len <= 1200)) return 16;
         if (a.prefix_len) {
