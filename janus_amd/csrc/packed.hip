@@ -607,8 +607,8 @@ __device__ __forceinline__ void few_columns(const PackedArgs &a, const Work &w, 
     const PackedArgs &z = late_args();
     constexpr uint32_t C = 16 * NT, OS = D + 4;    // padded: 16 columns meet 16 bank groups
     float *oo = (float *)smem;                     // [wave][column][OS], over the V tiles
-    float2 *ml = (float2 *)(smem + 4 * 32 * OS * 4);   // [wave][column]
-    float4 *fin = (float4 *)(ml + 4 * 32);         // [group][column]: m, l, 1 / l, row and head
+    float2 *ml = (float2 *)(smem + 4 * C * OS * 4);   // [wave][column]
+    float4 *fin = (float4 *)(ml + 4 * C);          // [group][column]: m, l, 1 / l, row and head
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         l[n] += swap16(l[n]);
@@ -981,9 +981,12 @@ __device__ __forceinline__ void wide_tile(const PackedArgs &a, const Work &w, ui
         }
 }
 
-// Q: _Float16 or float rows; KV: the cache's type.
-template <typename Q, typename KV, int D>
-__global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedArgs a) {
+// Q: _Float16 or float rows; KV: the cache's type; NARROW: 16 columns per workgroup,
+// whose LDS and registers let three workgroups share a CU (with 128 dims and two parts
+// two: three would spill, and scratch costs half the rate). 24 sequences of 2 to 50 rows
+// behind up to 200 at 16/1/128, binary32: 29 us with two, 23.4 with three.
+template <typename Q, typename KV, int D, bool NARROW>
+__global__ __launch_bounds__(256, !NARROW || (D == 128 && Range<Q, KV>::TWO) ? 2 : 3) void packed_attn_kernel(PackedArgs a) {
     constexpr bool H = sizeof(KV) == 2;
     extern __shared__ __align__(16) unsigned char smem[];
     // neighbouring workgroups take the KV heads, so that with 8 of them each XCD
@@ -1030,6 +1033,10 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedArgs a) {
             const size_t qat = (size_t)(w.row0 + row) * a.heads + kvh * a.G + (c - row * a.G);
             *(float2 *)(a.part_ml + 2 * (qat * a.slots + w.slot + 1 + x % none)) = make_float2(-INFINITY, 0.0f);
         }
+    }
+    if constexpr (NARROW) {
+        few_columns<Q, KV, D, 1>(a, w, kvh, ncols, p0, p1, 1, smem);
+        return;
     }
     if constexpr (H) {
         if (ncols - w.c0 > few_of<Q, KV>()) {
@@ -1105,20 +1112,28 @@ __global__ __launch_bounds__(256) void packed_join_kernel(PackedArgs a) {
     for (int i = 0; i < E; ++i) ((Q *)a.out)[at * D + E * lane + i] = (Q)(o[i] * inv);
 }
 
-template <typename Q, typename KV, int D>
-int launch(janus_ctx *ctx, const PackedArgs &a, uint32_t blocks) {
-    // two tiles of K and V, or the join of the wavefronts of few columns
-    constexpr size_t tiles = sizeof(KV) == 2 ? 4 * (sizeof(Q) == 2 ? 64 : 32) * D * 2 : 0;
-    constexpr size_t lds = std::max<size_t>(tiles, 4 * 32 * ((D + 4) * 4 + 8) + 64 * 16);
+template <typename Q, typename KV, int D, bool NARROW>
+int launch_attn(janus_ctx *ctx, const PackedArgs &a, uint32_t blocks) {
+    // two tiles of K and V (a V tile per wavefront), or the join of the wavefronts of few columns
+    constexpr size_t tiles = sizeof(KV) == 2 ? 4 * (sizeof(Q) == 2 && !NARROW ? 64 : 32) * D * 2 : 0;
+    constexpr size_t held = NARROW ? 16 : 32;
+    constexpr size_t lds = std::max<size_t>(tiles, 4 * held * ((D + 4) * 4 + 8) + 2 * held * 16);
     static std::atomic<uint64_t> asked{0};   // devices on which the kernel may take that much
     const uint64_t bit = 1ull << (ctx->device & 63);
     if (!(asked.load(std::memory_order_relaxed) & bit)) {
-        JANUS_HIP_CHECK(ctx, hipFuncSetAttribute((const void *)packed_attn_kernel<Q, KV, D>,
+        JANUS_HIP_CHECK(ctx, hipFuncSetAttribute((const void *)packed_attn_kernel<Q, KV, D, NARROW>,
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, lds));
         asked.fetch_or(bit, std::memory_order_relaxed);
     }
-    hipLaunchKernelGGL((packed_attn_kernel<Q, KV, D>), dim3(blocks), dim3(256), lds, ctx->stream, a);
+    hipLaunchKernelGGL((packed_attn_kernel<Q, KV, D, NARROW>), dim3(blocks), dim3(256), lds, ctx->stream, a);
     JANUS_LAUNCH_CHECK(ctx);
+    return JANUS_OK;
+}
+
+template <typename Q, typename KV, int D>
+int launch(janus_ctx *ctx, const PackedArgs &a, uint32_t blocks) {
+    if (int e = a.cols == 16 ? launch_attn<Q, KV, D, true>(ctx, a, blocks) : launch_attn<Q, KV, D, false>(ctx, a, blocks))
+        return e;
     if (a.slots) {
         const uint64_t heads = (uint64_t)a.rows * a.heads;
         hipLaunchKernelGGL((packed_join_kernel<Q, D>), dim3((uint32_t)((heads + 3) / 4)), dim3(256), 0, ctx->stream, a);
