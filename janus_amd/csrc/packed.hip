@@ -1188,7 +1188,8 @@ uint64_t plan_own(const janus_ctx *ctx, PackedArgs &a, int q_dt, int kv_dt, uint
 //   binary32 caches       256: 25.9 - 28.6 16.0, 1024: 119 - 106 116
 //   16 behind a prefix of 500, two parts: 12.9 12.9 13.1 11.3; binary32 20 - 15.8 11.6
 //   64 behind a prefix of 4000, two parts: 26 30 40 33; binary32 59 - 57 61
-//   8 behind a prefix of 10000, two parts: 21.7 21.7 - 17.9; 22: 25.6 32 - 30.5
+//   8 behind a prefix of 10000, two parts: 21.7 21.7 - 17.9, binary16 17.8 - - 16.5; 22:
+//     25.6 32 - 30.5, 19.5 - - 26.9; 45 at 32/32/128 behind 2000, binary16: 26 - - 20.4
 //   22 behind a prefix of 10000, binary32: - 64 53 61; of 500: - 21.0 16.3 12.6
 //   30 rows behind 500, binary16: 16 15.8 - 11.2; three of 2 to 40 behind up to 900: 15
 //     14.8 - 12.4, behind up to 1900: 20 20 - 31; two parts 21 20.2 - 14.5, 26 26 - 32
@@ -1211,10 +1212,11 @@ uint32_t plan_cols(const janus_ctx *ctx, const PackedArgs &a, int q_dt, int kv_d
         if (columns > 16 && columns <= 32 && max_len > 550) return 32;
         if (columns > 32 && columns <= 64 && max_len > 1100) return 64;
         if (tiles(64) >= (max_len <= 128 ? cus * 3 / 4 : max_len <= 256 ? cus * 7 / 4 : 3 * cus)) return 64;
-        return tiles(32) >= 2 * cus ? 32 : 16;
+        return max_len > 256 && tiles(32) >= 2 * cus ? 32 : 16;
     }
-    if (!a.prefix_len && columns > 32 && max_len <= 1100 && tiles(16) <= 2 * cus) return 16;
-    if (two_parts(q_dt, kv_dt)) {
+    const bool two = two_parts(q_dt, kv_dt);
+    if (!a.prefix_len && columns > 32 && max_len <= 1100 && tiles(16) <= (two && max_len > 512 ? 3 : 2) * cus) return 16;
+    if (two) {
         if (columns <= 16 || (columns <= 32 && max_len <= 1200)) return 16;
         if (a.prefix_len) {
             if (load <= 6 * cus && load * max_len <= 16384 * cus) return 16;
@@ -1222,8 +1224,12 @@ uint32_t plan_cols(const janus_ctx *ctx, const PackedArgs &a, int q_dt, int kv_d
             return 16;
         }
     }
+    if (a.prefix_len && !two) {   // long ones, or many requests' own positions beside the prefix's
+        if (max_len >= 4096 && load * max_len <= 10400 * cus) return 16;
+        if ((uint64_t)a.rows * a.kv_heads >= 2 * cus && load * max_len <= 12288 * cus) return 16;
+    }
     if (tiles(128) >= cus * 3 / 4) return 128;
-    return max_len <= (a.prefix_len && !two_parts(q_dt, kv_dt) ? 2048 : 1024) ? 64 : 128;
+    return max_len <= (a.prefix_len && !two ? 2048 : 1024) ? 64 : 128;
 }
 
 int run(janus_ctx *ctx, PackedArgs a, int q_dt, int kv_dt, uint32_t hd, uint64_t own_tasks) {
