@@ -31,10 +31,10 @@
 //
 // Measured (32/8/128 heads, binary16 unless named, the launches of a call back to
 // back): a prompt of 8192 rows 557 us, 986 TFLOP/s (a large matrix product reaches
-// 1050); 24 prompts of 3 to 700 rows 79 us (174 MB, 34 GFLOP); the last 512 binary32
-// rows of 8192 on a binary16 cache 145 us (67 GFLOP twice, for the two parts); six
+// 1050); 24 prompts of 3 to 700 rows 77 us (174 MB, 34 GFLOP); the last 512 binary32
+// rows of 8192 on a binary16 cache 140 us (67 GFLOP twice, for the two parts); six
 // prompts of 33 to 512 rows at 32/32/128 in binary32 70 us (4.5 GFLOP; 121 TFLOP/s
-// on long ones); five drafted tokens each of 16 requests 38 us (137 MB); 64 binary32
+// on long ones); five drafted tokens each of 16 requests 34 us (137 MB); 64 binary32
 // rows behind 16384 positions 70 us (206 MB).
 #include <algorithm>
 
@@ -1169,6 +1169,7 @@ uint64_t plan_own(const janus_ctx *ctx, PackedArgs &a, int q_dt, int kv_dt, uint
     const bool cheap = q_dt == JANUS_DT_F16 || (two_parts(q_dt, kv_dt) && a.cols == 16);
     const bool busy = 3 * likely * a.kv_heads >= 2ull * (uint32_t)ctx->num_cus;
     const uint32_t whole = a.prefix_splits ? 0 : cheap ? (busy ? 1280 : 640) : busy ? 768 : 384;
+    // parts of 256 positions, where more than 16 columns go through LDS (four tiles of 64)
     const uint32_t least = q_dt == JANUS_DT_F16 && columns > 16 && a.cols > 32 && !a.prefix_splits ? 256 : 128;
     const uint32_t want = max_len < whole ? 1 : plan_splits(ctx, likely * a.kv_heads, max_len, least);
     a.splits = 1;
