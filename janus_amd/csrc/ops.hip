@@ -236,8 +236,8 @@ int janus_prefix_attention(janus_ctx *ctx, const void *q, int q_dt, const void *
         return e;
     if (!d_seq_lens && seq_len > max_seq_len)
         return fail(ctx, JANUS_E_KV_OVERFLOW, "prefix_attention: seq_len exceeds max_seq_len");
-    if (prefix_row > 0x7fffffffu || prefix_len > 0x7fffffffu)
-        return fail(ctx, JANUS_E_INVALID_DIM, "prefix_attention: prefix beyond 2^31 rows");
+    if (prefix_row > 0x7fffffffu || prefix_len > 0x7fffffffu || (!d_seq_lens && seq_len > 0x7fffffffu))
+        return fail(ctx, JANUS_E_INVALID_DIM, "prefix_attention: prefix or sequence beyond 2^31 rows");
     if (batch == 0) return JANUS_OK;
     if (int e = need_device(ctx)) return e;
     DeviceGuard g(ctx->device);

@@ -1265,7 +1265,7 @@ int prompt_attention_launch(janus_ctx *ctx, const void *q, int q_dt, const void 
     a.max_seq = max_seq;
     a.seq_len = -1;
     a.scale2 = scale * 1.4426950408889634f;
-    max_len = std::min(max_len, max_seq);
+    max_len = std::min({max_len, max_seq, 0x7fffffffu});
     if (!seq_lens) max_len = std::min(max_len, q_start ? rows : rows / nseq);
     const uint64_t mean = (uint64_t)((rows + nseq - 1) / nseq) * a.G;   // columns of a sequence
     const uint32_t cols = a.cols = plan_cols(ctx, a, q_dt, kv_dt, nseq, mean, max_len);
@@ -1291,7 +1291,8 @@ int prefix_attention_launch(janus_ctx *ctx, const void *q, int q_dt, const void 
     a.seq_len = seq_len;
     a.prefix_row = prefix_row; a.prefix_len = prefix_len;
     a.scale2 = scale * 1.4426950408889634f;
-    const uint32_t cols = a.cols = plan_cols(ctx, a, q_dt, kv_dt, 1, (uint64_t)batch * a.G, std::max(prefix_len, std::min(max_len, max_seq)));
+    max_len = std::min({max_len, max_seq, 0x7fffffffu});
+    const uint32_t cols = a.cols = plan_cols(ctx, a, q_dt, kv_dt, 1, (uint64_t)batch * a.G, std::max(prefix_len, max_len));
     const uint64_t own_tiles = (uint64_t)batch * ((a.G + cols - 1) / cols);
     if (prefix_len) {
         a.prefix_tiles = (uint32_t)(((uint64_t)batch * a.G + cols - 1) / cols);
@@ -1304,7 +1305,7 @@ int prefix_attention_launch(janus_ctx *ctx, const void *q, int q_dt, const void 
         const uint32_t held = (uint32_t)std::min<uint64_t>((uint64_t)batch * a.G, cols);
         a.prefix_splits = plan_splits(ctx, 2ull * a.prefix_tiles * kv_heads, prefix_len, std::max(128u, 2 * held));
     }
-    const uint64_t tasks = plan_own(ctx, a, q_dt, kv_dt, a.G, own_tiles, own_tiles, std::min(max_len, max_seq));
+    const uint64_t tasks = plan_own(ctx, a, q_dt, kv_dt, a.G, own_tiles, own_tiles, max_len);
     a.slots = a.prefix_splits + a.splits > 1 ? a.prefix_splits + a.splits : 0;
     return run(ctx, a, q_dt, kv_dt, hd, tasks);
 }

@@ -303,6 +303,27 @@ def test_split_contexts_of_more_sequences_than_lanes(engine, types):
     _prompt(engine, types, 4, 1, 64, [((i * 5) % 3, (i * 211) % 1500) for i in range(131)], cap=1500, device=DEV)
 
 
+def test_max_seq_len_without_a_bound(engine):
+    """The largest max_seq_len with tables: it only bounds the lengths and plans."""
+    gen = torch.Generator().manual_seed(34)
+    q = _rand(gen, 3, 8, 64, dtype=torch.float16)
+    k, v = (_rand(gen, 900, 2, 64, dtype=torch.float16) for _ in range(2))
+    out = torch.empty(q.shape, dtype=q.dtype, device=DEV)
+    lens, base = [890, 3, 0], [0, 890, 5]
+    for hint in (0, 0xffffffff):
+        ops.prompt_attention(engine, q.to(DEV), k.to(DEV), v.to(DEV), out, 3, 0xffffffff, row_base=_i32(base),
+                             seq_lens=_i32(lens), max_len_hint=hint)
+        for r, (b, n) in enumerate(zip(base, lens)):
+            want, tol = attend(q[r:r + 1], k[b:b + n], v[b:b + n], [n], True, True)
+            check(out[r:r + 1], want, tol, (hint, r))
+        ops.prefix_attention(engine, q.to(DEV), k.to(DEV), v.to(DEV), out, 100, 50, 0xffffffff, row_base=_i32(base),
+                             seq_lens=_i32(lens), max_len_hint=hint)
+        for r, (b, n) in enumerate(zip(base, lens)):
+            kk, vv = (torch.cat([x[100:150], x[b:b + n]]) for x in (k, v))
+            want, tol = attend(q[r:r + 1], kk, vv, [50 + n], True, True)
+            check(out[r:r + 1], want, tol, (hint, r))
+
+
 @pytest.mark.parametrize("types", sorted(TYPES))
 @pytest.mark.parametrize("rows,n", [(1, 1), (3, 2000), (70, 70), (200, 1400)])
 def test_in_place(engine, types, rows, n):

@@ -68,6 +68,9 @@ def test_prefix_lengths(vctx):
     assert _call(vctx, "janus_prefix_attention", PREFIX, lens=None, seq_len=65)[0] == _lib.E_KV_OVERFLOW
     assert _call(vctx, "janus_prefix_attention", PREFIX, row=1 << 31)[0] == _lib.E_INVALID_DIM
     assert _call(vctx, "janus_prefix_attention", PREFIX, length=1 << 31)[0] == _lib.E_INVALID_DIM
+    far = dict(seq_len=1 << 31, max_seq=0xffffffff)
+    assert _call(vctx, "janus_prefix_attention", PREFIX, lens=None, **far)[0] == _lib.E_INVALID_DIM
+    assert _call(vctx, "janus_prefix_attention", PREFIX, **far)[0] == _lib.E_NO_DEVICE   # not looked at beside a table
 
 
 def test_head_refusals(vctx):
