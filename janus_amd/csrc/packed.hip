@@ -68,6 +68,7 @@ struct PackedArgs {
     uint32_t prefix_row, prefix_len, prefix_tiles, prefix_splits;
     uint32_t prefix_blocks, own_blocks, mix, pairs;   // workgroups; runs of `mix` of both alternate
     uint32_t longest;         // 1: tiles by the position that they reach
+    uint32_t light;           // 1: the Light kernel
     float scale2;             // scale * log2(e)
 };
 
@@ -867,17 +868,18 @@ __device__ __forceinline__ void wide_tile(const PackedArgs &a, const Work &w, ui
 #pragma unroll
             for (int t = 0; t < QN; ++t) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[n][t], qh[t], s[n], 0, 0, 0);
         }
-        // The operands of 32 positions are requested together, and those of the next
-        // 32 one by one behind the products: left to itself the compiler waits for
-        // each before it asks for the next.
-        __builtin_amdgcn_sched_group_barrier(0x100, QN, 0);
-        if constexpr (NB == 2)
+        // The operands of 32 positions (of half their dims in tiles of 32, which saves
+        // registers) are requested together, and the next ones one by one behind the
+        // products: left to itself the compiler waits for each before it asks for the next.
+        constexpr int AHEAD = NB == 2 || TWO ? QN : QN / 2;
+        __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+        if constexpr (!TWO)
 #pragma unroll
-            for (int t = 0; t < QN; ++t) {
+            for (int t = 0; t < NB * QN - AHEAD; ++t) {
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
                 __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             }
-        __builtin_amdgcn_sched_group_barrier(0x008, NB == 2 ? QN : 2 * QN, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, TWO ? 2 * QN : AHEAD, 0);
         if (p + TP > min(wave_lo, p1)) {
 #pragma unroll
             for (int n = 0; n < NB; ++n)
@@ -981,12 +983,19 @@ __device__ __forceinline__ void wide_tile(const PackedArgs &a, const Work &w, ui
         }
 }
 
-// Q: _Float16 or float rows; KV: the cache's type; NARROW: 16 columns per workgroup,
-// whose LDS and registers let three workgroups share a CU (with 128 dims and two parts
-// two: three would spill, and scratch costs half the rate). 24 sequences of 2 to 50 rows
-// behind up to 200 at 16/1/128, binary32: 29 us with two, 23.4 with three.
-template <typename Q, typename KV, int D, bool NARROW>
-__global__ __launch_bounds__(256, !NARROW || (D == 128 && Range<Q, KV>::TWO) ? 2 : 3) void packed_attn_kernel(PackedArgs a) {
+// Kernels of a launch. Few: 16 columns per workgroup, whose LDS and registers let three
+// workgroups share a CU (with 128 dims and two parts two: three would spill, and scratch
+// costs half the rate). 24 sequences of 2 to 50 rows behind up to 200 at 16/1/128,
+// binary32: 29 us with two, 23.4 with three. Light (binary16 rows, 128 dims): all
+// columns through wide_tile in tiles of 32 positions, three workgroups on a CU too. Any: the others.
+enum Kind { Any, Few, Light };
+template <typename Q, typename KV, int D, Kind K> constexpr int per_cu() {
+    return K == Any || (D == 128 && Range<Q, KV>::TWO) ? 2 : 3;
+}
+
+// Q: _Float16 or float rows; KV: the cache's type.
+template <typename Q, typename KV, int D, Kind K>
+__global__ __launch_bounds__(256, (per_cu<Q, KV, D, K>())) void packed_attn_kernel(PackedArgs a) {
     constexpr bool H = sizeof(KV) == 2;
     extern __shared__ __align__(16) unsigned char smem[];
     // neighbouring workgroups take the KV heads, so that with 8 of them each XCD
@@ -1034,8 +1043,12 @@ __global__ __launch_bounds__(256, !NARROW || (D == 128 && Range<Q, KV>::TWO) ? 2
             *(float2 *)(a.part_ml + 2 * (qat * a.slots + w.slot + 1 + x % none)) = make_float2(-INFINITY, 0.0f);
         }
     }
-    if constexpr (NARROW) {
+    if constexpr (K == Few) {
         few_columns<Q, KV, D, 1>(a, w, kvh, ncols, p0, p1, 1, smem);
+        return;
+    }
+    if constexpr (K == Light) {
+        wide_tile<Q, D, 32>(a, w, kvh, ncols, p0, p1, smem);
         return;
     }
     if constexpr (H) {
@@ -1112,28 +1125,35 @@ __global__ __launch_bounds__(256) void packed_join_kernel(PackedArgs a) {
     for (int i = 0; i < E; ++i) ((Q *)a.out)[at * D + E * lane + i] = (Q)(o[i] * inv);
 }
 
-template <typename Q, typename KV, int D, bool NARROW>
+template <typename Q, typename KV, int D, Kind K>
 int launch_attn(janus_ctx *ctx, const PackedArgs &a, uint32_t blocks) {
     // two tiles of K and V (a V tile per wavefront), or the join of the wavefronts of few columns
-    constexpr size_t tiles = sizeof(KV) == 2 ? 4 * (sizeof(Q) == 2 && !NARROW ? 64 : 32) * D * 2 : 0;
-    constexpr size_t held = NARROW ? 16 : 32;
+    constexpr size_t tiles = sizeof(KV) == 2 ? 4 * (sizeof(Q) == 2 && K == Any ? 64 : 32) * D * 2 : 0;
+    constexpr size_t held = K == Few ? 16 : K == Any ? 32 : 0;
     constexpr size_t lds = std::max<size_t>(tiles, 4 * held * ((D + 4) * 4 + 8) + 2 * held * 16);
     static std::atomic<uint64_t> asked{0};   // devices on which the kernel may take that much
     const uint64_t bit = 1ull << (ctx->device & 63);
     if (!(asked.load(std::memory_order_relaxed) & bit)) {
-        JANUS_HIP_CHECK(ctx, hipFuncSetAttribute((const void *)packed_attn_kernel<Q, KV, D, NARROW>,
+        JANUS_HIP_CHECK(ctx, hipFuncSetAttribute((const void *)packed_attn_kernel<Q, KV, D, K>,
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, lds));
         asked.fetch_or(bit, std::memory_order_relaxed);
     }
-    hipLaunchKernelGGL((packed_attn_kernel<Q, KV, D, NARROW>), dim3(blocks), dim3(256), lds, ctx->stream, a);
+    hipLaunchKernelGGL((packed_attn_kernel<Q, KV, D, K>), dim3(blocks), dim3(256), lds, ctx->stream, a);
     JANUS_LAUNCH_CHECK(ctx);
     return JANUS_OK;
 }
 
 template <typename Q, typename KV, int D>
 int launch(janus_ctx *ctx, const PackedArgs &a, uint32_t blocks) {
-    if (int e = a.cols == 16 ? launch_attn<Q, KV, D, true>(ctx, a, blocks) : launch_attn<Q, KV, D, false>(ctx, a, blocks))
-        return e;
+    int e = JANUS_OK;
+    if (a.cols == 16) {
+        e = launch_attn<Q, KV, D, Few>(ctx, a, blocks);
+    } else if (a.light) {
+        if constexpr (sizeof(Q) == 2 && D == 128) e = launch_attn<Q, KV, D, Light>(ctx, a, blocks);
+    } else {
+        e = launch_attn<Q, KV, D, Any>(ctx, a, blocks);
+    }
+    if (e) return e;
     if (a.slots) {
         const uint64_t heads = (uint64_t)a.rows * a.heads;
         hipLaunchKernelGGL((packed_join_kernel<Q, D>), dim3((uint32_t)((heads + 3) / 4)), dim3(256), 0, ctx->stream, a);
@@ -1275,6 +1295,11 @@ int prompt_attention_launch(janus_ctx *ctx, const void *q, int q_dt, const void 
     const uint64_t likely = (uint64_t)nseq * ((mean + cols - 1) / cols);
     const uint64_t tasks = plan_own(ctx, a, q_dt, kv_dt, mean, likely, tiles, max_len);
     a.slots = a.splits > 1 ? a.splits : 0;
+    // Three light workgroups hide each other's start, where there are more than two for
+    // each CU, on long contexts three (24 prompts of 3 to 700 rows: 83 us against 89; of 7
+    // to 150 behind 600: 34 against 40; three of 45 to 900, 576 workgroups: 33 against 31).
+    a.light = q_dt == JANUS_DT_F16 && hd == 128 && cols >= 64 && a.splits == 1 &&
+              likely * kv_heads > (max_len <= 800 ? 2u : 3u) * (uint32_t)ctx->num_cus;
     a.longest = kv_dt != JANUS_DT_F16 && a.splits == 1 && nseq > 1 && nseq <= 64 && likely * kv_heads > 2u * (uint32_t)ctx->num_cus;
     return run(ctx, a, q_dt, kv_dt, hd, tasks);
 }
@@ -1307,6 +1332,11 @@ int prefix_attention_launch(janus_ctx *ctx, const void *q, int q_dt, const void 
     }
     const uint64_t tasks = plan_own(ctx, a, q_dt, kv_dt, a.G, own_tiles, own_tiles, max_len);
     a.slots = a.prefix_splits + a.splits > 1 ? a.prefix_splits + a.splits : 0;
+    // light ones where the own positions weigh as much as the prefix (32 requests of up to
+    // 512 behind 4096: 19.3 us against 22.2; of up to 20, 45 behind 10000: 27 against 26)
+    // or are many workgroups (45 of 20 at 32/32/128 behind 5000: 24 against 30)
+    a.light = q_dt == JANUS_DT_F16 && hd == 128 && cols >= 64 &&
+              (own_tiles * kv_heads >= 2u * (uint32_t)ctx->num_cus || (uint64_t)batch * max_len >= prefix_len);
     return run(ctx, a, q_dt, kv_dt, hd, tasks);
 }
 

@@ -292,10 +292,11 @@ def test_drafts_behind_long_contexts(engine, types, rows, length):
 
 @pytest.mark.parametrize("types", sorted(TYPES))
 @pytest.mark.parametrize("nseq", [11, 20])
-def test_many_tiles_of_many_heads(engine, types, nseq):
+@pytest.mark.parametrize("hd", [64, 128])
+def test_many_tiles_of_many_heads(engine, types, nseq, hd):
     # more tiles than two for each CU: by the position they reach (few sequences on a binary32 cache) or in order
     seqs = [(128, 128), (5, 9), (0, 0), (100, 127), (2, 1), (128, 100)]
-    _prompt(engine, types, 32, 32, 64, [seqs[i % 6] if i % 7 else (110 + i % 9, 120) for i in range(nseq)], cap=128, device=DEV)
+    _prompt(engine, types, 32, 32, hd, [seqs[i % 6] if i % 7 else (110 + i % 9, 120) for i in range(nseq)], cap=128, device=DEV)
 
 
 @pytest.mark.parametrize("types", sorted(TYPES))
