@@ -30,12 +30,12 @@
 // limit; its parts and those of the requests' own positions are joined alike.
 //
 // Measured (32/8/128 heads, binary16 unless named, the launches of a call back to
-// back): a prompt of 8192 rows 557 us, 986 TFLOP/s (a large matrix product reaches
-// 1050); 24 prompts of 3 to 700 rows 77 us (174 MB, 34 GFLOP); the last 512 binary32
+// back): a prompt of 8192 rows 549 us, 1002 TFLOP/s (a large matrix product reaches
+// 1050); 24 prompts of 3 to 700 rows 72 us (174 MB, 34 GFLOP); the last 512 binary32
 // rows of 8192 on a binary16 cache 140 us (67 GFLOP twice, for the two parts); six
 // prompts of 33 to 512 rows at 32/32/128 in binary32 70 us (4.5 GFLOP; 121 TFLOP/s
 // on long ones); five drafted tokens each of 16 requests 34 us (137 MB); 64 binary32
-// rows behind 16384 positions 70 us (206 MB).
+// rows behind 16384 positions 68 us (206 MB).
 #include <algorithm>
 
 #include "internal.h"
