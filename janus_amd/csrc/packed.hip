@@ -66,7 +66,7 @@ struct PackedArgs {
     uint32_t target;          // parts per KV head to aim at
     uint32_t slots;           // partials per row and head (0: results are written)
     uint32_t prefix_row, prefix_len, prefix_tiles, prefix_splits;
-    uint32_t prefix_blocks, own_blocks, mix, pairs;   // workgroups; runs of `mix` of both alternate
+    uint32_t prefix_blocks;   // workgroups of the prefix, before the others
     uint32_t longest;         // 1: tiles by the position that they reach
     uint32_t light;           // 1: the Light kernel
     float scale2;             // scale * log2(e)
@@ -998,23 +998,11 @@ template <typename Q, typename KV, int D, Kind K>
 __global__ __launch_bounds__(256, (per_cu<Q, KV, D, K>())) void packed_attn_kernel(PackedArgs a) {
     constexpr bool H = sizeof(KV) == 2;
     extern __shared__ __align__(16) unsigned char smem[];
-    // neighbouring workgroups take the KV heads, so that with 8 of them each XCD
-    // keeps the K and V of one head in its L2
-    uint32_t block = blockIdx.x;
-    bool shared = block < a.prefix_blocks;
-    if (a.pairs) {   // runs of prefix and own workgroups in turn, then what is left of either
-        const uint32_t run = block / a.mix;
-        if (run < 2 * a.pairs) {
-            shared = !(run & 1u);
-            block -= (run + 1) / 2 * a.mix;
-        } else {
-            block -= a.pairs * a.mix;
-            shared = block < a.prefix_blocks;
-            if (!shared) block -= a.prefix_blocks - a.pairs * a.mix;
-        }
-    } else if (!shared) {
-        block -= a.prefix_blocks;
-    }
+    // Neighbouring workgroups take the KV heads, so that with 8 of them each XCD keeps
+    // the K and V of one head in its L2. The prefix's workgroups come first: every CU
+    // gets one, then those of the requests' own positions.
+    const bool shared = blockIdx.x < a.prefix_blocks;
+    const uint32_t block = blockIdx.x - (shared ? 0u : a.prefix_blocks);
     const uint32_t kvh = block % a.kv_heads, id = block / a.kv_heads;
     Work w;
     if (shared) {
@@ -1258,11 +1246,6 @@ int run(janus_ctx *ctx, PackedArgs a, int q_dt, int kv_dt, uint32_t hd, uint64_t
     if ((prefix + own) * 256 >= (1ull << 32) || (uint64_t)a.rows * a.heads >= (1ull << 25))
         return fail(ctx, JANUS_E_INVALID_DIM, "attention: more rows than one launch takes");
     a.prefix_blocks = (uint32_t)prefix;
-    a.own_blocks = (uint32_t)own;
-    // A prefix is bound by the matrix unit, the requests' own positions by memory: a
-    // CU gets one workgroup of each.
-    a.mix = ((uint32_t)ctx->num_cus + a.kv_heads - 1) / a.kv_heads * a.kv_heads;
-    a.pairs = std::min(a.prefix_blocks, a.own_blocks) / a.mix;
     if (a.slots) {
         const size_t parts = (size_t)a.rows * a.heads * a.slots;
         if (int e = ensure_attn_ws(ctx, parts * (hd + 2) * sizeof(float))) return e;

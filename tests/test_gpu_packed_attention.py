@@ -268,8 +268,7 @@ def test_prefix_alone_and_one_length_for_all(engine, types):
 
 
 @pytest.mark.parametrize("types", sorted(TYPES))
-def test_enough_prefix_and_own_workgroups_to_alternate(engine, types):
-    # 64 requests: two rounds of own workgroups, one and more of the prefix's
+def test_more_prefix_and_own_workgroups_than_cus(engine, types):
     _prefix(engine, types, 32, 8, 128, 64, 8300, [(i * 53) % 150 for i in range(64)], cap=150, device=DEV)
     _prefix(engine, types, 16, 8, 64, 130, 4200, [(i * 29) % 40 for i in range(130)], cap=40, device=DEV)
 
