@@ -372,7 +372,6 @@ __device__ __forceinline__ void few_columns(const PackedArgs &a, const Work &w, 
     float sc2[NT], qs[NT];
     uint32_t lim[NT], qat[NT];
     const Q *qp[NT];
-    bool q_inf = false;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         const uint32_t c = min(c0 + 16u * n + i, ncols - 1), row = c / a.G;
@@ -399,8 +398,8 @@ __device__ __forceinline__ void few_columns(const PackedArgs &a, const Work &w, 
             }
             qmax = fmaxf(qmax, swap16(qmax));
             qmax = fmaxf(qmax, swap32(qmax));
-            q_inf = q_inf || __any(qmax == INFINITY);
-            qs[n] = two_part_scale(qmax);
+            const bool inf = qmax == INFINITY;
+            qs[n] = inf ? 1.0f : two_part_scale(qmax);
             sc2[n] = a.scale2 / qs[n];
 #pragma unroll
             for (int t = 0; t < QN; ++t)
@@ -410,6 +409,18 @@ __device__ __forceinline__ void few_columns(const PackedArgs &a, const Work &w, 
                     qh[n][t][e] = (_Float16)y;
                     ql[n][t][e] = (_Float16)(y - (float)qh[n][t][e]);
                 }
+            // beside an infinity of q no finite element counts, and it has one part
+            if (__any(inf))
+#pragma unroll
+                for (int t = 0; t < QN; ++t)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float y = x[t][e >> 2][e & 3];
+                        if (inf) {
+                            qh[n][t][e] = (_Float16)(fabsf(y) == INFINITY ? y : y * 0.0f);
+                            ql[n][t][e] = (_Float16)0.0f;
+                        }
+                    }
         }
     }
     const uint32_t lo = c0 < ncols ? min(seen_of(w, c0 / a.G), p1) : 0u;   // every column sees [0, lo)
@@ -470,22 +481,28 @@ __device__ __forceinline__ void few_columns(const PackedArgs &a, const Work &w, 
             for (int b = 0; b < NB; ++b)
 #pragma unroll
                 for (int t = 0; t < KS; ++t) odd = odd_sum<KV>(kr[b][t], odd);
-            // an infinity times a part of q that is 0 or of the other sign would make a
+            // an infinity of K times a part of q that is 0 or of the other sign would make a
             // NaN of an infinite score: such steps take q whole
-            if (q_inf || __any(odd != odd)) {
+            if (__any(odd != odd)) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int b = 0; b < NB; ++b)
-#pragma unroll
-                        for (int v = 0; v < 4; ++v) {
-                            const uint32_t at = min(16u * b + 4u * g + v, e1 - 1 - p);
-                            const KV *k = (const KV *)(kc + (size_t)(p + at) * kvrow);
-                            float x = 0.0f;
+                    for (int b = 0; b < NB; ++b) {
+                        s[n][b] = (pf4){};
 #pragma unroll 1
-                            for (int d = 0; d < D; ++d) x = fmaf((float)qp[n][d], (float)k[d], x);
-                            s[n][b][v] = x * qs[n];
+                        for (int d = 0; d < D; d += 8) {
+                            const jf4 q0 = *(const jf4 *)(qp[n] + d), q1 = *(const jf4 *)(qp[n] + d + 4);
+#pragma unroll
+                            for (int v = 0; v < 4; ++v) {
+                                const uint32_t at = min(16u * b + 4u * g + v, e1 - 1 - p);
+                                const ph8 k = *(const ph8 *)((const KV *)(kc + (size_t)(p + at) * kvrow) + d);
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) s[n][b][v] = fmaf(e < 4 ? q0[e & 3] : q1[e & 3], (float)k[e], s[n][b][v]);
+                            }
                         }
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) s[n][b][v] *= qs[n];
+                    }
             }
         }
         if (more) load_k(p + stride);
@@ -493,10 +510,20 @@ __device__ __forceinline__ void few_columns(const PackedArgs &a, const Work &w, 
         float odd = 0.0f;
 #pragma unroll
         for (int j = 0; j < VS; ++j) odd = odd_sum<KV>(vr[j], odd);
-        const bool odd_v = __any(odd != odd);
-        if (odd_v)
+        uint32_t odd_v = 0;   // positions of the step that hold one
+        if (__any(odd != odd)) {
 #pragma unroll
-            for (int j = 0; j < VS; ++j) vr[j] = finite_part<KV>(vr[j]);
+            for (int j = 0; j < VS; ++j) {
+                const float x = odd_sum<KV>(vr[j], 0.0f);
+                const uint64_t hit = __ballot(x != x);
+                constexpr uint32_t L = H ? Y::SEGS : 16;   // lanes of a position
+#pragma unroll
+                for (uint32_t r = 0; r < 64 / L; ++r)
+                    if (hit >> (r * L) & ((1ull << L) - 1)) odd_v |= 1u << (H ? j * (64 / L) + r : 4 * r + j / (D / 64));
+                vr[j] = finite_part<KV>(vr[j]);
+            }
+            if (e1 - p < STEP) odd_v &= (1u << (e1 - p)) - 1;   // behind the last position lie copies of it
+        }
         if constexpr (H) {
 #pragma unroll
             for (int j = 0; j < VS; ++j) {
@@ -582,7 +609,8 @@ __device__ __forceinline__ void few_columns(const PackedArgs &a, const Work &w, 
         }
         if (odd_v) {
 #pragma unroll 1
-            for (uint32_t j = 0; j < min((uint32_t)STEP, e1 - p); ++j) {
+            for (; odd_v; odd_v &= odd_v - 1) {
+                const uint32_t j = __builtin_ctz(odd_v);
                 const KV *row = (const KV *)(vc + (size_t)(p + j) * kvrow);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
@@ -985,12 +1013,13 @@ __device__ __forceinline__ void wide_tile(const PackedArgs &a, const Work &w, ui
 
 // Kernels of a launch. Few: 16 columns per workgroup, whose LDS and registers let three
 // workgroups share a CU (with 128 dims and two parts two: three would spill, and scratch
-// costs half the rate). 24 sequences of 2 to 50 rows behind up to 200 at 16/1/128,
+// costs half the rate; with 64 dims four). 24 sequences of 2 to 50 rows behind up to 200 at 16/1/128,
 // binary32: 29 us with two, 23.4 with three. Light (binary16 rows, 128 dims): all
 // columns through wide_tile in tiles of 32 positions, three workgroups on a CU too. Any: the others.
 enum Kind { Any, Few, Light };
 template <typename Q, typename KV, int D, Kind K> constexpr int per_cu() {
-    return K == Any || (D == 128 && Range<Q, KV>::TWO) ? 2 : 3;
+    if (D == 128) return K == Any || Range<Q, KV>::TWO ? 2 : 3;
+    return K == Few ? 4 : 2;
 }
 
 // Q: _Float16 or float rows; KV: the cache's type.

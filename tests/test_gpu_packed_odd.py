@@ -181,3 +181,49 @@ def test_rising_scores(engine, types, shape):
         with torch.device(DEV):
             want, tol = attend(*(x.to(DEV) for x in (q[:n], k[:m], v[:m])), [m - n + 1 + r for r in range(n)], *f16, 0.05)
         check(out[starts[s]:starts[s + 1]], want.cpu(), tol.cpu(), (types, s))
+
+
+def _least_us(call):
+    """Least time of a call over three runs of ten."""
+    times = []
+    for _ in range(4):
+        start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        start.record()
+        for _ in range(10):
+            call()
+        end.record()
+        end.synchronize()
+        times.append(start.elapsed_time(end) * 100)
+    return min(times[1:])
+
+
+def _costs(engine, types, heads, kvh, seqs, most):
+    """One odd value of q, K or V, and scores of any size, take at most `most` times
+    as long as values without any."""
+    qt, kt = TYPES[types]
+    gen = torch.Generator(device=DEV).manual_seed(55)
+    cap = max(m for _, m in seqs)
+    starts = [0]
+    for n, _ in seqs:
+        starts.append(starts[-1] + n)
+    q = torch.randn(starts[-1], heads, 128, generator=gen, device=DEV).to(qt)
+    k, v = (torch.randn(len(seqs) * cap, kvh, 128, generator=gen, device=DEV).to(kt) for _ in range(2))
+    tables = dict(q_start=_i32(starts), seq_lens=_i32([m for _, m in seqs]))
+    out = torch.empty_like(q)
+
+    def took():
+        return _least_us(lambda: ops.prompt_attention(engine, q, k, v, out, len(seqs), cap, **tables))
+
+    clean = took()
+    for t, value in ((v, math.inf), (v, math.nan), (k, math.nan), (k, -math.inf), (q, math.inf), (q, math.nan)):
+        was = t[0, :, 3].clone()
+        t[0, :, 3] = value
+        assert took() <= most * clean, (types, value, clean)
+        t[0, :, 3] = was
+    q *= 3e4 / q.abs().max().item() if qt == torch.float16 else 1e8
+    assert took() <= most * clean, (types, "large", clean)
+
+
+@pytest.mark.parametrize("types", ["f32", "f32_f16"])
+def test_odd_values_cost_little_on_few_columns(engine, types):
+    _costs(engine, types, 32, 8, [(5, 1005)] * 16, 4)
