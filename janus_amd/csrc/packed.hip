@@ -330,7 +330,9 @@ __device__ __forceinline__ void few_columns(const PackedArgs &a, const Work &w, 
     constexpr int VS = STEP * D * (int)sizeof(KV) / 1024;   // 16-byte loads of V per step
     constexpr int ND = D / 16;
     constexpr uint32_t RB = D * sizeof(KV);
-    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    uint32_t tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));   // what follows from it stays out of the code before, which may need the registers
+    const uint32_t lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t i = lane & 15u, g = lane >> 4;
     const uint32_t pw = 4u / cw, cg = wave & (cw - 1u), pg = wave / cw;   // this wavefront's columns and positions
     const uint32_t c0 = w.c0 + 16u * NT * cg;
@@ -619,7 +621,7 @@ __device__ __forceinline__ void few_columns(const PackedArgs &a, const Work &w, 
                     for (int b = 0; b < NB; ++b)
 #pragma unroll
                         for (int v = 0; v < 4; ++v) mine = 4u * (j >> 4) + (j & 3u) == 4u * b + v ? s[n][b][v] : mine;
-                    const float pj = __shfl(mine, (int)(((j >> 2) & 3u) * 16u + i), 64);
+                    const float pj = __int_as_float(__builtin_amdgcn_ds_bpermute((int)(((j >> 2) & 3u) * 16u + i) * 4, __float_as_int(mine)));
 #pragma unroll
                     for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -676,7 +678,7 @@ __device__ __forceinline__ void few_columns(const PackedArgs &a, const Work &w, 
     }
     __syncthreads();
     const uint32_t cols = min(C * cw, ncols - w.c0);
-    for (uint32_t at = threadIdx.x; at < cols * (D / 4); at += 256) {
+    for (uint32_t at = tid; at < cols * (D / 4); at += 256) {
         const uint32_t x = at / (D / 4), dim = at % (D / 4) * 4u, group = x / C;
         const float4 f = fin[x];
         const float *from = oo + (size_t)(group * C + x % C) * OS + dim;   // wavefront `group`, then every cw-th
@@ -712,58 +714,6 @@ __device__ __forceinline__ void lds_request(const unsigned char *base, uint32_t 
 }
 #pragma clang diagnostic pop
 
-// Columns [c, end) of a tile that met an infinity or NaN, on one wavefront: lanes are
-// positions for the scores and dims for the output, everything in binary32, and
-// masked positions stay out of every sum.
-template <typename Q, int D>
-__device__ __forceinline__ void odd_columns(const PackedArgs &a, const Work &w, uint32_t kvh, uint32_t c, uint32_t end,
-                                         uint32_t p0, uint32_t p1) {
-    constexpr int E = D / 64;
-    constexpr float BIAS = Range<Q, _Float16>::BIAS;
-    const uint32_t lane = threadIdx.x & 63u;
-    const size_t kvrow = (size_t)a.kv_heads * D;
-    const _Float16 *kc = (const _Float16 *)a.kc + (w.kv_row * a.kv_heads + kvh) * D;
-    const _Float16 *vc = (const _Float16 *)a.vc + (w.kv_row * a.kv_heads + kvh) * D;
-#pragma unroll 1
-    for (; c < end; ++c) {
-        const uint32_t row = c / a.G, lim = min(seen_of(w, row), p1);
-        const size_t qat = (size_t)(w.row0 + row) * a.heads + kvh * a.G + (c - row * a.G);
-        const Q *q = (const Q *)a.q + qat * D;
-        float m = -INFINITY, l = 0.0f, o[E] = {};
-#pragma unroll 1
-        for (uint32_t p = p0; p < lim; p += 64) {
-            float s = 0.0f;
-            const _Float16 *k = kc + min(p + lane, lim - 1) * kvrow;
-#pragma unroll 1
-            for (int d = 0; d < D; ++d) s = fmaf((float)q[d], (float)k[d], s);
-            s = p + lane < lim ? s : -INFINITY;
-            const float mn = fmaxf(m, wave_max(s)), mr = mn == -INFINITY ? 0.0f : mn;
-            const float alpha = mn == m ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * a.scale2);
-            const float x = __builtin_amdgcn_exp2f(fmaf(s - mr, a.scale2, BIAS));   // parts are joined with others'
-            m = mn;
-            l = l * alpha + wave_sum(x);
-#pragma unroll
-            for (int e = 0; e < E; ++e) o[e] *= alpha;
-#pragma unroll 1
-            for (uint32_t j = 0; j < min(64u, lim - p); ++j) {
-                const float y = __shfl(x, (int)j, 64);
-#pragma unroll
-                for (int e = 0; e < E; ++e) o[e] = fmaf(y, (float)vc[(p + j) * kvrow + E * lane + e], o[e]);
-            }
-        }
-        if (a.slots) {
-            const size_t at = qat * a.slots + w.slot;
-            if (lane == 0) *(float2 *)(a.part_ml + 2 * at) = make_float2(m, l);
-#pragma unroll
-            for (int e = 0; e < E; ++e) a.part[at * D + E * lane + e] = o[e];
-        } else {
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-            for (int e = 0; e < E; ++e) ((Q *)a.out)[qat * D + E * lane + e] = (Q)(o[e] * inv);
-        }
-    }
-}
-
 // Up to 128 columns on a binary16 cache: K and V pass through LDS for all four
 // wavefronts, 32 columns each, requested a tile of TP positions ahead straight into LDS.
 //
@@ -777,7 +727,7 @@ __device__ __forceinline__ void odd_columns(const PackedArgs &a, const Work &w, 
 // (32 registers more, which spill).
 //   S^T: position 8 (v / 4) + 4 h + v % 4 of column lane % 32 in s[v], h = lane / 32
 template <typename Q, int D, int TP>
-__device__ __forceinline__ void wide_tile(const PackedArgs &a, const Work &w, uint32_t kvh, uint32_t ncols, uint32_t p0,
+__device__ __forceinline__ bool wide_tile(const PackedArgs &a, const Work &w, uint32_t kvh, uint32_t ncols, uint32_t p0,
                                           uint32_t p1, unsigned char *smem) {
     typedef Range<Q, _Float16> R;
     typedef Lay<D> Y;
@@ -819,6 +769,8 @@ __device__ __forceinline__ void wide_tile(const PackedArgs &a, const Work &w, ui
             }
         }
     };
+    uint32_t *again = (uint32_t *)(smem + 4 * TB);   // behind the tiles
+    if (threadIdx.x == 0) *again = 0;
     if (p0 < p1) request(p0, 0);
 
     const uint32_t wc0 = w.c0 + 32u * wave;
@@ -928,7 +880,7 @@ __device__ __forceinline__ void wide_tile(const PackedArgs &a, const Work &w, ui
             const float cn = fmaf(-m, sc2, R::BIAS), alpha = cn == c2 ? 1.0f : __builtin_amdgcn_exp2f(cn - c2);
             c2 = cn;
             l *= alpha;
-            // scores so large that c does not hold their last bits: odd_columns takes the difference instead
+            // scores so large that c does not hold their last bits: few_columns takes the difference instead
             if (fabsf(c2) > 4194304.0f && c2 != INFINITY) l = NAN;
 #pragma unroll
             for (int d = 0; d < ND; ++d)
@@ -976,26 +928,26 @@ __device__ __forceinline__ void wide_tile(const PackedArgs &a, const Work &w, ui
     for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int v = 0; v < 16; ++v) odd = fmaf(o[d][v], 0.0f, odd);
-    if (idle) return;
-    if (__any(odd != odd)) {
-        odd_columns<Q, D>(a, w, kvh, wc0, min(wc0 + 32u, ncols), p0, p1);
-        return;
+    if (p0 < p1) {   // else nothing is odd, and no barrier has followed the 0
+        if (__any(odd != odd) && lane == 0) *again = 1;
+        __syncthreads();
+        if (__builtin_amdgcn_readfirstlane(*again)) return true;
     }
-    if (wc0 + col >= ncols) return;
+    if (wc0 + col >= ncols) return false;
     const PackedArgs &z = late_args();
     if (z.slots) {
         const size_t at = qat * z.slots + w.slot;
         // what the rounding of c shifted, since the parts are joined by m
         const float back = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(R::BIAS - fmaf(m, sc2, c2));
         if (h == 0) *(float2 *)(z.part_ml + 2 * at) = make_float2(m / qs, l * back);
-        if (p0 >= p1) return;   // the join reads no output of a part without positions
+        if (p0 >= p1) return false;   // the join reads no output of a part without positions
         float *to = z.part + at * D;
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 *(jf4 *)(to + 32 * d + 8 * j + 4 * h) = jf4{o[d][4 * j] * back, o[d][4 * j + 1] * back, o[d][4 * j + 2] * back, o[d][4 * j + 3] * back};
-        return;
+        return false;
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;   // a row that sees nothing is 0
     Q *to = (Q *)z.out + qat * D;
@@ -1009,6 +961,7 @@ __device__ __forceinline__ void wide_tile(const PackedArgs &a, const Work &w, ui
             for (int i = 0; i < 4; ++i) y[i] = (Q)(o[d][4 * j + i] * inv);
             *(q4 *)(to + 32 * d + 8 * j + 4 * h) = y;
         }
+    return false;
 }
 
 // Kernels of a launch. Few: 16 columns per workgroup, whose LDS and registers let three
@@ -1064,15 +1017,10 @@ __global__ __launch_bounds__(256, (per_cu<Q, KV, D, K>())) void packed_attn_kern
         few_columns<Q, KV, D, 1>(a, w, kvh, ncols, p0, p1, 1, smem);
         return;
     }
-    if constexpr (K == Light) {
-        wide_tile<Q, D, 32>(a, w, kvh, ncols, p0, p1, smem);
-        return;
-    }
-    if constexpr (H) {
-        if (ncols - w.c0 > few_of<Q, KV>()) {
-            wide_tile<Q, D, sizeof(Q) == 2 ? 64 : 32>(a, w, kvh, ncols, p0, p1, smem);
-            return;
-        }
+    const uint32_t cols = ncols - w.c0;
+    bool wide = H, again = false;
+    if constexpr (K == Light) again = wide_tile<Q, D, 32>(a, w, kvh, ncols, p0, p1, smem);
+    if constexpr (H && K == Any) {
         // Few columns of a split context on binary16 rows: one wavefront computes and all
         // four request, a tile of 32 positions ahead, which keeps more reads in flight than
         // few_columns does (one token each of 16 requests behind up to 4000 positions: 29.5
@@ -1080,16 +1028,26 @@ __global__ __launch_bounds__(256, (per_cu<Q, KV, D, K>())) void packed_attn_kern
         // against 16.8). Not worth its start where parts are short and columns few (one
         // token of one request behind 4000: 13.4 against 12.0) or nothing is split (five
         // tokens behind up to 600: 14.2 against 12.5), nor with the products of two parts.
-        if constexpr (sizeof(Q) == 2) {
-            if (shared ? ncols - w.c0 > 16 : a.splits > 1 && (ncols - w.c0 > 16 || w.chunk >= 256)) {
-                wide_tile<Q, D, 32>(a, w, kvh, ncols, p0, p1, smem);
-                return;
-            }
+        const bool narrow = sizeof(Q) == 2 && (shared ? cols > 16 : a.splits > 1 && (cols > 16 || w.chunk >= 256));
+        if (cols > few_of<Q, KV>()) again = wide_tile<Q, D, sizeof(Q) == 2 ? 64 : 32>(a, w, kvh, ncols, p0, p1, smem);
+        else if (narrow) again = wide_tile<Q, D, 32>(a, w, kvh, ncols, p0, p1, smem);
+        else wide = false;
+    }
+    if (wide && !__builtin_amdgcn_readfirstlane(again)) return;   // one value for the workgroup
+    if constexpr (few_of<Q, KV>() == 32 && K == Any) {
+        if (!wide && cols > 16) {
+            few_columns<Q, KV, D, 2>(a, w, kvh, ncols, p0, p1, cols > 32 ? 2 : 1, smem);
+            return;
         }
     }
-    const uint32_t cols = ncols - w.c0;
-    if (few_of<Q, KV>() == 16 || cols <= 16) few_columns<Q, KV, D, 1>(a, w, kvh, ncols, p0, p1, 1, smem);
-    else few_columns<Q, KV, D, 2>(a, w, kvh, ncols, p0, p1, cols > 32 ? 2 : 1, smem);
+    // 16 columns, or all of a tile that met an infinity, a NaN or a score beyond 2^22. One
+    // prompt of 2048 rows at 32/8/128 with such a value at position 0, which every tile
+    // sees: 290 us, 56 without (binary16); 415 and 92 (two parts).
+    for (;;) {
+        few_columns<Q, KV, D, 1>(late_args(), w, kvh, ncols, p0, p1, 1, smem);
+        if ((w.c0 += 16) >= ncols) return;
+        __syncthreads();   // the outputs have been read from LDS
+    }
 }
 
 // Joins the parts of a row and head: a wavefront each. A part holds m, l and the
@@ -1144,9 +1102,9 @@ __global__ __launch_bounds__(256) void packed_join_kernel(PackedArgs a) {
 
 template <typename Q, typename KV, int D, Kind K>
 int launch_attn(janus_ctx *ctx, const PackedArgs &a, uint32_t blocks) {
-    // two tiles of K and V (a V tile per wavefront), or the join of the wavefronts of few columns
-    constexpr size_t tiles = sizeof(KV) == 2 ? 4 * (sizeof(Q) == 2 && K == Any ? 64 : 32) * D * 2 : 0;
-    constexpr size_t held = K == Few ? 16 : K == Any ? 32 : 0;
+    // two tiles of K and V (a V tile per wavefront) and a flag, or the join of the wavefronts of few columns
+    constexpr size_t tiles = sizeof(KV) == 2 ? 4 * (sizeof(Q) == 2 && K == Any ? 64 : 32) * D * 2 + 16 : 0;
+    constexpr size_t held = K == Any ? 32 : 16;
     constexpr size_t lds = std::max<size_t>(tiles, 4 * held * ((D + 4) * 4 + 8) + 2 * held * 16);
     static std::atomic<uint64_t> asked{0};   // devices on which the kernel may take that much
     const uint64_t bit = 1ull << (ctx->device & 63);

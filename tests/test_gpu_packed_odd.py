@@ -227,3 +227,10 @@ def _costs(engine, types, heads, kvh, seqs, most):
 @pytest.mark.parametrize("types", ["f32", "f32_f16"])
 def test_odd_values_cost_little_on_few_columns(engine, types):
     _costs(engine, types, 32, 8, [(5, 1005)] * 16, 4)
+
+
+@pytest.mark.parametrize("types", ["f16", "f32_f16"])
+@pytest.mark.parametrize("heads,kvh,seqs", [(32, 8, [(2048, 2048)]), (32, 8, [(5, 1005)] * 16), (32, 8, SPLIT), (32, 32, PACKED)])
+def test_odd_values_cost_little_on_many_columns(engine, types, heads, kvh, seqs):
+    # every tile of columns may be computed a second time, at a third to a fifth of the rate
+    _costs(engine, types, heads, kvh, seqs, 12)
