@@ -251,7 +251,7 @@ int janus_attention_noalloc(janus_ctx *ctx, const float *q, const void *k_cache,
  * call must go to different cache rows. q_out may be q where both are
  * contiguous and of one type; no other buffers may overlap. head_dim is even,
  * at most 1024; 64, 128 and 256 with 16-byte aligned buffers and strides take
- * the vector kernel. */
+ * the vector kernel. rows * (heads + 2 kv_heads) is at most 2^26 - 4. */
 int janus_qk_norm_rope(janus_ctx *ctx, const void *q, const void *k, const void *v, int in_dtype, uint32_t q_stride,
                        uint32_t k_stride, uint32_t v_stride, const float *q_gamma, const float *k_gamma, float eps,
                        const float *d_table, void *q_out, int out_dtype, void *k_cache, void *v_cache, int kv_dtype,

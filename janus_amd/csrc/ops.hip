@@ -272,8 +272,8 @@ int janus_qk_norm_rope(janus_ctx *ctx, const void *q, const void *k, const void 
         return fail(ctx, JANUS_E_KV_OVERFLOW, "KV cache position " + std::to_string(position) +
                                                   " exceeds max_seq_len " + std::to_string(max_seq_len));
     if (rows == 0) return JANUS_OK;
-    // one launch: at most 2^32 lanes, 64 for a head of any size
-    if ((uint64_t)rows * ((uint64_t)heads + 2 * kv_heads) >= (1ull << 26))
+    // one launch takes fewer than 2^32 lanes: workgroups of 256, 64 for a head of any size
+    if ((uint64_t)rows * ((uint64_t)heads + 2 * kv_heads) > (1ull << 26) - 4)
         return fail(ctx, JANUS_E_INVALID_DIM, "qk_norm_rope: more rows than one launch takes");
     if (int e = need_device(ctx)) return e;
     DeviceGuard g(ctx->device);
