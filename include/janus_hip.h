@@ -271,7 +271,9 @@ int janus_qk_norm_rope(janus_ctx *ctx, const void *q, const void *k, const void 
  * An infinity or NaN where a row does not look does not reach it. max_len_hint
  * (0: max_seq_len) is about the longest len_s: it plans the split, whatever the
  * lengths turn out to be. head_dim 64 or 128; q, caches and out 16-byte
- * aligned; out may be q. scale <= 0 selects 1/sqrt(head_dim). */
+ * aligned; out may be q. scale <= 0 selects 1/sqrt(head_dim). rows * heads is
+ * below 2^25 and nseq * kv_heads below 2^23 (up to 2^24 where the workgroups,
+ * each 16 to 128 rows * heads of a sequence and KV head, fit one launch). */
 int janus_prompt_attention(janus_ctx *ctx, const void *q, int dtype, const void *k_cache, const void *v_cache,
                            int kv_dtype, void *out, uint32_t rows, uint32_t nseq, uint32_t heads, uint32_t kv_heads,
                            uint32_t head_dim, uint32_t max_seq_len, const int32_t *d_q_start,
@@ -280,7 +282,8 @@ int janus_prompt_attention(janus_ctx *ctx, const void *q, int dtype, const void 
  * sequence b sees the cache rows [prefix_row, prefix_row + prefix_len), which
  * are read once for the whole batch, and then its own [row_base[b],
  * row_base[b] + len_b), len_b = d_seq_lens[b] (seq_len for all when NULL), at
- * most max_seq_len; both may be empty. Types, tables, hint and scale as above. */
+ * most max_seq_len; both may be empty. Types, tables, hint, scale and limits
+ * as above, with batch rows and sequences. */
 int janus_prefix_attention(janus_ctx *ctx, const void *q, int dtype, const void *k_cache, const void *v_cache,
                            int kv_dtype, void *out, uint32_t batch, uint32_t heads, uint32_t kv_heads,
                            uint32_t head_dim, uint32_t prefix_row, uint32_t prefix_len, uint32_t seq_len,

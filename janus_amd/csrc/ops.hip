@@ -190,7 +190,8 @@ int janus_attention_noalloc(janus_ctx *ctx, const float *q, const void *k_cache,
 namespace {
 // Host checks shared by the attentions of packed rows.
 int packed_args(janus_ctx *ctx, const char *name, const void *q, int q_dt, const void *k_cache, const void *v_cache,
-                int kv_dt, const void *out, uint32_t heads, uint32_t kv_heads, uint32_t hd) {
+                int kv_dt, const void *out, uint32_t rows, uint32_t nseq, uint32_t heads, uint32_t kv_heads,
+                uint32_t hd) {
     auto no = [&](int code, const char *why) { return fail(ctx, code, std::string(name) + ": " + why); };
     if (!q || !k_cache || !v_cache || !out) return no(JANUS_E_INVALID_ARG, "null buffer");
     if ((((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) & 15u) != 0)
@@ -203,6 +204,10 @@ int packed_args(janus_ctx *ctx, const char *name, const void *q, int q_dt, const
         return no(JANUS_E_INVALID_DIM, "heads must be a multiple of kv_heads");
     if (hd != 64 && hd != 128) return no(JANUS_E_INVALID_DIM, "head_dim must be 64 or 128");
     if (heads > 65536u) return no(JANUS_E_INVALID_DIM, "more than 65536 heads");
+    if (rows == 0 || nseq == 0) return JANUS_OK;
+    // the kernels count rows * heads in 32 bits, and every sequence and KV head is a workgroup at least
+    if ((uint64_t)rows * heads >= (1ull << 25)) return no(JANUS_E_INVALID_DIM, "rows * heads beyond 2^25");
+    if ((uint64_t)nseq * kv_heads >= (1ull << 24)) return no(JANUS_E_INVALID_DIM, "sequences * kv_heads beyond 2^24");
     return JANUS_OK;
 }
 }  // namespace
@@ -212,7 +217,8 @@ int janus_prompt_attention(janus_ctx *ctx, const void *q, int q_dt, const void *
                            uint32_t hd, uint32_t max_seq_len, const int32_t *d_q_start, const int32_t *d_row_base,
                            const int32_t *d_seq_lens, uint32_t max_len_hint, float scale) {
     if (check_ctx(ctx)) return JANUS_E_INVALID_ARG;
-    if (int e = packed_args(ctx, "prompt_attention", q, q_dt, k_cache, v_cache, kv_dt, out, heads, kv_heads, hd))
+    if (int e = packed_args(ctx, "prompt_attention", q, q_dt, k_cache, v_cache, kv_dt, out, rows, nseq, heads, kv_heads,
+                            hd))
         return e;
     if (rows == 0 || nseq == 0) return JANUS_OK;
     if (!d_q_start && rows % nseq)
@@ -232,7 +238,8 @@ int janus_prefix_attention(janus_ctx *ctx, const void *q, int q_dt, const void *
                            uint32_t prefix_row, uint32_t prefix_len, uint32_t seq_len, uint32_t max_seq_len,
                            const int32_t *d_row_base, const int32_t *d_seq_lens, uint32_t max_len_hint, float scale) {
     if (check_ctx(ctx)) return JANUS_E_INVALID_ARG;
-    if (int e = packed_args(ctx, "prefix_attention", q, q_dt, k_cache, v_cache, kv_dt, out, heads, kv_heads, hd))
+    if (int e = packed_args(ctx, "prefix_attention", q, q_dt, k_cache, v_cache, kv_dt, out, batch, batch, heads, kv_heads,
+                            hd))
         return e;
     if (!d_seq_lens && seq_len > max_seq_len)
         return fail(ctx, JANUS_E_KV_OVERFLOW, "prefix_attention: seq_len exceeds max_seq_len");

@@ -1230,8 +1230,9 @@ uint32_t plan_cols(const janus_ctx *ctx, const PackedArgs &a, int q_dt, int kv_d
 
 int run(janus_ctx *ctx, PackedArgs a, int q_dt, int kv_dt, uint32_t hd, uint64_t own_tasks) {
     const uint64_t prefix = (uint64_t)a.prefix_tiles * a.prefix_splits * a.kv_heads, own = own_tasks * a.kv_heads;
-    if ((prefix + own) * 256 >= (1ull << 32) || (uint64_t)a.rows * a.heads >= (1ull << 25))
-        return fail(ctx, JANUS_E_INVALID_DIM, "attention: more rows than one launch takes");
+    // with rows * heads below 2^25 only where sequences * kv_heads is 2^23 or more
+    if ((prefix + own) * 256 >= (1ull << 32))
+        return fail(ctx, JANUS_E_INVALID_DIM, "attention: more sequences than one launch takes");
     a.prefix_blocks = (uint32_t)prefix;
     if (a.slots) {
         const size_t parts = (size_t)a.rows * a.heads * a.slots;
