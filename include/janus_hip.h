@@ -262,8 +262,8 @@ int janus_qk_norm_rope(janus_ctx *ctx, const void *q, const void *k, const void 
  * s has the q rows [q_start[s], q_start[s+1]) (d_q_start: nseq + 1 ascending
  * values; NULL: rows / nseq rows each), which are the last of its len_s
  * positions: its row i of n sees positions [0, len_s - n + 1 + i) at cache rows
- * row_base[s] + position. len_s = d_seq_lens[s] (NULL: n, a whole prompt),
- * at most max_seq_len; d_row_base NULL means s * max_seq_len (d_q_start itself
+ * row_base[s] + position, of them those below max_seq_len. len_s = d_seq_lens[s]
+ * (NULL: n, a whole prompt); d_row_base NULL means s * max_seq_len (d_q_start itself
  * for K and V packed like q). A row that sees nothing (len_s < n - i, or a
  * negative row base) is 0; rows outside the sequences are left as they are.
  * q and out are [rows][heads][head_dim] of dtype: F32 on an F32 or F16 cache,

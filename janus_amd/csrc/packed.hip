@@ -77,8 +77,9 @@ struct Work {
     uint32_t row0, n;         // rows of the sequence (of the batch, for a prefix)
     uint32_t c0;              // first column
     size_t kv_row;            // cache row of position 0
-    uint32_t len;             // positions
-    bool causal;
+    uint32_t len;             // positions that there are
+    int32_t first;            // of those, row 0 sees so many (below 1: none) and each row one more than the last
+    bool causal;              // else every row sees all
     uint32_t part, parts, chunk, slot;   // positions [part chunk, + chunk); slot of the partials
 };
 
@@ -135,8 +136,9 @@ __device__ __forceinline__ void sequence_of(const PackedArgs &a, uint32_t s, Wor
         w.n = a.rows / a.nseq;
         w.row0 = s * w.n;
     }
-    const uint32_t len = a.seq_lens ? (uint32_t)max(given, 0) : a.seq_len < 0 ? w.n : (uint32_t)a.seq_len;
+    const uint32_t len = a.seq_lens ? (uint32_t)max(given, 0) : a.seq_len < 0 ? w.n : (uint32_t)a.seq_len;   // below 2^31
     w.len = base < 0 ? 0u : min(len, a.max_seq);
+    w.first = (int32_t)(len + 1u - w.n);   // n > 0 wherever it is used
     w.kv_row = base < 0 ? 0 : (size_t)base;
 }
 
@@ -180,6 +182,7 @@ __device__ __forceinline__ bool find_task(const PackedArgs &a, uint32_t t, Work 
         w.row0 = pick(x.row0);
         w.n = pick(x.n);
         w.len = pick(x.len);
+        w.first = (int32_t)pick((uint32_t)x.first);
         w.kv_row = pick((uint32_t)x.kv_row);   // below 2^31
         w.c0 = tile << shift;
         return true;
@@ -239,11 +242,10 @@ __device__ __forceinline__ bool find_task(const PackedArgs &a, uint32_t t, Work 
     }
 }
 
-// Positions that row i of the work sees: all, or len - n + 1 + i.
+// Positions that row i of the work sees: all, or first + i of them, which is at most
+// the sequence's own length and may be more than there are (max_seq_len is shorter).
 __device__ __forceinline__ uint32_t seen_of(const Work &w, uint32_t i) {
-    if (!w.causal) return w.len;
-    const int64_t s = (int64_t)w.len - w.n + 1 + i;
-    return s < 0 ? 0u : (uint32_t)s;
+    return w.causal ? min((uint32_t)max(w.first + (int32_t)i, 0), w.len) : w.len;
 }
 
 // LDS of a tile of TP positions: K rows, then V rows, 16-byte segments permuted
@@ -997,6 +999,7 @@ __global__ __launch_bounds__(256, (per_cu<Q, KV, D, K>())) void packed_attn_kern
         w.c0 = id / a.prefix_splits * a.cols;
         w.kv_row = a.prefix_row;
         w.len = a.prefix_len;
+        w.first = 0;
         w.causal = false;
     } else {
         if (!find_task(a, id, w)) return;
