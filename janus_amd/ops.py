@@ -248,6 +248,9 @@ def compute_attention_noalloc(engine, query, key_cache, value_cache, output, bat
 
 # ---- heads and attention of packed rows ----------------------------------------------
 
+_U32 = 0xffffffff   # the library's sizes
+
+
 def _buf(t: torch.Tensor, dev: int, name: str) -> int:
     """Address of a contiguous tensor on the engine's device."""
     if t.get_device() != dev or not t.is_contiguous():
@@ -273,6 +276,8 @@ def _stride(t: torch.Tensor, rows: int, heads: int, hd: int, dev: int, name: str
     if t.get_device() != dev or (one != 1 and hd != 1) or (head != hd and heads != 1) or (row < heads * hd and rows > 1):
         raise ValueError(f"{name}: [rows, heads, head_dim] on cuda:{dev} with contiguous rows expected, got {t.device}, "
                          f"strides {t.stride()}")
+    if row > _U32 and rows > 1:
+        raise ValueError(f"{name}: rows {row} elements apart, beyond 32 bits")
     return row if rows > 1 else heads * hd
 
 
@@ -313,6 +318,8 @@ def qk_norm_rope(engine, query, key, value, q_gamma, k_gamma, epsilon: float, ro
         raise ValueError("query, key and value: one type expected")
     if max_seq_len < 0 or (row_base is None and rows * max_seq_len > cache_rows):
         raise ValueError("max_seq_len below 0, or without row_base fewer cache rows than max_seq_len for each row")
+    if max_seq_len > _U32 or (positions is None and not -0x80000000 <= position <= _U32):
+        raise ValueError("max_seq_len or position beyond 32 bits")
     f32, i32 = torch.float32, torch.int32
     status = engine.lib.janus_qk_norm_rope(
         engine.ctx, query.data_ptr(), key.data_ptr(), value.data_ptr(), _dt(query),
@@ -341,6 +348,8 @@ def prompt_attention(engine, query, key_cache, value_cache, output, nseq: int, m
     if nseq < 0 or max_seq_len < 0 or (row_base is None and nseq * max_seq_len > cache_rows):
         raise ValueError("nseq or max_seq_len below 0, or without row_base fewer cache rows than max_seq_len for each "
                          "sequence")
+    if max_seq_len > _U32 or nseq > _U32:
+        raise ValueError("nseq or max_seq_len beyond 32 bits")
     i32 = torch.int32
     status = engine.lib.janus_prompt_attention(
         engine.ctx, _buf(query, dev, "query"), _dt(query), kc, vc, kv_dt, _buf(output, dev, "output"), rows, nseq,
@@ -370,6 +379,8 @@ def prefix_attention(engine, query, key_cache, value_cache, output, prefix_row: 
                                           and batch * max_seq_len > cache_rows):
         raise ValueError("max_seq_len or seq_len below 0, or without row_base fewer cache rows than max_seq_len for each "
                          "sequence")
+    if max_seq_len > _U32 or (seq_lens is None and seq_len > _U32):
+        raise ValueError("max_seq_len or seq_len beyond 32 bits")
     i32 = torch.int32
     status = engine.lib.janus_prefix_attention(
         engine.ctx, _buf(query, dev, "query"), _dt(query), kc, vc, kv_dt, _buf(output, dev, "output"), batch, heads,

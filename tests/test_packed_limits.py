@@ -1,7 +1,8 @@
 """Sizes at the limits of the packed-row operators, checked on the host."""
 import pytest
+import torch
 
-from janus_amd import _lib
+from janus_amd import _lib, ops
 from test_packed_args import HEADS, PREFIX, PROMPT, _call, vctx  # noqa: F401 (fixture)
 
 
@@ -30,3 +31,34 @@ def test_sizes_of_an_attention(vctx, name, good, rows, seqs):  # noqa: F811
         assert status == (_lib.E_NO_DEVICE if fits else _lib.E_INVALID_DIM), n
         assert fits or "2^24" in said
     assert _call(vctx, name, good, **{rows: 0}, **({seqs: 2 ** 25} if seqs != rows else {}))[0] == _lib.OK
+
+
+def test_numbers_beyond_32_bits():
+    """The library takes 32 bits; what does not fit is refused, not cut."""
+    eng = ops.ComputeEngine(-1)   # CPU tensors are on its device: every good call reaches the library's device check
+    q, kv, far = torch.zeros(4, 8, 64), torch.zeros(32, 2, 64), 2 ** 32 + 8
+    i4 = torch.zeros(4, dtype=torch.int32)
+
+    def prompt(nseq=4, max_seq_len=8, base=i4):
+        ops.prompt_attention(eng, q, kv, kv, q, nseq, max_seq_len, row_base=base, seq_lens=base)
+
+    def prefix(max_seq_len=8, seq_len=0):
+        ops.prefix_attention(eng, q, kv, kv, q, 0, 8, max_seq_len, seq_len=seq_len, row_base=i4)
+
+    def heads(key=kv[:4], value=kv[:4], query=q, position=0):
+        ops.qk_norm_rope(eng, query, key, value, None, None, 1e-5, torch.zeros(8 * 64), torch.zeros(4, 8, 64), kv, kv, 8,
+                         position=position)
+
+    for call in (prompt, prefix, heads):
+        with pytest.raises(ops.JanusError, match="device"):
+            call()
+    with pytest.raises(ops.JanusError, match="device"):
+        prompt(max_seq_len=2 ** 32 - 1)
+    # rows 2^32 elements apart, of a meta tensor: only shape, strides and type are looked at
+    wide_kv, wide_q = (torch.empty_strided((4, n, 64), (2 ** 32, 64, 1), device="meta") for n in (2, 8))
+    for bad in (lambda: prompt(max_seq_len=far), lambda: prompt(nseq=far, max_seq_len=0, base=None),
+                lambda: prefix(max_seq_len=far), lambda: prefix(seq_len=far, max_seq_len=2 ** 32 - 1),
+                lambda: heads(position=far), lambda: heads(position=-2 ** 32), lambda: heads(key=wide_kv),
+                lambda: heads(value=wide_kv), lambda: heads(query=wide_q)):
+        with pytest.raises(ValueError, match="32 bits"):
+            bad()
