@@ -247,9 +247,12 @@ int janus_attention_noalloc(janus_ctx *ctx, const float *q, const void *k_cache,
  * q, k and v are of in_dtype, rows *_stride elements apart (0: contiguous), so
  * that the parts of one fused product can be passed. d_row_base NULL means
  * r * max_seq_len. A row whose position is outside [0, max_seq_len) is left
- * out; one whose row base is negative (padding) is not appended. Rows of one
- * call must go to different cache rows. q_out may be q where both are
- * contiguous and of one type; no other buffers may overlap. head_dim is even,
+ * out; one whose row base is negative (padding) is not appended, whatever
+ * row_base[r] + p. (Where positions go on behind a shared prefix, the base is
+ * the sequence's first own row - prefix_len: those rows start at cache row
+ * prefix_len or beyond.) Rows of one call must go to different cache rows.
+ * q_out may be q where both are contiguous and of one type; no other buffers
+ * may overlap. head_dim is even,
  * at most 1024; 64, 128 and 256 with 16-byte aligned buffers and strides take
  * the vector kernel. rows * (heads + 2 kv_heads) is at most 2^26 - 4. */
 int janus_qk_norm_rope(janus_ctx *ctx, const void *q, const void *k, const void *v, int in_dtype, uint32_t q_stride,

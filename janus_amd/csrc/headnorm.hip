@@ -10,10 +10,13 @@
 // Bound by HBM: every value is read and written once. A head is held by the lanes
 // that load it, 16 bytes of either half each, so the norm is a sum over 4 to 32
 // lanes and the turn stays in a lane. Outputs are stored past the caches: 8192
-// binary16 rows of a 32/8/128 product (202 MB) take 38.8 us (5.2 TB/s; a copy
-// reaches 4.7), 47 with ordinary stores; followed by the attention that reads
-// them, both take the same. Four heads of a row per lane group (the table read
-// once for them) took 41 us, and 49.5 with ordinary stores.
+// binary16 rows of a 32/8/128 product (202 MB) take 37 us (5.4 TB/s; a copy reaches
+// 4.7), 40 with ordinary stores; binary32 rows into a binary16 cache (370 MB) 64 and
+// 68; 4096 binary16 rows at 32/8/256 (203 MB) 37 and 40. Four heads of a row per lane
+// group (the table read once for them) were slower. Head dims and alignments that the
+// vectors do not fit take a wavefront per head and a value per load, at a quarter of
+// the rate: 8192 binary16 rows at 32/8/96 (152 MB) 160 us, the 202 MB above at odd
+// addresses 170; 48 rows of a decode step are bound by the call, 9 us, either way.
 #include "internal.h"
 
 namespace janus {

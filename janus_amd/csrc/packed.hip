@@ -30,12 +30,12 @@
 // limit; its parts and those of the requests' own positions are joined alike.
 //
 // Measured (32/8/128 heads, binary16 unless named, the launches of a call back to
-// back): a prompt of 8192 rows 549 us, 1002 TFLOP/s (a large matrix product reaches
-// 1050); 24 prompts of 3 to 700 rows 72 us (174 MB, 34 GFLOP); the last 512 binary32
-// rows of 8192 on a binary16 cache 140 us (67 GFLOP twice, for the two parts); six
-// prompts of 33 to 512 rows at 32/32/128 in binary32 70 us (4.5 GFLOP; 121 TFLOP/s
-// on long ones); five drafted tokens each of 16 requests 34 us (137 MB); 64 binary32
-// rows behind 16384 positions 68 us (206 MB).
+// back, here and below): a prompt of 8192 rows 558 us, 985 TFLOP/s (a large matrix
+// product reaches 1050); 24 prompts of 3 to 700 rows 72 us (174 MB, 34 GFLOP); the last
+// 512 binary32 rows of 8192 on a binary16 cache 142 us (67 GFLOP twice, for the two
+// parts); six prompts of 33 to 512 rows at 32/32/128 in binary32 67 us (4.5 GFLOP; 121
+// TFLOP/s on long ones); five drafted tokens each of 16 requests 34 us (137 MB); 64
+// binary32 rows behind 16384 positions 68 us (206 MB).
 #include <algorithm>
 
 #include "internal.h"
@@ -146,18 +146,17 @@ __device__ __forceinline__ void sequence_of(const PackedArgs &a, uint32_t s, Wor
 // go from its last to its first.
 //
 // Splitting (few tiles): the tables give the positions of all tiles, and every part
-// gets as many, so that long and short contexts take equal workgroups (drafted
-// tokens of 16 requests with 200 to 4000 positions: 44 -> 39 us against equal counts
-// of parts). Every workgroup finds the same numbers.
+// gets as many, so that long and short contexts take equal workgroups. Every workgroup
+// finds the same numbers.
 //
 // With `longest`, the tiles of all sequences go by the position that they reach, the
 // farthest first, so that no long one is begun when the others are done; else the
 // sequences follow each other, which keeps their K and V in L2. Binary32 caches take
-// the former (six prompts of 33 to 512 rows at 32/32/128: 92 -> 75 us; 20 of 3 to 69
-// behind 85 positions: 38 -> 33), where a position costs 16 times the matrix time;
-// binary16 caches the latter (24 prompts of 3 to 700 rows at 32/8/128: 94 against 98
-// us; binary32 rows on them: 20 of 3 to 69 rows at 32/32/128 21 against 22.6, six of
-// 31 to 633 at 40/8/128 47 against 42).
+// the former, where a position costs 16 times the matrix time (six prompts of 33 to 512
+// rows at 32/32/128: 67 us against 86; 20 of 3 to 69 behind up to 85 positions: 37
+// against 35); binary16 caches the latter (24 prompts of 3 to 700 rows at 32/8/128: 70
+// us either way; binary32 rows on them: 117 either way, 20 of 3 to 69 rows at 32/32/128
+// 18.6 against 19.9, six of 31 to 633 at 40/8/128 48 against 47).
 __device__ __forceinline__ bool find_task(const PackedArgs &a, uint32_t t, Work &w) {
     const uint32_t lane = threadIdx.x & 63u, shift = 31u - __builtin_clz(a.cols);
     w.causal = true;
@@ -968,9 +967,10 @@ __device__ __forceinline__ bool wide_tile(const PackedArgs &a, const Work &w, ui
 
 // Kernels of a launch. Few: 16 columns per workgroup, whose LDS and registers let three
 // workgroups share a CU (with 128 dims and two parts two: three would spill, and scratch
-// costs half the rate; with 64 dims four). 24 sequences of 2 to 50 rows behind up to 200 at 16/1/128,
-// binary32: 29 us with two, 23.4 with three. Light (binary16 rows, 128 dims): all
-// columns through wide_tile in tiles of 32 positions, three workgroups on a CU too. Any: the others.
+// costs half the rate; with 64 dims four). 24 sequences of 2 to 50 rows behind up to 200
+// at 16/1/128, binary32: 25.1 us with two, 22.7 with three. Light (binary16 rows, 128
+// dims): all columns through wide_tile in tiles of 32 positions, three workgroups on a
+// CU too. Any: the others.
 enum Kind { Any, Few, Light };
 template <typename Q, typename KV, int D, Kind K> constexpr int per_cu() {
     if (D == 128) return K == Any || Range<Q, KV>::TWO ? 2 : 3;
@@ -1026,11 +1026,11 @@ __global__ __launch_bounds__(256, (per_cu<Q, KV, D, K>())) void packed_attn_kern
     if constexpr (H && K == Any) {
         // Few columns of a split context on binary16 rows: one wavefront computes and all
         // four request, a tile of 32 positions ahead, which keeps more reads in flight than
-        // few_columns does (one token each of 16 requests behind up to 4000 positions: 29.5
-        // us against 31.8; five: 33.8 against 37.1; 8 requests behind 4096 shared: 16.0
-        // against 16.8). Not worth its start where parts are short and columns few (one
-        // token of one request behind 4000: 13.4 against 12.0) or nothing is split (five
-        // tokens behind up to 600: 14.2 against 12.5), nor with the products of two parts.
+        // few_columns does (five tokens each of 16 requests behind up to 4000 positions: 33
+        // us against 36; one each: 36 either way). Not worth its start where parts are short
+        // and columns few or nothing is split (five tokens of one request behind 600: 16.0
+        // against 12.4, of 16 behind up to 600: 16.3 against 13.6), nor with the products of
+        // two parts.
         const bool narrow = sizeof(Q) == 2 && (shared ? cols > 16 : a.splits > 1 && (cols > 16 || w.chunk >= 256));
         if (cols > few_of<Q, KV>()) again = wide_tile<Q, D, sizeof(Q) == 2 ? 64 : 32>(a, w, kvh, ncols, p0, p1, smem);
         else if (narrow) again = wide_tile<Q, D, 32>(a, w, kvh, ncols, p0, p1, smem);
@@ -1161,7 +1161,7 @@ bool two_parts(int q_dt, int kv_dt) { return q_dt != kv_dt; }
 // launch (about 5 us) unless the results are joined anyway, and where there is a tile
 // for nearly every CU a second workgroup on each gains only a quarter to a third. So
 // contexts stay whole below some lengths, by the time that a position takes (one
-// prompt of 512 rows at 32/8/128 in binary16: 16 us in one part, 25 in two).
+// prompt of 512 rows at 32/8/128 in binary16: 15 us in one part, 22 in two).
 uint64_t plan_own(const janus_ctx *ctx, PackedArgs &a, int q_dt, int kv_dt, uint64_t columns, uint64_t likely,
                   uint64_t tiles, uint32_t max_len) {
     const bool cheap = q_dt == JANUS_DT_F16 || (two_parts(q_dt, kv_dt) && a.cols == 16);
@@ -1181,24 +1181,32 @@ uint64_t plan_own(const janus_ctx *ctx, PackedArgs &a, int q_dt, int kv_dt, uint
 // Columns per workgroup for `groups` runs of `columns` columns each on up to max_len
 // positions (of the caches' capacity, where the caller gave no hint). Many columns
 // share the K and V that a workgroup reads and few fill the CUs without splitting the
-// positions. At 32/8/128, us with 128 (or 64 for binary32 caches), 64, 32 and 16:
-//   binary16              one prompt of 256: 15.7 14.8 19.1 10.7, 1024: 43 28 39 57
-//   two parts             256: 19.3 17.8 19.5 12.5, 1024: 58 44 51 63
-//   binary32 caches       256: 25.9 - 28.6 16.0, 1024: 119 - 106 116
-//   16 behind a prefix of 500, two parts: 12.9 12.9 13.1 11.3; binary32 20 - 15.8 11.6
-//   64 behind a prefix of 4000, two parts: 26 30 40 33; binary32 59 - 57 61
-//   8 behind a prefix of 10000, two parts: 21.7 21.7 - 17.9, binary16 17.8 - - 16.5; 22:
-//     25.6 32 - 30.5, 19.5 - - 26.9; 45 at 32/32/128 behind 2000, binary16: 26 - - 20.4
-//   22 behind a prefix of 10000, binary32: - 64 53 61; of 500: - 21.0 16.3 12.6
-//   30 rows behind 500, binary16: 16 15.8 - 11.2; three of 2 to 40 behind up to 900: 15
-//     14.8 - 12.4, behind up to 1900: 20 20 - 31; two parts 21 20.2 - 14.5, 26 26 - 32
-//   11 prompts of 12 to 244: binary16 15.5 19.5 28 36, two parts 21 25 33 43,
-//     binary32 43 - 50 57
+// positions. Us with 128, 64, 32 and 16 (binary32 caches: 64, 32, 16), * what is taken,
+// at 32/8/128 unless named; requests behind a prefix have up to 40 positions of their own:
+//                               binary16              two parts             binary32
+//   one prompt of 256           11.1 9.9 10.0 9.9*    16.5 15.2 14.2 11.9*  26.8 17.9 15.2*
+//   one prompt of 1024          26* 26 36 47          54* 40 46 58          110 97* 99
+//     at 24/8/64                17* 17 17 23          34* 27 26 26          58 44* 48
+//   11 prompts of 12 to 244     17.7* 17.7 32 33      25* 28 37 50          48* 60 58
+//     at 40/8/128               19* 21 39 40          28* 32 44 62          59* 76 74
+//   30 rows behind 500          16 15 12.6 10.3*      16 15 13.7 11.6*      22 17 16*
+//   3 of 2 to 40 behind 900     14.1 12.5 13.5 14.6*  17 15 16 19*          23 24 21*
+//     behind 1900               15.6* 15.8 15.2 18    19* 19 18 22          28 26 29*
+//   16 times 5 rows behind 400  12.1 12.2 12.2 10.1*  16 16 16 11.5*        24 24 17*
+//     behind 1000               19* 19 19 15          24 24 24 16*          35* 35 30
+//     behind 1200               15* 15 15 17          20 19 19 18*          31* 31 34
+//     behind 4000               43* 43 43 51          50* 50 50 53          80 80* 92
+//   16 times 12 behind 4000     47* 47 60 73          55* 55 76 75          129* 123 153
+//   16 requests, prefix of 500  10.6 10.7* 10.3 10.5  13 13 13 10.2*        20 15 11*
+//   22 of 500                   11.7 10.9* 10.5 10.0  15 13 13 11.6*        20 16 13*
+//   8 of 10000                  16.6 16.6 16.7 16.3*  21 21 21 17*          29 28 28*
+//   22 of 10000                 19* 22 28 27          25* 31 39 28          62 52* 60
+//   64 of 4000                  20* 20 28 28          25* 27 39 30          54 52* 57
+//   45 of 2000 at 32/32/128     20.0 20.0 24 19.9*    29 29 28 27*          43 39* 38
+//   32 of 4096 at 40/8/128      19* 19 23 23          24* 26 31 25          48 41* 44
+//     at 24/8/64                13* 13 15 13          15.3 16 18 14.4*      23 21* 21
 // Once a context is long enough to be split, the columns of a sequence stay together,
-// since each tile of them reads K and V: 16 times 5 rows (20 columns) behind up to 1200
-// positions, binary32: 27 with 32, 35 with 16; up to 400: 23 and 16; two parts behind
-// up to 4000: 36 with 128, 58 with 16, up to 1000: 19 and 17.6; 12 rows (48 columns)
-// behind up to 4000, binary32: 100 with 64, 150 with 16.
+// since each tile of them reads K and V.
 uint32_t plan_cols(const janus_ctx *ctx, const PackedArgs &a, int q_dt, int kv_dt, uint64_t groups, uint64_t columns,
                    uint32_t max_len) {
     const uint64_t cus = (uint64_t)ctx->num_cus, load = columns * a.kv_heads;
@@ -1270,8 +1278,9 @@ int prompt_attention_launch(janus_ctx *ctx, const void *q, int q_dt, const void 
     const uint64_t tasks = plan_own(ctx, a, q_dt, kv_dt, mean, likely, tiles, max_len);
     a.slots = a.splits > 1 ? a.splits : 0;
     // Three light workgroups hide each other's start, where there are more than two for
-    // each CU, on long contexts three (24 prompts of 3 to 700 rows: 83 us against 89; of 7
-    // to 150 behind 600: 34 against 40; three of 45 to 900, 576 workgroups: 33 against 31).
+    // each CU, on long contexts three (24 prompts of 3 to 700 rows: 70 us against 75; one
+    // of 8192: 557 against 560; 24 of 7 to 150 behind up to 600: 36 against 35; three of 45
+    // to 900, 576 workgroups: 32.2 against 31.4).
     a.light = q_dt == JANUS_DT_F16 && hd == 128 && cols >= 64 && a.splits == 1 &&
               likely * kv_heads > (max_len <= 800 ? 2u : 3u) * (uint32_t)ctx->num_cus;
     a.longest = kv_dt != JANUS_DT_F16 && a.splits == 1 && nseq > 1 && nseq <= 64 && likely * kv_heads > 2u * (uint32_t)ctx->num_cus;
@@ -1295,20 +1304,21 @@ int prefix_attention_launch(janus_ctx *ctx, const void *q, int q_dt, const void 
     const uint64_t own_tiles = (uint64_t)batch * ((a.G + cols - 1) / cols);
     if (prefix_len) {
         a.prefix_tiles = (uint32_t)(((uint64_t)batch * a.G + cols - 1) / cols);
-        // One workgroup per CU, beside those of the own positions: half the partials of
-        // two per CU (64 requests behind 16384 positions: 78 against 88 us; 32 behind
-        // 8192 with one own: 27 against 34). A part reads K and V once and writes a row
-        // per column, so it has at least two positions for each column, and 128 for the
-        // four wavefronts (16 requests behind 3000 positions: 15.7 us, with 256 18; 32
-        // behind 4096: 22.6 us with 256, 26.6 with 128).
+        // At most one workgroup per CU, beside those of the own positions: half the
+        // partials of two per CU (64 requests behind 16384 positions: 61 against 69 us, in
+        // two parts 67 against 85; 32 behind 8192 with one own: 20 either way). A part
+        // reads K and V once and writes a row per column, so it has at least two positions
+        // for each column, and 128 for the four wavefronts (16 requests behind 3000
+        // positions: 12.5 us, with 256 13.1, with 512 17; 32 behind 4096: 16.3 us with 256,
+        // 17.3 with 128, 19 with 512).
         const uint32_t held = (uint32_t)std::min<uint64_t>((uint64_t)batch * a.G, cols);
         a.prefix_splits = plan_splits(ctx, 2ull * a.prefix_tiles * kv_heads, prefix_len, std::max(128u, 2 * held));
     }
     const uint64_t tasks = plan_own(ctx, a, q_dt, kv_dt, a.G, own_tiles, own_tiles, max_len);
     a.slots = a.prefix_splits + a.splits > 1 ? a.prefix_splits + a.splits : 0;
     // light ones where the own positions weigh as much as the prefix (32 requests of up to
-    // 512 behind 4096: 19.3 us against 22.2; of up to 20, 45 behind 10000: 27 against 26)
-    // or are many workgroups (45 of 20 at 32/32/128 behind 5000: 24 against 30)
+    // 512 behind 4096: 19.7 us against 21.4; of up to 20, 45 behind 10000: 25.7 against 24.7)
+    // or are many workgroups (45 of up to 20 at 32/32/128 behind 5000: 25.5 against 29.3)
     a.light = q_dt == JANUS_DT_F16 && hd == 128 && cols >= 64 &&
               (own_tiles * kv_heads >= 2u * (uint32_t)ctx->num_cus || (uint64_t)batch * max_len >= prefix_len);
     return run(ctx, a, q_dt, kv_dt, hd, tasks);

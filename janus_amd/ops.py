@@ -305,7 +305,9 @@ def qk_norm_rope(engine, query, key, value, q_gamma, k_gamma, epsilon: float, ro
     for no norm), rotation, and the append of K and V to the cache, in one pass
     (janus_qk_norm_rope in include/janus_hip.h). query, key and value are [rows,
     heads, head_dim], also as parts of one fused product's rows; output [rows,
-    heads, head_dim] receives the rotated queries and may be query."""
+    heads, head_dim] receives the rotated queries and may be query. K and V of row
+    r go to cache row row_base[r] + position; a negative row_base[r] is padding and
+    appends nothing."""
     dev = engine.device
     shape = _three(query, "query")
     rows, heads, hd = shape
