@@ -423,6 +423,13 @@ __device__ __forceinline__ uint32_t sampler_key_index(uint64_t key, int mode) {
     return mode == SAMPLE_WGSL ? (~(uint32_t)key) & 0xffffffu : (uint32_t)key;
 }
 
+// Value of lane ^ 32.
+__device__ __forceinline__ float swap32(float v) {
+    const uint32_t u = __float_as_uint(v);
+    auto p = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __uint_as_float((__lane_id() & 32) ? p[0] : p[1]);
+}
+
 // Sum over all 64 lanes of a wavefront; every lane receives the total.
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll

@@ -83,12 +83,6 @@ struct Work {
     uint32_t part, parts, chunk, slot;   // positions [part chunk, + chunk); slot of the partials
 };
 
-__device__ __forceinline__ float swap32(float v) {   // value of lane ^ 32
-    const uint32_t u = __float_as_uint(v);
-    auto p = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-    return __uint_as_float((__lane_id() & 32) ? p[0] : p[1]);
-}
-
 __device__ __forceinline__ float swap16(float v) {   // value of lane ^ 16
     const uint32_t u = __float_as_uint(v);
     auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);

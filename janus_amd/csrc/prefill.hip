@@ -54,12 +54,6 @@ struct PrefillArgs {
     int out_f16;
 };
 
-__device__ __forceinline__ float swap32(float v) {   // value of lane ^ 32
-    const uint32_t u = __float_as_uint(v);
-    auto p = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-    return __uint_as_float((__lane_id() & 32) ? p[0] : p[1]);
-}
-
 // LDS of one K/V tile. binary16: K rows padded to D + 8 halves; V transposed,
 // [dim][position] rows padded to PT + 4 halves (8-byte reads of 4 positions).
 // binary32: K rows padded to D + 4 floats, V rows as they are. Behind them one
