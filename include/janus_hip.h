@@ -293,6 +293,85 @@ int janus_prefix_attention(janus_ctx *ctx, const void *q, int dtype, const void 
                            uint32_t max_seq_len, const int32_t *d_row_base, const int32_t *d_seq_lens,
                            uint32_t max_len_hint, float scale);
 
+/* ---- a cache of 4-bit values --------------------------------------------- */
+/* No counterpart in the reference. One layer's slice of such a cache is, for K and
+ * for V, values [cache_rows][kv_heads][head_dim / 2] (bytes; element 2i in the low
+ * half of byte i) and scales [cache_rows][kv_heads][head_dim / 32] (bytes): blocks of
+ * 32 values of a head share a scale. A value is an e2m1 code (sign, then 0, 0.5, 1,
+ * 1.5, 2, 3, 4 or 6) times 2^(b - 127), b the scale byte; b below 104 counts as 104,
+ * b above 140 makes the block NaN. 4.25 bits a value against 16. A cache of zero
+ * bytes holds zeros. Values are 16-byte aligned, scales 4-byte.
+ *
+ * Whatever the tables hold, no call reads or writes beyond cache_rows: rows outside
+ * are left out.
+ *
+ * Appends rows of K and V (in_dtype, F32 or F16, rows *_stride elements apart, 0:
+ * contiguous): row r at position p = d_positions[r] (position for all when NULL) goes
+ * to cache row row_base[r] + p (d_row_base NULL: r * max_seq_len). A row whose position
+ * is outside [0, max_seq_len), whose row base is negative (padding) or whose cache row is
+ * not below cache_rows is left out. Rows of one call must go to different cache rows.
+ * A block x gets the scale 2^e, e = floor(log2 max|x|) - 2, one more where max|x| is
+ * above 7/8 of the next power of two, within [-23, 13] (byte e + 127), and every
+ * value goes to the nearest code, ties to the even one, at most 6 (magnitudes above
+ * 49152 become 49152). A block with an infinity or NaN becomes NaN (byte 255, codes 0).
+ * head_dim is a multiple of 32, at most 1024. */
+int janus_kv_update_fp4(janus_ctx *ctx, const void *k, const void *v, int in_dtype, uint32_t k_stride, uint32_t v_stride,
+                        void *k_cache, void *k_scales, void *v_cache, void *v_scales, uint32_t rows, uint32_t kv_heads,
+                        uint32_t head_dim, uint32_t cache_rows, uint32_t position, uint32_t max_seq_len,
+                        const int32_t *d_row_base, const int32_t *d_positions);
+/* Cache rows back: k_out and v_out [rows][kv_heads][head_dim] of out_dtype (16-byte
+ * aligned; F32 and F16 hold every value exactly) receive cache row d_rows[r]
+ * (first_row + r when NULL); rows outside [0, cache_rows) are left as they are. */
+int janus_kv_read_fp4(janus_ctx *ctx, const void *k_cache, const void *k_scales, const void *v_cache, const void *v_scales,
+                      void *k_out, void *v_out, int out_dtype, uint32_t rows, uint32_t kv_heads, uint32_t head_dim,
+                      uint32_t cache_rows, uint32_t first_row, const int32_t *d_rows);
+/* janus_prompt_attention over a 4-bit cache: causal attention of packed rows, from one
+ * decode step's single tokens (rows = nseq, d_q_start NULL) to drafted tokens and
+ * prompts, with the tables, hint, scale, results for rows that see nothing and limits
+ * described there; positions at cache rows of cache_rows and above do not exist. q and out are
+ * [rows][heads][head_dim] of dtype F32 (K and V exact, q and the probabilities to 22
+ * bits) or F16 (probabilities rounded to binary16); head_dim 64 or 128; out may be
+ * q. A row of q with an infinity or NaN gives NaN; a NaN block reaches the rows that
+ * see it, all dims of the head where it is K's, its 32 where it is V's. Split
+ * partials go into the context's attention workspace (janus_set_stream): a first call
+ * of a shape outside any capture makes it large enough. */
+int janus_fp4_attention(janus_ctx *ctx, const void *q, int dtype, const void *k_cache, const void *k_scales,
+                        const void *v_cache, const void *v_scales, void *out, uint32_t rows, uint32_t nseq, uint32_t heads,
+                        uint32_t kv_heads, uint32_t head_dim, uint32_t cache_rows, uint32_t max_seq_len,
+                        const int32_t *d_q_start, const int32_t *d_row_base, const int32_t *d_seq_lens,
+                        uint32_t max_len_hint, float scale);
+
+/* ---- beam search ----------------------------------------------------------- */
+/* No counterpart in the reference. The n best continuations of each of `batch` requests
+ * with `beams` beams: token t of beam b has the value
+ *   scores[b] + (logits[b][t] - log sum_u exp(logits[b][u])),
+ * and d_out_scores, d_out_parents (the beam, 0 .. beams - 1) and d_out_tokens, all
+ * [batch][n], receive the n largest in descending order, equal ones by beam and then token.
+ * Values are compared in binary64 (within a beam by the logit) and returned as
+ * binary32. logits: [batch][beams][vocab], d_scores: [batch][beams] or NULL for zeros.
+ * A beam with the score -infinity has ended (or not begun: set all but one so at the
+ * first step): all its values are -infinity and its logits are not read. A beam whose
+ * logits are all -infinity likewise; one with a NaN or +infinity among its logits, or as
+ * its score, has NaN for all its values, which comes before every number, so that it is
+ * seen. 1 to 64 beams, n 1 to 64 and at most beams * vocab, beams * vocab below 2^31.
+ * Partials go into the context's GEMM workspace (janus_set_stream). */
+int janus_beam_select(janus_ctx *ctx, const float *logits, const float *d_scores, float *d_out_scores,
+                      int32_t *d_out_parents, int32_t *d_out_tokens, uint32_t batch, uint32_t beams, uint32_t vocab,
+                      uint32_t n);
+/* Lets every beam of `groups` requests go on from its parent, in place, for up to
+ * JANUS_REORDER_BUFFERS buffers (host array of device pointers: K and V, their scales)
+ * of [layers][cache_rows] rows of row_bytes[i] bytes: the first len rows of slot i of a
+ * request, at row_base[i], become those that its slot parents[i] held before the call.
+ * d_row_base and d_parents: [groups][beams], parents counted within the request;
+ * len = d_seq_lens[i] ([groups][beams], NULL: max_seq_len), at most max_seq_len and
+ * what lies inside the cache. A slot whose parent is itself, or outside [0, beams),
+ * or whose row base or its parent's is negative, stays. Slots must not overlap. Forks as
+ * well (all parents 0) and moves. 1 to 32 beams. */
+#define JANUS_REORDER_BUFFERS 8
+int janus_kv_reorder(janus_ctx *ctx, uint32_t n_buffers, void *const *buffers, const uint64_t *row_bytes, uint32_t layers,
+                     uint32_t groups, uint32_t beams, uint32_t cache_rows, uint32_t max_seq_len, const int32_t *d_row_base,
+                     const int32_t *d_parents, const int32_t *d_seq_lens);
+
 /* ---- embedding (model/transformer/embedding.rs:16-198) ---------------- */
 /* out[b][:] = table[ids[b]][:] decoded as the table's binary16 values.
  * h_ids are host token ids checked against the vocabulary. */

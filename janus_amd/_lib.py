@@ -104,6 +104,11 @@ _SIGNATURES = {
                                  U32, U32, P, P]),
     "janus_prompt_attention": (I32, [P, P, I32, P, P, I32, P, U32, U32, U32, U32, U32, U32, P, P, P, U32, F32]),
     "janus_prefix_attention": (I32, [P, P, I32, P, P, I32, P, U32, U32, U32, U32, U32, U32, U32, U32, P, P, U32, F32]),
+    "janus_kv_update_fp4": (I32, [P, P, P, I32, U32, U32, P, P, P, P, U32, U32, U32, U32, U32, U32, P, P]),
+    "janus_kv_read_fp4": (I32, [P, P, P, P, P, P, P, I32, U32, U32, U32, U32, U32, P]),
+    "janus_fp4_attention": (I32, [P, P, I32, P, P, P, P, P, U32, U32, U32, U32, U32, U32, U32, P, P, P, U32, F32]),
+    "janus_beam_select": (I32, [P, P, P, P, P, P, U32, U32, U32, U32]),
+    "janus_kv_reorder": (I32, [P, U32, P, P, U32, U32, U32, U32, U32, P, P, P]),
     "janus_embed": (I32, [P, P, P, U32, P]),
     "janus_embed_device": (I32, [P, P, P, U32, P]),
     "janus_argmax": (I32, [P, P, P, U32, U32, I32]),

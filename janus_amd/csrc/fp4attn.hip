@@ -1,0 +1,721 @@
+// fp4attn.hip -- causal attention of packed rows over a KV cache of 4-bit values
+// (kvfp4.hip): decode steps, drafted tokens, prompts.
+//
+// The queries of a KV head that read the same K and V are columns of one matrix
+// product: column c of a sequence of n rows is query head c % G of its row c / G (G
+// heads per KV head). A wavefront takes NT tiles of 16 columns and positions 32 at a
+// time, and keeps the running maximum m, the sum l and the output O^T in registers:
+//   S^T = K Q^T (positions x columns), p = 2^(scale log2(e) s - m + bias),
+//   l <- l 2^(m_old - m) + sum p,  O^T <- O^T 2^(m_old - m) + V^T P^T.
+// Every 4-bit value times its power-of-two scale is a binary16 number, so K and V
+// enter the binary16 matrix unit exactly, converted in registers, two values an
+// instruction with the scale applied. Nothing goes through LDS:
+//   K: a lane's bytes of one position lie in one block of 32 dims, and the order of
+//     dims in the sum is free, so 16 (8) consecutive bytes are its operand of the
+//     D / 32 products.
+//   S -> P: the result layout of two score tiles (16 positions each) is the operand
+//     layout of 32 positions, in the order {4g .. 4g + 3, 16 + 4g .. 16 + 4g + 3} of
+//     the lane's group g = lane / 16; V takes its positions in the same order.
+//   V: lane a = lane % 16 loads dims [a D / 16, (a + 1) D / 16) of its eight positions;
+//     product i takes dim i of every lane's, after pairs of positions are put
+//     together (v_perm).
+// A lane's outputs are D / 4 consecutive dims of its column.
+//
+// binary16 rows round P to binary16 (the weights are summed before that); binary32 rows
+// have q, divided by a power of two per column, and P in two binary16 parts (22 bits).
+//
+// A scale byte above 140 is a block of NaN. The loop only notes the largest byte; a
+// wavefront that met one looks its scales up again and sets what saw it: every output of
+// a column whose positions include a NaN of K, the block's dims where it is V's. A row
+// of q with an infinity or NaN gives NaN, as its formula does.
+#include <algorithm>
+#include <cmath>
+
+#include "internal.h"
+
+namespace janus {
+namespace {
+
+typedef _Float16 fh8 __attribute__((ext_vector_type(8)));
+typedef float ff4 __attribute__((ext_vector_type(4)));
+
+struct Fp4Args {
+    const void *q;                        // [rows][heads][D]
+    const uint8_t *kc, *ks, *vc, *vs;     // [cache rows][kv_heads][D / 2] and [D / 32]
+    void *out;                            // [rows][heads][D]
+    float *part, *part_ml;                // split: [task][kv_heads][cols][D] and (m, l)
+    uint32_t *meta;                       // split: [rows * G] (first task, parts | column << 24)
+    const int32_t *q_start, *row_base, *seq_lens;
+    uint32_t rows, nseq, heads, kv_heads, G;
+    uint32_t cache_rows, max_seq;
+    uint32_t cols;                        // columns of a workgroup
+    uint32_t hw, ph;                      // its wavefronts: KV heads x position phases (x columns)
+    uint32_t head_groups, tasks;          // workgroups of a task; most tasks
+    uint32_t target, least;               // split: parts to aim at (0: never), fewest positions of one
+    float scale2;                         // scale * log2(e)
+};
+
+__device__ __forceinline__ float swap16f(float v) {   // value of lane ^ 16
+    const uint32_t u = __float_as_uint(v);
+    auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return __uint_as_float((__lane_id() & 16) ? p[0] : p[1]);
+}
+__device__ __forceinline__ float groups_max(float v) {   // over the four lanes of a column
+    v = fmaxf(v, swap16f(v));
+    return fmaxf(v, swap32(v));
+}
+__device__ __forceinline__ float groups_sum(float v) {
+    v += swap16f(v);
+    return v + swap32(v);
+}
+__device__ __forceinline__ uint32_t groups_umax(uint32_t v) {
+    v = max(v, __float_as_uint(swap16f(__uint_as_float(v))));
+    return max(v, __float_as_uint(swap32(__uint_as_float(v))));
+}
+
+// What a sequence is, whatever the tables hold: rows inside [0, rows), positions inside the cache.
+struct SeqRows {
+    uint32_t row0, n;    // its rows
+    uint32_t avail;      // positions that its last row sees
+    int64_t first;       // positions that row 0 sees (may be below 1)
+    int64_t base;        // cache row of position 0
+};
+__device__ __forceinline__ SeqRows seq_rows(const Fp4Args &a, uint32_t s) {
+    SeqRows q{};
+    if (s >= a.nseq) return q;
+    int64_t r0, r1;
+    if (a.q_start) {
+        r0 = a.q_start[s];
+        r1 = a.q_start[s + 1];
+    } else {
+        const uint32_t each = a.rows / a.nseq;
+        r0 = (int64_t)s * each;
+        r1 = r0 + each;
+    }
+    r0 = min(max(r0, (int64_t)0), (int64_t)a.rows);
+    r1 = min(max(r1, r0), (int64_t)a.rows);
+    q.row0 = (uint32_t)r0;
+    q.n = (uint32_t)(r1 - r0);
+    const int64_t len = a.seq_lens ? (int64_t)a.seq_lens[s] : (int64_t)q.n;
+    q.base = a.row_base ? (int64_t)a.row_base[s] : (int64_t)s * a.max_seq;
+    q.first = len - q.n + 1;
+    int64_t avail = min(len, (int64_t)a.max_seq);
+    avail = q.base < 0 ? 0 : min(avail, (int64_t)a.cache_rows - q.base);
+    q.avail = (uint32_t)max(avail, (int64_t)0);
+    return q;
+}
+
+template <typename T> __device__ __forceinline__ T wave_scan(T v) {   // sum over the lanes up to this one
+    const uint32_t lane = threadIdx.x & 63u;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const T u = __shfl_up(v, o, 64);
+        if (lane >= (uint32_t)o) v += u;
+    }
+    return v;
+}
+
+struct Task {
+    SeqRows s;
+    uint32_t c0;           // first column
+    uint32_t part, parts, chunk;
+    uint32_t first_task;   // of the tile's parts
+};
+
+// Finds what task t is; false past the last one.
+__device__ bool find_task(const Fp4Args &a, uint32_t t, Task &w) {
+    const uint32_t lane = threadIdx.x & 63u;
+    uint32_t chunk = 0xffffffffu;
+    if (a.target) {
+        uint64_t total = 0;   // positions of all tiles
+        for (uint32_t s0 = 0; s0 < a.nseq; s0 += 64) {
+            const SeqRows q = seq_rows(a, s0 + lane);
+            const uint32_t tiles = (uint32_t)(((uint64_t)q.n * a.G + a.cols - 1) / a.cols);
+            total += wave_scan((uint64_t)tiles * q.avail);
+        }
+        total = __shfl(total, 63, 64);
+        const uint64_t step = 32u * a.ph;
+        uint64_t c = (total + a.target - 1) / a.target;
+        c = max((c + step - 1) / step * step, (uint64_t)a.least);
+        chunk = (uint32_t)min(c, (uint64_t)0x80000000u);
+    }
+    uint32_t before = 0;
+    for (uint32_t s0 = 0; s0 < a.nseq; s0 += 64) {
+        const SeqRows q = seq_rows(a, s0 + lane);
+        const uint32_t tiles = (uint32_t)(((uint64_t)q.n * a.G + a.cols - 1) / a.cols);
+        const uint32_t parts = a.target ? max(1u, (uint32_t)(((uint64_t)q.avail + chunk - 1) / chunk)) : 1u;
+        const uint32_t upto = before + wave_scan(tiles * parts);
+        const uint64_t here = __ballot(t < upto);
+        if (here) {
+            const uint32_t at = (uint32_t)__builtin_ctzll(here);
+            const uint32_t s = s0 + at;
+            w.parts = __shfl(parts, at, 64);
+            const uint32_t in = t - (__shfl(upto, at, 64) - __shfl(tiles * parts, at, 64));
+            w.s = seq_rows(a, __builtin_amdgcn_readfirstlane(s));
+            w.part = in % w.parts;
+            w.c0 = in / w.parts * a.cols;
+            w.chunk = chunk;
+            w.first_task = t - w.part;
+            return true;
+        }
+        before = __shfl(upto, 63, 64);
+    }
+    return false;
+}
+
+// Raw bytes of 32 positions of a KV head.
+template <int D> struct Raw {
+    uint32_t k[2][D / 32];
+    uint32_t ks[2], v[8], vs[8];
+};
+
+template <int D> struct Offsets {   // of a lane, from the first of the 32 positions
+    uint32_t k[2], ks[2], v[8], vs[8];
+};
+
+// Offsets of the positions min(i, last) of a tile.
+template <int D> __device__ __forceinline__ void set_offsets(Offsets<D> &o, uint32_t kv_heads, uint32_t last) {
+    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, at = lane & 15u;
+    const uint32_t row = kv_heads * (D / 2), srow = kv_heads * (D / 32);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const uint32_t p = min(at + 16u * t, last);
+        o.k[t] = p * row + g * (D / 8);
+        o.ks[t] = p * srow + g * (D / 8) / 16;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const uint32_t p = min((j >> 2) * 16u + 4u * g + (j & 3), last);
+        o.v[j] = p * row + at * (D / 32);
+        o.vs[j] = p * srow + at * (D / 16) / 32;
+    }
+}
+
+template <int D>
+__device__ __forceinline__ void load_raw(Raw<D> &r, const Offsets<D> &o, const uint8_t *kc, const uint8_t *ks,
+                                         const uint8_t *vc, const uint8_t *vs) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        typedef uint32_t vec __attribute__((ext_vector_type(D / 32)));
+        const vec x = *(const vec *)(kc + o.k[t]);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) r.k[t][i] = x[i];
+        r.ks[t] = ks[o.ks[t]];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        if constexpr (D == 128) r.v[j] = *(const uint32_t *)(vc + o.v[j]);
+        else r.v[j] = *(const uint16_t *)(vc + o.v[j]);
+        r.vs[j] = vs[o.vs[j]];
+    }
+}
+
+__device__ __forceinline__ float scale_of(uint32_t byte) {
+    return __uint_as_float(min(max(byte, 104u), 140u) << 23);
+}
+
+template <int BYTE> __device__ __forceinline__ uint32_t fp4_pair(uint32_t w, float scale) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, BYTE));
+}
+
+__device__ __forceinline__ fh8 h8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __builtin_bit_cast(fh8, make_uint4(a, b, c, d));
+}
+__device__ __forceinline__ uint32_t half_pair(float a, float b) {
+    jh2 h = {(_Float16)a, (_Float16)b};
+    return __builtin_bit_cast(uint32_t, h);
+}
+__device__ __forceinline__ ff4 mfma(fh8 a, fh8 b, ff4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+// Columns of a wavefront.
+template <typename T, int D, int NT> struct Columns {
+    static constexpr int P = sizeof(T) == 4 ? 2 : 1;   // binary16 parts of q and of P
+    // The maximum may grow by kSlack powers of two before anything is rescaled; p, up to
+    // 2^(kBias + kSlack), stays finite in binary16, and small ones normal (in two parts the
+    // second is off by 2^-25 of 2^kBias).
+    static constexpr float kBias = P == 2 ? 13.0f : 7.0f, kSlack = P == 2 ? 2.0f : 8.0f;
+    fh8 q[NT][P][D / 32];
+    float cs[NT];                   // factor from s to the exponent
+    float m[NT], l[NT];
+    ff4 o[NT][D / 16];
+    uint32_t vis[NT];               // positions that the lane's column sees
+    uint32_t bad;                   // bit t: column of tile t has an infinity or NaN in q
+
+    __device__ __forceinline__ void load(const Fp4Args &a, const Task &w, uint32_t c0, uint32_t kvh) {
+        const uint32_t lane = threadIdx.x & 63u, g = lane >> 4;
+        bad = 0;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const uint64_t c = (uint64_t)c0 + t * 16u + (lane & 15u);
+            const uint32_t row = (uint32_t)(c / a.G);
+            const bool there = row < w.s.n;
+            vis[t] = 0;
+            float x[D / 4];
+            uint32_t top = 0;
+            if (there) {
+                vis[t] = (uint32_t)min(max(w.s.first + (int64_t)row, (int64_t)0), (int64_t)w.s.avail);
+                const T *src = (const T *)a.q + ((size_t)(w.s.row0 + row) * a.heads + (size_t)kvh * a.G + (uint32_t)(c % a.G)) * D + g * (D / 4);
+                typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
+#pragma unroll
+                for (int i = 0; i < D / 4; i += 16 / (int)sizeof(T)) {
+                    const vec v = *(const vec *)(src + i);
+#pragma unroll
+                    for (int j = 0; j < 16 / (int)sizeof(T); ++j) x[i + j] = (float)v[j];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < D / 4; ++i) x[i] = 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < D / 4; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+            top = groups_umax(top);
+            if (top >= 0x7f800000u) {
+                bad |= 1u << t;
+                top = 0;
+#pragma unroll
+                for (int i = 0; i < D / 4; ++i) x[i] = 0.0f;
+            }
+            if constexpr (P == 1) {
+                cs[t] = a.scale2;
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i)
+                    q[t][0][i] = h8(half_pair(x[8 * i], x[8 * i + 1]), half_pair(x[8 * i + 2], x[8 * i + 3]),
+                                    half_pair(x[8 * i + 4], x[8 * i + 5]), half_pair(x[8 * i + 6], x[8 * i + 7]));
+            } else {
+                // the column's largest into [2^14, 2^15): the second part of what is 2^-17 of it is subnormal, off by 2^-39 of it
+                const int e = max((int)(top >> 23), 1) - 127 - 14;
+                cs[t] = ldexpf(a.scale2, e);
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) {
+                    fh8 hi, lo;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float y = ldexpf(x[8 * i + j], -e);
+                        hi[j] = (_Float16)y;
+                        lo[j] = (_Float16)(y - (float)hi[j]);
+                    }
+                    q[t][0][i] = hi;
+                    q[t][1][i] = lo;
+                }
+            }
+            cs[t] = fmaxf(cs[t], 1e-37f);   // not 0: it also multiplies -infinity
+            m[t] = -INFINITY;
+            l[t] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) o[t][i] = ff4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+    }
+
+    // 32 positions from p on. masked: some column of the wavefront does not see all of them.
+    __device__ __forceinline__ void step(const Raw<D> &r, uint32_t p, bool masked) {
+        const uint32_t g = (threadIdx.x & 63u) >> 4;
+        ff4 s[NT][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const float sc = scale_of(r.ks[h]);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) s[t][h] = ff4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) {
+                const uint32_t w = r.k[h][i];
+                const fh8 k = h8(fp4_pair<0>(w, sc), fp4_pair<1>(w, sc), fp4_pair<2>(w, sc), fp4_pair<3>(w, sc));
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    if constexpr (P == 2) s[t][h] = mfma(k, q[t][1][i], s[t][h]);
+                    s[t][h] = mfma(k, q[t][0][i], s[t][h]);
+                }
+            }
+        }
+        if (masked) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (p + 16u * h + 4u * g + j >= vis[t]) s[t][h][j] = -INFINITY;
+        }
+        uint32_t pp[NT][P][4];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            float mx = s[t][0][0];
+#pragma unroll
+            for (int j = 1; j < 8; ++j) mx = fmaxf(mx, s[t][j >> 2][j & 3]);
+            mx = groups_max(mx) * cs[t];
+            if (__any(mx > m[t] + kSlack)) {
+                const float now = fmaxf(m[t], mx);
+                const float f = m[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[t] - now);
+                l[t] *= f;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) o[t][i] *= f;
+                m[t] = now;
+            }
+            const float off = m[t] == -INFINITY ? 0.0f : kBias - m[t];
+            float x[8], sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                x[j] = __builtin_amdgcn_exp2f(fmaf(s[t][j >> 2][j & 3], cs[t], off));
+                sum += x[j];
+            }
+            l[t] += sum;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const _Float16 h0 = (_Float16)x[2 * j], h1 = (_Float16)x[2 * j + 1];
+                pp[t][0][j] = __builtin_bit_cast(uint32_t, jh2{h0, h1});
+                if constexpr (P == 2) pp[t][1][j] = half_pair(x[2 * j] - (float)h0, x[2 * j + 1] - (float)h1);
+            }
+        }
+        float sc[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sc[j] = scale_of(r.vs[j]);
+        auto two = [&](auto byte) {
+            constexpr int B = decltype(byte)::value;
+            uint32_t h[8], lo[4], hi[4];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) h[j] = fp4_pair<B>(r.v[j], sc[j]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                lo[j] = __builtin_amdgcn_perm(h[2 * j + 1], h[2 * j], 0x05040100u);
+                hi[j] = __builtin_amdgcn_perm(h[2 * j + 1], h[2 * j], 0x07060302u);
+            }
+            const fh8 v0 = h8(lo[0], lo[1], lo[2], lo[3]), v1 = h8(hi[0], hi[1], hi[2], hi[3]);
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int u = 0; u < P; ++u) {
+                    const fh8 x = h8(pp[t][u][0], pp[t][u][1], pp[t][u][2], pp[t][u][3]);
+                    o[t][2 * B] = mfma(v0, x, o[t][2 * B]);
+                    o[t][2 * B + 1] = mfma(v1, x, o[t][2 * B + 1]);
+                }
+        };
+        two(std::integral_constant<int, 0>{});
+        two(std::integral_constant<int, 1>{});
+        if constexpr (D == 128) {
+            two(std::integral_constant<int, 2>{});
+            two(std::integral_constant<int, 3>{});
+        }
+    }
+};
+
+// First positions with a NaN block of K (x), and of V in the lane's output dims (y),
+// among 32 positions from each of p, p + step, ... below end.
+template <int D>
+__device__ __forceinline__ uint2 first_nans(const uint8_t *ks, const uint8_t *vs, uint32_t srow, uint32_t p, uint32_t end,
+                                            uint32_t step) {
+    const uint32_t lane = threadIdx.x & 63u, mine = (lane >> 4) * (D / 4) / 32;
+    uint2 at = make_uint2(0xffffffffu, 0xffffffffu);
+    for (; p < end; p += step) {
+        const uint32_t i = p + (lane & 31u);
+        bool kn = false;
+        for (uint32_t b = 0; b < D / 32; ++b) {
+            bool vn = false;
+            if (i < end) {
+                kn |= ks[(size_t)i * srow + b] > 140;
+                vn = vs[(size_t)i * srow + b] > 140;
+            }
+            const uint32_t some = (uint32_t)__ballot(vn);
+            if (some && b == mine) at.y = min(at.y, p + (uint32_t)__builtin_ctz(some));
+        }
+        const uint32_t some = (uint32_t)__ballot(kn);
+        if (some) at.x = min(at.x, p + (uint32_t)__builtin_ctz(some));
+    }
+    return at;
+}
+
+template <typename T, int D, int NT, int NW, int MINB>
+__global__ __launch_bounds__(NW * 64, MINB) void fp4_attn_kernel(Fp4Args a) {
+    constexpr uint32_t DL = D / 4;   // output dims of a lane
+    extern __shared__ float lds[];
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
+    // the head groups of a task one behind the other on one XCD (workgroup b runs on XCD b % 8): they share lines of the cache
+    const uint32_t j = blockIdx.x >> 3;
+    const uint32_t task = j / a.head_groups * 8u + (blockIdx.x & 7u), hg = j % a.head_groups;
+    Task w;
+    if (task >= a.tasks || !find_task(a, task, w)) return;
+    const uint32_t hwave = wave % a.hw, phase = wave / a.hw % a.ph, cwave = wave / (a.hw * a.ph);
+    const uint32_t kvh = hg * a.hw + hwave;
+    const uint32_t c0 = w.c0 + cwave * (16u * NT);
+    const uint32_t columns = w.s.n * a.G;   // below 2^25
+
+    Columns<T, D, NT> col;
+    col.load(a, w, c0, kvh);
+    uint32_t most = 0, fewest = 0xffffffffu;   // positions that columns of the wavefront see
+    if (c0 < columns) {
+        const uint32_t last = (min(c0 + 16u * NT, columns) - 1) / a.G;
+        most = (uint32_t)min(max(w.s.first + (int64_t)last, (int64_t)0), (int64_t)w.s.avail);
+        fewest = (uint32_t)min(max(w.s.first + (int64_t)(c0 / a.G), (int64_t)0), (int64_t)w.s.avail);
+    }
+    const uint64_t from = (uint64_t)w.part * (w.parts > 1 ? w.chunk : 0);
+    const uint32_t end = __builtin_amdgcn_readfirstlane((uint32_t)min((uint64_t)most, w.parts > 1 ? from + w.chunk : (uint64_t)most));
+    uint32_t p = __builtin_amdgcn_readfirstlane((uint32_t)min(from, (uint64_t)0xffffffc0u)) + 32u * phase;
+    const uint32_t step = 32u * a.ph;
+    const size_t row = (size_t)a.kv_heads * (D / 2), srow = (size_t)a.kv_heads * (D / 32);
+    const size_t base = (size_t)w.s.base;   // used where there are positions: not negative then
+    const uint8_t *kc = a.kc + base * row + kvh * (D / 2), *ks = a.ks + base * srow + kvh * (D / 32);
+    const uint8_t *vc = a.vc + base * row + kvh * (D / 2), *vs = a.vs + base * srow + kvh * (D / 32);
+    if (p < end) {
+        Offsets<D> off;
+        set_offsets<D>(off, a.kv_heads, min(31u, end - 1 - p));
+        Raw<D> now, next;
+        uint32_t worst = 0;
+        load_raw<D>(now, off, kc + p * row, ks + p * srow, vc + p * row, vs + p * srow);
+        const uint32_t p0 = p;
+        for (;;) {
+            const uint32_t ahead = p + step;
+            const bool more = ahead < end;
+            if (more) {
+                if (end - ahead < 32u) set_offsets<D>(off, a.kv_heads, end - 1 - ahead);
+                load_raw<D>(next, off, kc + ahead * row, ks + ahead * srow, vc + ahead * row, vs + ahead * srow);
+            }
+            worst = max(worst, max(now.ks[0], now.ks[1]));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) worst = max(worst, now.vs[i]);
+            col.step(now, p, p + 32u > fewest || p + 32u > end);
+            if (!more) break;
+            now = next;
+            p = ahead;
+        }
+        if (__any(worst > 140u)) {
+            const uint2 at = first_nans<D>(ks, vs, (uint32_t)srow, p0, end, step);
+            const float nan = __uint_as_float(0x7fc00000u);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                if (at.x < col.vis[t]) col.l[t] = nan;
+                if (at.y < col.vis[t])
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) col.o[t][i] = ff4{nan, nan, nan, nan};
+            }
+        }
+    }
+
+    // the phases of a head and column tile join in its first one
+#pragma unroll
+    for (int t = 0; t < NT; ++t) col.l[t] = groups_sum(col.l[t]);
+    if (a.ph > 1) {
+        constexpr uint32_t kArea = NT * (D / 4 + 2) * 64u;   // floats of a wavefront
+        float *mine = lds + ((phase - 1) * a.hw + hwave) * kArea;
+        if (phase > 0) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                float *at = mine + t * (D / 4 + 2) * 64u + lane;
+                at[0] = col.m[t];
+                at[64] = col.l[t];
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) at[(2 + 4 * i + r) * 64] = col.o[t][i][r];
+            }
+        }
+        __syncthreads();
+        if (phase > 0) return;
+        for (uint32_t h = 1; h < a.ph; ++h) {
+            const float *other = lds + ((h - 1) * a.hw + hwave) * kArea + lane;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const float *at = other + t * (D / 4 + 2) * 64u;
+                const float m2 = at[0], now = fmaxf(col.m[t], m2);
+                const float f1 = col.m[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(col.m[t] - now);
+                const float f2 = m2 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m2 - now);
+                // what has seen nothing is 0, or NaN where a block was marked
+                col.l[t] = col.l[t] * f1 + at[64] * f2;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) col.o[t][i][r] = col.o[t][i][r] * f1 + at[(2 + 4 * i + r) * 64] * f2;
+                col.m[t] = now;
+            }
+        }
+    }
+    const uint32_t g = lane >> 4;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const uint32_t c = c0 + t * 16u + (lane & 15u);
+        if (c >= columns) continue;
+        const uint32_t r = c / a.G, gh = c % a.G;
+        if ((col.bad >> t & 1u) && col.vis[t]) col.l[t] = __uint_as_float(0x7fc00000u);
+        if (w.parts > 1) {
+            const size_t at = ((size_t)task * a.kv_heads + kvh) * a.cols + (c - w.c0);
+            float *to = a.part + at * D + g * DL;
+#pragma unroll
+            for (int rr = 0; rr < 4; ++rr)
+#pragma unroll
+                for (int i = 0; i < D / 16; i += 4)
+                    *(ff4 *)(to + rr * (D / 16) + i) = ff4{col.o[t][i][rr], col.o[t][i + 1][rr], col.o[t][i + 2][rr], col.o[t][i + 3][rr]};
+            if (g == 0) {
+                a.part_ml[2 * at] = col.m[t];
+                a.part_ml[2 * at + 1] = col.l[t];
+            }
+        } else {
+            const float inv = col.vis[t] ? 1.0f / col.l[t] : 0.0f;
+            T *to = (T *)a.out + ((size_t)(w.s.row0 + r) * a.heads + (size_t)kvh * a.G + gh) * D + g * DL;
+#pragma unroll
+            for (int rr = 0; rr < 4; ++rr) {
+                typedef T vec __attribute__((ext_vector_type(D / 16 * sizeof(T) > 16 ? 4 : D / 16)));
+                constexpr int N = sizeof(vec) / sizeof(T);
+#pragma unroll
+                for (int i = 0; i < D / 16; i += N) {
+                    vec v;
+#pragma unroll
+                    for (int u = 0; u < N; ++u) v[u] = col.vis[t] ? (T)(col.o[t][i + u][rr] * inv) : (T)0.0f;
+                    *(vec *)(to + rr * (D / 16) + i) = v;
+                }
+            }
+        }
+        if (a.target && w.part == 0 && kvh == 0 && g == 0) {
+            uint32_t *to = a.meta + 2 * ((size_t)w.s.row0 * a.G + c);
+            to[0] = w.first_task;
+            to[1] = w.parts | (c - w.c0) << 24;
+        }
+    }
+}
+
+// One workgroup per row and head: its parts by wavefront, then the wavefronts'.
+template <typename T, int D> __global__ __launch_bounds__(256) void fp4_join_kernel(Fp4Args a) {
+    __shared__ float sm[4], sl[4], so[4][D];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint32_t row = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
+    const uint32_t kvh = head / a.G, gh = head % a.G;
+    uint32_t seq = row / max(1u, a.rows / a.nseq);
+    if (a.q_start) {
+        seq = 0xffffffffu;
+        for (uint32_t s0 = 0; s0 < a.nseq && seq == 0xffffffffu; s0 += 64) {
+            const uint32_t s = s0 + lane;
+            const uint64_t mine = __ballot(s < a.nseq && a.q_start[s] <= (int64_t)row && (int64_t)row < a.q_start[s + 1]);
+            if (mine) seq = s0 + (uint32_t)__builtin_ctzll(mine);
+        }
+        if (seq == 0xffffffffu) return;   // a row of no sequence
+    }
+    const SeqRows of = seq_rows(a, seq);
+    const bool sees = of.avail && of.first + (int64_t)(row - of.row0) > 0;
+    const uint32_t *meta = a.meta + 2 * ((size_t)row * a.G + gh);
+    const uint32_t first = meta[0], parts = meta[1] & 0xffffffu, c = meta[1] >> 24;
+    if (parts < 2 || (uint64_t)first + parts > a.tasks || c >= a.cols) return;
+    constexpr int E = D / 64;
+    const size_t stride = (size_t)a.kv_heads * a.cols;
+    const size_t at0 = ((size_t)first * a.kv_heads + kvh) * a.cols + c;
+    float m = -INFINITY, l = 0.0f, o[E] = {};
+    for (uint32_t i0 = wave * 8; i0 < parts; i0 += 32) {
+        float pm[8], pl[8], po[8][E];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const bool there = i0 + i < parts;
+            const size_t at = at0 + (size_t)(there ? i0 + i : i0) * stride;
+            pm[i] = there ? a.part_ml[2 * at] : -INFINITY;
+            pl[i] = there ? a.part_ml[2 * at + 1] : 0.0f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) po[i][e] = there ? a.part[at * D + lane * E + e] : 0.0f;
+        }
+        float now = m;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) now = fmaxf(now, pm[i]);
+        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - now);
+        l *= f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] *= f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float fi = pm[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(pm[i] - now);
+            l += pl[i] * fi;
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] += po[i][e] * fi;
+        }
+        m = now;
+    }
+    if (lane == 0) {
+        sm[wave] = m;
+        sl[wave] = l;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) so[wave][lane * E + e] = o[e];
+    __syncthreads();
+    if (threadIdx.x >= D) return;
+    const float now = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+    float total = 0.0f, sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float f = sm[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm[i] - now);
+        total += sl[i] * f;
+        sum += so[i][threadIdx.x] * f;
+    }
+    ((T *)a.out)[((size_t)row * a.heads + head) * D + threadIdx.x] = sees ? (T)(sum / total) : (T)0.0f;
+}
+
+template <typename T, int D, int NT, int NW, int MINB> int launch_attn(janus_ctx *ctx, const Fp4Args &a) {
+    const uint32_t lds = (a.ph - 1) * a.hw * NT * (D / 4 + 2) * 64u * 4u;
+    const uint64_t blocks = (uint64_t)(a.tasks + 7) / 8 * 8 * a.head_groups;
+    if (blocks * (NW * 64) >= (1ull << 32)) return fail(ctx, JANUS_E_INVALID_DIM, "fp4_attention: more workgroups than one launch takes");
+    hipLaunchKernelGGL((fp4_attn_kernel<T, D, NT, NW, MINB>), dim3((uint32_t)blocks), dim3(NW * 64), lds, ctx->stream, a);
+    JANUS_LAUNCH_CHECK(ctx);
+    if (a.target) {
+        hipLaunchKernelGGL((fp4_join_kernel<T, D>), dim3(a.rows * a.heads), dim3(256), 0, ctx->stream, a);
+        JANUS_LAUNCH_CHECK(ctx);
+    }
+    return JANUS_OK;
+}
+
+template <typename T, int D> int launch_dim(janus_ctx *ctx, Fp4Args &a, uint32_t max_len) {
+    const uint32_t mean = (a.rows + a.nseq - 1) / a.nseq;   // rows of a sequence
+    const bool few = (uint64_t)mean * a.G <= 16;
+    if (few) {
+        a.cols = 16;
+        a.hw = a.kv_heads % 8 == 0 ? 8 : a.kv_heads % 4 == 0 ? 4 : a.kv_heads % 2 == 0 ? 2 : 1;
+        a.ph = 8 / a.hw;
+    } else {
+        a.cols = 4 * 16 * 2;
+        a.hw = a.ph = 1;
+    }
+    a.head_groups = a.kv_heads / a.hw;
+    // every tile of every sequence, one more where rows do not fill the last
+    const uint64_t tiles = (uint64_t)a.rows * a.G / a.cols + a.nseq;
+    const uint64_t want = (uint64_t)ctx->num_cus * 2 / a.head_groups;
+    a.least = 32 * a.ph;
+    a.target = 0;
+    uint64_t tasks = tiles;
+    const uint64_t busy = std::min<uint64_t>(tiles, ((uint64_t)a.rows * a.G + a.cols - 1) / a.cols + a.nseq - 1);
+    if (max_len > 4 * a.least && busy * 2 < want * 3) {
+        a.target = (uint32_t)std::max<uint64_t>(want, 1);
+        tasks += a.target;
+    }
+    if (tasks >= (1u << 23)) return fail(ctx, JANUS_E_INVALID_DIM, "fp4_attention: more tiles than one launch takes");
+    a.tasks = (uint32_t)tasks;
+    if (a.target) {
+        const size_t cells = (size_t)a.tasks * a.kv_heads * a.cols;
+        const size_t meta = ((size_t)a.rows * a.G * 8 + 255) / 256 * 256;
+        if (int e = ensure_attn_ws(ctx, meta + cells * (D + 2) * 4)) return e;
+        a.meta = (uint32_t *)ctx->attn_ws;
+        a.part = (float *)((char *)ctx->attn_ws + meta);
+        a.part_ml = a.part + cells * D;
+    }
+    if (few) return launch_attn<T, D, 1, 8, 2>(ctx, a);
+    return launch_attn<T, D, 2, 4, 1>(ctx, a);
+}
+
+}  // namespace
+
+int fp4_attention_launch(janus_ctx *ctx, const void *q, int q_dt, const uint8_t *kc, const uint8_t *ks,
+                         const uint8_t *vc, const uint8_t *vs, void *out, uint32_t rows, uint32_t nseq, uint32_t heads,
+                         uint32_t kv_heads, uint32_t hd, uint32_t cache_rows, uint32_t max_seq, const int32_t *q_start,
+                         const int32_t *row_base, const int32_t *seq_lens, uint32_t max_len, float scale) {
+    Fp4Args a{};
+    a.q = q;
+    a.kc = kc;
+    a.ks = ks;
+    a.vc = vc;
+    a.vs = vs;
+    a.out = out;
+    a.q_start = q_start;
+    a.row_base = row_base;
+    a.seq_lens = seq_lens;
+    a.rows = rows;
+    a.nseq = nseq;
+    a.heads = heads;
+    a.kv_heads = kv_heads;
+    a.G = heads / kv_heads;
+    a.cache_rows = cache_rows;
+    a.max_seq = max_seq;
+    a.scale2 = scale * 1.44269504088896340736f;
+    if (q_dt == JANUS_DT_F16) return hd == 128 ? launch_dim<_Float16, 128>(ctx, a, max_len) : launch_dim<_Float16, 64>(ctx, a, max_len);
+    return hd == 128 ? launch_dim<float, 128>(ctx, a, max_len) : launch_dim<float, 64>(ctx, a, max_len);
+}
+
+}  // namespace janus

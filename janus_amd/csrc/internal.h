@@ -291,6 +291,26 @@ int qk_norm_rope_launch(janus_ctx *ctx, const void *q, const void *k, const void
                         const float *table, void *q_out, int out_dt, void *kc, void *vc, int kv_dt, uint32_t rows,
                         uint32_t heads, uint32_t kv_heads, uint32_t hd, uint32_t position, uint32_t max_seq,
                         const int32_t *row_base, const int32_t *positions);
+// K and V rows of in_dt into a 4-bit cache, and cache rows back as out_dt (kvfp4.hip).
+int kv_update_fp4_launch(janus_ctx *ctx, const void *k, const void *v, int in_dt, uint32_t k_stride, uint32_t v_stride,
+                         uint8_t *kc, uint8_t *ks, uint8_t *vc, uint8_t *vs, uint32_t rows, uint32_t kv_heads,
+                         uint32_t hd, uint32_t cache_rows, uint32_t position, uint32_t max_seq,
+                         const int32_t *row_base, const int32_t *positions);
+int kv_read_fp4_launch(janus_ctx *ctx, const uint8_t *kc, const uint8_t *ks, const uint8_t *vc, const uint8_t *vs,
+                       void *k_out, void *v_out, int out_dt, uint32_t rows, uint32_t kv_heads, uint32_t hd,
+                       uint32_t cache_rows, uint32_t first_row, const int32_t *d_rows);
+// Causal attention of packed rows over a 4-bit cache (fp4attn.hip); otherwise as prompt_attention_launch.
+int fp4_attention_launch(janus_ctx *ctx, const void *q, int q_dt, const uint8_t *kc, const uint8_t *ks,
+                         const uint8_t *vc, const uint8_t *vs, void *out, uint32_t rows, uint32_t nseq, uint32_t heads,
+                         uint32_t kv_heads, uint32_t hd, uint32_t cache_rows, uint32_t max_seq, const int32_t *q_start,
+                         const int32_t *row_base, const int32_t *seq_lens, uint32_t max_len, float scale);
+// Beam search (beam.hip): the n best continuations of each request's beams (partials go into the GEMM workspace, grown
+// on demand), and the permutation of the beams' cache rows.
+int beam_select_launch(janus_ctx *ctx, const float *logits, const float *scores, float *out, int32_t *parents,
+                       int32_t *tokens, uint32_t batch, uint32_t beams, uint32_t vocab, uint32_t n);
+int kv_reorder_launch(janus_ctx *ctx, uint32_t bufs, void *const *buf, const uint64_t *row_bytes, uint32_t layers,
+                      uint32_t groups, uint32_t beams, uint32_t cache_rows, uint32_t max_seq, const int32_t *row_base,
+                      const int32_t *parents, const int32_t *seq_lens);
 // Looks up, once per device, the device address of the fixed attention
 // scratch (kAttnScratchBytes) and stores it in ctx->attn_scratch. Called by
 // janus_create with the context's device current.

@@ -289,6 +289,141 @@ int janus_qk_norm_rope(janus_ctx *ctx, const void *q, const void *k, const void 
                                max_seq_len, d_row_base, d_positions);
 }
 
+namespace {
+// Host checks of a 4-bit cache's buffers and sizes.
+int fp4_args(janus_ctx *ctx, const char *name, const void *k_cache, const void *k_scales, const void *v_cache,
+             const void *v_scales, uint32_t kv_heads, uint32_t hd, uint32_t cache_rows) {
+    auto no = [&](int code, const char *why) { return fail(ctx, code, std::string(name) + ": " + why); };
+    if (!k_cache || !k_scales || !v_cache || !v_scales) return no(JANUS_E_INVALID_ARG, "null buffer");
+    if ((((uintptr_t)k_cache | (uintptr_t)v_cache) & 15u) || (((uintptr_t)k_scales | (uintptr_t)v_scales) & 3u))
+        return no(JANUS_E_INVALID_ARG, "values must be 16-byte and scales 4-byte aligned");
+    if (hd == 0 || hd % 32 || hd > 1024) return no(JANUS_E_INVALID_DIM, "head_dim must be a multiple of 32, at most 1024");
+    if (kv_heads == 0 || kv_heads > 65536u) return no(JANUS_E_INVALID_DIM, "1 to 65536 heads");
+    if (cache_rows > 0x80000000u) return no(JANUS_E_INVALID_DIM, "a cache beyond 2^31 rows");
+    return JANUS_OK;
+}
+bool fp4_fits(uint32_t rows, uint32_t kv_heads, uint32_t hd) {   // one launch takes fewer than 2^32 lanes, 8 values each
+    const uint64_t lanes = ((uint64_t)2 * kv_heads * (hd / 8) + 255) / 256 * 256;
+    return rows * lanes < (1ull << 32);
+}
+}  // namespace
+
+int janus_kv_update_fp4(janus_ctx *ctx, const void *k, const void *v, int in_dt, uint32_t k_stride, uint32_t v_stride,
+                        void *k_cache, void *k_scales, void *v_cache, void *v_scales, uint32_t rows, uint32_t kv_heads,
+                        uint32_t hd, uint32_t cache_rows, uint32_t position, uint32_t max_seq_len,
+                        const int32_t *d_row_base, const int32_t *d_positions) {
+    if (check_ctx(ctx)) return JANUS_E_INVALID_ARG;
+    if (!k || !v) return fail(ctx, JANUS_E_INVALID_ARG, "kv_update_fp4: null buffer");
+    if (!is_act_dtype(in_dt)) return fail(ctx, JANUS_E_UNSUPPORTED_DTYPE, "kv_update_fp4: rows must be F32 or F16");
+    if (int e = fp4_args(ctx, "kv_update_fp4", k_cache, k_scales, v_cache, v_scales, kv_heads, hd, cache_rows)) return e;
+    if (((uintptr_t)k | (uintptr_t)v) % act_bytes(in_dt))
+        return fail(ctx, JANUS_E_INVALID_ARG, "kv_update_fp4: rows must be aligned to their type");
+    if (!k_stride) k_stride = kv_heads * hd;
+    if (!v_stride) v_stride = kv_heads * hd;
+    if (k_stride < kv_heads * hd || v_stride < kv_heads * hd)
+        return fail(ctx, JANUS_E_INVALID_DIM, "kv_update_fp4: a row stride is shorter than the row");
+    if (!d_positions && position >= max_seq_len)
+        return fail(ctx, JANUS_E_KV_OVERFLOW, "KV cache position " + std::to_string(position) +
+                                                  " exceeds max_seq_len " + std::to_string(max_seq_len));
+    if (rows == 0 || cache_rows == 0) return JANUS_OK;
+    if (!fp4_fits(rows, kv_heads, hd))
+        return fail(ctx, JANUS_E_INVALID_DIM, "kv_update_fp4: more rows than one launch takes");
+    if (int e = need_device(ctx)) return e;
+    DeviceGuard g(ctx->device);
+    return kv_update_fp4_launch(ctx, k, v, in_dt, k_stride, v_stride, (uint8_t *)k_cache, (uint8_t *)k_scales,
+                                (uint8_t *)v_cache, (uint8_t *)v_scales, rows, kv_heads, hd, cache_rows, position,
+                                max_seq_len, d_row_base, d_positions);
+}
+
+int janus_kv_read_fp4(janus_ctx *ctx, const void *k_cache, const void *k_scales, const void *v_cache,
+                      const void *v_scales, void *k_out, void *v_out, int out_dt, uint32_t rows, uint32_t kv_heads,
+                      uint32_t hd, uint32_t cache_rows, uint32_t first_row, const int32_t *d_rows) {
+    if (check_ctx(ctx)) return JANUS_E_INVALID_ARG;
+    if (!k_out || !v_out) return fail(ctx, JANUS_E_INVALID_ARG, "kv_read_fp4: null buffer");
+    if (((uintptr_t)k_out | (uintptr_t)v_out) & 15u)
+        return fail(ctx, JANUS_E_INVALID_ARG, "kv_read_fp4: the outputs must be 16-byte aligned");
+    if (!is_act_dtype(out_dt)) return fail(ctx, JANUS_E_UNSUPPORTED_DTYPE, "kv_read_fp4: outputs must be F32 or F16");
+    if (int e = fp4_args(ctx, "kv_read_fp4", k_cache, k_scales, v_cache, v_scales, kv_heads, hd, cache_rows)) return e;
+    if (!d_rows && (uint64_t)first_row + rows > cache_rows)
+        return fail(ctx, JANUS_E_KV_OVERFLOW, "kv_read_fp4: rows beyond the cache");
+    if (rows == 0 || cache_rows == 0) return JANUS_OK;
+    if (!fp4_fits(rows, kv_heads, hd)) return fail(ctx, JANUS_E_INVALID_DIM, "kv_read_fp4: more rows than one launch takes");
+    if (int e = need_device(ctx)) return e;
+    DeviceGuard g(ctx->device);
+    return kv_read_fp4_launch(ctx, (const uint8_t *)k_cache, (const uint8_t *)k_scales, (const uint8_t *)v_cache,
+                              (const uint8_t *)v_scales, k_out, v_out, out_dt, rows, kv_heads, hd, cache_rows, first_row,
+                              d_rows);
+}
+
+int janus_fp4_attention(janus_ctx *ctx, const void *q, int q_dt, const void *k_cache, const void *k_scales,
+                        const void *v_cache, const void *v_scales, void *out, uint32_t rows, uint32_t nseq,
+                        uint32_t heads, uint32_t kv_heads, uint32_t hd, uint32_t cache_rows, uint32_t max_seq_len,
+                        const int32_t *d_q_start, const int32_t *d_row_base, const int32_t *d_seq_lens,
+                        uint32_t max_len_hint, float scale) {
+    if (check_ctx(ctx)) return JANUS_E_INVALID_ARG;
+    if (int e = fp4_args(ctx, "fp4_attention", k_cache, k_scales, v_cache, v_scales, kv_heads, hd, cache_rows)) return e;
+    if (int e = packed_args(ctx, "fp4_attention", q, q_dt, k_cache, v_cache, JANUS_DT_F16, out, rows, nseq, heads,
+                            kv_heads, hd))
+        return e;
+    if (rows == 0 || nseq == 0) return JANUS_OK;
+    if (!d_q_start && rows % nseq)
+        return fail(ctx, JANUS_E_INVALID_DIM, "fp4_attention: without q_start, rows must be a multiple of nseq");
+    if (!d_q_start && !d_seq_lens && rows / nseq > max_seq_len)
+        return fail(ctx, JANUS_E_KV_OVERFLOW, "fp4_attention: rows of a sequence exceed max_seq_len");
+    if (int e = need_device(ctx)) return e;
+    DeviceGuard g(ctx->device);
+    if (!(scale > 0.0f)) scale = 1.0f / sqrtf((float)hd);
+    return fp4_attention_launch(ctx, q, q_dt, (const uint8_t *)k_cache, (const uint8_t *)k_scales,
+                                (const uint8_t *)v_cache, (const uint8_t *)v_scales, out, rows, nseq, heads, kv_heads,
+                                hd, cache_rows, max_seq_len, d_q_start, d_row_base, d_seq_lens,
+                                max_len_hint ? max_len_hint : max_seq_len, scale);
+}
+
+int janus_beam_select(janus_ctx *ctx, const float *logits, const float *d_scores, float *d_out_scores,
+                      int32_t *d_out_parents, int32_t *d_out_tokens, uint32_t batch, uint32_t beams, uint32_t vocab,
+                      uint32_t n) {
+    if (check_ctx(ctx)) return JANUS_E_INVALID_ARG;
+    if (!logits || !d_out_scores || !d_out_parents || !d_out_tokens)
+        return fail(ctx, JANUS_E_INVALID_ARG, "beam_select: null buffer");
+    if (beams == 0 || beams > 64) return fail(ctx, JANUS_E_INVALID_DIM, "beam_select: 1 to 64 beams");
+    if (vocab == 0 || (uint64_t)beams * vocab >= (1ull << 31))
+        return fail(ctx, JANUS_E_INVALID_DIM, "beam_select: beams * vocab must be 1 to 2^31 - 1");
+    if (n == 0 || n > 64 || n > (uint64_t)beams * vocab)
+        return fail(ctx, JANUS_E_INVALID_DIM, "beam_select: n must be 1 to 64, at most beams * vocab");
+    if (batch == 0) return JANUS_OK;
+    // a workgroup of 256 lanes for each 8192 logits of a row
+    if ((uint64_t)batch * beams * ((vocab + 8191u) / 8192u) >= (1ull << 24))
+        return fail(ctx, JANUS_E_INVALID_DIM, "beam_select: more logits than one launch takes");
+    if (int e = need_device(ctx)) return e;
+    DeviceGuard g(ctx->device);
+    return beam_select_launch(ctx, logits, d_scores, d_out_scores, d_out_parents, d_out_tokens, batch, beams, vocab, n);
+}
+
+int janus_kv_reorder(janus_ctx *ctx, uint32_t n_buffers, void *const *buffers, const uint64_t *row_bytes,
+                     uint32_t layers, uint32_t groups, uint32_t beams, uint32_t cache_rows, uint32_t max_seq_len,
+                     const int32_t *d_row_base, const int32_t *d_parents, const int32_t *d_seq_lens) {
+    if (check_ctx(ctx)) return JANUS_E_INVALID_ARG;
+    if (n_buffers > JANUS_REORDER_BUFFERS) return fail(ctx, JANUS_E_INVALID_DIM, "kv_reorder: too many buffers");
+    if (n_buffers && (!buffers || !row_bytes)) return fail(ctx, JANUS_E_INVALID_ARG, "kv_reorder: null buffer list");
+    for (uint32_t i = 0; i < n_buffers; ++i) {
+        if (!buffers[i]) return fail(ctx, JANUS_E_INVALID_ARG, "kv_reorder: null buffer");
+        if (row_bytes[i] == 0 || row_bytes[i] > (1ull << 30))
+            return fail(ctx, JANUS_E_INVALID_DIM, "kv_reorder: rows of 1 byte to 2^30");
+    }
+    if (!d_row_base || !d_parents) return fail(ctx, JANUS_E_INVALID_ARG, "kv_reorder: null table");
+    if (beams == 0 || beams > 32) return fail(ctx, JANUS_E_INVALID_DIM, "kv_reorder: 1 to 32 beams");
+    if (cache_rows > 0x80000000u) return fail(ctx, JANUS_E_INVALID_DIM, "kv_reorder: a cache beyond 2^31 rows");
+    if (n_buffers == 0 || layers == 0 || groups == 0 || beams == 1 || cache_rows == 0 || max_seq_len == 0) return JANUS_OK;
+    // a workgroup of 256 lanes at least for each layer, buffer and group
+    if ((uint64_t)groups * beams >= (1ull << 31) || (uint64_t)layers * n_buffers >= (1ull << 24) ||
+        (uint64_t)layers * n_buffers * groups >= (1ull << 24))
+        return fail(ctx, JANUS_E_INVALID_DIM, "kv_reorder: more layers and groups than one launch takes");
+    if (int e = need_device(ctx)) return e;
+    DeviceGuard g(ctx->device);
+    return kv_reorder_launch(ctx, n_buffers, buffers, row_bytes, layers, groups, beams, cache_rows, max_seq_len,
+                             d_row_base, d_parents, d_seq_lens);
+}
+
 int janus_embed(janus_ctx *ctx, const janus_weight *table, const uint32_t *h_ids, uint32_t batch, float *out) {
     if (check_ctx(ctx)) return JANUS_E_INVALID_ARG;
     if (!table || !h_ids || !out) return fail(ctx, JANUS_E_INVALID_ARG, "embed: null argument");

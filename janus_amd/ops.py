@@ -392,6 +392,169 @@ def prefix_attention(engine, query, key_cache, value_cache, output, prefix_row: 
         engine._check(status)
 
 
+# ---- a cache of 4-bit values -----------------------------------------------------------
+
+def _fp4_caches(k_cache, k_scales, v_cache, v_scales, hd, dev: int):
+    """(addresses of K, its scales, V, its scales, rows, kv heads) of one layer's 4-bit
+    caches: values [rows, kv_heads, head_dim / 2] and scales [rows, kv_heads, head_dim / 32]."""
+    shape, u8 = k_cache.shape, torch.uint8
+    if len(shape) != 3 or shape[2] * 2 != hd or v_cache.shape != shape:
+        raise ValueError(f"4-bit caches: [rows, kv_heads, {hd} / 2] expected, got {tuple(shape)} and "
+                         f"{tuple(v_cache.shape)}")
+    scales = (shape[0], shape[1], hd // 32)
+    if k_scales.shape != scales or v_scales.shape != scales:
+        raise ValueError(f"scales: {scales} expected, got {tuple(k_scales.shape)} and {tuple(v_scales.shape)}")
+    if k_cache.dtype is not u8 or k_scales.dtype is not u8 or v_cache.dtype is not u8 or v_scales.dtype is not u8:
+        raise ValueError("4-bit caches and scales: torch.uint8 expected")
+    return (_buf(k_cache, dev, "k_cache"), _buf(k_scales, dev, "k_scales"), _buf(v_cache, dev, "v_cache"),
+            _buf(v_scales, dev, "v_scales"), shape[0], shape[1])
+
+
+def kv_update_fp4(engine, key, value, k_cache, k_scales, v_cache, v_scales, max_seq_len: int, position: int = 0,
+                  row_base: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None) -> None:
+    """Append rows of K and V to a cache of 4-bit values (janus_kv_update_fp4 in
+    include/janus_hip.h). key and value are [rows, kv_heads, head_dim] of float32 or
+    float16, also as parts of one fused product's rows; row r goes to cache row
+    row_base[r] + positions[r] (without row_base r * max_seq_len, without positions
+    `position`). The caches are torch.uint8: values [cache rows, kv_heads, head_dim / 2],
+    scales [cache rows, kv_heads, head_dim / 32]; a cache of zeros holds zeros."""
+    dev = engine.device
+    shape = _three(key, "key")
+    rows, kvh, hd = shape
+    kc, ks, vc, vs, cache_rows, cache_heads = _fp4_caches(k_cache, k_scales, v_cache, v_scales, hd, dev)
+    if value.shape != shape or value.dtype is not key.dtype or cache_heads != kvh:
+        raise ValueError(f"value: {tuple(shape)} of key's type and caches of {kvh} heads expected, got "
+                         f"{tuple(value.shape)} and {cache_heads}")
+    if max_seq_len < 0 or (row_base is None and rows * max_seq_len > cache_rows):
+        raise ValueError("max_seq_len below 0, or without row_base fewer cache rows than max_seq_len for each row")
+    if max_seq_len > _U32 or (positions is None and not 0 <= position <= _U32):
+        raise ValueError("max_seq_len or position beyond 32 bits")
+    i32 = torch.int32
+    status = engine.lib.janus_kv_update_fp4(
+        engine.ctx, key.data_ptr(), value.data_ptr(), _dt(key), _stride(key, rows, kvh, hd, dev, "key"),
+        _stride(value, rows, kvh, hd, dev, "value"), kc, ks, vc, vs, rows, kvh, hd, cache_rows, position, max_seq_len,
+        _table(row_base, i32, rows, dev, "row_base"), _table(positions, i32, rows, dev, "positions"))
+    if status:
+        engine._check(status)
+
+
+def kv_read_fp4(engine, k_cache, k_scales, v_cache, v_scales, k_out, v_out, first_row: int = 0,
+                rows: Optional[torch.Tensor] = None) -> None:
+    """Rows of a 4-bit cache as float32 or float16 values, which hold them exactly
+    (janus_kv_read_fp4 in include/janus_hip.h): k_out and v_out [n, kv_heads, head_dim]
+    receive cache row rows[r], or first_row + r."""
+    dev = engine.device
+    shape = _three(k_out, "k_out")
+    n, kvh, hd = shape
+    kc, ks, vc, vs, cache_rows, cache_heads = _fp4_caches(k_cache, k_scales, v_cache, v_scales, hd, dev)
+    if v_out.shape != shape or v_out.dtype is not k_out.dtype or cache_heads != kvh:
+        raise ValueError(f"v_out: {tuple(shape)} of k_out's type and caches of {kvh} heads expected, got "
+                         f"{tuple(v_out.shape)} and {cache_heads}")
+    if rows is None and not 0 <= first_row <= cache_rows - n:
+        raise ValueError("the rows lie beyond the cache")
+    status = engine.lib.janus_kv_read_fp4(engine.ctx, kc, ks, vc, vs, _buf(k_out, dev, "k_out"),
+                                          _buf(v_out, dev, "v_out"), _dt(k_out), n, kvh, hd, cache_rows,
+                                          first_row if rows is None else 0, _table(rows, torch.int32, n, dev, "rows"))
+    if status:
+        engine._check(status)
+
+
+def fp4_attention(engine, query, k_cache, k_scales, v_cache, v_scales, output, nseq: int, max_seq_len: int,
+                  q_start: Optional[torch.Tensor] = None, row_base: Optional[torch.Tensor] = None,
+                  seq_lens: Optional[torch.Tensor] = None, max_len_hint: int = 0, scale: float = 0.0) -> None:
+    """prompt_attention over a 4-bit cache (janus_fp4_attention in include/janus_hip.h):
+    causal attention of the packed rows of nseq sequences, sequence s with the rows
+    [q_start[s], q_start[s + 1]) of query [rows, heads, head_dim] (rows / nseq each
+    without q_start: a decode step has one), the last of its seq_lens[s] positions,
+    which lie in the cache from row_base[s] on."""
+    dev = engine.device
+    shape = _three(query, "query")
+    rows, heads, hd = shape
+    kc, ks, vc, vs, cache_rows, kvh = _fp4_caches(k_cache, k_scales, v_cache, v_scales, hd, dev)
+    if output.shape != shape or output.dtype is not query.dtype:
+        raise ValueError("output: the query's shape and type expected")
+    if nseq < 0 or max_seq_len < 0 or (row_base is None and nseq * max_seq_len > cache_rows):
+        raise ValueError("nseq or max_seq_len below 0, or without row_base fewer cache rows than max_seq_len for each "
+                         "sequence")
+    if max_seq_len > _U32 or nseq > _U32 or not 0 <= max_len_hint <= _U32:
+        raise ValueError("nseq, max_seq_len or max_len_hint beyond 32 bits")
+    i32 = torch.int32
+    status = engine.lib.janus_fp4_attention(
+        engine.ctx, _buf(query, dev, "query"), _dt(query), kc, ks, vc, vs, _buf(output, dev, "output"), rows, nseq,
+        heads, kvh, hd, cache_rows, max_seq_len, _table(q_start, i32, nseq + 1, dev, "q_start"),
+        _table(row_base, i32, nseq, dev, "row_base"), _table(seq_lens, i32, nseq, dev, "seq_lens"), max_len_hint,
+        scale)
+    if status:
+        engine._check(status)
+
+
+# ---- beam search -------------------------------------------------------------------------
+
+def beam_select(engine, logits, scores, out_scores, out_parents, out_tokens) -> None:
+    """The best continuations of each request's beams (janus_beam_select in
+    include/janus_hip.h). logits [batch * beams, vocab] float32 (or [batch, beams,
+    vocab]), scores [batch, beams] float32; out_scores (float32), out_parents and
+    out_tokens (int32), [batch, n], receive the n largest of scores + log_softmax(logits)
+    of each request in descending order, equal ones by beam, then token. A beam whose score
+    is -infinity has ended."""
+    dev = engine.device
+    if scores.dim() != 2 or out_scores.dim() != 2 or out_scores.shape[0] != scores.shape[0]:
+        raise ValueError(f"scores: [batch, beams] and out_scores: [batch, n] expected, got {tuple(scores.shape)} and "
+                         f"{tuple(out_scores.shape)}")
+    batch, beams = scores.shape
+    n, vocab = out_scores.shape[1], logits.shape[-1] if logits.dim() else 0
+    if logits.numel() != batch * beams * vocab:
+        raise ValueError(f"logits: {batch} x {beams} rows expected, got {tuple(logits.shape)}")
+    if out_parents.shape != out_scores.shape or out_tokens.shape != out_scores.shape:
+        raise ValueError("out_parents and out_tokens: out_scores' shape expected")
+    f32, i32 = torch.float32, torch.int32
+    if logits.dtype is not f32 or scores.dtype is not f32 or out_scores.dtype is not f32 or out_parents.dtype is not i32 \
+            or out_tokens.dtype is not i32:
+        raise ValueError("logits and scores: torch.float32, parents and tokens: torch.int32 expected")
+    status = engine.lib.janus_beam_select(engine.ctx, _buf(logits, dev, "logits"), _buf(scores, dev, "scores"),
+                                          _buf(out_scores, dev, "out_scores"), _buf(out_parents, dev, "out_parents"),
+                                          _buf(out_tokens, dev, "out_tokens"), batch, beams, vocab, n)
+    if status:
+        engine._check(status)
+
+
+def kv_reorder(engine, caches: Sequence[torch.Tensor], beams: int, max_seq_len: int, row_base: torch.Tensor,
+               parents: torch.Tensor, seq_lens: Optional[torch.Tensor] = None, layers: int = 0) -> None:
+    """Every beam goes on from its parent, in place (janus_kv_reorder in
+    include/janus_hip.h): slot i of a request, the cache rows from row_base[i] on, takes
+    the first seq_lens[i] (max_seq_len) rows that the request's slot parents[i] held.
+    caches: up to 8 tensors of one number of rows, [rows, ...] or, with `layers`, [layers,
+    rows, ...] (K and V, a 4-bit cache's scales beside them). row_base, parents and
+    seq_lens hold `beams` values for each request, those of a request one behind the
+    other; parents count within the request."""
+    dev, lead = engine.device, 1 if layers else 0
+    if not caches or len(caches) > 8:
+        raise ValueError(f"1 to 8 caches expected, got {len(caches)}")
+    slots = parents.numel()
+    if beams < 1 or layers < 0 or max_seq_len < 0 or slots % beams:
+        raise ValueError("beams below 1, layers or max_seq_len below 0, or parents not of whole requests")
+    if max_seq_len > _U32 or layers > _U32:
+        raise ValueError("max_seq_len or layers beyond 32 bits")
+    rows = caches[0].shape[lead] if caches[0].dim() > lead else 0
+    sizes = []
+    for c in caches:
+        shape = c.shape
+        if len(shape) <= lead or shape[lead] != rows or (lead and shape[0] != layers):
+            raise ValueError(f"caches: {f'[{layers}, {rows}, ...]' if lead else f'[{rows}, ...]'} expected, got {tuple(shape)}")
+        sizes.append(c.numel() * c.element_size() // max(1, rows * (layers or 1)))
+    if not rows:
+        return
+    k = len(caches)
+    bufs = (C.c_void_p * k)(*[_buf(c, dev, "cache") for c in caches])
+    i32 = torch.int32
+    status = engine.lib.janus_kv_reorder(
+        engine.ctx, k, bufs, (C.c_uint64 * k)(*sizes), layers or 1, slots // beams, beams, rows, max_seq_len,
+        _table(row_base, i32, slots, dev, "row_base"), _table(parents, i32, slots, dev, "parents"),
+        _table(seq_lens, i32, slots, dev, "seq_lens"))
+    if status:
+        engine._check(status)
+
+
 # ---- embedding and sampling ---------------------------------------------------------
 
 def embed_tokens(engine, table: GpuTensor, token_ids: Sequence[int], output) -> None:

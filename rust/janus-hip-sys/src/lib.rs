@@ -50,6 +50,7 @@ pub const JANUS_WEIGHT_Q6K_REF_ORDER: u32 = 2;
 pub const JANUS_TIE_LAST: c_int = 0;
 pub const JANUS_TIE_WGSL: c_int = 1;
 pub const JANUS_ATTN_SCRATCH_BYTES: usize = 0x1000000;
+pub const JANUS_REORDER_BUFFERS: u32 = 8;
 pub const JANUS_SAMPLER_ARGMAX: c_int = 0;
 pub const JANUS_SAMPLER_PENALTY: c_int = 1;
 pub const JANUS_SAMPLER_WGSL: c_int = 2;
@@ -316,6 +317,90 @@ unsafe extern "C" {
         d_seq_lens: *const i32,
         max_len_hint: u32,
         scale: c_float,
+    ) -> c_int;
+    pub fn janus_kv_update_fp4(
+        ctx: *mut janus_ctx,
+        k: *const c_void,
+        v: *const c_void,
+        in_dtype: c_int,
+        k_stride: u32,
+        v_stride: u32,
+        k_cache: *mut c_void,
+        k_scales: *mut c_void,
+        v_cache: *mut c_void,
+        v_scales: *mut c_void,
+        rows: u32,
+        kv_heads: u32,
+        head_dim: u32,
+        cache_rows: u32,
+        position: u32,
+        max_seq_len: u32,
+        d_row_base: *const i32,
+        d_positions: *const i32,
+    ) -> c_int;
+    pub fn janus_kv_read_fp4(
+        ctx: *mut janus_ctx,
+        k_cache: *const c_void,
+        k_scales: *const c_void,
+        v_cache: *const c_void,
+        v_scales: *const c_void,
+        k_out: *mut c_void,
+        v_out: *mut c_void,
+        out_dtype: c_int,
+        rows: u32,
+        kv_heads: u32,
+        head_dim: u32,
+        cache_rows: u32,
+        first_row: u32,
+        d_rows: *const i32,
+    ) -> c_int;
+    pub fn janus_fp4_attention(
+        ctx: *mut janus_ctx,
+        q: *const c_void,
+        dtype: c_int,
+        k_cache: *const c_void,
+        k_scales: *const c_void,
+        v_cache: *const c_void,
+        v_scales: *const c_void,
+        out: *mut c_void,
+        rows: u32,
+        nseq: u32,
+        heads: u32,
+        kv_heads: u32,
+        head_dim: u32,
+        cache_rows: u32,
+        max_seq_len: u32,
+        d_q_start: *const i32,
+        d_row_base: *const i32,
+        d_seq_lens: *const i32,
+        max_len_hint: u32,
+        scale: c_float,
+    ) -> c_int;
+    pub fn janus_beam_select(
+        ctx: *mut janus_ctx,
+        logits: *const c_float,
+        d_scores: *const c_float,
+        d_out_scores: *mut c_float,
+        d_out_parents: *mut i32,
+        d_out_tokens: *mut i32,
+        batch: u32,
+        beams: u32,
+        vocab: u32,
+        n: u32,
+    ) -> c_int;
+    pub fn janus_kv_reorder(
+        ctx: *mut janus_ctx,
+        n_buffers: u32,
+        buffers: *mut *mut c_void,
+        row_bytes: *const u64,
+        layers: u32,
+        groups: u32,
+        beams: u32,
+        cache_rows: u32,
+        max_seq_len: u32,
+        d_row_base: *const i32,
+        d_parents: *const i32,
+        d_seq_lens: *const i32,
     ) -> c_int;
     pub fn janus_embed(
         ctx: *mut janus_ctx,

@@ -1,0 +1,297 @@
+"""janus_fp4_attention against 64 bits, with the bounds of packed_ref (a 4-bit value is a binary16 number)."""
+import math
+
+import pytest
+import torch
+
+from janus_amd import ops
+from fp4_ref import decode, random_cache
+from packed_ref import attend, check
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+TYPES = {"f16": torch.float16, "f32": torch.float32}
+
+
+def _i32(v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+def _case(heads, kvh, hd, seqs, dtype, cap=None, seed=0, sigma=1.5, behind=0, poison=True, lo=122, hi=129):
+    """seqs: (rows, length) of each. Cache rows that no sequence owns hold NaN blocks."""
+    gen = torch.Generator().manual_seed(seed)
+    rows = sum(n for n, _ in seqs)
+    cap = cap or max(1, max(m for _, m in seqs))
+    q = (torch.randn(rows + behind, heads, hd, generator=gen) * sigma).to(dtype)
+    cache = [*random_cache(gen, len(seqs) * cap + 1, kvh, hd, lo, hi), *random_cache(gen, len(seqs) * cap + 1, kvh, hd, lo, hi)]
+    slots = torch.randperm(len(seqs), generator=gen).tolist()
+    k, v = decode(*cache[:2]), decode(*cache[2:])
+    if poison:
+        for s, (_, m) in zip(slots, seqs):
+            for c in cache[1::2]:
+                c[s * cap + max(0, m):(s + 1) * cap] = 255
+    starts = [0]
+    for n, _ in seqs:
+        starts.append(starts[-1] + n)
+    return q, [c.to(DEV) for c in cache], k, v, slots, starts, cap
+
+
+def _run(engine, heads, kvh, hd, seqs, types, hint=0, scale=0.0, device="cpu", **kw):
+    dtype = TYPES[types]
+    q, cache, k, v, slots, starts, cap = _case(heads, kvh, hd, seqs, dtype, **kw)
+    out = torch.full(q.shape, 7.0, dtype=dtype, device=DEV)
+    ops.fp4_attention(engine, q.to(DEV), *cache, out, len(seqs), cap, q_start=_i32(starts),
+                      row_base=_i32([s * cap for s in slots]), seq_lens=_i32([m for _, m in seqs]), max_len_hint=hint,
+                      scale=scale)
+    engine.sync()
+    for s, (n, m), i in zip(slots, seqs, starts):
+        m = max(0, m)
+        with torch.device(device):
+            want, tol = attend(q[i:i + n].to(device), k[s * cap:s * cap + m].to(device), v[s * cap:s * cap + m].to(device),
+                               [max(0, m - n + 1 + r) for r in range(n)], types == "f16", True, scale or None)
+        check(out[i:i + n], want.cpu(), tol.cpu(), (types, heads, kvh, hd, n, m))
+    assert (out[starts[-1]:] == 7.0).all()
+
+
+LAYOUTS = [(4, 2, 64), (8, 2, 128), (3, 3, 128), (5, 1, 64), (8, 8, 128), (12, 4, 64)]
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("heads,kvh,hd", LAYOUTS)
+def test_one_row_of_each(engine, types, heads, kvh, hd):
+    # a decode step: lengths at and around 16 and 32, none, one
+    _run(engine, heads, kvh, hd, [(1, m) for m in (1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 0, 130)], types)
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("heads,kvh,hd", LAYOUTS)
+def test_whole_prompts(engine, types, heads, kvh, hd):
+    _run(engine, heads, kvh, hd, [(1, 1), (31, 31), (0, 0), (32, 32), (33, 33), (2, 2), (129, 129), (200, 200)], types, behind=3)
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("heads,kvh,hd", [(8, 2, 128), (4, 4, 64), (12, 4, 128), (40, 8, 128), (16, 1, 128), (40, 1, 64)])
+def test_rows_behind_a_context(engine, types, heads, kvh, hd):
+    # chunks, drafted tokens and single tokens of one call
+    _run(engine, heads, kvh, hd, [(5, 64), (1, 63), (1, 65), (64, 200), (7, 700), (40, 41), (1, 1)], types, behind=3)
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+def test_rows_that_see_nothing(engine, types):
+    # fewer positions than rows: the first rows see none; lengths of zero and below
+    _run(engine, 8, 2, 64, [(9, 4), (3, 0), (70, 2), (1, 0), (2, 2), (1, -5), (4, -1)], types, cap=80)
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("heads,kvh,hd", [(32, 8, 128), (40, 1, 128), (32, 32, 128), (4, 2, 64), (16, 1, 128), (24, 8, 64)])
+def test_long_context_is_split(engine, types, heads, kvh, hd):
+    _run(engine, heads, kvh, hd, [(1, 2100)], types)
+    _run(engine, heads, kvh, hd, [(1, 1900), (3, 333), (1, 5), (0, 0), (1, 0)], types, seed=1)
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("hint", [1, 100, 100000])
+def test_hint_only_plans(engine, types, hint):
+    _run(engine, 8, 2, 64, [(2, 1500), (130, 900)], types, hint=hint)
+    _run(engine, 8, 8, 128, [(1, 1500), (1, 3)], types, hint=hint)
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+def test_many_sequences(engine, types):
+    # more sequences than a wavefront has lanes, some without rows
+    _run(engine, 4, 2, 64, [((i * 7) % 5, 3 + (i * 7) % 5 + i % 11) for i in range(150)], types, cap=24)
+    _run(engine, 4, 4, 128, [(1, 1 + i * 13 % 90) for i in range(130)], types, cap=90)
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("sigma", [0.0, 1e-6, 40.0])
+def test_score_ranges(engine, types, sigma):
+    # equal scores, tiny queries, and one position that takes nearly all weight
+    _run(engine, 4, 2, 128, [(70, 300), (1, 200)], types, sigma=sigma)
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+def test_scales_of_many_binades(engine, types):
+    _run(engine, 8, 2, 128, [(1, 300), (40, 90)], types, lo=114, hi=131, sigma=0.5, scale=0.01)
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("size", [1e-30, 1e-3, 3e4])
+def test_query_magnitudes(engine, types, size):
+    """Rows of q from tiny to large, with a scale that makes their scores ordinary."""
+    if types == "f16" and size < 1e-3:
+        pytest.skip("not a binary16 number")
+    _run(engine, 8, 2, 128, [(3, 120), (1, 700)], types, sigma=size / 3, scale=min(1e30, 0.3 / size))
+
+
+def test_a_long_prompt(engine):
+    _run(engine, 8, 2, 128, [(1500, 1500)], "f16", device=DEV)
+    _run(engine, 8, 2, 128, [(700, 2000), (300, 300)], "f32", device=DEV)
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+def test_decode_step_without_tables(engine, types):
+    """Without q_start every sequence has rows / nseq; without lengths as many positions as rows."""
+    dtype = TYPES[types]
+    gen = torch.Generator().manual_seed(11)
+    heads, kvh, hd, cap = 8, 2, 64, 24
+    q = torch.randn(12, heads, hd, generator=gen).to(dtype)
+    cache = [*random_cache(gen, 4 * cap, kvh, hd), *random_cache(gen, 4 * cap, kvh, hd)]
+    k, v = decode(*cache[:2]), decode(*cache[2:])
+    dev = [c.to(DEV) for c in cache]
+    out = torch.empty(12, heads, hd, dtype=dtype, device=DEV)
+    ops.fp4_attention(engine, q.to(DEV), *dev, out, 4, cap)
+    for s in range(4):
+        want, tol = attend(q[3 * s:3 * s + 3], k[s * cap:s * cap + 3], v[s * cap:s * cap + 3], [1, 2, 3], types == "f16", True)
+        check(out[3 * s:3 * s + 3], want, tol, s)
+    out4 = torch.empty(4, heads, hd, dtype=dtype, device=DEV)
+    ops.fp4_attention(engine, q[:4].to(DEV).contiguous(), *dev, out4, 4, cap, seq_lens=_i32([cap, 1, 7, 20]))
+    for s, n in enumerate((cap, 1, 7, 20)):
+        want, tol = attend(q[s:s + 1], k[s * cap:s * cap + n], v[s * cap:s * cap + n], [n], types == "f16", True)
+        check(out4[s:s + 1], want, tol, s)
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+def test_lengths_beyond_the_slot_and_the_cache(engine, types):
+    """Positions of max_seq_len and above, and cache rows beyond the cache, do not exist; nothing is read there."""
+    dtype = TYPES[types]
+    gen = torch.Generator().manual_seed(12)
+    heads, kvh, hd = 4, 2, 64
+    cache = [*random_cache(gen, 100, kvh, hd), *random_cache(gen, 100, kvh, hd)]
+    k, v = decode(*cache[:2]), decode(*cache[2:])
+    dev = [c.to(DEV) for c in cache]
+    q = torch.randn(5, heads, hd, generator=gen).to(dtype)
+    out = torch.empty(5, heads, hd, dtype=dtype, device=DEV)
+    base, lens = [0, 90, 99, 200, -3], [50, 50, 2 ** 31 - 1, 10, 10]
+    ops.fp4_attention(engine, q.to(DEV), *dev, out, 5, 40, row_base=_i32(base), seq_lens=_i32(lens))
+    for s, n in enumerate((40, 10, 1, 0, 0)):
+        want, tol = attend(q[s:s + 1], k[base[s]:base[s] + n] if n else k[:0], v[base[s]:base[s] + n] if n else v[:0], [n], types == "f16", True)
+        check(out[s:s + 1], want, tol, s)
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("rows,length", [(1, 40), (1, 2500), (6, 700), (90, 300)])
+def test_nan_blocks(engine, types, rows, length):
+    """A NaN block of K reaches every dim of the heads that read it, one of V its 32 dims;
+    rows that do not see it are untouched. q with an infinity or NaN: NaN for its head."""
+    heads, kvh, hd = 8, 4, 128
+    q, cache, k, v, slots, starts, cap = _case(heads, kvh, hd, [(rows, length)], TYPES[types], seed=5)
+    at = length - max(1, rows // 2)   # the last rows see it, with many rows the first do not
+    cache[1][at, 0, 2] = 255
+    cache[3][at, 2, 1] = 141
+    cache[3][3, 3, 0] = 200
+    q[rows - 1, 2, 7] = math.inf      # KV head 1
+    out = torch.empty(q.shape, dtype=q.dtype, device=DEV)
+    ops.fp4_attention(engine, q.to(DEV), *cache, out, 1, cap, seq_lens=_i32([length]))
+    got = out.float().cpu()
+    clean = torch.where(torch.isfinite(q), q, 0)
+    want, tol = attend(clean, k[:length], v[:length], [length - rows + 1 + r for r in range(rows)], types == "f16", True)
+    sees = torch.tensor([length - rows + 1 + r > at for r in range(rows)])
+    assert sees.any() and (rows == 1 or not sees.all())
+    nan = torch.zeros(got.shape, dtype=torch.bool)
+    nan[:, 0:2] = sees[:, None, None]
+    nan[:, 4:6, 32:64] = sees[:, None, None]
+    nan[:, 6:8, 0:32] = True
+    nan[rows - 1, 2] = True
+    assert torch.equal(got.isnan(), nan)
+    got[nan] = want[nan].float()
+    check(got, want, tol, (types, rows, length))
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+def test_in_place_on_another_stream(engine, types):
+    q, cache, k, v, slots, starts, cap = _case(8, 2, 64, [(1, 1300), (4, 90)], TYPES[types], seed=8)
+    tables = dict(q_start=_i32(starts), row_base=_i32([s * cap for s in slots]), seq_lens=_i32([1300, 90]))
+    want = torch.empty(q.shape, dtype=q.dtype, device=DEV)
+    dev = q.to(DEV)
+    ops.fp4_attention(engine, dev, *cache, want, 2, cap, **tables)
+    engine.sync()
+    stream = torch.cuda.Stream()
+    engine.bind_stream(stream)
+    try:
+        ops.fp4_attention(engine, dev, *cache, dev, 2, cap, **tables)
+        engine.sync()
+    finally:
+        engine.bind_stream(torch.cuda.default_stream())
+    assert torch.equal(dev, want)
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+def test_captured_calls_follow_their_tables(engine, types):
+    """A captured call, replayed with other lengths, equals the eager one; two graphs of one context share its workspace."""
+    dtype = TYPES[types]
+    heads, kvh, hd, cap = 8, 2, 128, 1500
+    q, cache, k, v, slots, starts, _ = _case(heads, kvh, hd, [(1, cap), (1, cap), (1, cap)], dtype, seed=9)
+    q2 = torch.randn(3 * 40, heads, hd, generator=torch.Generator().manual_seed(10)).to(dtype).to(DEV)
+    dev, base, lens = q.to(DEV), _i32([s * cap for s in slots]), _i32([5, 700, cap])
+    out, out2 = torch.zeros_like(dev), torch.zeros_like(q2)
+
+    def step():
+        ops.fp4_attention(engine, dev, *cache, out, 3, cap, row_base=base, seq_lens=lens)
+
+    def chunk():
+        ops.fp4_attention(engine, q2, *cache, out2, 3, cap, row_base=base, seq_lens=lens)
+
+    stream = torch.cuda.Stream()
+    graphs = []
+    with torch.cuda.stream(stream):
+        engine.bind_stream(stream)
+        try:
+            for call in (step, chunk):
+                call()
+                stream.synchronize()
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g, stream=stream):
+                    call()
+                graphs.append(g)
+            for new in ([5, 700, cap], [1, 1, 1], [cap, 0, 33], [40, 1200, 64]):
+                lens.copy_(_i32(new))
+                got = []
+                for g, o in zip(graphs, (out, out2)):
+                    o.fill_(3)
+                    g.replay()
+                for o in (out, out2):
+                    got.append(o.clone())
+                step()
+                chunk()
+                stream.synchronize()
+                assert torch.equal(got[0], out) and torch.equal(got[1], out2), new
+        finally:
+            engine.bind_stream(torch.cuda.default_stream())
+
+
+def test_runs_repeat(engine):
+    """The same call twice gives the same bits."""
+    for types, seqs in (("f16", [(1, 3000), (1, 40)]), ("f32", [(3, 900), (50, 60)])):
+        q, cache, k, v, slots, starts, cap = _case(8, 8, 128, seqs, TYPES[types], seed=13)
+        outs = []
+        for _ in range(2):
+            out = torch.empty(q.shape, dtype=q.dtype, device=DEV)
+            ops.fp4_attention(engine, q.to(DEV), *cache, out, len(seqs), cap, q_start=_i32(starts),
+                              row_base=_i32([s * cap for s in slots]), seq_lens=_i32([m for _, m in seqs]))
+            outs.append(out)
+        assert torch.equal(*outs)
+
+
+def test_offsets_beyond_32_bits(engine):
+    """A slot whose values lie beyond 2^32 bytes."""
+    heads, kvh, hd, n = 32, 32, 128, 70
+    rows = 2 ** 32 // (kvh * hd // 2) + n
+    gen = torch.Generator().manual_seed(14)
+    part = [*random_cache(gen, n, kvh, hd), *random_cache(gen, n, kvh, hd)]
+    cache = []
+    for p in part:
+        c = torch.zeros(rows, *p.shape[1:], dtype=torch.uint8, device=DEV)
+        c[rows - n:] = p.to(DEV)
+        cache.append(c)
+    q = torch.randn(1, heads, hd, generator=gen)
+    out = torch.empty(1, heads, hd, device=DEV)
+    ops.fp4_attention(engine, q.to(DEV), *cache, out, 1, n, row_base=_i32([rows - n]), seq_lens=_i32([n]))
+    want, tol = attend(q, decode(*part[:2]), decode(*part[2:]), [n], False, True)
+    check(out, want, tol)
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+def test_rows_that_see_nothing_of_a_split_context(engine, types):
+    _run(engine, 8, 2, 128, [(40, 1500), (40, 0), (40, 33)], types, cap=1500)
+    _run(engine, 8, 8, 64, [(2, 1000), (2, 1), (1, 0), (9, 70)], types)
