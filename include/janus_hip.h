@@ -327,8 +327,9 @@ int janus_kv_read_fp4(janus_ctx *ctx, const void *k_cache, const void *k_scales,
                       uint32_t cache_rows, uint32_t first_row, const int32_t *d_rows);
 /* janus_prompt_attention over a 4-bit cache: causal attention of packed rows, from one
  * decode step's single tokens (rows = nseq, d_q_start NULL) to drafted tokens and
- * prompts, with the tables, hint, scale, results for rows that see nothing and limits
- * described there; positions at cache rows of cache_rows and above do not exist. q and out are
+ * prompts, with the tables, hint, scale and results for rows that see nothing described
+ * there (rows * heads below 2^25, nseq * kv_heads below 2^22); positions at cache rows
+ * of cache_rows and above do not exist. q and out are
  * [rows][heads][head_dim] of dtype F32 (K and V exact, q and the probabilities to 22
  * bits) or F16 (probabilities rounded to binary16); head_dim 64 or 128; out may be
  * q. A row of q with an infinity or NaN gives NaN; a NaN block reaches the rows that

@@ -51,7 +51,7 @@ struct Fp4Args {
     uint32_t cols;                        // columns of a workgroup
     uint32_t hw, ph;                      // its wavefronts: KV heads x position phases (x columns)
     uint32_t head_groups, tasks;          // workgroups of a task; most tasks
-    uint32_t target, least;               // split: parts to aim at (0: never), fewest positions of one
+    uint32_t target, least, step;         // split: parts to aim at (0: never), fewest positions of one, which are a multiple of step
     float scale2;                         // scale * log2(e)
 };
 
@@ -134,7 +134,7 @@ __device__ bool find_task(const Fp4Args &a, uint32_t t, Task &w) {
             total += wave_scan((uint64_t)tiles * q.avail);
         }
         total = __shfl(total, 63, 64);
-        const uint64_t step = 32u * a.ph;
+        const uint64_t step = a.step;
         uint64_t c = (total + a.target - 1) / a.target;
         c = max((c + step - 1) / step * step, (uint64_t)a.least);
         chunk = (uint32_t)min(c, (uint64_t)0x80000000u);
@@ -153,7 +153,7 @@ __device__ bool find_task(const Fp4Args &a, uint32_t t, Task &w) {
             const uint32_t in = t - (__shfl(upto, at, 64) - __shfl(tiles * parts, at, 64));
             w.s = seq_rows(a, __builtin_amdgcn_readfirstlane(s));
             w.part = in % w.parts;
-            w.c0 = in / w.parts * a.cols;
+            w.c0 = (__shfl(tiles, at, 64) - 1 - in / w.parts) * a.cols;   // the last rows see most: they come first
             w.chunk = chunk;
             w.first_task = t - w.part;
             return true;
@@ -341,20 +341,20 @@ template <typename T, int D, int NT> struct Columns {
             float mx = s[t][0][0];
 #pragma unroll
             for (int j = 1; j < 8; ++j) mx = fmaxf(mx, s[t][j >> 2][j & 3]);
-            mx = groups_max(mx) * cs[t];
-            if (__any(mx > m[t] + kSlack)) {
+            mx = groups_max(mx);
+            if (__any((mx - m[t]) * cs[t] > kSlack)) {
                 const float now = fmaxf(m[t], mx);
-                const float f = m[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[t] - now);
+                const float f = m[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[t] - now) * cs[t]);
                 l[t] *= f;
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i) o[t][i] *= f;
                 m[t] = now;
             }
-            const float off = m[t] == -INFINITY ? 0.0f : kBias - m[t];
+            const float m0 = m[t] == -INFINITY ? 0.0f : m[t];
             float x[8], sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                x[j] = __builtin_amdgcn_exp2f(fmaf(s[t][j >> 2][j & 3], cs[t], off));
+                x[j] = __builtin_amdgcn_exp2f(fmaf(s[t][j >> 2][j & 3] - m0, cs[t], kBias));   // large scores keep their last bits
                 sum += x[j];
             }
             l[t] += sum;
@@ -490,7 +490,10 @@ __global__ __launch_bounds__(NW * 64, MINB) void fp4_attn_kernel(Fp4Args a) {
 
     // the phases of a head and column tile join in its first one
 #pragma unroll
-    for (int t = 0; t < NT; ++t) col.l[t] = groups_sum(col.l[t]);
+    for (int t = 0; t < NT; ++t) {
+        col.l[t] = groups_sum(col.l[t]);
+        col.m[t] = col.m[t] == -INFINITY ? col.m[t] : col.m[t] * col.cs[t];   // in powers of two from here on
+    }
     if (a.ph > 1) {
         constexpr uint32_t kArea = NT * (D / 4 + 2) * 64u;   // floats of a wavefront
         float *mine = lds + ((phase - 1) * a.hw + hwave) * kArea;
@@ -640,16 +643,341 @@ template <typename T, int D> __global__ __launch_bounds__(256) void fp4_join_ker
     ((T *)a.out)[((size_t)row * a.heads + head) * D + threadIdx.x] = sees ? (T)(sum / total) : (T)0.0f;
 }
 
-template <typename T, int D, int NT, int NW, int MINB> int launch_attn(janus_ctx *ctx, const Fp4Args &a) {
-    const uint32_t lds = (a.ph - 1) * a.hw * NT * (D / 4 + 2) * 64u * 4u;
-    const uint64_t blocks = (uint64_t)(a.tasks + 7) / 8 * 8 * a.head_groups;
-    if (blocks * (NW * 64) >= (1ull << 32)) return fail(ctx, JANUS_E_INVALID_DIM, "fp4_attention: more workgroups than one launch takes");
-    hipLaunchKernelGGL((fp4_attn_kernel<T, D, NT, NW, MINB>), dim3((uint32_t)blocks), dim3(NW * 64), lds, ctx->stream, a);
-    JANUS_LAUNCH_CHECK(ctx);
-    if (a.target) {
-        hipLaunchKernelGGL((fp4_join_kernel<T, D>), dim3(a.rows * a.heads), dim3(256), 0, ctx->stream, a);
-        JANUS_LAUNCH_CHECK(ctx);
+// ---- many columns -----------------------------------------------------------------
+//
+// Four wavefronts of 32 columns share K and V: tiles of TP positions are loaded in 4 bits
+// into registers two tiles ahead, converted one tile ahead and written to LDS as
+// the operands of v_mfma_f32_32x32x16_f16 that they will be, 16 bytes a lane, so that every
+// wavefront reads them in a straight line.
+//   K: operand (position n, dims 16 s + 8 h ..) at slot ((n / 32) D / 16 + s) 64 + 32 h + n % 32
+//   S^T: position 8 (v / 4) + 4 h + v % 4 of column lane % 32 in s[v], h = lane / 32, which is
+//     the operand order of 16 positions for P;
+//   V: operand (dim i, positions 4 h .. and 8 + 4 h .. of 16) at slot (.. D / 32 + i / 32) 64 + 32 h + i % 32;
+//     a lane converts four positions of 8 dims and writes 8 bytes of each; the slots of 8
+//     dims are permuted by the dims' number so that lanes meet different banks.
+
+// First positions of a NaN block of K, and of V by block, among [p, end).
+template <int D> struct Nans {
+    uint32_t k, v[D / 32];
+};
+template <int D> __device__ __forceinline__ Nans<D> all_nans(const uint8_t *ks, const uint8_t *vs, uint32_t srow, uint32_t p, uint32_t end) {
+    const uint32_t lane = threadIdx.x & 63u;
+    Nans<D> at;
+    at.k = 0xffffffffu;
+#pragma unroll
+    for (int b = 0; b < D / 32; ++b) at.v[b] = 0xffffffffu;
+    for (; p < end; p += 64) {
+        const uint32_t i = p + lane;
+        bool kn = false;
+#pragma unroll
+        for (int b = 0; b < D / 32; ++b) {
+            bool vn = false;
+            if (i < end) {
+                kn |= ks[(size_t)i * srow + b] > 140;
+                vn = vs[(size_t)i * srow + b] > 140;
+            }
+            const uint64_t some = __ballot(vn);
+            if (some) at.v[b] = min(at.v[b], p + (uint32_t)__builtin_ctzll(some));
+        }
+        const uint64_t some = __ballot(kn);
+        if (some) at.k = min(at.k, p + (uint32_t)__builtin_ctzll(some));
     }
+    return at;
+}
+
+template <typename T, int D, int TP>
+__global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args a) {
+    constexpr int P = sizeof(T) == 4 ? 2 : 1, NB = TP / 32, QN = D / 16, ND = D / 32;
+    constexpr float kBias = P == 2 ? 13.0f : 7.0f, kSlack = P == 2 ? 2.0f : 8.0f;
+    constexpr uint32_t kTile = TP * D * 2u;   // bytes of a tile of K, and of V
+    constexpr uint32_t kUnits = TP * D / 32;  // 16-byte pieces of K, and quads of positions x 8 dims of V
+    static_assert(kUnits == 256 || kUnits == 128, "a lane has one unit of each, or of one of them");
+    extern __shared__ uint8_t smem[];         // K, V, K, V
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t col = lane & 31u, h = lane >> 5;
+    // KV heads change fastest, so with eight of them an XCD's L2 holds the lines of one or two
+    const uint32_t task = blockIdx.x / a.kv_heads, kvh = blockIdx.x % a.kv_heads;
+    Task w;
+    if (task >= a.tasks || !find_task(a, task, w)) return;
+    const uint32_t columns = w.s.n * a.G;
+    auto seen = [&](uint32_t c) { return (uint32_t)min(max(w.s.first + (int64_t)(c / a.G), (int64_t)0), (int64_t)w.s.avail); };
+    const uint32_t group_hi = seen(min(w.c0 + 127u, columns - 1));   // the last column sees most
+    const uint64_t from = w.parts > 1 ? (uint64_t)w.part * w.chunk : 0u;
+    const uint32_t p0 = __builtin_amdgcn_readfirstlane((uint32_t)min(from, (uint64_t)group_hi));
+    const uint32_t p1 = __builtin_amdgcn_readfirstlane(w.parts > 1 ? (uint32_t)min((uint64_t)group_hi, from + w.chunk) : group_hi);
+    const uint32_t c0 = w.c0 + 32u * wave;
+    const bool idle = c0 >= columns;
+    const uint32_t wave_lo = idle ? 0u : __builtin_amdgcn_readfirstlane(seen(c0));
+    const uint32_t wave_hi = idle ? 0u : __builtin_amdgcn_readfirstlane(min(seen(min(c0 + 31u, columns - 1)), p1));
+    const uint32_t c = min(c0 + col, columns - 1), vis = seen(c);
+    const size_t qat = (size_t)(w.s.row0 + c / a.G) * a.heads + (size_t)kvh * a.G + c % a.G;
+
+    const uint32_t row = a.kv_heads * (D / 2), srow = a.kv_heads * (D / 32);
+    const size_t base = (size_t)w.s.base;
+    const uint8_t *kc = a.kc + base * row + kvh * (D / 2), *ks = a.ks + base * srow + kvh * (D / 32);
+    const uint8_t *vc = a.vc + base * row + kvh * (D / 2), *vs = a.vs + base * srow + kvh * (D / 32);
+
+    // what a lane loads of a tile: block kb of position kn of K, and dims 8 vd .. of positions 4 vq .. of V
+    const uint32_t ku = threadIdx.x, vu = kUnits == 256 ? threadIdx.x : threadIdx.x ^ 128u;
+    const bool has_k = ku < kUnits, has_v = vu < kUnits;
+    const uint32_t kn = (ku & 15u) + ku / (D / 2) * 16u, kb = ku / 16u % (D / 32), vd = vu % (D / 8), vq = vu / (D / 8);
+    ju4 kr;
+    uint32_t ksr = 0, vr[4], vsr[4] = {};
+    auto load = [&](uint32_t p) {
+        const uint32_t last = p1 - 1 - p;   // rows beyond the part repeat its last one
+        if (has_k) {
+            const uint32_t n = min(kn, last);
+            kr = *(const ju4 *)(kc + (size_t)p * row + (n * row + kb * 16u));
+            ksr = (ks + (size_t)p * srow)[n * srow + kb];
+        }
+        if (has_v) {
+            const uint8_t *vp = vc + (size_t)p * row, *vsp = vs + (size_t)p * srow;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t n = min(4u * vq + i, last);
+                vr[i] = *(const uint32_t *)(vp + (n * row + vd * 4u));
+                vsr[i] = vsp[n * srow + vd / 4u];
+            }
+        }
+    };
+    uint32_t worst = 0;
+    auto store = [&](uint32_t b) {
+        uint8_t *kt = smem + b * 2 * kTile, *vt = kt + kTile;
+        if (has_k) {
+            const float sc = scale_of(ksr);
+            worst = max(worst, ksr);
+            uint8_t *to = kt + ((kn / 32 * QN + 2 * kb) * 64u + kn % 32) * 16u;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *(ju4 *)(to + ((i >> 1) * 64u + (i & 1) * 32u) * 16u) =
+                    ju4{fp4_pair<0>(kr[i], sc), fp4_pair<1>(kr[i], sc), fp4_pair<2>(kr[i], sc), fp4_pair<3>(kr[i], sc)};
+        }
+        if (has_v) {
+            float sc[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                sc[i] = scale_of(vsr[i]);
+                worst = max(worst, vsr[i]);
+            }
+            // block vd / 4, slots 8 (vd % 4) .. of its 32; quad vq % 4: half vq % 2, first or second 8 bytes
+            uint8_t *to = vt + ((vq / 4 * ND + vd / 4) * 64u + (vq & 1u) * 32u + (vd & 3u) * 8u) * 16u + (vq >> 1 & 1u) * 8u;
+            const uint32_t turn = (vd & 7u) * 16u;
+            auto two = [&](auto byte) {
+                constexpr int B = decltype(byte)::value;
+                uint32_t x[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = fp4_pair<B>(vr[i], sc[i]);
+                *(uint2 *)(to + ((2 * B * 16u) ^ turn)) = make_uint2(__builtin_amdgcn_perm(x[1], x[0], 0x05040100u), __builtin_amdgcn_perm(x[3], x[2], 0x05040100u));
+                *(uint2 *)(to + (((2 * B + 1) * 16u) ^ turn)) = make_uint2(__builtin_amdgcn_perm(x[1], x[0], 0x07060302u), __builtin_amdgcn_perm(x[3], x[2], 0x07060302u));
+            };
+            two(std::integral_constant<int, 0>{});
+            two(std::integral_constant<int, 1>{});
+            two(std::integral_constant<int, 2>{});
+            two(std::integral_constant<int, 3>{});
+        }
+    };
+    if (p0 < p1) load(p0);
+
+    // q of the lane's column
+    const T *qp = (const T *)a.q + qat * D;
+    fh8 q[P][QN];
+    float cs = a.scale2;
+    bool bad = false;
+    {
+        float x[QN][8];
+        uint32_t top = 0;
+#pragma unroll
+        for (int s = 0; s < QN; ++s) {
+            typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
+#pragma unroll
+            for (int i = 0; i < 8; i += 16 / (int)sizeof(T)) {
+                const vec v = *(const vec *)(qp + 16 * s + 8 * h + i);
+#pragma unroll
+                for (int j = 0; j < 16 / (int)sizeof(T); ++j) x[s][i + j] = (float)v[j];
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[s][i]) & 0x7fffffffu);
+        }
+        top = max(top, __float_as_uint(swap32(__uint_as_float(top))));
+        bad = top >= 0x7f800000u;
+        const int e = P == 2 && !bad ? max((int)(top >> 23), 1) - 127 - 14 : 0;
+        if constexpr (P == 2) cs = ldexpf(a.scale2, e);
+        cs = fmaxf(cs, 1e-37f);
+#pragma unroll
+        for (int s = 0; s < QN; ++s)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float y = bad ? 0.0f : P == 2 ? ldexpf(x[s][i], -e) : x[s][i];
+                q[0][s][i] = (_Float16)y;
+                if constexpr (P == 2) q[1][s][i] = (_Float16)(y - (float)q[0][s][i]);
+            }
+    }
+    typedef float f16v __attribute__((ext_vector_type(16)));
+    f16v o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[d] = (f16v){};
+    // p = 2^(s cs + c2), c2 = kBias - m cs rounded (infinite while nothing was seen); where that would cost
+    // the last bits of a score (far) the difference to m is taken first
+    float m = -INFINITY, c2 = INFINITY, l = 0.0f;
+    bool far = false;
+    const uint32_t kat = lane * 16u;
+    uint32_t vat[2];   // of even and odd blocks of dims: the slots are permuted by (dim / 8) % 8
+#pragma unroll
+    for (int d = 0; d < 2; ++d) vat[d] = (((col >> 3) * 8u + ((col & 7u) ^ ((4u * d + (col >> 3)) & 7u))) + 32u * h) * 16u;
+    uint32_t b = 0;
+    if (p0 < p1) {
+        store(0);
+        if (p0 + TP < p1) load(p0 + TP);
+    }
+    for (uint32_t p = p0; p < p1; p += TP, b ^= 1u) {
+        __syncthreads();   // this tile is there, the other buffer has been read
+        if (p + TP < p1) {
+            store(b ^ 1u);
+            if (p + 2 * TP < p1) load(p + 2 * TP);
+        }
+        if (p >= wave_hi) continue;
+        const uint8_t *kt = smem + b * 2 * kTile, *vt = kt + kTile;
+        f16v s[NB];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            fh8 k[QN];
+#pragma unroll
+            for (int t = 0; t < QN; ++t) k[t] = *(const fh8 *)(kt + kat + (n * QN + t) * 1024u);
+            s[n] = (f16v){};
+            if constexpr (P == 2)
+#pragma unroll
+                for (int t = 0; t < QN; ++t) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[t], q[1][t], s[n], 0, 0, 0);
+#pragma unroll
+            for (int t = 0; t < QN; ++t) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[t], q[0][t], s[n], 0, 0, 0);
+        }
+        if (p + TP > min(wave_lo, p1)) {
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int v = 0; v < 16; ++v)
+                    if (p + 32 * n + 8 * (v >> 2) + 4 * h + (v & 3) >= vis) s[n][v] = -INFINITY;
+            // positions beyond the part are not its own
+            if (p + TP > p1)
+#pragma unroll
+                for (int n = 0; n < NB; ++n)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v)
+                        if (p + 32 * n + 8 * (v >> 2) + 4 * h + (v & 3) >= p1) s[n][v] = -INFINITY;
+        }
+        float top[2] = {s[0][0], s[0][1]};
+#pragma unroll
+        for (int x = 2; x < 16 * NB; ++x) top[x & 1] = fmaxf(top[x & 1], s[x >> 4][x & 15]);
+        float bm = fmaxf(top[0], top[1]);
+        bm = fmaxf(bm, swap32(bm));
+        if (__any(fmaf(bm, cs, c2) > kBias + kSlack)) {
+            const float now = fmaxf(m, bm), cn = now == -INFINITY ? INFINITY : fmaf(-now, cs, kBias);
+            float f;
+            if (far || __any(fabsf(cn) > 4194304.0f && cn != INFINITY)) {
+                // from c2 as it was rounded to the difference: kBias - c2 is exact
+                const float r = far ? 0.0f : fmaf(-m, cs, kBias - c2);
+                f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(fmaf(m - now, cs, r));
+                far = true;
+            } else {
+                f = cn == c2 ? 1.0f : __builtin_amdgcn_exp2f(cn - c2);
+            }
+            m = now;
+            c2 = cn;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) o[d][v] *= f;
+        }
+        const float off = c2 == INFINITY ? 0.0f : c2;
+        if (far) {
+            const float m0 = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) s[n][v] = __builtin_amdgcn_exp2f(fmaf(s[n][v] - m0, cs, kBias));
+        } else {
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) s[n][v] = __builtin_amdgcn_exp2f(fmaf(s[n][v], cs, off));
+        }
+        float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int t = 0; t < 2 * NB; ++t) {
+            fh8 ph, pl;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float x = s[t >> 1][8 * (t & 1) + e];
+                ph[e] = (_Float16)x;
+                if constexpr (P == 2) {
+                    pl[e] = (_Float16)(x - (float)ph[e]);
+                    sum[e & 1] += x;
+                }
+            }
+            if constexpr (P == 1) {   // of P as rounded: both sums see the same weights
+                const jh2 one = {(_Float16)1.0f, (_Float16)1.0f};
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) sum[(e >> 1) & 1] = __builtin_amdgcn_fdot2(jh2{ph[e], ph[e + 1]}, one, sum[(e >> 1) & 1], false);
+            }
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                const fh8 v = *(const fh8 *)(vt + vat[d & 1] + (t * ND + d) * 1024u);
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph, o[d], 0, 0, 0);
+                if constexpr (P == 2) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl, o[d], 0, 0, 0);
+            }
+        }
+        l += sum[0] + sum[1];
+    }
+    l += swap32(l);
+    const float nan = __uint_as_float(0x7fc00000u);
+    if (p0 < p1 && __syncthreads_or(worst > 140u) && !idle) {
+        const Nans<D> at = all_nans<D>(ks, vs, srow, p0, wave_hi);
+        if (at.k < vis) l = nan;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+            if (at.v[d] < vis)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) o[d][v] = nan;
+    }
+    if (c0 + col >= columns) return;
+    if (bad && vis) l = nan;
+    if (w.parts > 1) {
+        const size_t at = ((size_t)task * a.kv_heads + kvh) * a.cols + (c - w.c0);
+        float *to = a.part + at * D;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) *(jf4 *)(to + 32 * d + 8 * j + 4 * h) = jf4{o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]};
+        if (h == 0) {
+            // in powers of two, less what the rounding of c2 has moved
+            a.part_ml[2 * at] = m == -INFINITY ? m : far ? m * cs : kBias - c2;
+            a.part_ml[2 * at + 1] = l;
+        }
+    } else {
+        const float inv = vis ? 1.0f / l : 0.0f;
+        T *to = (T *)a.out + qat * D;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                typedef T t4 __attribute__((ext_vector_type(4)));
+                t4 y;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] = vis ? (T)(o[d][4 * j + i] * inv) : (T)0.0f;
+                *(t4 *)(to + 32 * d + 8 * j + 4 * h) = y;
+            }
+    }
+    if (a.target && w.part == 0 && kvh == 0 && h == 0) {
+        uint32_t *to = a.meta + 2 * ((size_t)w.s.row0 * a.G + c);
+        to[0] = w.first_task;
+        to[1] = w.parts | (c - w.c0) << 24;
+    }
+}
+
+template <typename T, int D> int launch_join(janus_ctx *ctx, const Fp4Args &a) {
+    if (!a.target) return JANUS_OK;
+    hipLaunchKernelGGL((fp4_join_kernel<T, D>), dim3(a.rows * a.heads), dim3(256), 0, ctx->stream, a);
+    JANUS_LAUNCH_CHECK(ctx);
     return JANUS_OK;
 }
 
@@ -660,15 +988,17 @@ template <typename T, int D> int launch_dim(janus_ctx *ctx, Fp4Args &a, uint32_t
         a.cols = 16;
         a.hw = a.kv_heads % 8 == 0 ? 8 : a.kv_heads % 4 == 0 ? 4 : a.kv_heads % 2 == 0 ? 2 : 1;
         a.ph = 8 / a.hw;
+        a.step = 32 * a.ph;
     } else {
-        a.cols = 4 * 16 * 2;
+        a.cols = 128;
         a.hw = a.ph = 1;
+        a.step = 64;
     }
     a.head_groups = a.kv_heads / a.hw;
     // every tile of every sequence, one more where rows do not fill the last
     const uint64_t tiles = (uint64_t)a.rows * a.G / a.cols + a.nseq;
     const uint64_t want = (uint64_t)ctx->num_cus * 2 / a.head_groups;
-    a.least = 32 * a.ph;
+    a.least = a.step;
     a.target = 0;
     uint64_t tasks = tiles;
     const uint64_t busy = std::min<uint64_t>(tiles, ((uint64_t)a.rows * a.G + a.cols - 1) / a.cols + a.nseq - 1);
@@ -676,8 +1006,7 @@ template <typename T, int D> int launch_dim(janus_ctx *ctx, Fp4Args &a, uint32_t
         a.target = (uint32_t)std::max<uint64_t>(want, 1);
         tasks += a.target;
     }
-    if (tasks >= (1u << 23)) return fail(ctx, JANUS_E_INVALID_DIM, "fp4_attention: more tiles than one launch takes");
-    a.tasks = (uint32_t)tasks;
+    a.tasks = (uint32_t)tasks;   // * head_groups below 2^21 + 2^22 + 2^10, 512 lanes each
     if (a.target) {
         const size_t cells = (size_t)a.tasks * a.kv_heads * a.cols;
         const size_t meta = ((size_t)a.rows * a.G * 8 + 255) / 256 * 256;
@@ -686,8 +1015,16 @@ template <typename T, int D> int launch_dim(janus_ctx *ctx, Fp4Args &a, uint32_t
         a.part = (float *)((char *)ctx->attn_ws + meta);
         a.part_ml = a.part + cells * D;
     }
-    if (few) return launch_attn<T, D, 1, 8, 2>(ctx, a);
-    return launch_attn<T, D, 2, 4, 1>(ctx, a);
+    if (few) {
+        const uint32_t lds = (a.ph - 1) * a.hw * (D / 4 + 2) * 64u * 4u;
+        const dim3 grid((a.tasks + 7) / 8 * 8 * a.head_groups), block(512);
+        hipLaunchKernelGGL((fp4_attn_kernel<T, D, 1, 8, 2>), grid, block, lds, ctx->stream, a);
+    } else {
+        constexpr int TP = D == 128 && sizeof(T) == 4 ? 32 : 64;
+        hipLaunchKernelGGL((fp4_wide_kernel<T, D, TP>), dim3(a.tasks * a.kv_heads), dim3(256), 4 * TP * D * 2, ctx->stream, a);
+    }
+    JANUS_LAUNCH_CHECK(ctx);
+    return launch_join<T, D>(ctx, a);
 }
 
 }  // namespace

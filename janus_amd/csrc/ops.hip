@@ -366,6 +366,8 @@ int janus_fp4_attention(janus_ctx *ctx, const void *q, int q_dt, const void *k_c
                             kv_heads, hd))
         return e;
     if (rows == 0 || nseq == 0) return JANUS_OK;
+    if ((uint64_t)nseq * kv_heads >= (1ull << 22))
+        return fail(ctx, JANUS_E_INVALID_DIM, "fp4_attention: sequences * kv_heads beyond 2^22");
     if (!d_q_start && rows % nseq)
         return fail(ctx, JANUS_E_INVALID_DIM, "fp4_attention: without q_start, rows must be a multiple of nseq");
     if (!d_q_start && !d_seq_lens && rows / nseq > max_seq_len)

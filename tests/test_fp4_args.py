@@ -85,12 +85,12 @@ def test_attention_refusals(vctx):  # noqa: F811
     for bad in (dict(q=None), dict(out=None), dict(q=P + 8), dict(out=P + 4)):
         assert _call(vctx, name, ATTEND, **bad)[0] == _lib.E_INVALID_ARG, bad
     for bad in (dict(heads=9), dict(heads=0), dict(hd=32), dict(hd=96), dict(hd=256), dict(heads=1 << 17, kv_heads=1),
-                dict(start=None, rows=5), dict(rows=2 ** 22), dict(nseq=2 ** 23, rows=8)):
+                dict(start=None, rows=5), dict(rows=2 ** 22), dict(nseq=2 ** 21, rows=8)):
         assert _call(vctx, name, ATTEND, **bad)[0] == _lib.E_INVALID_DIM, bad
     assert _call(vctx, name, ATTEND, start=None, lens=None, rows=130)[0] == _lib.E_KV_OVERFLOW
     for fine in (dict(rows=0), dict(nseq=0)):
         assert _call(vctx, name, ATTEND, **fine)[0] == _lib.OK
-    for fine in (dict(dtype=F32), dict(hd=64), dict(base=None), dict(scale=0.3), dict(start=None, lens=None, rows=128)):
+    for fine in (dict(nseq=2 ** 21 - 1), dict(rows=2 ** 22 - 1), dict(dtype=F32), dict(hd=64), dict(base=None), dict(scale=0.3), dict(start=None, lens=None, rows=128)):
         assert _call(vctx, name, ATTEND, **fine)[0] == _lib.E_NO_DEVICE, fine
 
 

@@ -295,3 +295,28 @@ def test_offsets_beyond_32_bits(engine):
 def test_rows_that_see_nothing_of_a_split_context(engine, types):
     _run(engine, 8, 2, 128, [(40, 1500), (40, 0), (40, 33)], types, cap=1500)
     _run(engine, 8, 8, 64, [(2, 1000), (2, 1), (1, 0), (9, 70)], types)
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("rows", [3, 70])
+def test_scores_beyond_their_own_last_bits(engine, types, rows):
+    """Scores whose spacing is far above 1: the farthest ahead takes all weight, equal ones share it."""
+    dtype = TYPES[types]
+    gen = torch.Generator().manual_seed(21)
+    hd, n, size = 128, 1100, 3e4 if types == "f16" else 1e8
+    q = (torch.randn(rows, 2, hd, generator=gen).sign() * size).to(dtype)
+    cache = random_cache(gen, n, 1, hd, 127, 128), random_cache(gen, n, 1, hd)
+    codes = torch.where(torch.rand(n, 1, hd // 2, generator=gen) < 0.5, 0x66, 0xEE) ^ torch.where(
+        torch.rand(n, 1, hd // 2, generator=gen) < 0.5, 0x80, 0)   # 4 and -4
+    k, v = decode(codes.to(torch.uint8), cache[0][1]), decode(*cache[1])
+    k, v = k * 16, v   # scale byte 131
+    dev = [c.to(DEV) for c in (codes.to(torch.uint8), cache[0][1] + 4, *cache[1])]
+    out = torch.empty(q.shape, dtype=dtype, device=DEV)
+    ops.fp4_attention(engine, q.to(DEV), *dev, out, 1, n, seq_lens=_i32([n]))
+    s = torch.einsum("rhd,jd->rhj", q.double(), k[:, 0])
+    for r in range(rows):
+        seen = s[r, :, :n - rows + 1 + r]
+        first = (seen == seen.amax(-1, keepdim=True)).double()
+        want = first @ v[:seen.shape[1], 0] / first.sum(-1, keepdim=True)
+        tol = 2.0 ** (-10 if types == "f16" else -20) * v.abs().max()
+        check(out[r], want, tol.expand_as(want), (types, r))
