@@ -133,7 +133,7 @@ __device__ bool find_task(const Fp4Args &a, uint32_t t, Task &w) {
             const uint32_t tiles = (uint32_t)(((uint64_t)q.n * a.G + a.cols - 1) / a.cols);
             total += wave_scan((uint64_t)tiles * q.avail);
         }
-        total = __shfl(total, 63, 64);
+        total = (uint64_t)__builtin_amdgcn_readlane((uint32_t)(total >> 32), 63) << 32 | (uint32_t)__builtin_amdgcn_readlane((uint32_t)total, 63);
         const uint64_t step = a.step;
         uint64_t c = (total + a.target - 1) / a.target;
         c = max((c + step - 1) / step * step, (uint64_t)a.least);
@@ -147,18 +147,18 @@ __device__ bool find_task(const Fp4Args &a, uint32_t t, Task &w) {
         const uint32_t upto = before + wave_scan(tiles * parts);
         const uint64_t here = __ballot(t < upto);
         if (here) {
-            const uint32_t at = (uint32_t)__builtin_ctzll(here);
+            const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)__builtin_ctzll(here));
             const uint32_t s = s0 + at;
-            w.parts = __shfl(parts, at, 64);
-            const uint32_t in = t - (__shfl(upto, at, 64) - __shfl(tiles * parts, at, 64));
-            w.s = seq_rows(a, __builtin_amdgcn_readfirstlane(s));
+            w.parts = __builtin_amdgcn_readlane(parts, at);
+            const uint32_t in = t - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(tiles * parts, at));
+            w.s = seq_rows(a, s);
             w.part = in % w.parts;
-            w.c0 = (__shfl(tiles, at, 64) - 1 - in / w.parts) * a.cols;   // the last rows see most: they come first
+            w.c0 = (__builtin_amdgcn_readlane(tiles, at) - 1 - in / w.parts) * a.cols;   // the last rows see most: they come first
             w.chunk = chunk;
             w.first_task = t - w.part;
             return true;
         }
-        before = __shfl(upto, 63, 64);
+        before = __builtin_amdgcn_readlane(upto, 63);
     }
     return false;
 }
@@ -456,24 +456,24 @@ __global__ __launch_bounds__(NW * 64, MINB) void fp4_attn_kernel(Fp4Args a) {
     if (p < end) {
         Offsets<D> off;
         set_offsets<D>(off, a.kv_heads, min(31u, end - 1 - p));
-        Raw<D> now, next;
+        Raw<D> ra, rb;
         uint32_t worst = 0;
-        load_raw<D>(now, off, kc + p * row, ks + p * srow, vc + p * row, vs + p * srow);
-        const uint32_t p0 = p;
-        for (;;) {
-            const uint32_t ahead = p + step;
-            const bool more = ahead < end;
-            if (more) {
-                if (end - ahead < 32u) set_offsets<D>(off, a.kv_heads, end - 1 - ahead);
-                load_raw<D>(next, off, kc + ahead * row, ks + ahead * srow, vc + ahead * row, vs + ahead * srow);
-            }
-            worst = max(worst, max(now.ks[0], now.ks[1]));
+        const uint32_t p0 = p, last = p0 + (end - 1 - p0) / step * step;
+        load_raw<D>(ra, off, kc + p * row, ks + p * srow, vc + p * row, vs + p * srow);
+        // The next positions are loaded before these are used; past the end the last ones
+        // again, since under a condition the compiler would wait for the loads at once.
+        auto pass = [&](const Raw<D> &use, Raw<D> &fill) {
+            const uint32_t ahead = min(p + step, last);
+            if (end - ahead < 32u) set_offsets<D>(off, a.kv_heads, end - 1 - ahead);
+            load_raw<D>(fill, off, kc + ahead * row, ks + ahead * srow, vc + ahead * row, vs + ahead * srow);
+            worst = max(worst, max(use.ks[0], use.ks[1]));
 #pragma unroll
-            for (int i = 0; i < 8; ++i) worst = max(worst, now.vs[i]);
-            col.step(now, p, p + 32u > fewest || p + 32u > end);
-            if (!more) break;
-            now = next;
-            p = ahead;
+            for (int i = 0; i < 8; i += 2) worst = max(worst, max(use.vs[i], use.vs[i + 1]));
+            col.step(use, p, p + 32u > fewest || p + 32u > end);
+            p += step;
+            return p < end;
+        };
+        while (pass(ra, rb) && pass(rb, ra)) {
         }
         if (__any(worst > 140u)) {
             const uint2 at = first_nans<D>(ks, vs, (uint32_t)srow, p0, end, step);
@@ -719,26 +719,36 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args a) {
 
     // what a lane loads of a tile: block kb of position kn of K, and dims 8 vd .. of positions 4 vq .. of V
     const uint32_t ku = threadIdx.x, vu = kUnits == 256 ? threadIdx.x : threadIdx.x ^ 128u;
-    const bool has_k = ku < kUnits, has_v = vu < kUnits;
+    const bool has_k = kUnits == 256 || ku < kUnits, has_v = kUnits == 256 || vu < kUnits;
     const uint32_t kn = (ku & 15u) + ku / (D / 2) * 16u, kb = ku / 16u % (D / 32), vd = vu % (D / 8), vq = vu / (D / 8);
     ju4 kr;
     uint32_t ksr = 0, vr[4], vsr[4] = {};
-    auto load = [&](uint32_t p) {
-        const uint32_t last = p1 - 1 - p;   // rows beyond the part repeat its last one
-        if (has_k) {
-            const uint32_t n = min(kn, last);
-            kr = *(const ju4 *)(kc + (size_t)p * row + (n * row + kb * 16u));
-            ksr = (ks + (size_t)p * srow)[n * srow + kb];
+    uint32_t ko, kso, vo[4], vso[4];   // offsets of a lane's bytes from the tile's first position
+    auto offsets = [&](uint32_t last) {   // rows beyond the part repeat its last one
+        const uint32_t n = min(kn, last);
+        ko = n * row + kb * 16u;
+        kso = n * srow + kb;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t n = min(4u * vq + i, last);
+            vo[i] = n * row + vd * 4u;
+            vso[i] = n * srow + vd / 4u;
         }
-        if (has_v) {
-            const uint8_t *vp = vc + (size_t)p * row, *vsp = vs + (size_t)p * srow;
+    };
+    offsets(min((uint32_t)TP, p1 - p0) - 1);
+    auto load = [&](uint32_t p) {
+        if (p + TP > p1) offsets(p1 - 1 - p);
+        const uint8_t *kp = kc + (size_t)p * row, *ksp = ks + (size_t)p * srow, *vp = vc + (size_t)p * row, *vsp = vs + (size_t)p * srow;
+        if (has_k) {
+            kr = *(const ju4 *)(kp + ko);
+            ksr = ksp[kso];
+        }
+        if (has_v)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint32_t n = min(4u * vq + i, last);
-                vr[i] = *(const uint32_t *)(vp + (n * row + vd * 4u));
-                vsr[i] = vsp[n * srow + vd / 4u];
+                vr[i] = *(const uint32_t *)(vp + vo[i]);
+                vsr[i] = vsp[vso[i]];
             }
-        }
     };
     uint32_t worst = 0;
     auto store = [&](uint32_t b) {
@@ -776,6 +786,7 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args a) {
             two(std::integral_constant<int, 3>{});
         }
     };
+    const uint32_t last_tile = p0 + (p1 > p0 ? (p1 - p0 - 1) / TP * TP : 0u);
     if (p0 < p1) load(p0);
 
     // q of the lane's column
@@ -819,7 +830,7 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args a) {
     // p = 2^(s cs + c2), c2 = kBias - m cs rounded (infinite while nothing was seen); where that would cost
     // the last bits of a score (far) the difference to m is taken first
     float m = -INFINITY, c2 = INFINITY, l = 0.0f;
-    bool far = false;
+    uint32_t far = 0;   // uniform
     const uint32_t kat = lane * 16u;
     uint32_t vat[2];   // of even and odd blocks of dims: the slots are permuted by (dim / 8) % 8
 #pragma unroll
@@ -827,42 +838,50 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args a) {
     uint32_t b = 0;
     if (p0 < p1) {
         store(0);
-        if (p0 + TP < p1) load(p0 + TP);
+        load(min(p0 + TP, last_tile));
     }
     for (uint32_t p = p0; p < p1; p += TP, b ^= 1u) {
         __syncthreads();   // this tile is there, the other buffer has been read
         if (p + TP < p1) {
             store(b ^ 1u);
-            if (p + 2 * TP < p1) load(p + 2 * TP);
+            // past the end the last tile again: under a condition the compiler would wait for these loads at once
+            load(min(p + 2 * TP, last_tile));
         }
         if (p >= wave_hi) continue;
         const uint8_t *kt = smem + b * 2 * kTile, *vt = kt + kTile;
         f16v s[NB];
+        fh8 k[NB][QN];
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int t = 0; t < QN; ++t) k[n][t] = *(const fh8 *)(kt + kat + (n * QN + t) * 1024u);
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-            fh8 k[QN];
-#pragma unroll
-            for (int t = 0; t < QN; ++t) k[t] = *(const fh8 *)(kt + kat + (n * QN + t) * 1024u);
             s[n] = (f16v){};
-            if constexpr (P == 2)
+            if constexpr (P == 2)   // the small parts first
 #pragma unroll
-                for (int t = 0; t < QN; ++t) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[t], q[1][t], s[n], 0, 0, 0);
+                for (int t = 0; t < QN; ++t) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[n][t], q[1][t], s[n], 0, 0, 0);
 #pragma unroll
-            for (int t = 0; t < QN; ++t) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[t], q[0][t], s[n], 0, 0, 0);
+            for (int t = 0; t < QN; ++t) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[n][t], q[0][t], s[n], 0, 0, 0);
         }
-        if (p + TP > min(wave_lo, p1)) {
+        // half the operands are requested together, the others one by one behind the products: left to
+        // itself the compiler waits for every two before it asks for the next
+        if constexpr (P == 1) {
+            constexpr int kAhead = NB * QN / 2;
+            __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+            for (int t = 0; t < NB * QN - kAhead; ++t) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
+        }
+        if (p + TP > min(wave_lo, p1)) {   // some column does not see all, or positions beyond the part are not its own
+            const uint32_t below = min(vis, p1);
 #pragma unroll
             for (int n = 0; n < NB; ++n)
 #pragma unroll
-                for (int v = 0; v < 16; ++v)
-                    if (p + 32 * n + 8 * (v >> 2) + 4 * h + (v & 3) >= vis) s[n][v] = -INFINITY;
-            // positions beyond the part are not its own
-            if (p + TP > p1)
-#pragma unroll
-                for (int n = 0; n < NB; ++n)
-#pragma unroll
-                    for (int v = 0; v < 16; ++v)
-                        if (p + 32 * n + 8 * (v >> 2) + 4 * h + (v & 3) >= p1) s[n][v] = -INFINITY;
+                for (int v = 0; v < 16; ++v) s[n][v] = p + 32 * n + 8 * (v >> 2) + 4 * h + (v & 3) < below ? s[n][v] : -INFINITY;
         }
         float top[2] = {s[0][0], s[0][1]};
 #pragma unroll
@@ -872,11 +891,11 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args a) {
         if (__any(fmaf(bm, cs, c2) > kBias + kSlack)) {
             const float now = fmaxf(m, bm), cn = now == -INFINITY ? INFINITY : fmaf(-now, cs, kBias);
             float f;
-            if (far || __any(fabsf(cn) > 4194304.0f && cn != INFINITY)) {
+            if (__builtin_amdgcn_readfirstlane(far | (__any(fabsf(cn) > 4194304.0f && cn != INFINITY) ? 1u : 0u))) {
                 // from c2 as it was rounded to the difference: kBias - c2 is exact
                 const float r = far ? 0.0f : fmaf(-m, cs, kBias - c2);
                 f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(fmaf(m - now, cs, r));
-                far = true;
+                far = 1;
             } else {
                 f = cn == c2 ? 1.0f : __builtin_amdgcn_exp2f(cn - c2);
             }
@@ -888,18 +907,14 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args a) {
 #pragma unroll
                 for (int v = 0; v < 16; ++v) o[d][v] *= f;
         }
-        const float off = c2 == INFINITY ? 0.0f : c2;
-        if (far) {
+        float off = c2 == INFINITY ? 0.0f : c2;
+        if (__builtin_amdgcn_readfirstlane(far)) {
             const float m0 = m == -INFINITY ? 0.0f : m;
+            off = kBias;
 #pragma unroll
             for (int n = 0; n < NB; ++n)
 #pragma unroll
-                for (int v = 0; v < 16; ++v) s[n][v] = __builtin_amdgcn_exp2f(fmaf(s[n][v] - m0, cs, kBias));
-        } else {
-#pragma unroll
-            for (int n = 0; n < NB; ++n)
-#pragma unroll
-                for (int v = 0; v < 16; ++v) s[n][v] = __builtin_amdgcn_exp2f(fmaf(s[n][v], cs, off));
+                for (int v = 0; v < 16; ++v) s[n][v] -= m0;
         }
         float sum[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -907,7 +922,7 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args a) {
             fh8 ph, pl;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float x = s[t >> 1][8 * (t & 1) + e];
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[t >> 1][8 * (t & 1) + e], cs, off));
                 ph[e] = (_Float16)x;
                 if constexpr (P == 2) {
                     pl[e] = (_Float16)(x - (float)ph[e]);
