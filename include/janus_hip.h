@@ -298,9 +298,9 @@ int janus_prefix_attention(janus_ctx *ctx, const void *q, int dtype, const void 
  * for V, values [cache_rows][kv_heads][head_dim / 2] (bytes; element 2i in the low
  * half of byte i) and scales [cache_rows][kv_heads][head_dim / 32] (bytes): blocks of
  * 32 values of a head share a scale. A value is an e2m1 code (sign, then 0, 0.5, 1,
- * 1.5, 2, 3, 4 or 6) times 2^(b - 127), b the scale byte; b below 104 counts as 104,
- * b above 140 makes the block NaN. 4.25 bits a value against 16. A cache of zero
- * bytes holds zeros. Values are 16-byte aligned, scales 4-byte.
+ * 1.5, 2, 3, 4 or 6) times 2^(b - 127), b the scale byte, rounded to binary16 (which
+ * holds what the append writes, scales 104 to 140, exactly); b above 140 makes the block
+ * NaN. 4.25 bits a value against 16. A cache of zero bytes holds zeros. Values are 16-byte aligned, scales 4-byte.
  *
  * Whatever the tables hold, no call reads or writes beyond cache_rows: rows outside
  * are left out.

@@ -43,15 +43,16 @@ struct Fp4Args {
     const void *q;                        // [rows][heads][D]
     const uint8_t *kc, *ks, *vc, *vs;     // [cache rows][kv_heads][D / 2] and [D / 32]
     void *out;                            // [rows][heads][D]
-    float *part, *part_ml;                // split: [task][kv_heads][cols][D] and (m, l)
-    uint32_t *meta;                       // split: [rows * G] (first task, parts | column << 24)
+    float *part, *part_ml;                // split: [slot][kv_heads][cols][D] and (m, l)
+    uint32_t *meta;                       // split: [rows * G] (first slot, parts | column << 24)
     const int32_t *q_start, *row_base, *seq_lens;
     uint32_t rows, nseq, heads, kv_heads, G;
     uint32_t cache_rows, max_seq;
     uint32_t cols;                        // columns of a workgroup
     uint32_t hw, ph;                      // its wavefronts: KV heads x position phases (x columns)
-    uint32_t head_groups, tasks;          // workgroups of a task; most tasks
-    uint32_t target, least, step;         // split: parts to aim at (0: never), fewest positions of one, which are a multiple of step
+    uint32_t head_groups, shares;         // workgroups of a share of the work; shares
+    uint32_t target, least, step;         // split: shares to aim at (0: a tile each), their fewest units of `step` positions
+    uint32_t slots;                       // split: places for partial results
     float scale2;                         // scale * log2(e)
 };
 
@@ -105,114 +106,182 @@ __device__ __forceinline__ SeqRows seq_rows(const Fp4Args &a, uint32_t s) {
     return q;
 }
 
-template <typename T> __device__ __forceinline__ T wave_scan(T v) {   // sum over the lanes up to this one
-    const uint32_t lane = threadIdx.x & 63u;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const T u = __shfl_up(v, o, 64);
-        if (lane >= (uint32_t)o) v += u;
-    }
+// Sum over the lanes up to this one, without LDS traffic.
+__device__ __forceinline__ uint32_t scan_dpp(uint32_t v) {
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);   // row_shr:1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);   // row_bcast:15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);   // row_bcast:31 into rows 2 and 3
     return v;
 }
+__device__ __forceinline__ uint32_t lane_value(uint32_t v, uint32_t lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)lane); }
+__device__ __forceinline__ int64_t lane_value(int64_t v, uint32_t lane) {
+    return (int64_t)((uint64_t)lane_value((uint32_t)((uint64_t)v >> 32), lane) << 32 | lane_value((uint32_t)v, lane));
+}
 
+// The kernel's arguments, read again where they are used: held from the start they fill the
+// scalar registers, and what spills takes vector registers and scratch.
+__device__ __forceinline__ const Fp4Args &late_args() {
+    auto at = (const Fp4Args __attribute__((address_space(4))) *)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(at));
+    return *(const Fp4Args *)at;
+}
+
+// A lane's number that the compiler takes for a new one each time: what follows from it is
+// made again for every share of columns and does not hold registers in between.
+__device__ __forceinline__ uint32_t fresh_thread() {
+    uint32_t t = threadIdx.x;
+    asm volatile("" : "+v"(t));
+    return t;
+}
+
+// What a workgroup works on: columns of a sequence, and positions [from, to) of theirs.
 struct Task {
     SeqRows s;
-    uint32_t c0;           // first column
-    uint32_t part, parts, chunk;
-    uint32_t first_task;   // of the tile's parts
+    uint32_t c0;                        // first column
+    uint32_t from, to;
+    uint32_t slot, first_slot, parts;   // its place among the parts of these columns; 1 part: the result
 };
 
-// Finds what task t is; false past the last one.
-__device__ bool find_task(const Fp4Args &a, uint32_t t, Task &w) {
-    const uint32_t lane = threadIdx.x & 63u;
-    uint32_t chunk = 0xffffffffu;
-    if (a.target) {
-        uint64_t total = 0;   // positions of all tiles
-        for (uint32_t s0 = 0; s0 < a.nseq; s0 += 64) {
-            const SeqRows q = seq_rows(a, s0 + lane);
-            const uint32_t tiles = (uint32_t)(((uint64_t)q.n * a.G + a.cols - 1) / a.cols);
-            total += wave_scan((uint64_t)tiles * q.avail);
+__device__ __forceinline__ uint64_t quotient(uint64_t a, uint64_t b) { return (a | b) >> 32 ? a / b : (uint32_t)a / (uint32_t)b; }
+
+// The work of share `share` that starts `done` units into it; false if there is none.
+// Without a split a share is a tile, that is, cols columns of a sequence. Else
+// the positions of all tiles, one behind the other in units of a.step, are cut into
+// shares of equal length, wherever tiles begin and end: CUs get an equal part of the
+// memory's rate, so all have to be given the same amount. (Parts of 840 positions that began
+// anew with each of 64 sequences of up to 8000: 93 us, some CUs with three of them and some with two.)
+// A share and a tile that meet have the slot share + tile, both counted from 0, of the
+// partial results: a step along the positions raises one of them or both.
+template <bool SPLIT> __device__ __forceinline__ bool find_task(const Fp4Args &a, uint32_t share, uint64_t &done, Task &w) {
+    const uint32_t lane = threadIdx.x & 63u, shift = 31u - (uint32_t)__builtin_clz(a.cols);   // cols is a power of two
+    SeqRows q = seq_rows(a, lane);
+    auto tiles_of = [&]() { return (q.n * a.G + a.cols - 1) >> shift; };   // rows * heads is below 2^25
+    auto units_of = [&]() { return SPLIT ? max(1u, (uint32_t)(((uint64_t)q.avail + a.step - 1) / a.step)) : 1u; };
+    uint64_t quota = 1;
+    if constexpr (SPLIT) {
+        uint64_t total = 0;
+        for (uint32_t s0 = 0;;) {
+            // (the sum of 64 products of 2^19 tiles and 2^26 units would pass 32 bits: in two halves)
+            const uint64_t units = (uint64_t)tiles_of() * units_of();
+            total += (uint64_t)lane_value(scan_dpp((uint32_t)(units & 0xffffffu)), 63) + ((uint64_t)lane_value(scan_dpp((uint32_t)(units >> 24)), 63) << 24);
+            if ((s0 += 64) >= a.nseq) break;
+            q = seq_rows(a, s0 + lane);
         }
-        total = (uint64_t)__builtin_amdgcn_readlane((uint32_t)(total >> 32), 63) << 32 | (uint32_t)__builtin_amdgcn_readlane((uint32_t)total, 63);
-        const uint64_t step = a.step;
-        uint64_t c = (total + a.target - 1) / a.target;
-        c = max((c + step - 1) / step * step, (uint64_t)a.least);
-        chunk = (uint32_t)min(c, (uint64_t)0x80000000u);
+        if (a.nseq > 64) q = seq_rows(a, lane);
+        quota = max(quotient(total + a.target - 1, a.target), (uint64_t)a.least);
+        if (done >= quota) return false;
     }
-    uint32_t before = 0;
-    for (uint32_t s0 = 0; s0 < a.nseq; s0 += 64) {
-        const SeqRows q = seq_rows(a, s0 + lane);
-        const uint32_t tiles = (uint32_t)(((uint64_t)q.n * a.G + a.cols - 1) / a.cols);
-        const uint32_t parts = a.target ? max(1u, (uint32_t)(((uint64_t)q.avail + chunk - 1) / chunk)) : 1u;
-        const uint32_t upto = before + wave_scan(tiles * parts);
-        const uint64_t here = __ballot(t < upto);
+    uint64_t at = share * quota + done, before = 0;   // units from the first tile on; tiles before these sequences
+    uint64_t start = 0;                                         // units before these sequences
+    for (uint32_t s0 = 0;;) {
+        const uint32_t tiles = tiles_of(), per = units_of();
+        const uint64_t units = (uint64_t)tiles * per;
+        const uint32_t lo = scan_dpp((uint32_t)(units & 0xffffffu)), hi = scan_dpp((uint32_t)(units >> 24)), upto_tiles = scan_dpp(tiles);
+        const uint64_t upto = start + lo + ((uint64_t)hi << 24);
+        const uint64_t here = __ballot(at < upto);
         if (here) {
-            const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)__builtin_ctzll(here));
-            const uint32_t s = s0 + at;
-            w.parts = __builtin_amdgcn_readlane(parts, at);
-            const uint32_t in = t - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(tiles * parts, at));
-            w.s = seq_rows(a, s);
-            w.part = in % w.parts;
-            w.c0 = (__builtin_amdgcn_readlane(tiles, at) - 1 - in / w.parts) * a.cols;   // the last rows see most: they come first
-            w.chunk = chunk;
-            w.first_task = t - w.part;
+            const uint32_t l = __builtin_amdgcn_readfirstlane((uint32_t)__builtin_ctzll(here));
+            w.s.row0 = lane_value(q.row0, l);
+            w.s.n = lane_value(q.n, l);
+            w.s.avail = lane_value(q.avail, l);
+            w.s.first = lane_value(q.first, l);
+            w.s.base = lane_value(q.base, l);
+            const uint32_t each = lane_value(per, l), all = lane_value(tiles, l);
+            const uint64_t first = (uint64_t)lane_value((int64_t)upto, l) - (uint64_t)all * each;   // the sequence's first unit
+            const uint32_t in = (uint32_t)(at - first), tile = each == 1 ? in : in / each, off = in - tile * each;
+            w.c0 = (all - 1 - tile) << shift;   // the last rows see most: they come first
+            if constexpr (!SPLIT) {
+                w.from = 0;
+                w.to = w.s.avail;
+                w.parts = 1;
+                return true;
+            }
+            const uint32_t n = (uint32_t)min(quota - done, (uint64_t)(each - off));
+            w.from = (uint32_t)min((uint64_t)off * a.step, (uint64_t)w.s.avail);
+            w.to = (uint32_t)min(((uint64_t)off + n) * a.step, (uint64_t)w.s.avail);
+            const uint32_t number = (uint32_t)before + lane_value(upto_tiles, l) - all + tile;
+            const uint64_t u0 = first + (uint64_t)tile * each;
+            const uint32_t s_first = (uint32_t)quotient(u0, quota), s_last = (uint32_t)quotient(u0 + each - 1, quota);
+            w.parts = s_last - s_first + 1;
+            w.slot = share + number;
+            w.first_slot = s_first + number;
+            done += n;
             return true;
         }
-        before = __builtin_amdgcn_readlane(upto, 63);
+        start = (uint64_t)lane_value((int64_t)upto, 63);
+        before += lane_value(upto_tiles, 63);
+        if ((s0 += 64) >= a.nseq) return false;
+        q = seq_rows(a, s0 + lane);
     }
-    return false;
 }
 
-// Raw bytes of 32 positions of a KV head.
+// Bytes of 32 positions of a KV head, as lane 16 g + at uses them: K of the positions at
+// and 16 + at, the lane's dims of V of the eight positions {4g .., 16 + 4g ..}; all scales
+// of a position and head in one word: K's of the two positions, V's of the (at % 8)-th
+// of the eight.
 template <int D> struct Raw {
     uint32_t k[2][D / 32];
-    uint32_t ks[2], v[8], vs[8];
+    uint32_t v[8], ks[2], vs;
 };
 
-template <int D> struct Offsets {   // of a lane, from the first of the 32 positions
-    uint32_t k[2], ks[2], v[8], vs[8];
+// 16 bytes per lane from base + off straight into LDS at lds + 16 * lane (lds is
+// uniform and goes to M0), past the caches: what few columns read is read once. Inline
+// assembly, so that the compiler does not wait for these requests at its LDS reads: the
+// loop waits for them itself.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void lds_request(const uint8_t *base, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(off), "s"(base), "s"(lds)
+                 : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+// A tile of 32 ph positions of hw KV heads, whose rows of hw D / 2 bytes lie one behind the
+// other in LDS (16 KB of K, then of V, for 128 dims). Whole rows are requested, 1 KB an
+// instruction: 270000 positions of 8 heads come at 6.4 TB/s like this and at 4.9 where
+// every wavefront loads its own head's 64 bytes of a row. The 16-byte segments of a row
+// are permuted by the heads' number of segments (U), so that 16 positions of a head (K), or four
+// positions four apart (V), lie in different banks.
+template <int D> struct Tile {
+    static constexpr uint32_t U = D / 32, kBytes = 128u * D;       // segments of a head; bytes of K
+    static constexpr int N = kBytes / 8192;                        // requests of a wavefront for K
+    const uint8_t *kc, *ks, *vc, *vs;   // of the workgroup's first head at position 0
+    uint32_t row, srow;                 // bytes from a position to the next
+    uint32_t segs, heads, fold;         // segments of a row of the tile; hw - 1; log2 of the positions in 256 bytes
+    uint32_t ko[N], vo[N];              // of the lane, from the tile's first position
+
+    __device__ __forceinline__ uint32_t k_turn(uint32_t pos) const { return (pos >> fold & heads) * U; }
+    __device__ __forceinline__ uint32_t v_turn(uint32_t pos) const { return (pos >> 2 & heads) * U; }
+    // The lane's offsets, positions from `last` on repeated.
+    __device__ __forceinline__ void offsets(uint32_t lane, uint32_t wave, uint32_t last) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t slot = (wave * N + i) * 64u + lane, pos = slot / segs, seg = slot & (segs - 1), n = min(pos, last);
+            ko[i] = n * row + (seg ^ k_turn(pos)) * 16u;
+            vo[i] = n * row + (seg ^ v_turn(pos)) * 16u;
+        }
+    }
+    __device__ __forceinline__ void request(uint32_t p, uint32_t wave, uint32_t lds) const {
+        const uint8_t *kp = kc + (size_t)p * row, *vp = vc + (size_t)p * row;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            lds_request(kp, ko[i], lds + (wave * N + i) * 1024u);
+            lds_request(vp, vo[i], lds + kBytes + (wave * N + i) * 1024u);
+        }
+    }
 };
 
-// Offsets of the positions min(i, last) of a tile.
-template <int D> __device__ __forceinline__ void set_offsets(Offsets<D> &o, uint32_t kv_heads, uint32_t last) {
-    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, at = lane & 15u;
-    const uint32_t row = kv_heads * (D / 2), srow = kv_heads * (D / 32);
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        const uint32_t p = min(at + 16u * t, last);
-        o.k[t] = p * row + g * (D / 8);
-        o.ks[t] = p * srow + g * (D / 8) / 16;
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const uint32_t p = min((j >> 2) * 16u + 4u * g + (j & 3), last);
-        o.v[j] = p * row + at * (D / 32);
-        o.vs[j] = p * srow + at * (D / 16) / 32;
-    }
+// High bit of every byte above 140.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x73737373u) & w & 0x80808080u; }
+__device__ __forceinline__ uint32_t without_nans(uint32_t w) {
+    const uint32_t m = (nan_bytes(w) >> 7) * 255u;
+    return (w & ~m) | (m & 0x7f7f7f7fu);
 }
 
-template <int D>
-__device__ __forceinline__ void load_raw(Raw<D> &r, const Offsets<D> &o, const uint8_t *kc, const uint8_t *ks,
-                                         const uint8_t *vc, const uint8_t *vs) {
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        typedef uint32_t vec __attribute__((ext_vector_type(D / 32)));
-        const vec x = *(const vec *)(kc + o.k[t]);
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) r.k[t][i] = x[i];
-        r.ks[t] = ks[o.ks[t]];
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        if constexpr (D == 128) r.v[j] = *(const uint32_t *)(vc + o.v[j]);
-        else r.v[j] = *(const uint16_t *)(vc + o.v[j]);
-        r.vs[j] = vs[o.vs[j]];
-    }
-}
-
-__device__ __forceinline__ float scale_of(uint32_t byte) {
-    return __uint_as_float(min(max(byte, 104u), 140u) << 23);
-}
+__device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(min(byte, 140u) << 23); }
 
 template <int BYTE> __device__ __forceinline__ uint32_t fp4_pair(uint32_t w, float scale) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, BYTE));
@@ -241,20 +310,19 @@ template <typename T, int D, int NT> struct Columns {
     uint32_t vis[NT];               // positions that the lane's column sees
     uint32_t bad;                   // bit t: column of tile t has an infinity or NaN in q
 
-    __device__ __forceinline__ void load(const Fp4Args &a, const Task &w, uint32_t c0, uint32_t kvh) {
-        const uint32_t lane = threadIdx.x & 63u, g = lane >> 4;
+    __device__ __forceinline__ void load(const Fp4Args &a, const Task &w, uint32_t lane, uint32_t c0, uint32_t kvh) {
+        const uint32_t g = lane >> 4;
         bad = 0;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            const uint64_t c = (uint64_t)c0 + t * 16u + (lane & 15u);
-            const uint32_t row = (uint32_t)(c / a.G);
+            const uint32_t c = c0 + t * 16u + (lane & 15u), row = c / a.G;   // below 2^25
             const bool there = row < w.s.n;
             vis[t] = 0;
             float x[D / 4];
             uint32_t top = 0;
             if (there) {
                 vis[t] = (uint32_t)min(max(w.s.first + (int64_t)row, (int64_t)0), (int64_t)w.s.avail);
-                const T *src = (const T *)a.q + ((size_t)(w.s.row0 + row) * a.heads + (size_t)kvh * a.G + (uint32_t)(c % a.G)) * D + g * (D / 4);
+                const T *src = (const T *)a.q + ((size_t)(w.s.row0 + row) * a.heads + (size_t)kvh * a.G + (c - row * a.G)) * D + g * (D / 4);
                 typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
 #pragma unroll
                 for (int i = 0; i < D / 4; i += 16 / (int)sizeof(T)) {
@@ -307,12 +375,21 @@ template <typename T, int D, int NT> struct Columns {
     }
 
     // 32 positions from p on. masked: some column of the wavefront does not see all of them.
-    __device__ __forceinline__ void step(const Raw<D> &r, uint32_t p, bool masked) {
-        const uint32_t g = (threadIdx.x & 63u) >> 4;
+    // Returns whether a block among them is NaN; its scale counts as 1 then.
+    __device__ __forceinline__ bool step(Raw<D> &r, uint32_t lane, uint32_t p, bool masked) {
+        const uint32_t g = lane >> 4;
+        const bool odd = __any((nan_bytes(r.ks[0]) | nan_bytes(r.ks[1]) | nan_bytes(r.vs)) != 0);
+        if (odd) {
+            r.ks[0] = without_nans(r.ks[0]);
+            r.ks[1] = without_nans(r.ks[1]);
+            r.vs = without_nans(r.vs);
+        }
+        const uint32_t kshift = g * (D / 4) / 32 * 8;   // the lane's block of K, and of V
+        const uint32_t vblock = (lane & 15u) * (D / 16) / 32, vmask = 0xffu << (8u * vblock), vturn = (8u * vblock - 23u) & 31u;
         ff4 s[NT][2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const float sc = scale_of(r.ks[h]);
+            const float sc = __uint_as_float((r.ks[h] >> kshift & 0xffu) << 23);
 #pragma unroll
             for (int t = 0; t < NT; ++t) s[t][h] = ff4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -365,9 +442,20 @@ template <typename T, int D, int NT> struct Columns {
                 if constexpr (P == 2) pp[t][1][j] = half_pair(x[2 * j] - (float)h0, x[2 * j + 1] - (float)h1);
             }
         }
+        // the byte of position j, which lane j of the 16 holds, at the exponent's place
         float sc[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sc[j] = scale_of(r.vs[j]);
+        auto spread = [&](auto j) {
+            const uint32_t w = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)r.vs, 0x150 + decltype(j)::value, 0xf, 0xf, false) & vmask;   // row_newbcast
+            sc[decltype(j)::value] = __uint_as_float(__builtin_amdgcn_alignbit(w, w, vturn));
+        };
+        spread(std::integral_constant<int, 0>{});
+        spread(std::integral_constant<int, 1>{});
+        spread(std::integral_constant<int, 2>{});
+        spread(std::integral_constant<int, 3>{});
+        spread(std::integral_constant<int, 4>{});
+        spread(std::integral_constant<int, 5>{});
+        spread(std::integral_constant<int, 6>{});
+        spread(std::integral_constant<int, 7>{});
         auto two = [&](auto byte) {
             constexpr int B = decltype(byte)::value;
             uint32_t h[8], lo[4], hi[4];
@@ -394,6 +482,7 @@ template <typename T, int D, int NT> struct Columns {
             two(std::integral_constant<int, 2>{});
             two(std::integral_constant<int, 3>{});
         }
+        return odd;
     }
 };
 
@@ -422,61 +511,104 @@ __device__ __forceinline__ uint2 first_nans(const uint8_t *ks, const uint8_t *vs
     return at;
 }
 
-template <typename T, int D, int NT, int NW, int MINB>
-__global__ __launch_bounds__(NW * 64, MINB) void fp4_attn_kernel(Fp4Args a) {
+// Up to 16 NT columns of a sequence and positions [from, to): the eight wavefronts of a
+// workgroup take hw KV heads and ph phases of 32 positions each.
+template <typename T, int D, int NT, bool SPLIT>
+__global__ __launch_bounds__(512, sizeof(T) == 4 && D == 128 ? 2 : 4) void fp4_attn_kernel(Fp4Args args) {
     constexpr uint32_t DL = D / 4;   // output dims of a lane
-    extern __shared__ float lds[];
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
-    // the head groups of a task one behind the other on one XCD (workgroup b runs on XCD b % 8): they share lines of the cache
+    extern __shared__ uint8_t smem[];   // two tiles, then the phases' results
+    float *const lds = (float *)smem;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)smem;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // the head groups of a share one behind the other on one XCD (workgroup b runs on XCD b % 8): they share lines of the scales
     const uint32_t j = blockIdx.x >> 3;
-    const uint32_t task = j / a.head_groups * 8u + (blockIdx.x & 7u), hg = j % a.head_groups;
+    const uint32_t share = j / args.head_groups * 8u + (blockIdx.x & 7u);
+    if (share >= args.shares) return;
     Task w;
-    if (task >= a.tasks || !find_task(a, task, w)) return;
-    const uint32_t hwave = wave % a.hw, phase = wave / a.hw % a.ph, cwave = wave / (a.hw * a.ph);
-    const uint32_t kvh = hg * a.hw + hwave;
-    const uint32_t c0 = w.c0 + cwave * (16u * NT);
-    const uint32_t columns = w.s.n * a.G;   // below 2^25
+    for (uint64_t done = 0; find_task<SPLIT>(late_args(), share, done, w);) {
+    const Fp4Args &a = late_args();
+    const uint32_t lane = fresh_thread() & 63u, g = lane >> 4, at = lane & 15u;
+    const uint32_t hwave = wave & (a.hw - 1), phase = wave / a.hw, head0 = (blockIdx.x >> 3) % a.head_groups * a.hw, kvh = head0 + hwave;
+    const uint32_t c0 = w.c0, columns = w.s.n * a.G;   // below 2^25
 
-    Columns<T, D, NT> col;
-    col.load(a, w, c0, kvh);
-    uint32_t most = 0, fewest = 0xffffffffu;   // positions that columns of the wavefront see
-    if (c0 < columns) {
-        const uint32_t last = (min(c0 + 16u * NT, columns) - 1) / a.G;
-        most = (uint32_t)min(max(w.s.first + (int64_t)last, (int64_t)0), (int64_t)w.s.avail);
-        fewest = (uint32_t)min(max(w.s.first + (int64_t)(c0 / a.G), (int64_t)0), (int64_t)w.s.avail);
-    }
-    const uint64_t from = (uint64_t)w.part * (w.parts > 1 ? w.chunk : 0);
-    const uint32_t end = __builtin_amdgcn_readfirstlane((uint32_t)min((uint64_t)most, w.parts > 1 ? from + w.chunk : (uint64_t)most));
-    uint32_t p = __builtin_amdgcn_readfirstlane((uint32_t)min(from, (uint64_t)0xffffffc0u)) + 32u * phase;
-    const uint32_t step = 32u * a.ph;
-    const size_t row = (size_t)a.kv_heads * (D / 2), srow = (size_t)a.kv_heads * (D / 32);
+    // positions that columns of the tile see: the last ones the most
+    const uint32_t most = (uint32_t)min(max(w.s.first + (int64_t)((min(c0 + 16u * NT, columns) - 1) / a.G), (int64_t)0), (int64_t)w.s.avail);
+    const uint32_t fewest = (uint32_t)min(max(w.s.first + (int64_t)(c0 / a.G), (int64_t)0), (int64_t)w.s.avail);
+    const uint32_t end = __builtin_amdgcn_readfirstlane(min(most, w.to)), from = __builtin_amdgcn_readfirstlane(w.from), step = 32u * a.ph;
     const size_t base = (size_t)w.s.base;   // used where there are positions: not negative then
-    const uint8_t *kc = a.kc + base * row + kvh * (D / 2), *ks = a.ks + base * srow + kvh * (D / 32);
-    const uint8_t *vc = a.vc + base * row + kvh * (D / 2), *vs = a.vs + base * srow + kvh * (D / 32);
-    if (p < end) {
-        Offsets<D> off;
-        set_offsets<D>(off, a.kv_heads, min(31u, end - 1 - p));
-        Raw<D> ra, rb;
-        uint32_t worst = 0;
-        const uint32_t p0 = p, last = p0 + (end - 1 - p0) / step * step;
-        load_raw<D>(ra, off, kc + p * row, ks + p * srow, vc + p * row, vs + p * srow);
-        // The next positions are loaded before these are used; past the end the last ones
-        // again, since under a condition the compiler would wait for the loads at once.
-        auto pass = [&](const Raw<D> &use, Raw<D> &fill) {
-            const uint32_t ahead = min(p + step, last);
-            if (end - ahead < 32u) set_offsets<D>(off, a.kv_heads, end - 1 - ahead);
-            load_raw<D>(fill, off, kc + ahead * row, ks + ahead * srow, vc + ahead * row, vs + ahead * srow);
-            worst = max(worst, max(use.ks[0], use.ks[1]));
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) worst = max(worst, max(use.vs[i], use.vs[i + 1]));
-            col.step(use, p, p + 32u > fewest || p + 32u > end);
-            p += step;
-            return p < end;
-        };
-        while (pass(ra, rb) && pass(rb, ra)) {
+    const uint32_t rows = a.cache_rows - (uint32_t)base;   // of the cache from position 0 on
+    Tile<D> tile;
+    tile.row = a.kv_heads * (D / 2);
+    tile.srow = a.kv_heads * (D / 32);
+    tile.kc = a.kc + base * tile.row + head0 * (D / 2);
+    tile.vc = a.vc + base * tile.row + head0 * (D / 2);
+    tile.ks = a.ks + base * tile.srow + kvh * (D / 32);   // the wavefront's own
+    tile.vs = a.vs + base * tile.srow + kvh * (D / 32);
+    tile.segs = a.hw * Tile<D>::U;
+    tile.heads = a.hw - 1;
+    tile.fold = tile.segs >= 16u ? 0u : 4u - (31u - (uint32_t)__builtin_clz(tile.segs));
+    tile.offsets(lane, wave, step - 1);
+    // the scales of the wavefront's 32 positions of a tile
+    typedef std::conditional_t<D == 128, uint32_t, uint16_t> word;
+    uint32_t ks0 = 0, ks1 = 0, vs0 = 0, kso = at * tile.srow, kso2 = (at + 16u) * tile.srow, vso = ((at & 4u) * 4u + 4u * g + (at & 3u)) * tile.srow;
+    auto fetch = [&](uint32_t p, uint32_t b) {
+        uint32_t q = p + 32u * phase;
+        if (p + step > rows) {   // the cache ends inside the tile: its last row again
+            tile.offsets(lane, wave, rows - 1 - p);
+            q = min(q, rows - 1);
+            kso = min(at, rows - 1 - q) * tile.srow;
+            kso2 = min(at + 16u, rows - 1 - q) * tile.srow;
+            vso = min((at & 4u) * 4u + 4u * g + (at & 3u), rows - 1 - q) * tile.srow;
         }
-        if (__any(worst > 140u)) {
-            const uint2 at = first_nans<D>(ks, vs, (uint32_t)srow, p0, end, step);
+        // rows behind the sequence's end are other sequences' or none's, and no column sees them
+        tile.request(p, wave, lds0 + b * (2 * Tile<D>::kBytes));
+        const uint8_t *ks = tile.ks + (size_t)q * tile.srow, *vs = tile.vs + (size_t)q * tile.srow;
+        ks0 = *(const word *)(ks + kso);
+        ks1 = *(const word *)(ks + kso2);
+        vs0 = *(const word *)(vs + vso);
+    };
+    if (from < end) fetch(from, 0);
+    Columns<T, D, NT> col;
+    col.load(a, w, lane, c0, kvh);
+    if (from < end) {
+        bool odd = false;
+        // offsets of the lane's operands in a tile
+        const uint32_t pos0 = 32u * phase, seg0 = hwave * Tile<D>::U;
+        const uint32_t kat = (pos0 + at) * tile.segs * 16u + ((seg0 + g * (D / 8) / 16) ^ tile.k_turn(pos0 + at)) * 16u + (D == 64 ? (g & 1u) * 8u : 0u);
+        const uint32_t kat2 = (pos0 + 16u + at) * tile.segs * 16u + ((seg0 + g * (D / 8) / 16) ^ tile.k_turn(pos0 + 16u + at)) * 16u + (D == 64 ? (g & 1u) * 8u : 0u);
+        // positions 4 g + r lie r rows behind 4 g, under the same turn
+        const uint32_t vat = (pos0 + 4u * g) * tile.segs * 16u + ((seg0 + at * (D / 32) / 16) ^ tile.v_turn(pos0 + 4u * g)) * 16u + at * (D / 32) % 16u;
+        const uint32_t vat2 = (pos0 + 16u + 4u * g) * tile.segs * 16u + ((seg0 + at * (D / 32) / 16) ^ tile.v_turn(pos0 + 16u + 4u * g)) * 16u + at * (D / 32) % 16u;
+        uint32_t b = 0;
+        for (uint32_t p = from; p < end; p += step, b ^= 1u) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();   // this tile is there, the other one has been read
+            Raw<D> r;
+            r.ks[0] = ks0;
+            r.ks[1] = ks1;
+            r.vs = vs0;
+            // in registers before the next ones are asked for: a wait for them later would be one for the next tile too
+            asm volatile("" : "+v"(r.ks[0]), "+v"(r.ks[1]), "+v"(r.vs));
+            if (p + step < end) fetch(p + step, b ^ 1u);
+            const uint32_t mine = p + 32u * phase;
+            if (mine >= end) continue;
+            const uint8_t *kt = smem + b * (2 * Tile<D>::kBytes), *vt = kt + Tile<D>::kBytes;
+            typedef uint32_t vec __attribute__((ext_vector_type(D / 32)));
+            const vec k0 = *(const vec *)(kt + kat), k1 = *(const vec *)(kt + kat2);
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) {
+                r.k[0][i] = k0[i];
+                r.k[1][i] = k1[i];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                r.v[i] = *(const word *)(vt + vat + i * tile.segs * 16u);
+                r.v[4 + i] = *(const word *)(vt + vat2 + i * tile.segs * 16u);
+            }
+            odd |= col.step(r, lane, mine, mine + 32u > fewest || mine + 32u > end);
+        }
+        if (odd) {
+            const uint2 at = first_nans<D>(tile.ks, tile.vs, tile.srow, from + 32u * phase, end, step);
             const float nan = __uint_as_float(0x7fc00000u);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
@@ -488,6 +620,7 @@ __global__ __launch_bounds__(NW * 64, MINB) void fp4_attn_kernel(Fp4Args a) {
         }
     }
 
+    if (SPLIT || a.ph > 1) __syncthreads();   // the tiles have been read
     // the phases of a head and column tile join in its first one
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -510,7 +643,7 @@ __global__ __launch_bounds__(NW * 64, MINB) void fp4_attn_kernel(Fp4Args a) {
             }
         }
         __syncthreads();
-        if (phase > 0) return;
+        if (phase == 0)
         for (uint32_t h = 1; h < a.ph; ++h) {
             const float *other = lds + ((h - 1) * a.hw + hwave) * kArea + lane;
 #pragma unroll
@@ -528,29 +661,34 @@ __global__ __launch_bounds__(NW * 64, MINB) void fp4_attn_kernel(Fp4Args a) {
                 col.m[t] = now;
             }
         }
+        if constexpr (SPLIT) __syncthreads();   // the areas are written again for the next columns
+        if (phase > 0) {
+            if constexpr (SPLIT) continue;
+            else return;
+        }
     }
-    const uint32_t g = lane >> 4;
+    const Fp4Args &z = late_args();
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         const uint32_t c = c0 + t * 16u + (lane & 15u);
         if (c >= columns) continue;
-        const uint32_t r = c / a.G, gh = c % a.G;
+        const uint32_t r = c / z.G, gh = c % z.G;
         if ((col.bad >> t & 1u) && col.vis[t]) col.l[t] = __uint_as_float(0x7fc00000u);
-        if (w.parts > 1) {
-            const size_t at = ((size_t)task * a.kv_heads + kvh) * a.cols + (c - w.c0);
-            float *to = a.part + at * D + g * DL;
+        if (SPLIT && w.parts > 1) {
+            const size_t at = ((size_t)w.slot * z.kv_heads + kvh) * z.cols + (c - w.c0);
+            float *to = z.part + at * D + g * DL;
 #pragma unroll
             for (int rr = 0; rr < 4; ++rr)
 #pragma unroll
                 for (int i = 0; i < D / 16; i += 4)
                     *(ff4 *)(to + rr * (D / 16) + i) = ff4{col.o[t][i][rr], col.o[t][i + 1][rr], col.o[t][i + 2][rr], col.o[t][i + 3][rr]};
             if (g == 0) {
-                a.part_ml[2 * at] = col.m[t];
-                a.part_ml[2 * at + 1] = col.l[t];
+                z.part_ml[2 * at] = col.m[t];
+                z.part_ml[2 * at + 1] = col.l[t];
             }
         } else {
             const float inv = col.vis[t] ? 1.0f / col.l[t] : 0.0f;
-            T *to = (T *)a.out + ((size_t)(w.s.row0 + r) * a.heads + (size_t)kvh * a.G + gh) * D + g * DL;
+            T *to = (T *)z.out + ((size_t)(w.s.row0 + r) * z.heads + (size_t)kvh * z.G + gh) * D + g * DL;
 #pragma unroll
             for (int rr = 0; rr < 4; ++rr) {
                 typedef T vec __attribute__((ext_vector_type(D / 16 * sizeof(T) > 16 ? 4 : D / 16)));
@@ -564,20 +702,27 @@ __global__ __launch_bounds__(NW * 64, MINB) void fp4_attn_kernel(Fp4Args a) {
                 }
             }
         }
-        if (a.target && w.part == 0 && kvh == 0 && g == 0) {
-            uint32_t *to = a.meta + 2 * ((size_t)w.s.row0 * a.G + c);
-            to[0] = w.first_task;
+        if (SPLIT && w.slot == w.first_slot && kvh == 0 && g == 0) {
+            uint32_t *to = z.meta + 2 * ((size_t)w.s.row0 * z.G + c);
+            to[0] = w.first_slot;
             to[1] = w.parts | (c - w.c0) << 24;
         }
     }
+    if constexpr (!SPLIT) break;
+    }
 }
 
-// One workgroup per row and head: its parts by wavefront, then the wavefronts'.
-template <typename T, int D> __global__ __launch_bounds__(256) void fp4_join_kernel(Fp4Args a) {
-    __shared__ float sm[4], sl[4], so[4][D];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    const uint32_t row = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
-    const uint32_t kvh = head / a.G, gh = head % a.G;
+// Joins the parts of a row and head: W wavefronts take them in turn, eight at a time,
+// and are joined themselves. Workgroups of 4 units for W = 1, else of one.
+template <typename T, int D, int W> __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void fp4_join_kernel(Fp4Args a) {
+    __shared__ float sm[W], sl[W], so[W][D];
+    const uint32_t lane = threadIdx.x & 63u, wave = W == 1 ? 0u : threadIdx.x >> 6;
+    const uint32_t unit = __builtin_amdgcn_readfirstlane(W == 1 ? blockIdx.x * 4u + (threadIdx.x >> 6) : blockIdx.x);
+    const uint32_t row = unit / a.heads, head = unit - row * a.heads;
+    if (row >= a.rows) return;
+    const uint32_t kvh = head / a.G, gh = head - kvh * a.G;
+    const uint32_t *meta = a.meta + 2 * ((size_t)row * a.G + gh);
+    const uint32_t first = meta[0], parts = meta[1] & 0xffffffu, c = meta[1] >> 24;
     uint32_t seq = row / max(1u, a.rows / a.nseq);
     if (a.q_start) {
         seq = 0xffffffffu;
@@ -586,61 +731,72 @@ template <typename T, int D> __global__ __launch_bounds__(256) void fp4_join_ker
             const uint64_t mine = __ballot(s < a.nseq && a.q_start[s] <= (int64_t)row && (int64_t)row < a.q_start[s + 1]);
             if (mine) seq = s0 + (uint32_t)__builtin_ctzll(mine);
         }
-        if (seq == 0xffffffffu) return;   // a row of no sequence
+        if (seq == 0xffffffffu) return;   // a row of no sequence: what meta holds is not its own
     }
+    if (parts < 2 || (uint64_t)first + parts > a.slots || c >= a.cols) return;
     const SeqRows of = seq_rows(a, seq);
     const bool sees = of.avail && of.first + (int64_t)(row - of.row0) > 0;
-    const uint32_t *meta = a.meta + 2 * ((size_t)row * a.G + gh);
-    const uint32_t first = meta[0], parts = meta[1] & 0xffffffu, c = meta[1] >> 24;
-    if (parts < 2 || (uint64_t)first + parts > a.tasks || c >= a.cols) return;
     constexpr int E = D / 64;
+    typedef float vec __attribute__((ext_vector_type(E)));
     const size_t stride = (size_t)a.kv_heads * a.cols;
     const size_t at0 = ((size_t)first * a.kv_heads + kvh) * a.cols + c;
-    float m = -INFINITY, l = 0.0f, o[E] = {};
-    for (uint32_t i0 = wave * 8; i0 < parts; i0 += 32) {
-        float pm[8], pl[8], po[8][E];
+    float m = -INFINITY, l = 0.0f;
+    vec o = {};
+    for (uint32_t i0 = wave * 8; i0 < parts; i0 += W * 8) {
+        float2 ml[8];
+        vec po[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const bool there = i0 + i < parts;
-            const size_t at = at0 + (size_t)(there ? i0 + i : i0) * stride;
-            pm[i] = there ? a.part_ml[2 * at] : -INFINITY;
-            pl[i] = there ? a.part_ml[2 * at + 1] : 0.0f;
-#pragma unroll
-            for (int e = 0; e < E; ++e) po[i][e] = there ? a.part[at * D + lane * E + e] : 0.0f;
+            const size_t at = at0 + (size_t)min(i0 + i, parts - 1) * stride;
+            ml[i] = *(const float2 *)(a.part_ml + 2 * at);
+            po[i] = *(const vec *)(a.part + at * D + lane * E);
         }
         float now = m;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) now = fmaxf(now, pm[i]);
+        for (int i = 0; i < 8; ++i) {
+            if (i0 + i >= parts) ml[i].x = -INFINITY;
+            now = fmaxf(now, ml[i].x);
+        }
         const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - now);
         l *= f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] *= f;
+        o *= f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float fi = pm[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(pm[i] - now);
-            l += pl[i] * fi;
-#pragma unroll
-            for (int e = 0; e < E; ++e) o[e] += po[i][e] * fi;
+            const float fi = ml[i].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[i].x - now);
+            // a part that has seen nothing holds zeros, or NaN where a block was marked
+            if (i0 + i < parts) {
+                l += ml[i].y * fi;
+                o += po[i] * fi;
+            }
         }
         m = now;
     }
-    if (lane == 0) {
-        sm[wave] = m;
-        sl[wave] = l;
-    }
+    T *out = (T *)a.out + ((size_t)row * a.heads + head) * D;
+    if constexpr (W == 1) {
+        const float inv = 1.0f / l;
 #pragma unroll
-    for (int e = 0; e < E; ++e) so[wave][lane * E + e] = o[e];
-    __syncthreads();
-    if (threadIdx.x >= D) return;
-    const float now = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-    float total = 0.0f, sum = 0.0f;
+        for (int e = 0; e < E; ++e) out[lane * E + e] = sees ? (T)(o[e] * inv) : (T)0.0f;
+    } else {
+        if (lane == 0) {
+            sm[wave] = m;
+            sl[wave] = l;
+        }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float f = sm[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm[i] - now);
-        total += sl[i] * f;
-        sum += so[i][threadIdx.x] * f;
+        for (int e = 0; e < E; ++e) so[wave][lane * E + e] = o[e];
+        __syncthreads();
+        if (threadIdx.x >= D) return;
+        float now = sm[0];
+#pragma unroll
+        for (int i = 1; i < W; ++i) now = fmaxf(now, sm[i]);
+        float total = 0.0f, sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            const float f = sm[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm[i] - now);
+            total += sl[i] * f;
+            sum += so[i][threadIdx.x] * f;
+        }
+        out[threadIdx.x] = sees ? (T)(sum / total) : (T)0.0f;
     }
-    ((T *)a.out)[((size_t)row * a.heads + head) * D + threadIdx.x] = sees ? (T)(sum / total) : (T)0.0f;
 }
 
 // ---- many columns -----------------------------------------------------------------
@@ -685,26 +841,25 @@ template <int D> __device__ __forceinline__ Nans<D> all_nans(const uint8_t *ks, 
     return at;
 }
 
-template <typename T, int D, int TP>
-__global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args a) {
+template <typename T, int D, int TP, bool SPLIT>
+__global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
     constexpr int P = sizeof(T) == 4 ? 2 : 1, NB = TP / 32, QN = D / 16, ND = D / 32;
     constexpr float kBias = P == 2 ? 13.0f : 7.0f, kSlack = P == 2 ? 2.0f : 8.0f;
     constexpr uint32_t kTile = TP * D * 2u;   // bytes of a tile of K, and of V
     constexpr uint32_t kUnits = TP * D / 32;  // 16-byte pieces of K, and quads of positions x 8 dims of V
     static_assert(kUnits == 256 || kUnits == 128, "a lane has one unit of each, or of one of them");
     extern __shared__ uint8_t smem[];         // K, V, K, V
-    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t col = lane & 31u, h = lane >> 5;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // KV heads change fastest, so with eight of them an XCD's L2 holds the lines of one or two
-    const uint32_t task = blockIdx.x / a.kv_heads, kvh = blockIdx.x % a.kv_heads;
+    const uint32_t share = blockIdx.x / args.kv_heads, kvh = blockIdx.x % args.kv_heads;
     Task w;
-    if (task >= a.tasks || !find_task(a, task, w)) return;
+    for (uint64_t done = 0; find_task<SPLIT>(late_args(), share, done, w);) {
+    const Fp4Args &a = late_args();
+    const uint32_t tid = fresh_thread(), lane = tid & 63u, col = lane & 31u, h = lane >> 5;
     const uint32_t columns = w.s.n * a.G;
     auto seen = [&](uint32_t c) { return (uint32_t)min(max(w.s.first + (int64_t)(c / a.G), (int64_t)0), (int64_t)w.s.avail); };
     const uint32_t group_hi = seen(min(w.c0 + 127u, columns - 1));   // the last column sees most
-    const uint64_t from = w.parts > 1 ? (uint64_t)w.part * w.chunk : 0u;
-    const uint32_t p0 = __builtin_amdgcn_readfirstlane((uint32_t)min(from, (uint64_t)group_hi));
-    const uint32_t p1 = __builtin_amdgcn_readfirstlane(w.parts > 1 ? (uint32_t)min((uint64_t)group_hi, from + w.chunk) : group_hi);
+    const uint32_t p0 = __builtin_amdgcn_readfirstlane(min(w.from, group_hi)), p1 = __builtin_amdgcn_readfirstlane(min(w.to, group_hi));
     const uint32_t c0 = w.c0 + 32u * wave;
     const bool idle = c0 >= columns;
     const uint32_t wave_lo = idle ? 0u : __builtin_amdgcn_readfirstlane(seen(c0));
@@ -718,7 +873,7 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args a) {
     const uint8_t *vc = a.vc + base * row + kvh * (D / 2), *vs = a.vs + base * srow + kvh * (D / 32);
 
     // what a lane loads of a tile: block kb of position kn of K, and dims 8 vd .. of positions 4 vq .. of V
-    const uint32_t ku = threadIdx.x, vu = kUnits == 256 ? threadIdx.x : threadIdx.x ^ 128u;
+    const uint32_t ku = tid, vu = kUnits == 256 ? tid : tid ^ 128u;
     const bool has_k = kUnits == 256 || ku < kUnits, has_v = kUnits == 256 || vu < kUnits;
     const uint32_t kn = (ku & 15u) + ku / (D / 2) * 16u, kb = ku / 16u % (D / 32), vd = vu % (D / 8), vq = vu / (D / 8);
     ju4 kr;
@@ -954,23 +1109,28 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args a) {
 #pragma unroll
                 for (int v = 0; v < 16; ++v) o[d][v] = nan;
     }
-    if (c0 + col >= columns) return;
+    if constexpr (SPLIT) __syncthreads();   // the tiles are written again for the next columns
+    if (c0 + col >= columns) {
+        if constexpr (SPLIT) continue;
+        else return;
+    }
     if (bad && vis) l = nan;
-    if (w.parts > 1) {
-        const size_t at = ((size_t)task * a.kv_heads + kvh) * a.cols + (c - w.c0);
-        float *to = a.part + at * D;
+    const Fp4Args &z = late_args();
+    if (SPLIT && w.parts > 1) {
+        const size_t at = ((size_t)w.slot * z.kv_heads + kvh) * z.cols + (c - w.c0);
+        float *to = z.part + at * D;
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
             for (int j = 0; j < 4; ++j) *(jf4 *)(to + 32 * d + 8 * j + 4 * h) = jf4{o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]};
         if (h == 0) {
             // in powers of two, less what the rounding of c2 has moved
-            a.part_ml[2 * at] = m == -INFINITY ? m : far ? m * cs : kBias - c2;
-            a.part_ml[2 * at + 1] = l;
+            z.part_ml[2 * at] = m == -INFINITY ? m : far ? m * cs : kBias - c2;
+            z.part_ml[2 * at + 1] = l;
         }
     } else {
         const float inv = vis ? 1.0f / l : 0.0f;
-        T *to = (T *)a.out + qat * D;
+        T *to = (T *)z.out + qat * D;
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -982,16 +1142,22 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args a) {
                 *(t4 *)(to + 32 * d + 8 * j + 4 * h) = y;
             }
     }
-    if (a.target && w.part == 0 && kvh == 0 && h == 0) {
-        uint32_t *to = a.meta + 2 * ((size_t)w.s.row0 * a.G + c);
-        to[0] = w.first_task;
+    if (SPLIT && w.slot == w.first_slot && kvh == 0 && h == 0) {
+        uint32_t *to = z.meta + 2 * ((size_t)w.s.row0 * z.G + c);
+        to[0] = w.first_slot;
         to[1] = w.parts | (c - w.c0) << 24;
+    }
+    if constexpr (!SPLIT) break;
     }
 }
 
-template <typename T, int D> int launch_join(janus_ctx *ctx, const Fp4Args &a) {
+template <typename T, int D> int launch_join(janus_ctx *ctx, const Fp4Args &a, uint64_t tiles) {
     if (!a.target) return JANUS_OK;
-    hipLaunchKernelGGL((fp4_join_kernel<T, D>), dim3(a.rows * a.heads), dim3(256), 0, ctx->stream, a);
+    const uint32_t units = a.rows * a.heads;
+    const uint64_t parts = a.shares / tiles + 1;   // of a tile, in the mean
+    if (parts <= 8) hipLaunchKernelGGL((fp4_join_kernel<T, D, 1>), dim3((units + 3) / 4), dim3(256), 0, ctx->stream, a);
+    else if (parts <= 32) hipLaunchKernelGGL((fp4_join_kernel<T, D, 4>), dim3(units), dim3(256), 0, ctx->stream, a);
+    else hipLaunchKernelGGL((fp4_join_kernel<T, D, 16>), dim3(units), dim3(1024), 0, ctx->stream, a);
     JANUS_LAUNCH_CHECK(ctx);
     return JANUS_OK;
 }
@@ -999,6 +1165,7 @@ template <typename T, int D> int launch_join(janus_ctx *ctx, const Fp4Args &a) {
 template <typename T, int D> int launch_dim(janus_ctx *ctx, Fp4Args &a, uint32_t max_len) {
     const uint32_t mean = (a.rows + a.nseq - 1) / a.nseq;   // rows of a sequence
     const bool few = (uint64_t)mean * a.G <= 16;
+    constexpr int kFewCu = sizeof(T) == 4 && D == 128 ? 1 : 2;   // workgroups that a CU holds
     if (few) {
         a.cols = 16;
         a.hw = a.kv_heads % 8 == 0 ? 8 : a.kv_heads % 4 == 0 ? 4 : a.kv_heads % 2 == 0 ? 2 : 1;
@@ -1012,18 +1179,16 @@ template <typename T, int D> int launch_dim(janus_ctx *ctx, Fp4Args &a, uint32_t
     a.head_groups = a.kv_heads / a.hw;
     // every tile of every sequence, one more where rows do not fill the last
     const uint64_t tiles = (uint64_t)a.rows * a.G / a.cols + a.nseq;
-    const uint64_t want = (uint64_t)ctx->num_cus * 2 / a.head_groups;
-    a.least = a.step;
+    const uint64_t busy = std::max<uint64_t>(1, std::min<uint64_t>(tiles, ((uint64_t)a.rows * a.G + a.cols - 1) / a.cols + a.nseq - 1));
+    // shares that run at once
+    const uint64_t slots = std::max<uint64_t>(1, (uint64_t)ctx->num_cus * (few ? kFewCu : 2) / a.head_groups);
+    a.least = 2;
     a.target = 0;
-    uint64_t tasks = tiles;
-    const uint64_t busy = std::min<uint64_t>(tiles, ((uint64_t)a.rows * a.G + a.cols - 1) / a.cols + a.nseq - 1);
-    if (max_len > 4 * a.least && busy * 2 < want * 3) {
-        a.target = (uint32_t)std::max<uint64_t>(want, 1);
-        tasks += a.target;
-    }
-    a.tasks = (uint32_t)tasks;   // * head_groups below 2^21 + 2^22 + 2^10, 512 lanes each
-    if (a.target) {
-        const size_t cells = (size_t)a.tasks * a.kv_heads * a.cols;
+    a.shares = (uint32_t)tiles;   // * head_groups below 2^21 + 2^22, up to 512 lanes each
+    if (max_len > 4 * a.step && (few ? busy < 4 * slots : 2 * busy <= slots)) {
+        a.shares = a.target = (uint32_t)slots;
+        a.slots = (uint32_t)(slots + tiles);
+        const size_t cells = (size_t)a.slots * a.kv_heads * a.cols;
         const size_t meta = ((size_t)a.rows * a.G * 8 + 255) / 256 * 256;
         if (int e = ensure_attn_ws(ctx, meta + cells * (D + 2) * 4)) return e;
         a.meta = (uint32_t *)ctx->attn_ws;
@@ -1031,15 +1196,18 @@ template <typename T, int D> int launch_dim(janus_ctx *ctx, Fp4Args &a, uint32_t
         a.part_ml = a.part + cells * D;
     }
     if (few) {
-        const uint32_t lds = (a.ph - 1) * a.hw * (D / 4 + 2) * 64u * 4u;
-        const dim3 grid((a.tasks + 7) / 8 * 8 * a.head_groups), block(512);
-        hipLaunchKernelGGL((fp4_attn_kernel<T, D, 1, 8, 2>), grid, block, lds, ctx->stream, a);
+        const uint32_t lds = 4 * Tile<D>::kBytes;   // at least 7 (D / 4 + 2) 256 for the phases
+        const dim3 grid((a.shares + 7) / 8 * 8 * a.head_groups), block(512);
+        if (a.target) hipLaunchKernelGGL((fp4_attn_kernel<T, D, 1, true>), grid, block, lds, ctx->stream, a);
+        else hipLaunchKernelGGL((fp4_attn_kernel<T, D, 1, false>), grid, block, lds, ctx->stream, a);
     } else {
         constexpr int TP = D == 128 && sizeof(T) == 4 ? 32 : 64;
-        hipLaunchKernelGGL((fp4_wide_kernel<T, D, TP>), dim3(a.tasks * a.kv_heads), dim3(256), 4 * TP * D * 2, ctx->stream, a);
+        const dim3 grid(a.shares * a.kv_heads), block(256);
+        if (a.target) hipLaunchKernelGGL((fp4_wide_kernel<T, D, TP, true>), grid, block, 4 * TP * D * 2, ctx->stream, a);
+        else hipLaunchKernelGGL((fp4_wide_kernel<T, D, TP, false>), grid, block, 4 * TP * D * 2, ctx->stream, a);
     }
     JANUS_LAUNCH_CHECK(ctx);
-    return launch_join<T, D>(ctx, a);
+    return launch_join<T, D>(ctx, a, busy);
 }
 
 }  // namespace

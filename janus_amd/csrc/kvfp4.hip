@@ -95,19 +95,16 @@ template <typename T> __global__ __launch_bounds__(256) void kv_read_fp4_kernel(
     const uint32_t b = (is_v ? a.vs : a.ks)[at / 32];
     T *out = (T *)(is_v ? a.v : a.k) + (size_t)r * a.elems + i;
     typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
+    // binary16 holds every value that the append wrote; what others wrote is rounded to it
     const bool odd = b > 140u;
-    const float s = __uint_as_float(min(max(b, 104u), 140u) << 23);
-    float x[8];
-    jf2 f;
-    f = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, s, 0); x[0] = f[0]; x[1] = f[1];
-    f = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, s, 1); x[2] = f[0]; x[3] = f[1];
-    f = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, s, 2); x[4] = f[0]; x[5] = f[1];
-    f = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, s, 3); x[6] = f[0]; x[7] = f[1];
+    const float s = __uint_as_float(min(b, 140u) << 23);
+    const jh2 x[4] = {__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(code, s, 0), __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(code, s, 1),
+                      __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(code, s, 2), __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(code, s, 3)};
 #pragma unroll
     for (int j = 0; j < 8; j += 16 / (int)sizeof(T)) {
         vec w;
 #pragma unroll
-        for (int t = 0; t < 16 / (int)sizeof(T); ++t) w[t] = (T)(odd ? __uint_as_float(0x7fc00000u) : x[j + t]);
+        for (int t = 0; t < 16 / (int)sizeof(T); ++t) w[t] = odd ? (T)__uint_as_float(0x7fc00000u) : (T)x[(j + t) >> 1][t & 1];
         *(vec *)(out + j) = w;
     }
 }

@@ -217,5 +217,6 @@ def test_the_reference_of_the_format():
         x[0, 3] = odd
         codes, scales = encode(x)
         assert scales.item() == 255 and not codes.any() and decode(codes, scales).isnan().all()
-    assert decode(torch.tensor([[0x21] * 16], dtype=torch.uint8), torch.zeros(1, 1, dtype=torch.uint8))[0, :2].tolist() == \
-        [0.5 * 2.0 ** -23, 2.0 ** -23]
+    codes = torch.tensor([[0x21] * 16], dtype=torch.uint8)
+    for byte, pair in ((104, [0.5 * 2.0 ** -23, 2.0 ** -23]), (103, [0.0, 2.0 ** -24]), (102, [0.0, 0.0]), (0, [0.0, 0.0]), (140, [4096.0, 8192.0])):
+        assert decode(codes, torch.tensor([[byte]], dtype=torch.uint8))[0, :2].tolist() == pair

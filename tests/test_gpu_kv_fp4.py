@@ -109,7 +109,7 @@ def test_rows_that_are_left_out(engine):
 
 
 def test_read_of_foreign_scales(engine):
-    """Scale bytes that no append writes: below 104 they count as 104, above 140 the block is NaN."""
+    """Scale bytes that no append writes: below 104 the values are rounded to binary16, above 140 the block is NaN."""
     gen = torch.Generator().manual_seed(6)
     kc, _ = random_cache(gen, 256, 1, 32)
     ks = torch.arange(256, dtype=torch.uint8).view(256, 1, 1)
