@@ -44,7 +44,7 @@ struct Fp4Args {
     const uint8_t *kc, *ks, *vc, *vs;     // [cache rows][kv_heads][D / 2] and [D / 32]
     void *out;                            // [rows][heads][D]
     float *part, *part_ml;                // split: [slot][kv_heads][cols][D] and (m, l)
-    uint32_t *meta;                       // split: [rows * G] (first slot, parts | column << 24)
+    uint32_t *meta;                       // split: [rows * G] (first slot, parts | sees nothing << 23 | column << 24)
     const int32_t *q_start, *row_base, *seq_lens;
     uint32_t rows, nseq, heads, kv_heads, G;
     uint32_t cache_rows, max_seq;
@@ -78,33 +78,33 @@ __device__ __forceinline__ uint32_t groups_umax(uint32_t v) {
 struct SeqRows {
     uint32_t row0, n;    // its rows
     uint32_t avail;      // positions that its last row sees
-    int64_t first;       // positions that row 0 sees (may be below 1)
-    int64_t base;        // cache row of position 0
+    int32_t first;       // positions that row 0 sees (may be below 1), each row one more than the last
+    uint32_t base;       // cache row of position 0 (0 where avail is)
 };
 __device__ __forceinline__ SeqRows seq_rows(const Fp4Args &a, uint32_t s) {
     SeqRows q{};
     if (s >= a.nseq) return q;
-    int64_t r0, r1;
+    const uint32_t each = a.rows / a.nseq;
+    int32_t r0 = (int32_t)(s * each), r1 = r0 + (int32_t)each;   // rows are below 2^25
     if (a.q_start) {
         r0 = a.q_start[s];
         r1 = a.q_start[s + 1];
-    } else {
-        const uint32_t each = a.rows / a.nseq;
-        r0 = (int64_t)s * each;
-        r1 = r0 + each;
     }
-    r0 = min(max(r0, (int64_t)0), (int64_t)a.rows);
-    r1 = min(max(r1, r0), (int64_t)a.rows);
+    const int32_t given = a.seq_lens ? a.seq_lens[s] : 0x7fffffff;
+    const int64_t base = a.row_base ? (int64_t)a.row_base[s] : (int64_t)((uint64_t)s * a.max_seq);
+    r0 = min(max(r0, 0), (int32_t)a.rows);
+    r1 = min(max(r1, r0), (int32_t)a.rows);
     q.row0 = (uint32_t)r0;
     q.n = (uint32_t)(r1 - r0);
-    const int64_t len = a.seq_lens ? (int64_t)a.seq_lens[s] : (int64_t)q.n;
-    q.base = a.row_base ? (int64_t)a.row_base[s] : (int64_t)s * a.max_seq;
-    q.first = len - q.n + 1;
-    int64_t avail = min(len, (int64_t)a.max_seq);
-    avail = q.base < 0 ? 0 : min(avail, (int64_t)a.cache_rows - q.base);
-    q.avail = (uint32_t)max(avail, (int64_t)0);
+    const int32_t len = max(a.seq_lens ? given : r1 - r0, -(1 << 26));
+    q.first = len - (r1 - r0) + 1;
+    const bool inside = base >= 0 && base < (int64_t)a.cache_rows;
+    q.base = inside ? (uint32_t)base : 0u;
+    q.avail = inside && len > 0 ? min(min((uint32_t)len, a.max_seq), a.cache_rows - q.base) : 0u;
     return q;
 }
+// Positions that row r of a sequence sees.
+__device__ __forceinline__ uint32_t seen_of(const SeqRows &s, uint32_t r) { return (uint32_t)min(max(s.first + (int32_t)r, 0), (int32_t)min(s.avail, 0x7fffffffu)); }
 
 // Sum over the lanes up to this one, without LDS traffic.
 __device__ __forceinline__ uint32_t scan_dpp(uint32_t v) {
@@ -117,9 +117,6 @@ __device__ __forceinline__ uint32_t scan_dpp(uint32_t v) {
     return v;
 }
 __device__ __forceinline__ uint32_t lane_value(uint32_t v, uint32_t lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)lane); }
-__device__ __forceinline__ int64_t lane_value(int64_t v, uint32_t lane) {
-    return (int64_t)((uint64_t)lane_value((uint32_t)((uint64_t)v >> 32), lane) << 32 | lane_value((uint32_t)v, lane));
-}
 
 // The kernel's arguments, read again where they are used: held from the start they fill the
 // scalar registers, and what spills takes vector registers and scratch.
@@ -145,8 +142,6 @@ struct Task {
     uint32_t slot, first_slot, parts;   // its place among the parts of these columns; 1 part: the result
 };
 
-__device__ __forceinline__ uint64_t quotient(uint64_t a, uint64_t b) { return (a | b) >> 32 ? a / b : (uint32_t)a / (uint32_t)b; }
-
 // The work of share `share` that starts `done` units into it; false if there is none.
 // Without a split a share is a tile, that is, cols columns of a sequence. Else
 // the positions of all tiles, one behind the other in units of a.step, are cut into
@@ -155,43 +150,41 @@ __device__ __forceinline__ uint64_t quotient(uint64_t a, uint64_t b) { return (a
 // anew with each of 64 sequences of up to 8000: 93 us, some CUs with three of them and some with two.)
 // A share and a tile that meet have the slot share + tile, both counted from 0, of the
 // partial results: a step along the positions raises one of them or both.
-template <bool SPLIT> __device__ __forceinline__ bool find_task(const Fp4Args &a, uint32_t share, uint64_t &done, Task &w) {
+template <bool SPLIT> __device__ __forceinline__ bool find_task(const Fp4Args &a, uint32_t share, uint32_t &done, Task &w) {
     const uint32_t lane = threadIdx.x & 63u, shift = 31u - (uint32_t)__builtin_clz(a.cols);   // cols is a power of two
+    const uint32_t unit = SPLIT ? 31u - (uint32_t)__builtin_clz(a.step) : 0u;                 // and so is step
     SeqRows q = seq_rows(a, lane);
-    auto tiles_of = [&]() { return (q.n * a.G + a.cols - 1) >> shift; };   // rows * heads is below 2^25
-    auto units_of = [&]() { return SPLIT ? max(1u, (uint32_t)(((uint64_t)q.avail + a.step - 1) / a.step)) : 1u; };
-    uint64_t quota = 1;
+    // the host has seen to it that all units together are below 2^31
+    auto tiles_of = [&]() { return (q.n * a.G + a.cols - 1) >> shift; };
+    auto units_of = [&]() { return SPLIT ? max(1u, (q.avail + a.step - 1) >> unit) : 1u; };
+    uint32_t quota = 1;
     if constexpr (SPLIT) {
-        uint64_t total = 0;
+        uint32_t total = 0;
         for (uint32_t s0 = 0;;) {
-            // (the sum of 64 products of 2^19 tiles and 2^26 units would pass 32 bits: in two halves)
-            const uint64_t units = (uint64_t)tiles_of() * units_of();
-            total += (uint64_t)lane_value(scan_dpp((uint32_t)(units & 0xffffffu)), 63) + ((uint64_t)lane_value(scan_dpp((uint32_t)(units >> 24)), 63) << 24);
+            total += lane_value(scan_dpp(tiles_of() * units_of()), 63);
             if ((s0 += 64) >= a.nseq) break;
             q = seq_rows(a, s0 + lane);
         }
         if (a.nseq > 64) q = seq_rows(a, lane);
-        quota = max(quotient(total + a.target - 1, a.target), (uint64_t)a.least);
+        quota = max((total + a.target - 1) / a.target, a.least);
         if (done >= quota) return false;
     }
-    uint64_t at = share * quota + done, before = 0;   // units from the first tile on; tiles before these sequences
-    uint64_t start = 0;                                         // units before these sequences
+    uint32_t at = share * quota + done, start = 0, before = 0;   // units from the first tile on; units and tiles before these sequences
+    if (SPLIT && (uint64_t)share * quota + done >= 0x80000000u) return false;
     for (uint32_t s0 = 0;;) {
         const uint32_t tiles = tiles_of(), per = units_of();
-        const uint64_t units = (uint64_t)tiles * per;
-        const uint32_t lo = scan_dpp((uint32_t)(units & 0xffffffu)), hi = scan_dpp((uint32_t)(units >> 24)), upto_tiles = scan_dpp(tiles);
-        const uint64_t upto = start + lo + ((uint64_t)hi << 24);
+        const uint32_t upto = start + scan_dpp(tiles * per), upto_tiles = SPLIT ? scan_dpp(tiles) : 0u;
         const uint64_t here = __ballot(at < upto);
         if (here) {
             const uint32_t l = __builtin_amdgcn_readfirstlane((uint32_t)__builtin_ctzll(here));
             w.s.row0 = lane_value(q.row0, l);
             w.s.n = lane_value(q.n, l);
             w.s.avail = lane_value(q.avail, l);
-            w.s.first = lane_value(q.first, l);
+            w.s.first = (int32_t)lane_value((uint32_t)q.first, l);
             w.s.base = lane_value(q.base, l);
             const uint32_t each = lane_value(per, l), all = lane_value(tiles, l);
-            const uint64_t first = (uint64_t)lane_value((int64_t)upto, l) - (uint64_t)all * each;   // the sequence's first unit
-            const uint32_t in = (uint32_t)(at - first), tile = each == 1 ? in : in / each, off = in - tile * each;
+            const uint32_t first = lane_value(upto, l) - all * each;   // the sequence's first unit
+            const uint32_t in = at - first, tile = SPLIT ? in / each : in, off = SPLIT ? in - tile * each : 0u;
             w.c0 = (all - 1 - tile) << shift;   // the last rows see most: they come first
             if constexpr (!SPLIT) {
                 w.from = 0;
@@ -199,20 +192,19 @@ template <bool SPLIT> __device__ __forceinline__ bool find_task(const Fp4Args &a
                 w.parts = 1;
                 return true;
             }
-            const uint32_t n = (uint32_t)min(quota - done, (uint64_t)(each - off));
-            w.from = (uint32_t)min((uint64_t)off * a.step, (uint64_t)w.s.avail);
-            w.to = (uint32_t)min(((uint64_t)off + n) * a.step, (uint64_t)w.s.avail);
-            const uint32_t number = (uint32_t)before + lane_value(upto_tiles, l) - all + tile;
-            const uint64_t u0 = first + (uint64_t)tile * each;
-            const uint32_t s_first = (uint32_t)quotient(u0, quota), s_last = (uint32_t)quotient(u0 + each - 1, quota);
+            const uint32_t n = min(quota - done, each - off);
+            w.from = min(off << unit, w.s.avail);
+            w.to = min((off + n) << unit, w.s.avail);
+            const uint32_t number = before + lane_value(upto_tiles, l) - all + tile;
+            const uint32_t u0 = first + tile * each, s_first = u0 / quota, s_last = (u0 + each - 1) / quota;
             w.parts = s_last - s_first + 1;
             w.slot = share + number;
             w.first_slot = s_first + number;
             done += n;
             return true;
         }
-        start = (uint64_t)lane_value((int64_t)upto, 63);
-        before += lane_value(upto_tiles, 63);
+        start = lane_value(upto, 63);
+        if constexpr (SPLIT) before += lane_value(upto_tiles, 63);
         if ((s0 += 64) >= a.nseq) return false;
         q = seq_rows(a, s0 + lane);
     }
@@ -321,7 +313,7 @@ template <typename T, int D, int NT> struct Columns {
             float x[D / 4];
             uint32_t top = 0;
             if (there) {
-                vis[t] = (uint32_t)min(max(w.s.first + (int64_t)row, (int64_t)0), (int64_t)w.s.avail);
+                vis[t] = seen_of(w.s, row);
                 const T *src = (const T *)a.q + ((size_t)(w.s.row0 + row) * a.heads + (size_t)kvh * a.G + (c - row * a.G)) * D + g * (D / 4);
                 typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
 #pragma unroll
@@ -525,18 +517,17 @@ __global__ __launch_bounds__(512, sizeof(T) == 4 && D == 128 ? 2 : 4) void fp4_a
     const uint32_t share = j / args.head_groups * 8u + (blockIdx.x & 7u);
     if (share >= args.shares) return;
     Task w;
-    for (uint64_t done = 0; find_task<SPLIT>(late_args(), share, done, w);) {
+    for (uint32_t done = 0; find_task<SPLIT>(late_args(), share, done, w);) {
     const Fp4Args &a = late_args();
     const uint32_t lane = fresh_thread() & 63u, g = lane >> 4, at = lane & 15u;
     const uint32_t hwave = wave & (a.hw - 1), phase = wave / a.hw, head0 = (blockIdx.x >> 3) % a.head_groups * a.hw, kvh = head0 + hwave;
     const uint32_t c0 = w.c0, columns = w.s.n * a.G;   // below 2^25
 
     // positions that columns of the tile see: the last ones the most
-    const uint32_t most = (uint32_t)min(max(w.s.first + (int64_t)((min(c0 + 16u * NT, columns) - 1) / a.G), (int64_t)0), (int64_t)w.s.avail);
-    const uint32_t fewest = (uint32_t)min(max(w.s.first + (int64_t)(c0 / a.G), (int64_t)0), (int64_t)w.s.avail);
+    const uint32_t most = seen_of(w.s, (min(c0 + 16u * NT, columns) - 1) / a.G), fewest = seen_of(w.s, c0 / a.G);
     const uint32_t end = __builtin_amdgcn_readfirstlane(min(most, w.to)), from = __builtin_amdgcn_readfirstlane(w.from), step = 32u * a.ph;
-    const size_t base = (size_t)w.s.base;   // used where there are positions: not negative then
-    const uint32_t rows = a.cache_rows - (uint32_t)base;   // of the cache from position 0 on
+    const size_t base = w.s.base;
+    const uint32_t rows = a.cache_rows - w.s.base;   // of the cache from position 0 on
     Tile<D> tile;
     tile.row = a.kv_heads * (D / 2);
     tile.srow = a.kv_heads * (D / 32);
@@ -705,7 +696,7 @@ __global__ __launch_bounds__(512, sizeof(T) == 4 && D == 128 ? 2 : 4) void fp4_a
         if (SPLIT && w.slot == w.first_slot && kvh == 0 && g == 0) {
             uint32_t *to = z.meta + 2 * ((size_t)w.s.row0 * z.G + c);
             to[0] = w.first_slot;
-            to[1] = w.parts | (c - w.c0) << 24;
+            to[1] = w.parts | (col.vis[t] ? 0u : 1u << 23) | (c - w.c0) << 24;
         }
     }
     if constexpr (!SPLIT) break;
@@ -721,21 +712,15 @@ template <typename T, int D, int W> __global__ __launch_bounds__(W == 1 ? 256 : 
     const uint32_t row = unit / a.heads, head = unit - row * a.heads;
     if (row >= a.rows) return;
     const uint32_t kvh = head / a.G, gh = head - kvh * a.G;
-    const uint32_t *meta = a.meta + 2 * ((size_t)row * a.G + gh);
-    const uint32_t first = meta[0], parts = meta[1] & 0xffffffu, c = meta[1] >> 24;
-    uint32_t seq = row / max(1u, a.rows / a.nseq);
-    if (a.q_start) {
-        seq = 0xffffffffu;
-        for (uint32_t s0 = 0; s0 < a.nseq && seq == 0xffffffffu; s0 += 64) {
-            const uint32_t s = s0 + lane;
-            const uint64_t mine = __ballot(s < a.nseq && a.q_start[s] <= (int64_t)row && (int64_t)row < a.q_start[s + 1]);
-            if (mine) seq = s0 + (uint32_t)__builtin_ctzll(mine);
-        }
-        if (seq == 0xffffffffu) return;   // a row of no sequence: what meta holds is not its own
+    const uint2 meta = *(const uint2 *)(a.meta + 2 * ((size_t)row * a.G + gh));
+    if (a.q_start) {   // a row of no sequence: what meta holds is not its own
+        bool mine = false;
+        for (uint32_t s = lane; s < a.nseq; s += 64) mine |= a.q_start[s] <= (int32_t)row && (int32_t)row < a.q_start[s + 1];
+        if (!__any(mine)) return;
     }
+    const uint32_t first = meta.x, parts = meta.y & 0x7fffffu, c = meta.y >> 24;
+    const bool sees = !(meta.y >> 23 & 1u);
     if (parts < 2 || (uint64_t)first + parts > a.slots || c >= a.cols) return;
-    const SeqRows of = seq_rows(a, seq);
-    const bool sees = of.avail && of.first + (int64_t)(row - of.row0) > 0;
     constexpr int E = D / 64;
     typedef float vec __attribute__((ext_vector_type(E)));
     const size_t stride = (size_t)a.kv_heads * a.cols;
@@ -853,11 +838,11 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
     // KV heads change fastest, so with eight of them an XCD's L2 holds the lines of one or two
     const uint32_t share = blockIdx.x / args.kv_heads, kvh = blockIdx.x % args.kv_heads;
     Task w;
-    for (uint64_t done = 0; find_task<SPLIT>(late_args(), share, done, w);) {
+    for (uint32_t done = 0; find_task<SPLIT>(late_args(), share, done, w);) {
     const Fp4Args &a = late_args();
     const uint32_t tid = fresh_thread(), lane = tid & 63u, col = lane & 31u, h = lane >> 5;
     const uint32_t columns = w.s.n * a.G;
-    auto seen = [&](uint32_t c) { return (uint32_t)min(max(w.s.first + (int64_t)(c / a.G), (int64_t)0), (int64_t)w.s.avail); };
+    auto seen = [&](uint32_t c) { return seen_of(w.s, c / a.G); };
     const uint32_t group_hi = seen(min(w.c0 + 127u, columns - 1));   // the last column sees most
     const uint32_t p0 = __builtin_amdgcn_readfirstlane(min(w.from, group_hi)), p1 = __builtin_amdgcn_readfirstlane(min(w.to, group_hi));
     const uint32_t c0 = w.c0 + 32u * wave;
@@ -868,7 +853,7 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
     const size_t qat = (size_t)(w.s.row0 + c / a.G) * a.heads + (size_t)kvh * a.G + c % a.G;
 
     const uint32_t row = a.kv_heads * (D / 2), srow = a.kv_heads * (D / 32);
-    const size_t base = (size_t)w.s.base;
+    const size_t base = w.s.base;
     const uint8_t *kc = a.kc + base * row + kvh * (D / 2), *ks = a.ks + base * srow + kvh * (D / 32);
     const uint8_t *vc = a.vc + base * row + kvh * (D / 2), *vs = a.vs + base * srow + kvh * (D / 32);
 
@@ -1145,7 +1130,7 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
     if (SPLIT && w.slot == w.first_slot && kvh == 0 && h == 0) {
         uint32_t *to = z.meta + 2 * ((size_t)w.s.row0 * z.G + c);
         to[0] = w.first_slot;
-        to[1] = w.parts | (c - w.c0) << 24;
+        to[1] = w.parts | (vis ? 0u : 1u << 23) | (c - w.c0) << 24;
     }
     if constexpr (!SPLIT) break;
     }
@@ -1185,7 +1170,9 @@ template <typename T, int D> int launch_dim(janus_ctx *ctx, Fp4Args &a, uint32_t
     a.least = 2;
     a.target = 0;
     a.shares = (uint32_t)tiles;   // * head_groups below 2^21 + 2^22, up to 512 lanes each
-    if (max_len > 4 * a.step && (few ? busy < 4 * slots : 2 * busy <= slots)) {
+    // units of all tiles below 2^31
+    const bool counts = tiles * (std::min(a.max_seq, a.cache_rows) / a.step + 1) < (1ull << 31);
+    if (counts && max_len > 4 * a.step && (few ? busy < 4 * slots : 2 * busy <= slots)) {
         a.shares = a.target = (uint32_t)slots;
         a.slots = (uint32_t)(slots + tiles);
         const size_t cells = (size_t)a.slots * a.kv_heads * a.cols;
