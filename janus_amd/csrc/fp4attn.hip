@@ -140,6 +140,7 @@ struct Task {
     uint32_t c0;                        // first column
     uint32_t from, to;
     uint32_t slot, first_slot, parts;   // its place among the parts of these columns; 1 part: the result
+    bool more;                          // whether the share goes on behind them
 };
 
 // The work of share `share` that starts `done` units into it; false if there is none.
@@ -190,6 +191,7 @@ template <bool SPLIT> __device__ __forceinline__ bool find_task(const Fp4Args &a
                 w.from = 0;
                 w.to = w.s.avail;
                 w.parts = 1;
+                w.more = false;
                 return true;
             }
             const uint32_t n = min(quota - done, each - off);
@@ -201,6 +203,7 @@ template <bool SPLIT> __device__ __forceinline__ bool find_task(const Fp4Args &a
             w.slot = share + number;
             w.first_slot = s_first + number;
             done += n;
+            w.more = done < quota;
             return true;
         }
         start = lane_value(upto, 63);
@@ -211,12 +214,11 @@ template <bool SPLIT> __device__ __forceinline__ bool find_task(const Fp4Args &a
 }
 
 // Bytes of 32 positions of a KV head, as lane 16 g + at uses them: K of the positions at
-// and 16 + at, the lane's dims of V of the eight positions {4g .., 16 + 4g ..}; all scales
-// of a position and head in one word: K's of the two positions, V's of the (at % 8)-th
-// of the eight.
+// and 16 + at; all scales of a position and head in one word, K's of the two positions,
+// V's of the (at % 8)-th of the eight positions {4g .., 16 + 4g ..}.
 template <int D> struct Raw {
     uint32_t k[2][D / 32];
-    uint32_t v[8], ks[2], vs;
+    uint32_t ks[2], vs;
 };
 
 // 16 bytes per lane from base + off straight into LDS at lds + 16 * lane (lds is
@@ -231,15 +233,16 @@ __device__ __forceinline__ void lds_request(const uint8_t *base, uint32_t off, u
 }
 #pragma clang diagnostic pop
 
-// A tile of 32 ph positions of hw KV heads, whose rows of hw D / 2 bytes lie one behind the
-// other in LDS (16 KB of K, then of V, for 128 dims). Whole rows are requested, 1 KB an
+// A tile of 32 S ph positions of hw KV heads, whose rows of hw D / 2 bytes lie one behind the
+// other in LDS (2 S KB a wavefront of K, then of V, for 128 dims). Whole rows are requested, 1 KB an
 // instruction: 270000 positions of 8 heads come at 6.4 TB/s like this and at 4.9 where
 // every wavefront loads its own head's 64 bytes of a row. The 16-byte segments of a row
 // are permuted by the heads' number of segments (U), so that 16 positions of a head (K), or four
 // positions four apart (V), lie in different banks.
-template <int D> struct Tile {
-    static constexpr uint32_t U = D / 32, kBytes = 128u * D;       // segments of a head; bytes of K
-    static constexpr int N = kBytes / 8192;                        // requests of a wavefront for K
+template <int D, int S, int NW> struct Tile {
+    static constexpr uint32_t U = D / 32, kBytes = 16u * NW * D * S;   // segments of a head; bytes of K
+    static constexpr int N = kBytes / (1024 * NW);                     // requests of a wavefront for K
+    static constexpr uint32_t kLds = 4 * kBytes;                       // two tiles
     const uint8_t *kc, *ks, *vc, *vs;   // of the workgroup's first head at position 0
     uint32_t row, srow;                 // bytes from a position to the next
     uint32_t segs, heads, fold;         // segments of a row of the tile; hw - 1; log2 of the positions in 256 bytes
@@ -366,50 +369,63 @@ template <typename T, int D, int NT> struct Columns {
         }
     }
 
-    // 32 positions from p on. masked: some column of the wavefront does not see all of them.
-    // Returns whether a block among them is NaN; its scale counts as 1 then.
-    __device__ __forceinline__ bool step(Raw<D> &r, uint32_t lane, uint32_t p, bool masked) {
+    // 32 S positions from p on. masked: some column of the wavefront does not see all of
+    // them. v(u, j): the lane's bytes of V at position j of 32 u. Returns whether a block among
+    // them is NaN; its scale counts as 1 then.
+    template <int S, typename V> __device__ __forceinline__ bool step(Raw<D> (&r)[S], uint32_t lane, uint32_t p, bool masked, V v) {
         const uint32_t g = lane >> 4;
-        const bool odd = __any((nan_bytes(r.ks[0]) | nan_bytes(r.ks[1]) | nan_bytes(r.vs)) != 0);
+        uint32_t nans = 0;
+#pragma unroll
+        for (int u = 0; u < S; ++u) nans |= nan_bytes(r[u].ks[0]) | nan_bytes(r[u].ks[1]) | nan_bytes(r[u].vs);
+        const bool odd = __any(nans != 0);
         if (odd) {
-            r.ks[0] = without_nans(r.ks[0]);
-            r.ks[1] = without_nans(r.ks[1]);
-            r.vs = without_nans(r.vs);
+#pragma unroll
+            for (int u = 0; u < S; ++u) {
+                r[u].ks[0] = without_nans(r[u].ks[0]);
+                r[u].ks[1] = without_nans(r[u].ks[1]);
+                r[u].vs = without_nans(r[u].vs);
+            }
         }
         const uint32_t kshift = g * (D / 4) / 32 * 8;   // the lane's block of K, and of V
         const uint32_t vblock = (lane & 15u) * (D / 16) / 32, vmask = 0xffu << (8u * vblock), vturn = (8u * vblock - 23u) & 31u;
-        ff4 s[NT][2];
+        ff4 s[NT][2 * S];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const float sc = __uint_as_float((r.ks[h] >> kshift & 0xffu) << 23);
+        for (int h = 0; h < 2 * S; ++h) {
+            const float sc = __uint_as_float((r[h >> 1].ks[h & 1] >> kshift & 0xffu) << 23);
+            ff4 small[P == 2 ? NT : 1];
 #pragma unroll
-            for (int t = 0; t < NT; ++t) s[t][h] = ff4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int t = 0; t < NT; ++t) {
+                s[t][h] = ff4{0.0f, 0.0f, 0.0f, 0.0f};
+                if constexpr (P == 2) small[t] = s[t][h];
+            }
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) {
-                const uint32_t w = r.k[h][i];
+                const uint32_t w = r[h >> 1].k[h & 1][i];
                 const fh8 k = h8(fp4_pair<0>(w, sc), fp4_pair<1>(w, sc), fp4_pair<2>(w, sc), fp4_pair<3>(w, sc));
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    if constexpr (P == 2) s[t][h] = mfma(k, q[t][1][i], s[t][h]);
+                    if constexpr (P == 2) small[t] = mfma(k, q[t][1][i], small[t]);
                     s[t][h] = mfma(k, q[t][0][i], s[t][h]);
                 }
             }
+            if constexpr (P == 2)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) s[t][h] += small[t];
         }
         if (masked) {
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                for (int h = 0; h < 2 * S; ++h)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (p + 16u * h + 4u * g + j >= vis[t]) s[t][h][j] = -INFINITY;
+                    for (int j = 0; j < 4; ++j) s[t][h][j] = p + 16u * h + 4u * g + j < vis[t] ? s[t][h][j] : -INFINITY;
         }
-        uint32_t pp[NT][P][4];
+        float m0[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             float mx = s[t][0][0];
 #pragma unroll
-            for (int j = 1; j < 8; ++j) mx = fmaxf(mx, s[t][j >> 2][j & 3]);
+            for (int j = 1; j < 8 * S; ++j) mx = fmaxf(mx, s[t][j >> 2][j & 3]);
             mx = groups_max(mx);
             if (__any((mx - m[t]) * cs[t] > kSlack)) {
                 const float now = fmaxf(m[t], mx);
@@ -419,96 +435,99 @@ template <typename T, int D, int NT> struct Columns {
                 for (int i = 0; i < D / 16; ++i) o[t][i] *= f;
                 m[t] = now;
             }
-            const float m0 = m[t] == -INFINITY ? 0.0f : m[t];
-            float x[8], sum = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                x[j] = __builtin_amdgcn_exp2f(fmaf(s[t][j >> 2][j & 3] - m0, cs[t], kBias));   // large scores keep their last bits
-                sum += x[j];
-            }
-            l[t] += sum;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const _Float16 h0 = (_Float16)x[2 * j], h1 = (_Float16)x[2 * j + 1];
-                pp[t][0][j] = __builtin_bit_cast(uint32_t, jh2{h0, h1});
-                if constexpr (P == 2) pp[t][1][j] = half_pair(x[2 * j] - (float)h0, x[2 * j + 1] - (float)h1);
-            }
+            m0[t] = m[t] == -INFINITY ? 0.0f : m[t];
         }
-        // the byte of position j, which lane j of the 16 holds, at the exponent's place
-        float sc[8];
-        auto spread = [&](auto j) {
-            const uint32_t w = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)r.vs, 0x150 + decltype(j)::value, 0xf, 0xf, false) & vmask;   // row_newbcast
-            sc[decltype(j)::value] = __uint_as_float(__builtin_amdgcn_alignbit(w, w, vturn));
-        };
-        spread(std::integral_constant<int, 0>{});
-        spread(std::integral_constant<int, 1>{});
-        spread(std::integral_constant<int, 2>{});
-        spread(std::integral_constant<int, 3>{});
-        spread(std::integral_constant<int, 4>{});
-        spread(std::integral_constant<int, 5>{});
-        spread(std::integral_constant<int, 6>{});
-        spread(std::integral_constant<int, 7>{});
-        auto two = [&](auto byte) {
-            constexpr int B = decltype(byte)::value;
-            uint32_t h[8], lo[4], hi[4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) h[j] = fp4_pair<B>(r.v[j], sc[j]);
+        for (int u = 0; u < S; ++u) {
+            fh8 pp[NT][P];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                lo[j] = __builtin_amdgcn_perm(h[2 * j + 1], h[2 * j], 0x05040100u);
-                hi[j] = __builtin_amdgcn_perm(h[2 * j + 1], h[2 * j], 0x07060302u);
-            }
-            const fh8 v0 = h8(lo[0], lo[1], lo[2], lo[3]), v1 = h8(hi[0], hi[1], hi[2], hi[3]);
+            for (int t = 0; t < NT; ++t) {
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int u = 0; u < P; ++u) {
-                    const fh8 x = h8(pp[t][u][0], pp[t][u][1], pp[t][u][2], pp[t][u][3]);
-                    o[t][2 * B] = mfma(v0, x, o[t][2 * B]);
-                    o[t][2 * B + 1] = mfma(v1, x, o[t][2 * B + 1]);
+                for (int j = 0; j < 8; ++j) {
+                    const float x = __builtin_amdgcn_exp2f(fmaf(s[t][2 * u + (j >> 2)][j & 3] - m0[t], cs[t], kBias));   // large scores keep their last bits
+                    l[t] += x;
+                    pp[t][0][j] = (_Float16)x;
+                    if constexpr (P == 2) pp[t][1][j] = (_Float16)(x - (float)pp[t][0][j]);
                 }
-        };
-        two(std::integral_constant<int, 0>{});
-        two(std::integral_constant<int, 1>{});
-        if constexpr (D == 128) {
-            two(std::integral_constant<int, 2>{});
-            two(std::integral_constant<int, 3>{});
+            }
+            // the byte of position j, which lane j of the 16 holds, at the exponent's place
+            float sc[8];
+            auto spread = [&](auto j) {
+                const uint32_t w = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)r[u].vs, 0x150 + decltype(j)::value, 0xf, 0xf, false) & vmask;   // row_newbcast
+                sc[decltype(j)::value] = __uint_as_float(__builtin_amdgcn_alignbit(w, w, vturn));
+            };
+            spread(std::integral_constant<int, 0>{});
+            spread(std::integral_constant<int, 1>{});
+            spread(std::integral_constant<int, 2>{});
+            spread(std::integral_constant<int, 3>{});
+            spread(std::integral_constant<int, 4>{});
+            spread(std::integral_constant<int, 5>{});
+            spread(std::integral_constant<int, 6>{});
+            spread(std::integral_constant<int, 7>{});
+            uint32_t raw[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) raw[j] = v(u, j);
+            auto two = [&](auto byte) {
+                constexpr int B = decltype(byte)::value;
+                uint32_t h[8], lo[4], hi[4];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) h[j] = fp4_pair<B>(raw[j], sc[j]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    lo[j] = __builtin_amdgcn_perm(h[2 * j + 1], h[2 * j], 0x05040100u);
+                    hi[j] = __builtin_amdgcn_perm(h[2 * j + 1], h[2 * j], 0x07060302u);
+                }
+                const fh8 v0 = h8(lo[0], lo[1], lo[2], lo[3]), v1 = h8(hi[0], hi[1], hi[2], hi[3]);
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int w = 0; w < P; ++w) {
+                        o[t][2 * B] = mfma(v0, pp[t][w], o[t][2 * B]);
+                        o[t][2 * B + 1] = mfma(v1, pp[t][w], o[t][2 * B + 1]);
+                    }
+            };
+            two(std::integral_constant<int, 0>{});
+            two(std::integral_constant<int, 1>{});
+            if constexpr (D == 128) {
+                two(std::integral_constant<int, 2>{});
+                two(std::integral_constant<int, 3>{});
+            }
         }
         return odd;
     }
 };
 
 // First positions with a NaN block of K (x), and of V in the lane's output dims (y),
-// among 32 positions from each of p, p + step, ... below end.
+// among `span` (32 or 64) positions from each of p, p + step, ... below end.
 template <int D>
 __device__ __forceinline__ uint2 first_nans(const uint8_t *ks, const uint8_t *vs, uint32_t srow, uint32_t p, uint32_t end,
-                                            uint32_t step) {
+                                            uint32_t step, uint32_t span) {
     const uint32_t lane = threadIdx.x & 63u, mine = (lane >> 4) * (D / 4) / 32;
     uint2 at = make_uint2(0xffffffffu, 0xffffffffu);
     for (; p < end; p += step) {
-        const uint32_t i = p + (lane & 31u);
+        const uint32_t i = p + lane;
         bool kn = false;
         for (uint32_t b = 0; b < D / 32; ++b) {
             bool vn = false;
-            if (i < end) {
+            if (lane < span && i < end) {
                 kn |= ks[(size_t)i * srow + b] > 140;
                 vn = vs[(size_t)i * srow + b] > 140;
             }
-            const uint32_t some = (uint32_t)__ballot(vn);
-            if (some && b == mine) at.y = min(at.y, p + (uint32_t)__builtin_ctz(some));
+            const uint64_t some = __ballot(vn);
+            if (some && b == mine) at.y = min(at.y, p + (uint32_t)__builtin_ctzll(some));
         }
-        const uint32_t some = (uint32_t)__ballot(kn);
-        if (some) at.x = min(at.x, p + (uint32_t)__builtin_ctz(some));
+        const uint64_t some = __ballot(kn);
+        if (some) at.x = min(at.x, p + (uint32_t)__builtin_ctzll(some));
     }
     return at;
 }
 
-// Up to 16 NT columns of a sequence and positions [from, to): the eight wavefronts of a
-// workgroup take hw KV heads and ph phases of 32 positions each.
-template <typename T, int D, int NT, bool SPLIT>
-__global__ __launch_bounds__(512, sizeof(T) == 4 && D == 128 ? 2 : 4) void fp4_attn_kernel(Fp4Args args) {
+// Up to 16 NT columns of a sequence and positions [from, to): the NW wavefronts of a
+// workgroup take hw KV heads and ph phases of 32 S positions each; PER of them share a SIMD.
+template <typename T, int D, int NT, int S, int NW, int PER, bool SPLIT>
+__global__ __launch_bounds__(NW * 64, PER) void fp4_attn_kernel(Fp4Args args) {
     constexpr uint32_t DL = D / 4;   // output dims of a lane
-    extern __shared__ uint8_t smem[];   // two tiles, then the phases' results
+    extern __shared__ __align__(16) uint8_t smem[];   // two tiles, then the phases' results
     float *const lds = (float *)smem;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)smem;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -517,7 +536,8 @@ __global__ __launch_bounds__(512, sizeof(T) == 4 && D == 128 ? 2 : 4) void fp4_a
     const uint32_t share = j / args.head_groups * 8u + (blockIdx.x & 7u);
     if (share >= args.shares) return;
     Task w;
-    for (uint32_t done = 0; find_task<SPLIT>(late_args(), share, done, w);) {
+    w.more = true;
+    for (uint32_t done = 0; w.more && find_task<SPLIT>(late_args(), share, done, w);) {
     const Fp4Args &a = late_args();
     const uint32_t lane = fresh_thread() & 63u, g = lane >> 4, at = lane & 15u;
     const uint32_t hwave = wave & (a.hw - 1), phase = wave / a.hw, head0 = (blockIdx.x >> 3) % a.head_groups * a.hw, kvh = head0 + hwave;
@@ -525,81 +545,90 @@ __global__ __launch_bounds__(512, sizeof(T) == 4 && D == 128 ? 2 : 4) void fp4_a
 
     // positions that columns of the tile see: the last ones the most
     const uint32_t most = seen_of(w.s, (min(c0 + 16u * NT, columns) - 1) / a.G), fewest = seen_of(w.s, c0 / a.G);
-    const uint32_t end = __builtin_amdgcn_readfirstlane(min(most, w.to)), from = __builtin_amdgcn_readfirstlane(w.from), step = 32u * a.ph;
+    const uint32_t end = __builtin_amdgcn_readfirstlane(min(most, w.to)), from = __builtin_amdgcn_readfirstlane(w.from), step = 32u * S * a.ph;
     const size_t base = w.s.base;
     const uint32_t rows = a.cache_rows - w.s.base;   // of the cache from position 0 on
-    Tile<D> tile;
+    Tile<D, S, NW> tile;
     tile.row = a.kv_heads * (D / 2);
     tile.srow = a.kv_heads * (D / 32);
     tile.kc = a.kc + base * tile.row + head0 * (D / 2);
     tile.vc = a.vc + base * tile.row + head0 * (D / 2);
     tile.ks = a.ks + base * tile.srow + kvh * (D / 32);   // the wavefront's own
     tile.vs = a.vs + base * tile.srow + kvh * (D / 32);
-    tile.segs = a.hw * Tile<D>::U;
+    tile.segs = a.hw * Tile<D, S, NW>::U;
     tile.heads = a.hw - 1;
     tile.fold = tile.segs >= 16u ? 0u : 4u - (31u - (uint32_t)__builtin_clz(tile.segs));
     tile.offsets(lane, wave, step - 1);
     // the scales of the wavefront's 32 positions of a tile
     typedef std::conditional_t<D == 128, uint32_t, uint16_t> word;
-    uint32_t ks0 = 0, ks1 = 0, vs0 = 0, kso = at * tile.srow, kso2 = (at + 16u) * tile.srow, vso = ((at & 4u) * 4u + 4u * g + (at & 3u)) * tile.srow;
+    uint32_t ks0[S] = {}, ks1[S] = {}, vs0[S] = {};
+    const uint32_t kpos = at, vpos = (at & 4u) * 4u + 4u * g + (at & 3u);
+    const uint32_t kso = kpos * tile.srow, vso = vpos * tile.srow;
     auto fetch = [&](uint32_t p, uint32_t b) {
-        uint32_t q = p + 32u * phase;
+        const uint32_t q = p + 32u * S * phase;
         if (p + step > rows) {   // the cache ends inside the tile: its last row again
             tile.offsets(lane, wave, rows - 1 - p);
-            q = min(q, rows - 1);
-            kso = min(at, rows - 1 - q) * tile.srow;
-            kso2 = min(at + 16u, rows - 1 - q) * tile.srow;
-            vso = min((at & 4u) * 4u + 4u * g + (at & 3u), rows - 1 - q) * tile.srow;
+            tile.request(p, wave, lds0 + b * (2 * Tile<D, S, NW>::kBytes));
+#pragma unroll
+            for (int u = 0; u < S; ++u) {
+                ks0[u] = *(const word *)(tile.ks + (size_t)min(q + 32u * u + kpos, rows - 1) * tile.srow);
+                ks1[u] = *(const word *)(tile.ks + (size_t)min(q + 32u * u + kpos + 16u, rows - 1) * tile.srow);
+                vs0[u] = *(const word *)(tile.vs + (size_t)min(q + 32u * u + vpos, rows - 1) * tile.srow);
+            }
+            return;
         }
         // rows behind the sequence's end are other sequences' or none's, and no column sees them
-        tile.request(p, wave, lds0 + b * (2 * Tile<D>::kBytes));
-        const uint8_t *ks = tile.ks + (size_t)q * tile.srow, *vs = tile.vs + (size_t)q * tile.srow;
-        ks0 = *(const word *)(ks + kso);
-        ks1 = *(const word *)(ks + kso2);
-        vs0 = *(const word *)(vs + vso);
+        tile.request(p, wave, lds0 + b * (2 * Tile<D, S, NW>::kBytes));
+#pragma unroll
+        for (int u = 0; u < S; ++u) {
+            ks0[u] = *(const word *)(tile.ks + (size_t)(q + 32u * u) * tile.srow + kso);
+            ks1[u] = *(const word *)(tile.ks + (size_t)(q + 32u * u + 16u) * tile.srow + kso);
+            vs0[u] = *(const word *)(tile.vs + (size_t)(q + 32u * u) * tile.srow + vso);
+        }
     };
     if (from < end) fetch(from, 0);
     Columns<T, D, NT> col;
     col.load(a, w, lane, c0, kvh);
     if (from < end) {
         bool odd = false;
-        // offsets of the lane's operands in a tile
-        const uint32_t pos0 = 32u * phase, seg0 = hwave * Tile<D>::U;
-        const uint32_t kat = (pos0 + at) * tile.segs * 16u + ((seg0 + g * (D / 8) / 16) ^ tile.k_turn(pos0 + at)) * 16u + (D == 64 ? (g & 1u) * 8u : 0u);
-        const uint32_t kat2 = (pos0 + 16u + at) * tile.segs * 16u + ((seg0 + g * (D / 8) / 16) ^ tile.k_turn(pos0 + 16u + at)) * 16u + (D == 64 ? (g & 1u) * 8u : 0u);
-        // positions 4 g + r lie r rows behind 4 g, under the same turn
-        const uint32_t vat = (pos0 + 4u * g) * tile.segs * 16u + ((seg0 + at * (D / 32) / 16) ^ tile.v_turn(pos0 + 4u * g)) * 16u + at * (D / 32) % 16u;
-        const uint32_t vat2 = (pos0 + 16u + 4u * g) * tile.segs * 16u + ((seg0 + at * (D / 32) / 16) ^ tile.v_turn(pos0 + 16u + 4u * g)) * 16u + at * (D / 32) % 16u;
+        // offsets of the lane's operands in a tile: K of position at of 16, V of 4 g of 16 (r rows on under the same turn)
+        const uint32_t pos0 = 32u * S * phase, seg0 = hwave * Tile<D, S, NW>::U, line = tile.segs * 16u;
+        uint32_t kat[2 * S], vat[2 * S];
+#pragma unroll
+        for (int h = 0; h < 2 * S; ++h) {
+            const uint32_t kn = pos0 + 16u * h + at, vn = pos0 + 16u * h + 4u * g;
+            kat[h] = kn * line + ((seg0 + g * (D / 8) / 16) ^ tile.k_turn(kn)) * 16u + (D == 64 ? (g & 1u) * 8u : 0u);
+            vat[h] = vn * line + ((seg0 + at * (D / 32) / 16) ^ tile.v_turn(vn)) * 16u + at * (D / 32) % 16u;
+        }
         uint32_t b = 0;
         for (uint32_t p = from; p < end; p += step, b ^= 1u) {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();   // this tile is there, the other one has been read
-            Raw<D> r;
-            r.ks[0] = ks0;
-            r.ks[1] = ks1;
-            r.vs = vs0;
-            // in registers before the next ones are asked for: a wait for them later would be one for the next tile too
-            asm volatile("" : "+v"(r.ks[0]), "+v"(r.ks[1]), "+v"(r.vs));
+            Raw<D> r[S];
+            // the scales are in registers before the next ones are asked for: a wait for them later would be one for the next tile too
+#pragma unroll
+            for (int u = 0; u < S; ++u) {
+                r[u].ks[0] = ks0[u];
+                r[u].ks[1] = ks1[u];
+                r[u].vs = vs0[u];
+                asm volatile("" : "+v"(r[u].ks[0]), "+v"(r[u].ks[1]), "+v"(r[u].vs));
+            }
             if (p + step < end) fetch(p + step, b ^ 1u);
-            const uint32_t mine = p + 32u * phase;
+            const uint32_t mine = p + 32u * S * phase;
             if (mine >= end) continue;
-            const uint8_t *kt = smem + b * (2 * Tile<D>::kBytes), *vt = kt + Tile<D>::kBytes;
-            typedef uint32_t vec __attribute__((ext_vector_type(D / 32)));
-            const vec k0 = *(const vec *)(kt + kat), k1 = *(const vec *)(kt + kat2);
+            const uint8_t *kt = smem + b * (2 * Tile<D, S, NW>::kBytes), *vt = kt + Tile<D, S, NW>::kBytes;
 #pragma unroll
-            for (int i = 0; i < D / 32; ++i) {
-                r.k[0][i] = k0[i];
-                r.k[1][i] = k1[i];
-            }
+            for (int h = 0; h < 2 * S; ++h) {
+                typedef uint32_t vec __attribute__((ext_vector_type(D / 32)));
+                const vec k = *(const vec *)(kt + kat[h]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                r.v[i] = *(const word *)(vt + vat + i * tile.segs * 16u);
-                r.v[4 + i] = *(const word *)(vt + vat2 + i * tile.segs * 16u);
+                for (int i = 0; i < D / 32; ++i) r[h >> 1].k[h & 1][i] = k[i];
             }
-            odd |= col.step(r, lane, mine, mine + 32u > fewest || mine + 32u > end);
+            odd |= col.step(r, lane, mine, mine + 32u * S > fewest || mine + 32u * S > end,
+                            [&](int u, int j) -> uint32_t { return *(const word *)(vt + vat[2 * u + (j >> 2)] + (j & 3) * line); });
         }
         if (odd) {
-            const uint2 at = first_nans<D>(tile.ks, tile.vs, tile.srow, from + 32u * phase, end, step);
+            const uint2 at = first_nans<D>(tile.ks, tile.vs, tile.srow, from + 32u * S * phase, end, step, 32u * S);
             const float nan = __uint_as_float(0x7fc00000u);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
@@ -699,7 +728,6 @@ __global__ __launch_bounds__(512, sizeof(T) == 4 && D == 128 ? 2 : 4) void fp4_a
             to[1] = w.parts | (col.vis[t] ? 0u : 1u << 23) | (c - w.c0) << 24;
         }
     }
-    if constexpr (!SPLIT) break;
     }
 }
 
@@ -833,12 +861,13 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
     constexpr uint32_t kTile = TP * D * 2u;   // bytes of a tile of K, and of V
     constexpr uint32_t kUnits = TP * D / 32;  // 16-byte pieces of K, and quads of positions x 8 dims of V
     static_assert(kUnits == 256 || kUnits == 128, "a lane has one unit of each, or of one of them");
-    extern __shared__ uint8_t smem[];         // K, V, K, V
+    extern __shared__ __align__(16) uint8_t smem[];         // K, V, K, V
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // KV heads change fastest, so with eight of them an XCD's L2 holds the lines of one or two
     const uint32_t share = blockIdx.x / args.kv_heads, kvh = blockIdx.x % args.kv_heads;
     Task w;
-    for (uint32_t done = 0; find_task<SPLIT>(late_args(), share, done, w);) {
+    w.more = true;
+    for (uint32_t done = 0; w.more && find_task<SPLIT>(late_args(), share, done, w);) {
     const Fp4Args &a = late_args();
     const uint32_t tid = fresh_thread(), lane = tid & 63u, col = lane & 31u, h = lane >> 5;
     const uint32_t columns = w.s.n * a.G;
@@ -1132,8 +1161,16 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
         to[0] = w.first_slot;
         to[1] = w.parts | (vis ? 0u : 1u << 23) | (c - w.c0) << 24;
     }
-    if constexpr (!SPLIT) break;
     }
+}
+
+// A launch with more LDS than a kernel has without asking.
+template <typename K> int launch_lds(janus_ctx *ctx, K kernel, dim3 grid, dim3 block, uint32_t lds, const Fp4Args &a) {
+    if (lds > 64 * 1024)
+        JANUS_HIP_CHECK(ctx, hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    hipLaunchKernelGGL(kernel, grid, block, lds, ctx->stream, a);
+    JANUS_LAUNCH_CHECK(ctx);
+    return JANUS_OK;
 }
 
 template <typename T, int D> int launch_join(janus_ctx *ctx, const Fp4Args &a, uint64_t tiles) {
@@ -1150,12 +1187,18 @@ template <typename T, int D> int launch_join(janus_ctx *ctx, const Fp4Args &a, u
 template <typename T, int D> int launch_dim(janus_ctx *ctx, Fp4Args &a, uint32_t max_len) {
     const uint32_t mean = (a.rows + a.nseq - 1) / a.nseq;   // rows of a sequence
     const bool few = (uint64_t)mean * a.G <= 16;
-    constexpr int kFewCu = sizeof(T) == 4 && D == 128 ? 1 : 2;   // workgroups that a CU holds
+    // Two-part q and P of 128 dims take 163 registers: three workgroups of four wavefronts
+    // share a CU; the others fit 128, two of eight.
+    constexpr int S = 1, NW = D == 128 && sizeof(T) == 4 ? 4 : 8, PER = D == 128 && sizeof(T) == 4 ? 3 : 4;
+    constexpr int kFewCu = PER * 4 / NW;   // workgroups that a CU holds
+    typedef Tile<D, S, NW> Few;
+    static_assert(kFewCu * Few::kLds <= 160 * 1024 && Few::kLds >= (NW - 1) * (D / 4 + 2) * 256, "tiles, or the phases' results");
     if (few) {
         a.cols = 16;
-        a.hw = a.kv_heads % 8 == 0 ? 8 : a.kv_heads % 4 == 0 ? 4 : a.kv_heads % 2 == 0 ? 2 : 1;
-        a.ph = 8 / a.hw;
-        a.step = 32 * a.ph;
+        a.hw = NW;
+        while (a.kv_heads % a.hw) a.hw /= 2;
+        a.ph = NW / a.hw;
+        a.step = 32 * S * a.ph;
     } else {
         a.cols = 128;
         a.hw = a.ph = 1;
@@ -1183,17 +1226,17 @@ template <typename T, int D> int launch_dim(janus_ctx *ctx, Fp4Args &a, uint32_t
         a.part_ml = a.part + cells * D;
     }
     if (few) {
-        const uint32_t lds = 4 * Tile<D>::kBytes;   // at least 7 (D / 4 + 2) 256 for the phases
-        const dim3 grid((a.shares + 7) / 8 * 8 * a.head_groups), block(512);
-        if (a.target) hipLaunchKernelGGL((fp4_attn_kernel<T, D, 1, true>), grid, block, lds, ctx->stream, a);
-        else hipLaunchKernelGGL((fp4_attn_kernel<T, D, 1, false>), grid, block, lds, ctx->stream, a);
+        const dim3 grid((a.shares + 7) / 8 * 8 * a.head_groups), block(NW * 64);
+        int e = a.target ? launch_lds(ctx, fp4_attn_kernel<T, D, 1, S, NW, PER, true>, grid, block, Few::kLds, a)
+                         : launch_lds(ctx, fp4_attn_kernel<T, D, 1, S, NW, PER, false>, grid, block, Few::kLds, a);
+        if (e) return e;
     } else {
         constexpr int TP = D == 128 && sizeof(T) == 4 ? 32 : 64;
         const dim3 grid(a.shares * a.kv_heads), block(256);
-        if (a.target) hipLaunchKernelGGL((fp4_wide_kernel<T, D, TP, true>), grid, block, 4 * TP * D * 2, ctx->stream, a);
-        else hipLaunchKernelGGL((fp4_wide_kernel<T, D, TP, false>), grid, block, 4 * TP * D * 2, ctx->stream, a);
+        int e = a.target ? launch_lds(ctx, fp4_wide_kernel<T, D, TP, true>, grid, block, 4 * TP * D * 2, a)
+                         : launch_lds(ctx, fp4_wide_kernel<T, D, TP, false>, grid, block, 4 * TP * D * 2, a);
+        if (e) return e;
     }
-    JANUS_LAUNCH_CHECK(ctx);
     return launch_join<T, D>(ctx, a, busy);
 }
 
