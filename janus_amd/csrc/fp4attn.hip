@@ -53,6 +53,7 @@ struct Fp4Args {
     uint32_t head_groups, shares;         // workgroups of a share of the work; shares
     uint32_t target, least, step;         // split: shares to aim at (0: a tile each), their fewest units of `step` positions
     uint32_t slots;                       // split: places for partial results
+    uint32_t mean_parts;                  // host: parts of a tile, in the mean
     float scale2;                         // scale * log2(e)
 };
 
@@ -1173,71 +1174,81 @@ template <typename K> int launch_lds(janus_ctx *ctx, K kernel, dim3 grid, dim3 b
     return JANUS_OK;
 }
 
-template <typename T, int D> int launch_join(janus_ctx *ctx, const Fp4Args &a, uint64_t tiles) {
+// How a launch is cut up. cols columns a workgroup, of per_cu on a CU.
+void plan(janus_ctx *ctx, Fp4Args &a, uint32_t cols, uint32_t hw, uint32_t ph, uint32_t step, uint32_t per_cu, uint32_t max_len) {
+    a.cols = cols;
+    a.hw = hw;
+    a.ph = ph;
+    a.step = step;
+    a.head_groups = a.kv_heads / hw;
+    a.least = 2;
+    a.target = 0;
+    // every tile of every sequence, one more where rows do not fill the last
+    const uint64_t tiles = (uint64_t)a.rows * a.G / cols + a.nseq, mean = (a.rows + a.nseq - 1) / a.nseq;
+    a.shares = (uint32_t)tiles;   // * head_groups below 2^21 + 2^22, up to 512 lanes each
+    a.slots = 0;
+    const uint64_t busy = std::max<uint64_t>(1, std::min<uint64_t>(tiles, ((uint64_t)a.rows * a.G + cols - 1) / cols + a.nseq - 1));
+    const uint64_t at_once = std::max<uint64_t>(1, (uint64_t)ctx->num_cus * per_cu / a.head_groups);
+    const bool counts = tiles * (std::min(a.max_seq, a.cache_rows) / step + 1) < (1ull << 31);   // units of all tiles
+    const bool split = cols <= 32 ? max_len > 12 * step && busy < 4 * at_once
+                                  : max_len > 16 * step && 2 * busy <= at_once && 4 * mean <= max_len;
+    if (counts && split) {
+        a.shares = a.target = (uint32_t)at_once;
+        a.slots = (uint32_t)(at_once + tiles);
+        a.mean_parts = (uint32_t)(at_once / busy) + 1;
+    }
+}
+
+int reserve(janus_ctx *ctx, Fp4Args &a, uint32_t D) {
     if (!a.target) return JANUS_OK;
-    const uint32_t units = a.rows * a.heads;
-    const uint64_t parts = a.shares / tiles + 1;   // of a tile, in the mean
-    if (parts <= 8) hipLaunchKernelGGL((fp4_join_kernel<T, D, 1>), dim3((units + 3) / 4), dim3(256), 0, ctx->stream, a);
-    else if (parts <= 32) hipLaunchKernelGGL((fp4_join_kernel<T, D, 4>), dim3(units), dim3(256), 0, ctx->stream, a);
-    else hipLaunchKernelGGL((fp4_join_kernel<T, D, 16>), dim3(units), dim3(1024), 0, ctx->stream, a);
-    JANUS_LAUNCH_CHECK(ctx);
+    const size_t cells = (size_t)a.slots * a.kv_heads * a.cols;
+    const size_t meta = ((size_t)a.rows * a.G * 8 + 255) / 256 * 256;
+    if (int e = ensure_attn_ws(ctx, meta + cells * (D + 2) * 4)) return e;
+    a.meta = (uint32_t *)ctx->attn_ws;
+    a.part = (float *)((char *)ctx->attn_ws + meta);
+    a.part_ml = a.part + cells * D;
     return JANUS_OK;
 }
 
+template <typename T, int D, int NT, int NW, int PER> int launch_few(janus_ctx *ctx, Fp4Args &a, uint32_t max_len) {
+    constexpr int S = 1;
+    uint32_t hw = NW;
+    while (a.kv_heads % hw) hw /= 2;
+    const uint32_t ph = NW / hw;
+    // two tiles, or the phases' results
+    const uint32_t lds = std::max<uint32_t>(Tile<D, S, NW>::kLds, (ph - 1) * hw * NT * (D / 4 + 2) * 256u);
+    plan(ctx, a, 16 * NT, hw, ph, 32 * S * ph, std::min<uint32_t>(PER * 4 / NW, 160 * 1024 / lds), max_len);
+    if (int e = reserve(ctx, a, D)) return e;
+    const dim3 grid((a.shares + 7) / 8 * 8 * a.head_groups), block(NW * 64);
+    if (a.target) return launch_lds(ctx, fp4_attn_kernel<T, D, NT, S, NW, PER, true>, grid, block, lds, a);
+    return launch_lds(ctx, fp4_attn_kernel<T, D, NT, S, NW, PER, false>, grid, block, lds, a);
+}
+
+template <typename T, int D> int launch_wide(janus_ctx *ctx, Fp4Args &a, uint32_t max_len) {
+    constexpr int TP = D == 128 && sizeof(T) == 4 ? 32 : 64;
+    plan(ctx, a, 128, 1, 1, 64, 2, max_len);
+    if (int e = reserve(ctx, a, D)) return e;
+    const dim3 grid(a.shares * a.kv_heads), block(256);
+    if (a.target) return launch_lds(ctx, fp4_wide_kernel<T, D, TP, true>, grid, block, 4 * TP * D * 2, a);
+    return launch_lds(ctx, fp4_wide_kernel<T, D, TP, false>, grid, block, 4 * TP * D * 2, a);
+}
+
 template <typename T, int D> int launch_dim(janus_ctx *ctx, Fp4Args &a, uint32_t max_len) {
-    const uint32_t mean = (a.rows + a.nseq - 1) / a.nseq;   // rows of a sequence
-    const bool few = (uint64_t)mean * a.G <= 16;
-    // Two-part q and P of 128 dims take 163 registers: three workgroups of four wavefronts
-    // share a CU; the others fit 128, two of eight.
-    constexpr int S = 1, NW = D == 128 && sizeof(T) == 4 ? 4 : 8, PER = D == 128 && sizeof(T) == 4 ? 3 : 4;
-    constexpr int kFewCu = PER * 4 / NW;   // workgroups that a CU holds
-    typedef Tile<D, S, NW> Few;
-    static_assert(kFewCu * Few::kLds <= 160 * 1024 && Few::kLds >= (NW - 1) * (D / 4 + 2) * 256, "tiles, or the phases' results");
-    if (few) {
-        a.cols = 16;
-        a.hw = NW;
-        while (a.kv_heads % a.hw) a.hw /= 2;
-        a.ph = NW / a.hw;
-        a.step = 32 * S * a.ph;
-    } else {
-        a.cols = 128;
-        a.hw = a.ph = 1;
-        a.step = 64;
-    }
-    a.head_groups = a.kv_heads / a.hw;
-    // every tile of every sequence, one more where rows do not fill the last
-    const uint64_t tiles = (uint64_t)a.rows * a.G / a.cols + a.nseq;
-    const uint64_t busy = std::max<uint64_t>(1, std::min<uint64_t>(tiles, ((uint64_t)a.rows * a.G + a.cols - 1) / a.cols + a.nseq - 1));
-    // shares that run at once
-    const uint64_t slots = std::max<uint64_t>(1, (uint64_t)ctx->num_cus * (few ? kFewCu : 2) / a.head_groups);
-    a.least = 2;
-    a.target = 0;
-    a.shares = (uint32_t)tiles;   // * head_groups below 2^21 + 2^22, up to 512 lanes each
-    // units of all tiles below 2^31
-    const bool counts = tiles * (std::min(a.max_seq, a.cache_rows) / a.step + 1) < (1ull << 31);
-    if (counts && max_len > 4 * a.step && (few ? busy < 4 * slots : 2 * busy <= slots)) {
-        a.shares = a.target = (uint32_t)slots;
-        a.slots = (uint32_t)(slots + tiles);
-        const size_t cells = (size_t)a.slots * a.kv_heads * a.cols;
-        const size_t meta = ((size_t)a.rows * a.G * 8 + 255) / 256 * 256;
-        if (int e = ensure_attn_ws(ctx, meta + cells * (D + 2) * 4)) return e;
-        a.meta = (uint32_t *)ctx->attn_ws;
-        a.part = (float *)((char *)ctx->attn_ws + meta);
-        a.part_ml = a.part + cells * D;
-    }
-    if (few) {
-        const dim3 grid((a.shares + 7) / 8 * 8 * a.head_groups), block(NW * 64);
-        int e = a.target ? launch_lds(ctx, fp4_attn_kernel<T, D, 1, S, NW, PER, true>, grid, block, Few::kLds, a)
-                         : launch_lds(ctx, fp4_attn_kernel<T, D, 1, S, NW, PER, false>, grid, block, Few::kLds, a);
-        if (e) return e;
-    } else {
-        constexpr int TP = D == 128 && sizeof(T) == 4 ? 32 : 64;
-        const dim3 grid(a.shares * a.kv_heads), block(256);
-        int e = a.target ? launch_lds(ctx, fp4_wide_kernel<T, D, TP, true>, grid, block, 4 * TP * D * 2, a)
-                         : launch_lds(ctx, fp4_wide_kernel<T, D, TP, false>, grid, block, 4 * TP * D * 2, a);
-        if (e) return e;
-    }
-    return launch_join<T, D>(ctx, a, busy);
+    const uint64_t columns = (uint64_t)((a.rows + a.nseq - 1) / a.nseq) * a.G;   // of a sequence and KV head, in the mean
+    // what fits the registers: q and O of 16 columns in 128 of them (two workgroups of eight wavefronts on a CU),
+    // with two-part q of 128 dims in 160 (three of four wavefronts)
+    constexpr bool kTwo = sizeof(T) == 4 && D == 128;
+    int e;
+    if (columns <= 16) e = launch_few<T, D, 1, kTwo ? 4 : 8, kTwo ? 3 : 4>(ctx, a, max_len);
+    else if (columns <= 32) e = launch_few<T, D, 2, 4, D == 128 ? 2 : 3>(ctx, a, max_len);
+    else e = launch_wide<T, D>(ctx, a, max_len);
+    if (e || !a.target) return e;
+    const uint32_t units = a.rows * a.heads;
+    if (a.mean_parts <= 8) hipLaunchKernelGGL((fp4_join_kernel<T, D, 1>), dim3((units + 3) / 4), dim3(256), 0, ctx->stream, a);
+    else if (a.mean_parts <= 32) hipLaunchKernelGGL((fp4_join_kernel<T, D, 4>), dim3(units), dim3(256), 0, ctx->stream, a);
+    else hipLaunchKernelGGL((fp4_join_kernel<T, D, 16>), dim3(units), dim3(1024), 0, ctx->stream, a);
+    JANUS_LAUNCH_CHECK(ctx);
+    return JANUS_OK;
 }
 
 }  // namespace
