@@ -8,12 +8,10 @@
 //     registers), and keeps its maximum, its sum of exponentials and its n best logits.
 //   select_join_kernel: a workgroup per request sums the parts to L_b and takes the n
 //     best of all parts by v in binary64.
-// The n best: the best of every 8 logits gives a lower bound (its n-th value, found bit
-// by bit with ballots); what is not below it, n values and a few more, is ranked by
-// counting.
-// Bound by the read of the logits. L_b is kept to about 1e-8 (exponents in two parts,
-// sums of many terms in binary64), so that beams are compared by more than the last
-// bits of binary32.
+// The n best: the lanes' best values give a lower bound, found bit by bit with ballots;
+// what is not below it, n values and a few more, is ranked by counting.
+// Bound by the read of the logits. L_b is kept to some 1e-8 (the sums of many terms in
+// binary64), so that beams are compared by more than the last bits of binary32.
 //
 // Reordering. Position by position the slots of a request's beams are permuted: a lane
 // reads its 16 bytes of every slot that is gone on from and then writes them to the
@@ -48,15 +46,13 @@ __device__ __forceinline__ double value64(uint64_t k) {
     return k == ~0ull ? __longlong_as_double(0x7ff8000000000000ll) : __longlong_as_double((long long)(k >> 63 ? k ^ 0x8000000000000000ull : ~k));
 }
 
-// The n-th largest of a wavefront's 64 G keys, bit by bit; 0 where fewer than n are not 0.
-// (Or a value below it with nothing in between: it stops where exactly n are left.)
-template <int G> __device__ __forceinline__ uint32_t nth_key(const uint32_t (&key)[G], uint32_t n) {
+// A lower bound of the n-th largest of a wavefront's 64 keys (0 where fewer than n are not
+// 0): the key bit by bit, until exactly n are left above.
+__device__ __forceinline__ uint32_t nth_key(uint32_t key, uint32_t n) {
     uint32_t t = 0;
     for (int b = 31; b >= 0; --b) {
         const uint32_t at = t | 1u << b;
-        uint32_t have = 0;
-#pragma unroll
-        for (int i = 0; i < G; ++i) have += (uint32_t)__popcll(__ballot(key[i] >= at));
+        const uint32_t have = (uint32_t)__popcll(__ballot(key >= at));
         if (have >= n) t = at;
         if (have == n) break;
     }
@@ -74,12 +70,11 @@ __device__ __forceinline__ uint64_t wave_umax(uint64_t v) {
     return v;
 }
 
-// e^t for t <= 0, off by about a step of binary32 (the product with log2 e in two parts).
+// e^t for t <= 0: log2 e in two parts, whose error would be common to all terms of a sum;
+// the rounding of the product is not.
 __device__ __forceinline__ float exp_neg(float t) {
     constexpr float kL = 1.44269502162933349609375f, kL2 = 1.92596299112661746887e-8f;   // log2 e = kL + kL2
-    const float hi = t * kL, lo = fmaf(t, kL, -hi) + t * kL2;
-    const float e = __builtin_amdgcn_exp2f(hi);
-    return t > -126.0f ? fmaf(e * 0.693147182f, lo, e) : e;   // t = -infinity has no second part
+    return __builtin_amdgcn_exp2f(fmaf(t, kL2, t * kL));
 }
 
 struct SelectArgs {
@@ -94,7 +89,7 @@ struct SelectArgs {
 
 template <bool VEC> __global__ __launch_bounds__(kPartWaves * 64) void select_part_kernel(SelectArgs a) {
     __shared__ uint64_t list[kList];
-    __shared__ uint32_t nth[kPartWaves], share[kPartWaves];
+    __shared__ uint32_t share[kPartWaves];
     __shared__ float maxes[kPartWaves];
     __shared__ double sums[kPartWaves];
     __shared__ uint32_t found;
@@ -103,8 +98,9 @@ template <bool VEC> __global__ __launch_bounds__(kPartWaves * 64) void select_pa
     if (a.scores && a.scores[row] == -INFINITY) return;   // an ended beam
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const float *x = a.logits + (size_t)row * a.vocab;
-    const uint32_t t0 = part * kPart + wave * (64u * kLaneLogits) + lane * 4u;
-    auto token = [&](uint32_t i) { return t0 + (i >> 2) * 256u + (i & 3u); };
+    // 1 KB for each wavefront in turn, so that all have their share of a short part too
+    const uint32_t t0 = part * kPart + threadIdx.x * 4u;
+    auto token = [&](uint32_t i) { return t0 + (i >> 2) * (kPartWaves * 256u) + (i & 3u); };
     if (threadIdx.x == 0) found = 0;
     float v[kLaneLogits];
 #pragma unroll
@@ -119,56 +115,56 @@ template <bool VEC> __global__ __launch_bounds__(kPartWaves * 64) void select_pa
             for (uint32_t j = 0; j < 4; ++j) v[i + j] = t + j < a.vocab ? x[t + j] : -INFINITY;
         }
     }
-    constexpr int G = kLaneLogits / 8;
-    uint32_t key[G];   // the best of each group of 8
-    float m = -INFINITY;
-    bool odd = false;
+    float m = v[0];
 #pragma unroll
-    for (int k = 0; k < G; ++k) {
-        float top = v[8 * k];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            top = fmaxf(top, v[8 * k + i]);
-            odd |= !(v[8 * k + i] < INFINITY);
-        }
-        key[k] = token(8u * k) < a.vocab ? order32(top) : 0u;
-        m = fmaxf(m, top);
-    }
+    for (uint32_t i = 1; i < kLaneLogits; ++i) m = fmaxf(m, v[i]);
+    // Each wavefront's n / 4-th best lane: the part has n values that are not below the least of the four.
+    const uint32_t key = t0 < a.vocab ? order32(m) : 0u;
+    const uint32_t ks = nth_key(key, (a.n + kPartWaves - 1) / kPartWaves);
+    if (lane == 0) share[wave] = ks;
     m = wave_max(m);
-    odd = __any(odd);
+    // a NaN makes the sum a NaN, and so does +infinity by its difference to itself
     float s = 0.0f;
-    if (m != -INFINITY)
+    if (m != -INFINITY) {
 #pragma unroll
         for (uint32_t i = 0; i < kLaneLogits; ++i) s += exp_neg(v[i] - m);
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < kLaneLogits; ++i) s += v[i] != v[i] ? v[i] : 0.0f;
+    }
     const double sum = wave_dsum((double)s);
-    // n of the part's values are at least the n-th best group of any wavefront, and at least the n / kPartWaves-th of all
-    const uint32_t kn = nth_key<G>(key, a.n), ks = nth_key<G>(key, (a.n + kPartWaves - 1) / kPartWaves);
     if (lane == 0) {
-        nth[wave] = kn;
-        share[wave] = ks;
-        maxes[wave] = odd ? __uint_as_float(0x7fc00000u) : m;
+        maxes[wave] = m;
         sums[wave] = sum;
     }
     __syncthreads();
-    uint32_t least = share[0], some = nth[0];
+    uint32_t least = share[0];
 #pragma unroll
-    for (uint32_t w = 1; w < kPartWaves; ++w) {
-        least = min(least, share[w]);
-        some = max(some, nth[w]);
-    }
-    least = max(least, some);
+    for (uint32_t w = 1; w < kPartWaves; ++w) least = min(least, share[w]);
+    auto collect = [&]() {
+        if (key && key >= least)
 #pragma unroll
-    for (int k = 0; k < G; ++k)
-        if (key[k] && key[k] >= least)
-#pragma unroll
-            for (uint32_t i = 8 * k; i < 8u * (k + 1); ++i) {
+            for (uint32_t i = 0; i < kLaneLogits; ++i) {
                 const uint32_t o = order32(v[i]);
                 if (o >= least && token(i) < a.vocab) {
                     const uint32_t to = atomicAdd(&found, 1u);
                     if (to < kList) list[to] = (uint64_t)o << 32 | (uint32_t)~token(i);
                 }
             }
-    __syncthreads();
+        __syncthreads();
+    };
+    collect();
+    if (found > kList) {
+        // a wavefront without large values has kept the bound down: that of the n-th best lane of the best one
+        __syncthreads();
+        const uint32_t kn = nth_key(key, a.n);
+        if (lane == 0) share[wave] = kn;
+        if (threadIdx.x == 0) found = 0;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t w = 0; w < kPartWaves; ++w) least = max(least, share[w]);
+        collect();
+    }
     const size_t at = (size_t)row * a.parts + part;
     uint64_t *keys = a.keys + at * a.n;
     const uint32_t have = found;
@@ -201,15 +197,13 @@ template <bool VEC> __global__ __launch_bounds__(kPartWaves * 64) void select_pa
     }
     if (threadIdx.x == 0) {
         float top = maxes[0];
-        bool nan = top != top;
-        for (uint32_t w = 1; w < kPartWaves; ++w) {
-            nan |= maxes[w] != maxes[w];
-            top = fmaxf(top, maxes[w]);
-        }
+#pragma unroll
+        for (uint32_t w = 1; w < kPartWaves; ++w) top = fmaxf(top, maxes[w]);
         double total = 0.0;
+#pragma unroll
         for (uint32_t w = 0; w < kPartWaves; ++w)
-            if (maxes[w] > -INFINITY) total += sums[w] * exp((double)maxes[w] - (double)top);
-        a.part_max[at] = nan ? __uint_as_float(0x7fc00000u) : top;
+            total += maxes[w] == -INFINITY ? sums[w] : sums[w] * (maxes[w] == top ? 1.0 : exp((double)maxes[w] - (double)top));
+        a.part_max[at] = total != total ? __uint_as_float(0x7fc00000u) : top;
         a.part_sum[at] = total;
     }
 }
@@ -223,12 +217,18 @@ struct Cand {
 
 __global__ __launch_bounds__(kJoinWaves * 64) void select_join_kernel(SelectArgs a) {
     __shared__ Cand list[kList];
-    __shared__ uint32_t nth[kJoinWaves], share[kJoinWaves];
+    __shared__ uint32_t share[kJoinWaves];
     __shared__ double lse[kMostBeams], score[kMostBeams];
     __shared__ int state[kMostBeams];
     __shared__ uint32_t found;
     __shared__ Cand best[kJoinWaves];
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row0 = blockIdx.x * a.beams;
+    const uint32_t per_beam = a.parts * a.n, total = a.beams * per_beam;
+    // the lane's first candidates are on their way while the sums are made (those of ended beams are whatever lies there)
+    constexpr uint32_t kHeld = 8, kStep = kJoinWaves * 64u;
+    uint64_t held[kHeld];
+#pragma unroll
+    for (uint32_t i = 0; i < kHeld; ++i) held[i] = threadIdx.x + i * kStep < total ? a.keys[(size_t)row0 * per_beam + threadIdx.x + i * kStep] : 0ull;
     if (threadIdx.x == 0) found = 0;
     for (uint32_t b = wave; b < a.beams; b += kJoinWaves) {
         const float sc = a.scores ? a.scores[row0 + b] : 0.0f;
@@ -262,48 +262,65 @@ __global__ __launch_bounds__(kJoinWaves * 64) void select_join_kernel(SelectArgs
         }
     }
     __syncthreads();
-    const uint32_t per_beam = a.parts * a.n, total = a.beams * per_beam;
-    auto get = [&](uint32_t c) {
-        const uint32_t b = c / per_beam, k = c % per_beam;
+    auto value_of = [&](uint32_t c, uint64_t key) {
+        const uint32_t b = c / per_beam, k = c - b * per_beam;
         if (state[b] != BEAM_FINE)   // all its tokens are alike: the first n stand for them
             return k < min(a.n, a.vocab) ? Cand{state[b] == BEAM_NAN ? ~0ull : order64(-INFINITY), b * a.vocab + k} : Cand{0, 0};
-        const uint64_t key = a.keys[(size_t)(row0 + b) * per_beam + k];
         if (!key) return Cand{0, 0};
         return Cand{order64(score[b] + ((double)value32((uint32_t)(key >> 32)) - lse[b])), b * a.vocab + (uint32_t)~key};
     };
+    auto far = [&](uint32_t c) { return value_of(c, a.keys[(size_t)row0 * per_beam + c]); };   // beyond the held ones
     auto comes_before = [](const Cand &p, const Cand &q) { return p.hi > q.hi || (p.hi == q.hi && p.idx < q.idx); };
-    uint32_t top[1] = {0};   // upper half of the lane's best
-    for (uint32_t c = threadIdx.x; c < total; c += kJoinWaves * 64u) top[0] = max(top[0], (uint32_t)(get(c).hi >> 32));
-    const uint32_t kn = nth_key<1>(top, a.n), ks = nth_key<1>(top, (a.n + kJoinWaves - 1) / kJoinWaves);
-    if (lane == 0) {
-        nth[wave] = kn;
-        share[wave] = ks;
-    }
-    __syncthreads();
-    uint32_t least = share[0], some = nth[0];
+    Cand mine[kHeld];
+    uint32_t top = 0;   // upper half of the lane's best
 #pragma unroll
-    for (uint32_t w = 1; w < kJoinWaves; ++w) {
-        least = min(least, share[w]);
-        some = max(some, nth[w]);
+    for (uint32_t i = 0; i < kHeld; ++i) {
+        mine[i] = threadIdx.x + i * kStep < total ? value_of(threadIdx.x + i * kStep, held[i]) : Cand{0, 0};
+        top = max(top, (uint32_t)(mine[i].hi >> 32));
     }
-    least = max(least, some);
-    for (uint32_t c = threadIdx.x; c < total; c += kJoinWaves * 64u) {
-        const Cand k = get(c);
-        if (k.hi && (uint32_t)(k.hi >> 32) >= least) {
-            const uint32_t to = atomicAdd(&found, 1u);
-            if (to < kList) list[to] = k;
-        }
-    }
+    for (uint32_t c = threadIdx.x + kHeld * kStep; c < total; c += kStep) top = max(top, (uint32_t)(far(c).hi >> 32));
+    // as in the parts: the least of the wavefronts' shares, or else the best wavefront's n-th
+    const uint32_t ks = nth_key(top, (a.n + kJoinWaves - 1) / kJoinWaves);
+    if (lane == 0) share[wave] = ks;
     __syncthreads();
+    uint32_t least = share[0];
+#pragma unroll
+    for (uint32_t w = 1; w < kJoinWaves; ++w) least = min(least, share[w]);
+    auto collect = [&]() {
+        auto take = [&](const Cand &k) {
+            if (k.hi && (uint32_t)(k.hi >> 32) >= least) {
+                const uint32_t to = atomicAdd(&found, 1u);
+                if (to < kList) list[to] = k;
+            }
+        };
+        if (top >= least) {
+#pragma unroll
+            for (uint32_t i = 0; i < kHeld; ++i) take(mine[i]);
+            for (uint32_t c = threadIdx.x + kHeld * kStep; c < total; c += kStep) take(far(c));
+        }
+        __syncthreads();
+    };
+    collect();
+    if (found > kList / 4) {
+        __syncthreads();
+        const uint32_t kn = nth_key(top, a.n);
+        if (lane == 0) share[wave] = kn;
+        if (threadIdx.x == 0) found = 0;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t w = 0; w < kJoinWaves; ++w) least = max(least, share[w]);
+        collect();
+    }
     const size_t at = (size_t)blockIdx.x * a.n;
     auto write = [&](uint32_t rank, const Cand &k) {
+        const uint32_t b = k.idx / a.vocab;
         a.out[at + rank] = (float)value64(k.hi);
-        a.parents[at + rank] = (int32_t)(k.idx / a.vocab);
-        a.tokens[at + rank] = (int32_t)(k.idx % a.vocab);
+        a.parents[at + rank] = (int32_t)b;
+        a.tokens[at + rank] = (int32_t)(k.idx - b * a.vocab);
     };
     const uint32_t have = found;
     if (have <= kList) {
-        for (uint32_t i = threadIdx.x; i < have; i += kJoinWaves * 64u) {
+        for (uint32_t i = threadIdx.x; i < have; i += kStep) {
             const Cand k = list[i];
             uint32_t rank = 0;
             for (uint32_t j = 0; j < have; ++j) rank += comes_before(list[j], k) ? 1u : 0u;
@@ -312,17 +329,19 @@ __global__ __launch_bounds__(kJoinWaves * 64) void select_join_kernel(SelectArgs
     } else {
         Cand last{0, 0};
         for (uint32_t r = 0; r < a.n; ++r) {
-            Cand mine{0, 0xffffffffu};
-            for (uint32_t c = threadIdx.x; c < total; c += kJoinWaves * 64u) {
-                const Cand k = get(c);
-                if (k.hi && (r == 0 || comes_before(last, k)) && comes_before(k, mine)) mine = k;
-            }
+            Cand next{0, 0xffffffffu};
+            auto look = [&](const Cand &k) {
+                if (k.hi && (r == 0 || comes_before(last, k)) && comes_before(k, next)) next = k;
+            };
+#pragma unroll
+            for (uint32_t i = 0; i < kHeld; ++i) look(mine[i]);
+            for (uint32_t c = threadIdx.x + kHeld * kStep; c < total; c += kStep) look(far(c));
 #pragma unroll
             for (int o = 32; o > 0; o >>= 1) {
-                const Cand k{(uint64_t)__shfl_xor((unsigned long long)mine.hi, o, 64), (uint32_t)__shfl_xor((int)mine.idx, o, 64)};
-                if (comes_before(k, mine)) mine = k;
+                const Cand k{(uint64_t)__shfl_xor((unsigned long long)next.hi, o, 64), (uint32_t)__shfl_xor((int)next.idx, o, 64)};
+                if (comes_before(k, next)) next = k;
             }
-            if (lane == 0) best[wave] = mine;
+            if (lane == 0) best[wave] = next;
             __syncthreads();
             last = best[0];
 #pragma unroll
@@ -346,57 +365,67 @@ struct ReorderArgs {
     uint32_t bufs, groups, beams, cache_rows, max_seq, chunks;
 };
 
+// What a beam takes: `rows` rows from one slot to another. A beam that stays has 0, and
+// the source of one that moves: its loads are made all the same (of lines that are there),
+// so that no load waits behind a branch.
 struct Move {
-    uint64_t from, to;   // rows
-    uint32_t rows;
+    uint32_t from, to, rows, rows_from;   // rows_from: rows that may be read at `from`
 };
 
-template <typename V, int B> __device__ __forceinline__ void permute(char *base, uint64_t row_bytes, const Move *moves, uint32_t chunk, uint32_t chunks,
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+
+template <typename V, int B> __device__ __forceinline__ void permute(char *base, uint64_t row, const Move *moves, uint32_t chunk, uint32_t chunks,
                                                                      uint32_t longest) {
-    V *const at = (V *)base;
-    const uint64_t row = row_bytes / sizeof(V), end = row * longest;
-    for (uint64_t e = (uint64_t)chunk * 256u + threadIdx.x; e < end; e += (uint64_t)chunks * 256u) {
+    // a workgroup's 256 vectors at a time
+    for (uint64_t off = (uint64_t)chunk * (256 * sizeof(V)); off < row * longest; off += (uint64_t)chunks * (256 * sizeof(V))) {
+        const uint64_t e = off + threadIdx.x * sizeof(V);
         V v[B];
 #pragma unroll
-        for (int i = 0; i < B; ++i)
-            if (e < moves[i].rows * row) v[i] = at[moves[i].from * row + e];
+        for (int i = 0; i < B; ++i) {
+            const uint64_t end = row * uniform(moves[i].rows_from) - sizeof(V);
+            v[i] = __builtin_nontemporal_load((const V *)(base + row * uniform(moves[i].from) + min(e, end)));
+        }
 #pragma unroll
         for (int i = 0; i < B; ++i)
-            if (e < moves[i].rows * row) at[moves[i].to * row + e] = v[i];
+            if (e < row * uniform(moves[i].rows)) __builtin_nontemporal_store(v[i], (V *)(base + row * uniform(moves[i].to) + e));
     }
 }
 
 template <int B> __global__ __launch_bounds__(256) void kv_reorder_kernel(ReorderArgs a) {
     __shared__ Move moves[B];
-    __shared__ uint32_t longest;
     const uint32_t chunk = blockIdx.x % a.chunks, unit = blockIdx.x / a.chunks;
     const uint32_t group = unit % a.groups, buf = unit / a.groups % a.bufs, layer = unit / a.groups / a.bufs;
-    if (threadIdx.x == 0) longest = 0;
-    __syncthreads();
-    if (threadIdx.x < B) {
-        Move m{0, 0, 0};
-        const uint32_t i = threadIdx.x;
-        if (i < a.beams) {
-            const size_t g0 = (size_t)group * a.beams;
-            const int32_t p = a.parents[g0 + i];
-            if (p >= 0 && (uint32_t)p < a.beams && (uint32_t)p != i) {
-                const int64_t from = a.row_base[g0 + p], to = a.row_base[g0 + i];
-                int64_t n = a.seq_lens ? (int64_t)a.seq_lens[g0 + i] : (int64_t)a.max_seq;
-                n = min(n, (int64_t)a.max_seq);
-                n = min(n, (int64_t)a.cache_rows - max(from, to));
-                if (from >= 0 && to >= 0 && from != to && n > 0) m = Move{(uint64_t)from, (uint64_t)to, (uint32_t)n};
-            }
+    const uint32_t i = threadIdx.x & 63u;   // every wavefront finds the moves, the first one keeps them
+    Move m{0, 0, 0, 0};
+    if (i < B && i < a.beams) {
+        const size_t g0 = (size_t)group * a.beams;
+        const int32_t p = a.parents[g0 + i];
+        if (p >= 0 && (uint32_t)p < a.beams && (uint32_t)p != i) {
+            const int32_t from = a.row_base[g0 + p], to = a.row_base[g0 + i];
+            int64_t n = a.seq_lens ? (int64_t)a.seq_lens[g0 + i] : (int64_t)a.max_seq;
+            n = min(n, (int64_t)a.max_seq);
+            n = min(n, (int64_t)a.cache_rows - max(from, to));
+            if (from >= 0 && to >= 0 && from != to && n > 0) m = Move{(uint32_t)from, (uint32_t)to, (uint32_t)n, (uint32_t)n};
         }
-        moves[i] = m;
-        if (m.rows) atomicMax(&longest, m.rows);
     }
+    const uint64_t some = __ballot(m.rows != 0);
+    if (!some) return;
+    const uint32_t one = (uint32_t)__builtin_ctzll(some);
+    const uint32_t from = __shfl((int)m.from, one, 64), rows_from = __shfl((int)m.rows, one, 64);
+    uint32_t longest = m.rows;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) longest = max(longest, (uint32_t)__shfl_xor((int)longest, o, 64));
+    if (!m.rows) {
+        m.from = from;
+        m.rows_from = rows_from;
+    }
+    if (threadIdx.x < B) moves[threadIdx.x] = m;
     __syncthreads();
-    const uint32_t n = longest;
-    if (!n) return;
     char *base = a.buf[buf] + layer * a.layer_bytes[buf];
-    if (a.vec[buf] == 16) permute<ju4, B>(base, a.row_bytes[buf], moves, chunk, a.chunks, n);
-    else if (a.vec[buf] == 4) permute<uint32_t, B>(base, a.row_bytes[buf], moves, chunk, a.chunks, n);
-    else permute<uint8_t, B>(base, a.row_bytes[buf], moves, chunk, a.chunks, n);
+    longest = uniform(longest);
+    if (a.vec[buf] == 16) permute<ju4, B>(base, a.row_bytes[buf], moves, chunk, a.chunks, longest);
+    else if (a.vec[buf] == 4) permute<uint32_t, B>(base, a.row_bytes[buf], moves, chunk, a.chunks, longest);
+    else permute<uint8_t, B>(base, a.row_bytes[buf], moves, chunk, a.chunks, longest);
 }
 
 }  // namespace
