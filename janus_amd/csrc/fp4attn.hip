@@ -205,7 +205,7 @@ template <bool SPLIT> __device__ __forceinline__ bool find_task(const Fp4Args &a
             w.first_slot = s_first + number;
             done += n;
             w.more = done < quota;
-            return true;
+            return w.parts == 1 || w.slot < a.slots;   // more tiles than there can be: sequences that overlap
         }
         start = lane_value(upto, 63);
         if constexpr (SPLIT) before += lane_value(upto_tiles, 63);
@@ -234,14 +234,14 @@ __device__ __forceinline__ void lds_request(const uint8_t *base, uint32_t off, u
 }
 #pragma clang diagnostic pop
 
-// A tile of 32 S ph positions of hw KV heads, whose rows of hw D / 2 bytes lie one behind the
-// other in LDS (2 S KB a wavefront of K, then of V, for 128 dims). Whole rows are requested, 1 KB an
+// A tile of 32 ph positions of hw KV heads, whose rows of hw D / 2 bytes lie one behind the
+// other in LDS (2 KB a wavefront of K, then of V, for 128 dims). Whole rows are requested, 1 KB an
 // instruction: 270000 positions of 8 heads come at 6.4 TB/s like this and at 4.9 where
 // every wavefront loads its own head's 64 bytes of a row. The 16-byte segments of a row
 // are permuted by the heads' number of segments (U), so that 16 positions of a head (K), or four
 // positions four apart (V), lie in different banks.
-template <int D, int S, int NW> struct Tile {
-    static constexpr uint32_t U = D / 32, kBytes = 16u * NW * D * S;   // segments of a head; bytes of K
+template <int D, int NW> struct Tile {
+    static constexpr uint32_t U = D / 32, kBytes = 16u * NW * D;   // segments of a head; bytes of K
     static constexpr int N = kBytes / (1024 * NW);                     // requests of a wavefront for K
     static constexpr uint32_t kLds = 4 * kBytes;                       // two tiles
     const uint8_t *kc, *ks, *vc, *vs;   // of the workgroup's first head at position 0
@@ -370,29 +370,23 @@ template <typename T, int D, int NT> struct Columns {
         }
     }
 
-    // 32 S positions from p on. masked: some column of the wavefront does not see all of
-    // them. v(u, j): the lane's bytes of V at position j of 32 u. Returns whether a block among
+    // 32 positions from p on. masked: some column of the wavefront does not see all of
+    // them. v(j): the lane's bytes of V at its position j. Returns whether a block among
     // them is NaN; its scale counts as 1 then.
-    template <int S, typename V> __device__ __forceinline__ bool step(Raw<D> (&r)[S], uint32_t lane, uint32_t p, bool masked, V v) {
+    template <typename V> __device__ __forceinline__ bool step(Raw<D> &r, uint32_t lane, uint32_t p, bool masked, V v) {
         const uint32_t g = lane >> 4;
-        uint32_t nans = 0;
-#pragma unroll
-        for (int u = 0; u < S; ++u) nans |= nan_bytes(r[u].ks[0]) | nan_bytes(r[u].ks[1]) | nan_bytes(r[u].vs);
-        const bool odd = __any(nans != 0);
+        const bool odd = __any((nan_bytes(r.ks[0]) | nan_bytes(r.ks[1]) | nan_bytes(r.vs)) != 0);
         if (odd) {
-#pragma unroll
-            for (int u = 0; u < S; ++u) {
-                r[u].ks[0] = without_nans(r[u].ks[0]);
-                r[u].ks[1] = without_nans(r[u].ks[1]);
-                r[u].vs = without_nans(r[u].vs);
-            }
+            r.ks[0] = without_nans(r.ks[0]);
+            r.ks[1] = without_nans(r.ks[1]);
+            r.vs = without_nans(r.vs);
         }
         const uint32_t kshift = g * (D / 4) / 32 * 8;   // the lane's block of K, and of V
         const uint32_t vblock = (lane & 15u) * (D / 16) / 32, vmask = 0xffu << (8u * vblock), vturn = (8u * vblock - 23u) & 31u;
-        ff4 s[NT][2 * S];
+        ff4 s[NT][2];
 #pragma unroll
-        for (int h = 0; h < 2 * S; ++h) {
-            const float sc = __uint_as_float((r[h >> 1].ks[h & 1] >> kshift & 0xffu) << 23);
+        for (int h = 0; h < 2; ++h) {
+            const float sc = __uint_as_float((r.ks[h] >> kshift & 0xffu) << 23);
             ff4 small[P == 2 ? NT : 1];
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
@@ -401,7 +395,7 @@ template <typename T, int D, int NT> struct Columns {
             }
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) {
-                const uint32_t w = r[h >> 1].k[h & 1][i];
+                const uint32_t w = r.k[h][i];
                 const fh8 k = h8(fp4_pair<0>(w, sc), fp4_pair<1>(w, sc), fp4_pair<2>(w, sc), fp4_pair<3>(w, sc));
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
@@ -417,7 +411,7 @@ template <typename T, int D, int NT> struct Columns {
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int h = 0; h < 2 * S; ++h)
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) s[t][h][j] = p + 16u * h + 4u * g + j < vis[t] ? s[t][h][j] : -INFINITY;
         }
@@ -426,7 +420,7 @@ template <typename T, int D, int NT> struct Columns {
         for (int t = 0; t < NT; ++t) {
             float mx = s[t][0][0];
 #pragma unroll
-            for (int j = 1; j < 8 * S; ++j) mx = fmaxf(mx, s[t][j >> 2][j & 3]);
+            for (int j = 1; j < 8; ++j) mx = fmaxf(mx, s[t][j >> 2][j & 3]);
             mx = groups_max(mx);
             if (__any((mx - m[t]) * cs[t] > kSlack)) {
                 const float now = fmaxf(m[t], mx);
@@ -438,71 +432,68 @@ template <typename T, int D, int NT> struct Columns {
             }
             m0[t] = m[t] == -INFINITY ? 0.0f : m[t];
         }
+        fh8 pp[NT][P];
 #pragma unroll
-        for (int u = 0; u < S; ++u) {
-            fh8 pp[NT][P];
+        for (int t = 0; t < NT; ++t) {
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float x = __builtin_amdgcn_exp2f(fmaf(s[t][2 * u + (j >> 2)][j & 3] - m0[t], cs[t], kBias));   // large scores keep their last bits
-                    l[t] += x;
-                    pp[t][0][j] = (_Float16)x;
-                    if constexpr (P == 2) pp[t][1][j] = (_Float16)(x - (float)pp[t][0][j]);
-                }
+            for (int j = 0; j < 8; ++j) {
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[t][j >> 2][j & 3] - m0[t], cs[t], kBias));   // large scores keep their last bits
+                l[t] += x;
+                pp[t][0][j] = (_Float16)x;
+                if constexpr (P == 2) pp[t][1][j] = (_Float16)(x - (float)pp[t][0][j]);
             }
-            // the byte of position j, which lane j of the 16 holds, at the exponent's place
-            float sc[8];
-            auto spread = [&](auto j) {
-                const uint32_t w = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)r[u].vs, 0x150 + decltype(j)::value, 0xf, 0xf, false) & vmask;   // row_newbcast
-                sc[decltype(j)::value] = __uint_as_float(__builtin_amdgcn_alignbit(w, w, vturn));
-            };
-            spread(std::integral_constant<int, 0>{});
-            spread(std::integral_constant<int, 1>{});
-            spread(std::integral_constant<int, 2>{});
-            spread(std::integral_constant<int, 3>{});
-            spread(std::integral_constant<int, 4>{});
-            spread(std::integral_constant<int, 5>{});
-            spread(std::integral_constant<int, 6>{});
-            spread(std::integral_constant<int, 7>{});
-            uint32_t raw[8];
+        }
+        // the byte of position j, which lane j of the 16 holds, at the exponent's place
+        float sc[8];
+        auto spread = [&](auto j) {
+            const uint32_t w = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)r.vs, 0x150 + decltype(j)::value, 0xf, 0xf, false) & vmask;   // row_newbcast
+            sc[decltype(j)::value] = __uint_as_float(__builtin_amdgcn_alignbit(w, w, vturn));
+        };
+        spread(std::integral_constant<int, 0>{});
+        spread(std::integral_constant<int, 1>{});
+        spread(std::integral_constant<int, 2>{});
+        spread(std::integral_constant<int, 3>{});
+        spread(std::integral_constant<int, 4>{});
+        spread(std::integral_constant<int, 5>{});
+        spread(std::integral_constant<int, 6>{});
+        spread(std::integral_constant<int, 7>{});
+        uint32_t raw[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) raw[j] = v(u, j);
-            auto two = [&](auto byte) {
-                constexpr int B = decltype(byte)::value;
-                uint32_t h[8], lo[4], hi[4];
+        for (int j = 0; j < 8; ++j) raw[j] = v(j);
+        auto two = [&](auto byte) {
+            constexpr int B = decltype(byte)::value;
+            uint32_t h[8], lo[4], hi[4];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) h[j] = fp4_pair<B>(raw[j], sc[j]);
+            for (int j = 0; j < 8; ++j) h[j] = fp4_pair<B>(raw[j], sc[j]);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    lo[j] = __builtin_amdgcn_perm(h[2 * j + 1], h[2 * j], 0x05040100u);
-                    hi[j] = __builtin_amdgcn_perm(h[2 * j + 1], h[2 * j], 0x07060302u);
-                }
-                const fh8 v0 = h8(lo[0], lo[1], lo[2], lo[3]), v1 = h8(hi[0], hi[1], hi[2], hi[3]);
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int w = 0; w < P; ++w) {
-                        o[t][2 * B] = mfma(v0, pp[t][w], o[t][2 * B]);
-                        o[t][2 * B + 1] = mfma(v1, pp[t][w], o[t][2 * B + 1]);
-                    }
-            };
-            two(std::integral_constant<int, 0>{});
-            two(std::integral_constant<int, 1>{});
-            if constexpr (D == 128) {
-                two(std::integral_constant<int, 2>{});
-                two(std::integral_constant<int, 3>{});
+            for (int j = 0; j < 4; ++j) {
+                lo[j] = __builtin_amdgcn_perm(h[2 * j + 1], h[2 * j], 0x05040100u);
+                hi[j] = __builtin_amdgcn_perm(h[2 * j + 1], h[2 * j], 0x07060302u);
             }
+            const fh8 v0 = h8(lo[0], lo[1], lo[2], lo[3]), v1 = h8(hi[0], hi[1], hi[2], hi[3]);
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int w = 0; w < P; ++w) {
+                    o[t][2 * B] = mfma(v0, pp[t][w], o[t][2 * B]);
+                    o[t][2 * B + 1] = mfma(v1, pp[t][w], o[t][2 * B + 1]);
+                }
+        };
+        two(std::integral_constant<int, 0>{});
+        two(std::integral_constant<int, 1>{});
+        if constexpr (D == 128) {
+            two(std::integral_constant<int, 2>{});
+            two(std::integral_constant<int, 3>{});
         }
         return odd;
     }
 };
 
 // First positions with a NaN block of K (x), and of V in the lane's output dims (y),
-// among `span` (32 or 64) positions from each of p, p + step, ... below end.
+// among 32 positions from each of p, p + step, ... below end.
 template <int D>
 __device__ __forceinline__ uint2 first_nans(const uint8_t *ks, const uint8_t *vs, uint32_t srow, uint32_t p, uint32_t end,
-                                            uint32_t step, uint32_t span) {
+                                            uint32_t step) {
     const uint32_t lane = threadIdx.x & 63u, mine = (lane >> 4) * (D / 4) / 32;
     uint2 at = make_uint2(0xffffffffu, 0xffffffffu);
     for (; p < end; p += step) {
@@ -510,7 +501,7 @@ __device__ __forceinline__ uint2 first_nans(const uint8_t *ks, const uint8_t *vs
         bool kn = false;
         for (uint32_t b = 0; b < D / 32; ++b) {
             bool vn = false;
-            if (lane < span && i < end) {
+            if (lane < 32u && i < end) {
                 kn |= ks[(size_t)i * srow + b] > 140;
                 vn = vs[(size_t)i * srow + b] > 140;
             }
@@ -524,8 +515,8 @@ __device__ __forceinline__ uint2 first_nans(const uint8_t *ks, const uint8_t *vs
 }
 
 // Up to 16 NT columns of a sequence and positions [from, to): the NW wavefronts of a
-// workgroup take hw KV heads and ph phases of 32 S positions each; PER of them share a SIMD.
-template <typename T, int D, int NT, int S, int NW, int PER, bool SPLIT>
+// workgroup take hw KV heads and ph phases of 32 positions each; PER of them share a SIMD.
+template <typename T, int D, int NT, int NW, int PER, bool SPLIT>
 __global__ __launch_bounds__(NW * 64, PER) void fp4_attn_kernel(Fp4Args args) {
     constexpr uint32_t DL = D / 4;   // output dims of a lane
     extern __shared__ __align__(16) uint8_t smem[];   // two tiles, then the phases' results
@@ -539,196 +530,187 @@ __global__ __launch_bounds__(NW * 64, PER) void fp4_attn_kernel(Fp4Args args) {
     Task w;
     w.more = true;
     for (uint32_t done = 0; w.more && find_task<SPLIT>(late_args(), share, done, w);) {
-    const Fp4Args &a = late_args();
-    const uint32_t lane = fresh_thread() & 63u, g = lane >> 4, at = lane & 15u;
-    const uint32_t hwave = wave & (a.hw - 1), phase = wave / a.hw, head0 = (blockIdx.x >> 3) % a.head_groups * a.hw, kvh = head0 + hwave;
-    const uint32_t c0 = w.c0, columns = w.s.n * a.G;   // below 2^25
+        const Fp4Args &a = late_args();
+        const uint32_t lane = fresh_thread() & 63u, g = lane >> 4, at = lane & 15u;
+        const uint32_t hwave = wave & (a.hw - 1), phase = wave / a.hw, head0 = (blockIdx.x >> 3) % a.head_groups * a.hw, kvh = head0 + hwave;
+        const uint32_t c0 = w.c0, columns = w.s.n * a.G;   // below 2^25
 
-    // positions that columns of the tile see: the last ones the most
-    const uint32_t most = seen_of(w.s, (min(c0 + 16u * NT, columns) - 1) / a.G), fewest = seen_of(w.s, c0 / a.G);
-    const uint32_t end = __builtin_amdgcn_readfirstlane(min(most, w.to)), from = __builtin_amdgcn_readfirstlane(w.from), step = 32u * S * a.ph;
-    const size_t base = w.s.base;
-    const uint32_t rows = a.cache_rows - w.s.base;   // of the cache from position 0 on
-    Tile<D, S, NW> tile;
-    tile.row = a.kv_heads * (D / 2);
-    tile.srow = a.kv_heads * (D / 32);
-    tile.kc = a.kc + base * tile.row + head0 * (D / 2);
-    tile.vc = a.vc + base * tile.row + head0 * (D / 2);
-    tile.ks = a.ks + base * tile.srow + kvh * (D / 32);   // the wavefront's own
-    tile.vs = a.vs + base * tile.srow + kvh * (D / 32);
-    tile.segs = a.hw * Tile<D, S, NW>::U;
-    tile.heads = a.hw - 1;
-    tile.fold = tile.segs >= 16u ? 0u : 4u - (31u - (uint32_t)__builtin_clz(tile.segs));
-    tile.offsets(lane, wave, step - 1);
-    // the scales of the wavefront's 32 positions of a tile
-    typedef std::conditional_t<D == 128, uint32_t, uint16_t> word;
-    uint32_t ks0[S] = {}, ks1[S] = {}, vs0[S] = {};
-    const uint32_t kpos = at, vpos = (at & 4u) * 4u + 4u * g + (at & 3u);
-    const uint32_t kso = kpos * tile.srow, vso = vpos * tile.srow;
-    auto fetch = [&](uint32_t p, uint32_t b) {
-        const uint32_t q = p + 32u * S * phase;
-        if (p + step > rows) {   // the cache ends inside the tile: its last row again
-            tile.offsets(lane, wave, rows - 1 - p);
-            tile.request(p, wave, lds0 + b * (2 * Tile<D, S, NW>::kBytes));
-#pragma unroll
-            for (int u = 0; u < S; ++u) {
-                ks0[u] = *(const word *)(tile.ks + (size_t)min(q + 32u * u + kpos, rows - 1) * tile.srow);
-                ks1[u] = *(const word *)(tile.ks + (size_t)min(q + 32u * u + kpos + 16u, rows - 1) * tile.srow);
-                vs0[u] = *(const word *)(tile.vs + (size_t)min(q + 32u * u + vpos, rows - 1) * tile.srow);
+        // positions that columns of the tile see: the last ones the most
+        const uint32_t most = seen_of(w.s, (min(c0 + 16u * NT, columns) - 1) / a.G), fewest = seen_of(w.s, c0 / a.G);
+        const uint32_t end = __builtin_amdgcn_readfirstlane(min(most, w.to)), from = __builtin_amdgcn_readfirstlane(w.from), step = 32u * a.ph;
+        const size_t base = w.s.base;
+        const uint32_t rows = a.cache_rows - w.s.base;   // of the cache from position 0 on
+        Tile<D, NW> tile;
+        tile.row = a.kv_heads * (D / 2);
+        tile.srow = a.kv_heads * (D / 32);
+        tile.kc = a.kc + base * tile.row + head0 * (D / 2);
+        tile.vc = a.vc + base * tile.row + head0 * (D / 2);
+        tile.ks = a.ks + base * tile.srow + kvh * (D / 32);   // the wavefront's own
+        tile.vs = a.vs + base * tile.srow + kvh * (D / 32);
+        tile.segs = a.hw * Tile<D, NW>::U;
+        tile.heads = a.hw - 1;
+        tile.fold = tile.segs >= 16u ? 0u : 4u - (31u - (uint32_t)__builtin_clz(tile.segs));
+        tile.offsets(lane, wave, step - 1);
+        // the scales of the wavefront's 32 positions of a tile
+        typedef std::conditional_t<D == 128, uint32_t, uint16_t> word;
+        uint32_t ks0 = 0, ks1 = 0, vs0 = 0;
+        const uint32_t kpos = at, vpos = (at & 4u) * 4u + 4u * g + (at & 3u);
+        const uint32_t kso = kpos * tile.srow, vso = vpos * tile.srow;
+        auto fetch = [&](uint32_t p, uint32_t b) {
+            const uint32_t q = p + 32u * phase;
+            if (p + step > rows) {   // the cache ends inside the tile: its last row again
+                tile.offsets(lane, wave, rows - 1 - p);
+                tile.request(p, wave, lds0 + b * (2 * Tile<D, NW>::kBytes));
+                ks0 = *(const word *)(tile.ks + (size_t)min(q + kpos, rows - 1) * tile.srow);
+                ks1 = *(const word *)(tile.ks + (size_t)min(q + kpos + 16u, rows - 1) * tile.srow);
+                vs0 = *(const word *)(tile.vs + (size_t)min(q + vpos, rows - 1) * tile.srow);
+                return;
             }
-            return;
-        }
-        // rows behind the sequence's end are other sequences' or none's, and no column sees them
-        tile.request(p, wave, lds0 + b * (2 * Tile<D, S, NW>::kBytes));
+            // rows behind the sequence's end are other sequences' or none's, and no column sees them
+            tile.request(p, wave, lds0 + b * (2 * Tile<D, NW>::kBytes));
+            ks0 = *(const word *)(tile.ks + (size_t)q * tile.srow + kso);
+            ks1 = *(const word *)(tile.ks + (size_t)(q + 16u) * tile.srow + kso);
+            vs0 = *(const word *)(tile.vs + (size_t)q * tile.srow + vso);
+        };
+        if (from < end) fetch(from, 0);
+        Columns<T, D, NT> col;
+        col.load(a, w, lane, c0, kvh);
+        if (from < end) {
+            bool odd = false;
+            // offsets of the lane's operands in a tile: K of position at of 16, V of 4 g of 16 (r rows on under the same turn)
+            const uint32_t pos0 = 32u * phase, seg0 = hwave * Tile<D, NW>::U, line = tile.segs * 16u;
+            uint32_t kat[2], vat[2];
 #pragma unroll
-        for (int u = 0; u < S; ++u) {
-            ks0[u] = *(const word *)(tile.ks + (size_t)(q + 32u * u) * tile.srow + kso);
-            ks1[u] = *(const word *)(tile.ks + (size_t)(q + 32u * u + 16u) * tile.srow + kso);
-            vs0[u] = *(const word *)(tile.vs + (size_t)(q + 32u * u) * tile.srow + vso);
-        }
-    };
-    if (from < end) fetch(from, 0);
-    Columns<T, D, NT> col;
-    col.load(a, w, lane, c0, kvh);
-    if (from < end) {
-        bool odd = false;
-        // offsets of the lane's operands in a tile: K of position at of 16, V of 4 g of 16 (r rows on under the same turn)
-        const uint32_t pos0 = 32u * S * phase, seg0 = hwave * Tile<D, S, NW>::U, line = tile.segs * 16u;
-        uint32_t kat[2 * S], vat[2 * S];
-#pragma unroll
-        for (int h = 0; h < 2 * S; ++h) {
-            const uint32_t kn = pos0 + 16u * h + at, vn = pos0 + 16u * h + 4u * g;
-            kat[h] = kn * line + ((seg0 + g * (D / 8) / 16) ^ tile.k_turn(kn)) * 16u + (D == 64 ? (g & 1u) * 8u : 0u);
-            vat[h] = vn * line + ((seg0 + at * (D / 32) / 16) ^ tile.v_turn(vn)) * 16u + at * (D / 32) % 16u;
-        }
-        uint32_t b = 0;
-        for (uint32_t p = from; p < end; p += step, b ^= 1u) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();   // this tile is there, the other one has been read
-            Raw<D> r[S];
-            // the scales are in registers before the next ones are asked for: a wait for them later would be one for the next tile too
-#pragma unroll
-            for (int u = 0; u < S; ++u) {
-                r[u].ks[0] = ks0[u];
-                r[u].ks[1] = ks1[u];
-                r[u].vs = vs0[u];
-                asm volatile("" : "+v"(r[u].ks[0]), "+v"(r[u].ks[1]), "+v"(r[u].vs));
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t kn = pos0 + 16u * h + at, vn = pos0 + 16u * h + 4u * g;
+                kat[h] = kn * line + ((seg0 + g * (D / 8) / 16) ^ tile.k_turn(kn)) * 16u + (D == 64 ? (g & 1u) * 8u : 0u);
+                vat[h] = vn * line + ((seg0 + at * (D / 32) / 16) ^ tile.v_turn(vn)) * 16u + at * (D / 32) % 16u;
             }
-            if (p + step < end) fetch(p + step, b ^ 1u);
-            const uint32_t mine = p + 32u * S * phase;
-            if (mine >= end) continue;
-            const uint8_t *kt = smem + b * (2 * Tile<D, S, NW>::kBytes), *vt = kt + Tile<D, S, NW>::kBytes;
+            uint32_t b = 0;
+            for (uint32_t p = from; p < end; p += step, b ^= 1u) {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __syncthreads();   // this tile is there, the other one has been read
+                Raw<D> r;
+                // the scales are in registers before the next ones are asked for: a wait for them later would be one for the next tile too
+                r.ks[0] = ks0;
+                r.ks[1] = ks1;
+                r.vs = vs0;
+                asm volatile("" : "+v"(r.ks[0]), "+v"(r.ks[1]), "+v"(r.vs));
+                if (p + step < end) fetch(p + step, b ^ 1u);
+                const uint32_t mine = p + 32u * phase;
+                if (mine >= end) continue;
+                const uint8_t *kt = smem + b * (2 * Tile<D, NW>::kBytes), *vt = kt + Tile<D, NW>::kBytes;
 #pragma unroll
-            for (int h = 0; h < 2 * S; ++h) {
-                typedef uint32_t vec __attribute__((ext_vector_type(D / 32)));
-                const vec k = *(const vec *)(kt + kat[h]);
+                for (int h = 0; h < 2; ++h) {
+                    typedef uint32_t vec __attribute__((ext_vector_type(D / 32)));
+                    const vec k = *(const vec *)(kt + kat[h]);
 #pragma unroll
-                for (int i = 0; i < D / 32; ++i) r[h >> 1].k[h & 1][i] = k[i];
+                    for (int i = 0; i < D / 32; ++i) r.k[h][i] = k[i];
+                }
+                odd |= col.step(r, lane, mine, mine + 32u > fewest || mine + 32u > end,
+                                [&](int j) -> uint32_t { return *(const word *)(vt + vat[j >> 2] + (j & 3) * line); });
             }
-            odd |= col.step(r, lane, mine, mine + 32u * S > fewest || mine + 32u * S > end,
-                            [&](int u, int j) -> uint32_t { return *(const word *)(vt + vat[2 * u + (j >> 2)] + (j & 3) * line); });
-        }
-        if (odd) {
-            const uint2 at = first_nans<D>(tile.ks, tile.vs, tile.srow, from + 32u * S * phase, end, step, 32u * S);
-            const float nan = __uint_as_float(0x7fc00000u);
+            if (odd) {
+                const uint2 at = first_nans<D>(tile.ks, tile.vs, tile.srow, from + 32u * phase, end, step);
+                const float nan = __uint_as_float(0x7fc00000u);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                if (at.x < col.vis[t]) col.l[t] = nan;
-                if (at.y < col.vis[t])
+                for (int t = 0; t < NT; ++t) {
+                    if (at.x < col.vis[t]) col.l[t] = nan;
+                    if (at.y < col.vis[t])
 #pragma unroll
-                    for (int i = 0; i < D / 16; ++i) col.o[t][i] = ff4{nan, nan, nan, nan};
-            }
-        }
-    }
-
-    if (SPLIT || a.ph > 1) __syncthreads();   // the tiles have been read
-    // the phases of a head and column tile join in its first one
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        col.l[t] = groups_sum(col.l[t]);
-        col.m[t] = col.m[t] == -INFINITY ? col.m[t] : col.m[t] * col.cs[t];   // in powers of two from here on
-    }
-    if (a.ph > 1) {
-        constexpr uint32_t kArea = NT * (D / 4 + 2) * 64u;   // floats of a wavefront
-        float *mine = lds + ((phase - 1) * a.hw + hwave) * kArea;
-        if (phase > 0) {
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                float *at = mine + t * (D / 4 + 2) * 64u + lane;
-                at[0] = col.m[t];
-                at[64] = col.l[t];
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) at[(2 + 4 * i + r) * 64] = col.o[t][i][r];
-            }
-        }
-        __syncthreads();
-        if (phase == 0)
-        for (uint32_t h = 1; h < a.ph; ++h) {
-            const float *other = lds + ((h - 1) * a.hw + hwave) * kArea + lane;
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const float *at = other + t * (D / 4 + 2) * 64u;
-                const float m2 = at[0], now = fmaxf(col.m[t], m2);
-                const float f1 = col.m[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(col.m[t] - now);
-                const float f2 = m2 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m2 - now);
-                // what has seen nothing is 0, or NaN where a block was marked
-                col.l[t] = col.l[t] * f1 + at[64] * f2;
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) col.o[t][i][r] = col.o[t][i][r] * f1 + at[(2 + 4 * i + r) * 64] * f2;
-                col.m[t] = now;
-            }
-        }
-        if constexpr (SPLIT) __syncthreads();   // the areas are written again for the next columns
-        if (phase > 0) {
-            if constexpr (SPLIT) continue;
-            else return;
-        }
-    }
-    const Fp4Args &z = late_args();
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const uint32_t c = c0 + t * 16u + (lane & 15u);
-        if (c >= columns) continue;
-        const uint32_t r = c / z.G, gh = c % z.G;
-        if ((col.bad >> t & 1u) && col.vis[t]) col.l[t] = __uint_as_float(0x7fc00000u);
-        if (SPLIT && w.parts > 1) {
-            const size_t at = ((size_t)w.slot * z.kv_heads + kvh) * z.cols + (c - w.c0);
-            float *to = z.part + at * D + g * DL;
-#pragma unroll
-            for (int rr = 0; rr < 4; ++rr)
-#pragma unroll
-                for (int i = 0; i < D / 16; i += 4)
-                    *(ff4 *)(to + rr * (D / 16) + i) = ff4{col.o[t][i][rr], col.o[t][i + 1][rr], col.o[t][i + 2][rr], col.o[t][i + 3][rr]};
-            if (g == 0) {
-                z.part_ml[2 * at] = col.m[t];
-                z.part_ml[2 * at + 1] = col.l[t];
-            }
-        } else {
-            const float inv = col.vis[t] ? 1.0f / col.l[t] : 0.0f;
-            T *to = (T *)z.out + ((size_t)(w.s.row0 + r) * z.heads + (size_t)kvh * z.G + gh) * D + g * DL;
-#pragma unroll
-            for (int rr = 0; rr < 4; ++rr) {
-                typedef T vec __attribute__((ext_vector_type(D / 16 * sizeof(T) > 16 ? 4 : D / 16)));
-                constexpr int N = sizeof(vec) / sizeof(T);
-#pragma unroll
-                for (int i = 0; i < D / 16; i += N) {
-                    vec v;
-#pragma unroll
-                    for (int u = 0; u < N; ++u) v[u] = col.vis[t] ? (T)(col.o[t][i + u][rr] * inv) : (T)0.0f;
-                    *(vec *)(to + rr * (D / 16) + i) = v;
+                        for (int i = 0; i < D / 16; ++i) col.o[t][i] = ff4{nan, nan, nan, nan};
                 }
             }
         }
-        if (SPLIT && w.slot == w.first_slot && kvh == 0 && g == 0) {
-            uint32_t *to = z.meta + 2 * ((size_t)w.s.row0 * z.G + c);
-            to[0] = w.first_slot;
-            to[1] = w.parts | (col.vis[t] ? 0u : 1u << 23) | (c - w.c0) << 24;
+
+        if (SPLIT || a.ph > 1) __syncthreads();   // the tiles have been read
+        // the phases of a head and column tile join in its first one
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            col.l[t] = groups_sum(col.l[t]);
+            col.m[t] = col.m[t] == -INFINITY ? col.m[t] : col.m[t] * col.cs[t];   // in powers of two from here on
         }
-    }
+        if (a.ph > 1) {
+            constexpr uint32_t kArea = NT * (D / 4 + 2) * 64u;   // floats of a wavefront
+            float *mine = lds + ((phase - 1) * a.hw + hwave) * kArea;
+            if (phase > 0) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    float *at = mine + t * (D / 4 + 2) * 64u + lane;
+                    at[0] = col.m[t];
+                    at[64] = col.l[t];
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) at[(2 + 4 * i + r) * 64] = col.o[t][i][r];
+                }
+            }
+            __syncthreads();
+            if (phase == 0)
+            for (uint32_t h = 1; h < a.ph; ++h) {
+                const float *other = lds + ((h - 1) * a.hw + hwave) * kArea + lane;
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const float *at = other + t * (D / 4 + 2) * 64u;
+                    const float m2 = at[0], now = fmaxf(col.m[t], m2);
+                    const float f1 = col.m[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(col.m[t] - now);
+                    const float f2 = m2 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m2 - now);
+                    // what has seen nothing is 0, or NaN where a block was marked
+                    col.l[t] = col.l[t] * f1 + at[64] * f2;
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) col.o[t][i][r] = col.o[t][i][r] * f1 + at[(2 + 4 * i + r) * 64] * f2;
+                    col.m[t] = now;
+                }
+            }
+            if constexpr (SPLIT) __syncthreads();   // the areas are written again for the next columns
+            if (phase > 0) {
+                if constexpr (SPLIT) continue;
+                else return;
+            }
+        }
+        const Fp4Args &z = late_args();
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const uint32_t c = c0 + t * 16u + (lane & 15u);
+            if (c >= columns) continue;
+            const uint32_t r = c / z.G, gh = c % z.G;
+            if ((col.bad >> t & 1u) && col.vis[t]) col.l[t] = __uint_as_float(0x7fc00000u);
+            if (SPLIT && w.parts > 1) {
+                const size_t at = ((size_t)w.slot * z.kv_heads + kvh) * z.cols + (c - w.c0);
+                float *to = z.part + at * D + g * DL;
+#pragma unroll
+                for (int rr = 0; rr < 4; ++rr)
+#pragma unroll
+                    for (int i = 0; i < D / 16; i += 4)
+                        *(ff4 *)(to + rr * (D / 16) + i) = ff4{col.o[t][i][rr], col.o[t][i + 1][rr], col.o[t][i + 2][rr], col.o[t][i + 3][rr]};
+                if (g == 0) {
+                    z.part_ml[2 * at] = col.m[t];
+                    z.part_ml[2 * at + 1] = col.l[t];
+                }
+            } else {
+                const float inv = col.vis[t] ? 1.0f / col.l[t] : 0.0f;
+                T *to = (T *)z.out + ((size_t)(w.s.row0 + r) * z.heads + (size_t)kvh * z.G + gh) * D + g * DL;
+#pragma unroll
+                for (int rr = 0; rr < 4; ++rr) {
+                    typedef T vec __attribute__((ext_vector_type(D / 16 * sizeof(T) > 16 ? 4 : D / 16)));
+                    constexpr int N = sizeof(vec) / sizeof(T);
+#pragma unroll
+                    for (int i = 0; i < D / 16; i += N) {
+                        vec v;
+#pragma unroll
+                        for (int u = 0; u < N; ++u) v[u] = col.vis[t] ? (T)(col.o[t][i + u][rr] * inv) : (T)0.0f;
+                        *(vec *)(to + rr * (D / 16) + i) = v;
+                    }
+                }
+            }
+            if (SPLIT && w.slot == w.first_slot && kvh == 0 && g == 0) {
+                uint32_t *to = z.meta + 2 * ((size_t)w.s.row0 * z.G + c);
+                to[0] = w.first_slot;
+                to[1] = w.parts | (col.vis[t] ? 0u : 1u << 23) | (c - w.c0) << 24;
+            }
+        }
     }
 }
 
@@ -855,6 +837,18 @@ template <int D> __device__ __forceinline__ Nans<D> all_nans(const uint8_t *ks, 
     return at;
 }
 
+// A wavefront's 32 rows of q or of the output pass through LDS, so that memory sees whole
+// lines: a lane has (needs) 16 or 8 bytes of a row at a time, and 32 rows' next ones.
+// Rows of `Rows::kBytes` bytes, their 16-byte pieces permuted by the row's number.
+template <typename T, int D, int TP> struct Rows {
+    static constexpr uint32_t kBytes = TP * D / 32, kPieces = kBytes / 16, kDims = kBytes / sizeof(T);
+    static constexpr int kPasses = D * sizeof(T) / kBytes, kTurns = kPieces / 2;   // 64 pieces a turn
+    static_assert(kBytes >= 128 && kPasses * kDims == D, "whole lines");
+    static __device__ __forceinline__ uint32_t place(uint32_t row, uint32_t piece) {
+        return row * kBytes + (piece ^ ((kPieces == 16 ? row : row >> 1) & (kPieces - 1))) * 16u;
+    }
+};
+
 template <typename T, int D, int TP, bool SPLIT>
 __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
     constexpr int P = sizeof(T) == 4 ? 2 : 1, NB = TP / 32, QN = D / 16, ND = D / 32;
@@ -869,299 +863,331 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
     Task w;
     w.more = true;
     for (uint32_t done = 0; w.more && find_task<SPLIT>(late_args(), share, done, w);) {
-    const Fp4Args &a = late_args();
-    const uint32_t tid = fresh_thread(), lane = tid & 63u, col = lane & 31u, h = lane >> 5;
-    const uint32_t columns = w.s.n * a.G;
-    auto seen = [&](uint32_t c) { return seen_of(w.s, c / a.G); };
-    const uint32_t group_hi = seen(min(w.c0 + 127u, columns - 1));   // the last column sees most
-    const uint32_t p0 = __builtin_amdgcn_readfirstlane(min(w.from, group_hi)), p1 = __builtin_amdgcn_readfirstlane(min(w.to, group_hi));
-    const uint32_t c0 = w.c0 + 32u * wave;
-    const bool idle = c0 >= columns;
-    const uint32_t wave_lo = idle ? 0u : __builtin_amdgcn_readfirstlane(seen(c0));
-    const uint32_t wave_hi = idle ? 0u : __builtin_amdgcn_readfirstlane(min(seen(min(c0 + 31u, columns - 1)), p1));
-    const uint32_t c = min(c0 + col, columns - 1), vis = seen(c);
-    const size_t qat = (size_t)(w.s.row0 + c / a.G) * a.heads + (size_t)kvh * a.G + c % a.G;
+        const Fp4Args &a = late_args();
+        const uint32_t tid = fresh_thread(), lane = tid & 63u, col = lane & 31u, h = lane >> 5;
+        const uint32_t columns = w.s.n * a.G;
+        auto seen = [&](uint32_t c) { return seen_of(w.s, c / a.G); };
+        const uint32_t group_hi = seen(min(w.c0 + 127u, columns - 1));   // the last column sees most
+        const uint32_t p0 = __builtin_amdgcn_readfirstlane(min(w.from, group_hi)), p1 = __builtin_amdgcn_readfirstlane(min(w.to, group_hi));
+        const uint32_t c0 = w.c0 + 32u * wave;
+        const bool idle = c0 >= columns;
+        const uint32_t wave_lo = idle ? 0u : __builtin_amdgcn_readfirstlane(seen(c0));
+        const uint32_t wave_hi = idle ? 0u : __builtin_amdgcn_readfirstlane(min(seen(min(c0 + 31u, columns - 1)), p1));
+        const uint32_t c = min(c0 + col, columns - 1), vis = seen(c);
+        const uint32_t qat = (w.s.row0 + c / a.G) * a.heads + kvh * a.G + c % a.G;   // rows * heads is below 2^25
 
-    const uint32_t row = a.kv_heads * (D / 2), srow = a.kv_heads * (D / 32);
-    const size_t base = w.s.base;
-    const uint8_t *kc = a.kc + base * row + kvh * (D / 2), *ks = a.ks + base * srow + kvh * (D / 32);
-    const uint8_t *vc = a.vc + base * row + kvh * (D / 2), *vs = a.vs + base * srow + kvh * (D / 32);
+        const uint32_t row = a.kv_heads * (D / 2), srow = a.kv_heads * (D / 32);
+        const size_t base = w.s.base;
+        const uint8_t *kc = a.kc + base * row + kvh * (D / 2), *ks = a.ks + base * srow + kvh * (D / 32);
+        const uint8_t *vc = a.vc + base * row + kvh * (D / 2), *vs = a.vs + base * srow + kvh * (D / 32);
 
-    // what a lane loads of a tile: block kb of position kn of K, and dims 8 vd .. of positions 4 vq .. of V
-    const uint32_t ku = tid, vu = kUnits == 256 ? tid : tid ^ 128u;
-    const bool has_k = kUnits == 256 || ku < kUnits, has_v = kUnits == 256 || vu < kUnits;
-    const uint32_t kn = (ku & 15u) + ku / (D / 2) * 16u, kb = ku / 16u % (D / 32), vd = vu % (D / 8), vq = vu / (D / 8);
-    ju4 kr;
-    uint32_t ksr = 0, vr[4], vsr[4] = {};
-    uint32_t ko, kso, vo[4], vso[4];   // offsets of a lane's bytes from the tile's first position
-    auto offsets = [&](uint32_t last) {   // rows beyond the part repeat its last one
-        const uint32_t n = min(kn, last);
-        ko = n * row + kb * 16u;
-        kso = n * srow + kb;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t n = min(4u * vq + i, last);
-            vo[i] = n * row + vd * 4u;
-            vso[i] = n * srow + vd / 4u;
-        }
-    };
-    offsets(min((uint32_t)TP, p1 - p0) - 1);
-    auto load = [&](uint32_t p) {
-        if (p + TP > p1) offsets(p1 - 1 - p);
-        const uint8_t *kp = kc + (size_t)p * row, *ksp = ks + (size_t)p * srow, *vp = vc + (size_t)p * row, *vsp = vs + (size_t)p * srow;
-        if (has_k) {
-            kr = *(const ju4 *)(kp + ko);
-            ksr = ksp[kso];
-        }
-        if (has_v)
+        // what a lane loads of a tile: block kb of position kn of K, and dims 8 vd .. of positions 4 vq .. of V
+        const uint32_t ku = tid, vu = kUnits == 256 ? tid : tid ^ 128u;
+        const bool has_k = kUnits == 256 || ku < kUnits, has_v = kUnits == 256 || vu < kUnits;
+        const uint32_t kn = (ku & 15u) + ku / (D / 2) * 16u, kb = ku / 16u % (D / 32), vd = vu % (D / 8), vq = vu / (D / 8);
+        ju4 kr;
+        uint32_t ksr = 0, vr[4], vsr[4] = {};
+        uint32_t ko, kso, vo[4], vso[4];   // offsets of a lane's bytes from the tile's first position
+        auto offsets = [&](uint32_t last) {   // rows beyond the part repeat its last one
+            const uint32_t n = min(kn, last);
+            ko = n * row + kb * 16u;
+            kso = n * srow + kb;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                vr[i] = *(const uint32_t *)(vp + vo[i]);
-                vsr[i] = vsp[vso[i]];
+                const uint32_t n = min(4u * vq + i, last);
+                vo[i] = n * row + vd * 4u;
+                vso[i] = n * srow + vd / 4u;
             }
-    };
-    uint32_t worst = 0;
-    auto store = [&](uint32_t b) {
-        uint8_t *kt = smem + b * 2 * kTile, *vt = kt + kTile;
-        if (has_k) {
-            const float sc = scale_of(ksr);
-            worst = max(worst, ksr);
-            uint8_t *to = kt + ((kn / 32 * QN + 2 * kb) * 64u + kn % 32) * 16u;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                *(ju4 *)(to + ((i >> 1) * 64u + (i & 1) * 32u) * 16u) =
-                    ju4{fp4_pair<0>(kr[i], sc), fp4_pair<1>(kr[i], sc), fp4_pair<2>(kr[i], sc), fp4_pair<3>(kr[i], sc)};
-        }
-        if (has_v) {
-            float sc[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                sc[i] = scale_of(vsr[i]);
-                worst = max(worst, vsr[i]);
+        };
+        offsets(min((uint32_t)TP, p1 - p0) - 1);
+        auto load = [&](uint32_t p) {
+            if (p + TP > p1) offsets(p1 - 1 - p);
+            const uint8_t *kp = kc + (size_t)p * row, *ksp = ks + (size_t)p * srow, *vp = vc + (size_t)p * row, *vsp = vs + (size_t)p * srow;
+            if (has_k) {
+                kr = *(const ju4 *)(kp + ko);
+                ksr = ksp[kso];
             }
-            // block vd / 4, slots 8 (vd % 4) .. of its 32; quad vq % 4: half vq % 2, first or second 8 bytes
-            uint8_t *to = vt + ((vq / 4 * ND + vd / 4) * 64u + (vq & 1u) * 32u + (vd & 3u) * 8u) * 16u + (vq >> 1 & 1u) * 8u;
-            const uint32_t turn = (vd & 7u) * 16u;
-            auto two = [&](auto byte) {
-                constexpr int B = decltype(byte)::value;
-                uint32_t x[4];
+            if (has_v)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = fp4_pair<B>(vr[i], sc[i]);
-                *(uint2 *)(to + ((2 * B * 16u) ^ turn)) = make_uint2(__builtin_amdgcn_perm(x[1], x[0], 0x05040100u), __builtin_amdgcn_perm(x[3], x[2], 0x05040100u));
-                *(uint2 *)(to + (((2 * B + 1) * 16u) ^ turn)) = make_uint2(__builtin_amdgcn_perm(x[1], x[0], 0x07060302u), __builtin_amdgcn_perm(x[3], x[2], 0x07060302u));
-            };
-            two(std::integral_constant<int, 0>{});
-            two(std::integral_constant<int, 1>{});
-            two(std::integral_constant<int, 2>{});
-            two(std::integral_constant<int, 3>{});
-        }
-    };
-    const uint32_t last_tile = p0 + (p1 > p0 ? (p1 - p0 - 1) / TP * TP : 0u);
-    if (p0 < p1) load(p0);
+                for (int i = 0; i < 4; ++i) {
+                    vr[i] = *(const uint32_t *)(vp + vo[i]);
+                    vsr[i] = vsp[vso[i]];
+                }
+        };
+        uint32_t worst = 0;
+        auto store = [&](uint32_t b) {
+            uint8_t *kt = smem + b * 2 * kTile, *vt = kt + kTile;
+            if (has_k) {
+                const float sc = scale_of(ksr);
+                worst = max(worst, ksr);
+                uint8_t *to = kt + ((kn / 32 * QN + 2 * kb) * 64u + kn % 32) * 16u;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    *(ju4 *)(to + ((i >> 1) * 64u + (i & 1) * 32u) * 16u) =
+                        ju4{fp4_pair<0>(kr[i], sc), fp4_pair<1>(kr[i], sc), fp4_pair<2>(kr[i], sc), fp4_pair<3>(kr[i], sc)};
+            }
+            if (has_v) {
+                float sc[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    sc[i] = scale_of(vsr[i]);
+                    worst = max(worst, vsr[i]);
+                }
+                // block vd / 4, slots 8 (vd % 4) .. of its 32; quad vq % 4: half vq % 2, first or second 8 bytes
+                uint8_t *to = vt + ((vq / 4 * ND + vd / 4) * 64u + (vq & 1u) * 32u + (vd & 3u) * 8u) * 16u + (vq >> 1 & 1u) * 8u;
+                const uint32_t turn = (vd & 7u) * 16u;
+                auto two = [&](auto byte) {
+                    constexpr int B = decltype(byte)::value;
+                    uint32_t x[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i] = fp4_pair<B>(vr[i], sc[i]);
+                    *(uint2 *)(to + ((2 * B * 16u) ^ turn)) = make_uint2(__builtin_amdgcn_perm(x[1], x[0], 0x05040100u), __builtin_amdgcn_perm(x[3], x[2], 0x05040100u));
+                    *(uint2 *)(to + (((2 * B + 1) * 16u) ^ turn)) = make_uint2(__builtin_amdgcn_perm(x[1], x[0], 0x07060302u), __builtin_amdgcn_perm(x[3], x[2], 0x07060302u));
+                };
+                two(std::integral_constant<int, 0>{});
+                two(std::integral_constant<int, 1>{});
+                two(std::integral_constant<int, 2>{});
+                two(std::integral_constant<int, 3>{});
+            }
+        };
+        const uint32_t last_tile = p0 + (p1 > p0 ? (p1 - p0 - 1) / TP * TP : 0u);
+        if (p0 < p1) load(p0);
 
-    // q of the lane's column
-    const T *qp = (const T *)a.q + qat * D;
-    fh8 q[P][QN];
-    float cs = a.scale2;
-    bool bad = false;
-    {
-        float x[QN][8];
-        uint32_t top = 0;
+        // q of the lane's column
+        fh8 q[P][QN];
+        float cs = a.scale2;
+        bool bad = false;
+        {
+            float x[QN][8];
+            uint32_t top = 0;
+            typedef Rows<T, D, TP> R;
+            uint8_t *const stage = smem + 2 * kTile + wave * (32u * R::kBytes);   // of the second tile, which nobody writes before the loop's first barrier
+            const uint32_t piece = lane % R::kPieces, r0 = lane / R::kPieces;
+            ju4 raw[R::kPasses][R::kTurns];
 #pragma unroll
-        for (int s = 0; s < QN; ++s) {
-            typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
+            for (int i = 0; i < R::kTurns; ++i) {
+                const T *src = (const T *)a.q + (size_t)__shfl(qat, (int)(r0 + i * (64u / R::kPieces))) * D + piece * (16 / sizeof(T));
 #pragma unroll
-            for (int i = 0; i < 8; i += 16 / (int)sizeof(T)) {
-                const vec v = *(const vec *)(qp + 16 * s + 8 * h + i);
-#pragma unroll
-                for (int j = 0; j < 16 / (int)sizeof(T); ++j) x[s][i + j] = (float)v[j];
+                for (int k = 0; k < R::kPasses; ++k) raw[k][i] = *(const ju4 *)(src + k * R::kDims);
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[s][i]) & 0x7fffffffu);
-        }
-        top = max(top, __float_as_uint(swap32(__uint_as_float(top))));
-        bad = top >= 0x7f800000u;
-        const int e = P == 2 && !bad ? max((int)(top >> 23), 1) - 127 - 14 : 0;
-        if constexpr (P == 2) cs = ldexpf(a.scale2, e);
-        cs = fmaxf(cs, 1e-37f);
+            for (int k = 0; k < R::kPasses; ++k) {
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-        for (int s = 0; s < QN; ++s)
+                for (int i = 0; i < R::kTurns; ++i) *(ju4 *)(stage + R::place(r0 + i * (64u / R::kPieces), piece)) = raw[k][i];
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float y = bad ? 0.0f : P == 2 ? ldexpf(x[s][i], -e) : x[s][i];
-                q[0][s][i] = (_Float16)y;
-                if constexpr (P == 2) q[1][s][i] = (_Float16)(y - (float)q[0][s][i]);
+                for (int s = 0; s < QN / R::kPasses; ++s) {
+                    typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
+#pragma unroll
+                    for (int i = 0; i < 8; i += 16 / (int)sizeof(T)) {
+                        const vec v = *(const vec *)(stage + R::place(col, (16u * s + 8u * h + i) * sizeof(T) / 16u));
+#pragma unroll
+                        for (int j = 0; j < 16 / (int)sizeof(T); ++j) x[k * (QN / R::kPasses) + s][i + j] = (float)v[j];
+                    }
+                }
             }
-    }
-    typedef float f16v __attribute__((ext_vector_type(16)));
-    f16v o[ND];
 #pragma unroll
-    for (int d = 0; d < ND; ++d) o[d] = (f16v){};
-    // p = 2^(s cs + c2), c2 = kBias - m cs rounded (infinite while nothing was seen); where that would cost
-    // the last bits of a score (far) the difference to m is taken first
-    float m = -INFINITY, c2 = INFINITY, l = 0.0f;
-    uint32_t far = 0;   // uniform
-    const uint32_t kat = lane * 16u;
-    uint32_t vat[2];   // of even and odd blocks of dims: the slots are permuted by (dim / 8) % 8
+            for (int s = 0; s < QN; ++s)
 #pragma unroll
-    for (int d = 0; d < 2; ++d) vat[d] = (((col >> 3) * 8u + ((col & 7u) ^ ((4u * d + (col >> 3)) & 7u))) + 32u * h) * 16u;
-    uint32_t b = 0;
-    if (p0 < p1) {
-        store(0);
-        load(min(p0 + TP, last_tile));
-    }
-    for (uint32_t p = p0; p < p1; p += TP, b ^= 1u) {
-        __syncthreads();   // this tile is there, the other buffer has been read
-        if (p + TP < p1) {
-            store(b ^ 1u);
-            // past the end the last tile again: under a condition the compiler would wait for these loads at once
-            load(min(p + 2 * TP, last_tile));
+                for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[s][i]) & 0x7fffffffu);
+            top = max(top, __float_as_uint(swap32(__uint_as_float(top))));
+            bad = top >= 0x7f800000u;
+            const int e = P == 2 && !bad ? max((int)(top >> 23), 1) - 127 - 14 : 0;
+            if constexpr (P == 2) cs = ldexpf(a.scale2, e);
+            cs = fmaxf(cs, 1e-37f);
+#pragma unroll
+            for (int s = 0; s < QN; ++s)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float y = bad ? 0.0f : P == 2 ? ldexpf(x[s][i], -e) : x[s][i];
+                    q[0][s][i] = (_Float16)y;
+                    if constexpr (P == 2) q[1][s][i] = (_Float16)(y - (float)q[0][s][i]);
+                }
         }
-        if (p >= wave_hi) continue;
-        const uint8_t *kt = smem + b * 2 * kTile, *vt = kt + kTile;
-        f16v s[NB];
-        fh8 k[NB][QN];
+        typedef float f16v __attribute__((ext_vector_type(16)));
+        f16v o[ND];
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
+        for (int d = 0; d < ND; ++d) o[d] = (f16v){};
+        // p = 2^(s cs + c2), c2 = kBias - m cs rounded (infinite while nothing was seen); where that would cost
+        // the last bits of a score (far) the difference to m is taken first
+        float m = -INFINITY, c2 = INFINITY, l = 0.0f;
+        uint32_t far = 0;   // uniform
+        const uint32_t kat = lane * 16u;
+        uint32_t vat[2];   // of even and odd blocks of dims: the slots are permuted by (dim / 8) % 8
 #pragma unroll
-            for (int t = 0; t < QN; ++t) k[n][t] = *(const fh8 *)(kt + kat + (n * QN + t) * 1024u);
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            s[n] = (f16v){};
-            if constexpr (P == 2)   // the small parts first
-#pragma unroll
-                for (int t = 0; t < QN; ++t) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[n][t], q[1][t], s[n], 0, 0, 0);
-#pragma unroll
-            for (int t = 0; t < QN; ++t) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[n][t], q[0][t], s[n], 0, 0, 0);
+        for (int d = 0; d < 2; ++d) vat[d] = (((col >> 3) * 8u + ((col & 7u) ^ ((4u * d + (col >> 3)) & 7u))) + 32u * h) * 16u;
+        uint32_t b = 0;
+        if (p0 < p1) {
+            store(0);
+            load(min(p0 + TP, last_tile));
         }
-        // half the operands are requested together, the others one by one behind the products: left to
-        // itself the compiler waits for every two before it asks for the next
-        if constexpr (P == 1) {
-            constexpr int kAhead = NB * QN / 2;
-            __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
-#pragma unroll
-            for (int t = 0; t < NB * QN - kAhead; ++t) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        for (uint32_t p = p0; p < p1; p += TP, b ^= 1u) {
+            __syncthreads();   // this tile is there, the other buffer has been read
+            if (p + TP < p1) {
+                store(b ^ 1u);
+                // past the end the last tile again: under a condition the compiler would wait for these loads at once
+                load(min(p + 2 * TP, last_tile));
             }
-            __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
-        }
-        if (p + TP > min(wave_lo, p1)) {   // some column does not see all, or positions beyond the part are not its own
-            const uint32_t below = min(vis, p1);
+            if (p >= wave_hi) continue;
+            const uint8_t *kt = smem + b * 2 * kTile, *vt = kt + kTile;
+            f16v s[NB];
+            fh8 k[NB][QN];
 #pragma unroll
             for (int n = 0; n < NB; ++n)
 #pragma unroll
-                for (int v = 0; v < 16; ++v) s[n][v] = p + 32 * n + 8 * (v >> 2) + 4 * h + (v & 3) < below ? s[n][v] : -INFINITY;
-        }
-        float top[2] = {s[0][0], s[0][1]};
+                for (int t = 0; t < QN; ++t) k[n][t] = *(const fh8 *)(kt + kat + (n * QN + t) * 1024u);
 #pragma unroll
-        for (int x = 2; x < 16 * NB; ++x) top[x & 1] = fmaxf(top[x & 1], s[x >> 4][x & 15]);
-        float bm = fmaxf(top[0], top[1]);
-        bm = fmaxf(bm, swap32(bm));
-        if (__any(fmaf(bm, cs, c2) > kBias + kSlack)) {
-            const float now = fmaxf(m, bm), cn = now == -INFINITY ? INFINITY : fmaf(-now, cs, kBias);
-            float f;
-            if (__builtin_amdgcn_readfirstlane(far | (__any(fabsf(cn) > 4194304.0f && cn != INFINITY) ? 1u : 0u))) {
-                // from c2 as it was rounded to the difference: kBias - c2 is exact
-                const float r = far ? 0.0f : fmaf(-m, cs, kBias - c2);
-                f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(fmaf(m - now, cs, r));
-                far = 1;
-            } else {
-                f = cn == c2 ? 1.0f : __builtin_amdgcn_exp2f(cn - c2);
+            for (int n = 0; n < NB; ++n) {
+                s[n] = (f16v){};
+                if constexpr (P == 2)   // the small parts first
+#pragma unroll
+                    for (int t = 0; t < QN; ++t) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[n][t], q[1][t], s[n], 0, 0, 0);
+#pragma unroll
+                for (int t = 0; t < QN; ++t) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[n][t], q[0][t], s[n], 0, 0, 0);
             }
-            m = now;
-            c2 = cn;
-            l *= f;
+            // half the operands are requested together, the others one by one behind the products: left to
+            // itself the compiler waits for every two before it asks for the next
+            if constexpr (P == 1) {
+                constexpr int kAhead = NB * QN / 2;
+                __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+                for (int t = 0; t < NB * QN - kAhead; ++t) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
+            }
+            if (p + TP > min(wave_lo, p1)) {   // some column does not see all, or positions beyond the part are not its own
+                const uint32_t below = min(vis, p1);
+#pragma unroll
+                for (int n = 0; n < NB; ++n)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) s[n][v] = p + 32 * n + 8 * (v >> 2) + 4 * h + (v & 3) < below ? s[n][v] : -INFINITY;
+            }
+            float top[2] = {s[0][0], s[0][1]};
+#pragma unroll
+            for (int x = 2; x < 16 * NB; ++x) top[x & 1] = fmaxf(top[x & 1], s[x >> 4][x & 15]);
+            float bm = fmaxf(top[0], top[1]);
+            bm = fmaxf(bm, swap32(bm));
+            if (__any(fmaf(bm, cs, c2) > kBias + kSlack)) {
+                const float now = fmaxf(m, bm), cn = now == -INFINITY ? INFINITY : fmaf(-now, cs, kBias);
+                float f;
+                if (__builtin_amdgcn_readfirstlane(far | (__any(fabsf(cn) > 4194304.0f && cn != INFINITY) ? 1u : 0u))) {
+                    // from c2 as it was rounded to the difference: kBias - c2 is exact
+                    const float r = far ? 0.0f : fmaf(-m, cs, kBias - c2);
+                    f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(fmaf(m - now, cs, r));
+                    far = 1;
+                } else {
+                    f = cn == c2 ? 1.0f : __builtin_amdgcn_exp2f(cn - c2);
+                }
+                m = now;
+                c2 = cn;
+                l *= f;
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) o[d][v] *= f;
+            }
+            float off = c2 == INFINITY ? 0.0f : c2;
+            if (__builtin_amdgcn_readfirstlane(far)) {
+                const float m0 = m == -INFINITY ? 0.0f : m;
+                off = kBias;
+#pragma unroll
+                for (int n = 0; n < NB; ++n)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) s[n][v] -= m0;
+            }
+            float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int t = 0; t < 2 * NB; ++t) {
+                fh8 ph, pl;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float x = __builtin_amdgcn_exp2f(fmaf(s[t >> 1][8 * (t & 1) + e], cs, off));
+                    ph[e] = (_Float16)x;
+                    if constexpr (P == 2) {
+                        pl[e] = (_Float16)(x - (float)ph[e]);
+                        sum[e & 1] += x;
+                    }
+                }
+                if constexpr (P == 1) {   // of P as rounded: both sums see the same weights
+                    const jh2 one = {(_Float16)1.0f, (_Float16)1.0f};
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) sum[(e >> 1) & 1] = __builtin_amdgcn_fdot2(jh2{ph[e], ph[e + 1]}, one, sum[(e >> 1) & 1], false);
+                }
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    const fh8 v = *(const fh8 *)(vt + vat[d & 1] + (t * ND + d) * 1024u);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph, o[d], 0, 0, 0);
+                    if constexpr (P == 2) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl, o[d], 0, 0, 0);
+                }
+            }
+            l += sum[0] + sum[1];
+        }
+        l += swap32(l);
+        const float nan = __uint_as_float(0x7fc00000u);
+        if (p0 < p1 && __syncthreads_or(worst > 140u) && !idle) {
+            const Nans<D> at = all_nans<D>(ks, vs, srow, p0, wave_hi);
+            if (at.k < vis) l = nan;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+                if (at.v[d] < vis)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) o[d][v] = nan;
+        }
+        __syncthreads();   // the tiles have been read: the results pass through them, or the next columns' do
+        const bool there = c0 + col < columns;
+        if (bad && vis) l = nan;
+        const Fp4Args &z = late_args();
+        if (SPLIT && w.parts > 1) {
+            const size_t at = ((size_t)w.slot * z.kv_heads + kvh) * z.cols + (c - w.c0);
+            float *to = z.part + at * D;
+            if (there)
 #pragma unroll
             for (int d = 0; d < ND; ++d)
 #pragma unroll
-                for (int v = 0; v < 16; ++v) o[d][v] *= f;
-        }
-        float off = c2 == INFINITY ? 0.0f : c2;
-        if (__builtin_amdgcn_readfirstlane(far)) {
-            const float m0 = m == -INFINITY ? 0.0f : m;
-            off = kBias;
+                for (int j = 0; j < 4; ++j) *(jf4 *)(to + 32 * d + 8 * j + 4 * h) = jf4{o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]};
+            if (there && h == 0) {
+                // in powers of two, less what the rounding of c2 has moved
+                z.part_ml[2 * at] = m == -INFINITY ? m : far ? m * cs : kBias - c2;
+                z.part_ml[2 * at + 1] = l;
+            }
+        } else {
+            typedef Rows<T, D, TP> R;
+            const float inv = vis ? 1.0f / l : 0.0f;
+            uint8_t *const stage = smem + 2 * kTile + wave * (32u * R::kBytes);
+            const uint32_t lane = fresh_thread() & 63u, col = lane & 31u, h = lane >> 5, piece = lane % R::kPieces, r0 = lane / R::kPieces;
 #pragma unroll
-            for (int n = 0; n < NB; ++n)
+            for (int k = 0; k < R::kPasses; ++k) {
+                constexpr int N = ND / R::kPasses;
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-                for (int v = 0; v < 16; ++v) s[n][v] -= m0;
-        }
-        float sum[2] = {0.0f, 0.0f};
+                for (int d = 0; d < N; ++d)
 #pragma unroll
-        for (int t = 0; t < 2 * NB; ++t) {
-            fh8 ph, pl;
+                    for (int j = 0; j < 4; ++j) {
+                        typedef T t4 __attribute__((ext_vector_type(4)));
+                        t4 y;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float x = __builtin_amdgcn_exp2f(fmaf(s[t >> 1][8 * (t & 1) + e], cs, off));
-                ph[e] = (_Float16)x;
-                if constexpr (P == 2) {
-                    pl[e] = (_Float16)(x - (float)ph[e]);
-                    sum[e & 1] += x;
+                        for (int i = 0; i < 4; ++i) y[i] = vis ? (T)(o[k * N + d][4 * j + i] * inv) : (T)0.0f;
+                        const uint32_t at = (32u * d + 8u * j + 4u * h) * sizeof(T);
+                        *(t4 *)(stage + R::place(col, at / 16u) + at % 16u) = y;
+                    }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+                for (int i = 0; i < R::kTurns; ++i) {
+                    const uint32_t r = r0 + i * (64u / R::kPieces);
+                    T *to = (T *)z.out + (size_t)__shfl(qat, (int)r) * D + k * R::kDims + piece * (16 / sizeof(T));
+                    const ju4 y = *(const ju4 *)(stage + R::place(r, piece));
+                    if (c0 + r < columns) *(ju4 *)to = y;
                 }
             }
-            if constexpr (P == 1) {   // of P as rounded: both sums see the same weights
-                const jh2 one = {(_Float16)1.0f, (_Float16)1.0f};
-#pragma unroll
-                for (int e = 0; e < 8; e += 2) sum[(e >> 1) & 1] = __builtin_amdgcn_fdot2(jh2{ph[e], ph[e + 1]}, one, sum[(e >> 1) & 1], false);
-            }
-#pragma unroll
-            for (int d = 0; d < ND; ++d) {
-                const fh8 v = *(const fh8 *)(vt + vat[d & 1] + (t * ND + d) * 1024u);
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph, o[d], 0, 0, 0);
-                if constexpr (P == 2) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl, o[d], 0, 0, 0);
-            }
         }
-        l += sum[0] + sum[1];
-    }
-    l += swap32(l);
-    const float nan = __uint_as_float(0x7fc00000u);
-    if (p0 < p1 && __syncthreads_or(worst > 140u) && !idle) {
-        const Nans<D> at = all_nans<D>(ks, vs, srow, p0, wave_hi);
-        if (at.k < vis) l = nan;
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-            if (at.v[d] < vis)
-#pragma unroll
-                for (int v = 0; v < 16; ++v) o[d][v] = nan;
-    }
-    if constexpr (SPLIT) __syncthreads();   // the tiles are written again for the next columns
-    if (c0 + col >= columns) {
-        if constexpr (SPLIT) continue;
-        else return;
-    }
-    if (bad && vis) l = nan;
-    const Fp4Args &z = late_args();
-    if (SPLIT && w.parts > 1) {
-        const size_t at = ((size_t)w.slot * z.kv_heads + kvh) * z.cols + (c - w.c0);
-        float *to = z.part + at * D;
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) *(jf4 *)(to + 32 * d + 8 * j + 4 * h) = jf4{o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]};
-        if (h == 0) {
-            // in powers of two, less what the rounding of c2 has moved
-            z.part_ml[2 * at] = m == -INFINITY ? m : far ? m * cs : kBias - c2;
-            z.part_ml[2 * at + 1] = l;
+        if (SPLIT && there && w.slot == w.first_slot && kvh == 0 && h == 0) {
+            uint32_t *to = z.meta + 2 * ((size_t)w.s.row0 * z.G + c);
+            to[0] = w.first_slot;
+            to[1] = w.parts | (vis ? 0u : 1u << 23) | (c - w.c0) << 24;
         }
-    } else {
-        const float inv = vis ? 1.0f / l : 0.0f;
-        T *to = (T *)z.out + qat * D;
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                typedef T t4 __attribute__((ext_vector_type(4)));
-                t4 y;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) y[i] = vis ? (T)(o[d][4 * j + i] * inv) : (T)0.0f;
-                *(t4 *)(to + 32 * d + 8 * j + 4 * h) = y;
-            }
-    }
-    if (SPLIT && w.slot == w.first_slot && kvh == 0 && h == 0) {
-        uint32_t *to = z.meta + 2 * ((size_t)w.s.row0 * z.G + c);
-        to[0] = w.first_slot;
-        to[1] = w.parts | (vis ? 0u : 1u << 23) | (c - w.c0) << 24;
-    }
     }
 }
 
@@ -1211,17 +1237,16 @@ int reserve(janus_ctx *ctx, Fp4Args &a, uint32_t D) {
 }
 
 template <typename T, int D, int NT, int NW, int PER> int launch_few(janus_ctx *ctx, Fp4Args &a, uint32_t max_len) {
-    constexpr int S = 1;
     uint32_t hw = NW;
     while (a.kv_heads % hw) hw /= 2;
     const uint32_t ph = NW / hw;
     // two tiles, or the phases' results
-    const uint32_t lds = std::max<uint32_t>(Tile<D, S, NW>::kLds, (ph - 1) * hw * NT * (D / 4 + 2) * 256u);
-    plan(ctx, a, 16 * NT, hw, ph, 32 * S * ph, std::min<uint32_t>(PER * 4 / NW, 160 * 1024 / lds), max_len);
+    const uint32_t lds = std::max<uint32_t>(Tile<D, NW>::kLds, (ph - 1) * hw * NT * (D / 4 + 2) * 256u);
+    plan(ctx, a, 16 * NT, hw, ph, 32 * ph, std::min<uint32_t>(PER * 4 / NW, 160 * 1024 / lds), max_len);
     if (int e = reserve(ctx, a, D)) return e;
     const dim3 grid((a.shares + 7) / 8 * 8 * a.head_groups), block(NW * 64);
-    if (a.target) return launch_lds(ctx, fp4_attn_kernel<T, D, NT, S, NW, PER, true>, grid, block, lds, a);
-    return launch_lds(ctx, fp4_attn_kernel<T, D, NT, S, NW, PER, false>, grid, block, lds, a);
+    if (a.target) return launch_lds(ctx, fp4_attn_kernel<T, D, NT, NW, PER, true>, grid, block, lds, a);
+    return launch_lds(ctx, fp4_attn_kernel<T, D, NT, NW, PER, false>, grid, block, lds, a);
 }
 
 template <typename T, int D> int launch_wide(janus_ctx *ctx, Fp4Args &a, uint32_t max_len) {
