@@ -3,7 +3,7 @@
 //
 // The queries of a KV head that read the same K and V are columns of one matrix
 // product: column c of a sequence of n rows is query head c % G of its row c / G (G
-// heads per KV head). A wavefront takes NT tiles of 16 columns and positions 32 at a
+// heads per KV head). A wavefront takes a tile of 16 columns and positions 32 at a
 // time, and keeps the running maximum m, the sum l and the output O^T in registers:
 //   S^T = K Q^T (positions x columns), p = 2^(scale log2(e) s - m + bias),
 //   l <- l 2^(m_old - m) + sum p,  O^T <- O^T 2^(m_old - m) + V^T P^T.
@@ -142,6 +142,7 @@ struct Task {
     uint32_t from, to;
     uint32_t slot, first_slot, parts;   // its place among the parts of these columns; 1 part: the result
     bool more;                          // whether the share goes on behind them
+    uint32_t quota, s0, start, before;  // split: units of a share; the sequences looked at, units and tiles before them
 };
 
 // The work of share `share` that starts `done` units into it; false if there is none.
@@ -155,25 +156,34 @@ struct Task {
 template <bool SPLIT> __device__ __forceinline__ bool find_task(const Fp4Args &a, uint32_t share, uint32_t &done, Task &w) {
     const uint32_t lane = threadIdx.x & 63u, shift = 31u - (uint32_t)__builtin_clz(a.cols);   // cols is a power of two
     const uint32_t unit = SPLIT ? 31u - (uint32_t)__builtin_clz(a.step) : 0u;                 // and so is step
-    SeqRows q = seq_rows(a, lane);
+    SeqRows q;
     // the host has seen to it that all units together are below 2^31
     auto tiles_of = [&]() { return (q.n * a.G + a.cols - 1) >> shift; };
     auto units_of = [&]() { return SPLIT ? max(1u, (q.avail + a.step - 1) >> unit) : 1u; };
-    uint32_t quota = 1;
-    if constexpr (SPLIT) {
-        uint32_t total = 0;
-        for (uint32_t s0 = 0;;) {
-            total += lane_value(scan_dpp(tiles_of() * units_of()), 63);
-            if ((s0 += 64) >= a.nseq) break;
-            q = seq_rows(a, s0 + lane);
+    uint32_t quota = 1, s0 = 0, start = 0, before = 0;   // units and tiles before the sequences from s0 on
+    if (!SPLIT || done == 0) {
+        q = seq_rows(a, lane);
+        if constexpr (SPLIT) {
+            uint32_t total = tiles_of() * units_of();
+#pragma unroll 4
+            for (uint32_t s = 64; s < a.nseq; s += 64) {
+                q = seq_rows(a, s + lane);
+                total += tiles_of() * units_of();
+            }
+            total = lane_value(scan_dpp(total), 63);
+            w.quota = max((total + a.target - 1) / a.target, a.least);
+            if (a.nseq > 64) q = seq_rows(a, lane);
         }
-        if (a.nseq > 64) q = seq_rows(a, lane);
-        quota = max((total + a.target - 1) / a.target, a.least);
-        if (done >= quota) return false;
+    } else {
+        s0 = w.s0;
+        start = w.start;
+        before = w.before;
+        q = seq_rows(a, s0 + lane);
     }
-    uint32_t at = share * quota + done, start = 0, before = 0;   // units from the first tile on; units and tiles before these sequences
-    if (SPLIT && (uint64_t)share * quota + done >= 0x80000000u) return false;
-    for (uint32_t s0 = 0;;) {
+    if constexpr (SPLIT) quota = w.quota;
+    if (SPLIT && (done >= quota || (uint64_t)share * quota + done >= 0x80000000u)) return false;
+    const uint32_t at = share * quota + done;   // units from the first tile on
+    for (;;) {
         const uint32_t tiles = tiles_of(), per = units_of();
         const uint32_t upto = start + scan_dpp(tiles * per), upto_tiles = SPLIT ? scan_dpp(tiles) : 0u;
         const uint64_t here = __ballot(at < upto);
@@ -204,6 +214,9 @@ template <bool SPLIT> __device__ __forceinline__ bool find_task(const Fp4Args &a
             w.slot = share + number;
             w.first_slot = s_first + number;
             done += n;
+            w.s0 = s0;
+            w.start = start;
+            w.before = before;
             w.more = done < quota;
             return w.parts == 1 || w.slot < a.slots;   // more tiles than there can be: sequences that overlap
         }
@@ -293,81 +306,78 @@ __device__ __forceinline__ uint32_t half_pair(float a, float b) {
 __device__ __forceinline__ ff4 mfma(fh8 a, fh8 b, ff4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
 // Columns of a wavefront.
-template <typename T, int D, int NT> struct Columns {
+template <typename T, int D> struct Columns {
     static constexpr int P = sizeof(T) == 4 ? 2 : 1;   // binary16 parts of q and of P
     // The maximum may grow by kSlack powers of two before anything is rescaled; p, up to
     // 2^(kBias + kSlack), stays finite in binary16, and small ones normal (in two parts the
     // second is off by 2^-25 of 2^kBias).
     static constexpr float kBias = P == 2 ? 13.0f : 7.0f, kSlack = P == 2 ? 2.0f : 8.0f;
-    fh8 q[NT][P][D / 32];
-    float cs[NT];                   // factor from s to the exponent
-    float m[NT], l[NT];
-    ff4 o[NT][D / 16];
-    uint32_t vis[NT];               // positions that the lane's column sees
-    uint32_t bad;                   // bit t: column of tile t has an infinity or NaN in q
+    fh8 q[P][D / 32];
+    float cs;                       // factor from s to the exponent
+    float m, l;
+    ff4 o[D / 16];
+    uint32_t vis;                   // positions that the lane's column sees
+    bool bad;                       // the column has an infinity or NaN in q
 
     __device__ __forceinline__ void load(const Fp4Args &a, const Task &w, uint32_t lane, uint32_t c0, uint32_t kvh) {
         const uint32_t g = lane >> 4;
-        bad = 0;
+        bad = false;
+        const uint32_t c = c0 + (lane & 15u), row = c / a.G;   // below 2^25
+        const bool there = row < w.s.n;
+        vis = 0;
+        float x[D / 4];
+        uint32_t top = 0;
+        if (there) {
+            vis = seen_of(w.s, row);
+            const T *src = (const T *)a.q + ((size_t)(w.s.row0 + row) * a.heads + (size_t)kvh * a.G + (c - row * a.G)) * D + g * (D / 4);
+            typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const uint32_t c = c0 + t * 16u + (lane & 15u), row = c / a.G;   // below 2^25
-            const bool there = row < w.s.n;
-            vis[t] = 0;
-            float x[D / 4];
-            uint32_t top = 0;
-            if (there) {
-                vis[t] = seen_of(w.s, row);
-                const T *src = (const T *)a.q + ((size_t)(w.s.row0 + row) * a.heads + (size_t)kvh * a.G + (c - row * a.G)) * D + g * (D / 4);
-                typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
+            for (int i = 0; i < D / 4; i += 16 / (int)sizeof(T)) {
+                const vec v = *(const vec *)(src + i);
 #pragma unroll
-                for (int i = 0; i < D / 4; i += 16 / (int)sizeof(T)) {
-                    const vec v = *(const vec *)(src + i);
-#pragma unroll
-                    for (int j = 0; j < 16 / (int)sizeof(T); ++j) x[i + j] = (float)v[j];
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < D / 4; ++i) x[i] = 0.0f;
+                for (int j = 0; j < 16 / (int)sizeof(T); ++j) x[i + j] = (float)v[j];
             }
+        } else {
 #pragma unroll
-            for (int i = 0; i < D / 4; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-            top = groups_umax(top);
-            if (top >= 0x7f800000u) {
-                bad |= 1u << t;
-                top = 0;
-#pragma unroll
-                for (int i = 0; i < D / 4; ++i) x[i] = 0.0f;
-            }
-            if constexpr (P == 1) {
-                cs[t] = a.scale2;
-#pragma unroll
-                for (int i = 0; i < D / 32; ++i)
-                    q[t][0][i] = h8(half_pair(x[8 * i], x[8 * i + 1]), half_pair(x[8 * i + 2], x[8 * i + 3]),
-                                    half_pair(x[8 * i + 4], x[8 * i + 5]), half_pair(x[8 * i + 6], x[8 * i + 7]));
-            } else {
-                // the column's largest into [2^14, 2^15): the second part of what is 2^-17 of it is subnormal, off by 2^-39 of it
-                const int e = max((int)(top >> 23), 1) - 127 - 14;
-                cs[t] = ldexpf(a.scale2, e);
-#pragma unroll
-                for (int i = 0; i < D / 32; ++i) {
-                    fh8 hi, lo;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float y = ldexpf(x[8 * i + j], -e);
-                        hi[j] = (_Float16)y;
-                        lo[j] = (_Float16)(y - (float)hi[j]);
-                    }
-                    q[t][0][i] = hi;
-                    q[t][1][i] = lo;
-                }
-            }
-            cs[t] = fmaxf(cs[t], 1e-37f);   // not 0: it also multiplies -infinity
-            m[t] = -INFINITY;
-            l[t] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) o[t][i] = ff4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int i = 0; i < D / 4; ++i) x[i] = 0.0f;
         }
+#pragma unroll
+        for (int i = 0; i < D / 4; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+        top = groups_umax(top);
+        if (top >= 0x7f800000u) {
+            bad = true;
+            top = 0;
+#pragma unroll
+            for (int i = 0; i < D / 4; ++i) x[i] = 0.0f;
+        }
+        if constexpr (P == 1) {
+            cs = a.scale2;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i)
+                q[0][i] = h8(half_pair(x[8 * i], x[8 * i + 1]), half_pair(x[8 * i + 2], x[8 * i + 3]),
+                                half_pair(x[8 * i + 4], x[8 * i + 5]), half_pair(x[8 * i + 6], x[8 * i + 7]));
+        } else {
+            // the column's largest into [2^14, 2^15): the second part of what is 2^-17 of it is subnormal, off by 2^-39 of it
+            const int e = max((int)(top >> 23), 1) - 127 - 14;
+            cs = ldexpf(a.scale2, e);
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) {
+                fh8 hi, lo;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float y = ldexpf(x[8 * i + j], -e);
+                    hi[j] = (_Float16)y;
+                    lo[j] = (_Float16)(y - (float)hi[j]);
+                }
+                q[0][i] = hi;
+                q[1][i] = lo;
+            }
+        }
+        cs = fmaxf(cs, 1e-37f);   // not 0: it also multiplies -infinity
+        m = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) o[i] = ff4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
     // 32 positions from p on. masked: some column of the wavefront does not see all of
@@ -383,65 +393,47 @@ template <typename T, int D, int NT> struct Columns {
         }
         const uint32_t kshift = g * (D / 4) / 32 * 8;   // the lane's block of K, and of V
         const uint32_t vblock = (lane & 15u) * (D / 16) / 32, vmask = 0xffu << (8u * vblock), vturn = (8u * vblock - 23u) & 31u;
-        ff4 s[NT][2];
+        ff4 s[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const float sc = __uint_as_float((r.ks[h] >> kshift & 0xffu) << 23);
-            ff4 small[P == 2 ? NT : 1];
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                s[t][h] = ff4{0.0f, 0.0f, 0.0f, 0.0f};
-                if constexpr (P == 2) small[t] = s[t][h];
-            }
+            ff4 small = {};
+            s[h] = ff4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) {
                 const uint32_t w = r.k[h][i];
                 const fh8 k = h8(fp4_pair<0>(w, sc), fp4_pair<1>(w, sc), fp4_pair<2>(w, sc), fp4_pair<3>(w, sc));
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    if constexpr (P == 2) small[t] = mfma(k, q[t][1][i], small[t]);
-                    s[t][h] = mfma(k, q[t][0][i], s[t][h]);
-                }
+                if constexpr (P == 2) small = mfma(k, q[1][i], small);
+                s[h] = mfma(k, q[0][i], s[h]);
             }
-            if constexpr (P == 2)
-#pragma unroll
-                for (int t = 0; t < NT; ++t) s[t][h] += small[t];
+            if constexpr (P == 2) s[h] += small;
         }
         if (masked) {
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) s[t][h][j] = p + 16u * h + 4u * g + j < vis[t] ? s[t][h][j] : -INFINITY;
+                for (int j = 0; j < 4; ++j) s[h][j] = p + 16u * h + 4u * g + j < vis ? s[h][j] : -INFINITY;
         }
-        float m0[NT];
+        float mx = s[0][0];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            float mx = s[t][0][0];
+        for (int j = 1; j < 8; ++j) mx = fmaxf(mx, s[j >> 2][j & 3]);
+        mx = groups_max(mx);
+        if (__any((mx - m) * cs > kSlack)) {
+            const float now = fmaxf(m, mx);
+            const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - now) * cs);
+            l *= f;
 #pragma unroll
-            for (int j = 1; j < 8; ++j) mx = fmaxf(mx, s[t][j >> 2][j & 3]);
-            mx = groups_max(mx);
-            if (__any((mx - m[t]) * cs[t] > kSlack)) {
-                const float now = fmaxf(m[t], mx);
-                const float f = m[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[t] - now) * cs[t]);
-                l[t] *= f;
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i) o[t][i] *= f;
-                m[t] = now;
-            }
-            m0[t] = m[t] == -INFINITY ? 0.0f : m[t];
+            for (int i = 0; i < D / 16; ++i) o[i] *= f;
+            m = now;
         }
-        fh8 pp[NT][P];
+        const float m0 = m == -INFINITY ? 0.0f : m;
+        fh8 pp[P];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float x = __builtin_amdgcn_exp2f(fmaf(s[t][j >> 2][j & 3] - m0[t], cs[t], kBias));   // large scores keep their last bits
-                l[t] += x;
-                pp[t][0][j] = (_Float16)x;
-                if constexpr (P == 2) pp[t][1][j] = (_Float16)(x - (float)pp[t][0][j]);
-            }
+        for (int j = 0; j < 8; ++j) {
+            const float x = __builtin_amdgcn_exp2f(fmaf(s[j >> 2][j & 3] - m0, cs, kBias));   // large scores keep their last bits
+            l += x;
+            pp[0][j] = (_Float16)x;
+            if constexpr (P == 2) pp[1][j] = (_Float16)(x - (float)pp[0][j]);
         }
         // the byte of position j, which lane j of the 16 holds, at the exponent's place
         float sc[8];
@@ -472,12 +464,10 @@ template <typename T, int D, int NT> struct Columns {
             }
             const fh8 v0 = h8(lo[0], lo[1], lo[2], lo[3]), v1 = h8(hi[0], hi[1], hi[2], hi[3]);
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int w = 0; w < P; ++w) {
-                    o[t][2 * B] = mfma(v0, pp[t][w], o[t][2 * B]);
-                    o[t][2 * B + 1] = mfma(v1, pp[t][w], o[t][2 * B + 1]);
-                }
+            for (int w = 0; w < P; ++w) {
+                o[2 * B] = mfma(v0, pp[w], o[2 * B]);
+                o[2 * B + 1] = mfma(v1, pp[w], o[2 * B + 1]);
+            }
         };
         two(std::integral_constant<int, 0>{});
         two(std::integral_constant<int, 1>{});
@@ -514,9 +504,9 @@ __device__ __forceinline__ uint2 first_nans(const uint8_t *ks, const uint8_t *vs
     return at;
 }
 
-// Up to 16 NT columns of a sequence and positions [from, to): the NW wavefronts of a
+// Up to 16 columns of a sequence and positions [from, to): the NW wavefronts of a
 // workgroup take hw KV heads and ph phases of 32 positions each; PER of them share a SIMD.
-template <typename T, int D, int NT, int NW, int PER, bool SPLIT>
+template <typename T, int D, int NW, int PER, bool SPLIT>
 __global__ __launch_bounds__(NW * 64, PER) void fp4_attn_kernel(Fp4Args args) {
     constexpr uint32_t DL = D / 4;   // output dims of a lane
     extern __shared__ __align__(16) uint8_t smem[];   // two tiles, then the phases' results
@@ -536,7 +526,7 @@ __global__ __launch_bounds__(NW * 64, PER) void fp4_attn_kernel(Fp4Args args) {
         const uint32_t c0 = w.c0, columns = w.s.n * a.G;   // below 2^25
 
         // positions that columns of the tile see: the last ones the most
-        const uint32_t most = seen_of(w.s, (min(c0 + 16u * NT, columns) - 1) / a.G), fewest = seen_of(w.s, c0 / a.G);
+        const uint32_t most = seen_of(w.s, (min(c0 + 16u, columns) - 1) / a.G), fewest = seen_of(w.s, c0 / a.G);
         const uint32_t end = __builtin_amdgcn_readfirstlane(min(most, w.to)), from = __builtin_amdgcn_readfirstlane(w.from), step = 32u * a.ph;
         const size_t base = w.s.base;
         const uint32_t rows = a.cache_rows - w.s.base;   // of the cache from position 0 on
@@ -573,7 +563,7 @@ __global__ __launch_bounds__(NW * 64, PER) void fp4_attn_kernel(Fp4Args args) {
             vs0 = *(const word *)(tile.vs + (size_t)q * tile.srow + vso);
         };
         if (from < end) fetch(from, 0);
-        Columns<T, D, NT> col;
+        Columns<T, D> col;
         col.load(a, w, lane, c0, kvh);
         if (from < end) {
             bool odd = false;
@@ -613,56 +603,42 @@ __global__ __launch_bounds__(NW * 64, PER) void fp4_attn_kernel(Fp4Args args) {
             if (odd) {
                 const uint2 at = first_nans<D>(tile.ks, tile.vs, tile.srow, from + 32u * phase, end, step);
                 const float nan = __uint_as_float(0x7fc00000u);
+                if (at.x < col.vis) col.l = nan;
+                if (at.y < col.vis)
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    if (at.x < col.vis[t]) col.l[t] = nan;
-                    if (at.y < col.vis[t])
-#pragma unroll
-                        for (int i = 0; i < D / 16; ++i) col.o[t][i] = ff4{nan, nan, nan, nan};
-                }
+                    for (int i = 0; i < D / 16; ++i) col.o[i] = ff4{nan, nan, nan, nan};
             }
         }
 
         if (SPLIT || a.ph > 1) __syncthreads();   // the tiles have been read
         // the phases of a head and column tile join in its first one
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            col.l[t] = groups_sum(col.l[t]);
-            col.m[t] = col.m[t] == -INFINITY ? col.m[t] : col.m[t] * col.cs[t];   // in powers of two from here on
-        }
+        col.l = groups_sum(col.l);
+        col.m = col.m == -INFINITY ? col.m : col.m * col.cs;   // in powers of two from here on
         if (a.ph > 1) {
-            constexpr uint32_t kArea = NT * (D / 4 + 2) * 64u;   // floats of a wavefront
+            constexpr uint32_t kArea = (D / 4 + 2) * 64u;   // floats of a wavefront
             float *mine = lds + ((phase - 1) * a.hw + hwave) * kArea;
             if (phase > 0) {
+                float *at = mine + lane;
+                at[0] = col.m;
+                at[64] = col.l;
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    float *at = mine + t * (D / 4 + 2) * 64u + lane;
-                    at[0] = col.m[t];
-                    at[64] = col.l[t];
+                for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-                    for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) at[(2 + 4 * i + r) * 64] = col.o[t][i][r];
-                }
+                    for (int r = 0; r < 4; ++r) at[(2 + 4 * i + r) * 64] = col.o[i][r];
             }
             __syncthreads();
-            if (phase == 0)
-            for (uint32_t h = 1; h < a.ph; ++h) {
-                const float *other = lds + ((h - 1) * a.hw + hwave) * kArea + lane;
+            for (uint32_t h = 1; phase == 0 && h < a.ph; ++h) {
+                const float *at = lds + ((h - 1) * a.hw + hwave) * kArea + lane;
+                const float m2 = at[0], now = fmaxf(col.m, m2);
+                const float f1 = col.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(col.m - now);
+                const float f2 = m2 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m2 - now);
+                // what has seen nothing is 0, or NaN where a block was marked
+                col.l = col.l * f1 + at[64] * f2;
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    const float *at = other + t * (D / 4 + 2) * 64u;
-                    const float m2 = at[0], now = fmaxf(col.m[t], m2);
-                    const float f1 = col.m[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(col.m[t] - now);
-                    const float f2 = m2 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m2 - now);
-                    // what has seen nothing is 0, or NaN where a block was marked
-                    col.l[t] = col.l[t] * f1 + at[64] * f2;
+                for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-                    for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) col.o[t][i][r] = col.o[t][i][r] * f1 + at[(2 + 4 * i + r) * 64] * f2;
-                    col.m[t] = now;
-                }
+                    for (int r = 0; r < 4; ++r) col.o[i][r] = col.o[i][r] * f1 + at[(2 + 4 * i + r) * 64] * f2;
+                col.m = now;
             }
             if constexpr (SPLIT) __syncthreads();   // the areas are written again for the next columns
             if (phase > 0) {
@@ -671,12 +647,10 @@ __global__ __launch_bounds__(NW * 64, PER) void fp4_attn_kernel(Fp4Args args) {
             }
         }
         const Fp4Args &z = late_args();
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const uint32_t c = c0 + t * 16u + (lane & 15u);
-            if (c >= columns) continue;
+        const uint32_t c = c0 + (lane & 15u);
+        if (c < columns) {   // no lane leaves the loop: the search for the next columns needs all
             const uint32_t r = c / z.G, gh = c % z.G;
-            if ((col.bad >> t & 1u) && col.vis[t]) col.l[t] = __uint_as_float(0x7fc00000u);
+            if (col.bad && col.vis) col.l = __uint_as_float(0x7fc00000u);
             if (SPLIT && w.parts > 1) {
                 const size_t at = ((size_t)w.slot * z.kv_heads + kvh) * z.cols + (c - w.c0);
                 float *to = z.part + at * D + g * DL;
@@ -684,13 +658,13 @@ __global__ __launch_bounds__(NW * 64, PER) void fp4_attn_kernel(Fp4Args args) {
                 for (int rr = 0; rr < 4; ++rr)
 #pragma unroll
                     for (int i = 0; i < D / 16; i += 4)
-                        *(ff4 *)(to + rr * (D / 16) + i) = ff4{col.o[t][i][rr], col.o[t][i + 1][rr], col.o[t][i + 2][rr], col.o[t][i + 3][rr]};
+                        *(ff4 *)(to + rr * (D / 16) + i) = ff4{col.o[i][rr], col.o[i + 1][rr], col.o[i + 2][rr], col.o[i + 3][rr]};
                 if (g == 0) {
-                    z.part_ml[2 * at] = col.m[t];
-                    z.part_ml[2 * at + 1] = col.l[t];
+                    z.part_ml[2 * at] = col.m;
+                    z.part_ml[2 * at + 1] = col.l;
                 }
             } else {
-                const float inv = col.vis[t] ? 1.0f / col.l[t] : 0.0f;
+                const float inv = col.vis ? 1.0f / col.l : 0.0f;
                 T *to = (T *)z.out + ((size_t)(w.s.row0 + r) * z.heads + (size_t)kvh * z.G + gh) * D + g * DL;
 #pragma unroll
                 for (int rr = 0; rr < 4; ++rr) {
@@ -700,7 +674,7 @@ __global__ __launch_bounds__(NW * 64, PER) void fp4_attn_kernel(Fp4Args args) {
                     for (int i = 0; i < D / 16; i += N) {
                         vec v;
 #pragma unroll
-                        for (int u = 0; u < N; ++u) v[u] = col.vis[t] ? (T)(col.o[t][i + u][rr] * inv) : (T)0.0f;
+                        for (int u = 0; u < N; ++u) v[u] = col.vis ? (T)(col.o[i + u][rr] * inv) : (T)0.0f;
                         *(vec *)(to + rr * (D / 16) + i) = v;
                     }
                 }
@@ -708,7 +682,7 @@ __global__ __launch_bounds__(NW * 64, PER) void fp4_attn_kernel(Fp4Args args) {
             if (SPLIT && w.slot == w.first_slot && kvh == 0 && g == 0) {
                 uint32_t *to = z.meta + 2 * ((size_t)w.s.row0 * z.G + c);
                 to[0] = w.first_slot;
-                to[1] = w.parts | (col.vis[t] ? 0u : 1u << 23) | (c - w.c0) << 24;
+                to[1] = w.parts | (col.vis ? 0u : 1u << 23) | (c - w.c0) << 24;
             }
         }
     }
@@ -1143,11 +1117,13 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
         if (SPLIT && w.parts > 1) {
             const size_t at = ((size_t)w.slot * z.kv_heads + kvh) * z.cols + (c - w.c0);
             float *to = z.part + at * D;
-            if (there)
+            if (there) {
 #pragma unroll
-            for (int d = 0; d < ND; ++d)
+                for (int d = 0; d < ND; ++d)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) *(jf4 *)(to + 32 * d + 8 * j + 4 * h) = jf4{o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]};
+                    for (int j = 0; j < 4; ++j)
+                        *(jf4 *)(to + 32 * d + 8 * j + 4 * h) = jf4{o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]};
+            }
             if (there && h == 0) {
                 // in powers of two, less what the rounding of c2 has moved
                 z.part_ml[2 * at] = m == -INFINITY ? m : far ? m * cs : kBias - c2;
@@ -1200,8 +1176,8 @@ template <typename K> int launch_lds(janus_ctx *ctx, K kernel, dim3 grid, dim3 b
     return JANUS_OK;
 }
 
-// How a launch is cut up. cols columns a workgroup, of per_cu on a CU.
-void plan(janus_ctx *ctx, Fp4Args &a, uint32_t cols, uint32_t hw, uint32_t ph, uint32_t step, uint32_t per_cu, uint32_t max_len) {
+// How a launch is cut up. cols columns a workgroup, of per_cu on a CU; many columns are split from `fewest` steps on.
+void plan(janus_ctx *ctx, Fp4Args &a, uint32_t cols, uint32_t hw, uint32_t ph, uint32_t step, uint32_t per_cu, uint32_t fewest, uint32_t max_len) {
     a.cols = cols;
     a.hw = hw;
     a.ph = ph;
@@ -1216,8 +1192,17 @@ void plan(janus_ctx *ctx, Fp4Args &a, uint32_t cols, uint32_t hw, uint32_t ph, u
     const uint64_t busy = std::max<uint64_t>(1, std::min<uint64_t>(tiles, ((uint64_t)a.rows * a.G + cols - 1) / cols + a.nseq - 1));
     const uint64_t at_once = std::max<uint64_t>(1, (uint64_t)ctx->num_cus * per_cu / a.head_groups);
     const bool counts = tiles * (std::min(a.max_seq, a.cache_rows) / step + 1) < (1ull << 31);   // units of all tiles
-    const bool split = cols <= 32 ? max_len > 12 * step && busy < 4 * at_once
-                                  : max_len > 16 * step && 2 * busy <= at_once && 4 * mean <= max_len;
+    // A split costs a second launch and a search over the sequences for every share; without one a
+    // workgroup takes 0.7 to 1.5 us for 32 positions. Where both were measured (8 KV heads of 128
+    // dims, up to 1000 sequences of up to 4000 positions) they meet at 10 steps and 20 more for
+    // as many workgroups as run at once: decode steps of 64 sequences of up to 1600 positions take
+    // 31 us split and 77 whole, 300 of up to 400 take 45 and 37, 300 of up to 1600 83 and 114.
+    // Many columns: whole tiles leave CUs idle where there are few, but shares of equal length count
+    // positions that early rows of a prompt do not see: 512 rows behind 1500 positions 41 us split and
+    // 50 whole, 1024 behind 1024 63 and 51, and 4 x 512 behind 2000 109 and 80.
+    const uint64_t steps = max_len / step;
+    const bool split = cols <= 16 ? steps * at_once > 10 * at_once + 20 * busy && busy < 4 * at_once
+                                  : steps > fewest && 2 * busy <= at_once && 3 * mean <= max_len;
     if (counts && split) {
         a.shares = a.target = (uint32_t)at_once;
         a.slots = (uint32_t)(at_once + tiles);
@@ -1236,22 +1221,22 @@ int reserve(janus_ctx *ctx, Fp4Args &a, uint32_t D) {
     return JANUS_OK;
 }
 
-template <typename T, int D, int NT, int NW, int PER> int launch_few(janus_ctx *ctx, Fp4Args &a, uint32_t max_len) {
+template <typename T, int D, int NW, int PER> int launch_few(janus_ctx *ctx, Fp4Args &a, uint32_t max_len) {
     uint32_t hw = NW;
     while (a.kv_heads % hw) hw /= 2;
     const uint32_t ph = NW / hw;
     // two tiles, or the phases' results
-    const uint32_t lds = std::max<uint32_t>(Tile<D, NW>::kLds, (ph - 1) * hw * NT * (D / 4 + 2) * 256u);
-    plan(ctx, a, 16 * NT, hw, ph, 32 * ph, std::min<uint32_t>(PER * 4 / NW, 160 * 1024 / lds), max_len);
+    const uint32_t lds = std::max<uint32_t>(Tile<D, NW>::kLds, (ph - 1) * hw * (D / 4 + 2) * 256u);
+    plan(ctx, a, 16, hw, ph, 32 * ph, std::min<uint32_t>(PER * 4 / NW, 160 * 1024 / lds), 0, max_len);
     if (int e = reserve(ctx, a, D)) return e;
     const dim3 grid((a.shares + 7) / 8 * 8 * a.head_groups), block(NW * 64);
-    if (a.target) return launch_lds(ctx, fp4_attn_kernel<T, D, NT, NW, PER, true>, grid, block, lds, a);
-    return launch_lds(ctx, fp4_attn_kernel<T, D, NT, NW, PER, false>, grid, block, lds, a);
+    if (a.target) return launch_lds(ctx, fp4_attn_kernel<T, D, NW, PER, true>, grid, block, lds, a);
+    return launch_lds(ctx, fp4_attn_kernel<T, D, NW, PER, false>, grid, block, lds, a);
 }
 
 template <typename T, int D> int launch_wide(janus_ctx *ctx, Fp4Args &a, uint32_t max_len) {
     constexpr int TP = D == 128 && sizeof(T) == 4 ? 32 : 64;
-    plan(ctx, a, 128, 1, 1, 64, 2, max_len);
+    plan(ctx, a, 128, 1, 1, 64, 2, sizeof(T) == 4 ? 10 : 16, max_len);   // a step of two-part rows takes twice as long
     if (int e = reserve(ctx, a, D)) return e;
     const dim3 grid(a.shares * a.kv_heads), block(256);
     if (a.target) return launch_lds(ctx, fp4_wide_kernel<T, D, TP, true>, grid, block, 4 * TP * D * 2, a);
@@ -1264,8 +1249,7 @@ template <typename T, int D> int launch_dim(janus_ctx *ctx, Fp4Args &a, uint32_t
     // with two-part q of 128 dims in 160 (three of four wavefronts)
     constexpr bool kTwo = sizeof(T) == 4 && D == 128;
     int e;
-    if (columns <= 16) e = launch_few<T, D, 1, kTwo ? 4 : 8, kTwo ? 3 : 4>(ctx, a, max_len);
-    else if (columns <= 32) e = launch_few<T, D, 2, 4, D == 128 ? 2 : 3>(ctx, a, max_len);
+    if (columns <= 16) e = launch_few<T, D, kTwo ? 4 : 8, kTwo ? 3 : 4>(ctx, a, max_len);
     else e = launch_wide<T, D>(ctx, a, max_len);
     if (e || !a.target) return e;
     const uint32_t units = a.rows * a.heads;
