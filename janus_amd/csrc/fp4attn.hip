@@ -3,30 +3,36 @@
 //
 // The queries of a KV head that read the same K and V are columns of one matrix
 // product: column c of a sequence of n rows is query head c % G of its row c / G (G
-// heads per KV head). A wavefront takes a tile of 16 columns and positions 32 at a
-// time, and keeps the running maximum m, the sum l and the output O^T in registers:
+// heads per KV head). Positions go by in steps, and the running maximum m, the sum l
+// and the output O^T stay in registers:
 //   S^T = K Q^T (positions x columns), p = 2^(scale log2(e) s - m + bias),
 //   l <- l 2^(m_old - m) + sum p,  O^T <- O^T 2^(m_old - m) + V^T P^T.
 // Every 4-bit value times its power-of-two scale is a binary16 number, so K and V
-// enter the binary16 matrix unit exactly, converted in registers, two values an
-// instruction with the scale applied. Nothing goes through LDS:
-//   K: a lane's bytes of one position lie in one block of 32 dims, and the order of
-//     dims in the sum is free, so 16 (8) consecutive bytes are its operand of the
-//     D / 32 products.
-//   S -> P: the result layout of two score tiles (16 positions each) is the operand
-//     layout of 32 positions, in the order {4g .. 4g + 3, 16 + 4g .. 16 + 4g + 3} of
-//     the lane's group g = lane / 16; V takes its positions in the same order.
-//   V: lane a = lane % 16 loads dims [a D / 16, (a + 1) D / 16) of its eight positions;
-//     product i takes dim i of every lane's, after pairs of positions are put
-//     together (v_perm).
-// A lane's outputs are D / 4 consecutive dims of its column.
+// enter the binary16 matrix unit exactly, converted two values an instruction with the
+// scale applied. binary16 rows round P to binary16; binary32 rows have q, divided by a
+// power of two per column, and P in two binary16 parts (22 bits), small parts first.
 //
-// binary16 rows round P to binary16 (the weights are summed before that); binary32 rows
-// have q, divided by a power of two per column, and P in two binary16 parts (22 bits).
+// Two kernels, by the columns of a sequence and KV head:
+//   up to 16 (decode steps, a few drafted rows): bound by the read of the cache. A
+//     wavefront has one KV head and 32 positions at a time, whose 4-bit rows come into LDS
+//     as they are. A decode step of 64 sequences of up to 8000 positions, 32 heads on 8, 128
+//     dims: 63 us, 4.6 TB/s, what a large copy reaches; one sequence of 8192 positions 14 us, where
+//     the two launches and the start of each count; 16 x 5 binary32 rows behind 2500 positions of
+//     32 KV heads 36 us, 2.6 TB/s: the conversions and two-part products take as long as the reads.
+//   more (prompts): bound by the matrix unit and what feeds it. Four wavefronts of 32 columns
+//     share K and V, converted once for all of them. A prompt of 6000 rows: 307 to 320 us, 920 to
+//     960 TFLOP/s of what the causal mask leaves, where a large matrix product reaches 1184; 20
+//     prompts of 3 to 611 rows 54 us, of which the read of q and the write of the output are
+//     22: a workgroup has ten steps at most, and its start and end are not hidden.
+//     From 17 columns on that is faster than tiles of 16 columns that each read K and V (12
+//     sequences of 20 columns behind 10574 positions 39 and 45 us, 40 of 30 columns behind 600
+//     23 and 39), but for binary32 rows behind long contexts (53 and 47, 54 and 51).
+// Where the tiles are few their positions are split into shares and a third kernel joins
+// the parts: a second launch of some 5 us.
 //
-// A scale byte above 140 is a block of NaN. The loop only notes the largest byte; a
-// wavefront that met one looks its scales up again and sets what saw it: every output of
-// a column whose positions include a NaN of K, the block's dims where it is V's. A row
+// A scale byte above 140 is a block of NaN. The loops count it as a finite scale and note that
+// there was one; the scales are then looked through again and what saw such a block is set: every
+// output of a column whose positions include a NaN of K, the block's dims where it is V's. A row
 // of q with an infinity or NaN gives NaN, as its formula does.
 #include <algorithm>
 #include <cmath>
@@ -255,8 +261,8 @@ __device__ __forceinline__ void lds_request(const uint8_t *base, uint32_t off, u
 // positions four apart (V), lie in different banks.
 template <int D, int NW> struct Tile {
     static constexpr uint32_t U = D / 32, kBytes = 16u * NW * D;   // segments of a head; bytes of K
-    static constexpr int N = kBytes / (1024 * NW);                     // requests of a wavefront for K
-    static constexpr uint32_t kLds = 4 * kBytes;                       // two tiles
+    static constexpr int N = kBytes / (1024 * NW);                  // requests of a wavefront for K
+    static constexpr uint32_t kLds = 4 * kBytes;                    // two tiles
     const uint8_t *kc, *ks, *vc, *vs;   // of the workgroup's first head at position 0
     uint32_t row, srow;                 // bytes from a position to the next
     uint32_t segs, heads, fold;         // segments of a row of the tile; hw - 1; log2 of the positions in 256 bytes
@@ -305,7 +311,15 @@ __device__ __forceinline__ uint32_t half_pair(float a, float b) {
 }
 __device__ __forceinline__ ff4 mfma(fh8 a, fh8 b, ff4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
-// Columns of a wavefront.
+// Sixteen columns of a wavefront. Lane 16 g + a:
+//   K: its bytes of a position lie in one block of 32 dims, and the order of dims in the sum is
+//     free, so D / 8 consecutive bytes are its operand of the D / 32 products;
+//   S -> P: the result layout of two score tiles (16 positions each) is the operand layout of 32
+//     positions, in the order {4g .. 4g + 3, 16 + 4g .. 16 + 4g + 3}; V takes its positions in
+//     the same order;
+//   V: it reads dims [a D / 16, (a + 1) D / 16) of its eight positions; product i takes dim i of
+//     every lane's, after pairs of positions are put together (v_perm).
+// Its outputs are D / 4 consecutive dims of column a.
 template <typename T, int D> struct Columns {
     static constexpr int P = sizeof(T) == 4 ? 2 : 1;   // binary16 parts of q and of P
     // The maximum may grow by kSlack powers of two before anything is rescaled; p, up to

@@ -320,3 +320,93 @@ def test_scores_beyond_their_own_last_bits(engine, types, rows):
         want = first @ v[:seen.shape[1], 0] / first.sum(-1, keepdim=True)
         tol = 2.0 ** (-10 if types == "f16" else -20) * v.abs().max()
         check(out[r], want, tol.expand_as(want), (types, r))
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("heads,kvh,hd,n", [(16, 2, 64, 2), (17, 1, 128, 1), (32, 1, 64, 1), (32, 2, 128, 1), (33, 3, 64, 1),
+                                            (40, 8, 128, 6), (12, 3, 128, 32), (4, 1, 64, 33), (10, 5, 128, 20)])
+def test_columns_at_the_kernels_borders(engine, types, heads, kvh, hd, n):
+    """16 and 17 columns of a sequence, 32 and 33, 128 and more, behind contexts that are split and that are not."""
+    for context in (0, 77, 1400):
+        _run(engine, heads, kvh, hd, [(n, context + n), (n, n), (max(1, n - 1), context // 2 + n)], types, seed=context)
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("heads,kvh,n", [(8, 8, 1), (4, 1, 20)])
+def test_many_sequences_share_a_split_context(engine, types, heads, kvh, n):
+    """More sequences than lanes on the split path; their slots overlap, as prompts with a common beginning may."""
+    gen = torch.Generator().manual_seed(31)
+    dtype, hd, nseq, cap = TYPES[types], 128, 130, 1500
+    cache = [*random_cache(gen, 2 * cap, kvh, hd), *random_cache(gen, 2 * cap, kvh, hd)]
+    k, v = decode(*cache[:2]), decode(*cache[2:])
+    q = torch.randn(nseq * n, heads, hd, generator=gen).to(dtype)
+    base = torch.randint(0, cap, (nseq,), generator=gen).tolist()
+    lens = torch.randint(n, cap + 1, (nseq,), generator=gen).tolist()
+    lens[3], lens[70], lens[129] = 0, cap, 1
+    out = torch.empty(q.shape, dtype=dtype, device=DEV)
+    ops.fp4_attention(engine, q.to(DEV), *[c.to(DEV) for c in cache], out, nseq, cap, row_base=_i32(base), seq_lens=_i32(lens))
+    for s in (*range(0, nseq, 9), 3, 70, 129):
+        b, m = base[s], lens[s]
+        want, tol = attend(q[s * n:(s + 1) * n], k[b:b + m], v[b:b + m], [max(0, m - n + 1 + r) for r in range(n)], types == "f16", True)
+        check(out[s * n:(s + 1) * n], want, tol, (types, s, m))
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+def test_nan_blocks_of_a_split_context(engine, types):
+    """Many columns and shares: a NaN of K for the rows from it on, one of V in its dims, others as they were."""
+    heads, kvh, hd, rows, length = 8, 2, 128, 40, 2600
+    q, cache, k, v, slots, starts, cap = _case(heads, kvh, hd, [(rows, length)], TYPES[types], seed=6)
+    at = length - 11
+    cache[1][at, 0, 3] = 255
+    cache[3][1700, 1, 2] = 141
+    out = torch.empty(q.shape, dtype=q.dtype, device=DEV)
+    ops.fp4_attention(engine, q.to(DEV), *cache, out, 1, cap, seq_lens=_i32([length]))
+    got = out.float().cpu()
+    want, tol = attend(q, k[:length], v[:length], [length - rows + 1 + r for r in range(rows)], types == "f16", True)
+    nan = torch.zeros(got.shape, dtype=torch.bool)
+    nan[rows - 11:, 0:4] = True
+    nan[:, 4:8, 64:96] = True
+    assert torch.equal(got.isnan(), nan)
+    got[nan] = want[nan].float()
+    check(got, want, tol, types)
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+def test_two_contexts_at_once(engine, types):
+    """Split calls of two contexts on two streams, side by side: each has its own workspace."""
+    other = ops.ComputeEngine(0)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    cases = [_case(8, 2, 128, [(1, 3000), (1, 70)], TYPES[types], seed=41), _case(8, 8, 128, [(6, 2500)], TYPES[types], seed=42)]
+    lens = [_i32([3000, 70]), _i32([2500])]
+    try:
+        q = [c[0].to(DEV) for c in cases]
+        base = [_i32([s * c[6] for s in c[4]]) for c in cases]
+        want = [torch.empty_like(x) for x in q]
+        for i in range(2):
+            ops.fp4_attention(engine, q[i], *cases[i][1], want[i], len(lens[i]), cases[i][6], row_base=base[i], seq_lens=lens[i])
+        outs = [[torch.empty_like(x) for _ in range(8)] for x in q]
+        torch.cuda.synchronize()
+        engine.bind_stream(streams[0])
+        other.bind_stream(streams[1])
+        for t in range(8):
+            for i, e in enumerate((engine, other)):
+                ops.fp4_attention(e, q[i], *cases[i][1], outs[i][t], len(lens[i]), cases[i][6], row_base=base[i], seq_lens=lens[i])
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert all(torch.equal(o, want[i]) for o in outs[i])
+    finally:
+        engine.bind_stream(torch.cuda.default_stream())
+        other.close()
+
+
+def test_rows_of_wider_tensors(engine):
+    """Rows of larger tensors: what lies beside them stays."""
+    heads, kvh, hd = 4, 2, 64
+    q, cache, k, v, slots, starts, cap = _case(heads, kvh, hd, [(3, 90)], torch.float16, seed=17)
+    wide = torch.full((5, heads, hd), 9.0, dtype=torch.float16, device=DEV)
+    wide[1:4] = q.to(DEV)
+    out = torch.full((5, heads, hd), 3.0, dtype=torch.float16, device=DEV)
+    ops.fp4_attention(engine, wide[1:4], *cache, out[1:4], 1, cap, seq_lens=_i32([90]))
+    want, tol = attend(q, k[:90], v[:90], [88, 89, 90], True, True)
+    check(out[1:4], want, tol)
+    assert (out[[0, 4]] == 3).all()

@@ -135,3 +135,44 @@ def test_offsets_beyond_32_bits(engine):
     want = decode(*encode(x))
     assert torch.equal(ko.cpu().double(), want) and torch.equal(vo.cpu().double(), -want)
     assert not kc[:8].any() and not vs[:8].any()
+
+
+def test_captured_append_and_read(engine):
+    """A captured append and read, replayed with other rows, positions and slots, equal the eager calls."""
+    gen = torch.Generator().manual_seed(8)
+    kvh, hd, n = 4, 64, 6
+    k, v = (torch.randn(n, kvh, hd, generator=gen).half().to(DEV) for _ in range(2))
+    base, pos, at = _i32([0] * n), _i32([0] * n), _i32([0] * n)
+    caches, ko, vo = _caches(40, kvh, hd), *(torch.zeros(n, kvh, hd, device=DEV) for _ in range(2))
+
+    def step():
+        ops.kv_update_fp4(engine, k, v, *caches, 5, row_base=base, positions=pos)
+        ops.kv_read_fp4(engine, *caches, ko, vo, rows=at)
+
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        engine.bind_stream(stream)
+        try:
+            step()
+            stream.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=stream):
+                step()
+            for i in range(4):
+                k.copy_(torch.randn(n, kvh, hd, generator=gen).half())
+                v.copy_(torch.randn(n, kvh, hd, generator=gen).half())
+                slot, p = torch.randperm(8, generator=gen)[:n] * 5, torch.randint(0, 5, (n,), generator=gen)
+                base.copy_(_i32(slot.tolist()))
+                pos.copy_(_i32(p.tolist()))
+                at.copy_(_i32((slot + p).tolist()))
+                for c in caches:
+                    c.fill_(7)
+                g.replay()
+                stream.synchronize()
+                for got, x, c in ((ko, k, 0), (vo, v, 2)):
+                    codes, scales = encode(x.cpu())
+                    assert torch.equal(caches[c].cpu()[slot + p], codes) and torch.equal(caches[c + 1].cpu()[slot + p], scales), i
+                    assert torch.equal(got.cpu().double(), decode(codes, scales)), i
+                    assert (caches[c].cpu() == 7).all(-1).all(-1).sum() >= 40 - n
+        finally:
+            engine.bind_stream(torch.cuda.default_stream())
