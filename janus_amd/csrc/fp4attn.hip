@@ -445,9 +445,16 @@ template <typename T, int D> struct Columns {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const float x = __builtin_amdgcn_exp2f(fmaf(s[j >> 2][j & 3] - m0, cs, kBias));   // large scores keep their last bits
-            l += x;
             pp[0][j] = (_Float16)x;
-            if constexpr (P == 2) pp[1][j] = (_Float16)(x - (float)pp[0][j]);
+            if constexpr (P == 2) {
+                l += x;
+                pp[1][j] = (_Float16)(x - (float)pp[0][j]);
+            }
+        }
+        if constexpr (P == 1) {   // of P as rounded: both sums see the same weights
+            const jh2 one = {(_Float16)1.0f, (_Float16)1.0f};
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) l = __builtin_amdgcn_fdot2(jh2{pp[0][j], pp[0][j + 1]}, one, l, false);
         }
         // the byte of position j, which lane j of the 16 holds, at the exponent's place
         float sc[8];

@@ -410,3 +410,24 @@ def test_rows_of_wider_tensors(engine):
     want, tol = attend(q, k[:90], v[:90], [88, 89, 90], True, True)
     check(out[1:4], want, tol)
     assert (out[[0, 4]] == 3).all()
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("rows,at", [(1, 3), (1, 4990), (20, 3)])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_weights_that_are_small_in_binary16(engine, types, rows, at, hd):
+    """One position 2^22 ahead of 4999 equal ones, whose weights are subnormal in binary16: together they count, in
+    the sum as in the output. A weight is off by half of 2^-24 / 2^-15 at most, the output by that and its own rounding."""
+    dtype, n = TYPES[types], 5000
+    q = torch.zeros(rows, 1, hd, dtype=dtype)
+    q[:, 0, 0] = 22 * math.log(2)
+    kc, vc = torch.zeros(n, 1, hd // 2, dtype=torch.uint8), torch.full((n, 1, hd // 2), 0x22, dtype=torch.uint8)
+    kc[at, 0, 0], vc[at] = 0x02, 0
+    one = torch.full((n, 1, hd // 32), 127, dtype=torch.uint8)
+    for values, tol in ((vc, 2.0 ** -9), (vc ^ 0x22, 2.0 ** -11)):   # of the many, of the one: w / (1 + w) and 1 / (1 + w)
+        out = torch.empty(rows, 1, hd, dtype=dtype, device=DEV)
+        ops.fp4_attention(engine, q.to(DEV), *(x.to(DEV) for x in (kc, one, values, one)), out, 1, n, seq_lens=_i32([n]), scale=1.0)
+        for r in range(rows):
+            w = (n - rows + r) * math.exp(-float(q[r, 0, 0]))
+            want = (w if values is vc else 1.0) / (1 + w)
+            assert (out[r].double().cpu() / want - 1).abs().max() < tol, (r, out[r].flatten()[:4], want)
