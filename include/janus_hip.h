@@ -366,8 +366,8 @@ int janus_beam_select(janus_ctx *ctx, const float *logits, const float *d_scores
  * d_row_base and d_parents: [groups][beams], parents counted within the request;
  * len = d_seq_lens[i] ([groups][beams], NULL: max_seq_len), at most max_seq_len and
  * what lies inside the cache. A slot whose parent is itself, or outside [0, beams),
- * or whose row base or its parent's is negative, stays. Slots must not overlap. Forks as
- * well (all parents 0) and moves. 1 to 32 beams. */
+ * or whose row base or its parent's is negative, stays. Slots must not overlap, nor
+ * buffers. Forks as well (all parents 0) and moves. 1 to 32 beams. */
 #define JANUS_REORDER_BUFFERS 8
 int janus_kv_reorder(janus_ctx *ctx, uint32_t n_buffers, void *const *buffers, const uint64_t *row_bytes, uint32_t layers,
                      uint32_t groups, uint32_t beams, uint32_t cache_rows, uint32_t max_seq_len, const int32_t *d_row_base,

@@ -1188,10 +1188,7 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
     }
 }
 
-// A launch with more LDS than a kernel has without asking.
-template <typename K> int launch_lds(janus_ctx *ctx, K kernel, dim3 grid, dim3 block, uint32_t lds, const Fp4Args &a) {
-    if (lds > 64 * 1024)
-        JANUS_HIP_CHECK(ctx, hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+template <typename K> int launch(janus_ctx *ctx, K kernel, dim3 grid, dim3 block, uint32_t lds, const Fp4Args &a) {
     hipLaunchKernelGGL(kernel, grid, block, lds, ctx->stream, a);
     JANUS_LAUNCH_CHECK(ctx);
     return JANUS_OK;
@@ -1246,13 +1243,13 @@ template <typename T, int D, int NW, int PER> int launch_few(janus_ctx *ctx, Fp4
     uint32_t hw = NW;
     while (a.kv_heads % hw) hw /= 2;
     const uint32_t ph = NW / hw;
-    // two tiles, or the phases' results
+    // two tiles, or the phases' results: 64 KB at most
     const uint32_t lds = std::max<uint32_t>(Tile<D, NW>::kLds, (ph - 1) * hw * (D / 4 + 2) * 256u);
     plan(ctx, a, 16, hw, ph, 32 * ph, std::min<uint32_t>(PER * 4 / NW, 160 * 1024 / lds), 0, max_len);
     if (int e = reserve(ctx, a, D)) return e;
     const dim3 grid((a.shares + 7) / 8 * 8 * a.head_groups), block(NW * 64);
-    if (a.target) return launch_lds(ctx, fp4_attn_kernel<T, D, NW, PER, true>, grid, block, lds, a);
-    return launch_lds(ctx, fp4_attn_kernel<T, D, NW, PER, false>, grid, block, lds, a);
+    if (a.target) return launch(ctx, fp4_attn_kernel<T, D, NW, PER, true>, grid, block, lds, a);
+    return launch(ctx, fp4_attn_kernel<T, D, NW, PER, false>, grid, block, lds, a);
 }
 
 template <typename T, int D> int launch_wide(janus_ctx *ctx, Fp4Args &a, uint32_t max_len) {
@@ -1260,8 +1257,8 @@ template <typename T, int D> int launch_wide(janus_ctx *ctx, Fp4Args &a, uint32_
     plan(ctx, a, 128, 1, 1, 64, 2, sizeof(T) == 4 ? 10 : 16, max_len);   // a step of two-part rows takes twice as long
     if (int e = reserve(ctx, a, D)) return e;
     const dim3 grid(a.shares * a.kv_heads), block(256);
-    if (a.target) return launch_lds(ctx, fp4_wide_kernel<T, D, TP, true>, grid, block, 4 * TP * D * 2, a);
-    return launch_lds(ctx, fp4_wide_kernel<T, D, TP, false>, grid, block, 4 * TP * D * 2, a);
+    if (a.target) return launch(ctx, fp4_wide_kernel<T, D, TP, true>, grid, block, 4 * TP * D * 2, a);
+    return launch(ctx, fp4_wide_kernel<T, D, TP, false>, grid, block, 4 * TP * D * 2, a);
 }
 
 template <typename T, int D> int launch_dim(janus_ctx *ctx, Fp4Args &a, uint32_t max_len) {

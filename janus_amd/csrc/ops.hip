@@ -412,6 +412,12 @@ int janus_kv_reorder(janus_ctx *ctx, uint32_t n_buffers, void *const *buffers, c
         if (row_bytes[i] == 0 || row_bytes[i] > (1ull << 30))
             return fail(ctx, JANUS_E_INVALID_DIM, "kv_reorder: rows of 1 byte to 2^30");
     }
+    for (uint32_t i = 0; i < n_buffers; ++i)   // a byte that two of them hold would be moved twice
+        for (uint32_t j = 0; j < n_buffers; ++j) {
+            const uint64_t from = (uint64_t)(uintptr_t)buffers[i], to = (uint64_t)(uintptr_t)buffers[j];
+            if (i != j && from <= to && (to - from) / row_bytes[i] < (uint64_t)layers * cache_rows)
+                return fail(ctx, JANUS_E_INVALID_ARG, "kv_reorder: buffers overlap");
+        }
     if (!d_row_base || !d_parents) return fail(ctx, JANUS_E_INVALID_ARG, "kv_reorder: null table");
     if (beams == 0 || beams > 32) return fail(ctx, JANUS_E_INVALID_DIM, "kv_reorder: 1 to 32 beams");
     if (cache_rows > 0x80000000u) return fail(ctx, JANUS_E_INVALID_DIM, "kv_reorder: a cache beyond 2^31 rows");

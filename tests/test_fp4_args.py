@@ -9,7 +9,7 @@ from fp4_ref import decode, encode
 from test_packed_args import vctx  # noqa: F401 (fixture)
 
 F32, F16 = _lib.DT_F32, _lib.DT_F16
-P = 0x10000
+P, FAR = 0x10000, 1 << 44
 CACHE = dict(kc=P, ks=P, vc=P, vs=P)
 STORE = dict(k=P, v=P, dtype=F32, k_stride=0, v_stride=0, **CACHE, rows=4, kv_heads=2, hd=128, cache_rows=256, position=0,
              max_seq=64, base=P, pos=P)
@@ -27,7 +27,7 @@ def _call(vctx, name, good, **changed):  # noqa: F811
     return status, lib.janus_last_error(ctx).decode()
 
 
-def _reorder(vctx, buffers=(P, P), row_bytes=(256, 32), layers=2, groups=3, beams=4, cache_rows=100, max_seq=8, base=P,  # noqa: F811
+def _reorder(vctx, buffers=(P, FAR), row_bytes=(256, 32), layers=2, groups=3, beams=4, cache_rows=100, max_seq=8, base=P,  # noqa: F811
              parents=P, lens=P, **other):
     lib, ctx = vctx
     k = len(buffers)
@@ -119,6 +119,12 @@ def test_reorder_refusals(vctx):  # noqa: F811
         assert _reorder(vctx, **fine)[0] == _lib.OK, fine
     for fine in (dict(lens=None), dict(row_bytes=(1, 2 ** 30)), dict(beams=32)):
         assert _reorder(vctx, **fine)[0] == _lib.E_NO_DEVICE, fine
+    size = 2 * 100 * 256   # of the first buffer: the second may begin behind it, or end before it
+    for other in (P + size, P - 2 * 100 * 32):
+        assert _reorder(vctx, (P, other))[0] == _lib.E_NO_DEVICE
+    for other in (P, P + 1, P + size - 1, P - 2 * 100 * 32 + 1):
+        status, said = _reorder(vctx, (P, other))
+        assert status == _lib.E_INVALID_ARG and "overlap" in said, other
 
 
 @pytest.fixture()
@@ -187,13 +193,15 @@ def test_beam_tensor_checks(cpu_engine):
     k = torch.zeros(40, 2, 64, dtype=torch.float16)
     i6 = torch.arange(6, dtype=torch.int32)
 
-    def reorder(caches=(k, k), beams=3, max_seq_len=5, row_base=i6, parents=i6, **kw):
+    def reorder(caches=(k, k.clone()), beams=3, max_seq_len=5, row_base=i6, parents=i6, **kw):
         ops.kv_reorder(eng, list(caches), beams, max_seq_len, row_base, parents, **kw)
 
-    for call in (reorder, lambda: reorder((k.view(4, 10, 2, 64),) * 2, layers=4), lambda: reorder((k, k[:, 0, 0].contiguous()))):
+    for call in (reorder, lambda: reorder((k.view(4, 10, 2, 64), k.clone().view(4, 10, 2, 64)), layers=4), lambda: reorder((k, k[:, 0, 0].contiguous()))):
         with pytest.raises(ops.JanusError, match="device"):
             call()
     reorder((k[:0],))
+    with pytest.raises(ops.JanusError, match="overlap"):
+        reorder((k, k))
     for bad in (dict(caches=()), dict(caches=(k,) * 9), dict(caches=(k, k[:39])), dict(beams=0), dict(beams=4), dict(max_seq_len=-1),
                 dict(max_seq_len=2 ** 32), dict(layers=-1), dict(layers=3), dict(row_base=i6[:5]), dict(parents=i6.long()),
                 dict(seq_lens=i6[:4]), dict(caches=(k.transpose(1, 2),))):
