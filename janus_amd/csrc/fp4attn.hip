@@ -19,14 +19,14 @@
 //     dims: 63 us, 4.6 TB/s, what a large copy reaches; one sequence of 8192 positions 14 us, where
 //     the two launches and the start of each count; 16 x 5 binary32 rows behind 2500 positions of
 //     32 KV heads 36 us, 2.6 TB/s: the conversions and two-part products take as long as the reads.
-//   more (prompts): bound by the matrix unit and what feeds it. Four wavefronts of 32 columns
-//     share K and V, converted once for all of them. A prompt of 6000 rows: 307 to 320 us, 920 to
+//   more (prompts): bound by the matrix unit and what feeds it. Four wavefronts of 32 columns, or
+//     two pairs of them for up to 64, share K and V, converted once for all of them. A prompt of 6000 rows: 307 to 320 us, 920 to
 //     960 TFLOP/s of what the causal mask leaves, where a large matrix product reaches 1184; 20
 //     prompts of 3 to 611 rows 54 us, of which the read of q and the write of the output are
 //     22: a workgroup has ten steps at most, and its start and end are not hidden.
 //     From 17 columns on that is faster than tiles of 16 columns that each read K and V (12
 //     sequences of 20 columns behind 10574 positions 39 and 45 us, 40 of 30 columns behind 600
-//     23 and 39), but for binary32 rows behind long contexts (53 and 47, 54 and 51).
+//     21 and 39; binary32 rows 46 and 47, 27 and 36).
 // Where the tiles are few their positions are split into shares and a third kernel joins
 // the parts: a second launch of some 5 us.
 //
@@ -792,7 +792,7 @@ template <typename T, int D, int W> __global__ __launch_bounds__(W == 1 ? 256 : 
 
 // ---- many columns -----------------------------------------------------------------
 //
-// Four wavefronts of 32 columns share K and V: tiles of TP positions are loaded in 4 bits
+// Wavefronts of 32 columns share K and V: tiles of TP positions are loaded in 4 bits
 // into registers two tiles ahead, converted one tile ahead and written to LDS as
 // the operands of v_mfma_f32_32x32x16_f16 that they will be, 16 bytes a lane, so that every
 // wavefront reads them in a straight line.
@@ -844,9 +844,14 @@ template <typename T, int D, int TP> struct Rows {
     }
 };
 
-template <typename T, int D, int TP, bool SPLIT>
+// PH 1: four wavefronts of 32 columns. PH 2: two, with two wavefronts each, which take every
+// other 32 positions and are joined at the end: for up to 64 columns of a sequence, where two of
+// four wavefronts or more would have none (12 binary32 sequences of 40 columns behind 10574 positions 53 us,
+// 66 with PH 1; 40 binary16 ones behind 600 23 and 27; one of 20 columns 18.5 and 18).
+template <typename T, int D, int TP, int PH, bool SPLIT>
 __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
-    constexpr int P = sizeof(T) == 4 ? 2 : 1, NB = TP / 32, QN = D / 16, ND = D / 32;
+    constexpr int P = sizeof(T) == 4 ? 2 : 1, NB = TP / 32 / PH, QN = D / 16, ND = D / 32;   // NB: of a wavefront
+    constexpr uint32_t kCols = 128 / PH;
     constexpr float kBias = P == 2 ? 13.0f : 7.0f, kSlack = P == 2 ? 2.0f : 8.0f;
     constexpr uint32_t kTile = TP * D * 2u;   // bytes of a tile of K, and of V
     constexpr uint32_t kUnits = TP * D / 32;  // 16-byte pieces of K, and quads of positions x 8 dims of V
@@ -862,9 +867,10 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
         const uint32_t tid = fresh_thread(), lane = tid & 63u, col = lane & 31u, h = lane >> 5;
         const uint32_t columns = w.s.n * a.G;
         auto seen = [&](uint32_t c) { return seen_of(w.s, c / a.G); };
-        const uint32_t group_hi = seen(min(w.c0 + 127u, columns - 1));   // the last column sees most
+        const uint32_t group_hi = seen(min(w.c0 + kCols - 1, columns - 1));   // the last column sees most
         const uint32_t p0 = __builtin_amdgcn_readfirstlane(min(w.from, group_hi)), p1 = __builtin_amdgcn_readfirstlane(min(w.to, group_hi));
-        const uint32_t c0 = w.c0 + 32u * wave;
+        const uint32_t phase = PH == 1 ? 0u : wave >> 1;
+        const uint32_t c0 = w.c0 + 32u * (PH == 1 ? wave : wave & 1u);
         const bool idle = c0 >= columns;
         const uint32_t wave_lo = idle ? 0u : __builtin_amdgcn_readfirstlane(seen(c0));
         const uint32_t wave_hi = idle ? 0u : __builtin_amdgcn_readfirstlane(min(seen(min(c0 + 31u, columns - 1)), p1));
@@ -1024,8 +1030,9 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
                 // past the end the last tile again: under a condition the compiler would wait for these loads at once
                 load(min(p + 2 * TP, last_tile));
             }
-            if (p >= wave_hi) continue;
-            const uint8_t *kt = smem + b * 2 * kTile, *vt = kt + kTile;
+            const uint32_t first = p + 32u * phase;   // NB blocks of 32 positions
+            if (first >= wave_hi) continue;
+            const uint8_t *kt = smem + b * 2 * kTile + phase * (QN * 1024u), *vt = smem + b * 2 * kTile + kTile + phase * (2 * ND * 1024u);
             f16v s[NB];
             fh8 k[NB][QN];
 #pragma unroll
@@ -1053,12 +1060,12 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
                 }
                 __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
             }
-            if (p + TP > min(wave_lo, p1)) {   // some column does not see all, or positions beyond the part are not its own
+            if (first + 32u * NB > min(wave_lo, p1)) {   // some column does not see all, or positions beyond the part are not its own
                 const uint32_t below = min(vis, p1);
 #pragma unroll
                 for (int n = 0; n < NB; ++n)
 #pragma unroll
-                    for (int v = 0; v < 16; ++v) s[n][v] = p + 32 * n + 8 * (v >> 2) + 4 * h + (v & 3) < below ? s[n][v] : -INFINITY;
+                    for (int v = 0; v < 16; ++v) s[n][v] = first + 32 * n + 8 * (v >> 2) + 4 * h + (v & 3) < below ? s[n][v] : -INFINITY;
             }
             float top[2] = {s[0][0], s[0][1]};
 #pragma unroll
@@ -1121,8 +1128,35 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
             l += sum[0] + sum[1];
         }
         l += swap32(l);
+        // in powers of two from here on, less what the rounding of c2 has moved
+        m = m == -INFINITY ? m : far ? m * cs : kBias - c2;
+        const bool odd = p0 < p1 && __syncthreads_or(worst > 140u);
+        if constexpr (PH == 2) {
+            // the second phase's state goes through the first tile, its m and l through where its rows were
+            float *const state = (float *)(smem + (wave & 1u) * kTile) + lane;
+            float *const sums = (float *)(smem + 2 * kTile + (2u + (wave & 1u)) * (kTile / 2)) + lane;
+            if (phase) {
+                sums[0] = m;
+                sums[64] = l;
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) state[(16 * d + v) * 64] = o[d][v];
+            }
+            __syncthreads();
+            if (!phase) {
+                const float m2 = sums[0], now = fmaxf(m, m2);
+                const float f1 = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - now), f2 = m2 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m2 - now);
+                l = l * f1 + sums[64] * f2;
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) o[d][v] = o[d][v] * f1 + state[(16 * d + v) * 64] * f2;
+                m = now;
+            }
+        }
         const float nan = __uint_as_float(0x7fc00000u);
-        if (p0 < p1 && __syncthreads_or(worst > 140u) && !idle) {
+        if (odd && !idle) {
             const Nans<D> at = all_nans<D>(ks, vs, srow, p0, wave_hi);
             if (at.k < vis) l = nan;
 #pragma unroll
@@ -1132,7 +1166,7 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
                     for (int v = 0; v < 16; ++v) o[d][v] = nan;
         }
         __syncthreads();   // the tiles have been read: the results pass through them, or the next columns' do
-        const bool there = c0 + col < columns;
+        const bool there = phase == 0 && c0 + col < columns;
         if (bad && vis) l = nan;
         const Fp4Args &z = late_args();
         if (SPLIT && w.parts > 1) {
@@ -1146,8 +1180,7 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
                         *(jf4 *)(to + 32 * d + 8 * j + 4 * h) = jf4{o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]};
             }
             if (there && h == 0) {
-                // in powers of two, less what the rounding of c2 has moved
-                z.part_ml[2 * at] = m == -INFINITY ? m : far ? m * cs : kBias - c2;
+                z.part_ml[2 * at] = m;
                 z.part_ml[2 * at + 1] = l;
             }
         } else {
@@ -1176,7 +1209,7 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
                     const uint32_t r = r0 + i * (64u / R::kPieces);
                     T *to = (T *)z.out + (size_t)__shfl(qat, (int)r) * D + k * R::kDims + piece * (16 / sizeof(T));
                     const ju4 y = *(const ju4 *)(stage + R::place(r, piece));
-                    if (c0 + r < columns) *(ju4 *)to = y;
+                    if (phase == 0 && c0 + r < columns) *(ju4 *)to = y;
                 }
             }
         }
@@ -1252,13 +1285,13 @@ template <typename T, int D, int NW, int PER> int launch_few(janus_ctx *ctx, Fp4
     return launch(ctx, fp4_attn_kernel<T, D, NW, PER, false>, grid, block, lds, a);
 }
 
-template <typename T, int D> int launch_wide(janus_ctx *ctx, Fp4Args &a, uint32_t max_len) {
-    constexpr int TP = D == 128 && sizeof(T) == 4 ? 32 : 64;
-    plan(ctx, a, 128, 1, 1, 64, 2, sizeof(T) == 4 ? 10 : 16, max_len);   // a step of two-part rows takes twice as long
+template <typename T, int D, int PH> int launch_wide(janus_ctx *ctx, Fp4Args &a, uint32_t max_len) {
+    constexpr int TP = PH == 1 && D == 128 && sizeof(T) == 4 ? 32 : 64;
+    plan(ctx, a, 128 / PH, 1, 1, 64, 2, sizeof(T) == 4 ? 10 : 16, max_len);   // a step of two-part rows takes twice as long
     if (int e = reserve(ctx, a, D)) return e;
     const dim3 grid(a.shares * a.kv_heads), block(256);
-    if (a.target) return launch(ctx, fp4_wide_kernel<T, D, TP, true>, grid, block, 4 * TP * D * 2, a);
-    return launch(ctx, fp4_wide_kernel<T, D, TP, false>, grid, block, 4 * TP * D * 2, a);
+    if (a.target) return launch(ctx, fp4_wide_kernel<T, D, TP, PH, true>, grid, block, 4 * TP * D * 2, a);
+    return launch(ctx, fp4_wide_kernel<T, D, TP, PH, false>, grid, block, 4 * TP * D * 2, a);
 }
 
 template <typename T, int D> int launch_dim(janus_ctx *ctx, Fp4Args &a, uint32_t max_len) {
@@ -1268,7 +1301,8 @@ template <typename T, int D> int launch_dim(janus_ctx *ctx, Fp4Args &a, uint32_t
     constexpr bool kTwo = sizeof(T) == 4 && D == 128;
     int e;
     if (columns <= 16) e = launch_few<T, D, kTwo ? 4 : 8, kTwo ? 3 : 4>(ctx, a, max_len);
-    else e = launch_wide<T, D>(ctx, a, max_len);
+    else if (columns <= 64) e = launch_wide<T, D, 2>(ctx, a, max_len);
+    else e = launch_wide<T, D, 1>(ctx, a, max_len);
     if (e || !a.target) return e;
     const uint32_t units = a.rows * a.heads;
     if (a.mean_parts <= 8) hipLaunchKernelGGL((fp4_join_kernel<T, D, 1>), dim3((units + 3) / 4), dim3(256), 0, ctx->stream, a);

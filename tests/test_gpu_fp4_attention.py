@@ -298,7 +298,7 @@ def test_rows_that_see_nothing_of_a_split_context(engine, types):
 
 
 @pytest.mark.parametrize("types", sorted(TYPES))
-@pytest.mark.parametrize("rows", [3, 70])
+@pytest.mark.parametrize("rows", [3, 20, 70])
 def test_scores_beyond_their_own_last_bits(engine, types, rows):
     """Scores whose spacing is far above 1: the farthest ahead takes all weight, equal ones share it."""
     dtype = TYPES[types]
@@ -332,7 +332,7 @@ def test_columns_at_the_kernels_borders(engine, types, heads, kvh, hd, n):
 
 
 @pytest.mark.parametrize("types", sorted(TYPES))
-@pytest.mark.parametrize("heads,kvh,n", [(8, 8, 1), (4, 1, 20)])
+@pytest.mark.parametrize("heads,kvh,n", [(8, 8, 1), (4, 1, 12), (4, 1, 20)])
 def test_many_sequences_share_a_split_context(engine, types, heads, kvh, n):
     """More sequences than lanes on the split path; their slots overlap, as prompts with a common beginning may."""
     gen = torch.Generator().manual_seed(31)
@@ -352,9 +352,10 @@ def test_many_sequences_share_a_split_context(engine, types, heads, kvh, n):
 
 
 @pytest.mark.parametrize("types", sorted(TYPES))
-def test_nan_blocks_of_a_split_context(engine, types):
+@pytest.mark.parametrize("rows", [12, 40])
+def test_nan_blocks_of_a_split_context(engine, types, rows):
     """Many columns and shares: a NaN of K for the rows from it on, one of V in its dims, others as they were."""
-    heads, kvh, hd, rows, length = 8, 2, 128, 40, 2600
+    heads, kvh, hd, length = 8, 2, 128, 2600
     q, cache, k, v, slots, starts, cap = _case(heads, kvh, hd, [(rows, length)], TYPES[types], seed=6)
     at = length - 11
     cache[1][at, 0, 3] = 255
