@@ -49,7 +49,7 @@ struct Fp4Args {
     const void *q;                        // [rows][heads][D]
     const uint8_t *kc, *ks, *vc, *vs;     // [cache rows][kv_heads][D / 2] and [D / 32]
     void *out;                            // [rows][heads][D]
-    float *part, *part_ml;                // split: [slot][kv_heads][cols][D] and (m, l)
+    float *part, *part_ml;                // split: [slot][kv_heads][cols][D], and (m, factor, l, -): the maximum is 2^(m factor)
     uint32_t *meta;                       // split: [rows * G] (first slot, parts | sees nothing << 23 | column << 24)
     const int32_t *q_start, *row_base, *seq_lens;
     uint32_t rows, nseq, heads, kv_heads, G;
@@ -634,7 +634,6 @@ __global__ __launch_bounds__(NW * 64, PER) void fp4_attn_kernel(Fp4Args args) {
         if (SPLIT || a.ph > 1) __syncthreads();   // the tiles have been read
         // the phases of a head and column tile join in its first one
         col.l = groups_sum(col.l);
-        col.m = col.m == -INFINITY ? col.m : col.m * col.cs;   // in powers of two from here on
         if (a.ph > 1) {
             constexpr uint32_t kArea = (D / 4 + 2) * 64u;   // floats of a wavefront
             float *mine = lds + ((phase - 1) * a.hw + hwave) * kArea;
@@ -651,8 +650,8 @@ __global__ __launch_bounds__(NW * 64, PER) void fp4_attn_kernel(Fp4Args args) {
             for (uint32_t h = 1; phase == 0 && h < a.ph; ++h) {
                 const float *at = lds + ((h - 1) * a.hw + hwave) * kArea + lane;
                 const float m2 = at[0], now = fmaxf(col.m, m2);
-                const float f1 = col.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(col.m - now);
-                const float f2 = m2 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m2 - now);
+                const float f1 = col.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((col.m - now) * col.cs);
+                const float f2 = m2 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m2 - now) * col.cs);
                 // what has seen nothing is 0, or NaN where a block was marked
                 col.l = col.l * f1 + at[64] * f2;
 #pragma unroll
@@ -680,10 +679,7 @@ __global__ __launch_bounds__(NW * 64, PER) void fp4_attn_kernel(Fp4Args args) {
 #pragma unroll
                     for (int i = 0; i < D / 16; i += 4)
                         *(ff4 *)(to + rr * (D / 16) + i) = ff4{col.o[i][rr], col.o[i + 1][rr], col.o[i + 2][rr], col.o[i + 3][rr]};
-                if (g == 0) {
-                    z.part_ml[2 * at] = col.m;
-                    z.part_ml[2 * at + 1] = col.l;
-                }
+                if (g == 0) *(ff4 *)(z.part_ml + 4 * at) = ff4{col.m, col.cs, col.l, 0.0f};
             } else {
                 const float inv = col.vis ? 1.0f / col.l : 0.0f;
                 T *to = (T *)z.out + ((size_t)(w.s.row0 + r) * z.heads + (size_t)kvh * z.G + gh) * D + g * DL;
@@ -710,9 +706,11 @@ __global__ __launch_bounds__(NW * 64, PER) void fp4_attn_kernel(Fp4Args args) {
 }
 
 // Joins the parts of a row and head: W wavefronts take them in turn, eight at a time,
-// and are joined themselves. Workgroups of 4 units for W = 1, else of one.
+// and are joined themselves. Workgroups of 4 units for W = 1, else of one. The exponents m factor
+// are exact in binary64: in 32 bits their rounding would be that of the parts' weights.
 template <typename T, int D, int W> __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void fp4_join_kernel(Fp4Args a) {
-    __shared__ float sm[W], sl[W], so[W][D];
+    __shared__ double sm[W];
+    __shared__ float sl[W], so[W][D];
     const uint32_t lane = threadIdx.x & 63u, wave = W == 1 ? 0u : threadIdx.x >> 6;
     const uint32_t unit = __builtin_amdgcn_readfirstlane(W == 1 ? blockIdx.x * 4u + (threadIdx.x >> 6) : blockIdx.x);
     const uint32_t row = unit / a.heads, head = unit - row * a.heads;
@@ -731,32 +729,34 @@ template <typename T, int D, int W> __global__ __launch_bounds__(W == 1 ? 256 : 
     typedef float vec __attribute__((ext_vector_type(E)));
     const size_t stride = (size_t)a.kv_heads * a.cols;
     const size_t at0 = ((size_t)first * a.kv_heads + kvh) * a.cols + c;
-    float m = -INFINITY, l = 0.0f;
+    double m = -INFINITY;
+    float l = 0.0f;
     vec o = {};
     for (uint32_t i0 = wave * 8; i0 < parts; i0 += W * 8) {
-        float2 ml[8];
+        ff4 ml[8];
+        double e[8];
         vec po[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const size_t at = at0 + (size_t)min(i0 + i, parts - 1) * stride;
-            ml[i] = *(const float2 *)(a.part_ml + 2 * at);
+            ml[i] = *(const ff4 *)(a.part_ml + 4 * at);
             po[i] = *(const vec *)(a.part + at * D + lane * E);
         }
-        float now = m;
+        double now = m;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            if (i0 + i >= parts) ml[i].x = -INFINITY;
-            now = fmaxf(now, ml[i].x);
+            e[i] = i0 + i < parts ? (double)ml[i][0] * (double)ml[i][1] : -INFINITY;
+            now = fmax(now, e[i]);
         }
-        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - now);
+        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((float)(m - now));
         l *= f;
         o *= f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float fi = ml[i].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[i].x - now);
+            const float fi = e[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((float)(e[i] - now));
             // a part that has seen nothing holds zeros, or NaN where a block was marked
             if (i0 + i < parts) {
-                l += ml[i].y * fi;
+                l += ml[i][2] * fi;
                 o += po[i] * fi;
             }
         }
@@ -776,13 +776,13 @@ template <typename T, int D, int W> __global__ __launch_bounds__(W == 1 ? 256 : 
         for (int e = 0; e < E; ++e) so[wave][lane * E + e] = o[e];
         __syncthreads();
         if (threadIdx.x >= D) return;
-        float now = sm[0];
+        double now = sm[0];
 #pragma unroll
-        for (int i = 1; i < W; ++i) now = fmaxf(now, sm[i]);
+        for (int i = 1; i < W; ++i) now = fmax(now, sm[i]);
         float total = 0.0f, sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < W; ++i) {
-            const float f = sm[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm[i] - now);
+            const float f = sm[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((float)(sm[i] - now));
             total += sl[i] * f;
             sum += so[i][threadIdx.x] * f;
         }
@@ -1072,7 +1072,8 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
             for (int x = 2; x < 16 * NB; ++x) top[x & 1] = fmaxf(top[x & 1], s[x >> 4][x & 15]);
             float bm = fmaxf(top[0], top[1]);
             bm = fmaxf(bm, swap32(bm));
-            if (__any(fmaf(bm, cs, c2) > kBias + kSlack)) {
+            // far scores always enter: c2 may be rounded by more than the slack, and p would leave binary16's range
+            if (__builtin_amdgcn_readfirstlane(far | (__any(fmaf(bm, cs, c2) > kBias + kSlack) ? 1u : 0u))) {
                 const float now = fmaxf(m, bm), cn = now == -INFINITY ? INFINITY : fmaf(-now, cs, kBias);
                 float f;
                 if (__builtin_amdgcn_readfirstlane(far | (__any(fabsf(cn) > 4194304.0f && cn != INFINITY) ? 1u : 0u))) {
@@ -1128,16 +1129,20 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
             l += sum[0] + sum[1];
         }
         l += swap32(l);
-        // in powers of two from here on, less what the rounding of c2 has moved
-        m = m == -INFINITY ? m : far ? m * cs : kBias - c2;
+        // from here on the maximum is 2^(m cs), less what the rounding of c2 has moved
+        if (!far) {
+            m = m == -INFINITY ? m : kBias - c2;
+            cs = 1.0f;
+        }
         const bool odd = p0 < p1 && __syncthreads_or(worst > 140u);
         if constexpr (PH == 2) {
-            // the second phase's state goes through the first tile, its m and l through where its rows were
+            // the second phase's state goes through the first tile, its m, factor and l through where its rows were
             float *const state = (float *)(smem + (wave & 1u) * kTile) + lane;
             float *const sums = (float *)(smem + 2 * kTile + (2u + (wave & 1u)) * (kTile / 2)) + lane;
             if (phase) {
                 sums[0] = m;
-                sums[64] = l;
+                sums[64] = cs;
+                sums[128] = l;
 #pragma unroll
                 for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -1145,14 +1150,19 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
             }
             __syncthreads();
             if (!phase) {
-                const float m2 = sums[0], now = fmaxf(m, m2);
-                const float f1 = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - now), f2 = m2 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m2 - now);
-                l = l * f1 + sums[64] * f2;
+                const float m2 = sums[0], cs2 = sums[64];
+                const double e1 = (double)m * (double)cs, e2 = (double)m2 * (double)cs2;
+                const float f1 = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((float)(e1 - fmax(e1, e2)));
+                const float f2 = m2 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((float)(e2 - fmax(e1, e2)));
+                l = l * f1 + sums[128] * f2;
 #pragma unroll
                 for (int d = 0; d < ND; ++d)
 #pragma unroll
                     for (int v = 0; v < 16; ++v) o[d][v] = o[d][v] * f1 + state[(16 * d + v) * 64] * f2;
-                m = now;
+                if (e2 > e1) {
+                    m = m2;
+                    cs = cs2;
+                }
             }
         }
         const float nan = __uint_as_float(0x7fc00000u);
@@ -1179,10 +1189,7 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
                     for (int j = 0; j < 4; ++j)
                         *(jf4 *)(to + 32 * d + 8 * j + 4 * h) = jf4{o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]};
             }
-            if (there && h == 0) {
-                z.part_ml[2 * at] = m;
-                z.part_ml[2 * at + 1] = l;
-            }
+            if (there && h == 0) *(ff4 *)(z.part_ml + 4 * at) = ff4{m, cs, l, 0.0f};
         } else {
             typedef Rows<T, D, TP> R;
             const float inv = vis ? 1.0f / l : 0.0f;
@@ -1265,7 +1272,7 @@ int reserve(janus_ctx *ctx, Fp4Args &a, uint32_t D) {
     if (!a.target) return JANUS_OK;
     const size_t cells = (size_t)a.slots * a.kv_heads * a.cols;
     const size_t meta = ((size_t)a.rows * a.G * 8 + 255) / 256 * 256;
-    if (int e = ensure_attn_ws(ctx, meta + cells * (D + 2) * 4)) return e;
+    if (int e = ensure_attn_ws(ctx, meta + cells * (D + 4) * 4)) return e;
     a.meta = (uint32_t *)ctx->attn_ws;
     a.part = (float *)((char *)ctx->attn_ws + meta);
     a.part_ml = a.part + cells * D;

@@ -323,6 +323,33 @@ def test_scores_beyond_their_own_last_bits(engine, types, rows):
 
 
 @pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("rows,n,at", [(1, 200, 69), (20, 200, 69), (20, 200, 104), (40, 200, 69), (1, 8192, 6000),
+                                       (20, 6000, 4011), (40, 6000, 4011)])
+def test_a_maximum_that_rises_by_its_last_bit(engine, types, rows, n, at):
+    """Of two scores next to each other in 32 bits, near 2^31 before the scale, the later one is 16 powers of two
+    ahead. Of m = 65504 2^15 + 128 x, with this x, scale log2(e) m rounded to a multiple of 32 hides more than 14.3 of
+    them from an exponent that is taken as scale log2(e) s less that. In one step or the next, another phase, another share."""
+    dtype, x, hd = TYPES[types], 40, 128
+    q = torch.zeros(rows, 2, hd, dtype=dtype)
+    q[..., 0], q[..., 32], q[..., 64] = 65504.0, x, 1.0
+    codes, scales = torch.zeros(n, 1, hd // 2, dtype=torch.uint8), torch.full((n, 1, hd // 32), 132, dtype=torch.uint8)
+    codes[[0, at], 0, 0], codes[[0, at], 0, 16], codes[at, 0, 32] = 6, 6, 6   # 4 times the block's scale
+    scales[:, :, 0] = 140
+    cache = random_cache(torch.Generator().manual_seed(22), n, 1, hd)
+    k, v = decode(codes, scales)[:, 0], decode(*cache)[:, 0]
+    s = k @ q[0, 0].double()
+    assert s[0] == 65504 * 2.0 ** 15 + 128 * x and s[at] == s[0] + 128 and (s.float() == s).all()
+    out = torch.empty(q.shape, dtype=dtype, device=DEV)
+    ops.fp4_attention(engine, q.to(DEV), *[c.to(DEV) for c in (codes, scales, *cache)], out, 1, n, seq_lens=_i32([n]))
+    w = math.exp(-128 / math.sqrt(hd))
+    want = (v[at] + w * v[0]) / (1 + w)
+    # the output's own rounding (w v[0] alone is below 2^-14, where binary16 has steps of 2^-24), and the weights': w is
+    # below 2^-16, and its binary16 part off by 2^-11 of itself
+    tol = want.abs() * torch.finfo(dtype).eps + (v[at].abs() + v[0].abs()) * 2.0 ** -22 + (2.0 ** -25 if types == "f16" else 0)
+    check(out.flatten(0, 1), want.expand(2 * rows, hd), tol.expand(2 * rows, hd), (types, rows))
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
 @pytest.mark.parametrize("heads,kvh,hd,n", [(16, 2, 64, 2), (17, 1, 128, 1), (32, 1, 64, 1), (32, 2, 128, 1), (33, 3, 64, 1),
                                             (40, 8, 128, 6), (12, 3, 128, 32), (4, 1, 64, 33), (10, 5, 128, 20)])
 def test_columns_at_the_kernels_borders(engine, types, heads, kvh, hd, n):
