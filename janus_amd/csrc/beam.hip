@@ -4,13 +4,13 @@
 // Selection. Token t of beam b has the value v = score_b + (x_t - L_b), L_b = log sum
 // exp x; the n best of a request's beams x vocabulary are wanted, ties to the lowest
 // index. Within a beam v goes by the logit, so one pass over the logits suffices:
-//   select_part_kernel: a workgroup takes a part of a row (2048 logits a wavefront, in
+//   select_part_kernel: a workgroup takes a part of a row (1024 logits a wavefront, in
 //     registers), and keeps its maximum, its sum of exponentials and its n best logits.
 //   select_join_kernel: a workgroup per request sums the parts to L_b and takes the n
 //     best of all parts by v in binary64.
 // The n best: the lanes' best values give a lower bound, found bit by bit with ballots;
 // what is not below it, n values and a few more, is ranked by counting.
-// Bound by the read of the logits: 16 requests of 8 beams, 128256 logits each, take 29 us (20
+// Bound by the read of the logits: 16 requests of 8 beams, 128256 logits each, take 28 us (20
 // for the first kernel, 3.2 TB/s, 8 for the second), one of 4 beams 14, the two launches.
 // L_b is kept to some 1e-8 (the sums of many terms in binary64), so that beams are compared
 // by more than the last bits of binary32.
@@ -29,11 +29,12 @@
 namespace janus {
 namespace {
 
-constexpr uint32_t kPartWaves = 4;      // wavefronts of a part
-constexpr uint32_t kLaneLogits = 32;    // logits of a lane, in groups of 8
+constexpr uint32_t kPartWaves = 8;      // wavefronts of a part
+constexpr uint32_t kLaneLogits = 16;    // logits of a lane, in groups of 4: all wavefronts of a CU fit (64 registers)
 constexpr uint32_t kPart = kPartWaves * 64u * kLaneLogits;
 constexpr uint32_t kJoinWaves = 8;
 constexpr uint32_t kList = 1024;        // candidates that are ranked by counting
+constexpr uint32_t kFew = 96;           // so many, and 8 n, are ranked without a look for a better bound
 constexpr uint32_t kMostBeams = 64;
 
 // Order-preserving bits, never 0; zeros alike, NaN above all.
@@ -122,7 +123,7 @@ template <bool VEC> __global__ __launch_bounds__(kPartWaves * 64) void select_pa
     float m = v[0];
 #pragma unroll
     for (uint32_t i = 1; i < kLaneLogits; ++i) m = fmaxf(m, v[i]);
-    // Each wavefront's n / 4-th best lane: the part has n values that are not below the least of the four.
+    // Each wavefront's n / 8-th best lane: the part has n values that are not below the least of the eight.
     const uint32_t key = t0 < a.vocab ? order32(m) : 0u;
     const uint32_t ks = nth_key(key, (a.n + kPartWaves - 1) / kPartWaves);
     if (lane == 0) share[wave] = ks;
@@ -158,8 +159,9 @@ template <bool VEC> __global__ __launch_bounds__(kPartWaves * 64) void select_pa
         __syncthreads();
     };
     collect();
-    if (found > kList) {
-        // a wavefront without large values has kept the bound down: that of the n-th best lane of the best one
+    if (found > max(kFew, 8u * a.n)) {
+        // a wavefront without large values has kept the bound down, as in rows that leave some without any (3 beams of
+        // 580 logits: 34 us where up to kList were ranked, 13 now): that of the n-th best lane of the best one
         __syncthreads();
         const uint32_t kn = nth_key(key, a.n);
         if (lane == 0) share[wave] = kn;
@@ -176,6 +178,7 @@ template <bool VEC> __global__ __launch_bounds__(kPartWaves * 64) void select_pa
         for (uint32_t i = threadIdx.x; i < have; i += kPartWaves * 64u) {
             const uint64_t k = list[i];
             uint32_t rank = 0;
+#pragma unroll 8
             for (uint32_t j = 0; j < have; ++j) rank += list[j] > k ? 1u : 0u;
             if (rank < a.n) keys[rank] = k;
         }
@@ -224,16 +227,22 @@ __global__ __launch_bounds__(kJoinWaves * 64) void select_join_kernel(SelectArgs
     __shared__ uint32_t share[kJoinWaves];
     __shared__ double lse[kMostBeams], score[kMostBeams];
     __shared__ int state[kMostBeams];
-    __shared__ uint32_t found;
+    __shared__ uint32_t found, deep;
     __shared__ Cand best[kJoinWaves];
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row0 = blockIdx.x * a.beams;
     const uint32_t per_beam = a.parts * a.n, total = a.beams * per_beam;
     // the lane's first candidates are on their way while the sums are made (those of ended beams are whatever lies there)
     constexpr uint32_t kHeld = 8, kStep = kJoinWaves * 64u;
+    // Where there are more than the lanes hold, the parts' best ones come first, then the second ones and so on: what is
+    // not held is looked at only if a part's last held one is not below the bound. (8 requests of 16 beams, n 32: 26 us
+    // for this kernel when all were, 17 now; 4 of 16, n 64: 96 and 20.)
+    const uint32_t lists = a.beams * a.parts;
+    const bool many = total > kHeld * kStep;
+    auto place = [&](uint32_t c) { return many ? c % lists * a.n + c / lists : c; };
     uint64_t held[kHeld];
 #pragma unroll
-    for (uint32_t i = 0; i < kHeld; ++i) held[i] = threadIdx.x + i * kStep < total ? a.keys[(size_t)row0 * per_beam + threadIdx.x + i * kStep] : 0ull;
-    if (threadIdx.x == 0) found = 0;
+    for (uint32_t i = 0; i < kHeld; ++i) held[i] = threadIdx.x + i * kStep < total ? a.keys[(size_t)row0 * per_beam + place(threadIdx.x + i * kStep)] : 0ull;
+    if (threadIdx.x == 0) found = deep = 0;
     for (uint32_t b = wave; b < a.beams; b += kJoinWaves) {
         const float sc = a.scores ? a.scores[row0 + b] : 0.0f;
         int st = sc == -INFINITY ? BEAM_ENDED : (sc < INFINITY ? BEAM_FINE : BEAM_NAN);
@@ -273,16 +282,18 @@ __global__ __launch_bounds__(kJoinWaves * 64) void select_join_kernel(SelectArgs
         if (!key) return Cand{0, 0};
         return Cand{order64(score[b] + ((double)value32((uint32_t)(key >> 32)) - lse[b])), b * a.vocab + (uint32_t)~key};
     };
-    auto far = [&](uint32_t c) { return value_of(c, a.keys[(size_t)row0 * per_beam + c]); };   // beyond the held ones
+    auto far = [&](uint32_t c) {   // beyond the held ones
+        const uint32_t at = place(c);
+        return value_of(at, a.keys[(size_t)row0 * per_beam + at]);
+    };
     auto comes_before = [](const Cand &p, const Cand &q) { return p.hi > q.hi || (p.hi == q.hi && p.idx < q.idx); };
     Cand mine[kHeld];
     uint32_t top = 0;   // upper half of the lane's best
 #pragma unroll
     for (uint32_t i = 0; i < kHeld; ++i) {
-        mine[i] = threadIdx.x + i * kStep < total ? value_of(threadIdx.x + i * kStep, held[i]) : Cand{0, 0};
+        mine[i] = threadIdx.x + i * kStep < total ? value_of(place(threadIdx.x + i * kStep), held[i]) : Cand{0, 0};
         top = max(top, (uint32_t)(mine[i].hi >> 32));
     }
-    for (uint32_t c = threadIdx.x + kHeld * kStep; c < total; c += kStep) top = max(top, (uint32_t)(far(c).hi >> 32));
     // as in the parts: the least of the wavefronts' shares, or else the best wavefront's n-th
     const uint32_t ks = nth_key(top, (a.n + kJoinWaves - 1) / kJoinWaves);
     if (lane == 0) share[wave] = ks;
@@ -300,16 +311,24 @@ __global__ __launch_bounds__(kJoinWaves * 64) void select_join_kernel(SelectArgs
         if (top >= least) {
 #pragma unroll
             for (uint32_t i = 0; i < kHeld; ++i) take(mine[i]);
-            for (uint32_t c = threadIdx.x + kHeld * kStep; c < total; c += kStep) take(far(c));
+        }
+        if (many) {
+            const uint32_t whole = kHeld * kStep / lists;   // held of every part
+#pragma unroll
+            for (uint32_t i = 0; i < kHeld; ++i)
+                if ((uint32_t)(mine[i].hi >> 32) >= least && threadIdx.x + (i * kStep + lists) >= whole * lists) deep = 1;
+            __syncthreads();
+            if (deep)
+                for (uint32_t c = threadIdx.x + kHeld * kStep; c < total; c += kStep) take(far(c));
         }
         __syncthreads();
     };
     collect();
-    if (found > kList / 4) {
+    if (found > max(kFew, 8u * a.n)) {
         __syncthreads();
         const uint32_t kn = nth_key(top, a.n);
         if (lane == 0) share[wave] = kn;
-        if (threadIdx.x == 0) found = 0;
+        if (threadIdx.x == 0) found = deep = 0;
         __syncthreads();
 #pragma unroll
         for (uint32_t w = 0; w < kJoinWaves; ++w) least = max(least, share[w]);
@@ -327,6 +346,7 @@ __global__ __launch_bounds__(kJoinWaves * 64) void select_join_kernel(SelectArgs
         for (uint32_t i = threadIdx.x; i < have; i += kStep) {
             const Cand k = list[i];
             uint32_t rank = 0;
+#pragma unroll 8
             for (uint32_t j = 0; j < have; ++j) rank += comes_before(list[j], k) ? 1u : 0u;
             if (rank < a.n) write(rank, k);
         }

@@ -393,8 +393,8 @@ int janus_beam_select(janus_ctx *ctx, const float *logits, const float *d_scores
     if (n == 0 || n > 64 || n > (uint64_t)beams * vocab)
         return fail(ctx, JANUS_E_INVALID_DIM, "beam_select: n must be 1 to 64, at most beams * vocab");
     if (batch == 0) return JANUS_OK;
-    // a workgroup of 256 lanes for each 8192 logits of a row
-    if ((uint64_t)batch * beams * ((vocab + 8191u) / 8192u) >= (1ull << 24))
+    // a workgroup of 512 lanes for each 8192 logits of a row, and one for each request
+    if ((uint64_t)batch * beams * ((vocab + 8191u) / 8192u) >= (1ull << 23))
         return fail(ctx, JANUS_E_INVALID_DIM, "beam_select: more logits than one launch takes");
     if (int e = need_device(ctx)) return e;
     DeviceGuard g(ctx->device);

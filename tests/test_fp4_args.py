@@ -106,6 +106,13 @@ def test_select_refusals(vctx):  # noqa: F811
         assert _call(vctx, name, SELECT, **fine)[0] == _lib.E_NO_DEVICE, fine
 
 
+def test_select_takes_as_many_requests_as_one_launch(vctx):  # noqa: F811
+    # 512 lanes for each request and for each part of a row, fewer than 2^32 in all
+    small = dict(beams=1, vocab=7, n=1)
+    assert _call(vctx, "janus_beam_select", SELECT, batch=2 ** 23, **small)[0] == _lib.E_INVALID_DIM
+    assert _call(vctx, "janus_beam_select", SELECT, batch=2 ** 23 - 1, **small)[0] == _lib.E_NO_DEVICE
+
+
 def test_reorder_refusals(vctx):  # noqa: F811
     assert _reorder(vctx)[0] == _lib.E_NO_DEVICE
     for bad in (dict(buffers=(P, None)), dict(base=None), dict(parents=None)):

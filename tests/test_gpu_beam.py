@@ -83,6 +83,27 @@ def test_ties_go_to_the_lowest_index(engine, vocab, n):
     _check(engine, mixed, torch.zeros(1, 3), n)
 
 
+@pytest.mark.parametrize("beams,vocab", [(16, 40000), (64, 50001)])
+def test_many_parts_of_many_candidates(engine, beams, vocab):
+    """64 candidates of each of 80 and 448 parts: the best of all in one part, in one beam, everywhere alike."""
+    gen = torch.Generator().manual_seed(beams)
+    logits = torch.randn(2 * beams, vocab, generator=gen)
+    scores = -2 * torch.rand(2, beams, generator=gen)
+    _check(engine, logits, scores, 64)
+    one = logits.clone()
+    one[3, 8192:8300] += 30       # 64 of one part before all others of its beam
+    one[beams + 5, 7:20000:190] += 30
+    _check(engine, one, scores, 64)
+    _check(engine, logits, torch.where(torch.arange(beams) == 7, 0.0, scores - 40.0), 64)
+    levels = torch.randint(0, 2, (2 * beams, vocab), generator=gen).float()
+    _check(engine, levels, torch.full((2, beams), -1.0), 64)
+    ended = scores.clone()
+    ended[0, 1:] = ended[1] = -math.inf
+    _check(engine, logits, ended, 64)
+    logits[9, 3] = math.nan
+    _check(engine, logits, scores, 64)
+
+
 @pytest.mark.parametrize("order", [1, -1])
 def test_sorted_logits(engine, order):
     # the best ones lie in few lanes and in one wavefront
