@@ -13,7 +13,7 @@
 // power of two per column, and P in two binary16 parts (22 bits), small parts first.
 //
 // Two kernels, by the columns of a sequence and KV head:
-//   up to 16 (decode steps, a few drafted rows): bound by the read of the cache. A
+//   up to 16, and to 64 of one or two KV heads while all run at once (decode steps, drafted rows): bound by the read of the cache. A
 //     wavefront has one KV head and 32 positions at a time, whose 4-bit rows come into LDS
 //     as they are. A decode step of 64 sequences of up to 8000 positions, 32 heads on 8, 128
 //     dims: 63 us, 4.6 TB/s, what a large copy reaches; one sequence of 8192 positions 14 us, where
@@ -24,7 +24,7 @@
 //     960 TFLOP/s of what the causal mask leaves, where a large matrix product reaches 1184; 20
 //     prompts of 3 to 611 rows 54 us, of which the read of q and the write of the output are
 //     22: a workgroup has ten steps at most, and its start and end are not hidden.
-//     From 17 columns on that is faster than tiles of 16 columns that each read K and V (12
+//     From 17 columns of more heads on that is faster than tiles of 16 columns that each read K and V (12
 //     sequences of 20 columns behind 10574 positions 39 and 45 us, 40 of 30 columns behind 600
 //     21 and 39; binary32 rows 46 and 47, 27 and 36).
 // Where the tiles are few their positions are split into shares and a third kernel joins
@@ -525,7 +525,7 @@ __device__ __forceinline__ uint2 first_nans(const uint8_t *ks, const uint8_t *vs
     return at;
 }
 
-// Up to 16 columns of a sequence and positions [from, to): the NW wavefronts of a
+// A tile of up to 16 columns of a sequence and positions [from, to): the NW wavefronts of a
 // workgroup take hw KV heads and ph phases of 32 positions each; PER of them share a SIMD.
 template <typename T, int D, int NW, int PER, bool SPLIT>
 __global__ __launch_bounds__(NW * 64, PER) void fp4_attn_kernel(Fp4Args args) {
@@ -1262,9 +1262,11 @@ void plan(janus_ctx *ctx, Fp4Args &a, uint32_t cols, uint32_t hw, uint32_t ph, u
     const bool split = cols <= 16 ? steps * at_once > 10 * at_once + 20 * busy && busy < 4 * at_once
                                   : steps > fewest && 2 * busy <= at_once && 3 * mean <= max_len;
     if (counts && split) {
-        a.shares = a.target = (uint32_t)at_once;
-        a.slots = (uint32_t)(at_once + tiles);
-        a.mean_parts = (uint32_t)(at_once / busy) + 1;
+        // at most 128 parts of a tile, which the join's 16 wavefronts read in one go: a sequence of 16000 positions
+        // in 250 parts 21 us, in 125 18 to 19
+        a.shares = a.target = (uint32_t)std::min<uint64_t>(at_once, 128 * busy);
+        a.slots = (uint32_t)(a.shares + tiles);
+        a.mean_parts = (uint32_t)std::min<uint64_t>(a.shares / busy, steps / a.least) + 1;
     }
 }
 
@@ -1279,10 +1281,14 @@ int reserve(janus_ctx *ctx, Fp4Args &a, uint32_t D) {
     return JANUS_OK;
 }
 
+// KV heads of a few-column workgroup.
+uint32_t few_heads(uint32_t kv_heads, uint32_t waves) {
+    while (kv_heads % waves) waves /= 2;
+    return waves;
+}
+
 template <typename T, int D, int NW, int PER> int launch_few(janus_ctx *ctx, Fp4Args &a, uint32_t max_len) {
-    uint32_t hw = NW;
-    while (a.kv_heads % hw) hw /= 2;
-    const uint32_t ph = NW / hw;
+    const uint32_t hw = few_heads(a.kv_heads, NW), ph = NW / hw;
     // two tiles, or the phases' results: 64 KB at most
     const uint32_t lds = std::max<uint32_t>(Tile<D, NW>::kLds, (ph - 1) * hw * (D / 4 + 2) * 256u);
     plan(ctx, a, 16, hw, ph, 32 * ph, std::min<uint32_t>(PER * 4 / NW, 160 * 1024 / lds), 0, max_len);
@@ -1306,8 +1312,18 @@ template <typename T, int D> int launch_dim(janus_ctx *ctx, Fp4Args &a, uint32_t
     // what fits the registers: q and O of 16 columns in 128 of them (two workgroups of eight wavefronts on a CU),
     // with two-part q of 128 dims in 160 (three of four wavefronts)
     constexpr bool kTwo = sizeof(T) == 4 && D == 128;
+    constexpr int NW = kTwo ? 4 : 8, PER = kTwo ? 3 : 4;
+    // One or two KV heads leave a few-column workgroup many phases, 64 to 256 positions at a time where the other kernel
+    // takes 64: while all its tiles run at once that is the shorter chain, though each reads K and V (16/1/128, 64 x 3 rows
+    // behind up to 2000: 19 and 27 us, binary32 22 and 31; 40 x 3 behind 600 12 and 17, 12 and 22). Long contexts of
+    // binary16 rows are bound by those reads (64 x 3 behind up to 7800 43 and 36, binary32 44 and 44; 300 x 3 behind 1000
+    // 34 and 30), and with eight heads a step is 32 positions (32/8/128, 40 x 8 behind 600: 41 and 20).
+    const uint32_t hw = few_heads(a.kv_heads, NW);
+    const uint64_t tiles = ((uint64_t)a.rows * a.G + 15) / 16 + a.nseq - 1;
+    const bool many_phases = hw <= 2 && tiles * (a.kv_heads / hw) <= (uint64_t)ctx->num_cus * (PER * 4 / NW) &&
+                             (sizeof(T) == 4 || max_len <= 2048);
     int e;
-    if (columns <= 16) e = launch_few<T, D, kTwo ? 4 : 8, kTwo ? 3 : 4>(ctx, a, max_len);
+    if (columns <= 16 || (columns <= 64 && many_phases)) e = launch_few<T, D, NW, PER>(ctx, a, max_len);
     else if (columns <= 64) e = launch_wide<T, D, 2>(ctx, a, max_len);
     else e = launch_wide<T, D, 1>(ctx, a, max_len);
     if (e || !a.target) return e;
