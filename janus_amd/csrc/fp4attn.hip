@@ -20,7 +20,7 @@
 //     the two launches and the start of each count; 16 x 5 binary32 rows behind 2500 positions of
 //     32 KV heads 36 us, 2.6 TB/s: the conversions and two-part products take as long as the reads.
 //   more (prompts): bound by the matrix unit and what feeds it. Four wavefronts of 32 columns, or
-//     two pairs of them for up to 64, share K and V, converted once for all of them. A prompt of 6000 rows: 307 to 320 us, 920 to
+//     two pairs of them for up to 64 or where there are few tiles, share K and V, converted once for all of them. A prompt of 6000 rows: 307 to 320 us, 920 to
 //     960 TFLOP/s of what the causal mask leaves, where a large matrix product reaches 1184; 20
 //     prompts of 3 to 611 rows 54 us, of which the read of q and the write of the output are
 //     22: a workgroup has ten steps at most, and its start and end are not hidden.
@@ -846,7 +846,7 @@ template <typename T, int D, int TP> struct Rows {
 
 // PH 1: four wavefronts of 32 columns. PH 2: two, with two wavefronts each, which take every
 // other 32 positions and are joined at the end: for up to 64 columns of a sequence, where two of
-// four wavefronts or more would have none (12 binary32 sequences of 40 columns behind 10574 positions 53 us,
+// four wavefronts or more would have none, and for few tiles (12 binary32 sequences of 40 columns behind 10574 positions 53 us,
 // 66 with PH 1; 40 binary16 ones behind 600 23 and 27; one of 20 columns 18.5 and 18).
 template <typename T, int D, int TP, int PH, bool SPLIT>
 __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
@@ -1300,10 +1300,13 @@ template <typename T, int D, int NW, int PER> int launch_few(janus_ctx *ctx, Fp4
 
 template <typename T, int D, int PH> int launch_wide(janus_ctx *ctx, Fp4Args &a, uint32_t max_len) {
     constexpr int TP = PH == 1 && D == 128 && sizeof(T) == 4 ? 32 : 64;
-    plan(ctx, a, 128 / PH, 1, 1, 64, 2, sizeof(T) == 4 ? 10 : 16, max_len);   // a step of two-part rows takes twice as long
+    // a step of two-part rows takes twice as long; tiles of 128 such columns are more than the CUs (launch_dim) and stay whole
+    constexpr bool kWhole = PH == 1 && sizeof(T) == 4;
+    plan(ctx, a, 128 / PH, 1, 1, 64, 2, kWhole ? 0xffffffffu : sizeof(T) == 4 ? 10 : 16, max_len);
     if (int e = reserve(ctx, a, D)) return e;
     const dim3 grid(a.shares * a.kv_heads), block(256);
-    if (a.target) return launch(ctx, fp4_wide_kernel<T, D, TP, PH, true>, grid, block, 4 * TP * D * 2, a);
+    if constexpr (!kWhole)
+        if (a.target) return launch(ctx, fp4_wide_kernel<T, D, TP, PH, true>, grid, block, 4 * TP * D * 2, a);
     return launch(ctx, fp4_wide_kernel<T, D, TP, PH, false>, grid, block, 4 * TP * D * 2, a);
 }
 
@@ -1322,9 +1325,15 @@ template <typename T, int D> int launch_dim(janus_ctx *ctx, Fp4Args &a, uint32_t
     const uint64_t tiles = ((uint64_t)a.rows * a.G + 15) / 16 + a.nseq - 1;
     const bool many_phases = hw <= 2 && tiles * (a.kv_heads / hw) <= (uint64_t)ctx->num_cus * (PER * 4 / NW) &&
                              (sizeof(T) == 4 || max_len <= 2048);
+    // Pairs of wavefronts also where tiles of 128 columns would leave a place of every CU free: half the columns and
+    // half the work of each step. One prompt of 1000 rows at 32/8/128: 31 and 27 us, binary32 51 and 37; of 2000 at
+    // 16/1/128 51 and 42, 86 and 58. Short binary16 rows gain nothing from there being more of them (16 prompts of 120
+    // at 16/1/128: 11 and 13 us, 4 of 500 19 and 20, one of 300 at 32/8/128 14 and 13).
+    const uint64_t wide = (((uint64_t)a.rows * a.G + 127) / 128 + a.nseq - 1) * a.kv_heads, cus = (uint64_t)ctx->num_cus;
+    const bool pairs = columns <= 64 || 2 * wide <= cus || (wide <= cus && (sizeof(T) == 4 || a.rows / a.nseq >= 512));
     int e;
     if (columns <= 16 || (columns <= 64 && many_phases)) e = launch_few<T, D, NW, PER>(ctx, a, max_len);
-    else if (columns <= 64) e = launch_wide<T, D, 2>(ctx, a, max_len);
+    else if (pairs) e = launch_wide<T, D, 2>(ctx, a, max_len);
     else e = launch_wide<T, D, 1>(ctx, a, max_len);
     if (e || !a.target) return e;
     const uint32_t units = a.rows * a.heads;

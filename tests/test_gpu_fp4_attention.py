@@ -459,3 +459,69 @@ def test_weights_that_are_small_in_binary16(engine, types, rows, at, hd):
             w = (n - rows + r) * math.exp(-float(q[r, 0, 0]))
             want = (w if values is vc else 1.0) / (1 + w)
             assert (out[r].double().cpu() / want - 1).abs().max() < tol, (r, out[r].flatten()[:4], want)
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("sigma", [1.5, 40.0])
+def test_more_tiles_than_cus(engine, types, hd, sigma):
+    # 384 tiles of 128 columns and more: prompts of odd lengths, chunks behind a context, one row, none, more rows than positions
+    seqs = [(70, 70), (129, 129), (65, 200), (1, 300), (0, 0), (90, 65), (64, 64), (127, 127)]
+    _run(engine, 64, 32, hd, seqs, types, behind=2, sigma=sigma, device=DEV)
+
+
+@pytest.mark.parametrize("rows", [40, 70])
+def test_many_tiles_in_parts(engine, rows):
+    # 32 tiles of each of eight heads, 80 or 140 columns: binary16 rows behind a long context
+    _run(engine, 16, 8, 128, [(rows, 1900 + 30 * i) for i in range(16)], "f16", device=DEV)
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+def test_nan_blocks_of_many_tiles(engine, types):
+    heads, kvh, hd, n = 64, 32, 128, 150
+    dtype = TYPES[types]
+    gen = torch.Generator().manual_seed(31)
+    q = torch.randn(5 * n, heads, hd, generator=gen).to(dtype)
+    cache = [*random_cache(gen, 5 * n, kvh, hd), *random_cache(gen, 5 * n, kvh, hd)]
+    cache[1][n + 100, 3, 1] = 255       # K of sequence 1, head 3
+    cache[3][2 * n + 37, 5, 2] = 255    # V of sequence 2, head 5
+    k, v = decode(*cache[:2]), decode(*cache[2:])
+    out = torch.empty(q.shape, dtype=dtype, device=DEV)
+    ops.fp4_attention(engine, q.to(DEV), *[c.to(DEV) for c in cache], out, 5, n)
+    odd = torch.zeros(5 * n, heads, hd, dtype=torch.bool)
+    odd[n + 100:2 * n, 6:8] = True
+    odd[2 * n + 37:3 * n, 10:12, 64:96] = True
+    got = out.cpu()
+    assert torch.equal(got.isnan(), odd)
+    for s in (0, 1, 2, 4):
+        at = slice(s * n, (s + 1) * n)
+        with torch.device(DEV):
+            want, tol = attend(q[at].to(DEV), k[at].nan_to_num(0).to(DEV), v[at].nan_to_num(0).to(DEV),
+                               list(range(1, n + 1)), types == "f16", True, None)
+        fine = ~odd[at]
+        check(got[at][fine], want.cpu()[fine], tol.cpu()[fine], (types, s))
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+def test_far_scores_of_many_tiles(engine, types):
+    """As test_scores_beyond_their_own_last_bits, 32 KV heads of 140 columns, 4 sequences."""
+    dtype = TYPES[types]
+    gen = torch.Generator().manual_seed(33)
+    hd, kvh, n, size = 128, 32, 70, 3e4 if types == "f16" else 1e8
+    q = (torch.randn(4 * n, 2 * kvh, hd, generator=gen).sign() * size).to(dtype)
+    codes = torch.where(torch.rand(4 * n, kvh, hd // 2, generator=gen) < 0.5, 0x66, 0xEE).to(torch.uint8)   # 4 and -4
+    scales = torch.full((4 * n, kvh, hd // 32), 131, dtype=torch.uint8)
+    values = random_cache(gen, 4 * n, kvh, hd)
+    k, v = decode(codes, scales), decode(*values)
+    out = torch.empty(q.shape, dtype=dtype, device=DEV)
+    ops.fp4_attention(engine, q.to(DEV), *[c.to(DEV) for c in (codes, scales, *values)], out, 4, n)
+    got = out.cpu()
+    for s in (0, 3):
+        for h in (0, 7, 63):
+            at = slice(s * n, (s + 1) * n)
+            score = q[at, h].double() @ k[at, h // 2].t()
+            score = score.masked_fill(torch.ones(n, n).triu(1).bool(), -math.inf)
+            first = (score == score.amax(-1, keepdim=True)).double()
+            want = first @ v[at, h // 2] / first.sum(-1, keepdim=True)
+            tol = 2.0 ** (-10 if types == "f16" else -20) * v.abs().max()
+            check(got[at, h], want, tol.expand_as(want), (types, s, h))
