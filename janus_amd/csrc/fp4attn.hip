@@ -1328,9 +1328,13 @@ template <typename T, int D> int launch_dim(janus_ctx *ctx, Fp4Args &a, uint32_t
     // Pairs of wavefronts also where tiles of 128 columns would leave a place of every CU free: half the columns and
     // half the work of each step. One prompt of 1000 rows at 32/8/128: 31 and 27 us, binary32 51 and 37; of 2000 at
     // 16/1/128 51 and 42, 86 and 58. Short binary16 rows gain nothing from there being more of them (16 prompts of 120
-    // at 16/1/128: 11 and 13 us, 4 of 500 19 and 20, one of 300 at 32/8/128 14 and 13).
+    // at 16/1/128: 11 and 13 us, 4 of 500 19 and 20, one of 300 at 32/8/128 14 and 13). Where the steps of two-part rows
+    // of 128 dims are long, and those of binary16 ones of 64 short, also for both places of every CU (1500 rows at
+    // 32/8/128 binary32 72 and 61, at 24/8/64 binary16 29 and 26; 2000 binary16 ones at 32/8/128 59 and 66, 8 x 250
+    // binary32 ones at 24/8/64 17 and 22).
     const uint64_t wide = (((uint64_t)a.rows * a.G + 127) / 128 + a.nseq - 1) * a.kv_heads, cus = (uint64_t)ctx->num_cus;
-    const bool pairs = columns <= 64 || 2 * wide <= cus || (wide <= cus && (sizeof(T) == 4 || a.rows / a.nseq >= 512));
+    const bool pairs = columns <= 64 || 2 * wide <= cus || (wide <= (kTwo || (sizeof(T) == 2 && D == 64) ? 2 * cus : cus) &&
+                                                                 (sizeof(T) == 4 || a.rows / a.nseq >= 512));
     int e;
     if (columns <= 16 || (columns <= 64 && many_phases)) e = launch_few<T, D, NW, PER>(ctx, a, max_len);
     else if (pairs) e = launch_wide<T, D, 2>(ctx, a, max_len);
