@@ -16,11 +16,11 @@
 //   up to 16, and to 64 of one or two KV heads while all run at once (decode steps, drafted rows): bound by the read of the cache. A
 //     wavefront has one KV head and 32 positions at a time, whose 4-bit rows come into LDS
 //     as they are. A decode step of 64 sequences of up to 8000 positions, 32 heads on 8, 128
-//     dims: 63 us, 4.6 TB/s, what a large copy reaches; one sequence of 8192 positions 14 us, where
+//     dims: 63 us, 4.6 TB/s, what a large copy reaches; one sequence of 8192 positions 15 us, where
 //     the two launches and the start of each count; 16 x 5 binary32 rows behind 2500 positions of
 //     32 KV heads 36 us, 2.6 TB/s: the conversions and two-part products take as long as the reads.
 //   more (prompts): bound by the matrix unit and what feeds it. Four wavefronts of 32 columns, or
-//     two pairs of them for up to 64 or where there are few tiles, share K and V, converted once for all of them. A prompt of 6000 rows: 307 to 320 us, 920 to
+//     two pairs of them for up to 64 or where there are few tiles, share K and V, converted once for all of them. A prompt of 6000 rows: 307 to 335 us, 880 to
 //     960 TFLOP/s of what the causal mask leaves, where a large matrix product reaches 1184; 20
 //     prompts of 3 to 611 rows 54 us, of which the read of q and the write of the output are
 //     22: a workgroup has ten steps at most, and its start and end are not hidden.
