@@ -1076,7 +1076,7 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
             if (__builtin_amdgcn_readfirstlane(far | (__any(fmaf(bm, cs, c2) > kBias + kSlack) ? 1u : 0u))) {
                 const float now = fmaxf(m, bm), cn = now == -INFINITY ? INFINITY : fmaf(-now, cs, kBias);
                 float f;
-                if (__builtin_amdgcn_readfirstlane(far | (__any(fabsf(cn) > 4194304.0f && cn != INFINITY) ? 1u : 0u))) {
+                if (__builtin_amdgcn_readfirstlane(far | (__any(fabsf(cn) > 4194304.0f && now != -INFINITY) ? 1u : 0u))) {   // cn itself may be infinite
                     // from c2 as it was rounded to the difference: kBias - c2 is exact
                     const float r = far ? 0.0f : fmaf(-m, cs, kBias - c2);
                     f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(fmaf(m - now, cs, r));
@@ -1092,7 +1092,7 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
 #pragma unroll
                     for (int v = 0; v < 16; ++v) o[d][v] *= f;
             }
-            float off = c2 == INFINITY ? 0.0f : c2;
+            float off = m == -INFINITY ? 0.0f : c2;
             if (__builtin_amdgcn_readfirstlane(far)) {
                 const float m0 = m == -INFINITY ? 0.0f : m;
                 off = kBias;

@@ -1,0 +1,62 @@
+"""Weights of janus_fp4_attention whose exponents meet the limits of 32 bits."""
+import math
+
+import pytest
+import torch
+
+from janus_amd import ops
+from fp4_ref import decode, random_cache
+from packed_ref import U32, check
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+TYPES = {"f16": torch.float16, "f32": torch.float32}
+
+
+def _attend(engine, q, cache, n, scale, nseq=1):
+    out = torch.empty(q.shape, dtype=q.dtype, device=DEV)
+    ops.fp4_attention(engine, q.to(DEV), *[c.to(DEV) for c in cache], out, nseq, n,
+                      seq_lens=torch.full((nseq,), n, dtype=torch.int32, device=DEV), scale=scale)
+    return out.cpu()
+
+
+def _the_best_share(got, q, k, v, types):
+    """Scores so far apart that the largest of what a row sees takes all weight, equal ones share it."""
+    rows, heads, _ = q.shape
+    n, rep = k.shape[0], heads // k.shape[1]
+    seen = torch.arange(n)[None] < torch.arange(n - rows + 1, n + 1)[:, None]
+    for h in range(heads):
+        s = (q[:, h].double() @ k[:, h // rep].T).masked_fill(~seen, -math.inf)
+        first = (s == s.amax(-1, keepdim=True)).double()
+        want = first @ v[:, h // rep] / first.sum(-1, keepdim=True)
+        tol = 2.0 ** (-10 if types == "f16" else -20) * v.abs().max()
+        check(got[:, h], want, tol.expand_as(want), (types, h))
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("rows,heads,kvh,n", [(3, 4, 2, 1100), (20, 8, 8, 300), (70, 8, 8, 1100), (40, 8, 2, 90)])
+def test_scores_far_below_zero(engine, types, rows, heads, kvh, n):
+    """Every score is below -2^128 in powers of two, beyond binary32, though q, K and the scale are finite: the sums
+    q k are whole multiples of the size of q, exact in binary32, and what is not equal to the largest has no weight."""
+    gen = torch.Generator().manual_seed(51)
+    size, scale = (2.0 ** 14, 2.0 ** 112) if types == "f16" else (2.0 ** 122, 2.0)
+    q = torch.full((rows, heads, 128), size, dtype=TYPES[types])
+    codes = torch.where(torch.rand(n, kvh, 64, generator=gen) < 0.5, 0xEE, 0xDE).to(torch.uint8)   # -4, or -4 and -3
+    cache = [codes, torch.full((n, kvh, 4), 127, dtype=torch.uint8), *random_cache(gen, n, kvh, 128)]
+    k, v = decode(*cache[:2]), decode(*cache[2:])
+    assert (q[:1, :kvh].double() * k).sum(-1).max() * scale * math.log2(math.e) < -2.0 ** 128
+    _the_best_share(_attend(engine, q, cache, n, scale), q, k, v, types)
+
+
+def test_scores_far_below_zero_of_many_tiles(engine):
+    """As above, 32 KV heads of 140 columns, 4 sequences."""
+    gen = torch.Generator().manual_seed(52)
+    n, kvh = 70, 32
+    q = torch.full((4 * n, 2 * kvh, 128), 2.0 ** 14, dtype=torch.float16)
+    codes = torch.where(torch.rand(4 * n, kvh, 64, generator=gen) < 0.5, 0xEE, 0xDE).to(torch.uint8)
+    cache = [codes, torch.full((4 * n, kvh, 4), 127, dtype=torch.uint8), *random_cache(gen, 4 * n, kvh, 128)]
+    k, v = decode(*cache[:2]), decode(*cache[2:])
+    got = _attend(engine, q, cache, n, 2.0 ** 112, nseq=4)
+    for s in range(4):
+        at = slice(s * n, (s + 1) * n)
+        _the_best_share(got[at], q[at], k[at], v[at], "f16")
