@@ -876,7 +876,7 @@ __device__ __forceinline__ bool wide_tile(const PackedArgs &a, const Work &w, ui
             c2 = cn;
             l *= alpha;
             // scores so large that c does not hold their last bits: few_columns takes the difference instead
-            if (fabsf(c2) > 4194304.0f && c2 != INFINITY) l = NAN;
+            if (fabsf(c2) > 4194304.0f && m != -INFINITY) l = NAN;   // c itself may be infinite
 #pragma unroll
             for (int d = 0; d < ND; ++d)
 #pragma unroll
