@@ -1077,8 +1077,9 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
                 const float now = fmaxf(m, bm), cn = now == -INFINITY ? INFINITY : fmaf(-now, cs, kBias);
                 float f;
                 if (__builtin_amdgcn_readfirstlane(far | (__any(fabsf(cn) > 4194304.0f && now != -INFINITY) ? 1u : 0u))) {   // cn itself may be infinite
-                    // from c2 as it was rounded to the difference: kBias - c2 is exact
-                    const float r = far ? 0.0f : fmaf(-m, cs, kBias - c2);
+                    // from c2 as it was rounded to the difference: all but kBias of it cancels in one FMA
+                    // (kBias - c2 by itself loses 1/4 where c2 is below kBias - 2^22)
+                    const float r = far ? 0.0f : fmaf(-m, cs, -c2) + kBias;
                     f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(fmaf(m - now, cs, r));
                     far = 1;
                 } else {

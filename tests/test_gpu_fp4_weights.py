@@ -60,3 +60,29 @@ def test_scores_far_below_zero_of_many_tiles(engine):
     for s in range(4):
         at = slice(s * n, (s + 1) * n)
         _the_best_share(got[at], q[at], k[at], v[at], "f16")
+
+
+def _unit_keys(n, kvh, at):
+    """Codes and scales of K: 1 in the dims that `at` names for a position, else 0."""
+    codes = torch.zeros(n, kvh, 64, dtype=torch.uint8)
+    for p, dims in at.items():
+        for d in dims:
+            codes[p, :, d // 2] |= 2 << 4 * (d % 2)
+    return [codes, torch.full((n, kvh, 4), 127, dtype=torch.uint8)]
+
+
+@pytest.mark.parametrize("rows", [3, 20, 60])
+def test_a_maximum_that_goes_beyond_2_to_22(engine, rows):
+    """The running maximum, in powers of two, is 4194311.17 and later 4194318.38: on this way kBias less its offset
+    (-4194298.25) is not a binary32 number, the next ones are 1/4 away. The scores are exact, and the weight of the
+    first position is e^-5."""
+    a, later, n, kvh = 2907275, 5, 70 + rows, 8
+    q = torch.zeros(rows, kvh, 128)
+    q[..., 0], q[..., 1] = a, later
+    cache = _unit_keys(n, kvh, {0: [0], 64: [0, 1]}) + [*random_cache(torch.Generator().manual_seed(54), n, kvh, 128)]
+    v = decode(*cache[2:])
+    w = math.exp(-later)
+    want = ((v[64] + w * v[0]) / (1 + w)).expand(rows, kvh, 128)
+    # scale log2(e) is rounded (2 u of 5 log2(e)), the weight by 2^-22, each step of the joined sums by u
+    tol = w * (10 * 1.45 * U32 + 2.0 ** -22) * (v[64] - v[0]).abs() + 8 * U32 * (v[64].abs() + v[0].abs())
+    check(_attend(engine, q, cache, n, 1.0), want, tol.expand(rows, kvh, 128), rows)
