@@ -49,7 +49,7 @@ struct Fp4Args {
     const void *q;                        // [rows][heads][D]
     const uint8_t *kc, *ks, *vc, *vs;     // [cache rows][kv_heads][D / 2] and [D / 32]
     void *out;                            // [rows][heads][D]
-    float *part, *part_ml;                // split: [slot][kv_heads][cols][D], and (m, factor, l, -): the maximum is 2^(m factor)
+    float *part, *part_ml;                // split: [slot][kv_heads][cols][D], and (m, factor, l, b): weights are multiples of 2^(m factor - b)
     uint32_t *meta;                       // split: [rows * G] (first slot, parts | sees nothing << 23 | column << 24)
     const int32_t *q_start, *row_base, *seq_lens;
     uint32_t rows, nseq, heads, kv_heads, G;
@@ -679,7 +679,7 @@ __global__ __launch_bounds__(NW * 64, PER) void fp4_attn_kernel(Fp4Args args) {
 #pragma unroll
                     for (int i = 0; i < D / 16; i += 4)
                         *(ff4 *)(to + rr * (D / 16) + i) = ff4{col.o[i][rr], col.o[i + 1][rr], col.o[i + 2][rr], col.o[i + 3][rr]};
-                if (g == 0) *(ff4 *)(z.part_ml + 4 * at) = ff4{col.m, col.cs, col.l, 0.0f};
+                if (g == 0) *(ff4 *)(z.part_ml + 4 * at) = ff4{col.m, col.cs, col.l, 0.0f};   // kBias, in all parts alike, counts for nothing
             } else {
                 const float inv = col.vis ? 1.0f / col.l : 0.0f;
                 T *to = (T *)z.out + ((size_t)(w.s.row0 + r) * z.heads + (size_t)kvh * z.G + gh) * D + g * DL;
@@ -706,7 +706,7 @@ __global__ __launch_bounds__(NW * 64, PER) void fp4_attn_kernel(Fp4Args args) {
 }
 
 // Joins the parts of a row and head: W wavefronts take them in turn, eight at a time,
-// and are joined themselves. Workgroups of 4 units for W = 1, else of one. The exponents m factor
+// and are joined themselves. Workgroups of 4 units for W = 1, else of one. The exponents m factor - b
 // are exact in binary64: in 32 bits their rounding would be that of the parts' weights.
 template <typename T, int D, int W> __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void fp4_join_kernel(Fp4Args a) {
     __shared__ double sm[W];
@@ -745,7 +745,7 @@ template <typename T, int D, int W> __global__ __launch_bounds__(W == 1 ? 256 : 
         double now = m;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            e[i] = i0 + i < parts ? (double)ml[i][0] * (double)ml[i][1] : -INFINITY;
+            e[i] = i0 + i < parts ? (double)ml[i][0] * (double)ml[i][1] - (double)ml[i][3] : -INFINITY;
             now = fmax(now, e[i]);
         }
         const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((float)(m - now));
@@ -1130,20 +1130,23 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
             l += sum[0] + sum[1];
         }
         l += swap32(l);
-        // from here on the maximum is 2^(m cs), less what the rounding of c2 has moved
+        // from here on the weights are multiples of 2^(m cs - less), as the roundings have left them: kBias - c2 for m would
+        // be off by up to 2^-21 (1/4 near 2^22), and so would all weights of a phase or part, against those of the others
+        float less = far ? kBias : 0.0f;
         if (!far) {
-            m = m == -INFINITY ? m : kBias - c2;
+            m = m == -INFINITY ? m : -c2;
             cs = 1.0f;
         }
         const bool odd = p0 < p1 && __syncthreads_or(worst > 140u);
         if constexpr (PH == 2) {
-            // the second phase's state goes through the first tile, its m, factor and l through where its rows were
+            // the second phase's state goes through the first tile, its m, factor, less and l through where its rows were
             float *const state = (float *)(smem + (wave & 1u) * kTile) + lane;
             float *const sums = (float *)(smem + 2 * kTile + (2u + (wave & 1u)) * (kTile / 2)) + lane;
             if (phase) {
                 sums[0] = m;
                 sums[64] = cs;
                 sums[128] = l;
+                sums[192] = less;
 #pragma unroll
                 for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -1152,7 +1155,7 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
             __syncthreads();
             if (!phase) {
                 const float m2 = sums[0], cs2 = sums[64];
-                const double e1 = (double)m * (double)cs, e2 = (double)m2 * (double)cs2;
+                const double e1 = (double)m * (double)cs - less, e2 = (double)m2 * (double)cs2 - sums[192];
                 const float f1 = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((float)(e1 - fmax(e1, e2)));
                 const float f2 = m2 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((float)(e2 - fmax(e1, e2)));
                 l = l * f1 + sums[128] * f2;
@@ -1163,6 +1166,7 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
                 if (e2 > e1) {
                     m = m2;
                     cs = cs2;
+                    less = sums[192];
                 }
             }
         }
@@ -1190,7 +1194,7 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
                     for (int j = 0; j < 4; ++j)
                         *(jf4 *)(to + 32 * d + 8 * j + 4 * h) = jf4{o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]};
             }
-            if (there && h == 0) *(ff4 *)(z.part_ml + 4 * at) = ff4{m, cs, l, 0.0f};
+            if (there && h == 0) *(ff4 *)(z.part_ml + 4 * at) = ff4{m, cs, l, less};
         } else {
             typedef Rows<T, D, TP> R;
             const float inv = vis ? 1.0f / l : 0.0f;

@@ -86,3 +86,23 @@ def test_a_maximum_that_goes_beyond_2_to_22(engine, rows):
     # scale log2(e) is rounded (2 u of 5 log2(e)), the weight by 2^-22, each step of the joined sums by u
     tol = w * (10 * 1.45 * U32 + 2.0 ** -22) * (v[64] - v[0]).abs() + 8 * U32 * (v[64].abs() + v[0].abs())
     check(_attend(engine, q, cache, n, 1.0), want, tol.expand(rows, kvh, 128), rows)
+
+
+@pytest.mark.parametrize("rows", [3, 20, 60])
+@pytest.mark.parametrize("a,b", [(9.483467102050781, 9.483417510986328), (8.494361877441406, 8.49441146850586),
+                                 (2907272, 2907273), (2907274, 2907275)])
+def test_parts_are_joined_by_what_their_weights_mean(engine, rows, a, b):
+    """Positions 0 to 31 of 64 have the score a, the others b, which one wavefront, or one of a pair each, takes: both
+    are exact, but kBias less their offsets rounds to either side, by 2^-21 (1/4) in powers of two. With V of 1 and -1 the
+    output is (A - B) / (A + B), off by half the difference of the weights' errors of up to 2^-22 each."""
+    n, kvh = 64, 8
+    q = torch.zeros(rows, kvh, 128)
+    q[..., 0], q[..., 1] = a, b
+    cache = _unit_keys(n, kvh, {p: [0 if p < 32 else 1] for p in range(n)})
+    sign = torch.where(torch.arange(n) < 32, 0x22, 0xAA).to(torch.uint8)
+    cache += [sign[:, None, None].expand(n, kvh, 64).contiguous(), torch.full((n, kvh, 4), 127, dtype=torch.uint8)]
+    seen = torch.arange(n - rows + 1, n + 1).double()
+    one, two = seen.clamp(max=32), (seen - 32).clamp(min=0) * math.exp(b - a)
+    want = ((one - two) / (one + two))[:, None, None].expand(rows, kvh, 128)
+    tol = 2.0 ** -22 + 8 * U32 * want.abs() + 2 * 1.45 * U32 * abs(b - a)
+    check(_attend(engine, q, cache, n, 1.0), want, tol, (rows, a, b))
