@@ -311,6 +311,11 @@ __device__ __forceinline__ uint32_t half_pair(float a, float b) {
 }
 __device__ __forceinline__ ff4 mfma(fh8 a, fh8 b, ff4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
+// The factor from scores to exponents: not 0, since it also multiplies -infinity, nor infinite (a scale or a row of q
+// near the end of binary32), since it also multiplies differences of 0. The limits change no weight: scores, as the
+// products have them, are whole multiples of 2^-48 and below 2^39.
+__device__ __forceinline__ float finite_factor(float cs) { return fminf(fmaxf(cs, 1e-37f), 3e38f); }
+
 // Sixteen columns of a wavefront. Lane 16 g + a:
 //   K: its bytes of a position lie in one block of 32 dims, and the order of dims in the sum is
 //     free, so D / 8 consecutive bytes are its operand of the D / 32 products;
@@ -387,7 +392,7 @@ template <typename T, int D> struct Columns {
                 q[1][i] = lo;
             }
         }
-        cs = fmaxf(cs, 1e-37f);   // not 0: it also multiplies -infinity
+        cs = finite_factor(cs);
         m = -INFINITY;
         l = 0.0f;
 #pragma unroll
@@ -996,7 +1001,7 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
             bad = top >= 0x7f800000u;
             const int e = P == 2 && !bad ? max((int)(top >> 23), 1) - 127 - 14 : 0;
             if constexpr (P == 2) cs = ldexpf(a.scale2, e);
-            cs = fmaxf(cs, 1e-37f);
+            cs = finite_factor(cs);
 #pragma unroll
             for (int s = 0; s < QN; ++s)
 #pragma unroll

@@ -106,3 +106,17 @@ def test_parts_are_joined_by_what_their_weights_mean(engine, rows, a, b):
     want = ((one - two) / (one + two))[:, None, None].expand(rows, kvh, 128)
     tol = 2.0 ** -22 + 8 * U32 * want.abs() + 2 * 1.45 * U32 * abs(b - a)
     check(_attend(engine, q, cache, n, 1.0), want, tol, (rows, a, b))
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("rows,n", [(3, 200), (20, 200), (60, 1500)])
+def test_factors_beyond_32_bits(engine, types, rows, n):
+    """log2(e) times the scale, or that times a row's power of two, is above the largest binary32 number: what is
+    not equal to the largest score has no weight."""
+    gen = torch.Generator().manual_seed(55)
+    kvh = 8
+    size, scale = (1.0, 3e38) if types == "f16" else (2.0 ** 126, 2.0 ** 20)
+    q = torch.full((rows, kvh, 128), size, dtype=TYPES[types])
+    codes = torch.where(torch.rand(n, kvh, 64, generator=gen) < 0.5, 0x22, 0xA2).to(torch.uint8)   # 1, or 1 and -1
+    cache = [codes, torch.full((n, kvh, 4), 127, dtype=torch.uint8), *random_cache(gen, n, kvh, 128)]
+    _the_best_share(_attend(engine, q, cache, n, scale), q, decode(*cache[:2]), decode(*cache[2:]), types)
