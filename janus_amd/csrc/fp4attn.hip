@@ -104,7 +104,7 @@ __device__ __forceinline__ SeqRows seq_rows(const Fp4Args &a, uint32_t s) {
     q.row0 = (uint32_t)r0;
     q.n = (uint32_t)(r1 - r0);
     const int32_t len = max(a.seq_lens ? given : r1 - r0, -(1 << 26));
-    q.first = len - (r1 - r0) + 1;
+    q.first = (int32_t)((uint32_t)len + 1u - q.n);   // n > 0 wherever it is used
     const bool inside = base >= 0 && base < (int64_t)a.cache_rows;
     q.base = inside ? (uint32_t)base : 0u;
     q.avail = inside && len > 0 ? min(min((uint32_t)len, a.max_seq), a.cache_rows - q.base) : 0u;
