@@ -355,7 +355,9 @@ int janus_fp4_attention(janus_ctx *ctx, const void *q, int dtype, const void *k_
  * logits are all -infinity likewise; one with a NaN or +infinity among its logits, or as
  * its score, has NaN for all its values, which comes before every number, so that it is
  * seen. 1 to 64 beams, n 1 to 64 and at most beams * vocab, beams * vocab below 2^31.
- * Partials go into the context's GEMM workspace (janus_set_stream). */
+ * d_out_scores may be d_scores where n = beams; otherwise no output may overlap an
+ * input or another output. Partials go into the context's GEMM workspace
+ * (janus_set_stream). */
 int janus_beam_select(janus_ctx *ctx, const float *logits, const float *d_scores, float *d_out_scores,
                       int32_t *d_out_parents, int32_t *d_out_tokens, uint32_t batch, uint32_t beams, uint32_t vocab,
                       uint32_t n);

@@ -397,6 +397,21 @@ int janus_beam_select(janus_ctx *ctx, const float *logits, const float *d_scores
     if ((uint64_t)batch * beams * ((vocab + 8191u) / 8192u) >= (1ull << 23))
         return fail(ctx, JANUS_E_INVALID_DIM, "beam_select: more logits than one launch takes");
     if (int e = need_device(ctx)) return e;
+    // A request's workgroup writes its results while others still read theirs. Scores in place are its own where n is beams.
+    const uint64_t row = (uint64_t)batch * beams * 4, res = (uint64_t)batch * n * 4;
+    const struct { const void *p; uint64_t bytes; } out[3] = {{d_out_scores, res}, {d_out_parents, res}, {d_out_tokens, res}},
+                                                    in[2] = {{logits, row * vocab}, {d_scores, d_scores ? row : 0}};
+    auto meet = [](const auto &a, const auto &b) {
+        const uint64_t x = (uint64_t)(uintptr_t)a.p, y = (uint64_t)(uintptr_t)b.p;
+        return x <= y ? y - x < a.bytes && b.bytes : x - y < b.bytes && a.bytes;
+    };
+    for (int i = 0; i < 3; ++i) {
+        for (int j = 0; j < 2; ++j)
+            if (meet(out[i], in[j]) && !(i == 0 && j == 1 && d_out_scores == d_scores && n == beams))
+                return fail(ctx, JANUS_E_INVALID_ARG, "beam_select: an output overlaps an input");
+        for (int j = 0; j < i; ++j)
+            if (meet(out[i], out[j])) return fail(ctx, JANUS_E_INVALID_ARG, "beam_select: outputs overlap");
+    }
     DeviceGuard g(ctx->device);
     return beam_select_launch(ctx, logits, d_scores, d_out_scores, d_out_parents, d_out_tokens, batch, beams, vocab, n);
 }
