@@ -490,28 +490,30 @@ def fp4_attention(engine, query, k_cache, k_scales, v_cache, v_scales, output, n
 
 # ---- beam search -------------------------------------------------------------------------
 
-def beam_select(engine, logits, scores, out_scores, out_parents, out_tokens) -> None:
+def beam_select(engine, logits, scores: Optional[torch.Tensor], out_scores, out_parents, out_tokens) -> None:
     """The best continuations of each request's beams (janus_beam_select in
     include/janus_hip.h). logits [batch * beams, vocab] float32 (or [batch, beams,
-    vocab]), scores [batch, beams] float32; out_scores (float32), out_parents and
+    vocab]), scores [batch, beams] float32 or None for zeros; out_scores (float32), out_parents and
     out_tokens (int32), [batch, n], receive the n largest of scores + log_softmax(logits)
     of each request in descending order, equal ones by beam, then token. A beam whose score
-    is -infinity has ended."""
+    is -infinity has ended. out_scores may be scores where n is beams."""
     dev = engine.device
-    if scores.dim() != 2 or out_scores.dim() != 2 or out_scores.shape[0] != scores.shape[0]:
-        raise ValueError(f"scores: [batch, beams] and out_scores: [batch, n] expected, got {tuple(scores.shape)} and "
-                         f"{tuple(out_scores.shape)}")
-    batch, beams = scores.shape
-    n, vocab = out_scores.shape[1], logits.shape[-1] if logits.dim() else 0
+    if out_scores.dim() != 2 or (scores is not None and (scores.dim() != 2 or out_scores.shape[0] != scores.shape[0])):
+        raise ValueError(f"scores: [batch, beams] and out_scores: [batch, n] expected, got "
+                         f"{'none' if scores is None else tuple(scores.shape)} and {tuple(out_scores.shape)}")
+    batch, n = out_scores.shape
+    vocab = logits.shape[-1] if logits.dim() else 0
+    beams = scores.shape[1] if scores is not None else logits.numel() // (batch * vocab) if batch * vocab else 1
     if logits.numel() != batch * beams * vocab:
         raise ValueError(f"logits: {batch} x {beams} rows expected, got {tuple(logits.shape)}")
     if out_parents.shape != out_scores.shape or out_tokens.shape != out_scores.shape:
         raise ValueError("out_parents and out_tokens: out_scores' shape expected")
     f32, i32 = torch.float32, torch.int32
-    if logits.dtype is not f32 or scores.dtype is not f32 or out_scores.dtype is not f32 or out_parents.dtype is not i32 \
+    if logits.dtype is not f32 or (scores is not None and scores.dtype is not f32) or out_scores.dtype is not f32 or out_parents.dtype is not i32 \
             or out_tokens.dtype is not i32:
         raise ValueError("logits and scores: torch.float32, parents and tokens: torch.int32 expected")
-    status = engine.lib.janus_beam_select(engine.ctx, _buf(logits, dev, "logits"), _buf(scores, dev, "scores"),
+    status = engine.lib.janus_beam_select(engine.ctx, _buf(logits, dev, "logits"),
+                                          None if scores is None else _buf(scores, dev, "scores"),
                                           _buf(out_scores, dev, "out_scores"), _buf(out_parents, dev, "out_parents"),
                                           _buf(out_tokens, dev, "out_tokens"), batch, beams, vocab, n)
     if status:

@@ -52,3 +52,13 @@ def test_outputs_that_overlap_are_refused(engine):
         ints[2400:3600] = 0   # logits
         assert _call(engine, *args, batch, beams, vocab, n)[0] == _lib.OK
     engine.sync()
+
+
+@pytest.mark.parametrize("batch,beams,vocab,n", [(1, 1, 900, 4), (3, 4, 9000, 8)])
+def test_without_scores(engine, batch, beams, vocab, n):
+    logits = torch.randn(batch, beams, vocab, generator=torch.Generator().manual_seed(72))
+    out = torch.empty(batch, n, device=DEV)
+    parents, tokens = (torch.empty(batch, n, dtype=torch.int32, device=DEV) for _ in range(2))
+    ops.beam_select(engine, logits.to(DEV), None, out, parents, tokens)
+    _, at = _first(_reference(logits, torch.zeros(batch, beams)), n)
+    assert torch.equal(parents.cpu().long(), at // vocab) and torch.equal(tokens.cpu().long(), at % vocab)
