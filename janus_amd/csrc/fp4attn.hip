@@ -63,21 +63,16 @@ struct Fp4Args {
     float scale2;                         // scale * log2(e)
 };
 
-__device__ __forceinline__ float swap16f(float v) {   // value of lane ^ 16
-    const uint32_t u = __float_as_uint(v);
-    auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    return __uint_as_float((__lane_id() & 16) ? p[0] : p[1]);
-}
 __device__ __forceinline__ float groups_max(float v) {   // over the four lanes of a column
-    v = fmaxf(v, swap16f(v));
+    v = fmaxf(v, swap16(v));
     return fmaxf(v, swap32(v));
 }
 __device__ __forceinline__ float groups_sum(float v) {
-    v += swap16f(v);
+    v += swap16(v);
     return v + swap32(v);
 }
 __device__ __forceinline__ uint32_t groups_umax(uint32_t v) {
-    v = max(v, __float_as_uint(swap16f(__uint_as_float(v))));
+    v = max(v, __float_as_uint(swap16(__uint_as_float(v))));
     return max(v, __float_as_uint(swap32(__uint_as_float(v))));
 }
 
@@ -113,25 +108,7 @@ __device__ __forceinline__ SeqRows seq_rows(const Fp4Args &a, uint32_t s) {
 // Positions that row r of a sequence sees.
 __device__ __forceinline__ uint32_t seen_of(const SeqRows &s, uint32_t r) { return (uint32_t)min(max(s.first + (int32_t)r, 0), (int32_t)min(s.avail, 0x7fffffffu)); }
 
-// Sum over the lanes up to this one, without LDS traffic.
-__device__ __forceinline__ uint32_t scan_dpp(uint32_t v) {
-    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);   // row_shr:1, 2, 4, 8
-    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);   // row_bcast:15 into rows 1 and 3
-    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);   // row_bcast:31 into rows 2 and 3
-    return v;
-}
 __device__ __forceinline__ uint32_t lane_value(uint32_t v, uint32_t lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)lane); }
-
-// The kernel's arguments, read again where they are used: held from the start they fill the
-// scalar registers, and what spills takes vector registers and scratch.
-__device__ __forceinline__ const Fp4Args &late_args() {
-    auto at = (const Fp4Args __attribute__((address_space(4))) *)__builtin_amdgcn_kernarg_segment_ptr();
-    asm volatile("" : "+s"(at));
-    return *(const Fp4Args *)at;
-}
 
 // A lane's number that the compiler takes for a new one each time: what follows from it is
 // made again for every share of columns and does not hold registers in between.
@@ -241,18 +218,6 @@ template <int D> struct Raw {
     uint32_t ks[2], vs;
 };
 
-// 16 bytes per lane from base + off straight into LDS at lds + 16 * lane (lds is
-// uniform and goes to M0), past the caches: what few columns read is read once. Inline
-// assembly, so that the compiler does not wait for these requests at its LDS reads: the
-// loop waits for them itself.
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-__device__ __forceinline__ void lds_request(const uint8_t *base, uint32_t off, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(off), "s"(base), "s"(lds)
-                 : "memory", "m0");
-}
-#pragma clang diagnostic pop
-
 // A tile of 32 ph positions of hw KV heads, whose rows of hw D / 2 bytes lie one behind the
 // other in LDS (2 KB a wavefront of K, then of V, for 128 dims). Whole rows are requested, 1 KB an
 // instruction: 270000 positions of 8 heads come at 6.4 TB/s like this and at 4.9 where
@@ -283,8 +248,8 @@ template <int D, int NW> struct Tile {
         const uint8_t *kp = kc + (size_t)p * row, *vp = vc + (size_t)p * row;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            lds_request(kp, ko[i], lds + (wave * N + i) * 1024u);
-            lds_request(vp, vo[i], lds + kBytes + (wave * N + i) * 1024u);
+            lds_request<true>(kp, ko[i], lds + (wave * N + i) * 1024u);
+            lds_request<true>(vp, vo[i], lds + kBytes + (wave * N + i) * 1024u);
         }
     }
 };
@@ -545,8 +510,8 @@ __global__ __launch_bounds__(NW * 64, PER) void fp4_attn_kernel(Fp4Args args) {
     if (share >= args.shares) return;
     Task w;
     w.more = true;
-    for (uint32_t done = 0; w.more && find_task<SPLIT>(late_args(), share, done, w);) {
-        const Fp4Args &a = late_args();
+    for (uint32_t done = 0; w.more && find_task<SPLIT>(late_args<Fp4Args>(), share, done, w);) {
+        const Fp4Args &a = late_args<Fp4Args>();
         const uint32_t lane = fresh_thread() & 63u, g = lane >> 4, at = lane & 15u;
         const uint32_t hwave = wave & (a.hw - 1), phase = wave / a.hw, head0 = (blockIdx.x >> 3) % a.head_groups * a.hw, kvh = head0 + hwave;
         const uint32_t c0 = w.c0, columns = w.s.n * a.G;   // below 2^25
@@ -671,7 +636,7 @@ __global__ __launch_bounds__(NW * 64, PER) void fp4_attn_kernel(Fp4Args args) {
                 else return;
             }
         }
-        const Fp4Args &z = late_args();
+        const Fp4Args &z = late_args<Fp4Args>();
         const uint32_t c = c0 + (lane & 15u);
         if (c < columns) {   // no lane leaves the loop: the search for the next columns needs all
             const uint32_t r = c / z.G, gh = c % z.G;
@@ -867,8 +832,8 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
     const uint32_t share = blockIdx.x / args.kv_heads, kvh = blockIdx.x % args.kv_heads;
     Task w;
     w.more = true;
-    for (uint32_t done = 0; w.more && find_task<SPLIT>(late_args(), share, done, w);) {
-        const Fp4Args &a = late_args();
+    for (uint32_t done = 0; w.more && find_task<SPLIT>(late_args<Fp4Args>(), share, done, w);) {
+        const Fp4Args &a = late_args<Fp4Args>();
         const uint32_t tid = fresh_thread(), lane = tid & 63u, col = lane & 31u, h = lane >> 5;
         const uint32_t columns = w.s.n * a.G;
         auto seen = [&](uint32_t c) { return seen_of(w.s, c / a.G); };
@@ -1188,7 +1153,7 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
         __syncthreads();   // the tiles have been read: the results pass through them, or the next columns' do
         const bool there = phase == 0 && c0 + col < columns;
         if (bad && vis) l = nan;
-        const Fp4Args &z = late_args();
+        const Fp4Args &z = late_args<Fp4Args>();
         if (SPLIT && w.parts > 1) {
             const size_t at = ((size_t)w.slot * z.kv_heads + kvh) * z.cols + (c - w.c0);
             float *to = z.part + at * D;

@@ -450,6 +450,47 @@ __device__ __forceinline__ float swap32(float v) {
     return __uint_as_float((__lane_id() & 32) ? p[0] : p[1]);
 }
 
+// Value of lane ^ 16.
+__device__ __forceinline__ float swap16(float v) {
+    const uint32_t u = __float_as_uint(v);
+    auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return __uint_as_float((__lane_id() & 16) ? p[0] : p[1]);
+}
+
+// Sum over the lanes up to this one, without LDS traffic.
+__device__ __forceinline__ uint32_t scan_dpp(uint32_t v) {
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);   // row_shr:1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);   // row_bcast:15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);   // row_bcast:31 into rows 2 and 3
+    return v;
+}
+
+// The arguments of a kernel whose only parameter is an A, read again where they are used: held from
+// the start they fill the scalar registers, and what spills takes vector registers and scratch.
+template <typename A> __device__ __forceinline__ const A &late_args() {
+    auto at = (const A __attribute__((address_space(4))) *)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(at));
+    return *(const A *)at;
+}
+
+// 16 bytes per lane from base + off straight into LDS at lds + 16 * lane (lds is uniform and goes to
+// M0); ONCE: past the caches, for what is read once. Inline assembly, so that the compiler does not
+// wait for these requests at its LDS reads: the callers' loops wait for them themselves.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+template <bool ONCE> __device__ __forceinline__ void lds_request(const uint8_t *base, uint32_t off, uint32_t lds) {
+    if constexpr (ONCE)
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(off), "s"(base), "s"(lds)
+                     : "memory", "m0");
+    else
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds)
+                     : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
 // Sum over all 64 lanes of a wavefront; every lane receives the total.
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll

@@ -83,30 +83,7 @@ struct Work {
     uint32_t part, parts, chunk, slot;   // positions [part chunk, + chunk); slot of the partials
 };
 
-__device__ __forceinline__ float swap16(float v) {   // value of lane ^ 16
-    const uint32_t u = __float_as_uint(v);
-    auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    return __uint_as_float((__lane_id() & 16) ? p[0] : p[1]);
-}
-
-// The kernel's arguments, read where they are used: held from the start they fill the
-// scalar registers, and what spills takes vector registers and scratch.
-__device__ __forceinline__ const PackedArgs &late_args() {
-    auto at = (const PackedArgs __attribute__((address_space(4))) *)__builtin_amdgcn_kernarg_segment_ptr();
-    asm volatile("" : "+s"(at));
-    return *(const PackedArgs *)at;
-}
-
-// Sum over the lanes up to this one, and the maximum over all, without LDS traffic.
-__device__ __forceinline__ uint32_t scan_dpp(uint32_t v) {
-    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);   // row_shr:1, 2, 4, 8
-    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);   // row_bcast:15 into rows 1 and 3
-    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);   // row_bcast:31 into rows 2 and 3
-    return v;
-}
+// The maximum over all lanes, without LDS traffic.
 __device__ __forceinline__ uint32_t max_dpp(uint32_t v) {
     v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, false));   // row_ror:8, 4, 2, 1
     v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, false));
@@ -630,7 +607,7 @@ __device__ __forceinline__ void few_columns(const PackedArgs &a, const Work &w, 
     }
 
     // join the wavefronts of a group
-    const PackedArgs &z = late_args();
+    const PackedArgs &z = late_args<PackedArgs>();
     constexpr uint32_t C = 16 * NT, OS = D + 4;    // padded: 16 columns meet 16 bank groups
     float *oo = (float *)smem;                     // [wave][column][OS], over the V tiles
     float2 *ml = (float2 *)(smem + 4 * C * OS * 4);   // [wave][column]
@@ -698,17 +675,6 @@ __device__ __forceinline__ void few_columns(const PackedArgs &a, const Work &w, 
     }
 }
 
-// 16 bytes per lane from base + off straight into LDS at lds + 16 * lane (lds is
-// uniform and goes to M0). Inline assembly, so that the compiler does not wait for
-// these requests at its LDS reads: the loop below waits for them itself.
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-__device__ __forceinline__ void lds_request(const unsigned char *base, uint32_t off, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds)
-                 : "memory", "m0");
-}
-#pragma clang diagnostic pop
-
 // Up to 128 columns on a binary16 cache: K and V pass through LDS for all four
 // wavefronts, 32 columns each, requested a tile of TP positions ahead straight into LDS.
 //
@@ -752,15 +718,15 @@ __device__ __forceinline__ bool wide_tile(const PackedArgs &a, const Work &w, ui
         if (p + TP <= p1) {
 #pragma unroll
             for (int j = 0; j < LD; ++j) {
-                lds_request(kp, ko[j], to + j * 1024u);
-                lds_request(vp, vo[j], to + TB + j * 1024u);
+                lds_request<false>(kp, ko[j], to + j * 1024u);
+                lds_request<false>(vp, vo[j], to + TB + j * 1024u);
             }
         } else {   // rows beyond the part repeat its last one
 #pragma unroll
             for (int j = 0; j < LD; ++j) {
                 const uint32_t at = min(row_of(j), p1 - 1 - p) * kvrow;
-                lds_request(kp, at + seg_of(j, false), to + j * 1024u);
-                lds_request(vp, at + seg_of(j, true), to + TB + j * 1024u);
+                lds_request<false>(kp, at + seg_of(j, false), to + j * 1024u);
+                lds_request<false>(vp, at + seg_of(j, true), to + TB + j * 1024u);
             }
         }
     };
@@ -929,7 +895,7 @@ __device__ __forceinline__ bool wide_tile(const PackedArgs &a, const Work &w, ui
         if (__builtin_amdgcn_readfirstlane(*again)) return true;
     }
     if (wc0 + col >= ncols) return false;
-    const PackedArgs &z = late_args();
+    const PackedArgs &z = late_args<PackedArgs>();
     if (z.slots) {
         const size_t at = qat * z.slots + w.slot;
         // what the rounding of c shifted, since the parts are joined by m
@@ -1041,7 +1007,7 @@ __global__ __launch_bounds__(256, (per_cu<Q, KV, D, K>())) void packed_attn_kern
     // prompt of 2048 rows at 32/8/128 with such a value at position 0, which every tile
     // sees: 290 us, 56 without (binary16); 415 and 92 (two parts).
     for (;;) {
-        few_columns<Q, KV, D, 1>(late_args(), w, kvh, ncols, p0, p1, 1, smem);
+        few_columns<Q, KV, D, 1>(late_args<PackedArgs>(), w, kvh, ncols, p0, p1, 1, smem);
         if ((w.c0 += 16) >= ncols) return;
         __syncthreads();   // the outputs have been read from LDS
     }
