@@ -348,8 +348,11 @@ int janus_fp4_attention(janus_ctx *ctx, const void *q, int dtype, const void *k_
  *   scores[b] + (logits[b][t] - log sum_u exp(logits[b][u])),
  * and d_out_scores, d_out_parents (the beam, 0 .. beams - 1) and d_out_tokens, all
  * [batch][n], receive the n largest in descending order, equal ones by beam and then token.
- * Values are compared in binary64 (within a beam by the logit) and returned as
- * binary32. logits: [batch][beams][vocab], d_scores: [batch][beams] or NULL for zeros.
+ * Values are compared in binary64 and returned as binary32; the logarithm in them is
+ * off by some 3e-8 (the exponentials are binary32), so beams that are closer than that may
+ * come in either order. Within a beam the largest logits are taken; where they differ
+ * by less than the last bit of their value in binary64, which of them come and in which order
+ * is not defined. logits: [batch][beams][vocab], d_scores: [batch][beams] or NULL for zeros.
  * A beam with the score -infinity has ended (or not begun: set all but one so at the
  * first step): all its values are -infinity and its logits are not read. A beam whose
  * logits are all -infinity likewise; one with a NaN or +infinity among its logits, or as

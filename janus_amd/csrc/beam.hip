@@ -12,8 +12,8 @@
 // what is not below it, n values and a few more, is ranked by counting.
 // Bound by the read of the logits: 16 requests of 8 beams, 128256 logits each, take 28 us (20
 // for the first kernel, 3.2 TB/s, 8 for the second), one of 4 beams 14, the two launches.
-// L_b is kept to some 1e-8 (the sums of many terms in binary64), so that beams are compared
-// by more than the last bits of binary32.
+// L_b is off by some 3e-8 (9e-8 at most over normal logits of sigma 0.5 to 6): the exponentials and sums of 16 of them are
+// binary32, the sums of those binary64. Beams are compared by more than the last bits of their binary32 values.
 //
 // Reordering. Position by position the slots of a request's beams are permuted: a lane
 // reads its bytes of every slot that is gone on from and then writes them to the

@@ -11,14 +11,17 @@
 // enter the binary16 matrix unit exactly, converted two values an instruction with the
 // scale applied. binary16 rows round P to binary16; binary32 rows have q, divided by a
 // power of two per column, and P in two binary16 parts (22 bits), small parts first.
+// binary16 rows could have the two parts of P as well, for an error of 2.1e-4, that of their own
+// rounding, in place of 2.8e-4: 64 single rows behind up to 8000 positions then take 70 to 72 us
+// instead of 66, a prompt of 6000 rows 431 instead of 316. Who needs them has binary32 rows.
 //
 // Two kernels, by the columns of a sequence and KV head:
-//   up to 16, and to 64 of one or two KV heads while all run at once (decode steps, drafted rows): bound by the read of the cache. A
+//   up to 16, and to 64 where workgroups of one or two KV heads all run at once (decode steps, drafted rows): bound by the read of the cache. A
 //     wavefront has one KV head and 32 positions at a time, whose 4-bit rows come into LDS
 //     as they are. A decode step of 64 sequences of up to 8000 positions, 32 heads on 8, 128
 //     dims: 63 us, 4.6 TB/s, what a large copy reaches; one sequence of 8192 positions 15 us, where
 //     the two launches and the start of each count; 16 x 5 binary32 rows behind 2500 positions of
-//     32 KV heads 36 us, 2.6 TB/s: the conversions and two-part products take as long as the reads.
+//     32 KV heads 36 us, 2.6 TB/s: while a CU is busy it issues 84% of the time, vector instructions 63%.
 //   more (prompts): bound by the matrix unit and what feeds it. Four wavefronts of 32 columns, or
 //     two pairs of them for up to 64 or where there are few tiles, share K and V, converted once for all of them. A prompt of 6000 rows: 307 to 335 us, 880 to
 //     960 TFLOP/s of what the causal mask leaves, where a large matrix product reaches 1184; 20
@@ -29,6 +32,9 @@
 //     21 and 39; binary32 rows 46 and 47, 27 and 36).
 // Where the tiles are few their positions are split into shares and a third kernel joins
 // the parts: a second launch of some 5 us.
+// One kernel takes all sequences of a call, by the columns that they have in the mean: 63 single rows behind up to 8000
+// positions and a chunk of 512 behind 4000 take 180 us in one call, 66 and 76 in two (with 16 single rows and a chunk of
+// 512 without a context 157, 35 and 18).
 //
 // A scale byte above 140 is a block of NaN. The loops count it as a finite scale and note that
 // there was one; the scales are then looked through again and what saw such a block is set: every
@@ -980,7 +986,7 @@ __global__ __launch_bounds__(256, 2) void fp4_wide_kernel(Fp4Args args) {
         f16v o[ND];
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[d] = (f16v){};
-        // p = 2^(s cs + c2), c2 = kBias - m cs rounded (infinite while nothing was seen); where that would cost
+        // p = 2^(s cs + c2), c2 = kBias - m cs rounded (infinite while m is -infinity); where that would cost
         // the last bits of a score (far) the difference to m is taken first
         float m = -INFINITY, c2 = INFINITY, l = 0.0f;
         uint32_t far = 0;   // uniform
@@ -1237,8 +1243,9 @@ void plan(janus_ctx *ctx, Fp4Args &a, uint32_t cols, uint32_t hw, uint32_t ph, u
     const bool split = cols <= 16 ? steps * at_once > 10 * at_once + 20 * busy && busy < 4 * at_once
                                   : steps > fewest && 2 * busy <= at_once && 3 * mean <= max_len;
     if (counts && split) {
-        // at most 128 parts of a tile, which the join's 16 wavefronts read in one go: a sequence of 16000 positions
-        // in 250 parts 21 us, in 125 18 to 19
+        // at most 128 parts of a tile in the mean, which the join's 16 wavefronts read in one go: a sequence of 16000
+        // positions in 250 parts 21 us, in 125 18 to 19. The lengths are on the device: a long sequence beside short ones has
+        // more parts, and a join for the mean (that one and one of a single position 22 us, and 63 of 20 positions 64)
         a.shares = a.target = (uint32_t)std::min<uint64_t>(at_once, 128 * busy);
         a.slots = (uint32_t)(a.shares + tiles);
         a.mean_parts = (uint32_t)std::min<uint64_t>(a.shares / busy, steps / a.least) + 1;
@@ -1291,11 +1298,14 @@ template <typename T, int D> int launch_dim(janus_ctx *ctx, Fp4Args &a, uint32_t
     // with two-part q of 128 dims in 160 (three of four wavefronts)
     constexpr bool kTwo = sizeof(T) == 4 && D == 128;
     constexpr int NW = kTwo ? 4 : 8, PER = kTwo ? 3 : 4;
-    // One or two KV heads leave a few-column workgroup many phases, 64 to 256 positions at a time where the other kernel
-    // takes 64: while all its tiles run at once that is the shorter chain, though each reads K and V (16/1/128, 64 x 3 rows
+    // A few-column workgroup of one or two KV heads (hw: the largest power of two in their number, up to NW) has many
+    // phases, 64 to 256 positions at a time where the other kernel takes 64: while all its tiles run at once that is the shorter chain, though each reads K and V (16/1/128, 64 x 3 rows
     // behind up to 2000: 19 and 27 us, binary32 22 and 31; 40 x 3 behind 600 12 and 17, 12 and 22). Long contexts of
     // binary16 rows are bound by those reads (64 x 3 behind up to 7800 43 and 36, binary32 44 and 44; 300 x 3 behind 1000
-    // 34 and 30), and with eight heads a step is 32 positions (32/8/128, 40 x 8 behind 600: 41 and 20).
+    // 34 and 30), and with eight heads a step is 32 positions (32/8/128, 40 x 8 behind 600: 41 and 20). Three, five, six and
+    // ten KV heads go the same way: 12 x 40 columns behind 600 12 and 19 at 24/3/128, 13 and 19 at 40/5/128, 15 and 19 at
+    // 24/6/128, 16 and 20 at 40/10/128 (binary32 13 and 24, 13 and 24, 17 and 24, 18 and 24); 60 columns of ten heads behind
+    // 2000 lose (4 sequences 31 and 26, 12 33 and 34, binary32 52 and 40).
     const uint32_t hw = few_heads(a.kv_heads, NW);
     const uint64_t tiles = ((uint64_t)a.rows * a.G + 15) / 16 + a.nseq - 1;
     const bool many_phases = hw <= 2 && tiles * (a.kv_heads / hw) <= (uint64_t)ctx->num_cus * (PER * 4 / NW) &&
